@@ -1,0 +1,430 @@
+// The paged cache: rows quantised as they are written, read back, and the entry points of the attention over it.
+//
+// Writing and reading are bound by HBM (16-bit rows in, codes out).  D / 8 lanes take a row of one token and head, eight elements
+// a lane, and the token's four parts in turn, their loads in flight together; a row's largest element crosses its lanes by shuffles, so
+// the row is read once.
+#include "tritt_cache.cuh"
+
+namespace tritt {
+namespace {
+
+constexpr int kThreads = 256;
+
+struct WriteArgs {
+  CacheArgs cache;
+  tritt_rows_t rows[4];   // k1, k2, raw v1, v2
+  int parts;              // the first 3 or all 4
+};
+
+template <typename T, int CODE, int D>
+__global__ void __launch_bounds__(kThreads) cache_write_kernel(const __grid_constant__ WriteArgs w) {
+  constexpr int L = D / 8, kSlots = kThreads / L;
+  const CacheArgs& a = w.cache;
+  const int col = threadIdx.x % L * 8;
+  // neighbouring slots: heads of a token
+  const long long slot = (long long)blockIdx.x * kSlots + threadIdx.x / L;
+  const int head = (int)(slot % a.c.N);
+  const long long token = slot / a.c.N;
+  const int b = (int)(token / a.c.n), i = (int)(token % a.c.n);
+  bool on = b < a.c.B && i < new_tokens(a, b);
+  Place at{-1, 0};
+  if (on) {
+    at = place_of(a, b, __ldg(a.c.context + b) + i);
+    if (at.page < 0) {
+      on = false;
+      if (a.status) atomicOr(a.status, kStatusPlace);
+    }
+  }
+  float f[4][8];
+#pragma unroll
+  for (int part = 0; part < 4; ++part) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[part][e] = 0.f;
+    // (k1, k2, raw v1, v2 in the order of the parts)
+    if (on && part < w.parts) load8((const T*)w.rows[part].p + rows_at(w.rows[part], b, head, i) + col, f[part]);
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[kPartV1][e] = silu_f(f[kPartV1][e]);
+#pragma unroll
+  for (int part = 0; part < 4; ++part)
+    if (part < w.parts) store_row<CODE, L>(a, on, at, part, head, col, f[part]);
+}
+
+struct ReadArgs {
+  CacheArgs cache;
+  void* parts[4];
+  float* lse;
+};
+
+template <typename T, int CODE, int D>
+__global__ void __launch_bounds__(kThreads) cache_read_kernel(const __grid_constant__ ReadArgs r) {
+  constexpr int L = D / 8, kSlots = kThreads / L;
+  const CacheArgs& a = r.cache;
+  const int col = threadIdx.x % L * 8;
+  // neighbouring slots: tokens of a head, whose rows are neighbours in a page and in the result
+  const long long slot = (long long)blockIdx.x * kSlots + threadIdx.x / L;
+  const int i = (int)(slot % a.c.n);
+  const long long bh = slot / a.c.n;
+  const int head = (int)(bh % a.c.N), b = (int)(bh / a.c.N);
+  if (b >= a.c.B) return;
+  Place at{-1, 0};
+  if (i < new_tokens(a, b)) {
+    at = place_of(a, b, __ldg(a.c.context + b) + i);
+    if (at.page < 0 && a.status) atomicOr(a.status, kStatusPlace);
+  }
+  Codes8<CODE> codes[4];
+  int byte[4];
+#pragma unroll
+  for (int part = 0; part < 4; ++part) {
+    if (at.page < 0) continue;
+    const size_t row = row_of(a, at, part, head);
+    codes[part].load((const uint8_t*)a.c.codes + row * (size_t)(D * (CODE == TRITT_CODE_F16 ? 2 : 1)), col);
+    byte[part] = a.c.exponents[row];
+  }
+#pragma unroll
+  for (int part = 0; part < 4; ++part) {
+    float f[8];
+    if (at.page < 0) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = 0.f;
+    } else {
+      code_values<CODE>(codes[part], code_scale(byte[part]), f);
+    }
+    store8((T*)r.parts[part] + (size_t)slot * D + col, f);
+  }
+  if (r.lse && col == 0) r.lse[slot] = at.page < 0 ? 0.f : a.c.lse[lse_of(a, at, head)];
+}
+
+// One warp a row: D / 8 of its lanes hold eight elements each.  The splits' maxima and sums are looked at twice, their results once.
+template <typename T, int CODE>
+__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ JoinArgs j) {
+  // (the split kernel may still be running when this one is launched early)
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const CacheArgs& a = j.cache;
+  const int lane = threadIdx.x & 31, col = lane * 8, D = a.c.D;
+  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (row >= (long long)a.c.B * a.c.N * a.c.n) return;
+  const int i = (int)(row % a.c.n), head = (int)(row / a.c.n % a.c.N), b = (int)(row / a.c.n / a.c.N);
+  const float* part = j.part + (size_t)row * j.splits * (D + 2);
+  // a maximum of -infinity: a split that has seen nothing; of NaN (which the comparisons below let through): a row of the cache that reads as NaN
+  float m = -INFINITY;
+  for (int s = lane; s < j.splits; s += 32) m = fmaxf(m, part[(size_t)s * (D + 2)]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  float l = 0.f, f[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] = 0.f;
+  for (int s = 0; s < j.splits; ++s) {
+    const float* p = part + (size_t)s * (D + 2);
+    const float ms = p[0], ls = p[1];
+    if (ms == -INFINITY && ls == 0.f) continue;   // (its result is not written)
+    const float weight = exp2f(ms - m);
+    l = fmaf(ls, weight, l);
+    if (col < D) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = fmaf(p[2 + col + e], weight, f[e]);
+    }
+  }
+  const bool none = m == -INFINITY && l == 0.f;
+  const float inv = none ? 0.f : 1.f / l, lse = none ? -INFINITY : l != l ? l : (m + log2f(l)) * kLn2;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] *= inv;
+  if (j.o) {
+    if (col < D) store8((T*)j.o + (size_t)row * D + col, f);
+    if (j.lse && lane == 0) j.lse[row] = lse;
+    return;
+  }
+  // append: W into the cache (a token that is not there has no place)
+  bool on = i < new_tokens(a, b);
+  Place at{-1, 0};
+  if (on) {
+    at = place_of(a, b, __ldg(a.c.context + b) + i);
+    on = at.page >= 0;
+  }
+  if (on && col < D) {
+    float v[8];
+    load8((const T*)j.v2.p + rows_at(j.v2, b, head, i) + col, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] *= v[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = 0.f;
+  }
+  // (lanes past the row have zeros, which change no maximum)
+  const int byte = exponent_byte<CODE>(largest_of_row<32>(largest8(f)));
+  if (!on) return;
+  const size_t to = row_of(a, at, kPartV2, head);
+  if (lane == 0) {
+    a.c.exponents[to] = (unsigned char)byte;
+    a.c.lse[lse_of(a, at, head)] = lse;
+  }
+  if (col < D) {
+    const float scale = to_code_scale(byte);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = byte == 255 ? 0.f : f[e] * scale;
+    Codes8<CODE> codes;
+    codes.encode(f);
+    codes.store((uint8_t*)a.c.codes + to * (size_t)(D * (CODE == TRITT_CODE_F16 ? 2 : 1)), col);
+  }
+}
+
+template <typename T, int CODE, int D> int write_for(const WriteArgs& w, cudaStream_t stream) {
+  const long long slots = (long long)w.cache.c.B * w.cache.c.n * w.cache.c.N;
+  constexpr int kSlots = kThreads / (D / 8);
+  cache_write_kernel<T, CODE, D><<<(unsigned)((slots + kSlots - 1) / kSlots), kThreads, 0, stream>>>(w);
+  count_launch();
+  TRITT_CUDA_OK(cudaGetLastError());
+  return 0;
+}
+template <typename T, int CODE, int D> int read_for(const ReadArgs& r, cudaStream_t stream) {
+  const long long slots = (long long)r.cache.c.B * r.cache.c.n * r.cache.c.N;
+  constexpr int kSlots = kThreads / (D / 8);
+  cache_read_kernel<T, CODE, D><<<(unsigned)((slots + kSlots - 1) / kSlots), kThreads, 0, stream>>>(r);
+  count_launch();
+  TRITT_CUDA_OK(cudaGetLastError());
+  return 0;
+}
+
+template <typename T, int CODE> int write_d(const WriteArgs& w, cudaStream_t s) {
+  switch (w.cache.c.D) {
+    case 16: return write_for<T, CODE, 16>(w, s);
+    case 32: return write_for<T, CODE, 32>(w, s);
+    case 64: return write_for<T, CODE, 64>(w, s);
+    case 128: return write_for<T, CODE, 128>(w, s);
+    default: return write_for<T, CODE, 256>(w, s);
+  }
+}
+template <typename T, int CODE> int read_d(const ReadArgs& r, cudaStream_t s) {
+  switch (r.cache.c.D) {
+    case 16: return read_for<T, CODE, 16>(r, s);
+    case 32: return read_for<T, CODE, 32>(r, s);
+    case 64: return read_for<T, CODE, 64>(r, s);
+    case 128: return read_for<T, CODE, 128>(r, s);
+    default: return read_for<T, CODE, 256>(r, s);
+  }
+}
+template <typename T, int CODE> int join_for(const JoinArgs& j, cudaStream_t stream, bool early) {
+  const long long rows = (long long)j.cache.c.B * j.cache.c.N * j.cache.c.n;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)((rows + 3) / 4));
+  cfg.blockDim = dim3(128);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = early ? 1 : 0;
+  TRITT_CUDA_OK(cudaLaunchKernelEx(&cfg, join_kernel<T, CODE>, j));
+  count_launch();
+  return 0;
+}
+
+// f(type, code) with the types of a call
+template <typename F> int by_type(int dtype, int code, F f) {
+  auto with = [&](auto t) {
+    using T = decltype(t);
+    if (code == TRITT_CODE_F16) return f(T{}, std::integral_constant<int, TRITT_CODE_F16>{});
+    if (code == TRITT_CODE_E4M3) return f(T{}, std::integral_constant<int, TRITT_CODE_E4M3>{});
+    return f(T{}, std::integral_constant<int, TRITT_CODE_INT8>{});
+  };
+  if (dtype == TRITT_F32) return with(float{});
+  return dtype == TRITT_F16 ? with(__half{}) : with(__nv_bfloat16{});
+}
+
+int check_scratch(size_t need, const void* ws, size_t have) {
+  if (!ws || have < need || ((uintptr_t)ws & 255)) {
+    set_error("workspace too small or not 256-byte aligned: need %zu bytes, got %zu", need, ws ? have : (size_t)0);
+    return -6;
+  }
+  return 0;
+}
+
+int check_out(const void* p) {
+  if (!p) {
+    set_error("null tensor pointer");
+    return -4;
+  }
+  if ((uintptr_t)p & 15) {
+    set_error("tensor pointer is not 16-byte aligned");
+    return -5;
+  }
+  return 0;
+}
+
+bool fast(int op, int D, int dtype, int flags) { (void)op; (void)D; (void)dtype; (void)flags; return false; }
+
+size_t part_bytes(const tritt_cache_t& c, int splits) {
+  return align_up((size_t)c.B * c.N * c.n * splits * (c.D + 2) * 4, 256);
+}
+
+int window(int w) { return w < 0 ? 0 : w; }
+
+}  // namespace
+
+CacheArgs cache_args(const tritt_cache_t& c, int* status) {
+  CacheArgs a{c, 0, status};
+  while ((1 << a.page_log2) < c.page_size) ++a.page_log2;
+  return a;
+}
+
+int check_cache(const tritt_cache_t* c) {
+  if (!c || c->B <= 0 || c->N <= 0 || c->n <= 0 || c->pages <= 0 || c->table_pages <= 0) {
+    set_error("sequences, heads, tokens and pages must be positive");
+    return -1;
+  }
+  if (c->D != 16 && c->D != 32 && c->D != 64 && c->D != 128 && c->D != 256) {
+    set_error("head_dim must be 16, 32, 64, 128 or 256, got %d", c->D);
+    return -2;
+  }
+  if (c->code != TRITT_CODE_F16 && c->code != TRITT_CODE_E4M3 && c->code != TRITT_CODE_INT8) {
+    set_error("unknown code type %d", c->code);
+    return -3;
+  }
+  if (c->page_size < 8 || (c->page_size & (c->page_size - 1)) || (long long)c->page_size * c->table_pages > (1LL << 30)) {
+    set_error("a page must have a power of two from 8 tokens on, a table at most 2^30 in all (page_size %d, %d pages)", c->page_size,
+              c->table_pages);
+    return -14;
+  }
+  if (!c->codes || !c->exponents || !c->table || !c->context) {
+    set_error("null cache pointer");
+    return -4;
+  }
+  if (((uintptr_t)c->codes & 15) || ((uintptr_t)c->table & 3) || ((uintptr_t)c->context & 3)) {
+    set_error("cache pointer is not aligned");
+    return -5;
+  }
+  if (c->ancestors && c->n > TRITT_MAX_ANCESTORS) {
+    set_error("at most %d new tokens with ancestors, got %d", TRITT_MAX_ANCESTORS, c->n);
+    return -15;
+  }
+  if ((long long)c->B * c->N > 65535 || (long long)c->B * c->N * c->n > (1LL << 30)) {
+    set_error("B*N = %lld, or with n = %d new tokens, is too much for one call; split the batch", (long long)c->B * c->N, c->n);
+    return -11;
+  }
+  return 0;
+}
+
+int check_rows(const tritt_rows_t* rows, int count, int dtype) {
+  if (dtype != TRITT_F32 && dtype != TRITT_F16 && dtype != TRITT_BF16) {
+    set_error("unknown dtype code %d", dtype);
+    return -3;
+  }
+  const long long unit = dtype == TRITT_F32 ? 4 : 8;
+  for (int i = 0; i < count; ++i) {
+    if (!rows || !rows[i].p) {
+      set_error("null tensor pointer");
+      return -4;
+    }
+    if (((uintptr_t)rows[i].p & 15) || rows[i].stride_b % unit || rows[i].stride_n % unit || rows[i].stride_t % unit) {
+      set_error("rows must start on 16-byte boundaries");
+      return -5;
+    }
+  }
+  return 0;
+}
+
+int launch_write(const CacheArgs& a, const tritt_rows_t* rows, int dtype, int parts, cudaStream_t stream) {
+  WriteArgs w{a, {rows[0], rows[1], rows[2], rows[3]}, parts};
+  return by_type(dtype, a.c.code, [&](auto t, auto code) { return write_d<decltype(t), decltype(code)::value>(w, stream); });
+}
+
+int launch_join(const JoinArgs& j, cudaStream_t stream, bool early) {
+  return by_type(j.dtype, j.cache.c.code, [&](auto t, auto code) { return join_for<decltype(t), decltype(code)::value>(j, stream, early); });
+}
+
+}  // namespace tritt
+
+using namespace tritt;
+
+extern "C" {
+
+int tritt_cache_write(const tritt_cache_t* c, const tritt_rows_t* rows, int dtype, int* status_word, tritt_stream_t stream) {
+  if (int rc = check_cache(c)) return rc;
+  if (int rc = check_rows(rows, 4, dtype)) return rc;
+  return launch_write(cache_args(*c, status_word), rows, dtype, 4, (cudaStream_t)stream);
+}
+
+int tritt_cache_read(const tritt_cache_t* c, void* const* parts, float* lse, int dtype, int* status_word, tritt_stream_t stream) {
+  if (int rc = check_cache(c)) return rc;
+  if (!parts) {
+    set_error("null tensor pointer");
+    return -4;
+  }
+  ReadArgs r{cache_args(*c, status_word), {parts[0], parts[1], parts[2], parts[3]}, c->lse ? lse : nullptr};
+  for (int i = 0; i < 4; ++i) {
+    const tritt_rows_t row{parts[i], 0, 0, 0};
+    if (int rc = check_rows(&row, 1, dtype)) return rc;
+  }
+  return by_type(dtype, c->code, [&](auto t, auto code) { return read_d<decltype(t), decltype(code)::value>(r, (cudaStream_t)stream); });
+}
+
+int tritt_decode_path(int op, int D, int dtype, int flags) { return fast(op, D, dtype, flags) ? TRITT_PATH_TCGEN05 : TRITT_PATH_SIMT; }
+
+size_t tritt_decode_workspace(int op, const tritt_cache_t* c, int dtype, int k1_window, int k2_window, int flags) {
+  if (check_cache(c)) return 0;
+  (void)op; (void)dtype; (void)k1_window; (void)k2_window; (void)flags;
+  return part_bytes(*c, simt_decode_splits(*c));
+}
+
+int tritt_tdp_decode(const tritt_cache_t* c, const tritt_rows_t* q, void* o, float* lse, int dtype, float alpha, int k1_window,
+                     int k2_window, int kk_left, int kk_right, void* workspace, size_t workspace_bytes, int* status_word, int flags,
+                     tritt_stream_t stream) {
+  if (int rc = check_cache(c)) return rc;
+  if (int rc = check_rows(q, 1, dtype)) return rc;
+  if (int rc = check_out(o)) return rc;
+  if (k1_window < 0 || k2_window < 0 || kk_left < 0 || kk_right < 0) {
+    set_error("window arguments must be >= 0 (got %d, %d, %d, %d)", k1_window, k2_window, kk_left, kk_right);
+    return -10;
+  }
+  const size_t need = tritt_decode_workspace(TRITT_OP_TDP_DECODE, c, dtype, k1_window, k2_window, flags);
+  if (int rc = check_scratch(need, workspace, workspace_bytes)) return rc;
+  TdpDecodeArgs a{cache_args(*c, status_word), *q, dtype, k1_window, k2_window, kk_left, kk_right, alpha * kLog2e, (float*)workspace, 0};
+  JoinArgs j{a.cache, a.part, 0, dtype, o, lse, {}};
+  j.splits = a.splits = simt_decode_splits(*c);
+  if (int rc = simt_tdp_decode(a, (cudaStream_t)stream)) return rc;
+  return launch_join(j, (cudaStream_t)stream, false);
+}
+
+int tritt_dps_append(const tritt_cache_t* c, const tritt_rows_t* rows, int dtype, float alpha, int k_diff, void* workspace,
+                     size_t workspace_bytes, int* status_word, int flags, tritt_stream_t stream) {
+  if (int rc = check_cache(c)) return rc;
+  if (int rc = check_rows(rows, 4, dtype)) return rc;
+  if (!c->lse) {
+    set_error("the cache has no log-sum-exps: it is not one of the dot-product-sum form");
+    return -16;
+  }
+  if (k_diff < 0) {
+    set_error("k_diff must be >= 0, got %d", k_diff);
+    return -10;
+  }
+  const size_t need = tritt_decode_workspace(TRITT_OP_DPS_APPEND, c, dtype, 0, 0, flags);
+  if (int rc = check_scratch(need, workspace, workspace_bytes)) return rc;
+  const CacheArgs cache = cache_args(*c, status_word);
+  if (int rc = launch_write(cache, rows, dtype, 3, (cudaStream_t)stream)) return rc;
+  DpsDecodeArgs a{cache, rows[1], dtype, kPartK1, kPartV1, 0, window(k_diff), alpha * kLog2e, (float*)workspace, 0};
+  JoinArgs j{cache, a.part, 0, dtype, nullptr, nullptr, rows[3]};
+  j.splits = a.splits = simt_decode_splits(*c);
+  if (int rc = simt_dps_decode(a, (cudaStream_t)stream)) return rc;
+  return launch_join(j, (cudaStream_t)stream, false);
+}
+
+int tritt_dps_decode(const tritt_cache_t* c, const tritt_rows_t* q, void* o, float* m, int dtype, float alpha, void* workspace,
+                     size_t workspace_bytes, int* status_word, int flags, tritt_stream_t stream) {
+  if (int rc = check_cache(c)) return rc;
+  if (int rc = check_rows(q, 1, dtype)) return rc;
+  if (int rc = check_out(o)) return rc;
+  if (!c->lse) {
+    set_error("the cache has no log-sum-exps: it is not one of the dot-product-sum form");
+    return -16;
+  }
+  const size_t need = tritt_decode_workspace(TRITT_OP_DPS_DECODE, c, dtype, 0, 0, flags);
+  if (int rc = check_scratch(need, workspace, workspace_bytes)) return rc;
+  const CacheArgs cache = cache_args(*c, status_word);
+  DpsDecodeArgs a{cache, *q, dtype, kPartK2, kPartV2, 1, 1 << 30, alpha * kLog2e, (float*)workspace, 0};
+  JoinArgs j{cache, a.part, 0, dtype, o, m, {}};
+  j.splits = a.splits = simt_decode_splits(*c);
+  if (int rc = simt_dps_decode(a, (cudaStream_t)stream)) return rc;
+  return launch_join(j, (cudaStream_t)stream, false);
+}
+
+}  // extern "C"

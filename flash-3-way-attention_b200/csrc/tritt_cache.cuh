@@ -1,0 +1,249 @@
+// A paged cache of quantised rows: places, codes, and which tokens a new one attends to.
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include "tritt_common.cuh"
+
+#include <type_traits>
+
+namespace tritt {
+
+enum { kPartK1 = 0, kPartK2 = 1, kPartV1 = 2, kPartV2 = 3 };
+enum { kStatusPosition = 256, kStatusPlace = 512, kStatusTdpDecode = 1024 };
+
+// The cache as kernels see it.
+struct CacheArgs {
+  tritt_cache_t c;
+  int page_log2;
+  int* status;
+};
+
+inline int code_bytes(int code) { return code == TRITT_CODE_F16 ? 2 : 1; }
+
+// 0, or the error code of what is wrong with a cache's description (host).
+int check_cache(const tritt_cache_t* c);
+int check_rows(const tritt_rows_t* rows, int count, int dtype);
+CacheArgs cache_args(const tritt_cache_t& c, int* status);
+
+// A token's place in the cache: its page and row, page -1 where the table or the cache have none.
+struct Place {
+  int page, row;
+};
+__device__ __forceinline__ Place place_of(const CacheArgs& a, int b, int token) {
+  const int i = token >> a.page_log2;
+  Place at{-1, token & (a.c.page_size - 1)};
+  if (token >= 0 && i < a.c.table_pages) {
+    const int page = __ldg(a.c.table + b * a.c.table_stride + i);
+    if (page >= 0 && page < a.c.pages) at.page = page;
+  }
+  return at;
+}
+// Number of a part's row among all rows of the cache (rows of D codes, one exponent each), and of a token's log-sum-exp.
+__device__ __forceinline__ size_t row_of(const CacheArgs& a, Place at, int part, int head) {
+  return ((((size_t)at.page * 4 + part) * a.c.N + head) << a.page_log2) + at.row;
+}
+__device__ __forceinline__ size_t lse_of(const CacheArgs& a, Place at, int head) {
+  return (((size_t)at.page * a.c.N + head) << a.page_log2) + at.row;
+}
+
+// New tokens that sequence b has in this call.
+__device__ __forceinline__ int new_tokens(const CacheArgs& a, int b) {
+  if (__ldg(a.c.context + b) < 0) return 0;
+  const int n = a.c.counts ? __ldg(a.c.counts + b) : a.c.n;
+  return n < 0 ? 0 : n > a.c.n ? a.c.n : n;
+}
+
+// Bit m: new token i attends to new token m (only with ancestors).
+__device__ __forceinline__ unsigned long long seen_word(const CacheArgs& a, int b, int i) {
+  const unsigned long long own = 1ull << i;
+  return ((unsigned long long)__ldg(a.c.ancestors + (size_t)b * a.c.n + i) & (own - 1)) | own;
+}
+// Position of new token i of sequence b, counted from its context.
+__device__ __forceinline__ int depth_of(const CacheArgs& a, int b, int i) {
+  return a.c.ancestors ? __popcll(seen_word(a, b, i)) - 1 : i;
+}
+
+// ---------------------------------------------------------------- codes
+// The exponent byte of a row whose largest |element| has these bits (those of a NaN are larger than any).
+template <int CODE> __device__ __forceinline__ int exponent_byte(uint32_t largest) {
+  const int field = (int)(largest >> 23);
+  const uint32_t mantissa = largest & 0x7fffffu;
+  if (field == 255) return 255;
+  const int e = CODE == TRITT_CODE_F16    ? field - 14                             // below 2^15
+                : CODE == TRITT_CODE_E4M3 ? field - 8 + (mantissa > 0x600000u)     // at most 448 = 1.75 * 2^8
+                                          : field - 6 + (mantissa > 0x7e0000u);    // at most 127 = 1.984375 * 2^6
+  return e < 1 ? 1 : e;
+}
+// What a row's elements are multiplied by before they are rounded to codes, and what codes stand for.
+__device__ __forceinline__ float to_code_scale(int byte) { return byte == 255 ? 0.f : __uint_as_float((uint32_t)(254 - byte) << 23); }
+__device__ __forceinline__ float code_scale(int byte) {
+  return byte == 255 ? __uint_as_float(0x7fffffffu) : __uint_as_float((uint32_t)byte << 23);
+}
+
+// Eight codes of neighbouring elements: 16 bytes of fp16, 8 of the others.  A row that is not finite has zeros.
+template <int CODE> struct Codes8;
+template <> struct Codes8<TRITT_CODE_F16> {
+  uint4 v;
+  __device__ __forceinline__ void load(const void* row, int col) { v = *reinterpret_cast<const uint4*>((const __half*)row + col); }
+  __device__ __forceinline__ void store(void* row, int col) const { *reinterpret_cast<uint4*>((__half*)row + col) = v; }
+  __device__ __forceinline__ void encode(const float (&f)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    v = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  __device__ __forceinline__ void halves(uint32_t (&w)[4]) const { w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w; }
+};
+// Four bytes as two pairs of fp16.
+template <int CODE> __device__ __forceinline__ void bytes_to_halves(uint32_t v, uint32_t& lo, uint32_t& hi) {
+  if constexpr (CODE == TRITT_CODE_E4M3) {
+    const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(v & 0xffffu), __NV_E4M3);
+    const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(v >> 16), __NV_E4M3);
+    lo = (uint32_t)a.x | (uint32_t)a.y << 16;
+    hi = (uint32_t)b.x | (uint32_t)b.y << 16;
+  } else {
+    // 0x64bb is 1024 + bb in fp16; with the sign bit turned over bb is the element + 128
+    const uint32_t u = v ^ 0x80808080u;
+    const __half2 off = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));   // 1152
+    uint32_t l = __byte_perm(u, 0x64646464u, 0x4140), h = __byte_perm(u, 0x64646464u, 0x4342);
+    const __half2 a = __hsub2(*reinterpret_cast<__half2*>(&l), off), b = __hsub2(*reinterpret_cast<__half2*>(&h), off);
+    lo = *reinterpret_cast<const uint32_t*>(&a);
+    hi = *reinterpret_cast<const uint32_t*>(&b);
+  }
+}
+template <int CODE> struct Codes8 {
+  uint2 v;
+  __device__ __forceinline__ void load(const void* row, int col) { v = *reinterpret_cast<const uint2*>((const uint8_t*)row + col); }
+  __device__ __forceinline__ void store(void* row, int col) const { *reinterpret_cast<uint2*>((uint8_t*)row + col) = v; }
+  __device__ __forceinline__ void encode(const float (&f)[8]) {
+    uint32_t w[2] = {0u, 0u};
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      uint32_t pair;
+      if constexpr (CODE == TRITT_CODE_E4M3)
+        pair = __nv_cvt_float2_to_fp8x2(make_float2(f[i], f[i + 1]), __NV_SATFINITE, __NV_E4M3);
+      else
+        pair = ((uint32_t)__float2int_rn(f[i]) & 255u) | ((uint32_t)__float2int_rn(f[i + 1]) & 255u) << 8;
+      w[i / 4] |= pair << (8 * (i % 4));
+    }
+    v = make_uint2(w[0], w[1]);
+  }
+  __device__ __forceinline__ void halves(uint32_t (&w)[4]) const {
+    bytes_to_halves<CODE>(v.x, w[0], w[1]);
+    bytes_to_halves<CODE>(v.y, w[2], w[3]);
+  }
+};
+template <int CODE> __device__ __forceinline__ void code_values(const Codes8<CODE>& c, float scale, float (&f)[8]) {
+  uint32_t w[4];
+  c.halves(w);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    f[2 * i] = v.x * scale;
+    f[2 * i + 1] = v.y * scale;
+  }
+}
+
+// Eight neighbouring elements of a row of any type.
+template <typename T> __device__ __forceinline__ void load8(const T* p, float (&f)[8]) {
+  const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    T lo, hi;
+    *reinterpret_cast<uint16_t*>(&lo) = (uint16_t)w[i];
+    *reinterpret_cast<uint16_t*>(&hi) = (uint16_t)(w[i] >> 16);
+    f[2 * i] = to_f(lo);
+    f[2 * i + 1] = to_f(hi);
+  }
+}
+template <> __device__ __forceinline__ void load8<float>(const float* p, float (&f)[8]) {
+  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+  f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+}
+template <typename T> __device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const T lo = from_f<T>(f[2 * i]), hi = from_f<T>(f[2 * i + 1]);
+    w[i] = (uint32_t)*reinterpret_cast<const uint16_t*>(&lo) | (uint32_t)*reinterpret_cast<const uint16_t*>(&hi) << 16;
+  }
+  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <> __device__ __forceinline__ void store8<float>(float* p, const float (&f)[8]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+}
+
+__device__ __forceinline__ size_t rows_at(const tritt_rows_t& r, int b, int n, int t) {
+  return (size_t)(b * r.stride_b + n * r.stride_n + t * r.stride_t);
+}
+
+// Largest |element| of eight, as bits; then over the L neighbouring lanes of a row.
+__device__ __forceinline__ uint32_t largest8(const float (&f)[8]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(f[e]) & 0x7fffffffu);
+  return m;
+}
+template <int L> __device__ __forceinline__ uint32_t largest_of_row(uint32_t m) {
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+  return m;
+}
+// A row's eight elements of this lane into its place.  All L lanes of the row call it; `on` is theirs in common.
+template <int CODE, int L>
+__device__ __forceinline__ void store_row(const CacheArgs& a, bool on, Place at, int part, int head, int col, const float (&f)[8]) {
+  const int byte = exponent_byte<CODE>(largest_of_row<L>(largest8(f)));
+  if (!on) return;
+  const float scale = to_code_scale(byte);
+  float y[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) y[e] = byte == 255 ? 0.f : f[e] * scale;
+  Codes8<CODE> codes;
+  codes.encode(y);
+  const size_t row = row_of(a, at, part, head);
+  codes.store((uint8_t*)a.c.codes + row * (size_t)(a.c.D * (CODE == TRITT_CODE_F16 ? 2 : 1)), col);
+  if (col == 0) a.c.exponents[row] = (unsigned char)byte;
+}
+
+// ---------------------------------------------------------------- parts of a row's soft-max, and what becomes of them
+// Each split of a new token's attended tokens leaves its maximum (log2 units), sum and unnormalised result in the workspace,
+// [rows][splits][D + 2] fp32 (rows = (b * N + head) * n + i), and a second kernel joins them.
+struct JoinArgs {
+  CacheArgs cache;
+  const float* part;
+  int splits, dtype;
+  void* o;            // [B, N, n, D], or null: append
+  float* lse;         // [B, N, n] or null
+  tritt_rows_t v2;    // append: W = result * v2 goes to the cache, and the log-sum-exp
+};
+int launch_join(const JoinArgs& j, cudaStream_t stream, bool early);
+int launch_write(const CacheArgs& a, const tritt_rows_t* rows, int dtype, int parts, cudaStream_t stream);
+
+// The CUDA cores' kernels (any type, fp32 arithmetic): triple dot product, and one soft-max attention over two parts of the cache.
+struct TdpDecodeArgs {
+  CacheArgs cache;
+  tritt_rows_t q;
+  int dtype, k1w, k2w, kkl, kkr;
+  float scale2;       // alpha * log2(e)
+  float* part;
+  int splits;
+};
+struct DpsDecodeArgs {
+  CacheArgs cache;
+  tritt_rows_t q;     // the rows that attend
+  int dtype, key_part, value_part, biased, window;
+  float scale2;
+  float* part;
+  int splits;
+};
+int simt_decode_splits(const tritt_cache_t& c);
+int simt_tdp_decode(const TdpDecodeArgs& a, cudaStream_t stream);
+int simt_dps_decode(const DpsDecodeArgs& a, cudaStream_t stream);
+
+}  // namespace tritt

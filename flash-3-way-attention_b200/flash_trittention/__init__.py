@@ -7,12 +7,24 @@ imported lazily so that ``import flash_trittention`` works without a GPU.
 
 __version__ = "0.1.0"
 
-__all__ = ["flash_trittention", "TrittentionTriton"]  # the reference's public names; TrittentionTDP is an extra
+__all__ = ["flash_trittention", "TrittentionTriton"]  # the reference's public names; the others are extras
 
 _LAZY_ATTRS = {
     "flash_trittention": (".triple_dot_product.flash_trittention", "flash_trittention"),
     "TrittentionTriton": (".dot_product_sum.trittention_triton", "TrittentionTriton"),
     "TrittentionTDP": (".ops", "TrittentionTDP"),  # torch.library operators + module (not in the reference)
+    # norms and position rotation of q, k1, k2, in front of either attention
+    "qk_norm_rotary": (".norm_rotary", "qk_norm_rotary"),
+    "rotary_tables": (".norm_rotary", "rotary_tables"),
+    # serving: a paged cache of quantised rows, and attention of new tokens over it
+    "TrittentionCache": (".cache", "TrittentionCache"),
+    "new_cache": (".cache", "new_cache"),
+    "cache_write": (".cache", "cache_write"),
+    "cache_read": (".cache", "cache_read"),
+    "tree_ancestors": (".cache", "tree_ancestors"),
+    "tdp_decode": (".cache", "tdp_decode"),
+    "dps_append": (".cache", "dps_append"),
+    "dps_decode": (".cache", "dps_decode"),
     # raises if a kernel of an earlier call gave up on a bounded barrier wait (not in the reference)
     "check_status": ("._native", "check_status"),
 }

@@ -19,6 +19,8 @@ LIB_PATH = os.path.join(_HERE, "libtritt_sm100.so")
 
 F32, F16, BF16 = 0, 1, 2
 OP_TDP_FWD, OP_TDP_BWD, OP_DPS_FWD, OP_DPS_BWD = 0, 1, 2, 3
+OP_TDP_DECODE, OP_DPS_APPEND, OP_DPS_DECODE = 4, 5, 6
+CODES = {torch.float16: 0, torch.float8_e4m3fn: 1, torch.int8: 2}  # what a cached element is held in
 FLAG_FORCE_SIMT, FLAG_BWD_PARTIAL, FLAG_WIDE_OPERANDS, FLAG_BWD_CTA_PAIRS = 1, 2, 4, 8
 PATH_SIMT, PATH_TCGEN05 = 0, 1
 
@@ -31,7 +33,9 @@ SYMBOLS = (
     "tritt_tdp_bwd", "tritt_tdp_bwd_finalize", "tritt_tdp_bwd_partials_offset", "tritt_dps_fwd",
     "tritt_dps_bwd", "tritt_dps_bwd_saved", "tritt_selftest_umma", "tritt_selftest_wait_expiry", "tritt_tdp_fwd_noalloc",
     "tritt_noalloc_scratch_bytes", "tritt_selftest_bwd_registers",
-    "tritt_tdp_bwd_plan",
+    "tritt_tdp_bwd_plan", "tritt_qk_norm_rotary_fwd", "tritt_qk_norm_rotary_bwd", "tritt_qk_norm_rotary_workspace",
+    "tritt_cache_write", "tritt_cache_read", "tritt_tdp_decode", "tritt_dps_append", "tritt_dps_decode", "tritt_decode_workspace",
+    "tritt_decode_path",
 )
 
 _lib = None
@@ -45,6 +49,31 @@ launches = 0  # kernels-enqueuing library calls made by this process (bench book
 
 class TrittError(RuntimeError):
     pass
+
+
+class Rows(C.Structure):
+    """``tritt_rows_t``: rows of a [B, N, T, D] tensor by its strides."""
+
+    _fields_ = [("p", C.c_void_p), ("stride_b", C.c_longlong), ("stride_n", C.c_longlong), ("stride_t", C.c_longlong)]
+
+
+class NormRotary(C.Structure):
+    """``tritt_norm_rotary_t``."""
+
+    _fields_ = [("x", Rows * 3), ("y", Rows * 3), ("dx", Rows * 3), ("w", C.c_void_p * 3), ("dw", C.c_void_p * 3),
+                ("cos", C.c_void_p), ("sin", C.c_void_p), ("positions", C.c_void_p), ("position_stride_b", C.c_longlong),
+                ("position_stride_t", C.c_longlong), ("positions64", C.c_int), ("table", C.c_int), ("rot", C.c_int),
+                ("interleaved", C.c_int), ("weight_heads", C.c_int), ("weight_dtype", C.c_int), ("B", C.c_int), ("N", C.c_int),
+                ("T", C.c_int), ("D", C.c_int), ("dtype", C.c_int), ("eps", C.c_float)]
+
+
+class Cache(C.Structure):
+    """``tritt_cache_t``."""
+
+    _fields_ = [("codes", C.c_void_p), ("exponents", C.c_void_p), ("lse", C.c_void_p), ("pages", C.c_int), ("page_size", C.c_int),
+                ("N", C.c_int), ("D", C.c_int), ("code", C.c_int), ("table", C.c_void_p), ("table_stride", C.c_longlong),
+                ("table_pages", C.c_int), ("context", C.c_void_p), ("counts", C.c_void_p), ("ancestors", C.c_void_p), ("B", C.c_int),
+                ("n", C.c_int)]
 
 
 def host_forward(*args):
@@ -128,6 +157,22 @@ def lib():
                 L.tritt_selftest_umma.argtypes = [vp] * 5 + [i, vp, vp]
                 L.tritt_selftest_wait_expiry.restype = i
                 L.tritt_selftest_wait_expiry.argtypes = [i, C.c_longlong, vp, vp]
+                norm, cache, rows = C.POINTER(NormRotary), C.POINTER(Cache), C.POINTER(Rows)
+                L.tritt_qk_norm_rotary_fwd.argtypes = [norm, vp, vp]
+                L.tritt_qk_norm_rotary_bwd.argtypes = [norm, vp, sz, vp, vp]
+                L.tritt_qk_norm_rotary_workspace.argtypes = [norm]
+                L.tritt_qk_norm_rotary_workspace.restype = sz
+                L.tritt_cache_write.argtypes = [cache, rows, i, vp, vp]
+                L.tritt_cache_read.argtypes = [cache, vp, vp, i, vp, vp]
+                L.tritt_tdp_decode.argtypes = [cache, rows, vp, vp, i, f] + [i] * 4 + [vp, sz, vp, i, vp]
+                L.tritt_dps_append.argtypes = [cache, rows, i, f, i, vp, sz, vp, i, vp]
+                L.tritt_dps_decode.argtypes = [cache, rows, vp, vp, i, f, vp, sz, vp, i, vp]
+                L.tritt_decode_workspace.argtypes = [i, cache] + [i] * 4
+                L.tritt_decode_workspace.restype = sz
+                L.tritt_decode_path.argtypes = [i] * 4
+                for name in ("qk_norm_rotary_fwd", "qk_norm_rotary_bwd", "cache_write", "cache_read", "tdp_decode", "dps_append", "dps_decode",
+                             "decode_path"):
+                    getattr(L, "tritt_" + name).restype = i
                 _load_host(L)
                 _lib = L
     return _lib
@@ -161,7 +206,8 @@ STATUS_BITS = {1: "self-test kernel", 2: "triple-dot-product forward", 4: "tripl
                8: "shared memory of a tensor-core kernel was not 1024-byte aligned",
                16: "soft-max attention forward (dot-product-sum)", 32: "soft-max attention backward (dot-product-sum)",
                64: "an input element beyond the fp16 operand range (65504) in an fp32 / wide-operand call",
-               128: "wait-expiry self-test"}
+               128: "wait-expiry self-test", 256: "a rotation whose position its tables do not have",
+               512: "a token without a place in its cache", 1024: "triple-dot-product attention over a cache"}
 
 
 def _device_index(device) -> int:
@@ -262,6 +308,21 @@ def aligned(t: torch.Tensor) -> torch.Tensor:
     if not t.is_contiguous():
         t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+def strided(t: torch.Tensor) -> torch.Tensor:
+    """``t`` ([B, N, T, D]) itself if its rows are contiguous and start on 16-byte boundaries, whatever its other strides; else
+    a contiguous copy."""
+    unit = 16 // t.element_size()
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(st % unit == 0 or size == 1 for st, size in zip(t.stride()[:3], t.shape)):
+        return t
+    return aligned(t.contiguous())
+
+
+def rows(t: torch.Tensor) -> Rows:
+    """The rows of a tensor that ``strided`` has returned."""
+    b, n, tt = (st if size > 1 else 0 for st, size in zip(t.stride()[:3], t.shape))
+    return Rows(t.data_ptr(), b, n, tt)
 
 
 # The current stream's handle and the current device without the Python objects around them (a call of a short sequence
@@ -417,3 +478,81 @@ def tdp_fwd_noalloc(q, k1, k2, v1, v2, o, lse, alpha, causal, k1w, k2w, kkl, kkr
                                          _status_address(q.device), flags, _stream(q.device))
     _check(rc, "tritt_tdp_fwd_noalloc")
     launches += 1
+
+
+def norm_rotary(a: NormRotary, dev: torch.device, backward: bool = False):
+    global launches
+    check_status(dev, synchronize=False)
+    L = lib()
+    with _on_device(dev):
+        if backward:
+            n = int(L.tritt_qk_norm_rotary_workspace(C.byref(a)))
+            ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+            rc = L.tritt_qk_norm_rotary_bwd(C.byref(a), 0 if ws is None else ws.data_ptr(), n, _status_address(dev), _stream(dev))
+        else:
+            rc = L.tritt_qk_norm_rotary_fwd(C.byref(a), _status_address(dev), _stream(dev))
+    _check(rc, "tritt_qk_norm_rotary")
+    launches += 1
+
+
+def cache_write(c: Cache, new, dtype: int, dev: torch.device):
+    global launches
+    check_status(dev, synchronize=False)
+    with _on_device(dev):
+        rc = lib().tritt_cache_write(C.byref(c), (Rows * 4)(*(rows(t) for t in new)), dtype, _status_address(dev), _stream(dev))
+    _check(rc, "tritt_cache_write")
+    launches += 1
+
+
+def cache_read(c: Cache, parts, lse, dtype: int, dev: torch.device):
+    global launches
+    check_status(dev, synchronize=False)
+    with _on_device(dev):
+        rc = lib().tritt_cache_read(C.byref(c), (C.c_void_p * 4)(*(t.data_ptr() for t in parts)), 0 if lse is None else lse.data_ptr(),
+                                    dtype, _status_address(dev), _stream(dev))
+    _check(rc, "tritt_cache_read")
+    launches += 1
+
+
+def _decode_scratch(op, c, dtype, k1w, k2w, flags, dev):
+    return torch.empty(max(int(lib().tritt_decode_workspace(op, C.byref(c), dtype, k1w, k2w, flags)), 256), dtype=torch.uint8, device=dev)
+
+
+def tdp_decode(c: Cache, q, o, lse, alpha, k1w, k2w, kkl, kkr, flags=0):
+    global launches
+    dev, dt = q.device, dtype_code(q.dtype)
+    check_status(dev, synchronize=False)
+    with _on_device(dev):
+        ws = _decode_scratch(OP_TDP_DECODE, c, dt, k1w, k2w, flags, dev)
+        rc = lib().tritt_tdp_decode(C.byref(c), C.byref(rows(q)), o.data_ptr(), 0 if lse is None else lse.data_ptr(), dt, alpha, k1w, k2w,
+                                    kkl, kkr, ws.data_ptr(), ws.numel(), _status_address(dev), flags, _stream(dev))
+    _check(rc, "tritt_tdp_decode")
+    launches += 1
+
+
+def dps_append(c: Cache, new, alpha, k_diff, flags=0):
+    global launches
+    dev, dt = new[0].device, dtype_code(new[0].dtype)
+    check_status(dev, synchronize=False)
+    with _on_device(dev):
+        ws = _decode_scratch(OP_DPS_APPEND, c, dt, 0, 0, flags, dev)
+        rc = lib().tritt_dps_append(C.byref(c), (Rows * 4)(*(rows(t) for t in new)), dt, alpha, k_diff, ws.data_ptr(), ws.numel(),
+                                    _status_address(dev), flags, _stream(dev))
+    _check(rc, "tritt_dps_append")
+    launches += 1
+
+
+def dps_decode(c: Cache, q, o, m, alpha, flags=0):
+    global launches
+    dev, dt = q.device, dtype_code(q.dtype)
+    check_status(dev, synchronize=False)
+    with _on_device(dev):
+        ws = _decode_scratch(OP_DPS_DECODE, c, dt, 0, 0, flags, dev)
+        rc = lib().tritt_dps_decode(C.byref(c), C.byref(rows(q)), o.data_ptr(), 0 if m is None else m.data_ptr(), dt, alpha, ws.data_ptr(),
+                                    ws.numel(), _status_address(dev), flags, _stream(dev))
+    _check(rc, "tritt_dps_decode")
+    launches += 1
+
+
+def decode_path(op, D, dtype, flags=0) -> int:
+    return lib().tritt_decode_path(op, D, dtype, flags)

@@ -19,8 +19,10 @@
  *   - `status_word` (an int the GPU can address: device memory or page-locked host memory; may be NULL)
  *     is OR-ed with a non-zero code by a kernel whose bounded barrier wait ran out (1 tensor-core
  *     self-test, 2 / 4 triple-dot-product forward / backward, 8 misaligned shared memory, 16 / 32
- *     soft-max attention forward / backward of the dot-product-sum path, 128 wait-expiry self-test) or,
- *     bit 64, by the fp16 operand conversion of an fp32 / wide-operand call that met an element beyond 65504;
+ *     soft-max attention forward / backward of the dot-product-sum path, 128 wait-expiry self-test, 1024
+ *     triple-dot-product attention over a cache) or,
+ *     bit 64, by the fp16 operand conversion of an fp32 / wide-operand call that met an element beyond 65504,
+ *     bit 256, by a rotation whose position its tables do not have, bit 512, by a call that met a place its cache does not have;
  *     the caller zeroes and reads it.  A non-zero word means the results of that call are invalid;
  *   - window arguments (k1_window, k2_window, kk_left, kk_right, k_diff) are distances >= 0; a value
  *     >= T means "unlimited".  Negative values are refused with an argument error when `causal` is set
@@ -43,6 +45,8 @@ enum { TRITT_F32 = 0, TRITT_F16 = 1, TRITT_BF16 = 2 };
 
 /* operations, for tritt_workspace_bytes() */
 enum { TRITT_OP_TDP_FWD = 0, TRITT_OP_TDP_BWD = 1, TRITT_OP_DPS_FWD = 2, TRITT_OP_DPS_BWD = 3 };
+/* and for tritt_decode_workspace() */
+enum { TRITT_OP_TDP_DECODE = 4, TRITT_OP_DPS_APPEND = 5, TRITT_OP_DPS_DECODE = 6 };
 
 /* flags */
 enum {
@@ -225,6 +229,114 @@ int tritt_tdp_bwd_plan(int T, int D, int dtype, int causal, int k1_window, int k
  * (0: `launched` registers per thread are what the split needs; -30: they are not).  No counterpart in the reference.
  */
 int tritt_selftest_bwd_registers(int launched);
+
+/* ------------------------------------------------------------------------------------------------------------------------
+ * Around the attention: norms and rotation in front of it, and serving one or a few new tokens over a cache.  None of these
+ * has a counterpart in the reference, which computes whole sequences from tensors that are normed and rotated elsewhere.
+ */
+
+/* Rows [B, N, T, D] of any of the three dtypes: element (b, n, t, d) at p + b*stride_b + n*stride_n + t*stride_t + d (strides in
+   elements; the rows themselves are contiguous, 16-byte aligned). */
+typedef struct {
+  const void* p;
+  long long stride_b, stride_n, stride_t;
+} tritt_rows_t;
+
+/*
+ * Norms of queries and keys for each head, with the position rotation in the same pass.  For each row x of q, k1 and k2:
+ *   u = x / sqrt(mean(x^2) + eps) * w;   of the first `rot` elements each pair (a, b) -> (a c - b s, b c + a s)
+ * with c, s = cos[position], sin[position] ([positions in the tables, rot / 2] fp32, contiguous).  Pairs are (i, i + rot / 2), or
+ * (2 i, 2 i + 1) if `interleaved`.  Head dimension 16, 32, 64, 128 or 256; `rot` 0 (norm alone) or a multiple of 16.
+ */
+typedef struct {
+  tritt_rows_t x[3];          /* q, k1, k2 */
+  tritt_rows_t y[3];          /* the results (forward: written); backward: their gradients (read) */
+  tritt_rows_t dx[3];         /* backward: gradients of x (written) */
+  const void* w[3];           /* weights [D] or, with weight_heads, [N, D]; null: 1 */
+  void* dw[3];                /* backward: their gradients, in the weights' type; null: not wanted */
+  const float *cos, *sin;     /* null: rot is 0 */
+  const void* positions;      /* int32 or int64 (positions64), element (b, t) at b*position_stride_b + t*position_stride_t; null: t.  A position
+                                 that the tables do not have sets status bit 256 and takes their nearest one */
+  long long position_stride_b, position_stride_t;
+  int positions64, table, rot, interleaved;   /* table: positions in the tables */
+  int weight_heads, weight_dtype;             /* the weights' type is the rows' or TRITT_F32 */
+  int B, N, T, D, dtype;
+  float eps;
+} tritt_norm_rotary_t;
+
+int tritt_qk_norm_rotary_fwd(const tritt_norm_rotary_t* a, int* status_word, tritt_stream_t stream);
+/* `workspace`: tritt_qk_norm_rotary_workspace() bytes (0 where no dw is wanted); gradients of the weights are summed in a fixed
+   order, a call repeats itself bit for bit. */
+int tritt_qk_norm_rotary_bwd(const tritt_norm_rotary_t* a, void* workspace, size_t workspace_bytes, int* status_word,
+                             tritt_stream_t stream);
+size_t tritt_qk_norm_rotary_workspace(const tritt_norm_rotary_t* a);
+
+/* What an element of a cache is held in. */
+enum { TRITT_CODE_F16 = 0, TRITT_CODE_E4M3 = 1, TRITT_CODE_INT8 = 2 };
+enum { TRITT_MAX_ANCESTORS = 64 };
+
+/*
+ * A paged cache of rows of D elements, four of a token and head (the parts): K1, K2, SiLU(V1), and V2 (triple dot product) or
+ * W (dot-product-sum: the inner attention's result times V2, whose log-sum-exp stands in `lse`).
+ * An element is code * 2^(exponent - 127) with one exponent byte for a row: the least with which the row's largest element is at
+ * most 448 (e4m3), at most 127 (int8) or below 2^15 (fp16), so codes are rounded once and powers of two are exact.  Elements below
+ * 2^-126 count as zero.  A row with an infinite or NaN element gets the exponent 255: all of it reads as NaN, and a
+ * token that attends to it gets NaN.
+ * Token t of sequence b is row t % page_size of page table[b][t / page_size].
+ * Each call is about n new tokens of B sequences: token i of sequence b is number context[b] + i, for i < counts[b] (counts null: n).
+ * It attends to the context[b] tokens before them and, of the new ones, to token m if bit m of ancestors[b][i] is set and m < i,
+ * and to itself (ancestors null: to all m <= i).  Its position is context[b] + the number of the new ones before it that it attends to, that
+ * of an older token is its number.  A place that the table or the cache does not have sets status bit 512 and is neither read
+ * nor written; context[b] < 0 is an unused sequence: nothing of it is read or written, its results are those of no attended token.
+ */
+typedef struct {
+  void* codes;                 /* [pages, 4, N, page_size, D] */
+  unsigned char* exponents;    /* [pages, 4, N, page_size] */
+  float* lse;                  /* [pages, N, page_size] natural-log units, or null (triple dot product) */
+  int pages, page_size, N, D, code;   /* page_size: a power of two from 8 on;  D: 16, 32, 64, 128 or 256 */
+  const int* table;            /* [B, table_pages] */
+  long long table_stride;      /* elements between two sequences' tables */
+  int table_pages;
+  const int* context;          /* [B] */
+  const int* counts;           /* [B] or null */
+  const long long* ancestors;  /* [B, n] or null; n <= TRITT_MAX_ANCESTORS with them */
+  int B, n;
+} tritt_cache_t;
+
+/* Quantises the new tokens' K1, K2, SiLU(V1) and V2 (`dtype`) into their places: of these arrays only the rows of the new tokens change.
+   rows: k1, k2, raw v1, v2 [B, N, n, D]. */
+int tritt_cache_write(const tritt_cache_t* c, const tritt_rows_t* rows, int dtype, int* status_word, tritt_stream_t stream);
+/* Reads the new tokens' four parts back into contiguous [B, N, n, D] tensors of `dtype`, and lse into [B, N, n] (where the cache has it
+   and lse is not null); zeros for i >= counts[b] and for places that there are not. */
+int tritt_cache_read(const tritt_cache_t* c, void* const* parts, float* lse, int dtype, int* status_word, tritt_stream_t stream);
+
+/*
+ * Triple-dot-product attention of the n new tokens, whose rows are in the cache already (tritt_cache_write):
+ *   S[q,j,k] = alpha sum_h q[q,h] K1[j,h] K2[k,h], soft-max over the attended pairs, o = sum P SiLU(V1)[j] V2[k]
+ * over pairs of attended tokens within the windows (distances of positions, as for tritt_tdp_fwd: q - j <= k1_window,
+ * q - k <= k2_window, k - j <= kk_left, j - k <= kk_right).  o: [B, N, n, D] contiguous; lse [B, N, n] or null.
+ * A token without an attended pair (i >= counts[b], context[b] < 0) gets o = 0, lse = -infinity.
+ */
+int tritt_tdp_decode(const tritt_cache_t* c, const tritt_rows_t* q, void* o, float* lse, int dtype, float alpha, int k1_window,
+                     int k2_window, int kk_left, int kk_right, void* workspace, size_t workspace_bytes, int* status_word, int flags,
+                     tritt_stream_t stream);
+/*
+ * Dot-product-sum attention of new tokens, in the two chained soft-maxes into which its score separates.  Append: writes K1, K2 and
+ * SiLU(V1) of the new tokens, attends from each token t (its unrounded k2) to the tokens s with position(t) - position(s) <= k_diff,
+ *   Y[t] = sum_s softmax_s(alpha K1[s].k2[t]) SiLU(V1)[s],  lse[t] = log sum_s exp(alpha K1[s].k2[t])
+ * and writes W[t] = Y[t] v2[t] and lse[t].
+ */
+int tritt_dps_append(const tritt_cache_t* c, const tritt_rows_t* rows, int dtype, float alpha, int k_diff, void* workspace,
+                     size_t workspace_bytes, int* status_word, int flags, tritt_stream_t stream);
+/* Decode: o[q] = sum_t softmax_t(alpha q.K2[t] + lse[t]) W[t], m its log-sum-exp; the new tokens are in the cache already. */
+int tritt_dps_decode(const tritt_cache_t* c, const tritt_rows_t* q, void* o, float* m, int dtype, float alpha, void* workspace,
+                     size_t workspace_bytes, int* status_word, int flags, tritt_stream_t stream);
+/* Bytes of scratch for the three calls above (op: TRITT_OP_TDP_DECODE, TRITT_OP_DPS_APPEND, TRITT_OP_DPS_DECODE); the windows of the
+   triple dot product as above (0 for the others). */
+size_t tritt_decode_workspace(int op, const tritt_cache_t* c, int dtype, int k1_window, int k2_window, int flags);
+/* Which kernel family such a call runs on (TRITT_PATH_SIMT or TRITT_PATH_TCGEN05; for the dot-product-sum the latter stands for warp-level
+   matrix instructions). */
+int tritt_decode_path(int op, int D, int dtype, int flags);
 
 #ifdef __cplusplus
 }
