@@ -29,7 +29,7 @@ __global__ void __launch_bounds__(kThreads) cache_write_kernel(const __grid_cons
   bool on = b < a.c.B && i < new_tokens(a, b);
   Place at{-1, 0};
   if (on) {
-    at = place_of(a, b, __ldg(a.c.context + b) + i);
+    at = place_of(a, b, context_of(a, b) + i);
     if (at.page < 0) {
       on = false;
       if (a.status) atomicOr(a.status, kStatusPlace);
@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(const __grid_const
   if (b >= a.c.B) return;
   Place at{-1, 0};
   if (i < new_tokens(a, b)) {
-    at = place_of(a, b, __ldg(a.c.context + b) + i);
+    at = place_of(a, b, context_of(a, b) + i);
     if (at.page < 0 && a.status) atomicOr(a.status, kStatusPlace);
   }
   Codes8<CODE> codes[4];
@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ JoinA
   bool on = i < new_tokens(a, b);
   Place at{-1, 0};
   if (on) {
-    at = place_of(a, b, __ldg(a.c.context + b) + i);
+    at = place_of(a, b, context_of(a, b) + i);
     on = at.page >= 0;
   }
   if (on && col < D) {
@@ -251,13 +251,16 @@ int check_out(const void* p) {
   return 0;
 }
 
-bool fast(int op, int D, int dtype, int flags) { (void)op; (void)D; (void)dtype; (void)flags; return false; }
+bool fast(int op, int D, int dtype, int flags) {
+  if (flags & TRITT_FLAG_FORCE_SIMT) return false;
+  return op == TRITT_OP_TDP_DECODE && sm100_tdp_decode_supported(D, dtype);
+}
 
 size_t part_bytes(const tritt_cache_t& c, int splits) {
   return align_up((size_t)c.B * c.N * c.n * splits * (c.D + 2) * 4, 256);
 }
 
-int window(int w) { return w < 0 ? 0 : w; }
+int window(int w) { return w < 0 ? 0 : w < 1 << 30 ? w : 1 << 30; }
 
 }  // namespace
 
@@ -280,8 +283,8 @@ int check_cache(const tritt_cache_t* c) {
     set_error("unknown code type %d", c->code);
     return -3;
   }
-  if (c->page_size < 8 || (c->page_size & (c->page_size - 1)) || (long long)c->page_size * c->table_pages > (1LL << 30)) {
-    set_error("a page must have a power of two from 8 tokens on, a table at most 2^30 in all (page_size %d, %d pages)", c->page_size,
+  if (c->page_size < 8 || (c->page_size & (c->page_size - 1)) || (long long)c->page_size * c->table_pages > (1LL << 28)) {
+    set_error("a page must have a power of two from 8 tokens on, a table at most 2^28 in all (page_size %d, %d pages)", c->page_size,
               c->table_pages);
     return -14;
   }
@@ -362,7 +365,8 @@ int tritt_decode_path(int op, int D, int dtype, int flags) { return fast(op, D, 
 
 size_t tritt_decode_workspace(int op, const tritt_cache_t* c, int dtype, int k1_window, int k2_window, int flags) {
   if (check_cache(c)) return 0;
-  (void)op; (void)dtype; (void)k1_window; (void)k2_window; (void)flags;
+  (void)k1_window;
+  if (op == TRITT_OP_TDP_DECODE && fast(op, c->D, dtype, flags)) return sm100_tdp_decode_workspace(*c, window(k2_window));
   return part_bytes(*c, simt_decode_splits(*c));
 }
 
@@ -378,7 +382,8 @@ int tritt_tdp_decode(const tritt_cache_t* c, const tritt_rows_t* q, void* o, flo
   }
   const size_t need = tritt_decode_workspace(TRITT_OP_TDP_DECODE, c, dtype, k1_window, k2_window, flags);
   if (int rc = check_scratch(need, workspace, workspace_bytes)) return rc;
-  TdpDecodeArgs a{cache_args(*c, status_word), *q, dtype, k1_window, k2_window, kk_left, kk_right, alpha * kLog2e, (float*)workspace, 0};
+  TdpDecodeArgs a{cache_args(*c, status_word), *q, dtype, window(k1_window), window(k2_window), window(kk_left), window(kk_right), alpha * kLog2e, (float*)workspace, 0};
+  if (fast(TRITT_OP_TDP_DECODE, c->D, dtype, flags)) return sm100_tdp_decode(a, workspace, o, lse, (cudaStream_t)stream);
   JoinArgs j{a.cache, a.part, 0, dtype, o, lse, {}};
   j.splits = a.splits = simt_decode_splits(*c);
   if (int rc = simt_tdp_decode(a, (cudaStream_t)stream)) return rc;

@@ -47,6 +47,12 @@ __device__ __forceinline__ size_t lse_of(const CacheArgs& a, Place at, int head)
   return (((size_t)at.page * a.c.N + head) << a.page_log2) + at.row;
 }
 
+// Tokens of sequence b before the new ones, at most what its table has places for (more is an error, and bounds every loop over them).
+__device__ __forceinline__ int context_of(const CacheArgs& a, int b) {
+  const int c = __ldg(a.c.context + b), most = a.c.table_pages << a.page_log2;
+  if (c > most && a.status) atomicOr(a.status, kStatusPlace);
+  return c < most ? c : most;
+}
 // New tokens that sequence b has in this call.
 __device__ __forceinline__ int new_tokens(const CacheArgs& a, int b) {
   if (__ldg(a.c.context + b) < 0) return 0;
@@ -242,6 +248,11 @@ struct DpsDecodeArgs {
   float* part;
   int splits;
 };
+// ... on the tensor cores (16-bit queries, head dimension 64 or 128), both kernels of it
+bool sm100_tdp_decode_supported(int D, int dtype);
+size_t sm100_tdp_decode_workspace(const tritt_cache_t& c, int k2_window);
+int sm100_tdp_decode(const TdpDecodeArgs& a, void* workspace, void* o, float* lse, cudaStream_t stream);
+
 int simt_decode_splits(const tritt_cache_t& c);
 int simt_tdp_decode(const TdpDecodeArgs& a, cudaStream_t stream);
 int simt_dps_decode(const DpsDecodeArgs& a, cudaStream_t stream);

@@ -101,7 +101,7 @@ __device__ __forceinline__ Row row_of_block(const CacheArgs& a, long long row) {
   r.i = (int)(r.row % a.c.n);
   r.head = (int)(r.row / a.c.n % a.c.N);
   r.b = (int)(r.row / a.c.n / a.c.N);
-  r.ctx = __ldg(a.c.context + r.b);
+  r.ctx = context_of(a, r.b);
   r.on = r.i < new_tokens(a, r.b);
   r.seen = a.c.ancestors ? seen_word(a, r.b, r.i) : 0;
   r.pos = r.ctx + depth_of(a, r.b, r.i);
@@ -112,7 +112,7 @@ __device__ __forceinline__ int attended(const CacheArgs& a, const Row& r, int t)
   if (t < r.ctx) return t;
   const int m = t - r.ctx;
   if (!a.c.ancestors) return t;
-  return (r.seen >> m & 1) ? r.ctx + depth_of(a, r.b, m) : -1;
+  return (r.seen >> m & 1) ? r.ctx + __popcll(r.seen & ((1ull << m) - 1)) : -1;
 }
 __device__ __forceinline__ Place find(const CacheArgs& a, int b, int t) {
   const Place at = place_of(a, b, t);

@@ -17,8 +17,7 @@ speculative decoding.  ``context`` (``[B]`` int32) holds how many tokens of each
 nothing of it is read or written.
 
 ``ancestors`` (``[B, n]`` int64, see ``tree_ancestors``) makes the new tokens a tree: token ``i`` attends to the context, to the earlier new
-tokens ``m`` whose bit is set in ``ancestors[b, i]``, and to itself; its position is ``context[b]`` plus the number of the new ones among
-them.  Without it the new tokens are a chain.  The drafts that are accepted are written again, as a chain.
+tokens ``m`` whose bit is set in ``ancestors[b, i]``, and to itself; windows count distances along these.  Without it the new tokens are a chain.  The drafts that are accepted are written again, as a chain.
 
 A place that the table or the cache does not have, and a kernel that gave up, are reported by the next call or ``check_status()``.  The
 calls enqueue work on the current stream, and can be captured; which tokens there are is read on the device.

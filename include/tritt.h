@@ -282,11 +282,11 @@ enum { TRITT_MAX_ANCESTORS = 64 };
  * most 448 (e4m3), at most 127 (int8) or below 2^15 (fp16), so codes are rounded once and powers of two are exact.  Elements below
  * 2^-126 count as zero.  A row with an infinite or NaN element gets the exponent 255: all of it reads as NaN, and a
  * token that attends to it gets NaN.
- * Token t of sequence b is row t % page_size of page table[b][t / page_size].
+ * Token t of sequence b is row t % page_size of page table[b][t / page_size]; a table has at most 2^28 tokens.
  * Each call is about n new tokens of B sequences: token i of sequence b is number context[b] + i, for i < counts[b] (counts null: n).
  * It attends to the context[b] tokens before them and, of the new ones, to token m if bit m of ancestors[b][i] is set and m < i,
- * and to itself (ancestors null: to all m <= i).  Its position is context[b] + the number of the new ones before it that it attends to, that
- * of an older token is its number.  A place that the table or the cache does not have sets status bit 512 and is neither read
+ * and to itself (ancestors null: to all m <= i).  Distances are counted along the tokens that it attends to: their positions are 0, 1, 2, ...
+ * in order, its own is the last.  A place that the table or the cache does not have sets status bit 512 and is neither read
  * nor written; context[b] < 0 is an unused sequence: nothing of it is read or written, its results are those of no attended token.
  */
 typedef struct {

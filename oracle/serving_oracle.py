@@ -68,11 +68,10 @@ def visible(i, ancestors):
 
 
 def _tokens(ctx, i, ancestors):
-    """(row numbers, positions) of the tokens that new token i attends to, and its own position."""
+    """(row numbers, positions) of the tokens that new token i attends to without a window, and its own position."""
     new = visible(i, ancestors)
     rows = list(range(ctx)) + [ctx + m for m in new]
-    pos = list(range(ctx)) + [ctx + len(visible(m, ancestors)) - 1 for m in new]
-    return torch.tensor(rows), torch.tensor(pos), ctx + len(new) - 1
+    return torch.tensor(rows), torch.arange(len(rows)), len(rows) - 1
 
 
 def tdp_row(q, k1, k2, v1, v2, ctx, i, alpha, windows=(None, None, None, None), ancestors=None):
