@@ -253,7 +253,7 @@ int check_out(const void* p) {
 
 bool fast(int op, int D, int dtype, int flags) {
   if (flags & TRITT_FLAG_FORCE_SIMT) return false;
-  return op == TRITT_OP_TDP_DECODE && sm100_tdp_decode_supported(D, dtype);
+  return op == TRITT_OP_TDP_DECODE ? sm100_tdp_decode_supported(D, dtype) : mma_dps_decode_supported(D, dtype);
 }
 
 size_t part_bytes(const tritt_cache_t& c, int splits) {
@@ -367,7 +367,7 @@ size_t tritt_decode_workspace(int op, const tritt_cache_t* c, int dtype, int k1_
   if (check_cache(c)) return 0;
   (void)k1_window;
   if (op == TRITT_OP_TDP_DECODE && fast(op, c->D, dtype, flags)) return sm100_tdp_decode_workspace(*c, window(k2_window));
-  return part_bytes(*c, simt_decode_splits(*c));
+  return part_bytes(*c, fast(op, c->D, dtype, flags) ? mma_dps_decode_splits(*c) : simt_decode_splits(*c));
 }
 
 int tritt_tdp_decode(const tritt_cache_t* c, const tritt_rows_t* q, void* o, float* lse, int dtype, float alpha, int k1_window,
@@ -408,8 +408,9 @@ int tritt_dps_append(const tritt_cache_t* c, const tritt_rows_t* rows, int dtype
   if (int rc = launch_write(cache, rows, dtype, 3, (cudaStream_t)stream)) return rc;
   DpsDecodeArgs a{cache, rows[1], dtype, kPartK1, kPartV1, 0, window(k_diff), alpha * kLog2e, (float*)workspace, 0};
   JoinArgs j{cache, a.part, 0, dtype, nullptr, nullptr, rows[3]};
-  j.splits = a.splits = simt_decode_splits(*c);
-  if (int rc = simt_dps_decode(a, (cudaStream_t)stream)) return rc;
+  const bool matrix = fast(TRITT_OP_DPS_DECODE, c->D, dtype, flags);
+  j.splits = a.splits = matrix ? mma_dps_decode_splits(*c) : simt_decode_splits(*c);
+  if (int rc = matrix ? mma_dps_decode(a, (cudaStream_t)stream) : simt_dps_decode(a, (cudaStream_t)stream)) return rc;
   return launch_join(j, (cudaStream_t)stream, false);
 }
 
@@ -427,8 +428,9 @@ int tritt_dps_decode(const tritt_cache_t* c, const tritt_rows_t* q, void* o, flo
   const CacheArgs cache = cache_args(*c, status_word);
   DpsDecodeArgs a{cache, *q, dtype, kPartK2, kPartV2, 1, 1 << 30, alpha * kLog2e, (float*)workspace, 0};
   JoinArgs j{cache, a.part, 0, dtype, o, m, {}};
-  j.splits = a.splits = simt_decode_splits(*c);
-  if (int rc = simt_dps_decode(a, (cudaStream_t)stream)) return rc;
+  const bool matrix = fast(TRITT_OP_DPS_DECODE, c->D, dtype, flags);
+  j.splits = a.splits = matrix ? mma_dps_decode_splits(*c) : simt_decode_splits(*c);
+  if (int rc = matrix ? mma_dps_decode(a, (cudaStream_t)stream) : simt_dps_decode(a, (cudaStream_t)stream)) return rc;
   return launch_join(j, (cudaStream_t)stream, false);
 }
 

@@ -253,6 +253,11 @@ bool sm100_tdp_decode_supported(int D, int dtype);
 size_t sm100_tdp_decode_workspace(const tritt_cache_t& c, int k2_window);
 int sm100_tdp_decode(const TdpDecodeArgs& a, void* workspace, void* o, float* lse, cudaStream_t stream);
 
+// ... the soft-max attention with warp-level matrix instructions (the same)
+bool mma_dps_decode_supported(int D, int dtype);
+int mma_dps_decode_splits(const tritt_cache_t& c);
+int mma_dps_decode(const DpsDecodeArgs& a, cudaStream_t stream);
+
 int simt_decode_splits(const tritt_cache_t& c);
 int simt_tdp_decode(const TdpDecodeArgs& a, cudaStream_t stream);
 int simt_dps_decode(const DpsDecodeArgs& a, cudaStream_t stream);
