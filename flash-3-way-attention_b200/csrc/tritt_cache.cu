@@ -283,8 +283,8 @@ int check_cache(const tritt_cache_t* c) {
     set_error("unknown code type %d", c->code);
     return -3;
   }
-  if (c->page_size < 8 || (c->page_size & (c->page_size - 1)) || (long long)c->page_size * c->table_pages > (1LL << 28)) {
-    set_error("a page must have a power of two from 8 tokens on, a table at most 2^28 in all (page_size %d, %d pages)", c->page_size,
+  if (c->page_size < 16 || (c->page_size & (c->page_size - 1)) || (long long)c->page_size * c->table_pages > (1LL << 28)) {
+    set_error("a page must have a power of two from 16 tokens on, a table at most 2^28 in all (page_size %d, %d pages)", c->page_size,
               c->table_pages);
     return -14;
   }
@@ -292,7 +292,7 @@ int check_cache(const tritt_cache_t* c) {
     set_error("null cache pointer");
     return -4;
   }
-  if (((uintptr_t)c->codes & 15) || ((uintptr_t)c->table & 3) || ((uintptr_t)c->context & 3)) {
+  if (((uintptr_t)c->codes & 15) || (((uintptr_t)c->table | (uintptr_t)c->context | (uintptr_t)c->exponents | (uintptr_t)c->lse) & 3)) {
     set_error("cache pointer is not aligned");
     return -5;
   }
@@ -406,7 +406,7 @@ int tritt_dps_append(const tritt_cache_t* c, const tritt_rows_t* rows, int dtype
   if (int rc = check_scratch(need, workspace, workspace_bytes)) return rc;
   const CacheArgs cache = cache_args(*c, status_word);
   if (int rc = launch_write(cache, rows, dtype, 3, (cudaStream_t)stream)) return rc;
-  DpsDecodeArgs a{cache, rows[1], dtype, kPartK1, kPartV1, 0, window(k_diff), alpha * kLog2e, (float*)workspace, 0};
+  DpsDecodeArgs a{cache, rows[1], dtype, kPartK1, kPartV1, 0, window(k_diff), 1, alpha * kLog2e, (float*)workspace, 0};
   JoinArgs j{cache, a.part, 0, dtype, nullptr, nullptr, rows[3]};
   const bool matrix = fast(TRITT_OP_DPS_DECODE, c->D, dtype, flags);
   j.splits = a.splits = matrix ? mma_dps_decode_splits(*c) : simt_decode_splits(*c);
@@ -426,7 +426,7 @@ int tritt_dps_decode(const tritt_cache_t* c, const tritt_rows_t* q, void* o, flo
   const size_t need = tritt_decode_workspace(TRITT_OP_DPS_DECODE, c, dtype, 0, 0, flags);
   if (int rc = check_scratch(need, workspace, workspace_bytes)) return rc;
   const CacheArgs cache = cache_args(*c, status_word);
-  DpsDecodeArgs a{cache, *q, dtype, kPartK2, kPartV2, 1, 1 << 30, alpha * kLog2e, (float*)workspace, 0};
+  DpsDecodeArgs a{cache, *q, dtype, kPartK2, kPartV2, 1, 1 << 30, 0, alpha * kLog2e, (float*)workspace, 0};
   JoinArgs j{cache, a.part, 0, dtype, o, m, {}};
   const bool matrix = fast(TRITT_OP_DPS_DECODE, c->D, dtype, flags);
   j.splits = a.splits = matrix ? mma_dps_decode_splits(*c) : simt_decode_splits(*c);

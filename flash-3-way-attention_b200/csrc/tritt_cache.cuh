@@ -243,7 +243,7 @@ struct TdpDecodeArgs {
 struct DpsDecodeArgs {
   CacheArgs cache;
   tritt_rows_t q;     // the rows that attend
-  int dtype, key_part, value_part, biased, window;
+  int dtype, key_part, value_part, biased, window, exact;   // exact: P in 22 bits (its result is quantised)
   float scale2;
   float* part;
   int splits;

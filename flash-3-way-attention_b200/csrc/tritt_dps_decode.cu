@@ -1,8 +1,11 @@
 // One soft-max attention of new tokens over two parts of the quantised cache, 16-bit queries, head dimension 64 or 128: either leg of the
 // dot-product-sum form (append: rows k2 over K1, SiLU(V1) within a window;  decode: rows q over K2, W with a bias for each token).
 //
-// Bound by HBM: a cached row is read once for up to 8 NT new tokens, 2 flops a byte and token.  There is no reuse to stage for, so
-// rows go from memory to registers and, as fp16, into warp-level matrix instructions with the cached rows as the 16-row operand:
+// Bound by HBM: a cached row is read once for up to 8 NT new tokens, 2 flops a byte and token.  Each warp has a ring of its own in
+// shared memory, filled by bulk copies (16 rows each, whole pages' neighbours) and 4-byte asynchronous ones (exponents, biases): no registers
+// wait for memory and nearly no instructions address it (a first form with loads to registers executed 1046 instructions for 32
+// tokens, more than HBM leaves time for: 253 us for a token of 32 x 8191).  Rows then go, as fp16, into warp-level matrix
+// instructions with the cached rows as the 16-row operand:
 //   S^T[16 tokens x 8 queries] = K Q^T,   O^T[D x 8 queries] += V^T P^T
 // (one token is an eighth of a tile instead of a sixteenth, and a query's statistics lie in the threads that hold its results).  The contraction of S
 // runs over the head dimension in any order, so a thread takes 16 contiguous bytes of a row for the elements that it needs; the rows of
@@ -11,10 +14,14 @@
 //
 // Codes are exact as fp16, the scores' powers of two are applied in fp32; P is formed times 2^(its row's exponent - the largest so far + 13),
 // so that values of any size meet in one accumulator, and its sum is taken before that.  Queries are brought to [1, 2) by a power of two.
+// Append forms P as the sum of two fp16 numbers (22 bits): its result is rounded again, to codes, and each element that a less exact one moves over
+// a border is off by a whole step (e4m3: 0.13 % of W's norm with one fp16 number, 2e-5 with two).
 #include "tritt_cache.cuh"
+#include "tritt_sm100.cuh"
 
 namespace tritt {
 namespace {
+using namespace sm100;
 
 constexpr int kWarps = 4;
 constexpr int kLift = 13;
@@ -43,28 +50,38 @@ __device__ __forceinline__ float power(int e) { return e > -127 ? __uint_as_floa
 template <int D, int CODE> struct Shape {
   static constexpr bool kWide = CODE == TRITT_CODE_F16;
   static constexpr int kRowBytes = D * (kWide ? 2 : 1);
-  static constexpr int kTokens = kRowBytes == 256 ? 16 : 32;    // of a tile: 2 to 4 KB of keys
+  static constexpr int kTokens = kRowBytes == 256 ? 16 : 32;    // of a tile: 4 or 8 KB of keys and values
   static constexpr int kBlocks = kTokens / 16;
   static constexpr int kKeyLoads = kRowBytes / 64;              // of 16 bytes, of a lane's row
   static constexpr int kValueWords = kRowBytes / 32;            // 32-bit words of a lane's eighth of a row
+  // a stage of the ring: keys, values, then biases, exponents of keys and values, and which tokens are there
+  static constexpr int kOffV = kTokens * kRowBytes, kOffBias = 2 * kOffV, kOffEk = kOffBias + 128, kOffEv = kOffEk + 32, kOffThere = kOffEv + 32;
+  static constexpr int kStage = kOffBias + 256;
+  static constexpr int kStages = 3;
+  static constexpr int kSmem = kWarps * kStages * kStage;
 };
 
-// A tile's keys: rows g and g + 8 of each block of 16 tokens; chunk t + 4 j of a row.
-template <int D, int CODE> struct Keys {
-  using S = Shape<D, CODE>;
-  uint4 v[S::kBlocks][2][S::kKeyLoads];
-};
-// Values: of tokens 2t, 2t + 1, 2t + 8, 2t + 9 of each block, the g-th eighth of the row.
-template <int D, int CODE> struct Values {
-  using S = Shape<D, CODE>;
-  uint32_t v[S::kBlocks][4][S::kValueWords];
-};
+// Copies of four bytes, and their arrival at a barrier.
+__device__ __forceinline__ void copy4(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
 
-template <int D, int CODE, int NT>
-__global__ void __launch_bounds__(kWarps * 32) dps_decode_kernel(const __grid_constant__ Params p) {
+template <int D, int CODE, int NT> constexpr int blocks_per_sm() {   // by registers and shared memory
+  return Shape<D, CODE>::kRowBytes == 64 ? (NT == 1 ? 4 : NT == 2 ? 3 : 2) : 2;
+}
+
+template <int D, int CODE, int NT, bool EXACT>
+__global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, CODE, NT>()) dps_decode_kernel(const __grid_constant__ Params p) {
   using S = Shape<D, CODE>;
-  constexpr int NB = S::kBlocks, TK = S::kTokens, KL = S::kKeyLoads, VW = S::kValueWords;
+  constexpr int NB = S::kBlocks, TK = S::kTokens, KL = S::kKeyLoads, VW = S::kValueWords, NS = S::kStages;
   constexpr int Q = 8 * NT;
+  extern __shared__ __align__(128) uint8_t ring_all[];
+  __shared__ uint64_t s_full[kWarps][NS];
+  __shared__ int s_abort;
+  __shared__ float4 s_side[kWarps][TK];   // of a tile's tokens: scale of scores, bias, scale of P
   __shared__ unsigned long long s_word[Q];
   __shared__ int s_lo[Q], s_pos[Q];
   __shared__ float s_scale[Q], s_m[kWarps][Q], s_l[kWarps][Q], s_out[Q][D + 4];
@@ -84,6 +101,64 @@ __global__ void __launch_bounds__(kWarps * 32) dps_decode_kernel(const __grid_co
   if (tile0 >= tile1) {
     for (int i = tid; i < rows; i += kWarps * 32) part[i * pitch] = -INFINITY, part[i * pitch + 1] = 0.f;
     return;
+  }
+
+  // --- the ring: this warp takes tiles tile0 + warp, + kWarps, ...
+  uint8_t* ring = ring_all + warp * NS * S::kStage;
+  uint64_t* full = s_full[warp];
+  if (lane == 0) {
+    for (int i = 0; i < NS; ++i) mbar_init(&full[i], 33);   // one arrival with the bulk copies' bytes, one of each lane
+    fence_barrier_init();
+  }
+  if (tid == 0) s_abort = 0;
+  const size_t part_rows = (size_t)ca.c.N << ca.page_log2;   // rows of one part of a page
+  const int row_mask = ca.c.page_size - 1;
+  // the page of this lane's token of a tile, -1: none, or no such token
+  auto find_page = [&](int tile) {
+    const int token = first + tile * TK + lane;
+    return lane < TK && tile < tile1 && token < end ? place_of(ca, b, token).page : -1;
+  };
+  auto fill = [&](int tile, int st, int page) {
+    uint8_t* to = ring + st * S::kStage;
+    const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
+    // (a group of 16 tokens lies in one page; its first token is there if any is)
+    if (lane == 0) {
+      *reinterpret_cast<uint32_t*>(to + S::kOffThere) = there;
+      mbar_arrive_expect_tx(&full[st], (uint32_t)(((there & 1u) + (there >> 16 & 1u)) * 2 * 16 * S::kRowBytes));
+    }
+    __syncwarp();
+    if (page >= 0) {
+      const int r = (first + tile * TK + lane) & row_mask;
+      const size_t at = (size_t)page * 4 * part_rows + ((size_t)head << ca.page_log2) + r;   // of part 0
+      // lanes 0, 16 copy a group's keys, lanes 1, 17 its values (lane 1's token may be behind the last: then lane 0 copies both)
+      const bool second = there >> (lane | 1) & 1;
+      if ((lane & 15) == 0) {
+        bulk_load(to + lane * S::kRowBytes, (const uint8_t*)ca.c.codes + (at + a.key_part * part_rows) * S::kRowBytes, 16 * S::kRowBytes, &full[st]);
+        if (!second)
+          bulk_load(to + S::kOffV + lane * S::kRowBytes, (const uint8_t*)ca.c.codes + (at + a.value_part * part_rows) * S::kRowBytes,
+                    16 * S::kRowBytes, &full[st]);
+      } else if ((lane & 15) == 1) {
+        bulk_load(to + S::kOffV + (lane - 1) * S::kRowBytes,
+                  (const uint8_t*)ca.c.codes + (at - 1 + a.value_part * part_rows) * S::kRowBytes, 16 * S::kRowBytes, &full[st]);
+      }
+      if (a.biased) copy4(to + S::kOffBias + lane * 4, ca.c.lse + (((size_t)page * ca.c.N + head) << ca.page_log2) + r);
+      if ((lane & 3) == 0) {
+        copy4(to + S::kOffEk + lane, ca.c.exponents + at + a.key_part * part_rows);
+        copy4(to + S::kOffEv + lane, ca.c.exponents + at + a.value_part * part_rows);
+      }
+    }
+    copies_arrive(&full[st]);
+  };
+  __syncwarp();
+  int next_page;   // of the tile that is filled next
+  {
+    int pg[NS + 1];
+#pragma unroll
+    for (int i = 0; i <= NS; ++i) pg[i] = find_page(tile0 + warp + i * kWarps);
+#pragma unroll
+    for (int i = 0; i < NS; ++i)
+      if (tile0 + warp + i * kWarps < tile1) fill(tile0 + warp + i * kWarps, i, pg[i]);
+    next_page = pg[NS];
   }
 
   // --- queries: fragments of Q^T, and what masks them
@@ -145,60 +220,6 @@ __global__ void __launch_bounds__(kWarps * 32) dps_decode_kernel(const __grid_co
     qs[nt][1] = s_scale[nt * 8 + 2 * t + 1];
   }
 
-  // --- tiles
-  const size_t part_rows = (size_t)ca.c.N << ca.page_log2;   // rows of one part of a page
-  auto row_base = [&](int page, int part_) { return ((size_t)page * 4 + part_) * part_rows + ((size_t)head << ca.page_log2); };
-  // pages of a tile's groups of eight tokens (one page each), in the first lanes
-  auto find_pages = [&](int tile) {
-    const int token = first + tile * TK + lane * 8;
-    return lane < TK / 8 && tile < tile1 && token < end ? place_of(ca, b, token).page : -1;
-  };
-  Keys<D, CODE> keys;
-  Values<D, CODE> values;
-  struct Side {                  // of this thread's tokens g, g + 8 of each block: exponents and biases
-    int ek[NB][2], ev[NB][2];
-    float bias[NB][2];
-  } side;
-  auto load_keys = [&](int tile, int pages) {
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int found = __shfl_sync(0xffffffffu, pages, nb * 2 + h), token = first + tile * TK + nb * 16 + h * 8 + g;
-        const int r = token & (ca.c.page_size - 1), page = token < end ? found : -1;
-        const size_t at = page >= 0 ? row_base(page, a.key_part) + r : 0;
-        const uint8_t* row = (const uint8_t*)ca.c.codes + at * S::kRowBytes + t * 16;
-#pragma unroll
-        for (int j = 0; j < KL; ++j)
-          keys.v[nb][h][j] = page >= 0 ? __ldg(reinterpret_cast<const uint4*>(row + j * 64)) : make_uint4(0u, 0u, 0u, 0u);
-        side.ek[nb][h] = page >= 0 ? __ldg(ca.c.exponents + at) : -1;
-        side.ev[nb][h] = page >= 0 ? __ldg(ca.c.exponents + row_base(page, a.value_part) + r) : -1;
-        side.bias[nb][h] = page >= 0 && a.biased ? __ldg(ca.c.lse + (((size_t)page * ca.c.N + head) << ca.page_log2) + r) : 0.f;
-      }
-  };
-  auto load_values = [&](int tile, int pages) {
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int found = __shfl_sync(0xffffffffu, pages, nb * 2 + (k >> 1));
-        const int token = first + tile * TK + nb * 16 + (k >> 1) * 8 + 2 * t + (k & 1);
-        const int r = token & (ca.c.page_size - 1), page = token < end ? found : -1;   // (what lies behind the last token is not looked at)
-        const uint8_t* row = (const uint8_t*)ca.c.codes + (page >= 0 ? row_base(page, a.value_part) + r : 0) * S::kRowBytes + g * (VW * 4);
-        uint32_t(&v)[VW] = values.v[nb][k];
-        if constexpr (VW == 2) {
-          const uint2 w = page >= 0 ? __ldg(reinterpret_cast<const uint2*>(row)) : make_uint2(0u, 0u);
-          v[0] = w.x, v[1] = w.y;
-        } else {
-#pragma unroll
-          for (int j = 0; j < VW / 4; ++j) {
-            const uint4 w = page >= 0 ? __ldg(reinterpret_cast<const uint4*>(row) + j) : make_uint4(0u, 0u, 0u, 0u);
-            v[4 * j] = w.x, v[4 * j + 1] = w.y, v[4 * j + 2] = w.z, v[4 * j + 3] = w.w;
-          }
-        }
-      }
-  };
-
   float acc[NT][D / 16][4], m[NT][2], l[NT][2];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
@@ -210,13 +231,45 @@ __global__ void __launch_bounds__(kWarps * 32) dps_decode_kernel(const __grid_co
     l[nt][0] = l[nt][1] = 0.f;
   }
   int v_exp = 0;   // largest exponent byte of the values so far
-  int tile = tile0 + warp;
-  int pages = find_pages(tile), pages_next = find_pages(tile + kWarps);
-  if (tile < tile1) {
-    load_keys(tile, pages);
-    load_values(tile, pages);
-  }
-  for (; tile < tile1; tile += kWarps) {
+  int st = 0, phase = 0;
+  for (int tile = tile0 + warp; tile < tile1; tile += kWarps) {
+    if (!__all_sync(0xffffffffu, mbar_wait(&full[st], phase, (volatile int*)&s_abort))) {
+      // give copies still in flight a bounded chance to land before the block ends
+      for (int i = 0; i < NS; ++i) {
+        const long long t0 = clock64();
+        while (!mbar_try_wait(&full[i], i < st ? phase ^ 1 : phase) && clock64() - t0 < kWaitTicks / 8) {
+        }
+      }
+      if (lane == 0 && ca.status) atomicOr(ca.status, 16);
+      break;
+    }
+    const uint8_t* from = ring + st * S::kStage;
+    const int token0 = first + tile * TK;
+    // one lane a token: scales, and whether all of the tile counts for every query
+    const uint32_t there = *reinterpret_cast<const uint32_t*>(from + S::kOffThere);
+    bool plain = token0 >= lo_all && token0 + TK <= ctx;
+    uint32_t bad;
+    {
+      const bool on = lane < TK && (there >> lane & 1);
+      const int ek = on ? from[S::kOffEk + lane] : 0, ev = on ? from[S::kOffEv + lane] : 0;
+      const float bias = on && a.biased ? *reinterpret_cast<const float*>(from + S::kOffBias + lane * 4) * kLog2e : 0.f;
+      bad = __ballot_sync(0xffffffffu, ek == 255 || ev == 255);
+      const int most = max(v_exp, (int)__reduce_max_sync(0xffffffffu, ev == 255 ? 0 : ev));
+      plain = plain && there == (TK == 32 ? 0xffffffffu : 0xffffu) && bad == 0u;
+      // (the products lie in the accumulator times 2^(largest exponent))
+      if (most > v_exp) {
+        const float grown = v_exp ? power(v_exp - most) : 1.f;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int mb = 0; mb < D / 16; ++mb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[nt][mb][e] *= grown;
+        v_exp = most;
+      }
+      if (lane < TK) s_side[warp][lane] = make_float4(power(ek - 127), bias, ev == 255 || !on ? 0.f : power(ev - most + kLift), 0.f);
+    }
+    __syncwarp();
     // S^T
     float s[NT][NB][4];
 #pragma unroll
@@ -227,52 +280,39 @@ __global__ void __launch_bounds__(kWarps * 32) dps_decode_kernel(const __grid_co
         for (int e = 0; e < 4; ++e) s[nt][nb][e] = 0.f;
 #pragma unroll
       for (int j = 0; j < KL; ++j) {
-        const uint32_t lo[4] = {keys.v[nb][0][j].x, keys.v[nb][0][j].y, keys.v[nb][0][j].z, keys.v[nb][0][j].w};
-        const uint32_t hi[4] = {keys.v[nb][1][j].x, keys.v[nb][1][j].y, keys.v[nb][1][j].z, keys.v[nb][1][j].w};
+        const uint4 r0 = *reinterpret_cast<const uint4*>(from + (nb * 16 + g) * S::kRowBytes + j * 64 + t * 16);
+        const uint4 r1 = *reinterpret_cast<const uint4*>(from + (nb * 16 + 8 + g) * S::kRowBytes + j * 64 + t * 16);
+        const uint32_t lo[4] = {r0.x, r0.y, r0.z, r0.w}, hi[4] = {r1.x, r1.y, r1.z, r1.w};
         constexpr int STEPS = S::kWide ? 2 : 4;   // contraction steps of 16 bytes
 #pragma unroll
-        for (int st = 0; st < STEPS; ++st) {
+        for (int k = 0; k < STEPS; ++k) {
           uint32_t f[4];
           if constexpr (S::kWide) {
-            f[0] = lo[2 * st], f[1] = hi[2 * st], f[2] = lo[2 * st + 1], f[3] = hi[2 * st + 1];
+            f[0] = lo[2 * k], f[1] = hi[2 * k], f[2] = lo[2 * k + 1], f[3] = hi[2 * k + 1];
           } else {
-            bytes_to_halves<CODE>(lo[st], f[0], f[2]);
-            bytes_to_halves<CODE>(hi[st], f[1], f[3]);
+            bytes_to_halves<CODE>(lo[k], f[0], f[2]);
+            bytes_to_halves<CODE>(hi[k], f[1], f[3]);
           }
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_16816(s[nt][nb], f, qf[nt][j * STEPS + st][0], qf[nt][j * STEPS + st][1]);
+          for (int nt = 0; nt < NT; ++nt) mma_16816(s[nt][nb], f, qf[nt][j * STEPS + k][0], qf[nt][j * STEPS + k][1]);
         }
       }
     }
-    const Side now = side;
-    if (tile + kWarps < tile1) load_keys(tile + kWarps, pages_next);
-    const int pages_after = find_pages(tile + 2 * kWarps);
-    // largest exponent of the values, and whether every token of the tile counts for every query
-    const int token0 = first + tile * TK;
-    bool plain = token0 >= lo_all && token0 + TK <= ctx;
-    int ev_most = 0;
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        plain = plain && now.ek[nb][h] >= 0 && now.ek[nb][h] != 255 && now.ev[nb][h] != 255;
-        ev_most = max(ev_most, now.ev[nb][h] == 255 ? 0 : now.ev[nb][h]);
-      }
-    plain = __all_sync(0xffffffffu, plain);
-    ev_most = max(v_exp, __reduce_max_sync(0xffffffffu, ev_most));
     // scores in log2 units
+    float vf[NB][2];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float kf = power(now.ek[nb][h] - 127), bias = now.bias[nb][h] * kLog2e;
+        const int k = nb * 16 + h * 8 + g;
+        const float4 side = s_side[warp][k];
+        vf[nb][h] = side.z;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int q = 0; q < 2; ++q) s[nt][nb][2 * h + q] = fmaf(s[nt][nb][2 * h + q] * kf, qs[nt][q], bias);
+          for (int q = 0; q < 2; ++q) s[nt][nb][2 * h + q] = fmaf(s[nt][nb][2 * h + q] * side.x, qs[nt][q], side.y);
         if (!plain) {
-          const int token = token0 + nb * 16 + h * 8 + g;
-          const bool there = now.ek[nb][h] >= 0, bad = now.ek[nb][h] == 255 || now.ev[nb][h] == 255;
+          const int token = token0 + k;
           bool missing = false;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
@@ -289,19 +329,18 @@ __global__ void __launch_bounds__(kWarps * 32) dps_decode_kernel(const __grid_co
                   seen = seen && token <= s_pos[i];
                 }
               }
-              missing = missing || (seen && !there);
+              missing = missing || (seen && !(there >> k & 1));
               float& x = s[nt][nb][2 * h + q];
-              x = seen && there ? (bad ? __uint_as_float(0x7fffffffu) : x) : -INFINITY;
+              x = seen && (there >> k & 1) ? (bad >> k & 1 ? __uint_as_float(0x7fffffffu) : x) : -INFINITY;
             }
           if (missing && ca.status) atomicOr(ca.status, kStatusPlace);
         }
       }
     // running maximum, P
-    uint32_t pf[NT][NB][2];
-    const float grown = power(v_exp - ev_most);
+    uint32_t pf[NT][NB][2], pl[EXACT ? NT : 1][NB][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      float corr[2], base[2];
+      float base[2], corr[2];
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         float mx = m[nt][q];
@@ -314,54 +353,89 @@ __global__ void __launch_bounds__(kWarps * 32) dps_decode_kernel(const __grid_co
         corr[q] = exp2f(m[nt][q] - base[q]);
         m[nt][q] = mx;
         l[nt][q] *= corr[q];
-        corr[q] *= grown;
       }
+      if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
 #pragma unroll
-      for (int mb = 0; mb < D / 16; ++mb)
+        for (int mb = 0; mb < D / 16; ++mb)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[nt][mb][e] *= corr[e & 1];
+          for (int e = 0; e < 4; ++e) acc[nt][mb][e] *= corr[e & 1];
+      }
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float vf = now.ev[nb][h] == 255 ? 0.f : power(now.ev[nb][h] - ev_most + kLift);
           const float p0 = exp2f(s[nt][nb][2 * h] - base[0]), p1 = exp2f(s[nt][nb][2 * h + 1] - base[1]);
           l[nt][0] += p0;
           l[nt][1] += p1;
-          pf[nt][nb][h] = transposed(pack_half(p0 * vf, p1 * vf));
+          const float x0 = p0 * vf[nb][h], x1 = p1 * vf[nb][h];
+          const uint32_t high = pack_half(x0, x1);
+          pf[nt][nb][h] = transposed(high);
+          if constexpr (EXACT) {
+            const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&high));
+            pl[nt][nb][h] = transposed(pack_half(x0 - r.x, x1 - r.y));
+          }
         }
     }
-    v_exp = ev_most;
     // O^T += V^T P^T
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
+    for (int nb = 0; nb < NB; ++nb) {
+      // of tokens 2t, 2t + 1, 2t + 8, 2t + 9 of the block, the g-th eighth of the row
+      uint32_t v[4][VW];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int row = nb * 16 + (k >> 1) * 8 + 2 * t + (k & 1);
+        const uint8_t* r = from + S::kOffV + row * S::kRowBytes + g * (VW * 4);
+        if constexpr (VW == 2) {
+          const uint2 w = *reinterpret_cast<const uint2*>(r);
+          v[k][0] = w.x, v[k][1] = w.y;
+        } else {
+#pragma unroll
+          for (int j = 0; j < VW / 4; ++j) {
+            const uint4 w = *(reinterpret_cast<const uint4*>(r) + j);
+            v[k][4 * j] = w.x, v[k][4 * j + 1] = w.y, v[k][4 * j + 2] = w.z, v[k][4 * j + 3] = w.w;
+          }
+        }
+        if (!plain && !(there >> row & 1)) {   // (what lies there is of another tile, or no number)
+#pragma unroll
+          for (int w = 0; w < VW; ++w) v[k][w] = 0u;
+        }
+      }
 #pragma unroll
       for (int w = 0; w < VW; ++w) {
         if constexpr (S::kWide) {
           // two elements of four tokens: one block of 16 rows of V^T
           uint32_t f[4];
-          f[0] = __byte_perm(values.v[nb][0][w], values.v[nb][1][w], 0x5410);
-          f[1] = __byte_perm(values.v[nb][0][w], values.v[nb][1][w], 0x7632);
-          f[2] = __byte_perm(values.v[nb][2][w], values.v[nb][3][w], 0x5410);
-          f[3] = __byte_perm(values.v[nb][2][w], values.v[nb][3][w], 0x7632);
+          f[0] = __byte_perm(v[0][w], v[1][w], 0x5410);
+          f[1] = __byte_perm(v[0][w], v[1][w], 0x7632);
+          f[2] = __byte_perm(v[2][w], v[3][w], 0x5410);
+          f[3] = __byte_perm(v[2][w], v[3][w], 0x7632);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_16816(acc[nt][w], f, pf[nt][nb][0], pf[nt][nb][1]);
+          for (int nt = 0; nt < NT; ++nt) {
+            mma_16816(acc[nt][w], f, pf[nt][nb][0], pf[nt][nb][1]);
+            if constexpr (EXACT) mma_16816(acc[nt][w], f, pl[nt][nb][0], pl[nt][nb][1]);
+          }
         } else {
           // four elements: two blocks
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            const uint32_t lo = __byte_perm(values.v[nb][0][w], values.v[nb][1][w], half ? 0x7362 : 0x5140);
-            const uint32_t hi = __byte_perm(values.v[nb][2][w], values.v[nb][3][w], half ? 0x7362 : 0x5140);
+            const uint32_t lo = __byte_perm(v[0][w], v[1][w], half ? 0x7362 : 0x5140);
+            const uint32_t hi = __byte_perm(v[2][w], v[3][w], half ? 0x7362 : 0x5140);
             uint32_t f[4];
             bytes_to_halves<CODE>(lo, f[0], f[1]);
             bytes_to_halves<CODE>(hi, f[2], f[3]);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_16816(acc[nt][2 * w + half], f, pf[nt][nb][0], pf[nt][nb][1]);
+            for (int nt = 0; nt < NT; ++nt) {
+              mma_16816(acc[nt][2 * w + half], f, pf[nt][nb][0], pf[nt][nb][1]);
+              if constexpr (EXACT) mma_16816(acc[nt][2 * w + half], f, pl[nt][nb][0], pl[nt][nb][1]);
+            }
           }
         }
       }
-    if (tile + kWarps < tile1) load_values(tile + kWarps, pages_next);
-    pages_next = pages_after;
+    }
+    __syncwarp();   // every lane has read this stage
+    if (tile + NS * kWarps < tile1) fill(tile + NS * kWarps, st, next_page);
+    next_page = find_page(tile + (NS + 1) * kWarps);
+    if (++st == NS) st = 0, phase ^= 1;
   }
 
   // --- the warps' results on their common maximum, added up in order
@@ -422,7 +496,9 @@ Plan plan_of(int n, int D) {
 }
 
 template <int D, int CODE, int NT> int launch(const Params& p, cudaStream_t stream) {
-  dps_decode_kernel<D, CODE, NT><<<dim3(p.a.splits, p.a.cache.c.B * p.a.cache.c.N, p.query_groups), kWarps * 32, 0, stream>>>(p);
+  auto kern = p.a.exact ? dps_decode_kernel<D, CODE, NT, true> : dps_decode_kernel<D, CODE, NT, false>;
+  TRITT_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D, CODE>::kSmem));
+  kern<<<dim3(p.a.splits, p.a.cache.c.B * p.a.cache.c.N, p.query_groups), kWarps * 32, Shape<D, CODE>::kSmem, stream>>>(p);
   count_launch();
   TRITT_CUDA_OK(cudaGetLastError());
   return 0;

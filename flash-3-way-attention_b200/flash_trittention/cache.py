@@ -53,11 +53,11 @@ class TrittentionCache(NamedTuple):
 
 def new_cache(pages: int, page_size: int, heads: int, head_dim: int, dtype: torch.dtype = torch.float8_e4m3fn, device="cuda",
               dps: bool = False) -> TrittentionCache:
-    """An empty cache of ``pages`` pages of ``page_size`` tokens (a power of two from 8 on); ``dps``: for the dot-product-sum form."""
+    """An empty cache of ``pages`` pages of ``page_size`` tokens (a power of two from 16 on); ``dps``: for the dot-product-sum form."""
     if dtype not in _native.CODES:
         raise ValueError(f"a cache is held in float16, float8_e4m3fn or int8, not {dtype}")
-    if page_size < 8 or page_size & (page_size - 1):
-        raise ValueError(f"page_size must be a power of 2 from 8 on, got {page_size}")
+    if page_size < 16 or page_size & (page_size - 1):
+        raise ValueError(f"page_size must be a power of 2 from 16 on, got {page_size}")
     if head_dim not in HEAD_DIMS:
         raise ValueError(f"head_dim must be one of {HEAD_DIMS}, got {head_dim}")
     shape = (pages, 4, heads, page_size)

@@ -293,7 +293,7 @@ typedef struct {
   void* codes;                 /* [pages, 4, N, page_size, D] */
   unsigned char* exponents;    /* [pages, 4, N, page_size] */
   float* lse;                  /* [pages, N, page_size] natural-log units, or null (triple dot product) */
-  int pages, page_size, N, D, code;   /* page_size: a power of two from 8 on;  D: 16, 32, 64, 128 or 256 */
+  int pages, page_size, N, D, code;   /* page_size: a power of two from 16 on;  D: 16, 32, 64, 128 or 256 */
   const int* table;            /* [B, table_pages] */
   long long table_stride;      /* elements between two sequences' tables */
   int table_pages;

@@ -43,10 +43,10 @@ def _rows(B, N, n, D, dtype, seed, strided):
 WRITES = [  # B N n D dtype code page contexts counts strided
     (1, 1, 1, 64, "bf16", "e4m3", 16, [0], None, False),
     (3, 4, 21, 64, "fp16", "e4m3", 16, [0, 5, 40], [21, 1, 0], True),
-    (2, 5, 9, 128, "bf16", "fp16", 8, [7, 8], None, True),
+    (2, 5, 9, 128, "bf16", "fp16", 16, [15, 16], None, True),
     (4, 3, 1, 128, "fp32", "int8", 64, [63, 64, 0, -1], None, False),
     (2, 2, 70, 32, "fp32", "fp16", 32, [3, 31], [70, 69], False),
-    (1, 6, 33, 16, "fp16", "int8", 8, [2], None, True),
+    (1, 6, 33, 16, "fp16", "int8", 16, [2], None, True),
     (2, 3, 12, 256, "bf16", "int8", 128, [120, 0], [12, 99], True),
 ]
 
@@ -188,7 +188,7 @@ TDP = [  # B N n D dtype code page contexts windows parents precision
     (2, 3, 5, 64, "fp16", "int8", 32, [37, 130], (None,) * 4, None),
     (2, 2, 7, 64, "bf16", "e4m3", 16, [150, 33], (None,) * 4, _tree(7, 2)),
     (2, 1, 9, 128, "fp16", "fp16", 64, [140, 0], (20, 50, 10, 3), _tree(9, 3)),
-    (1, 2, 4, 128, "bf16", "int8", 8, [260], (128, 128, 32, 32), None),
+    (1, 2, 4, 128, "bf16", "int8", 16, [260], (128, 128, 32, 32), None),
     (1, 1, 3, 64, "fp16", "fp16", 16, [300], (None, 0, None, None), [-1, 0, 0]),
     (1, 1, 3, 64, "fp16", "e4m3", 16, [200], (0, None, None, 0), None),
     (1, 2, 2, 64, "bf16", "fp16", 256, [257], (None, None, 0, 0), None),
@@ -234,7 +234,7 @@ DPS = [  # B N n D dtype code page contexts k_diff parents
     (2, 3, 5, 64, "fp16", "int8", 32, [37, 530], 100, None),
     (2, 2, 7, 64, "bf16", "e4m3", 16, [150, 33], 10, _tree(7, 2)),
     (2, 1, 9, 128, "fp16", "fp16", 64, [140, 0], 1024, _tree(9, 3)),
-    (1, 2, 17, 128, "bf16", "int8", 8, [260], 0, None),
+    (1, 2, 17, 128, "bf16", "int8", 16, [260], 0, None),
     (1, 2, 33, 64, "bf16", "fp16", 256, [257], 5000, _tree(33, 2)),
     (1, 1, 64, 128, "fp16", "e4m3", 16, [100], 64, _tree(64, 1)),
     (1, 1, 130, 64, "fp16", "fp16", 16, [10], 40, None),
@@ -563,7 +563,7 @@ def test_new_cache():
     c = ft.new_cache(3, 16, 2, 64, torch.int8, "cpu", dps=True)
     assert c.codes.shape == (3, 4, 2, 16, 64) and c.exponents.shape == (3, 4, 2, 16) and c.lse.shape == (3, 2, 16)
     assert ft.new_cache(1, 8, 1, 16, device="cpu").lse is None
-    for kw in (dict(dtype=torch.float32), dict(page_size=12), dict(page_size=4), dict(head_dim=48)):
+    for kw in (dict(dtype=torch.float32), dict(page_size=12), dict(page_size=8), dict(head_dim=48)):
         with pytest.raises(ValueError):
             ft.new_cache(**{**dict(pages=1, page_size=16, heads=1, head_dim=64, device="cpu"), **kw})
 
@@ -612,6 +612,7 @@ def test_refusals():
         lambda: ft.dps_decode(x, d._replace(lse=d.lse.half()), table, ctx),
         lambda: ft.tdp_decode(x, ft.TrittentionCache(c.codes[..., :16, :].float(), c.exponents), table, ctx),
         lambda: ft.tdp_decode(x, ft.TrittentionCache(c.codes[:, :, :, :12].contiguous(), c.exponents[..., :12].contiguous()), table, ctx),
+        lambda: ft.tdp_decode(x, ft.TrittentionCache(c.codes[:, :, :, :8].contiguous(), c.exponents[..., :8].contiguous()), table, ctx),
     ]
     for i, call in enumerate(bad):
         with pytest.raises(ValueError):
@@ -632,7 +633,7 @@ def test_the_librarys_own_refusals():
                 lib.tritt_dps_append(c, r, dtype, 0.1, 1, ws, size, None, 0, None), lib.tritt_dps_decode(c, r, o, None, dtype, 0.1, ws, size, None, 0, None)]
 
     for kw, rc in [(dict(B=0), -1), (dict(n=0), -1), (dict(pages=0), -1), (dict(D=48), -2), (dict(code=3), -3), (dict(page_size=12), -14),
-                   (dict(page_size=4), -14), (dict(page_size=1 << 20, table_pages=1 << 12), -14), (dict(codes=None), -4), (dict(table=None), -4),
+                   (dict(page_size=8), -14), (dict(page_size=1 << 20, table_pages=1 << 12), -14), (dict(codes=None), -4), (dict(table=None), -4),
                    (dict(context=None), -4), (dict(codes=p + 8), -5), (dict(ancestors=p, n=65), -15), (dict(B=32768, N=2), -11),
                    (dict(B=8192, N=2, n=1 << 20), -11)]:
         c = _native.Cache(**{**good, **kw})
