@@ -134,38 +134,7 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ JoinA
     if (j.lse && lane == 0) j.lse[row] = lse;
     return;
   }
-  // append: W into the cache (a token that is not there has no place)
-  bool on = i < new_tokens(a, b);
-  Place at{-1, 0};
-  if (on) {
-    at = place_of(a, b, context_of(a, b) + i);
-    on = at.page >= 0;
-  }
-  if (on && col < D) {
-    float v[8];
-    load8((const T*)j.v2.p + rows_at(j.v2, b, head, i) + col, v);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] *= v[e];
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = 0.f;
-  }
-  // (lanes past the row have zeros, which change no maximum)
-  const int byte = exponent_byte<CODE>(largest_of_row<32>(largest8(f)));
-  if (!on) return;
-  const size_t to = row_of(a, at, kPartV2, head);
-  if (lane == 0) {
-    a.c.exponents[to] = (unsigned char)byte;
-    a.c.lse[lse_of(a, at, head)] = lse;
-  }
-  if (col < D) {
-    const float scale = to_code_scale(byte);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = byte == 255 ? 0.f : f[e] * scale;
-    Codes8<CODE> codes;
-    codes.encode(f);
-    codes.store((uint8_t*)a.c.codes + to * (size_t)(D * (CODE == TRITT_CODE_F16 ? 2 : 1)), col);
-  }
+  join_into_cache<T, CODE>(a, b, head, i, col, f, lse, j.v2);
 }
 
 template <typename T, int CODE, int D> int write_for(const WriteArgs& w, cudaStream_t stream) {
@@ -367,7 +336,8 @@ size_t tritt_decode_workspace(int op, const tritt_cache_t* c, int dtype, int k1_
   if (check_cache(c)) return 0;
   (void)k1_window;
   if (op == TRITT_OP_TDP_DECODE && fast(op, c->D, dtype, flags)) return sm100_tdp_decode_workspace(*c, window(k2_window));
-  return part_bytes(*c, fast(op, c->D, dtype, flags) ? mma_dps_decode_splits(*c) : simt_decode_splits(*c));
+  if (fast(op, c->D, dtype, flags)) return mma_dps_decode_workspace(*c);
+  return part_bytes(*c, simt_decode_splits(*c));
 }
 
 int tritt_tdp_decode(const tritt_cache_t* c, const tritt_rows_t* q, void* o, float* lse, int dtype, float alpha, int k1_window,
@@ -407,10 +377,10 @@ int tritt_dps_append(const tritt_cache_t* c, const tritt_rows_t* rows, int dtype
   const CacheArgs cache = cache_args(*c, status_word);
   if (int rc = launch_write(cache, rows, dtype, 3, (cudaStream_t)stream)) return rc;
   DpsDecodeArgs a{cache, rows[1], dtype, kPartK1, kPartV1, 0, window(k_diff), 1, alpha * kLog2e, (float*)workspace, 0};
+  if (fast(TRITT_OP_DPS_APPEND, c->D, dtype, flags)) return mma_dps_decode(a, workspace, nullptr, nullptr, &rows[3], (cudaStream_t)stream);
   JoinArgs j{cache, a.part, 0, dtype, nullptr, nullptr, rows[3]};
-  const bool matrix = fast(TRITT_OP_DPS_DECODE, c->D, dtype, flags);
-  j.splits = a.splits = matrix ? mma_dps_decode_splits(*c) : simt_decode_splits(*c);
-  if (int rc = matrix ? mma_dps_decode(a, (cudaStream_t)stream) : simt_dps_decode(a, (cudaStream_t)stream)) return rc;
+  j.splits = a.splits = simt_decode_splits(*c);
+  if (int rc = simt_dps_decode(a, (cudaStream_t)stream)) return rc;
   return launch_join(j, (cudaStream_t)stream, false);
 }
 
@@ -427,10 +397,10 @@ int tritt_dps_decode(const tritt_cache_t* c, const tritt_rows_t* q, void* o, flo
   if (int rc = check_scratch(need, workspace, workspace_bytes)) return rc;
   const CacheArgs cache = cache_args(*c, status_word);
   DpsDecodeArgs a{cache, *q, dtype, kPartK2, kPartV2, 1, 1 << 30, 0, alpha * kLog2e, (float*)workspace, 0};
+  if (fast(TRITT_OP_DPS_DECODE, c->D, dtype, flags)) return mma_dps_decode(a, workspace, o, m, nullptr, (cudaStream_t)stream);
   JoinArgs j{cache, a.part, 0, dtype, o, m, {}};
-  const bool matrix = fast(TRITT_OP_DPS_DECODE, c->D, dtype, flags);
-  j.splits = a.splits = matrix ? mma_dps_decode_splits(*c) : simt_decode_splits(*c);
-  if (int rc = matrix ? mma_dps_decode(a, (cudaStream_t)stream) : simt_dps_decode(a, (cudaStream_t)stream)) return rc;
+  j.splits = a.splits = simt_decode_splits(*c);
+  if (int rc = simt_dps_decode(a, (cudaStream_t)stream)) return rc;
   return launch_join(j, (cudaStream_t)stream, false);
 }
 

@@ -107,10 +107,7 @@ template <> struct Codes8<TRITT_CODE_F16> {
 // Four bytes as two pairs of fp16.
 template <int CODE> __device__ __forceinline__ void bytes_to_halves(uint32_t v, uint32_t& lo, uint32_t& hi) {
   if constexpr (CODE == TRITT_CODE_E4M3) {
-    const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(v & 0xffffu), __NV_E4M3);
-    const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(v >> 16), __NV_E4M3);
-    lo = (uint32_t)a.x | (uint32_t)a.y << 16;
-    hi = (uint32_t)b.x | (uint32_t)b.y << 16;
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(v));
   } else {
     // 0x64bb is 1024 + bb in fp16; with the sign bit turned over bb is the element + 128
     const uint32_t u = v ^ 0x80808080u;
@@ -217,6 +214,44 @@ __device__ __forceinline__ void store_row(const CacheArgs& a, bool on, Place at,
   if (col == 0) a.c.exponents[row] = (unsigned char)byte;
 }
 
+// Append: a warp's row (eight elements from column `col` on of its first lanes) times v2 becomes W in the cache, with its log-sum-exp.  All
+// lanes call it; a token that is not there has no place.
+template <typename T, int CODE>
+__device__ __forceinline__ void join_into_cache(const CacheArgs& a, int b, int head, int i, int col, float (&f)[8], float lse, const tritt_rows_t& v2) {
+  const int D = a.c.D;
+  bool on = i < new_tokens(a, b);
+  Place at{-1, 0};
+  if (on) {
+    at = place_of(a, b, context_of(a, b) + i);
+    on = at.page >= 0;
+  }
+  if (on && col < D) {
+    float v[8];
+    load8((const T*)v2.p + rows_at(v2, b, head, i) + col, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] *= v[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = 0.f;
+  }
+  // (lanes past the row have zeros, which change no maximum)
+  const int byte = exponent_byte<CODE>(largest_of_row<32>(largest8(f)));
+  if (!on) return;
+  const size_t to = row_of(a, at, kPartV2, head);
+  if (col == 0) {
+    a.c.exponents[to] = (unsigned char)byte;
+    a.c.lse[lse_of(a, at, head)] = lse;
+  }
+  if (col < D) {
+    const float scale = to_code_scale(byte);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = byte == 255 ? 0.f : f[e] * scale;
+    Codes8<CODE> codes;
+    codes.encode(f);
+    codes.store((uint8_t*)a.c.codes + to * (size_t)(D * (CODE == TRITT_CODE_F16 ? 2 : 1)), col);
+  }
+}
+
 // ---------------------------------------------------------------- parts of a row's soft-max, and what becomes of them
 // Each split of a new token's attended tokens leaves its maximum (log2 units), sum and unnormalised result in the workspace,
 // [rows][splits][D + 2] fp32 (rows = (b * N + head) * n + i), and a second kernel joins them.
@@ -255,8 +290,8 @@ int sm100_tdp_decode(const TdpDecodeArgs& a, void* workspace, void* o, float* ls
 
 // ... the soft-max attention with warp-level matrix instructions (the same)
 bool mma_dps_decode_supported(int D, int dtype);
-int mma_dps_decode_splits(const tritt_cache_t& c);
-int mma_dps_decode(const DpsDecodeArgs& a, cudaStream_t stream);
+size_t mma_dps_decode_workspace(const tritt_cache_t& c);
+int mma_dps_decode(const DpsDecodeArgs& a, void* workspace, void* o, float* lse, const tritt_rows_t* v2, cudaStream_t stream);
 
 int simt_decode_splits(const tritt_cache_t& c);
 int simt_tdp_decode(const TdpDecodeArgs& a, cudaStream_t stream);

@@ -10,7 +10,11 @@
 // (one token is an eighth of a tile instead of a sixteenth, and a query's statistics lie in the threads that hold its results).  The contraction of S
 // runs over the head dimension in any order, so a thread takes 16 contiguous bytes of a row for the elements that it needs; the rows of
 // V^T are columns of V in any order, so a thread takes D / 8 contiguous elements of four tokens and pairs them by byte permutes.  P^T is
-// the transpose of S^T's fragments (movmatrix).  A warp walks its tiles of tokens with the next keys and values in flight.
+// the transpose of S^T's fragments (movmatrix).
+//
+// The line of all (sequence, head, group of new tokens, tile) steps is cut in equal parts, one for each block that the chip holds at
+// once: sequences differ in length, and nothing of it is known to the host.  A block's warps take its tiles in turn; each piece of a group
+// leaves maximum, sum and result, which a second kernel joins in a fixed order.
 //
 // Codes are exact as fp16, the scores' powers of two are applied in fp32; P is formed times 2^(its row's exponent - the largest so far + 13),
 // so that values of any size meet in one accumulator, and its sum is taken before that.  Queries are brought to [1, 2) by a power of two.
@@ -18,17 +22,32 @@
 // a border is off by a whole step (e4m3: 0.13 % of W's norm with one fp16 number, 2e-5 with two).
 #include "tritt_cache.cuh"
 #include "tritt_sm100.cuh"
+#include "tritt_sm100_tdp.cuh"
 
 namespace tritt {
 namespace {
 using namespace sm100;
 
 constexpr int kWarps = 4;
-constexpr int kLift = 13;
+constexpr int kLift = 5;        // P is formed times 2^5; the reference is raised when a score is 2^8 above it: at most 2^13
+constexpr float kGap = 8.f;
+constexpr int kLeastSteps = 8;  // of a block: two tiles a warp
+
+// What the line of steps has of one sequence.
+struct Line {
+  int ctx, cnt;          // tokens before the new ones, new ones
+  int groups, tiles;     // groups of new tokens; tiles of a group (the most of any)
+};
+struct LineEntry {       // in the workspace, for the kernel that joins
+  long long base, group_base;
+  Line line;
+};
 
 struct Params {
   DpsDecodeArgs a;
-  int query_groups;   // of 8 NT new tokens
+  LineEntry* table;      // [B]
+  float* part;           // [pieces][Q][D + 2]
+  int ctas;
 };
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -58,8 +77,16 @@ template <int D, int CODE> struct Shape {
   static constexpr int kOffV = kTokens * kRowBytes, kOffBias = 2 * kOffV, kOffEk = kOffBias + 128, kOffEv = kOffEk + 32, kOffThere = kOffEv + 32;
   static constexpr int kStage = kOffBias + 256;
   static constexpr int kStages = 3;
-  static constexpr int kSmem = kWarps * kStages * kStage;
+  static constexpr int kRing = kWarps * kStages * kStage;
 };
+// The ring's memory takes the warps' results at the end of a piece: [warps][Q][D + 4] fp32.
+template <int D, int CODE, int NT> constexpr int smem_bytes() {
+  constexpr int out = kWarps * 8 * NT * (D + 4) * 4;
+  return Shape<D, CODE>::kRing > out ? Shape<D, CODE>::kRing : out;
+}
+template <int D, int CODE, int NT> constexpr int blocks_per_sm() {   // by registers and shared memory
+  return Shape<D, CODE>::kRowBytes == 64 ? (NT == 1 ? 4 : NT == 2 ? 3 : 2) : 2;
+}
 
 // Copies of four bytes, and their arrival at a barrier.
 __device__ __forceinline__ void copy4(void* dst, const void* src) {
@@ -69,420 +96,573 @@ __device__ __forceinline__ void copies_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-template <int D, int CODE, int NT> constexpr int blocks_per_sm() {   // by registers and shared memory
-  return Shape<D, CODE>::kRowBytes == 64 ? (NT == 1 ? 4 : NT == 2 ? 3 : 2) : 2;
+// Which row of a block of 16 is row r of the fragments: with rows of 64 bytes, so that the four that a quarter of the lanes' value loads
+// touch lie in both halves of the banks.
+template <int ROW_BYTES> __device__ __forceinline__ int actual_row(int r) { return ROW_BYTES == 64 ? r ^ (r >> 1 & 1) : r; }
+
+template <int TK, int Q> __device__ __forceinline__ Line line_of(const DpsDecodeArgs& a, int b) {
+  Line l;
+  l.ctx = context_of(a.cache, b);
+  l.cnt = new_tokens(a.cache, b);
+  l.groups = (l.cnt + Q - 1) / Q;
+  l.tiles = l.cnt ? (min(l.ctx, a.window) + l.cnt + 15 + TK - 1) / TK : 0;   // (a group's first tile starts at a multiple of 16)
+  return l;
+}
+// CTAs that the line is cut for.
+__host__ __device__ __forceinline__ int parts_of(long long total, int ctas) {
+  const long long n = total / kLeastSteps;
+  return n < 1 ? 1 : n < ctas ? (int)n : ctas;
 }
 
-template <int D, int CODE, int NT, bool EXACT>
+// ONE: a single new token (a query's column of the fragments; the others are not worked on).
+template <int D, int CODE, int NT, bool ONE, bool EXACT>
 __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, CODE, NT>()) dps_decode_kernel(const __grid_constant__ Params p) {
   using S = Shape<D, CODE>;
-  constexpr int NB = S::kBlocks, TK = S::kTokens, KL = S::kKeyLoads, VW = S::kValueWords, NS = S::kStages;
-  constexpr int Q = 8 * NT;
+  constexpr int NB = S::kBlocks, TK = S::kTokens, KL = S::kKeyLoads, VW = S::kValueWords, NS = S::kStages, RB = S::kRowBytes;
+  constexpr int Q = 8 * NT, NQ = ONE ? 1 : 2;
   extern __shared__ __align__(128) uint8_t ring_all[];
   __shared__ uint64_t s_full[kWarps][NS];
   __shared__ int s_abort;
+  __shared__ long long s_total;
   __shared__ float4 s_side[kWarps][TK];   // of a tile's tokens: scale of scores, bias, scale of P
   __shared__ unsigned long long s_word[Q];
   __shared__ int s_lo[Q], s_pos[Q];
-  __shared__ float s_scale[Q], s_m[kWarps][Q], s_l[kWarps][Q], s_out[Q][D + 4];
+  __shared__ float s_scale[Q], s_m[kWarps][Q], s_l[kWarps][Q];
   const DpsDecodeArgs& a = p.a;
   const CacheArgs& ca = a.cache;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int head = blockIdx.y % ca.c.N, b = blockIdx.y / ca.c.N, split = blockIdx.x, i0 = blockIdx.z * Q;
-  const int ctx = context_of(ca, b), cnt = new_tokens(ca, b), nq = min(Q, cnt - i0);
-  const int rows = min(Q, ca.c.n - i0);   // rows of the result
-  float* part = a.part + (((size_t)blockIdx.y * ca.c.n + i0) * a.splits + split) * (D + 2);
-  const size_t pitch = (size_t)a.splits * (D + 2);
-
-  // tokens that any of these queries attends to: first .. end - 1, in tiles from a multiple of 16 on
-  const int first = nq > 0 ? max(0, min(ctx, ctx + (ca.c.ancestors ? 0 : i0) - a.window)) & ~15 : 0, end = nq > 0 ? ctx + i0 + nq : 0;
-  const int tiles = (end - first + TK - 1) / TK, each = (tiles + a.splits - 1) / a.splits;
-  const int tile0 = split * each, tile1 = min(tiles, tile0 + each);
-  if (tile0 >= tile1) {
-    for (int i = tid; i < rows; i += kWarps * 32) part[i * pitch] = -INFINITY, part[i * pitch + 1] = 0.f;
-    return;
-  }
-
-  // --- the ring: this warp takes tiles tile0 + warp, + kWarps, ...
   uint8_t* ring = ring_all + warp * NS * S::kStage;
   uint64_t* full = s_full[warp];
   if (lane == 0) {
     for (int i = 0; i < NS; ++i) mbar_init(&full[i], 33);   // one arrival with the bulk copies' bytes, one of each lane
     fence_barrier_init();
   }
-  if (tid == 0) s_abort = 0;
-  const size_t part_rows = (size_t)ca.c.N << ca.page_log2;   // rows of one part of a page
-  const int row_mask = ca.c.page_size - 1;
-  // the page of this lane's token of a tile, -1: none, or no such token
-  auto find_page = [&](int tile) {
-    const int token = first + tile * TK + lane;
-    return lane < TK && tile < tile1 && token < end ? place_of(ca, b, token).page : -1;
-  };
-  auto fill = [&](int tile, int st, int page) {
-    uint8_t* to = ring + st * S::kStage;
-    const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
-    // (a group of 16 tokens lies in one page; its first token is there if any is)
-    if (lane == 0) {
-      *reinterpret_cast<uint32_t*>(to + S::kOffThere) = there;
-      mbar_arrive_expect_tx(&full[st], (uint32_t)(((there & 1u) + (there >> 16 & 1u)) * 2 * 16 * S::kRowBytes));
-    }
-    __syncwarp();
-    if (page >= 0) {
-      const int r = (first + tile * TK + lane) & row_mask;
-      const size_t at = (size_t)page * 4 * part_rows + ((size_t)head << ca.page_log2) + r;   // of part 0
-      // lanes 0, 16 copy a group's keys, lanes 1, 17 its values (lane 1's token may be behind the last: then lane 0 copies both)
-      const bool second = there >> (lane | 1) & 1;
-      if ((lane & 15) == 0) {
-        bulk_load(to + lane * S::kRowBytes, (const uint8_t*)ca.c.codes + (at + a.key_part * part_rows) * S::kRowBytes, 16 * S::kRowBytes, &full[st]);
-        if (!second)
-          bulk_load(to + S::kOffV + lane * S::kRowBytes, (const uint8_t*)ca.c.codes + (at + a.value_part * part_rows) * S::kRowBytes,
-                    16 * S::kRowBytes, &full[st]);
-      } else if ((lane & 15) == 1) {
-        bulk_load(to + S::kOffV + (lane - 1) * S::kRowBytes,
-                  (const uint8_t*)ca.c.codes + (at - 1 + a.value_part * part_rows) * S::kRowBytes, 16 * S::kRowBytes, &full[st]);
+  if (warp == 0) {
+    // the whole line's length: 32 sequences at a time
+    long long total = 0, groups = 0;
+    for (int b0 = 0; b0 < ca.c.B; b0 += 32) {
+      const int b = b0 + lane;
+      Line l{};
+      if (b < ca.c.B) l = line_of<TK, Q>(a, b);
+      const long long ng = (long long)l.groups * ca.c.N, steps = ng * l.tiles;
+      long long s = steps, q = ng;   // sums up to this lane
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long s2 = __shfl_up_sync(0xffffffffu, s, o), q2 = __shfl_up_sync(0xffffffffu, q, o);
+        if (lane >= o) s += s2, q += q2;
       }
-      if (a.biased) copy4(to + S::kOffBias + lane * 4, ca.c.lse + (((size_t)page * ca.c.N + head) << ca.page_log2) + r);
-      if ((lane & 3) == 0) {
-        copy4(to + S::kOffEk + lane, ca.c.exponents + at + a.key_part * part_rows);
-        copy4(to + S::kOffEv + lane, ca.c.exponents + at + a.value_part * part_rows);
-      }
+      if (blockIdx.x == 0 && b < ca.c.B) p.table[b] = LineEntry{total + s - steps, groups + q - ng, l};
+      total += __shfl_sync(0xffffffffu, s, 31);
+      groups += __shfl_sync(0xffffffffu, q, 31);
     }
-    copies_arrive(&full[st]);
-  };
-  __syncwarp();
-  int next_page;   // of the tile that is filled next
-  {
-    int pg[NS + 1];
-#pragma unroll
-    for (int i = 0; i <= NS; ++i) pg[i] = find_page(tile0 + warp + i * kWarps);
-#pragma unroll
-    for (int i = 0; i < NS; ++i)
-      if (tile0 + warp + i * kWarps < tile1) fill(tile0 + warp + i * kWarps, i, pg[i]);
-    next_page = pg[NS];
-  }
-
-  // --- queries: fragments of Q^T, and what masks them
-  uint32_t qf[NT][D / 16][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int i = i0 + nt * 8 + g;
-    const bool on = nt * 8 + g < nq;
-    float f[D / 4];   // elements of this thread's positions, in the order of its fragments
-    uint32_t big = 0;
-    const size_t off = on ? rows_at(a.q, b, head, i) : 0;
-    constexpr int EPL = S::kWide ? 8 : 16;   // elements of 16 bytes of codes
-#pragma unroll
-    for (int j = 0; j < D / (4 * EPL); ++j)
-#pragma unroll
-      for (int c = 0; c < EPL / 8; ++c) {
-        float x[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = 0.f;
-        const size_t at = off + j * 4 * EPL + t * EPL + c * 8;
-        if (on) {
-          if (a.dtype == TRITT_F16)
-            load8((const __half*)a.q.p + at, x);
-          else
-            load8((const __nv_bfloat16*)a.q.p + at, x);
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          f[j * EPL + c * 8 + e] = x[e];
-          big = max(big, __float_as_uint(x[e]) & 0x7fffffffu);
-        }
-      }
-    big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
-    big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
-    const int up = max(min(254 - (int)(big >> 23), 253), 1);
-    const float mul = __uint_as_float((uint32_t)up << 23);
-#pragma unroll
-    for (int s = 0; s < D / 16; ++s) {
-      qf[nt][s][0] = pack_half(f[s * 4] * mul, f[s * 4 + 1] * mul);
-      qf[nt][s][1] = pack_half(f[s * 4 + 2] * mul, f[s * 4 + 3] * mul);
-    }
-    if (warp == 0 && t == 0) {
-      const unsigned long long word = on && ca.c.ancestors ? seen_word(ca, b, i) : 0;
-      const int pos = ctx + (ca.c.ancestors ? __popcll(word) - 1 : i);
-      s_word[nt * 8 + g] = word;
-      s_pos[nt * 8 + g] = on ? pos : -1;
-      s_lo[nt * 8 + g] = on ? max(0, pos - a.window) : 0x7fffffff;
-      s_scale[nt * 8 + g] = a.scale2 * __uint_as_float((uint32_t)(254 - up) << 23);
-    }
+    if (lane == 0) s_total = total, s_abort = 0;
   }
   __syncthreads();
-  // from lo_all on every query attends to all of the context (those that are not there take no part in this: their results are not looked at)
-  int lo_all = 0;
-  for (int i = 0; i < nq; ++i) lo_all = max(lo_all, s_lo[i]);
-  float qs[NT][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    qs[nt][0] = s_scale[nt * 8 + 2 * t];
-    qs[nt][1] = s_scale[nt * 8 + 2 * t + 1];
-  }
+  const long long total = s_total;
+  const int parts = parts_of(total, p.ctas);
+  if ((int)blockIdx.x >= parts) return;
+  long long x = (long long)blockIdx.x * total / parts, base = 0, group_base = 0;
+  const long long x_end = ((long long)blockIdx.x + 1) * total / parts;
+  if (x >= x_end) return;
+  const size_t part_rows = (size_t)ca.c.N << ca.page_log2;   // rows of one part of a page
+  const size_t page_bytes = 4 * part_rows * RB;
+  const int row_mask = ca.c.page_size - 1;
+  int st = 0, phase = 0;   // the ring's next stage
+  int b = 0;
+  Line line = line_of<TK, Q>(a, 0);
+  bool alive = true;
 
-  float acc[NT][D / 16][4], m[NT][2], l[NT][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-    for (int mb = 0; mb < D / 16; ++mb)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[nt][mb][e] = 0.f;
-    m[nt][0] = m[nt][1] = -INFINITY;
-    l[nt][0] = l[nt][1] = 0.f;
-  }
-  int v_exp = 0;   // largest exponent byte of the values so far
-  int st = 0, phase = 0;
-  for (int tile = tile0 + warp; tile < tile1; tile += kWarps) {
-    if (!__all_sync(0xffffffffu, mbar_wait(&full[st], phase, (volatile int*)&s_abort))) {
-      // give copies still in flight a bounded chance to land before the block ends
-      for (int i = 0; i < NS; ++i) {
-        const long long t0 = clock64();
-        while (!mbar_try_wait(&full[i], i < st ? phase ^ 1 : phase) && clock64() - t0 < kWaitTicks / 8) {
+  while (x < x_end && alive) {
+    // --- the next piece: tiles s0 .. s1 - 1 of one group of new tokens
+    while (x >= base + (long long)line.groups * line.tiles * ca.c.N) {
+      base += (long long)line.groups * line.tiles * ca.c.N;
+      group_base += (long long)line.groups * ca.c.N;
+      if (++b >= ca.c.B) return;   // (contexts that changed under the kernel)
+      line = line_of<TK, Q>(a, b);
+    }
+    const long long rel = x - base, grp = rel / line.tiles;
+    const int s0 = (int)(rel % line.tiles), s1 = (int)(line.tiles - s0 < x_end - x ? line.tiles : s0 + (x_end - x));
+    const int head = (int)(grp / line.groups), i0 = (int)(grp % line.groups) * Q;
+    float* part = p.part + (size_t)(group_base + grp + blockIdx.x) * Q * (D + 2);
+    x += s1 - s0;
+    const int ctx = line.ctx, nq = min(Q, line.cnt - i0);
+    // tokens that any of these queries attends to: first .. end - 1
+    const int first = max(0, ctx + (ca.c.ancestors ? 0 : i0) - a.window) & ~15, end = ctx + i0 + nq;
+    const int tile1 = min(s1, (end - first + TK - 1) / TK);
+    if (s0 >= tile1) {
+      for (int i = tid; i < nq; i += kWarps * 32) part[i * (D + 2)] = -INFINITY, part[i * (D + 2) + 1] = 0.f;
+      continue;
+    }
+
+    // --- the ring: this warp takes tiles s0 + warp, + kWarps, ...
+    const uint8_t* key_rows = (const uint8_t*)ca.c.codes + (a.key_part * part_rows + ((size_t)head << ca.page_log2)) * RB;
+    const long long to_values = (long long)(a.value_part - a.key_part) * (long long)part_rows;
+    const unsigned char* key_exp = ca.c.exponents + a.key_part * part_rows + ((size_t)head << ca.page_log2);
+    const float* biases = ca.c.lse + ((size_t)head << ca.page_log2);
+    // the page of this lane's token of a tile, -1: none, or no such token
+    auto find_page = [&](int tile) {
+      const int token = first + tile * TK + lane;
+      return lane < TK && tile < tile1 && token < end ? place_of(ca, b, token).page : -1;
+    };
+    auto fill = [&](int tile, int stage, int page) {
+      uint8_t* to = ring + stage * S::kStage;
+      const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
+      // (a group of 16 tokens lies in one page; its first token is there if any is)
+      if (lane == 0) {
+        *reinterpret_cast<uint32_t*>(to + S::kOffThere) = there;
+        mbar_arrive_expect_tx(&full[stage], (uint32_t)(((there & 1u) + (there >> 16 & 1u)) * 2 * 16 * RB));
+      }
+      const int row = (first + tile * TK + lane) & row_mask, group_page = __shfl_sync(0xffffffffu, page, lane & 16);
+      // lanes 0, 16 copy a group's keys, lanes 1, 17 its values
+      if ((lane & 14) == 0 && group_page >= 0) {
+        const uint8_t* from = key_rows + group_page * page_bytes + (size_t)(row & ~1) * RB + (lane & 1 ? to_values * RB : 0);
+        bulk_load(to + (lane & 1) * S::kOffV + (lane & 16) * RB, from, 16 * RB, &full[stage]);
+      }
+      if (page >= 0) {
+        if (a.biased) copy4(to + S::kOffBias + lane * 4, biases + page * part_rows + row);
+        if ((lane & 3) == 0) {
+          const unsigned char* e = key_exp + page * (4 * part_rows) + row;
+          copy4(to + S::kOffEk + lane, e);
+          copy4(to + S::kOffEv + lane, e + to_values);
         }
       }
-      if (lane == 0 && ca.status) atomicOr(ca.status, 16);
-      break;
-    }
-    const uint8_t* from = ring + st * S::kStage;
-    const int token0 = first + tile * TK;
-    // one lane a token: scales, and whether all of the tile counts for every query
-    const uint32_t there = *reinterpret_cast<const uint32_t*>(from + S::kOffThere);
-    bool plain = token0 >= lo_all && token0 + TK <= ctx;
-    uint32_t bad;
+      copies_arrive(&full[stage]);
+    };
+    int next_page;   // of the tile that is filled next
     {
-      const bool on = lane < TK && (there >> lane & 1);
-      const int ek = on ? from[S::kOffEk + lane] : 0, ev = on ? from[S::kOffEv + lane] : 0;
-      const float bias = on && a.biased ? *reinterpret_cast<const float*>(from + S::kOffBias + lane * 4) * kLog2e : 0.f;
-      bad = __ballot_sync(0xffffffffu, ek == 255 || ev == 255);
-      const int most = max(v_exp, (int)__reduce_max_sync(0xffffffffu, ev == 255 ? 0 : ev));
-      plain = plain && there == (TK == 32 ? 0xffffffffu : 0xffffu) && bad == 0u;
-      // (the products lie in the accumulator times 2^(largest exponent))
-      if (most > v_exp) {
-        const float grown = v_exp ? power(v_exp - most) : 1.f;
+      int pg[NS + 1];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+      for (int i = 0; i <= NS; ++i) pg[i] = find_page(s0 + warp + i * kWarps);
+      int f = st;
 #pragma unroll
-          for (int mb = 0; mb < D / 16; ++mb)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[nt][mb][e] *= grown;
-        v_exp = most;
+      for (int i = 0; i < NS; ++i) {
+        if (s0 + warp + i * kWarps < tile1) fill(s0 + warp + i * kWarps, f, pg[i]);
+        f = f + 1 == NS ? 0 : f + 1;
       }
-      if (lane < TK) s_side[warp][lane] = make_float4(power(ek - 127), bias, ev == 255 || !on ? 0.f : power(ev - most + kLift), 0.f);
+      next_page = pg[NS];
     }
-    __syncwarp();
-    // S^T
-    float s[NT][NB][4];
+
+    // --- queries: fragments of Q^T, and what masks them
+    uint32_t qf[NT][D / 16][2];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
+    for (int nt = 0; nt < NT; ++nt) {
+      const int i = i0 + nt * 8 + g;
+      const bool on = nt * 8 + g < nq;
+      float f[D / 4];   // elements of this thread's positions, in the order of its fragments
+      uint32_t big = 0;
+      const size_t off = on ? rows_at(a.q, b, head, i) : 0;
+      constexpr int EPL = S::kWide ? 8 : 16;   // elements of 16 bytes of codes
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int j = 0; j < D / (4 * EPL); ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[nt][nb][e] = 0.f;
+        for (int c = 0; c < EPL / 8; ++c) {
+          float v[8];
 #pragma unroll
-      for (int j = 0; j < KL; ++j) {
-        const uint4 r0 = *reinterpret_cast<const uint4*>(from + (nb * 16 + g) * S::kRowBytes + j * 64 + t * 16);
-        const uint4 r1 = *reinterpret_cast<const uint4*>(from + (nb * 16 + 8 + g) * S::kRowBytes + j * 64 + t * 16);
-        const uint32_t lo[4] = {r0.x, r0.y, r0.z, r0.w}, hi[4] = {r1.x, r1.y, r1.z, r1.w};
-        constexpr int STEPS = S::kWide ? 2 : 4;   // contraction steps of 16 bytes
-#pragma unroll
-        for (int k = 0; k < STEPS; ++k) {
-          uint32_t f[4];
-          if constexpr (S::kWide) {
-            f[0] = lo[2 * k], f[1] = hi[2 * k], f[2] = lo[2 * k + 1], f[3] = hi[2 * k + 1];
-          } else {
-            bytes_to_halves<CODE>(lo[k], f[0], f[2]);
-            bytes_to_halves<CODE>(hi[k], f[1], f[3]);
+          for (int e = 0; e < 8; ++e) v[e] = 0.f;
+          const size_t at = off + j * 4 * EPL + t * EPL + c * 8;
+          if (on) {
+            if (a.dtype == TRITT_F16)
+              load8((const __half*)a.q.p + at, v);
+            else
+              load8((const __nv_bfloat16*)a.q.p + at, v);
           }
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_16816(s[nt][nb], f, qf[nt][j * STEPS + k][0], qf[nt][j * STEPS + k][1]);
+          for (int e = 0; e < 8; ++e) {
+            f[j * EPL + c * 8 + e] = v[e];
+            big = max(big, __float_as_uint(v[e]) & 0x7fffffffu);
+          }
         }
+      big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
+      big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
+      const int up = max(min(254 - (int)(big >> 23), 253), 1);
+      const float mul = __uint_as_float((uint32_t)up << 23);
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s) {
+        qf[nt][s][0] = pack_half(f[s * 4] * mul, f[s * 4 + 1] * mul);
+        qf[nt][s][1] = pack_half(f[s * 4 + 2] * mul, f[s * 4 + 3] * mul);
+      }
+      if (warp == 0 && t == 0) {
+        const unsigned long long word = on && ca.c.ancestors ? seen_word(ca, b, i) : 0;
+        const int pos = ctx + (ca.c.ancestors ? __popcll(word) - 1 : i);
+        s_word[nt * 8 + g] = word;
+        s_pos[nt * 8 + g] = on ? pos : -1;
+        s_lo[nt * 8 + g] = on ? max(0, pos - a.window) : 0x7fffffff;
+        s_scale[nt * 8 + g] = a.scale2 * __uint_as_float((uint32_t)(254 - up) << 23);
       }
     }
-    // scores in log2 units
-    float vf[NB][2];
+    __syncthreads();
+    // from lo_all on every query attends to all of the context (those that are not there take no part in this: their results are not looked at)
+    int lo_all = 0;
+    for (int i = 0; i < nq; ++i) lo_all = max(lo_all, s_lo[i]);
+    float qs[NT][NQ];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int k = nb * 16 + h * 8 + g;
-        const float4 side = s_side[warp][k];
-        vf[nb][h] = side.z;
+      for (int q = 0; q < NQ; ++q) qs[nt][q] = s_scale[nt * 8 + 2 * t + q];
+
+    float acc[NT][D / 16][4], m[NT][NQ], l[NT][NQ];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-          for (int q = 0; q < 2; ++q) s[nt][nb][2 * h + q] = fmaf(s[nt][nb][2 * h + q] * side.x, qs[nt][q], side.y);
-        if (!plain) {
-          const int token = token0 + k;
-          bool missing = false;
+      for (int mb = 0; mb < D / 16; ++mb)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[nt][mb][e] = 0.f;
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) m[nt][q] = -INFINITY, l[nt][q] = 0.f;
+    }
+    int v_exp = 0;   // largest exponent byte of the values so far
+    for (int tile = s0 + warp; tile < tile1; tile += kWarps) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&full[st], phase, (volatile int*)&s_abort))) {
+        // give copies still in flight a bounded chance to land before the block ends
+        for (int i = 0; i < NS; ++i) {
+          const long long t0 = clock64();
+          while (!mbar_try_wait(&full[i], i < st ? phase ^ 1 : phase) && clock64() - t0 < kWaitTicks / 8) {
+          }
+        }
+        if (lane == 0 && ca.status) atomicOr(ca.status, 16);
+        break;
+      }
+      const uint8_t* from = ring + st * S::kStage;
+      const int token0 = first + tile * TK;
+      // one lane a token: scales, and whether all of the tile counts for every query
+      const uint32_t there = *reinterpret_cast<const uint32_t*>(from + S::kOffThere);
+      bool plain = token0 >= lo_all && token0 + TK <= ctx;
+      uint32_t bad;
+      {
+        const bool on = lane < TK && (there >> lane & 1);
+        const int ek = on ? from[S::kOffEk + lane] : 0, ev = on ? from[S::kOffEv + lane] : 0;
+        const float bias = on && a.biased ? *reinterpret_cast<const float*>(from + S::kOffBias + lane * 4) * kLog2e : 0.f;
+        bad = __ballot_sync(0xffffffffu, ek == 255 || ev == 255);
+        const int most = max(v_exp, (int)__reduce_max_sync(0xffffffffu, ev == 255 ? 0 : ev));
+        plain = plain && there == (TK == 32 ? 0xffffffffu : 0xffffu) && bad == 0u;
+        // (the products lie in the accumulator times 2^(largest exponent))
+        if (most > v_exp) {
+          const float grown = v_exp ? power(v_exp - most) : 1.f;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              const int i = nt * 8 + 2 * t + q;
-              bool seen = token >= s_lo[i] && token < end;
-              if (token >= ctx && token < end) {
-                const int n = token - ctx;
-                if (ca.c.ancestors) {
-                  const unsigned long long word = s_word[i];
-                  seen = (word >> n & 1) && ctx + __popcll(word & ((1ull << n) - 1)) >= s_lo[i];
-                } else {
-                  seen = seen && token <= s_pos[i];
-                }
-              }
-              missing = missing || (seen && !(there >> k & 1));
-              float& x = s[nt][nb][2 * h + q];
-              x = seen && (there >> k & 1) ? (bad >> k & 1 ? __uint_as_float(0x7fffffffu) : x) : -INFINITY;
+            for (int mb = 0; mb < D / 16; ++mb)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[nt][mb][e] *= grown;
+          v_exp = most;
+        }
+        if (lane < TK) s_side[warp][lane] = make_float4(power(ek - 127), bias, ev == 255 || !on ? 0.f : power(ev - most + kLift), 0.f);
+      }
+      __syncwarp();
+      // S^T
+      float s[NT][NB][4];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[nt][nb][e] = 0.f;
+        const uint8_t* row = from + (nb * 16 + actual_row<RB>(g)) * RB + t * 16;
+#pragma unroll
+        for (int j = 0; j < KL; ++j) {
+          const uint4 r0 = *reinterpret_cast<const uint4*>(row + j * 64), r1 = *reinterpret_cast<const uint4*>(row + 8 * RB + j * 64);
+          const uint32_t lo[4] = {r0.x, r0.y, r0.z, r0.w}, hi[4] = {r1.x, r1.y, r1.z, r1.w};
+          constexpr int STEPS = S::kWide ? 2 : 4;   // contraction steps of 16 bytes
+#pragma unroll
+          for (int k = 0; k < STEPS; ++k) {
+            uint32_t f[4];
+            if constexpr (S::kWide) {
+              f[0] = lo[2 * k], f[1] = hi[2 * k], f[2] = lo[2 * k + 1], f[3] = hi[2 * k + 1];
+            } else {
+              bytes_to_halves<CODE>(lo[k], f[0], f[2]);
+              bytes_to_halves<CODE>(hi[k], f[1], f[3]);
             }
-          if (missing && ca.status) atomicOr(ca.status, kStatusPlace);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_16816(s[nt][nb], f, qf[nt][j * STEPS + k][0], qf[nt][j * STEPS + k][1]);
+          }
         }
       }
-    // running maximum, P
-    uint32_t pf[NT][NB][2], pl[EXACT ? NT : 1][NB][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float base[2], corr[2];
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        float mx = m[nt][q];
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) mx = fmaxf(mx, fmaxf(s[nt][nb][q], s[nt][nb][2 + q]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-        base[q] = mx == -INFINITY ? 0.f : mx;   // (nothing attended so far: all P are 0)
-        corr[q] = exp2f(m[nt][q] - base[q]);
-        m[nt][q] = mx;
-        l[nt][q] *= corr[q];
-      }
-      if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
-#pragma unroll
-        for (int mb = 0; mb < D / 16; ++mb)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[nt][mb][e] *= corr[e & 1];
-      }
+      // scores in log2 units
+      float vf[NB][2];
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float p0 = exp2f(s[nt][nb][2 * h] - base[0]), p1 = exp2f(s[nt][nb][2 * h + 1] - base[1]);
-          l[nt][0] += p0;
-          l[nt][1] += p1;
-          const float x0 = p0 * vf[nb][h], x1 = p1 * vf[nb][h];
-          const uint32_t high = pack_half(x0, x1);
-          pf[nt][nb][h] = transposed(high);
-          if constexpr (EXACT) {
-            const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&high));
-            pl[nt][nb][h] = transposed(pack_half(x0 - r.x, x1 - r.y));
+          const int k = nb * 16 + h * 8 + actual_row<RB>(g);
+          const float4 side = s_side[warp][k];
+          vf[nb][h] = side.z;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) s[nt][nb][2 * h + q] = fmaf(s[nt][nb][2 * h + q] * side.x, qs[nt][q], side.y);
+          if (!plain) {
+            const int token = token0 + k;
+            bool missing = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int q = 0; q < NQ; ++q) {
+                const int i = nt * 8 + 2 * t + q;
+                bool seen = token >= s_lo[i] && token < end;
+                if (token >= ctx && token < end) {
+                  const int n = token - ctx;
+                  if (ca.c.ancestors) {
+                    const unsigned long long word = s_word[i];
+                    seen = (word >> n & 1) && ctx + __popcll(word & ((1ull << n) - 1)) >= s_lo[i];
+                  } else {
+                    seen = seen && token <= s_pos[i];
+                  }
+                }
+                missing = missing || (seen && !(there >> k & 1));
+                float& v = s[nt][nb][2 * h + q];
+                v = seen && (there >> k & 1) ? (bad >> k & 1 ? __uint_as_float(0x7fffffffu) : v) : -INFINITY;
+              }
+            if (missing && ca.status) atomicOr(ca.status, kStatusPlace);
           }
         }
-    }
-    // O^T += V^T P^T
+      // the reference (raised where a score is 2^8 above it), P
+      uint32_t pf[NT][NB][2], pl[EXACT ? NT : 1][NB][2];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      // of tokens 2t, 2t + 1, 2t + 8, 2t + 9 of the block, the g-th eighth of the row
-      uint32_t v[4][VW];
+      for (int nt = 0; nt < NT; ++nt) {
+        float mx[NQ], base2[NQ];
+        bool raise = false;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int row = nb * 16 + (k >> 1) * 8 + 2 * t + (k & 1);
-        const uint8_t* r = from + S::kOffV + row * S::kRowBytes + g * (VW * 4);
-        if constexpr (VW == 2) {
-          const uint2 w = *reinterpret_cast<const uint2*>(r);
-          v[k][0] = w.x, v[k][1] = w.y;
-        } else {
+        for (int q = 0; q < NQ; ++q) {
+          mx[q] = fmaxf(s[nt][0][q], s[nt][0][2 + q]);
 #pragma unroll
-          for (int j = 0; j < VW / 4; ++j) {
-            const uint4 w = *(reinterpret_cast<const uint4*>(r) + j);
-            v[k][4 * j] = w.x, v[k][4 * j + 1] = w.y, v[k][4 * j + 2] = w.z, v[k][4 * j + 3] = w.w;
+          for (int nb = 1; nb < NB; ++nb) mx[q] = fmaxf(mx[q], fmaxf(s[nt][nb][q], s[nt][nb][2 + q]));
+          raise = raise || mx[q] > m[nt][q] + kGap;
+        }
+        if (__any_sync(0xffffffffu, raise)) {
+          float corr[NQ];
+#pragma unroll
+          for (int q = 0; q < NQ; ++q) {
+            float v = fmaxf(mx[q], m[nt][q]);
+            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+            corr[q] = v == -INFINITY ? 1.f : exp2f(m[nt][q] - v);
+            m[nt][q] = v;
+            l[nt][q] *= corr[q];
           }
-        }
-        if (!plain && !(there >> row & 1)) {   // (what lies there is of another tile, or no number)
 #pragma unroll
-          for (int w = 0; w < VW; ++w) v[k][w] = 0u;
+          for (int mb = 0; mb < D / 16; ++mb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if ((e & 1) < NQ) acc[nt][mb][e] *= corr[e & 1 ? NQ - 1 : 0];
         }
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) base2[q] = m[nt][q] == -INFINITY ? 0.f : m[nt][q];   // (nothing attended so far: all P are 0)
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float v[2] = {0.f, 0.f};
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) {
+              const float e = exp2f(s[nt][nb][2 * h + q] - base2[q]);
+              l[nt][q] += e;
+              v[q] = e * vf[nb][h];
+            }
+            const uint32_t high = pack_half(v[0], v[1]);
+            pf[nt][nb][h] = transposed(high);
+            if constexpr (EXACT) {
+              const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&high));
+              pl[nt][nb][h] = transposed(pack_half(v[0] - r.x, v[1] - r.y));
+            }
+          }
       }
+      // O^T += V^T P^T
 #pragma unroll
-      for (int w = 0; w < VW; ++w) {
-        if constexpr (S::kWide) {
-          // two elements of four tokens: one block of 16 rows of V^T
-          uint32_t f[4];
-          f[0] = __byte_perm(v[0][w], v[1][w], 0x5410);
-          f[1] = __byte_perm(v[0][w], v[1][w], 0x7632);
-          f[2] = __byte_perm(v[2][w], v[3][w], 0x5410);
-          f[3] = __byte_perm(v[2][w], v[3][w], 0x7632);
+      for (int nb = 0; nb < NB; ++nb) {
+        // of tokens 2t, 2t + 1, 2t + 8, 2t + 9 of the block (as the fragments count), the g-th eighth of the row
+        uint32_t v[4][VW];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            mma_16816(acc[nt][w], f, pf[nt][nb][0], pf[nt][nb][1]);
-            if constexpr (EXACT) mma_16816(acc[nt][w], f, pl[nt][nb][0], pl[nt][nb][1]);
+        for (int k = 0; k < 4; ++k) {
+          const int row = nb * 16 + (k >> 1) * 8 + actual_row<RB>(2 * t + (k & 1));
+          const uint8_t* r = from + S::kOffV + row * RB + g * (VW * 4);
+          if constexpr (VW == 2) {
+            const uint2 w = *reinterpret_cast<const uint2*>(r);
+            v[k][0] = w.x, v[k][1] = w.y;
+          } else {
+#pragma unroll
+            for (int j = 0; j < VW / 4; ++j) {
+              const uint4 w = *(reinterpret_cast<const uint4*>(r) + j);
+              v[k][4 * j] = w.x, v[k][4 * j + 1] = w.y, v[k][4 * j + 2] = w.z, v[k][4 * j + 3] = w.w;
+            }
           }
-        } else {
-          // four elements: two blocks
+          if (!plain && !(there >> row & 1)) {   // (what lies there is of another tile, or no number)
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const uint32_t lo = __byte_perm(v[0][w], v[1][w], half ? 0x7362 : 0x5140);
-            const uint32_t hi = __byte_perm(v[2][w], v[3][w], half ? 0x7362 : 0x5140);
+            for (int w = 0; w < VW; ++w) v[k][w] = 0u;
+          }
+        }
+#pragma unroll
+        for (int w = 0; w < VW; ++w) {
+          if constexpr (S::kWide) {
+            // two elements of four tokens: one block of 16 rows of V^T
             uint32_t f[4];
-            bytes_to_halves<CODE>(lo, f[0], f[1]);
-            bytes_to_halves<CODE>(hi, f[2], f[3]);
+            f[0] = __byte_perm(v[0][w], v[1][w], 0x5410);
+            f[1] = __byte_perm(v[0][w], v[1][w], 0x7632);
+            f[2] = __byte_perm(v[2][w], v[3][w], 0x5410);
+            f[3] = __byte_perm(v[2][w], v[3][w], 0x7632);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              mma_16816(acc[nt][2 * w + half], f, pf[nt][nb][0], pf[nt][nb][1]);
-              if constexpr (EXACT) mma_16816(acc[nt][2 * w + half], f, pl[nt][nb][0], pl[nt][nb][1]);
+              mma_16816(acc[nt][w], f, pf[nt][nb][0], pf[nt][nb][1]);
+              if constexpr (EXACT) mma_16816(acc[nt][w], f, pl[nt][nb][0], pl[nt][nb][1]);
+            }
+          } else {
+            // four elements: two blocks
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const uint32_t lo = __byte_perm(v[0][w], v[1][w], half ? 0x7362 : 0x5140);
+              const uint32_t hi = __byte_perm(v[2][w], v[3][w], half ? 0x7362 : 0x5140);
+              uint32_t f[4];
+              bytes_to_halves<CODE>(lo, f[0], f[1]);
+              bytes_to_halves<CODE>(hi, f[2], f[3]);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                mma_16816(acc[nt][2 * w + half], f, pf[nt][nb][0], pf[nt][nb][1]);
+                if constexpr (EXACT) mma_16816(acc[nt][2 * w + half], f, pl[nt][nb][0], pl[nt][nb][1]);
+              }
             }
           }
         }
       }
+      __syncwarp();   // every lane has read this stage
+      if (tile + NS * kWarps < tile1) fill(tile + NS * kWarps, st, next_page);
+      next_page = find_page(tile + (NS + 1) * kWarps);
+      if (++st == NS) st = 0, phase ^= 1;
     }
-    __syncwarp();   // every lane has read this stage
-    if (tile + NS * kWarps < tile1) fill(tile + NS * kWarps, st, next_page);
-    next_page = find_page(tile + (NS + 1) * kWarps);
-    if (++st == NS) st = 0, phase ^= 1;
-  }
 
-  // --- the warps' results on their common maximum, added up in order
+    // --- the warps' results on their common maximum, added up in order
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      l[nt][q] += __shfl_xor_sync(0xffffffffu, l[nt][q], 4);
-      l[nt][q] += __shfl_xor_sync(0xffffffffu, l[nt][q], 8);
-      l[nt][q] += __shfl_xor_sync(0xffffffffu, l[nt][q], 16);
-      if (g == 0) {
-        s_m[warp][nt * 8 + 2 * t + q] = m[nt][q];
-        s_l[warp][nt * 8 + 2 * t + q] = l[nt][q];
+      for (int q = 0; q < NQ; ++q) {
+        float sum = l[nt][q];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        if (g == 0) {
+          s_m[warp][nt * 8 + 2 * t + q] = m[nt][q];
+          s_l[warp][nt * 8 + 2 * t + q] = sum;
+        }
+      }
+    __syncthreads();   // (and every warp is done with its ring)
+    alive = s_abort == 0;
+    float(*out)[Q][D + 4] = reinterpret_cast<float(*)[Q][D + 4]>(ring_all);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+        const int i = nt * 8 + 2 * t + q;
+        if (i >= nq) continue;
+        float top = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < kWarps; ++k) top = fmaxf(top, s_m[k][i]);
+        // (a warp without a value has v_exp 0 and adds nothing)
+        const float f = m[nt][q] == -INFINITY || v_exp == 0 ? 0.f : exp2f(m[nt][q] - top) * power(v_exp - 127) * (1.f / (1 << kLift));
+#pragma unroll
+        for (int mb = 0; mb < D / 16; ++mb)
+          *reinterpret_cast<float2*>(&out[warp][i][g * (D / 8) + 2 * mb]) =
+              f == 0.f ? make_float2(0.f, 0.f) : make_float2(acc[nt][mb][q] * f, acc[nt][mb][2 + q] * f);
+      }
+    __syncthreads();
+    for (int i = warp; i < nq; i += kWarps) {
+      float top = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) top = fmaxf(top, s_m[k][i]);
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k)
+        sum += s_m[k][i] == -INFINITY ? (s_l[k][i] != s_l[k][i] ? s_l[k][i] : 0.f) : s_l[k][i] * exp2f(s_m[k][i] - top);
+      float* to = part + i * (D + 2);
+      if (lane == 0) to[0] = top, to[1] = sum;
+#pragma unroll
+      for (int c = lane; c < D; c += 32) {
+        float v = out[0][i][c];
+#pragma unroll
+        for (int k = 1; k < kWarps; ++k) v += out[k][i][c];
+        to[2 + c] = v;
       }
     }
-  for (int i = tid; i < Q * (D + 4); i += kWarps * 32) (&s_out[0][0])[i] = 0.f;
-  __syncthreads();
-  for (int w = 0; w < kWarps; ++w) {
-    if (warp == w && v_exp > 0) {
-      // (exponents of values only scale the accumulator; a warp without a value has v_exp 0 and nothing to add)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const int i = nt * 8 + 2 * t + q;
-          float top = -INFINITY;
-          for (int k = 0; k < kWarps; ++k) top = fmaxf(top, s_m[k][i]);
-          const float f = m[nt][q] == -INFINITY ? 0.f : exp2f(m[nt][q] - top) * power(v_exp - 127) * (1.f / (1 << kLift));
-#pragma unroll
-          for (int mb = 0; mb < D / 16; ++mb) {
-            s_out[i][g * (D / 8) + 2 * mb] += f == 0.f ? 0.f : acc[nt][mb][q] * f;
-            s_out[i][g * (D / 8) + 2 * mb + 1] += f == 0.f ? 0.f : acc[nt][mb][2 + q] * f;
-          }
-        }
-    }
+    fence_async_smem();   // (the next piece's copies come into the same memory)
     __syncthreads();
   }
-  for (int i = warp; i < rows; i += kWarps) {
-    float top = -INFINITY, sum = 0.f;
-    for (int k = 0; k < kWarps; ++k) top = fmaxf(top, s_m[k][i]);
-    for (int k = 0; k < kWarps; ++k)
-      sum += s_m[k][i] == -INFINITY ? (s_l[k][i] != s_l[k][i] ? s_l[k][i] : 0.f) : s_l[k][i] * exp2f(s_m[k][i] - top);
-    float* out = part + i * pitch;
-    if (i >= nq) top = -INFINITY, sum = 0.f;   // (behind the sequence's last new token)
-    if (lane == 0) out[0] = top, out[1] = sum;
-    for (int c = lane; c < D; c += 32) out[2 + c] = s_out[i][c];
+}
+
+struct DpsJoinParams {
+  DpsDecodeArgs a;
+  const LineEntry* table;
+  const float* part;
+  int ctas, queries;     // of the first kernel; new tokens of a group
+  void* o;               // [B, N, n, D], or null: append
+  float* lse;            // [B, N, n]
+  tritt_rows_t v2;       // append: W = result * v2 goes to the cache, and the log-sum-exp
+};
+
+// One warp a row where a row has few pieces, else four that take its pieces in turn; D / 8 of a warp's lanes hold eight elements each.
+template <typename T, int CODE, int W>
+__global__ void __launch_bounds__(128) dps_join_kernel(const __grid_constant__ DpsJoinParams j) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  __shared__ float sm[4], sl[4], so[4][256];
+  const CacheArgs& ca = j.a.cache;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = lane * 8, D = ca.c.D;
+  const long long row = W == 1 ? (long long)blockIdx.x * 4 + warp : blockIdx.x;
+  if (row >= (long long)ca.c.B * ca.c.N * ca.c.n) return;
+  const int i = (int)(row % ca.c.n), head = (int)(row / ca.c.n % ca.c.N), b = (int)(row / ca.c.n / ca.c.N);
+  const LineEntry e = j.table[b], end = j.table[ca.c.B - 1];
+  const long long total = end.base + (long long)end.line.groups * end.line.tiles * ca.c.N;
+  const int parts = parts_of(total, j.ctas);
+  float m = -INFINITY, l = 0.f, f[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) f[k] = 0.f;
+  if (i < e.line.cnt) {
+    const long long grp = (long long)head * e.line.groups + i / j.queries, first = e.base + grp * e.line.tiles;
+    // CTA c has the steps from c total / parts to the next one's
+    const long long c0 = ((first + 1) * parts - 1) / total, c1 = ((first + e.line.tiles) * parts - 1) / total;
+    for (long long c = c0 + (W == 1 ? 0 : warp); c <= c1; c += W) {
+      const float* p = j.part + ((size_t)(e.group_base + grp + c) * j.queries + i % j.queries) * (D + 2);
+      const float mp = p[0], lp = p[1];
+      if (mp == -INFINITY && lp == 0.f) continue;   // (its result is not written)
+      const float mn = fmaxf(m, mp), w0 = m == -INFINITY ? 0.f : exp2f(m - mn), w1 = mp == -INFINITY ? 1.f : exp2f(mp - mn);
+      l = l * w0 + lp * w1;
+      if (col < D) {
+#pragma unroll
+        for (int k = 0; k < 8; k += 2) {
+          const float2 v = *reinterpret_cast<const float2*>(p + 2 + col + k);
+          f[k] = f[k] * w0 + v.x * w1;
+          f[k + 1] = f[k + 1] * w0 + v.y * w1;
+        }
+      }
+      m = mn;
+    }
   }
+  if constexpr (W > 1) {
+    if (lane == 0) sm[warp] = m, sl[warp] = l;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (col < D) so[warp][col + k] = f[k];
+    __syncthreads();
+    if (warp) return;
+    m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) m = fmaxf(m, sm[w]);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float x = sm[w] == -INFINITY ? (sl[w] != sl[w] ? 1.f : 0.f) : exp2f(sm[w] - m);
+      l += x == 0.f ? 0.f : sl[w] * x;
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (col < D && x != 0.f) f[k] = fmaf(so[w][col + k], x, f[k]);
+    }
+  }
+  const bool none = m == -INFINITY && l == 0.f;
+  const float inv = none ? 0.f : 1.f / l, lse = none ? -INFINITY : l != l ? l : (m + log2f(l)) * kLn2;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) f[k] = none ? 0.f : f[k] * inv;
+  if (j.o) {
+    if (col < D) store8((T*)j.o + (size_t)row * D + col, f);
+    if (j.lse && lane == 0) j.lse[row] = lse;
+    return;
+  }
+  join_into_cache<T, CODE>(ca, b, head, i, col, f, lse, j.v2);
 }
 
 constexpr int most_tiles(int D) { return D == 64 ? 4 : 3; }   // of 8 queries, by registers
@@ -494,46 +674,74 @@ Plan plan_of(int n, int D) {
   const int all = (n + 7) / 8, groups = (all + most_tiles(D) - 1) / most_tiles(D);
   return Plan{groups, (all + groups - 1) / groups};
 }
+size_t table_bytes(const tritt_cache_t& c) { return align_up((size_t)c.B * sizeof(LineEntry), 256); }
 
-template <int D, int CODE, int NT> int launch(const Params& p, cudaStream_t stream) {
-  auto kern = p.a.exact ? dps_decode_kernel<D, CODE, NT, true> : dps_decode_kernel<D, CODE, NT, false>;
-  TRITT_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D, CODE>::kSmem));
-  kern<<<dim3(p.a.splits, p.a.cache.c.B * p.a.cache.c.N, p.query_groups), kWarps * 32, Shape<D, CODE>::kSmem, stream>>>(p);
+template <int D, int CODE, int NT, bool ONE, bool EXACT> int launch_kernel(Params p, cudaStream_t stream, int& ctas) {
+  auto kern = dps_decode_kernel<D, CODE, NT, ONE, EXACT>;
+  constexpr int kSmem = smem_bytes<D, CODE, NT>();
+  TRITT_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+  p.ctas = ctas = num_sms() * blocks_per_sm<D, CODE, NT>();
+  kern<<<ctas, kWarps * 32, kSmem, stream>>>(p);
   count_launch();
   TRITT_CUDA_OK(cudaGetLastError());
   return 0;
 }
-template <int D, int CODE> int by_tiles(const Params& p, int tiles, cudaStream_t stream) {
+template <int D, int CODE, int NT> int launch(const Params& p, cudaStream_t stream, int& ctas) {
+  if constexpr (NT == 1) {
+    if (p.a.cache.c.n == 1)
+      return p.a.exact ? launch_kernel<D, CODE, 1, true, true>(p, stream, ctas) : launch_kernel<D, CODE, 1, true, false>(p, stream, ctas);
+  }
+  return p.a.exact ? launch_kernel<D, CODE, NT, false, true>(p, stream, ctas) : launch_kernel<D, CODE, NT, false, false>(p, stream, ctas);
+}
+template <int D, int CODE> int by_tiles(const Params& p, int tiles, cudaStream_t stream, int& ctas) {
   switch (tiles) {
-    case 1: return launch<D, CODE, 1>(p, stream);
-    case 2: return launch<D, CODE, 2>(p, stream);
-    case 3: return launch<D, CODE, 3>(p, stream);
+    case 1: return launch<D, CODE, 1>(p, stream, ctas);
+    case 2: return launch<D, CODE, 2>(p, stream, ctas);
+    case 3: return launch<D, CODE, 3>(p, stream, ctas);
     default:
-      if constexpr (most_tiles(D) >= 4) return launch<D, CODE, 4>(p, stream);
+      if constexpr (most_tiles(D) >= 4) return launch<D, CODE, 4>(p, stream, ctas);
       return -1;
   }
 }
-template <int D> int by_code(const Params& p, int tiles, cudaStream_t stream) {
-  if (p.a.cache.c.code == TRITT_CODE_F16) return by_tiles<D, TRITT_CODE_F16>(p, tiles, stream);
-  return p.a.cache.c.code == TRITT_CODE_E4M3 ? by_tiles<D, TRITT_CODE_E4M3>(p, tiles, stream) : by_tiles<D, TRITT_CODE_INT8>(p, tiles, stream);
+template <int D> int by_code(const Params& p, int tiles, cudaStream_t stream, int& ctas) {
+  if (p.a.cache.c.code == TRITT_CODE_F16) return by_tiles<D, TRITT_CODE_F16>(p, tiles, stream, ctas);
+  return p.a.cache.c.code == TRITT_CODE_E4M3 ? by_tiles<D, TRITT_CODE_E4M3>(p, tiles, stream, ctas) : by_tiles<D, TRITT_CODE_INT8>(p, tiles, stream, ctas);
+}
+
+template <typename T, int CODE> int launch_dps_join(const DpsJoinParams& j, cudaStream_t stream) {
+  const long long rows = (long long)j.a.cache.c.B * j.a.cache.c.N * j.a.cache.c.n;
+  // (pieces of a row: about ctas / rows and one more; four warps share more than two)
+  if (rows * 2 < j.ctas)
+    dps_join_kernel<T, CODE, 4><<<(unsigned)rows, 128, 0, stream>>>(j);
+  else
+    dps_join_kernel<T, CODE, 1><<<(unsigned)((rows + 3) / 4), 128, 0, stream>>>(j);
+  count_launch();
+  TRITT_CUDA_OK(cudaGetLastError());
+  return 0;
+}
+template <typename T> int join_by_code(const DpsJoinParams& j, cudaStream_t s) {
+  const int code = j.a.cache.c.code;
+  if (code == TRITT_CODE_F16) return launch_dps_join<T, TRITT_CODE_F16>(j, s);
+  return code == TRITT_CODE_E4M3 ? launch_dps_join<T, TRITT_CODE_E4M3>(j, s) : launch_dps_join<T, TRITT_CODE_INT8>(j, s);
 }
 
 }  // namespace
 
 bool mma_dps_decode_supported(int D, int dtype) { return (D == 64 || D == 128) && (dtype == TRITT_F16 || dtype == TRITT_BF16); }
 
-// Blocks for the chip four times over (three or four blocks an SM), so that sequences of unequal length even out; a split has at least 256 tokens.
-int mma_dps_decode_splits(const tritt_cache_t& c) {
-  const long long rows = (long long)c.B * c.N * plan_of(c.n, c.D).groups, want = (4 * 4 * 148 + rows - 1) / rows;
-  const long long most = ((long long)c.page_size * c.table_pages + 255) / 256;
-  const long long s = want < most ? want : most;
-  return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+size_t mma_dps_decode_workspace(const tritt_cache_t& c) {
+  const Plan plan = plan_of(c.n, c.D);
+  return table_bytes(c) + align_up((size_t)((long long)c.B * c.N * plan.groups + 4 * num_sms()) * 8 * plan.tiles * (c.D + 2) * 4, 256);
 }
 
-int mma_dps_decode(const DpsDecodeArgs& a, cudaStream_t stream) {
-  const Plan plan = plan_of(a.cache.c.n, a.cache.c.D);
-  const Params p{a, plan.groups};
-  return a.cache.c.D == 64 ? by_code<64>(p, plan.tiles, stream) : by_code<128>(p, plan.tiles, stream);
+int mma_dps_decode(const DpsDecodeArgs& a, void* workspace, void* o, float* lse, const tritt_rows_t* v2, cudaStream_t stream) {
+  const tritt_cache_t& c = a.cache.c;
+  const Plan plan = plan_of(c.n, c.D);
+  const Params p{a, (LineEntry*)workspace, (float*)((char*)workspace + table_bytes(c)), 0};
+  int ctas = 0;
+  if (int rc = c.D == 64 ? by_code<64>(p, plan.tiles, stream, ctas) : by_code<128>(p, plan.tiles, stream, ctas)) return rc;
+  const DpsJoinParams j{a, p.table, p.part, ctas, 8 * plan.tiles, o, lse, v2 ? *v2 : tritt_rows_t{}};
+  return a.dtype == TRITT_F16 ? join_by_code<__half>(j, stream) : join_by_code<__nv_bfloat16>(j, stream);
 }
 
 }  // namespace tritt
