@@ -261,7 +261,7 @@ int check_cache(const tritt_cache_t* c) {
     set_error("null cache pointer");
     return -4;
   }
-  if (((uintptr_t)c->codes & 15) || (((uintptr_t)c->table | (uintptr_t)c->context | (uintptr_t)c->exponents | (uintptr_t)c->lse) & 3)) {
+  if ((((uintptr_t)c->codes | (uintptr_t)c->exponents | (uintptr_t)c->lse) & 15) || (((uintptr_t)c->table | (uintptr_t)c->context) & 3)) {
     set_error("cache pointer is not aligned");
     return -5;
   }

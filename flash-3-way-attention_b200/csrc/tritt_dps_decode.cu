@@ -69,28 +69,26 @@ __device__ __forceinline__ float power(int e) { return e > -127 ? __uint_as_floa
 template <int D, int CODE> struct Shape {
   static constexpr bool kWide = CODE == TRITT_CODE_F16;
   static constexpr int kRowBytes = D * (kWide ? 2 : 1);
-  static constexpr int kTokens = kRowBytes == 256 ? 16 : 32;    // of a tile: 4 or 8 KB of keys and values
-  static constexpr int kBlocks = kTokens / 16;
+  static constexpr int kTokens = 4096 / kRowBytes;              // of a tile, 64 to 16: 8 KB of keys and values
+  static constexpr int kBlocks = kTokens / 16;                  // of 16 tokens, each in one page
   static constexpr int kKeyLoads = kRowBytes / 64;              // of 16 bytes, of a lane's row
   static constexpr int kValueWords = kRowBytes / 32;            // 32-bit words of a lane's eighth of a row
-  // a stage of the ring: keys, values, then biases, exponents of keys and values, and which tokens are there
-  static constexpr int kOffV = kTokens * kRowBytes, kOffBias = 2 * kOffV, kOffEk = kOffBias + 128, kOffEv = kOffEk + 32, kOffThere = kOffEv + 32;
-  static constexpr int kStage = kOffBias + 256;
-  static constexpr int kStages = 3;
-  static constexpr int kRing = kWarps * kStages * kStage;
+  // a stage of the ring: keys, values, then biases, exponents of keys and values, and which blocks are there
+  static constexpr int kOffV = 4096, kOffBias = 8192, kOffEk = kOffBias + 256, kOffEv = kOffEk + 64, kOffThere = kOffEv + 64;
+  static constexpr int kStage = 8704;
 };
+template <int NT> constexpr int kBlocksPerSm = NT == 1 ? 3 : 2;   // by registers
+// Stages of a warp's ring: of three blocks an SM each warp has one in flight and one that it works on.
+template <int NT> constexpr int kStages = kBlocksPerSm<NT> == 3 ? 2 : 3;
 // The ring's memory takes the warps' results at the end of a piece: [warps][Q][D + 4] fp32.
 template <int D, int CODE, int NT> constexpr int smem_bytes() {
-  constexpr int out = kWarps * 8 * NT * (D + 4) * 4;
-  return Shape<D, CODE>::kRing > out ? Shape<D, CODE>::kRing : out;
-}
-template <int D, int CODE, int NT> constexpr int blocks_per_sm() {   // by registers and shared memory
-  return Shape<D, CODE>::kRowBytes == 64 ? (NT == 1 ? 4 : NT == 2 ? 3 : 2) : 2;
+  constexpr int ring = kWarps * kStages<NT> * Shape<D, CODE>::kStage, out = kWarps * 8 * NT * (D + 4) * 4;
+  return ring > out ? ring : out;
 }
 
-// Copies of four bytes, and their arrival at a barrier.
-__device__ __forceinline__ void copy4(void* dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+// Asynchronous copies of 16 bytes, and their arrival at a barrier.
+__device__ __forceinline__ void copy16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
 __device__ __forceinline__ void copies_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -116,9 +114,9 @@ __host__ __device__ __forceinline__ int parts_of(long long total, int ctas) {
 
 // ONE: a single new token (a query's column of the fragments; the others are not worked on).
 template <int D, int CODE, int NT, bool ONE, bool EXACT>
-__global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, CODE, NT>()) dps_decode_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm<NT>) dps_decode_kernel(const __grid_constant__ Params p) {
   using S = Shape<D, CODE>;
-  constexpr int NB = S::kBlocks, TK = S::kTokens, KL = S::kKeyLoads, VW = S::kValueWords, NS = S::kStages, RB = S::kRowBytes;
+  constexpr int NB = S::kBlocks, TK = S::kTokens, KL = S::kKeyLoads, VW = S::kValueWords, NS = kStages<NT>, RB = S::kRowBytes;
   constexpr int Q = 8 * NT, NQ = ONE ? 1 : 2;
   extern __shared__ __align__(128) uint8_t ring_all[];
   __shared__ uint64_t s_full[kWarps][NS];
@@ -199,32 +197,30 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, CODE, NT>()) dps
     const long long to_values = (long long)(a.value_part - a.key_part) * (long long)part_rows;
     const unsigned char* key_exp = ca.c.exponents + a.key_part * part_rows + ((size_t)head << ca.page_log2);
     const float* biases = ca.c.lse + ((size_t)head << ca.page_log2);
-    // the page of this lane's token of a tile, -1: none, or no such token
+    // the page of a tile's block of 16 tokens lane % NB, -1: none, or no such tokens
     auto find_page = [&](int tile) {
-      const int token = first + tile * TK + lane;
-      return lane < TK && tile < tile1 && token < end ? place_of(ca, b, token).page : -1;
+      const int token = first + tile * TK + lane % NB * 16;
+      return tile < tile1 && token < end ? place_of(ca, b, token).page : -1;
     };
+    // (what a page has behind the last token comes along and is not looked at)
     auto fill = [&](int tile, int stage, int page) {
       uint8_t* to = ring + stage * S::kStage;
-      const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
-      // (a group of 16 tokens lies in one page; its first token is there if any is)
+      const uint32_t there = __ballot_sync(0xffffffffu, page >= 0) & ((1u << NB) - 1);
       if (lane == 0) {
         *reinterpret_cast<uint32_t*>(to + S::kOffThere) = there;
-        mbar_arrive_expect_tx(&full[stage], (uint32_t)(((there & 1u) + (there >> 16 & 1u)) * 2 * 16 * RB));
+        mbar_arrive_expect_tx(&full[stage], (uint32_t)__popc(there) * 2 * 16 * RB);
       }
-      const int row = (first + tile * TK + lane) & row_mask, group_page = __shfl_sync(0xffffffffu, page, lane & 16);
-      // lanes 0, 16 copy a group's keys, lanes 1, 17 its values
-      if ((lane & 14) == 0 && group_page >= 0) {
-        const uint8_t* from = key_rows + group_page * page_bytes + (size_t)(row & ~1) * RB + (lane & 1 ? to_values * RB : 0);
-        bulk_load(to + (lane & 1) * S::kOffV + (lane & 16) * RB, from, 16 * RB, &full[stage]);
-      }
+      __syncwarp();
       if (page >= 0) {
-        if (a.biased) copy4(to + S::kOffBias + lane * 4, biases + page * part_rows + row);
-        if ((lane & 3) == 0) {
-          const unsigned char* e = key_exp + page * (4 * part_rows) + row;
-          copy4(to + S::kOffEk + lane, e);
-          copy4(to + S::kOffEv + lane, e + to_values);
-        }
+        // lanes NB k .. NB k + NB - 1: keys, values, their exponents, and four times the quarters of the biases
+        const int blk = lane % NB, kind = lane / NB, row = (first + tile * TK + blk * 16) & row_mask;
+        if (kind < 2)
+          bulk_load(to + kind * S::kOffV + blk * 16 * RB, key_rows + page * page_bytes + (size_t)row * RB + (kind ? to_values * RB : 0), 16 * RB,
+                    &full[stage]);
+        else if (kind < 4)
+          copy16(to + (kind == 2 ? S::kOffEk : S::kOffEv) + blk * 16, key_exp + page * (4 * part_rows) + row + (kind == 2 ? 0 : to_values));
+        else if (kind < 8 && a.biased)
+          copy16(to + S::kOffBias + blk * 64 + (kind - 4) * 16, biases + page * part_rows + row + (kind - 4) * 4);
       }
       copies_arrive(&full[stage]);
     };
@@ -324,17 +320,24 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, CODE, NT>()) dps
       }
       const uint8_t* from = ring + st * S::kStage;
       const int token0 = first + tile * TK;
-      // one lane a token: scales, and whether all of the tile counts for every query
+      // one lane a token or two: scales, and whether all of the tile counts for every query
       const uint32_t there = *reinterpret_cast<const uint32_t*>(from + S::kOffThere);
-      bool plain = token0 >= lo_all && token0 + TK <= ctx;
-      uint32_t bad;
+      bool plain = token0 >= lo_all && token0 + TK <= ctx && there == (1u << NB) - 1;
       {
-        const bool on = lane < TK && (there >> lane & 1);
-        const int ek = on ? from[S::kOffEk + lane] : 0, ev = on ? from[S::kOffEv + lane] : 0;
-        const float bias = on && a.biased ? *reinterpret_cast<const float*>(from + S::kOffBias + lane * 4) * kLog2e : 0.f;
-        bad = __ballot_sync(0xffffffffu, ek == 255 || ev == 255);
-        const int most = max(v_exp, (int)__reduce_max_sync(0xffffffffu, ev == 255 ? 0 : ev));
-        plain = plain && there == (TK == 32 ? 0xffffffffu : 0xffffu) && bad == 0u;
+        constexpr int PER = (TK + 31) / 32;
+        int ek[PER], ev[PER], most = 0;
+        bool bad = false;
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+          const int token = k * 32 + lane;
+          const bool on = token < TK && token0 + token < end && (there >> (token >> 4) & 1);
+          ek[k] = on ? from[S::kOffEk + token] : 0;
+          ev[k] = on ? from[S::kOffEv + token] : 0;
+          bad = bad || ek[k] == 255 || ev[k] == 255;
+          most = max(most, ev[k] == 255 ? 0 : ev[k]);
+        }
+        plain = !__any_sync(0xffffffffu, bad) && plain;
+        most = max(v_exp, (int)__reduce_max_sync(0xffffffffu, most));
         // (the products lie in the accumulator times 2^(largest exponent))
         if (most > v_exp) {
           const float grown = v_exp ? power(v_exp - most) : 1.f;
@@ -346,7 +349,14 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, CODE, NT>()) dps
               for (int e = 0; e < 4; ++e) acc[nt][mb][e] *= grown;
           v_exp = most;
         }
-        if (lane < TK) s_side[warp][lane] = make_float4(power(ek - 127), bias, ev == 255 || !on ? 0.f : power(ev - most + kLift), 0.f);
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+          const int token = k * 32 + lane;
+          if (TK >= 32 || token < TK)
+            s_side[warp][token] = make_float4(
+                power(ek[k] - 127), a.biased ? *reinterpret_cast<const float*>(from + S::kOffBias + token * 4) * kLog2e : 0.f,
+                ev[k] == 255 || ev[k] == 0 ? 0.f : power(ev[k] - most + kLift), ek[k] == 255 || ev[k] == 255 ? 1.f : 0.f);
+        }
       }
       __syncwarp();
       // S^T
@@ -392,6 +402,7 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, CODE, NT>()) dps
             for (int q = 0; q < NQ; ++q) s[nt][nb][2 * h + q] = fmaf(s[nt][nb][2 * h + q] * side.x, qs[nt][q], side.y);
           if (!plain) {
             const int token = token0 + k;
+            const bool here = there >> (k >> 4) & 1;
             bool missing = false;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -408,9 +419,9 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, CODE, NT>()) dps
                     seen = seen && token <= s_pos[i];
                   }
                 }
-                missing = missing || (seen && !(there >> k & 1));
+                missing = missing || (seen && !here);
                 float& v = s[nt][nb][2 * h + q];
-                v = seen && (there >> k & 1) ? (bad >> k & 1 ? __uint_as_float(0x7fffffffu) : v) : -INFINITY;
+                v = seen && here ? (side.w != 0.f ? __uint_as_float(0x7fffffffu) : v) : -INFINITY;
               }
             if (missing && ca.status) atomicOr(ca.status, kStatusPlace);
           }
@@ -486,7 +497,7 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, CODE, NT>()) dps
               v[k][4 * j] = w.x, v[k][4 * j + 1] = w.y, v[k][4 * j + 2] = w.z, v[k][4 * j + 3] = w.w;
             }
           }
-          if (!plain && !(there >> row & 1)) {   // (what lies there is of another tile, or no number)
+          if (!plain && !(token0 + row < end && (there >> (row >> 4) & 1))) {   // (what lies there is of another tile, or no number)
 #pragma unroll
             for (int w = 0; w < VW; ++w) v[k][w] = 0u;
           }
@@ -680,7 +691,7 @@ template <int D, int CODE, int NT, bool ONE, bool EXACT> int launch_kernel(Param
   auto kern = dps_decode_kernel<D, CODE, NT, ONE, EXACT>;
   constexpr int kSmem = smem_bytes<D, CODE, NT>();
   TRITT_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
-  p.ctas = ctas = num_sms() * blocks_per_sm<D, CODE, NT>();
+  p.ctas = ctas = num_sms() * kBlocksPerSm<NT>;
   kern<<<ctas, kWarps * 32, kSmem, stream>>>(p);
   count_launch();
   TRITT_CUDA_OK(cudaGetLastError());

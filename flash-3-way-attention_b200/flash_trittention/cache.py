@@ -98,10 +98,8 @@ def _describe(cache, table, context, n, counts, ancestors):
         if t is not None and (t.shape != shape or t.dtype != dtype or t.device != dev):
             raise ValueError(f"{name} must be {dtype} of shape {list(shape)} on {dev}, got {t.dtype} {list(t.shape)} on {t.device}")
     for name, t in (("codes", codes), ("exponents", exponents), ("lse", lse)):
-        if t is not None and not t.is_contiguous():
-            raise ValueError(f"the cache's {name} must be contiguous")
-    if codes.data_ptr() % 16:
-        raise ValueError("the cache's codes must start on a 16-byte boundary")
+        if t is not None and (not t.is_contiguous() or t.data_ptr() % 16):
+            raise ValueError(f"the cache's {name} must be contiguous and start on a 16-byte boundary")
     if D not in HEAD_DIMS:
         raise ValueError(f"head_dim must be one of {HEAD_DIMS}, got {D}")
     if table.dim() != 2 or table.dtype != torch.int32 or table.device != dev or 0 in table.shape:
