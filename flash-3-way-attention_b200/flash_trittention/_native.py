@@ -85,8 +85,28 @@ def host_backward(*args):
     """The same for a backward call."""
 
 
+def host_norm_rotary(*args):
+    """The same for ``qk_norm_rotary``, ..."""
+
+
+def host_norm_rotary_backward(*args):
+    """... its backward,"""
+
+
+def host_cache_write(*args):
+    """``cache_write``,"""
+
+
+def host_cache_read(*args):
+    """``cache_read``,"""
+
+
+def host_decode(*args):
+    """and ``tdp_decode``, ``dps_append`` and ``dps_decode``."""
+
+
 def _load_host(L):
-    global _host, host_forward, host_backward
+    global _host, host_forward, host_backward, host_norm_rotary, host_norm_rotary_backward, host_cache_write, host_cache_read, host_decode
     try:
         host = importlib.import_module("._host", __package__)
         built_for = getattr(host, "torch_version", "another version")
@@ -97,12 +117,16 @@ def _load_host(L):
                       "with `python flash-3-way-attention_b200/build.py`", stacklevel=3)
         return
     _host = host
-    _host.init(*(C.cast(f, C.c_void_p).value for f in (L.tritt_tdp_fwd, L.tritt_tdp_bwd, L.tritt_dps_fwd, L.tritt_dps_bwd,
-                                                       L.tritt_dps_bwd_saved, L.tritt_workspace_bytes_flags,
-                                                       L.tritt_tdp_fwd_workspace)))
+    # (the order is that of the extension's own list)
+    _host.init(*(C.cast(getattr(L, "tritt_" + name), C.c_void_p).value for name in (
+        "tdp_fwd", "tdp_bwd", "dps_fwd", "dps_bwd", "dps_bwd_saved", "workspace_bytes_flags", "tdp_fwd_workspace", "qk_norm_rotary_fwd",
+        "qk_norm_rotary_bwd", "qk_norm_rotary_workspace", "cache_write", "cache_read", "tdp_decode", "dps_append", "dps_decode",
+        "decode_workspace")))
     for device, address in _status_ptr.items():
         _host.set_status(device, address)
     host_forward, host_backward = _host.forward, _host.backward
+    host_norm_rotary, host_norm_rotary_backward = _host.norm_rotary, _host.norm_rotary_backward
+    host_cache_write, host_cache_read, host_decode = _host.cache_write, _host.cache_read, _host.decode
 
 
 def lib():
@@ -186,9 +210,9 @@ def dtype_code(dt: torch.dtype) -> int:
 
 
 def host_result(out, what: str):
-    """The tensors of a host_forward / host_backward call; an error code is raised."""
+    """What a call of the extension returned, its tensors or 0; an error code is raised."""
     global launches
-    if out.__class__ is int:
+    if out.__class__ is int and out:
         _check(out, what)
     launches += 1
     return out

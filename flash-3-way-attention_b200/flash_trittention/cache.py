@@ -157,7 +157,11 @@ def _need_lse(cache):
 def cache_write(cache: TrittentionCache, table: Tensor, context: Tensor, k1: Tensor, k2: Tensor, v1: Tensor, v2: Tensor,
                 counts: Optional[Tensor] = None) -> None:
     """Quantises the new tokens' rows of K1, K2, SiLU(V1) and V2 into their places (``v1`` is the raw tensor); nothing else changes."""
-    new = _check_new(_cache(cache), table, (k1, k2, v1, v2))
+    done = _native.host_cache_write(*_cache(cache), table, context, counts, None, k1, k2, v1, v2)
+    if done is not None:
+        _native.host_result(done, "tritt_cache_write")
+        return
+    new = _check_new(cache, table, (k1, k2, v1, v2))
     c, keep = _describe(cache, table, context, new[0].shape[2], counts, None)
     _native.cache_write(c, new, _native.dtype_code(new[0].dtype), new[0].device)
 
@@ -166,7 +170,9 @@ def cache_read(cache: TrittentionCache, table: Tensor, context: Tensor, n: int, 
                counts: Optional[Tensor] = None) -> Tuple[Tensor, ...]:
     """``n`` tokens of each sequence from token ``context[b]`` on, read back: the four parts ``[B, N, n, D]`` in ``dtype`` and, of a
     dot-product-sum cache, the log-sum-exps ``[B, N, n]``.  Zeros for tokens past ``counts[b]``."""
-    _cache(cache)
+    out = _native.host_cache_read(*_cache(cache), table, context, counts, None, n, _native.dtype_code(dtype))
+    if out is not None:
+        return _native.host_result(out, "tritt_cache_read")
     c, keep = _describe(cache, table, context, int(n), counts, None)
     code, dev = _native.dtype_code(dtype), cache.codes.device
     parts = tuple(torch.empty(c.B, c.N, c.n, c.D, dtype=dtype, device=dev) for _ in range(4))
@@ -187,14 +193,20 @@ def tdp_decode(q: Tensor, cache: TrittentionCache, table: Tensor, context: Tenso
     significant bits, fp32 sums and soft-max.  fp32 queries, other head dimensions and ``input_precision="ieee"`` run in fp32 on the CUDA
     cores.  No gradient flows through the cache.
     """
-    q, = _check_new(_cache(cache), table, (q,))
+    flags, softmax_scale = _flags(input_precision), float(softmax_scale)
+    out = _native.host_decode(_native.OP_TDP_DECODE, *_cache(cache), table, context, counts, ancestors, flags, softmax_scale, q, k1_window,
+                              k2_window, kk_left, kk_right, bool(return_lse))
+    if out is not None:
+        o, lse = _native.host_result(out, "tritt_tdp_decode")
+        return (o, lse) if return_lse else o
+    q, = _check_new(cache, table, (q,))
     c, keep = _describe(cache, table, context, q.shape[2], counts, ancestors)
     windows = [_UNLIMITED if w is None else min(int(w), _UNLIMITED) for w in (k1_window, k2_window, kk_left, kk_right)]
     if min(windows) < 0:
         raise ValueError(f"window arguments must be >= 0, got {(k1_window, k2_window, kk_left, kk_right)}")
     o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if return_lse else None
-    _native.tdp_decode(c, q, o, lse, float(softmax_scale), *windows, flags=_flags(input_precision))
+    _native.tdp_decode(c, q, o, lse, softmax_scale, *windows, flags=flags)
     return (o, lse) if return_lse else o
 
 
@@ -204,12 +216,18 @@ def dps_append(cache: TrittentionCache, table: Tensor, context: Tensor, k1: Tens
     """Writes new tokens of the dot-product-sum form: K1, K2, SiLU(V1), and for each token ``t``, attending from its ``k2`` to the tokens ``s``
     with ``position(t) - position(s) <= k_diff``, the row ``W = softmax(softmax_scale * k1[s].k2[t]) SiLU(v1[s]) * v2[t]`` and the
     log-sum-exp.  These do not depend on a query and are computed once.  Kernels as for ``tdp_decode``."""
-    _need_lse(_cache(cache))
+    flags, softmax_scale = _flags(input_precision), float(softmax_scale)
+    done = _native.host_decode(_native.OP_DPS_APPEND, *_cache(cache), table, context, counts, ancestors, flags, softmax_scale, k1, k2, v1, v2,
+                               k_diff)
+    if done is not None:
+        _native.host_result(done, "tritt_dps_append")
+        return
+    _need_lse(cache)
     new = _check_new(cache, table, (k1, k2, v1, v2))
     c, keep = _describe(cache, table, context, new[0].shape[2], counts, ancestors)
     if k_diff < 0:
         raise ValueError(f"k_diff must be >= 0, got {k_diff}")
-    _native.dps_append(c, new, float(softmax_scale), min(int(k_diff), _UNLIMITED), flags=_flags(input_precision))
+    _native.dps_append(c, new, softmax_scale, min(int(k_diff), _UNLIMITED), flags=flags)
 
 
 def dps_decode(q: Tensor, cache: TrittentionCache, table: Tensor, context: Tensor, softmax_scale: float = 1 / 8,
@@ -217,10 +235,14 @@ def dps_decode(q: Tensor, cache: TrittentionCache, table: Tensor, context: Tenso
                input_precision: Optional[str] = None) -> Tuple[Tensor, Tensor]:
     """Dot-product-sum attention of new tokens that ``dps_append`` has written: ``(o [B, N, n, D], m [B, N, n] fp32 log-sum-exp)``, as the module
     ``TrittentionTriton`` returns them.  Rows past ``counts[b]`` or of a free slot are 0 and ``-inf``.  Kernels as for ``tdp_decode``."""
-    _need_lse(_cache(cache))
+    flags, softmax_scale = _flags(input_precision), float(softmax_scale)
+    out = _native.host_decode(_native.OP_DPS_DECODE, *_cache(cache), table, context, counts, ancestors, flags, softmax_scale, q)
+    if out is not None:
+        return _native.host_result(out, "tritt_dps_decode")
+    _need_lse(cache)
     q, = _check_new(cache, table, (q,))
     c, keep = _describe(cache, table, context, q.shape[2], counts, ancestors)
     o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     m = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
-    _native.dps_decode(c, q, o, m, float(softmax_scale), flags=_flags(input_precision))
+    _native.dps_decode(c, q, o, m, softmax_scale, flags=flags)
     return o, m

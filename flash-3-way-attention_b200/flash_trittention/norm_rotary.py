@@ -88,6 +88,9 @@ def _arguments(xs, ws, cos, sin, positions, eps, interleaved):
 
 
 def norm_rotary_forward(xs, ws, cos, sin, positions, eps, interleaved):
+    out = _native.host_norm_rotary(*xs, *ws, cos, sin, positions, eps, interleaved)
+    if out is not None:
+        return _native.host_result(out, "tritt_qk_norm_rotary_fwd")
     _check(xs, ws, cos, sin, positions)
     if not xs[0].is_cuda:
         raise RuntimeError("qk_norm_rotary runs on CUDA tensors only (there is no CPU path)")
@@ -101,6 +104,9 @@ def norm_rotary_forward(xs, ws, cos, sin, positions, eps, interleaved):
 
 def norm_rotary_backward(xs, ws, cos, sin, positions, eps, interleaved, dys, weights_too):
     """``(dq, dk1, dk2, dw, dw, dw)``; the inputs' gradients are laid out as the inputs, the weights' are ``None`` if not wanted."""
+    out = _native.host_norm_rotary_backward(*xs, *ws, cos, sin, positions, eps, interleaved, *dys, *weights_too)
+    if out is not None:
+        return _native.host_result(out, "tritt_qk_norm_rotary_bwd")
     a, keep = _arguments(xs, ws, cos, sin, positions, eps, interleaved)
     dys = [_native.strided(torch.zeros_like(x) if dy is None else dy) for x, dy in zip(xs, dys)]
     dxs = [torch.empty_like(x) for x in xs]

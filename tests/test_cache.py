@@ -548,6 +548,66 @@ def test_graphs_that_run_at_once_and_another_stream():
     ft.check_status(DEV)
 
 
+HOST = ("host_norm_rotary", "host_norm_rotary_backward", "host_cache_write", "host_cache_read", "host_decode")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("tree", [False, True])
+def test_calls_by_the_extension_and_by_the_python_code(dtype, tree, monkeypatch):
+    """The same bits; the extension takes every one of these calls, and leaves those that need help."""
+    _native.lib()
+    _native.status_word(DEV)
+    assert _native._host is not None, "the host extension is not built"
+
+    def calls():
+        bt = Batch(3, 2, 5, 64, dtype, "e4m3", 16, [20, 0, 33], dps=True, parents=_tree(5, 2) if tree else None)
+        q, out = bt.q.to(DEV), []
+        ct = torch.tensor([5, 2, 3], dtype=torch.int32, device=DEV)
+        kw = dict(counts=ct, ancestors=bt.ancestors)
+        out += [ft.tdp_decode(q, bt.cache, bt.table, bt.context, 0.1, 30, None, 20, **kw)]
+        out += ft.tdp_decode(q, bt.cache, bt.table, bt.context, 0.1, return_lse=True, input_precision="ieee", **kw)
+        ft.cache_write(bt.cache, bt.table, bt.context, q, q * 2, q, q, counts=ct)
+        ft.dps_append(bt.cache, bt.table, bt.context, q, q, q, q, 0.1, 20, **kw)
+        out += ft.dps_decode(q, bt.cache, bt.table, bt.context, 0.1, **kw)
+        out += ft.cache_read(bt.cache, bt.table, bt.context, 5, TYPES[dtype], counts=ct)
+        return out + [t.clone() for t in bt.cache]
+
+    taken = []
+    for name in HOST:
+        f = getattr(_native._host, name[5:])
+        monkeypatch.setattr(_native, name, lambda *a, f=f, name=name: taken.append((name, f(*a))) or taken[-1][1])
+    fast = calls()
+    assert len(taken) == 6 and all(r is not None for _, r in taken)
+    for name in HOST:
+        monkeypatch.setattr(_native, name, lambda *a: None)
+    slow = calls()
+    assert len(fast) == len(slow) and all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(fast, slow))
+    ft.check_status(DEV)
+
+
+@pytest.mark.gpu
+def test_calls_that_need_help():
+    """Rows that start off 16-byte boundaries or are not contiguous, a table with gaps, another current stream: copied first, the same result."""
+    bt = Batch(2, 2, 3, 64, "fp16", "e4m3", 16, [20, 33], dps=True)
+    q = bt.q.to(DEV)
+    want = ft.tdp_decode(q, bt.cache, bt.table, bt.context, 0.1)
+    store = torch.empty(q.numel() + 1, dtype=q.dtype, device=DEV)
+    odd = store[1:].view(q.shape).copy_(q)
+    gaps = torch.zeros(2, 2 * bt.table.shape[1], dtype=torch.int32, device=DEV)[:, ::2].copy_(bt.table)
+    wide = torch.zeros(2, 9, dtype=torch.int32, device=DEV)
+    wide[:, : bt.table.shape[1]] = bt.table
+    for x, table, ctx in [(odd, bt.table, bt.context), (q.transpose(2, 3).contiguous().transpose(2, 3), bt.table, bt.context),
+                          (q, gaps, bt.context), (q, wide[:, : bt.table.shape[1]], bt.context), (q, bt.table, bt.context.repeat_interleave(2)[::2])]:
+        assert torch.equal(ft.tdp_decode(x, bt.cache, table, ctx, 0.1), want)
+        with torch.cuda.stream(torch.cuda.Stream()):
+            torch.cuda.current_stream().wait_stream(torch.cuda.default_stream())
+            other = ft.tdp_decode(x, bt.cache, table, ctx, 0.1)
+        torch.cuda.synchronize()
+        assert torch.equal(other, want)
+    ft.check_status(DEV)
+
+
 # ---------------------------------------------------------------- refusals
 
 def test_tree_ancestors():
@@ -562,7 +622,7 @@ def test_tree_ancestors():
 def test_new_cache():
     c = ft.new_cache(3, 16, 2, 64, torch.int8, "cpu", dps=True)
     assert c.codes.shape == (3, 4, 2, 16, 64) and c.exponents.shape == (3, 4, 2, 16) and c.lse.shape == (3, 2, 16)
-    assert ft.new_cache(1, 8, 1, 16, device="cpu").lse is None
+    assert ft.new_cache(1, 16, 1, 16, device="cpu").lse is None
     for kw in (dict(dtype=torch.float32), dict(page_size=12), dict(page_size=8), dict(head_dim=48)):
         with pytest.raises(ValueError):
             ft.new_cache(**{**dict(pages=1, page_size=16, heads=1, head_dim=64, device="cpu"), **kw})

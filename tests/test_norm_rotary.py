@@ -180,6 +180,39 @@ def test_repeats_itself_and_is_captured():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_calls_by_the_extension_and_by_the_python_code(dtype, monkeypatch):
+    _native.lib()
+    _native.status_word(DEV)
+    assert _native._host is not None, "the host extension is not built"
+    xs, ws, cos, sin = _inputs(2, 3, 20, 64, dtype, "heads", 32, strided=True)
+    args = [t.to(DEV).requires_grad_(True) for t in xs] + [torch.nn.Parameter(w.to(DEV)) for w in ws]
+    positions = torch.arange(40, device=DEV).view(2, 20)
+    dys = [torch.randn(2, 20, 3, 64, device=DEV).to(dtype).transpose(1, 2) for _ in range(3)]
+
+    def calls():
+        y = ft.qk_norm_rotary(*args, cos.to(DEV), sin.to(DEV), positions, interleaved=True)
+        return [t.detach() for t in y] + list(torch.autograd.grad(y, args, dys))
+
+    taken = []
+    for name in ("host_norm_rotary", "host_norm_rotary_backward"):
+        f = getattr(_native._host, name[5:])
+        monkeypatch.setattr(_native, name, lambda *a, f=f: taken.append(f(*a)) or taken[-1])
+    fast = calls()
+    assert len(taken) == 2 and all(r is not None for r in taken)
+    for name in ("host_norm_rotary", "host_norm_rotary_backward"):
+        monkeypatch.setattr(_native, name, lambda *a: None)
+    slow = calls()
+    assert all(torch.equal(a, b) and a.stride() == b.stride() for a, b in zip(fast, slow))
+    # rows off 16-byte boundaries are copied, their gradients come back in their own layout
+    store = torch.empty(xs[0].numel() + 1, dtype=dtype, device=DEV)
+    odd = store[1:].view(2, 20, 3, 64).copy_(xs[0].to(DEV).transpose(1, 2)).transpose(1, 2).requires_grad_(True)
+    y = ft.qk_norm_rotary(odd, *args[1:], cos.to(DEV), sin.to(DEV), positions, interleaved=True)
+    again = torch.autograd.grad(y, [odd], dys)[0]
+    assert torch.equal(y[0], fast[0]) and torch.equal(again, fast[3])
+
+
+@pytest.mark.gpu
 def test_in_front_of_both_attentions():
     """One training step of norm, rotation and attention: gradients reach the projections' parts."""
     g = torch.Generator(device=DEV).manual_seed(0)
