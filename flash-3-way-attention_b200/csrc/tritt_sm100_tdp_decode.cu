@@ -15,18 +15,26 @@
 // accumulator, which is multiplied where it grows.  A is rounded once to 11 bits, P (times 2^7, fp16's lower range) once.
 //
 //   warp 0        issues tcgen05.mma: S_x = A_x K1^T, acc_x += P_x V1 for the tiles x = a, b in turn, P_x read from TMEM over S_x
-//   warps 4-7     producers: a warp loads 32 rows of a slab (pages, exponents, codes), converts and stores them with the 128-byte
-//                 swizzle; the loads of a tile are in flight before its stage is free
-//   warps 8-15    one row a thread: form A, then maximum, exponentials, P; at the end of a piece the group's sum
+//   warps 4-7     keys: a warp loads 32 rows of a slab (pages, exponents, codes), converts and stores them with the 128-byte swizzle;
+//                 the loads of a tile are in flight before its stage is free.  They form tile b's A, and tell its rows' masks and scales
+//   warps 8-11    values in the same way, and tile a's A
+//   warps 12-19   one row a thread: maximum, exponentials, P; at the end of a piece the group's sum
+// (Keys and values from the same warps: each tile's loads took 1.3 us that nothing hid, 690 us for 8 tokens over 2040 at D=128, 16 heads, of
+// which 290 were theirs.  A formed by the soft-max warps: 15 us a piece, of which the products of a narrow window are one.)
 #include "tritt_cache.cuh"
 #include "tritt_sm100.cuh"
 #include "tritt_sm100_tdp.cuh"
+
+#include <atomic>
 
 namespace tritt {
 namespace {
 using namespace sm100;
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 640;
+constexpr int kRegsLaunch = 96;   // a thread; the soft-max warps take what the others give up
+constexpr int kRegsIssue = 32, kRegsLoad = 88, kRegsSoftmax = 136;
+static_assert(kRegsIssue + 2 * kRegsLoad + 2 * kRegsSoftmax <= 5 * kRegsLaunch, "more registers than the launch has");
 constexpr float kGap = 8.f;      // the accumulator is rescaled when a row's maximum grew by more than 2^8
 constexpr float kLift = 7.f;     // P is formed times 2^7: at most 2^15, normal down to 2^-21 of the reference
 constexpr int kMetas = 6;        // slabs whose descriptions are kept: two more than the ring's depth (one is overwritten when S of the slab
@@ -39,22 +47,34 @@ template <int D> struct Cfg {
   static constexpr int kOffA = 0;                                  // two tiles
   static constexpr int kOffK = 2 * kTile;
   static constexpr int kOffV = kOffK + kStages * kTile;
-  static constexpr int kOffQ = kOffV + kStages * kTile;            // [8 warps][D] fp32
-  static constexpr int kOffMisc = kOffQ + 8 * D * 4;
+  static constexpr int kOffQ = kOffV + kStages * kTile;            // [8 warps][D] fp16
+  static constexpr int kOffRows = kOffQ + 8 * D * 2;               // two pieces' [256] RowInfo
+  static constexpr int kOffMisc = kOffRows + 2 * 256 * 32;
   static constexpr int kSmem = kOffMisc + 1024;
   static constexpr int kTmemO = 256;                               // S_a | S_b | acc_a | acc_b
 };
 
-struct Meta {             // of one slab, by the warp that loaded 32 of its rows
+struct __align__(16) Meta {   // of one slab, by the warp that loaded 32 of its rows
   uint32_t there[4];      // rows that have a place
   uint32_t nan[4];        // rows that read as NaN (K1 or V1)
   float scale[4];         // of the 32 columns' scores
   int v_exp[4];           // largest exponent byte of V1's rows
 };
 
+// A row of a tile, by the thread that formed its A for the one that works on its scores.
+struct __align__(16) RowInfo {
+  unsigned long long tree;   // of a tree's tokens, those that it attends to
+  size_t v2_row;             // its V2's number in the cache
+  float scale;               // of its scores
+  int c_lo, c_hi;            // columns that it attends to, by their numbers
+  int flags;                 // V2's exponent byte; kRowNan: it reads as NaN
+};
+static_assert(sizeof(RowInfo) == 32, "two 16-byte accesses");
+constexpr int kRowNan = 256;
+
 struct Misc {
   uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
-  uint64_t meta_full[kMetas], a_ready[2], s_ready[2], p_ready[2], o_done[2];
+  uint64_t meta_full[kMetas], a_ready[2], a_free[2], s_ready[2], p_ready[2], o_done[2];
   Meta meta[kMetas];
   uint32_t tmem_base;
   int abort_flag;
@@ -104,48 +124,76 @@ __device__ __forceinline__ Line line_of(const TdpDecodeArgs& a, int b) {
   return l;
 }
 __device__ __forceinline__ Columns columns_of(const TdpDecodeArgs& a, const Line& l, int pair) {
-  Columns c{kUnlimited, -1};
-  const int g1 = least(pair * 8 + 8, l.cnt * l.groups);
-  for (int g = pair * 8; g < g1; ++g) {
+  const int g0 = pair * 8, g1 = least(g0 + 8, l.cnt * l.groups);
+  int i = g0 / l.groups, r = (g0 - i * l.groups) * 32;
+  const int lo = most(0, l.ctx - a.k1w);
+  if (a.kkl >= l.ctx + l.cnt && a.kkr >= l.ctx + l.cnt) return Columns{lo, l.ctx + (g1 - 1) / l.groups};   // (no band)
+  Columns c{l.ctx, -1};
+  for (int g = g0; g < g1; ++g, r += 32) {
+    if (r == l.groups * 32) r = 0, ++i;
     // positions of the group's rows, whatever the token's depth in a tree (0 to i)
-    const int i = g / l.groups, r = (g - i * l.groups) * 32;
     const int ka = most(0, l.ctx - a.k2w) + r, kb = most(0, l.ctx + i - a.k2w) + r + 31;
-    c.lo = least(c.lo, most(most(0, l.ctx - a.k1w), ka - least(ka, a.kkl)));
+    c.lo = least(c.lo, most(lo, ka - least(ka, a.kkl)));
     c.hi = most(c.hi, kb + least(a.kkr, kUnlimited - 1) < l.ctx ? kb + a.kkr : l.ctx + i);
   }
-  c.lo = least(c.lo, l.ctx);
   return c;
 }
 
-// Steps of a CTA: walks the line from the CTA's first step to its last.
+// Steps of a CTA: walks the line from the CTA's first step to its last.  (Where it stands is found by division once, then by counting.)
 struct Walk {
-  long long x, end, base;   // present step, behind the last, first step of sequence b
-  long long pair_base;      // pairs before sequence b's
-  int b;
+  long long left;           // steps
+  long long pair_base;      // pairs before the present one, of all sequences
+  int b, head, pair, slab;
   Line l;
 };
 struct Piece {
   int b, head, pair, s0, s1;
   long long id;             // pieces are numbered by pair + CTA: each new pair and each cut makes one
 };
-__device__ __forceinline__ bool next_piece(const Params& p, Walk& w, Piece& s) {
-  if (w.x >= w.end) return false;
+__device__ __forceinline__ Walk start_walk(const Params& p, long long total) {
+  long long x = (long long)blockIdx.x * total / p.ctas;
+  Walk w{((long long)blockIdx.x + 1) * total / p.ctas - x, 0, 0, 0, 0, 0, {}};
+  if (w.left == 0) return w;
+  w.l = line_of(p.a, 0);
   while (true) {
-    const long long here = (long long)w.l.pairs * w.l.slabs * p.a.cache.c.N;
-    if (w.x < w.base + here) break;
-    if (w.b + 1 >= p.a.cache.c.B) return false;   // (contexts that changed under the kernel)
-    w.base += here;
-    w.pair_base += (long long)w.l.pairs * p.a.cache.c.N;
+    const long long pairs = (long long)w.l.pairs * p.a.cache.c.N, here = pairs * w.l.slabs;
+    if (x < here) break;
+    x -= here;
+    w.pair_base += pairs;
+    if (w.b + 1 >= p.a.cache.c.B) {   // (contexts that changed under the kernel)
+      w.left = 0;
+      return w;
+    }
     w.l = line_of(p.a, ++w.b);
   }
-  const long long rel = w.x - w.base, pair = rel / w.l.slabs;
+  const long long pair = x / w.l.slabs;
+  w.slab = (int)(x - pair * w.l.slabs);
+  w.head = (int)(pair / w.l.pairs);
+  w.pair = (int)(pair - (long long)w.head * w.l.pairs);
+  w.pair_base += pair;
+  return w;
+}
+__device__ __forceinline__ bool next_piece(const Params& p, Walk& w, Piece& s) {
+  if (w.left <= 0) return false;
+  while (w.slab == w.l.slabs) {   // the next pair, head, sequence (that has any)
+    if (w.l.slabs) ++w.pair_base, ++w.pair;
+    w.slab = 0;
+    if (w.pair < w.l.pairs) break;
+    w.pair = 0;
+    if (w.l.slabs && ++w.head < p.a.cache.c.N) break;
+    w.head = 0;
+    if (w.b + 1 >= p.a.cache.c.B) return false;
+    w.l = line_of(p.a, ++w.b);
+    if (w.l.slabs) break;
+  }
   s.b = w.b;
-  s.head = (int)(pair / w.l.pairs);
-  s.pair = (int)(pair % w.l.pairs);
-  s.s0 = (int)(rel % w.l.slabs);
-  s.s1 = (int)least((int)(w.l.slabs - s.s0 < w.end - w.x ? w.l.slabs - s.s0 : w.end - w.x), w.l.slabs) + s.s0;
-  s.id = w.pair_base + pair + blockIdx.x;
-  w.x += s.s1 - s.s0;
+  s.head = w.head;
+  s.pair = w.pair;
+  s.s0 = w.slab;
+  s.s1 = w.l.slabs - w.slab < w.left ? w.l.slabs : w.slab + (int)w.left;
+  s.id = w.pair_base + blockIdx.x;
+  w.left -= s.s1 - s.s0;
+  w.slab = s.s1;
   return true;
 }
 
@@ -170,20 +218,28 @@ template <int CODE> constexpr int kUp = CODE == TRITT_CODE_F16 ? 0 : CODE == TRI
 // q (largest element in [1, 2)) times a code times 2^-kDown is at most 2^9
 template <int CODE> constexpr int kDown = CODE == TRITT_CODE_F16 ? 7 : 0;
 
+__device__ __forceinline__ uint4 load16_if(const void* p, bool on) {   // zeros where not (a predicate: a branch would keep loads from overlapping)
+  uint4 v;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+      "@p ld.global.nc.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
+      : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
+      : "l"(p), "r"((int)on));
+  return v;
+}
+
 template <int D, int CODE> struct TileLoader {   // a warp's 32 rows of one part of a slab
   static constexpr int kChunks = CODE == TRITT_CODE_F16 ? D / 8 : D / 16;   // of 16 bytes of codes, a row
   uint4 v[kChunks];
-  // page: of the lane's own row, -1: none (zeros)
-  __device__ __forceinline__ void load(const CacheArgs& a, int part, int head, int token0, int page, int lane) {
+  // mine: the lane's own row, null: none (zeros)
+  __device__ __forceinline__ void load(const uint8_t* mine, int lane) {
+    const uint32_t lo = (uint32_t)(size_t)mine, hi = (uint32_t)((size_t)mine >> 32);
 #pragma unroll
     for (int it = 0; it < kChunks; ++it) {
       const int idx = it * 32 + lane, row = idx / kChunks, ch = idx % kChunks;
-      const int pg = __shfl_sync(0xffffffffu, page, row);
-      v[it] = make_uint4(0u, 0u, 0u, 0u);
-      if (pg >= 0) {
-        const size_t at = row_of(a, Place{pg, (token0 + row) & (a.c.page_size - 1)}, part, head);
-        v[it] = __ldg(reinterpret_cast<const uint4*>((const uint8_t*)a.c.codes + at * (size_t)(kChunks * 16)) + ch);
-      }
+      const uint32_t l = __shfl_sync(0xffffffffu, lo, row), h = __shfl_sync(0xffffffffu, hi, row);
+      const size_t at = (size_t)h << 32 | l;
+      v[it] = load16_if((const uint8_t*)at + ch * 16, at != 0);
     }
   }
   // to rows row0 .. row0 + 31 of a tile, each times the power of two of its lane
@@ -211,6 +267,107 @@ template <int D, int CODE> struct TileLoader {   // a warp's 32 rows of one part
   }
 };
 
+// A warp's 32 rows of a tile: token k of new token i each.  A = 2^-kDown q * code, q brought to [1, 2); the powers of two and alpha go to
+// the scores' scale.
+template <typename T16, int D, int CODE>
+__device__ __forceinline__ void form_rows(const TdpDecodeArgs& a, const Line& l, const Piece& s, int x, int wq, int lane, uint8_t* tile, __half* sq,
+                                          RowInfo* info) {
+  const CacheArgs& ca = a.cache;
+  const int g = s.pair * 8 + x * 4 + wq;
+  const bool any = g < l.cnt * l.groups;
+  const int i = any ? g / l.groups : 0;
+  const T16* qp = (const T16*)a.q.p + rows_at(a.q, s.b, s.head, i);
+  constexpr int E = D / 32;
+  float f[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) f[e] = to_f(qp[lane * E + e]);
+  const unsigned long long word = ca.c.ancestors ? seen_word(ca, s.b, i) : 0;
+  const int pos_q = l.ctx + (ca.c.ancestors ? __popcll(word) - 1 : i);
+  const int pk = most(0, pos_q - a.k2w) + (g - i * l.groups) * 32 + lane;
+  bool on = any && pk <= pos_q;
+  int token = pk;
+  if (ca.c.ancestors && pk >= l.ctx) {
+    unsigned long long left = word;
+    for (int c = l.ctx; c < pk && left; ++c) left &= left - 1;
+    token = l.ctx + (left ? __ffsll(left) - 1 : 0);
+  }
+  RowInfo r{0, 0, 0.f, kUnlimited, -1, 0};
+  const uint8_t* codes = (const uint8_t*)ca.c.codes;
+  int byte = 0;
+  if (on) {
+    const Place at = place_of(ca, s.b, token);
+    if (at.page < 0) {
+      on = false;
+      if (ca.status) atomicOr(ca.status, kStatusPlace);
+    } else {
+      const size_t row = row_of(ca, at, kPartK2, s.head);
+      r.v2_row = row_of(ca, at, kPartV2, s.head);
+      codes += row * (size_t)(D * (CODE == TRITT_CODE_F16 ? 2 : 1));
+      byte = __ldg(ca.c.exponents + row);
+      const int byte2 = __ldg(ca.c.exponents + r.v2_row);
+      r.flags = byte2 | (byte == 255 || byte2 == 255 ? kRowNan : 0);
+      // columns that the row attends to: numbers c_lo .. c_hi, and of a tree's tokens a word
+      const int last = pk < kUnlimited - a.kkr ? least(pos_q, pk + a.kkr) : pos_q;
+      r.c_lo = most(most(0, pos_q - a.k1w), pk - least(pk, a.kkl));
+      r.c_hi = ca.c.ancestors ? least(l.ctx - 1, last) : last;
+      if (ca.c.ancestors) {
+        unsigned long long left = word;
+        for (int c = l.ctx; left; ++c, left &= left - 1)
+          if (c >= r.c_lo && c <= last) r.tree |= left & (~left + 1);
+      }
+    }
+  }
+  uint32_t big = 0;
+#pragma unroll
+  for (int e = 0; e < E; ++e) big = max(big, __float_as_uint(f[e]) & 0x7fffffffu);
+  big = __reduce_max_sync(0xffffffffu, big);
+  const int power = max(min(254 - (int)(big >> 23), 253), 1);   // (the largest numbers are brought to [2, 4))
+  const float up = __uint_as_float((uint32_t)power << 23) * (a.scale2 < 0.f ? -1.f : 1.f);
+  __syncwarp();
+#pragma unroll
+  for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(sq + lane * E + e) = pack2<__half>(f[e] * up, f[e + 1] * up);
+  __syncwarp();
+  r.scale = fabsf(a.scale2) * (on && byte != 255 ? __uint_as_float((uint32_t)byte << 23) : 0.f) * (float)(1 << kDown<CODE>) *
+            __uint_as_float((uint32_t)(254 - power) << 23);
+  const int row = wq * 32 + lane;
+  // (q as fp16 is exact, and so is a code times 2^-kDown; their product is rounded once)
+  constexpr int kBytes = CODE == TRITT_CODE_F16 ? 16 : 8, kBatch = CODE == TRITT_CODE_F16 ? 4 : 8;   // of eight codes; chunks whose loads overlap
+  auto form_chunk = [&](int ch, uint32_t (&h)[4]) {
+    uint4 q = *reinterpret_cast<const uint4*>(sq + ch * 8);
+    const uint32_t qw[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      __half2 c = *reinterpret_cast<const __half2*>(&h[e]);
+      if (kDown<CODE> > 0) c = __hmul2(c, __float2half2_rn(1.f / (1 << kDown<CODE>)));
+      c = __hmul2(c, *reinterpret_cast<const __half2*>(&qw[e]));
+      h[e] = *reinterpret_cast<const uint32_t*>(&c);
+    }
+    *reinterpret_cast<uint4*>(tile + (ch >> 3) * 16384 + swz128(row, ch & 7)) = make_uint4(h[0], h[1], h[2], h[3]);
+  };
+#pragma unroll 1
+  for (int c0 = 0; c0 < D / 8; c0 += kBatch) {
+    uint4 v[kBatch * kBytes / 16];
+#pragma unroll
+    for (int k = 0; k < kBatch * kBytes / 16; ++k) v[k] = load16_if(codes + c0 * kBytes + k * 16, on);
+#pragma unroll
+    for (int k = 0; k < kBatch * kBytes / 16; ++k) {
+      if constexpr (CODE == TRITT_CODE_F16) {
+        uint32_t h[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+        form_chunk(c0 + k, h);
+      } else {
+        uint32_t h[4];
+        bytes_to_halves<CODE>(v[k].x, h[0], h[1]);
+        bytes_to_halves<CODE>(v[k].y, h[2], h[3]);
+        form_chunk(c0 + 2 * k, h);
+        bytes_to_halves<CODE>(v[k].z, h[0], h[1]);
+        bytes_to_halves<CODE>(v[k].w, h[2], h[3]);
+        form_chunk(c0 + 2 * k + 1, h);
+      }
+    }
+  }
+  info[row] = r;
+}
+
 template <typename T16, int D, int CODE>
 __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_constant__ Params p) {
   using C = Cfg<D>;
@@ -235,6 +392,7 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
     for (int i = 0; i < kMetas; ++i) mbar_init(&ms.meta_full[i], 4);
     for (int x = 0; x < 2; ++x) {
       mbar_init(&ms.a_ready[x], 128);
+      mbar_init(&ms.a_free[x], 1);
       mbar_init(&ms.s_ready[x], 1);
       mbar_init(&ms.p_ready[x], 128);
       mbar_init(&ms.o_done[x], 1);
@@ -270,336 +428,315 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
   tc_fence_after();
   const uint32_t tmem = ms.tmem_base;
   volatile int* abort_flag = &ms.abort_flag;
-  const long long total = ms.total;
-  Walk walk;
-  walk.x = (long long)blockIdx.x * total / p.ctas;
-  walk.end = ((long long)blockIdx.x + 1) * total / p.ctas;
-  walk.base = walk.pair_base = 0;
-  walk.b = 0;
+  Walk walk = start_walk(p, ms.total);
   Piece s;
-  if (walk.x < walk.end) walk.l = line_of(a, 0);
+  auto slabs_of = [&](const Columns& col) { return least(s.s1, (col.hi - col.lo + 128) / 128) - s.s0; };
+  auto tiles_of = [&]() { return walk.l.cnt * walk.l.groups - s.pair * 8 > 4 ? 2 : 1; };
+  uint8_t* const sA = smem + C::kOffA;
+  RowInfo* const sRows = reinterpret_cast<RowInfo*>(smem + C::kOffRows);
+  __half* const sQ = reinterpret_cast<__half*>(smem + C::kOffQ);
+  // (every lane has the same; the reduction tells the compiler so, which keeps what follows from it on the uniform datapath)
+  auto uniform = [](int v) -> int { return __reduce_max_sync(0xffffffffu, v); };
 
-  if (warp == 0) {
-    // ------------------------------------------------------------------ products
-    const bool leader = elect_one();
-    auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag)); };
-    auto commit = [&](uint64_t* bar) {
-      if (leader) mma_commit(bar);
-    };
-    constexpr uint32_t idesc_pv = make_idesc_f16(128, D, 0, false, true);
-    constexpr uint32_t kHi = desc_hi(1024);
-    const uint32_t aLo = desc_lo(smem_u32(smem + C::kOffA), 16);
-    int slab = 0, pieces[2] = {0, 0}, pcount[2] = {0, 0};   // slabs so far, each tile's pieces and P's
-    bool alive = true;
-    while (alive && next_piece(p, walk, s)) {
-      const Columns col = columns_of(a, walk.l, s.pair);
-      const int n = least(s.s1, (col.hi - col.lo + 128) / 128) - s.s0;
-      if (n <= 0) continue;
-      const int tiles = least(8, walk.l.cnt * walk.l.groups - s.pair * 8) > 4 ? 2 : 1;
-      auto width = [&](int i) { return least(128, col.hi + 1 - (col.lo + (s.s0 + i) * 128)); };
-      // S_x of slab i
-      auto issue_s = [&](int x, int i) {
-        const int pos = slab + i, st = pos % NS;
-        if (x == 0 && !wait_all(&ms.k_full[st], (pos / NS) & 1)) return false;
-        tc_fence_after();
-        const uint32_t bLo = desc_lo(smem_u32(smem + C::kOffK + st * C::kTile), 16);
-        const uint32_t idesc = make_idesc_f16(128, (width(i) + 31) / 32 * 32, 0, false, false);
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t kk = (k >> 2) * (16384 >> 4) + (k & 3) * 2;
-          if (leader) mma_ss_lo(tmem + x * 128, aLo + x * (C::kTile >> 4) + kk, bLo + kk, kHi, idesc, k > 0);
-        }
-        commit(&ms.s_ready[x]);
-        if (x == tiles - 1) commit(&ms.k_empty[st]);
-        return true;
+  if (warp < 4) {
+    set_regs<kRegsLaunch, kRegsIssue>();
+    if (warp == 0) {
+      // ------------------------------------------------------------------ products
+      // (the whole warp walks the schedule converged and one elected lane issues)
+      const bool leader = elect_one();
+      auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag)); };
+      auto commit = [&](uint64_t* bar) {
+        if (leader) mma_commit(bar);
       };
-      auto issue_pv = [&](int x, int i) {
-        const int pos = slab + i, st = pos % NS;
-        if (x == 0 && !wait_all(&ms.v_full[st], (pos / NS) & 1)) return false;
-        tc_fence_after();
-        const uint32_t bLo = desc_lo(smem_u32(smem + C::kOffV + st * C::kTile), 16384);
-        const int steps = (width(i) + 15) / 16;
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (leader && k < steps)
-            mma_ts_lo(tmem + C::kTmemO + x * D, tmem + x * 128 + k * 8, bLo + k * (2048 >> 4), kHi, idesc_pv, k > 0 || i > 0);
-        if (x == tiles - 1) commit(&ms.v_empty[st]);
-        if (i == n - 1) commit(&ms.o_done[x]);
-        return true;
-      };
-      for (int x = 0; x < tiles && alive; ++x) alive = wait_all(&ms.a_ready[x], pieces[x] & 1) && issue_s(x, 0);
-      for (int i = 0; i < n && alive; ++i)
-        for (int x = 0; x < tiles && alive; ++x) {
-          alive = wait_all(&ms.p_ready[x], pcount[x] & 1);
-          if (!alive) break;
-          pcount[x] += 1;
+      constexpr uint32_t idesc_s = make_idesc_f16(128, 128, 0, false, false), idesc_pv = make_idesc_f16(128, D, 0, false, true);
+      constexpr uint32_t kHi = desc_hi(1024);
+      const uint32_t aLo = desc_lo(smem_u32(sA), 16), kLo = desc_lo(smem_u32(smem + C::kOffK), 16), vLo = desc_lo(smem_u32(smem + C::kOffV), 16384);
+      int kst = 0, kph = 0, vst = 0, vph = 0;   // the rings' next stages
+      int pieces[2] = {0, 0}, pcount[2] = {0, 0};
+      bool alive = true;
+      while (alive && next_piece(p, walk, s)) {
+        const Columns col = columns_of(a, walk.l, s.pair);
+        const int n = uniform(slabs_of(col));
+        if (n <= 0) continue;
+        const int tiles = uniform(tiles_of());
+        const int wide = uniform(col.hi + 1 - (col.lo + s.s0 * 128));   // columns from the first slab on
+        // S_x of slab i into its scores, P_x V of slab i: all of the slab's columns, or as many blocks of 32 (16) as there are
+        auto issue_s = [&](auto xc, int i) {
+          constexpr int X = decltype(xc)::value;
+          if (X == 0 && !wait_all(&ms.k_full[kst], kph)) return false;
           tc_fence_after();
+          const uint32_t bLo = kLo + kst * (C::kTile >> 4);
+          const int w = wide - i * 128;
+          if (w > 96) {
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+              const uint32_t kk = (k >> 2) * (16384 >> 4) + (k & 3) * 2;
+              if (leader) mma_ss_lo(tmem + X * 128, aLo + X * (C::kTile >> 4) + kk, bLo + kk, kHi, idesc_s, k > 0);
+            }
+          } else {
+            const uint32_t idesc = make_idesc_f16(128, (w + 31) / 32 * 32, 0, false, false);
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+              const uint32_t kk = (k >> 2) * (16384 >> 4) + (k & 3) * 2;
+              if (leader) mma_ss_lo(tmem + X * 128, aLo + X * (C::kTile >> 4) + kk, bLo + kk, kHi, idesc, k > 0);
+            }
+          }
+          commit(&ms.s_ready[X]);
+          if (i == n - 1) commit(&ms.a_free[X]);
+          if (X == tiles - 1) {
+            commit(&ms.k_empty[kst]);
+            if (++kst == NS) kst = 0, kph ^= 1;
+          }
+          return true;
+        };
+        auto issue_pv = [&](auto xc, int i) {
+          constexpr int X = decltype(xc)::value;
+          if (!wait_all(&ms.p_ready[X], pcount[X] & 1)) return false;
+          ++pcount[X];
+          if (X == 0 && !wait_all(&ms.v_full[vst], vph)) return false;
+          tc_fence_after();
+          const uint32_t bLo = vLo + vst * (C::kTile >> 4);
+          const int w = wide - i * 128;
+          if (w > 112) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              if (leader)
+                mma_ts_lo(tmem + C::kTmemO + X * D, tmem + X * 128 + k * 8, bLo + k * (2048 >> 4), kHi, idesc_pv, k > 0 || i > 0);
+          } else {
+#pragma unroll 1
+            for (int k = 0; k * 16 < w; ++k)
+              if (leader)
+                mma_ts_lo(tmem + C::kTmemO + X * D, tmem + X * 128 + k * 8, bLo + k * (2048 >> 4), kHi, idesc_pv, k > 0 || i > 0);
+          }
+          if (i == n - 1) commit(&ms.o_done[X]);
+          if (X == tiles - 1) {
+            commit(&ms.v_empty[vst]);
+            if (++vst == NS) vst = 0, vph ^= 1;
+          }
+          return true;
+        };
+        constexpr std::integral_constant<int, 0> ta{};
+        constexpr std::integral_constant<int, 1> tb{};
+        alive = wait_all(&ms.a_ready[0], pieces[0] & 1) && issue_s(ta, 0) &&
+                (tiles == 1 || (wait_all(&ms.a_ready[1], pieces[1] & 1) && issue_s(tb, 0)));
+        for (int i = 0; i < n && alive; ++i) {
           // (S_x of the next slab overwrites P_x: the pipe runs it behind P_x V)
-          alive = issue_pv(x, i) && (i + 1 >= n || issue_s(x, i + 1));
+          alive = issue_pv(ta, i) && (i + 1 >= n || issue_s(ta, i + 1));
+          if (alive && tiles == 2) alive = issue_pv(tb, i) && (i + 1 >= n || issue_s(tb, i + 1));
         }
-      slab += n;
-      ++pieces[0];
-      pieces[1] += tiles - 1;
+        ++pieces[0];
+        pieces[1] += tiles - 1;
+      }
     }
-  } else if (warp >= 4 && warp < 8) {
-    // ------------------------------------------------------------------ producers
-    const int w = warp - 4;
-    int slab = 0;
+  } else if (warp < 12) {
+    set_regs<kRegsLaunch, kRegsLoad>();
+    // ------------------------------------------------------------------ keys and tile b's A (warps 4-7), values and tile a's A
+    const bool keys = warp < 8;
+    const int w = warp & 3, mine = keys ? 1 : 0;   // this warpgroup's tile
+    uint64_t* const full = keys ? ms.k_full : ms.v_full;
+    uint64_t* const empty = keys ? ms.k_empty : ms.v_empty;
+    uint8_t* const ring = smem + (keys ? C::kOffK : C::kOffV);
+    int slab = 0, st = 0, ph = 0, piece = 0, formed = 0;   // slabs and pieces so far, the ring's next stage, A's formed
     bool alive = true;
     while (alive && next_piece(p, walk, s)) {
-      const Columns col = columns_of(a, walk.l, s.pair);
-      const int n = least(s.s1, (col.hi - col.lo + 128) / 128) - s.s0;
+      Columns col = columns_of(a, walk.l, s.pair);
+      const int n = uniform(slabs_of(col));
+      if (n <= 0) continue;
+      col.lo = uniform(col.lo), col.hi = uniform(col.hi);
+      s.b = uniform(s.b), s.head = uniform(s.head), s.s0 = uniform(s.s0);
+      const size_t part_rows = (size_t)ca.c.N << ca.page_log2, head_rows = (size_t)s.head << ca.page_log2;
+      constexpr int kRowBytes = TileLoader<D, CODE>::kChunks * 16;
+      const size_t load_rows = (keys ? kPartK1 : kPartV1) * part_rows + head_rows, v_rows = kPartV1 * part_rows + head_rows;
+      auto form = [&]() {
+        if (!__all_sync(0xffffffffu, mbar_wait(&ms.a_free[mine], (formed & 1) ^ 1, abort_flag))) return false;
+        form_rows<T16, D, CODE>(a, walk.l, s, mine, w, lane, sA + mine * C::kTile, sQ + (mine * 4 + w) * D, sRows + (piece & 1) * 256 + mine * 128);
+        fence_async_smem();
+        mbar_arrive(&ms.a_ready[mine]);
+        ++formed;
+        return true;
+      };
+      const bool forms = mine < tiles_of();
+      if (!keys && forms) alive = form();
       int v_exp = 0;   // the largest exponent byte of V1's rows in this piece so far
       int token = col.lo + s.s0 * 128 + w * 32 + lane;
       auto page_of = [&](int t) { return t <= col.hi ? place_of(ca, s.b, t).page : -1; };
-      int page = n > 0 ? page_of(token) : -1;
+      int page = page_of(token);
       for (int i = 0; i < n && alive; ++i, token += 128) {
-        const int pos = slab + i, st = pos % NS, mt = pos % kMetas;
-        const int token0 = token - lane;
+        const int pos = slab + i, mt = pos % kMetas, token0 = token - lane;
         const bool any = token0 <= col.hi;   // (32 columns that no row looks at are not loaded)
         TileLoader<D, CODE> tile;
         int ek = 0, ev = 0;
+        const size_t row = (size_t)page * (4 * part_rows) + (token & (ca.c.page_size - 1));   // (but for the part and head)
         if (page >= 0) {
-          const Place at{page, token & (ca.c.page_size - 1)};
-          ek = __ldg(ca.c.exponents + row_of(ca, at, kPartK1, s.head));
-          ev = __ldg(ca.c.exponents + row_of(ca, at, kPartV1, s.head));
+          if (keys) ek = __ldg(ca.c.exponents + row + load_rows);
+          ev = __ldg(ca.c.exponents + row + v_rows);
         }
-        if (any) tile.load(ca, kPartK1, s.head, token0, page, lane);
+        if (any) tile.load(page >= 0 ? (const uint8_t*)ca.c.codes + (row + load_rows) * kRowBytes : nullptr, lane);
         const int next = i + 1 < n ? page_of(token + 128) : -1;
-        const uint32_t there = __ballot_sync(0xffffffffu, page >= 0), nan = __ballot_sync(0xffffffffu, page >= 0 && (ek == 255 || ev == 255));
-        if (ek == 255) ek = 0;   // (its codes are zeros)
-        if (ev == 255) ev = 0;
-        const int ek_most = __reduce_max_sync(0xffffffffu, ek), ev_most = __reduce_max_sync(0xffffffffu, ev);
-        if (!__all_sync(0xffffffffu, mbar_wait(&ms.k_empty[st], ((pos / NS) & 1) ^ 1, abort_flag))) {
-          alive = false;
-          break;
+        int up;   // the row's power of two
+        if (keys) {
+          const uint32_t there = __ballot_sync(0xffffffffu, page >= 0), nan = __ballot_sync(0xffffffffu, page >= 0 && (ek == 255 || ev == 255));
+          if (ek == 255) ek = 0;   // (its codes are zeros)
+          if (ev == 255) ev = 0;
+          const int ek_most = __reduce_max_sync(0xffffffffu, ek), ev_most = __reduce_max_sync(0xffffffffu, ev);
+          alive = __all_sync(0xffffffffu, mbar_wait(&empty[st], ph ^ 1, abort_flag));
+          if (!alive) break;
+          if (lane == 0) {
+            Meta& m = ms.meta[mt];
+            m.there[w] = there;
+            m.nan[w] = nan;
+            m.scale[w] = ek_most > kUp<CODE> ? __uint_as_float((uint32_t)(ek_most - kUp<CODE>) << 23) : 0.f;
+            m.v_exp[w] = ev_most;
+            mbar_arrive(&ms.meta_full[mt]);
+          }
+          up = kUp<CODE> + ek - ek_most;
+        } else {
+          if (ev == 255) ev = 0;
+          alive = __all_sync(0xffffffffu, mbar_wait(&ms.meta_full[mt], (pos / kMetas) & 1, abort_flag)) &&
+                  __all_sync(0xffffffffu, mbar_wait(&empty[st], ph ^ 1, abort_flag));
+          if (!alive) break;
+          const volatile Meta& m = ms.meta[mt];
+          v_exp = max(max(max(v_exp, m.v_exp[0]), m.v_exp[1]), max(m.v_exp[2], m.v_exp[3]));
+          up = kUp<CODE> + ev - v_exp;
         }
-        if (lane == 0) {
-          Meta& m = ms.meta[mt];
-          m.there[w] = there;
-          m.nan[w] = nan;
-          m.scale[w] = ek_most > kUp<CODE> ? __uint_as_float((uint32_t)(ek_most - kUp<CODE>) << 23) : 0.f;
-          m.v_exp[w] = ev_most;
-          mbar_arrive(&ms.meta_full[mt]);
-        }
-        if (any) tile.store(smem + C::kOffK + st * C::kTile, w * 32, half_power(kUp<CODE> + ek - ek_most), lane);
+        if (any) tile.store(ring + st * C::kTile, w * 32, half_power(up), lane);
         fence_async_smem();
-        mbar_arrive(&ms.k_full[st]);
-        if (any) tile.load(ca, kPartV1, s.head, token0, page, lane);
-        if (!__all_sync(0xffffffffu, mbar_wait(&ms.meta_full[mt], (pos / kMetas) & 1, abort_flag)) ||
-            !__all_sync(0xffffffffu, mbar_wait(&ms.v_empty[st], ((pos / NS) & 1) ^ 1, abort_flag))) {
-          alive = false;
-          break;
-        }
-        const volatile Meta& m = ms.meta[mt];
-        v_exp = max(max(max(v_exp, m.v_exp[0]), m.v_exp[1]), max(m.v_exp[2], m.v_exp[3]));
-        if (any) tile.store(smem + C::kOffV + st * C::kTile, w * 32, half_power(kUp<CODE> + ev - v_exp), lane);
-        fence_async_smem();
-        mbar_arrive(&ms.v_full[st]);
+        mbar_arrive(&full[st]);
+        if (++st == NS) st = 0, ph ^= 1;
         page = next;
+        if (keys && i == 0 && forms) alive = form();   // (the first keys are on their way before)
       }
-      if (n > 0) slab += n;
+      slab += n;
+      ++piece;
     }
-  } else if (warp >= 8) {
+  } else {
+    set_regs<kRegsLaunch, kRegsSoftmax>();
     // ------------------------------------------------------------------ soft-max, one row a thread
-    const int x = (warp - 8) >> 2, wq = warp & 3;
+    const int x = (warp - 12) >> 2, wq = warp & 3;
     const uint32_t lane_base = (uint32_t)(wq * 32) << 16;
     const uint32_t tS = tmem + lane_base + x * 128, tO = tmem + lane_base + C::kTmemO + x * D;
-    float* sq = reinterpret_cast<float*>(smem + C::kOffQ) + (warp - 8) * D;
-    int slab = 0, scount = 0, piece = 0;   // slabs so far, this tile's, its pieces
+    int slab = 0, scount = 0, piece = 0, mine = 0;   // slabs and pieces so far; this tile's
     bool alive = true;
     while (alive && next_piece(p, walk, s)) {
-      const Line l = walk.l;
-      const Columns col = columns_of(a, l, s.pair);
-      const int n = least(s.s1, (col.hi - col.lo + 128) / 128) - s.s0;
-      const int groups = l.cnt * l.groups, g = s.pair * 8 + x * 4 + wq;
+      const Columns col = columns_of(a, walk.l, s.pair);
+      const int n = uniform(slabs_of(col)), ctx = uniform(walk.l.ctx);
+      const bool used = s.pair * 8 + x * 4 + wq < walk.l.cnt * walk.l.groups;   // (the warp's rows are of a new token)
       float* out = p.part + (size_t)(s.id * 8 + x * 4 + wq) * (D + 2);
       if (n <= 0) {
-        if (lane == 0 && g < groups) out[0] = -INFINITY, out[1] = 0.f;
+        if (lane == 0 && used) out[0] = -INFINITY, out[1] = 0.f;
         continue;
       }
-      if (s.pair * 8 + x * 4 >= groups) {   // (no second tile)
+      if (x >= tiles_of()) {   // (no second tile)
         slab += n;
+        ++piece;
         continue;
       }
-      // --- this thread's row: token k of new token i
-      const int i = g < groups ? g / l.groups : 0;
-      const unsigned long long word = ca.c.ancestors ? seen_word(ca, s.b, i) : 0;
-      const int pos_q = l.ctx + (ca.c.ancestors ? __popcll(word) - 1 : i);
-      const int pk = most(0, pos_q - a.k2w) + (g % l.groups) * 32 + lane;
-      bool on = g < groups && pk <= pos_q;
-      int token = pk;
-      if (ca.c.ancestors && pk >= l.ctx) {
-        unsigned long long left = word;
-        for (int c = l.ctx; c < pk && left; ++c) left &= left - 1;
-        token = l.ctx + (left ? __ffsll(left) - 1 : 0);
-      }
-      int byte = 0, byte2 = 0;
-      Place at{-1, 0};
-      if (on) {
-        at = place_of(ca, s.b, token);
-        if (at.page < 0) {
-          on = false;
-          if (ca.status) atomicOr(ca.status, kStatusPlace);
-        }
-      }
-      if (on) {
-        byte = __ldg(ca.c.exponents + row_of(ca, at, kPartK2, s.head));
-        byte2 = __ldg(ca.c.exponents + row_of(ca, at, kPartV2, s.head));
-      }
-      // columns that the row attends to: numbers c_lo .. c_hi, and of a tree's tokens a word
-      const int c_lo = on ? most(most(0, pos_q - a.k1w), pk - least(pk, a.kkl)) : kUnlimited;
-      const int last = pk < kUnlimited - a.kkr ? least(pos_q, pk + a.kkr) : pos_q;
-      const int c_hi = !on ? -1 : ca.c.ancestors ? least(l.ctx - 1, last) : last;
-      unsigned long long tree = 0;
-      if (on && ca.c.ancestors) {
-        unsigned long long left = word;
-        for (int c = l.ctx; left; ++c, left &= left - 1)
-          if (c >= c_lo && c <= last) tree |= left & (~left + 1);
-      }
-      // --- A = 2^-kDown q * code, q brought to [1, 2); the powers of two and alpha go to the scores' scale
-      float row_scale;
-      {
-        const T16* q = (const T16*)a.q.p + rows_at(a.q, s.b, s.head, i);
-        constexpr int E = D / 32;
-        float f[E];
-        uint32_t big = 0;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          f[e] = to_f(q[lane * E + e]);
-          big = max(big, __float_as_uint(f[e]) & 0x7fffffffu);
-        }
-        big = __reduce_max_sync(0xffffffffu, big);
-        const int power = max(min(254 - (int)(big >> 23), 253), 1);   // (the largest numbers are brought to [2, 4))
-        const float up = __uint_as_float((uint32_t)power << 23);
-        const float sign = a.scale2 < 0.f ? -1.f : 1.f;
-        __syncwarp();
-#pragma unroll
-        for (int e = 0; e < E; ++e) sq[lane * E + e] = f[e] * up * sign;
-        __syncwarp();
-        row_scale = fabsf(a.scale2) * (on && byte != 255 ? __uint_as_float((uint32_t)byte << 23) : 0.f) * (float)(1 << kDown<CODE>);
-        row_scale *= __uint_as_float((uint32_t)(254 - power) << 23);
-      }
-      {
-        uint8_t* tile = smem + C::kOffA + x * C::kTile;
-        const uint8_t* codes = (const uint8_t*)ca.c.codes + (on ? row_of(ca, at, kPartK2, s.head) : 0) * (size_t)(D * (CODE == TRITT_CODE_F16 ? 2 : 1));
-#pragma unroll 4
-        for (int ch = 0; ch < D / 8; ++ch) {
-          uint32_t h[4] = {0u, 0u, 0u, 0u};
-          if (on) {
-            Codes8<CODE> c8;
-            c8.load(codes, ch * 8);
-            c8.halves(h);
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 c = __half22float2(*reinterpret_cast<const __half2*>(&h[e]));
-            const float2 q = *reinterpret_cast<const float2*>(sq + ch * 8 + 2 * e);
-            constexpr float down = 1.f / (1 << kDown<CODE>);
-            h[e] = pack2<__half>(q.x * (c.x * down), q.y * (c.y * down));
-          }
-          *reinterpret_cast<uint4*>(tile + (ch >> 3) * 16384 + swz128(wq * 32 + lane, ch & 7)) = make_uint4(h[0], h[1], h[2], h[3]);
-        }
-      }
-      fence_async_smem();
-      mbar_arrive(&ms.a_ready[x]);
-      // --- slabs
+      const int first = uniform(col.lo + s.s0 * 128), behind = uniform(col.hi + 1);
+      alive = __all_sync(0xffffffffu, mbar_wait(&ms.a_ready[x], mine & 1, abort_flag));
+      if (!alive) break;
+      const RowInfo r = sRows[(piece & 1) * 256 + x * 128 + wq * 32 + lane];
+      // --- slabs: a half of 64 columns at a time is read once, its maximum taken, and the row's reference raised where that is 2^8 above it
       float m_used = -INFINITY, l_sum = 0.f;
       int v_exp = 0;
       for (int t = 0; t < n; ++t, ++scount) {
-        const int pos = slab + t, c0 = col.lo + (s.s0 + t) * 128, wid = least(128, col.hi + 1 - c0);
-        const volatile Meta& m = ms.meta[pos % kMetas];
-        if (!__all_sync(0xffffffffu, mbar_wait(&ms.meta_full[pos % kMetas], (pos / kMetas) & 1, abort_flag)) ||
-            !__all_sync(0xffffffffu, mbar_wait(&ms.s_ready[x], scount & 1, abort_flag))) {
+        const int pos = slab + t, c0 = first + t * 128, wid = behind - c0;
+        const Meta& m = ms.meta[pos % kMetas];
+        if (!__all_sync(0xffffffffu, mbar_wait(&ms.meta_full[pos % kMetas], (pos / kMetas) & 1, abort_flag))) {
           alive = false;
           break;
         }
-        tc_fence_after();
-        float f[4];
-        bool clean = wid == 128;
-        int v_now = v_exp;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          f[c] = row_scale * m.scale[c];
-          clean = clean && m.there[c] == 0xffffffffu && m.nan[c] == 0u;
-          v_now = max(v_now, m.v_exp[c]);
-        }
-        const bool full = __all_sync(0xffffffffu, clean && c_lo <= c0 && c_hi >= c0 + 127);
-        // columns that count, and those of them that read as NaN
-        uint32_t mask[4], bad[4];
-        float mx = -INFINITY;
-        if (full) {
-#pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            uint32_t sr[64];
-            tmem_ld64(tS + hf * 64, sr);
-            tmem_wait_ld();
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              float m0 = -INFINITY, m1 = -INFINITY;
-#pragma unroll
-              for (int c = 0; c < 32; c += 2) {
-                m0 = fmaxf(m0, __uint_as_float(sr[q * 32 + c]));
-                m1 = fmaxf(m1, __uint_as_float(sr[q * 32 + c + 1]));
-              }
-              mx = fmaxf(mx, fmaxf(m0, m1) * f[hf * 2 + q]);
-            }
-          }
-        } else {
+        const uint4 there = *reinterpret_cast<const uint4*>(m.there), nan = *reinterpret_cast<const uint4*>(m.nan);
+        const float4 ks = *reinterpret_cast<const float4*>(m.scale);
+        const int4 ve = *reinterpret_cast<const int4*>(m.v_exp);
+        const bool clean = wid >= 128 && (there.x & there.y & there.z & there.w) == 0xffffffffu && (nan.x | nan.y | nan.z | nan.w) == 0u;
+        const bool full = __all_sync(0xffffffffu, clean && r.c_lo <= c0 && r.c_hi >= c0 + 127);
+        uint32_t mask[4] = {0u, 0u, 0u, 0u};   // columns that count
+        bool bad = false;                      // one of them reads as NaN
+        int some = 3;                          // halves with one, of any row of the warp
+        if (!full) {
+          const uint32_t th[4] = {there.x, there.y, there.z, there.w}, na[4] = {nan.x, nan.y, nan.z, nan.w};
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             const int c1 = c0 + c * 32;
-            const int lo = most(c_lo - c1, 0), hi = least(c_hi - c1, 31);
+            const int lo = most(r.c_lo - c1, 0), hi = least(r.c_hi - c1, 31);
             uint32_t b = lo > 31 || hi < lo ? 0u : (0xffffffffu << lo) & (0xffffffffu >> (31 - hi));
-            const int off = l.ctx - c1;   // of the first new token
-            if (tree && off < 32 && off > -64) b |= (uint32_t)(off >= 0 ? tree << off : tree >> -off);
-            mask[c] = b & m.there[c];
+            const int off = ctx - c1;   // of the first new token
+            if (r.tree && off < 32 && off > -64) b |= (uint32_t)(off >= 0 ? r.tree << off : r.tree >> -off);
+            mask[c] = b & th[c];
             if (mask[c] != b && ca.status) atomicOr(ca.status, kStatusPlace);
-            bad[c] = mask[c] & m.nan[c];
-            if (c * 32 < wid) {
-              uint32_t sr[32];
-              tmem_ld32(tS + c * 32, sr);
-              tmem_wait_ld();
-              float m0 = -INFINITY;
-#pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (mask[c] >> e & 1) m0 = fmaxf(m0, __uint_as_float(sr[e]));
-              if (m0 != -INFINITY) mx = fmaxf(mx, m0 * f[c]);
-            }
+            bad = bad || (mask[c] & na[c]);
           }
+          some = (__any_sync(0xffffffffu, mask[0] | mask[1]) ? 1 : 0) | (__any_sync(0xffffffffu, mask[2] | mask[3]) ? 2 : 0);
         }
-        if (t == 0) {
-          m_used = mx;
-        } else {
-          const bool grow = mx > m_used + kGap;
-          if (__any_sync(0xffffffffu, grow) || v_now != v_exp) {
-            // (s_ready of this slab was committed behind the previous slab's P V)
-            float corr = grow ? exp2f(m_used - mx) : 1.f;
-            if (grow) {
-              m_used = mx;
-              l_sum *= corr;
-            }
-            corr *= v_now - v_exp < 126 ? __uint_as_float((uint32_t)(127 - (v_now - v_exp)) << 23) : 0.f;
+        // (a scale of 0, of rows of zeros: any small one, so that masked columns' -infinity stays one)
+        const float f[4] = {fmaxf(r.scale * ks.x, 1e-37f), fmaxf(r.scale * ks.y, 1e-37f), fmaxf(r.scale * ks.z, 1e-37f), fmaxf(r.scale * ks.w, 1e-37f)};
+        const int v_now = max(max(max(v_exp, ve.x), ve.y), max(ve.z, ve.w));
+        alive = __all_sync(0xffffffffu, mbar_wait(&ms.s_ready[x], scount & 1, abort_flag));
+        if (!alive) break;
+        tc_fence_after();
+        // the accumulator times `corr` (s_ready of this slab was committed behind the previous slab's P V)
+        auto correct = [&](float corr) {
+#pragma unroll 1
+          for (int ch = 0; ch < D / 16; ++ch) {
+            uint32_t o[16];
+            tmem_ld16(tO + ch * 16, o);
+            tmem_wait_ld();
 #pragma unroll
-            for (int ch = 0; ch < D / 32; ++ch) {
-              uint32_t o[32];
-              tmem_ld32(tO + ch * 32, o);
-              tmem_wait_ld();
-#pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
-              tmem_st32(tO + ch * 32, o);
-            }
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+            tmem_st16(tO + ch * 16, o);
           }
-        }
+        };
+        if (t > 0 && v_now != v_exp) correct(v_now - v_exp < 126 ? __uint_as_float((uint32_t)(127 - (v_now - v_exp)) << 23) : 0.f);
         v_exp = v_now;
-        const float shift = kLift - m_used;
         float psum = 0.f;
-        if (full) {
 #pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            uint32_t sr[64], pk2[32];
+        for (int hf = 0; hf < 2; ++hf) {
+          uint32_t pk2[32];
+          if (some >> hf & 1) {
+            uint32_t sr[64];
             tmem_ld64(tS + hf * 64, sr);
             tmem_wait_ld();
+            if (!full) {
+#pragma unroll
+              for (int e = 0; e < 64; ++e) sr[e] = mask[hf * 2 + e / 32] >> (e % 32) & 1 ? sr[e] : 0xff800000u;
+            }
+            float mx;
+            {
+              float q[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                q[k] = fmaxf(__uint_as_float(sr[k * 16]), __uint_as_float(sr[k * 16 + 1]));
+#pragma unroll
+                for (int e = 2; e < 16; e += 2) q[k] = fmaxf(q[k], fmaxf(__uint_as_float(sr[k * 16 + e]), __uint_as_float(sr[k * 16 + e + 1])));
+              }
+              mx = fmaxf(fmaxf(q[0], q[1]) * f[hf * 2], fmaxf(q[2], q[3]) * f[hf * 2 + 1]);
+            }
+            const bool grow = mx > m_used + kGap;
+            if (__any_sync(0xffffffffu, grow)) {
+              const float corr = grow ? exp2f(m_used - mx) : 1.f;
+              if (grow) {
+                m_used = mx;
+                l_sum *= corr;
+                psum *= corr;
+              }
+              if (t > 0) correct(corr);
+              if (hf == 1) {   // (this slab's first half, formed already)
+#pragma unroll 1
+                for (int q = 0; q < 2; ++q) {
+                  uint32_t o[16];
+                  tmem_wait_st();
+                  tmem_ld16(tS + q * 16, o);
+                  tmem_wait_ld();
+#pragma unroll
+                  for (int e = 0; e < 16; ++e) {
+                    const float2 v = unpack2<__half>(o[e]);
+                    o[e] = pack2<__half>(v.x * corr, v.y * corr);
+                  }
+                  tmem_st16(tS + q * 16, o);
+                }
+              }
+            }
+            const float shift = kLift - (m_used == -INFINITY ? 0.f : m_used);
             float p0 = 0.f, p1 = 0.f;
 #pragma unroll
             for (int c = 0; c < 64; c += 2) {
@@ -610,35 +747,31 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
               pk2[c >> 1] = pack2<__half>(e0, e1);
             }
             psum += p0 + p1;
-            tmem_st32(tS + hf * 32, pk2);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) pk2[e] = 0u;
           }
-        } else {
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-            if (c * 32 < wid) {
-              uint32_t sr[32], pk2[16];
-              tmem_ld32(tS + c * 32, sr);
-              tmem_wait_ld();
-#pragma unroll
-              for (int e = 0; e < 32; e += 2) {
-                const float e0 = mask[c] >> e & 1 ? exp2f(fmaf(__uint_as_float(sr[e]), f[c], shift)) : 0.f;
-                const float e1 = mask[c] >> (e + 1) & 1 ? exp2f(fmaf(__uint_as_float(sr[e + 1]), f[c], shift)) : 0.f;
-                psum += e0 + e1;
-                pk2[e >> 1] = pack2<__half>(e0, e1);
-              }
-              if (bad[c]) psum = __uint_as_float(0x7fffffffu);
-              tmem_st16(tS + c * 16, pk2);
-            }
+          if (hf * 64 < wid) tmem_st32(tS + hf * 32, pk2);
         }
-        l_sum += psum;
+        l_sum += bad ? __uint_as_float(0x7fffffffu) : psum;
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(&ms.p_ready[x]);
       }
       if (!alive) break;
       slab += n;
-      // --- the group's sum: sum over its rows of 2^(m_row - m) acc V2, and of the sums
-      if (on && (byte == 255 || byte2 == 255) && l_sum > 0.f) l_sum = __uint_as_float(0x7fffffffu);
+      ++piece;
+      // --- the group's sum: sum over its rows of 2^(m_row - m) acc V2, and of the sums.  V2's codes come while the last products run
+      const uint8_t* codes = (const uint8_t*)ca.c.codes + r.v2_row * (size_t)(D * (CODE == TRITT_CODE_F16 ? 2 : 1));
+      // (a row that is not there has number 0 and weight 0)
+      constexpr int kWords = CODE == TRITT_CODE_F16 ? 4 : 2;   // 16-byte words of 32 columns' codes
+      uint4 now[kWords], next[kWords];
+      auto load_codes = [&](uint4 (&v)[kWords], int ch) {
+#pragma unroll
+        for (int k = 0; k < kWords; ++k) v[k] = __ldg(reinterpret_cast<const uint4*>(codes) + ch * kWords + k);
+      };
+      load_codes(now, 0);
+      if ((r.flags & kRowNan) && l_sum > 0.f) l_sum = __uint_as_float(0x7fffffffu);
       float m_all = m_used;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) m_all = fmaxf(m_all, __shfl_xor_sync(0xffffffffu, m_all, o));
@@ -647,35 +780,43 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) l_all += __shfl_xor_sync(0xffffffffu, l_all, o);
       // V1's and V2's powers of two (fp32's range is that of the result's own type and more)
-      const float vscale = weight == 0.f || byte2 == 255 ? 0.f : weight * exp2f((float)(v_exp - 127 - kUp<CODE>)) * exp2f((float)(byte2 - 127));
-      if (!__all_sync(0xffffffffu, mbar_wait(&ms.o_done[x], piece & 1, abort_flag))) {
+      const int byte2 = r.flags & 255;
+      const float vscale =
+          weight == 0.f || byte2 == 255 ? 0.f : weight * exp2f((float)(v_exp - 127 - kUp<CODE>)) * exp2f((float)(byte2 - 127));
+      if (!__all_sync(0xffffffffu, mbar_wait(&ms.o_done[x], mine & 1, abort_flag))) {
         alive = false;
         break;
       }
-      ++piece;
+      ++mine;
       tc_fence_after();
-      const uint8_t* codes = (const uint8_t*)ca.c.codes + (on ? row_of(ca, at, kPartV2, s.head) : 0) * (size_t)(D * (CODE == TRITT_CODE_F16 ? 2 : 1));
 #pragma unroll 1
       for (int ch = 0; ch < D / 32; ++ch) {
         uint32_t o[32];
-        float v[32];
         tmem_ld32(tO + ch * 32, o);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float c[8];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) c[k] = 0.f;
-          if (on) {
-            Codes8<CODE> c8;
-            c8.load(codes, ch * 32 + e * 8);
-            code_values<CODE>(c8, vscale, c);
-          }
-#pragma unroll
-          for (int k = 0; k < 8; ++k) v[e * 8 + k] = c[k];
-        }
+        if (ch + 1 < D / 32) load_codes(next, ch + 1);
         tmem_wait_ld(o);
+        float v[32];
+        auto times_codes = [&](uint32_t h, int at) {
+          const float2 c = unpack2<__half>(h);
+          v[at] = weight == 0.f ? 0.f : c.x * vscale * __uint_as_float(o[at]);
+          v[at + 1] = weight == 0.f ? 0.f : c.y * vscale * __uint_as_float(o[at + 1]);
+        };
 #pragma unroll
-        for (int e = 0; e < 32; ++e) v[e] = weight == 0.f ? 0.f : v[e] * __uint_as_float(o[e]);
+        for (int k = 0; k < kWords; ++k) {
+          const uint32_t w[4] = {now[k].x, now[k].y, now[k].z, now[k].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if constexpr (CODE == TRITT_CODE_F16) {
+              times_codes(w[e], k * 8 + e * 2);
+            } else {
+              uint32_t h0, h1;
+              bytes_to_halves<CODE>(w[e], h0, h1);
+              times_codes(h0, k * 16 + e * 4);
+              times_codes(h1, k * 16 + e * 4 + 2);
+            }
+          }
+          now[k] = next[k];
+        }
         // column sums over the warp: halves change hands until each lane has one column
 #pragma unroll
         for (int h = 16; h > 0; h >>= 1) {
@@ -686,9 +827,9 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
             v[e] = keep + __shfl_xor_sync(0xffffffffu, give, h);
           }
         }
-        if (g < groups) out[2 + ch * 32 + lane] = v[0];
+        if (used) out[2 + ch * 32 + lane] = v[0];
       }
-      if (g < groups && lane == 0) out[0] = m_all, out[1] = l_all;
+      if (used && lane == 0) out[0] = m_all, out[1] = l_all;
       tc_fence_before();
     }
   }
@@ -709,61 +850,115 @@ struct TdpJoinParams {
   int ctas;
 };
 
-// One block a row: its eight warps take the row's groups in turn, each all pieces of its group; then the warps' results are added up in order.
+// The next CTA behind c that has a step.
+__device__ __forceinline__ long long next_owner(long long c, long long total, int ctas) {
+  const long long x = (c + 1) * total / ctas;   // its first step
+  return ((x + 1) * ctas - 1) / total;
+}
+
+// One block a row.  A thread finds a group's pieces, whose maxima give the row's, 256 groups at a time; then the warps add up the groups'
+// results, whose weights no load waits for, and the warps' are added in order.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) tdp_join_kernel(const __grid_constant__ TdpJoinParams j) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  __shared__ float sm[8], sl[8], so[8][D];
+  __shared__ float s_top[8], s_sum[8], so[8][D];
+  __shared__ long long s_id[256];
+  __shared__ int s_pieces[256];
   const CacheArgs& ca = j.a.cache;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const long long row = blockIdx.x;
   const int i = (int)(row % ca.c.n), head = (int)(row / ca.c.n % ca.c.N), b = (int)(row / ca.c.n / ca.c.N);
-  const LineEntry e = j.table[b];
-  const LineEntry end = j.table[ca.c.B - 1];
+  const LineEntry e = j.table[b], end = j.table[ca.c.B - 1];
   const long long total = end.base + (long long)end.line.pairs * end.line.slabs * ca.c.N;
   constexpr int E = D / 32;
-  float m = -INFINITY, l = 0.f, acc[E];
+  float top = -INFINITY, sum = 0.f, acc[E];   // of this warp's groups
 #pragma unroll
   for (int k = 0; k < E; ++k) acc[k] = 0.f;
-  if (i < e.line.cnt)
-    for (int g = i * e.line.groups + warp; g < (i + 1) * e.line.groups; g += 8) {
-      const long long pair = (long long)head * e.line.pairs + g / 8, first = e.base + pair * e.line.slabs;
-      // CTA c has the steps from c total / ctas to the next one's
-      for (long long x = first; x < first + e.line.slabs;) {
-        const long long c = ((x + 1) * j.ctas - 1) / total;
-        x = (c + 1) * total / j.ctas;
-        const float* p = j.part + (size_t)((e.pair_base + pair + c) * 8 + g % 8) * (D + 2);
-        const float mp = p[0], lp = p[1];
-        if (mp == -INFINITY && lp == 0.f) continue;
-        const float mn = fmaxf(m, mp), w0 = m == -INFINITY ? 0.f : exp2f(m - mn), w1 = mp == -INFINITY ? 1.f : exp2f(mp - mn);
-        l = l * w0 + lp * w1;
+  const int groups = i < e.line.cnt ? e.line.groups : 0;
+  for (int g0 = 0; g0 < groups; g0 += 256) {
+    float m = -INFINITY;
+    __syncthreads();
+    if (g0 + tid < groups) {
+      const int g = i * e.line.groups + g0 + tid;
+      const long long pair = (long long)head * e.line.pairs + g / 8, first = e.base + pair * e.line.slabs, last = first + e.line.slabs - 1;
+      // CTA c has the steps from c total / ctas to the next one's; a piece of each that has any
+      const long long id = (e.pair_base + pair) * 8 + g % 8;
+      long long c;
+      int pieces = 0;
+      for (long long x = first; x <= last;) {
+        // (a division of 64 bits takes as long as the loads)
+        c = total < 1 << 20 ? ((uint32_t)(x + 1) * (uint32_t)j.ctas - 1) / (uint32_t)total : ((x + 1) * j.ctas - 1) / total;
+        x = total < 1 << 20 ? (uint32_t)(c + 1) * (uint32_t)total / (uint32_t)j.ctas : (c + 1) * total / j.ctas;
+        m = fmaxf(m, j.part[(size_t)(id + c * 8) * (D + 2)]);
+        if (pieces++ == 0) s_id[tid] = c;
+      }
+      // (with fewer steps than CTAs pieces are those of single steps: not every CTA has one)
+      s_pieces[tid] = pieces;
+    }
 #pragma unroll
-        for (int k = 0; k < E; ++k) acc[k] = acc[k] * w0 + p[2 + k * 32 + lane] * w1;
-        m = mn;
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (lane == 0) s_top[warp] = m;
+    __syncthreads();
+    float now = top;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) now = fmaxf(now, s_top[w]);
+    const float w0 = top == -INFINITY ? 0.f : exp2f(top - now);
+    sum *= top == -INFINITY && sum != sum ? 1.f : w0;
+#pragma unroll
+    for (int k = 0; k < E; ++k) acc[k] *= w0;
+    top = now;
+    const int here = groups - g0 < 256 ? groups - g0 : 256;
+#pragma unroll 4
+    for (int t = warp; t < here; t += 8) {
+      const int g = i * e.line.groups + g0 + t;
+      const long long pair = (long long)head * e.line.pairs + g / 8, id = (e.pair_base + pair) * 8 + g % 8;
+      long long c = s_id[t];
+      for (int k = s_pieces[t]; k > 0; --k) {
+        const float* p = j.part + (size_t)(id + c * 8) * (D + 2);
+        const float mp = p[0], lp = p[1];
+        float v[E];
+#pragma unroll
+        for (int q = 0; q < E; ++q) v[q] = p[2 + q * 32 + lane];
+        // (a group that has seen nothing has written no result; a maximum of -infinity with a sum of NaN is a row that reads as NaN)
+        const float w = mp == -INFINITY ? 0.f : exp2f(mp - top);
+        sum += mp == -INFINITY ? (lp != lp ? lp : 0.f) : lp * w;
+#pragma unroll
+        for (int q = 0; q < E; ++q) acc[q] += w == 0.f ? 0.f : v[q] * w;
+        if (k > 1) c = next_owner(c, total, j.ctas);
       }
     }
-  if (lane == 0) sm[warp] = m, sl[warp] = l;
+  }
+  if (lane == 0) s_sum[warp] = sum;
 #pragma unroll
   for (int k = 0; k < E; ++k) so[warp][k * 32 + lane] = acc[k];
   __syncthreads();
-  float top = -INFINITY, sum = 0.f;
+  float all = 0.f;
 #pragma unroll
-  for (int w = 0; w < 8; ++w) top = fmaxf(top, sm[w]);
-#pragma unroll
-  for (int w = 0; w < 8; ++w) sum += sm[w] == -INFINITY ? (sl[w] != sl[w] ? sl[w] : 0.f) : sl[w] * exp2f(sm[w] - top);
-  const bool none = top == -INFINITY && sum == 0.f;
-  for (int c = threadIdx.x; c < D; c += 256) {
+  for (int w = 0; w < 8; ++w) all += s_sum[w];
+  const bool none = top == -INFINITY && all == 0.f;
+  for (int c = tid; c < D; c += 256) {
     float v = 0.f;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) v += sm[w] == -INFINITY ? 0.f : so[w][c] * exp2f(sm[w] - top);
-    ((T*)j.o)[(size_t)row * D + c] = from_f<T>(none ? 0.f : sum != sum ? sum : v * (1.f / sum));
+    for (int w = 0; w < 8; ++w) v += so[w][c];
+    ((T*)j.o)[(size_t)row * D + c] = from_f<T>(none ? 0.f : all != all ? all : v * (1.f / all));
   }
-  if (j.lse && threadIdx.x == 0) j.lse[row] = none ? -INFINITY : sum != sum ? sum : (top + log2f(sum)) * kLn2;
+  if (j.lse && tid == 0) j.lse[row] = none ? -INFINITY : all != all ? all : (top + log2f(all)) * kLn2;
 }
 
 template <typename T16, int D, int CODE>
 int launch(const Params& p, const TdpJoinParams& j, cudaStream_t stream) {
   auto kern = tdp_decode_kernel<T16, D, CODE>;
+  // (the registers' split is of what the kernel is launched with: setmaxnreg.inc waits without a limit for more)
+  static std::atomic<int> regs{0};
+  if (regs.load(std::memory_order_relaxed) == 0) {
+    cudaFuncAttributes attr;
+    TRITT_CUDA_OK(cudaFuncGetAttributes(&attr, kern));
+    regs.store(attr.numRegs, std::memory_order_relaxed);
+  }
+  if (regs.load(std::memory_order_relaxed) != kRegsLaunch) {
+    set_error("the kernel over the cache was built with %d registers per thread, its split needs %d", regs.load(), kRegsLaunch);
+    return -30;
+  }
   TRITT_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmem));
   kern<<<p.ctas, kThreads, Cfg<D>::kSmem, stream>>>(p);
   count_launch();
