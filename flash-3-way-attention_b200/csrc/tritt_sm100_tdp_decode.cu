@@ -14,6 +14,8 @@
 // two, whatever lies 2^-38 below is lost.  K1's exponent joins the scale of the scores, for each 32 columns; V1's runs along with the
 // accumulator, which is multiplied where it grows.  A is rounded once to 11 bits, P (times 2^7, fp16's lower range) once.
 //
+//   warp 1        walks the line and tells the others each piece (a pair of tiles, a range of slabs) by a ring in shared memory: what each
+//                 role kept of the walk before cost it registers that it had not, and spills go to L2 beside 213 KB of shared memory
 //   warp 0        issues tcgen05.mma: S_x = A_x K1^T, acc_x += P_x V1 for the tiles x = a, b in turn, P_x read from TMEM over S_x
 //   warps 4-7     keys: a warp loads 32 rows of a slab (pages, exponents, codes), converts and stores them with the 128-byte swizzle;
 //                 the loads of a tile are in flight before its stage is free.  They form tile b's A, and tell its rows' masks and scales
@@ -33,7 +35,7 @@ using namespace sm100;
 
 constexpr int kThreads = 640;
 constexpr int kRegsLaunch = 96;   // a thread; the soft-max warps take what the others give up
-constexpr int kRegsIssue = 32, kRegsLoad = 88, kRegsSoftmax = 136;
+constexpr int kRegsIssue = 32, kRegsLoad = 96, kRegsSoftmax = 128;
 static_assert(kRegsIssue + 2 * kRegsLoad + 2 * kRegsSoftmax <= 5 * kRegsLaunch, "more registers than the launch has");
 constexpr float kGap = 8.f;      // the accumulator is rescaled when a row's maximum grew by more than 2^8
 constexpr float kLift = 7.f;     // P is formed times 2^7: at most 2^15, normal down to 2^-21 of the reference
@@ -50,7 +52,7 @@ template <int D> struct Cfg {
   static constexpr int kOffQ = kOffV + kStages * kTile;            // [8 warps][D] fp16
   static constexpr int kOffRows = kOffQ + 8 * D * 2;               // two pieces' [256] RowInfo
   static constexpr int kOffMisc = kOffRows + 2 * 256 * 32;
-  static constexpr int kSmem = kOffMisc + 1024;
+  static constexpr int kSmem = kOffMisc + 1536;
   static constexpr int kTmemO = 256;                               // S_a | S_b | acc_a | acc_b
 };
 
@@ -72,16 +74,28 @@ struct __align__(16) RowInfo {
 static_assert(sizeof(RowInfo) == 32, "two 16-byte accesses");
 constexpr int kRowNan = 256;
 
+// A piece, as the roles see it.  n = 0: there is no more.
+struct __align__(16) Item {
+  int n, tiles, first, behind;       // slabs, tiles; columns first .. behind - 1, 128 a slab
+  int b, head, g0, groups;           // groups g0 .. of the sequence's line; groups of a new token
+  int all_groups, ctx, flags, pad;   // groups of all its new tokens
+  float* out;                        // [8][D + 2]: the groups' results
+  float* pad2;
+};
+constexpr int kItems = 4;
+constexpr int kConsumers = 17;       // warps that read them
+
 struct Misc {
   uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
-  uint64_t meta_full[kMetas], a_ready[2], a_free[2], s_ready[2], p_ready[2], o_done[2];
+  uint64_t meta_full[kMetas], a_ready[2], a_free[2], s_ready[2], p_ready[2], o_done[2], item_full[kItems], item_free[kItems];
   Meta meta[kMetas];
+  Item items[kItems];
   uint32_t tmem_base;
   int abort_flag;
   int first_b;
   long long first_base, total;
 };
-static_assert(sizeof(Misc) <= 1024, "shared memory of the barriers");
+static_assert(sizeof(Misc) <= 1536, "shared memory of the barriers");
 
 // What the line of steps has of one sequence.
 struct Line {
@@ -270,26 +284,25 @@ template <int D, int CODE> struct TileLoader {   // a warp's 32 rows of one part
 // A warp's 32 rows of a tile: token k of new token i each.  A = 2^-kDown q * code, q brought to [1, 2); the powers of two and alpha go to
 // the scores' scale.
 template <typename T16, int D, int CODE>
-__device__ __forceinline__ void form_rows(const TdpDecodeArgs& a, const Line& l, const Piece& s, int x, int wq, int lane, uint8_t* tile, __half* sq,
-                                          RowInfo* info) {
+__device__ __forceinline__ void form_rows(const TdpDecodeArgs& a, const Item& s, int x, int wq, int lane, uint8_t* tile, __half* sq, RowInfo* info) {
   const CacheArgs& ca = a.cache;
-  const int g = s.pair * 8 + x * 4 + wq;
-  const bool any = g < l.cnt * l.groups;
-  const int i = any ? g / l.groups : 0;
+  const int g = s.g0 + x * 4 + wq, ctx = s.ctx;
+  const bool any = g < s.all_groups;
+  const int i = any ? g / s.groups : 0;
   const T16* qp = (const T16*)a.q.p + rows_at(a.q, s.b, s.head, i);
   constexpr int E = D / 32;
   float f[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) f[e] = to_f(qp[lane * E + e]);
   const unsigned long long word = ca.c.ancestors ? seen_word(ca, s.b, i) : 0;
-  const int pos_q = l.ctx + (ca.c.ancestors ? __popcll(word) - 1 : i);
-  const int pk = most(0, pos_q - a.k2w) + (g - i * l.groups) * 32 + lane;
+  const int pos_q = ctx + (ca.c.ancestors ? __popcll(word) - 1 : i);
+  const int pk = most(0, pos_q - a.k2w) + (g - i * s.groups) * 32 + lane;
   bool on = any && pk <= pos_q;
   int token = pk;
-  if (ca.c.ancestors && pk >= l.ctx) {
+  if (ca.c.ancestors && pk >= ctx) {
     unsigned long long left = word;
-    for (int c = l.ctx; c < pk && left; ++c) left &= left - 1;
-    token = l.ctx + (left ? __ffsll(left) - 1 : 0);
+    for (int c = ctx; c < pk && left; ++c) left &= left - 1;
+    token = ctx + (left ? __ffsll(left) - 1 : 0);
   }
   RowInfo r{0, 0, 0.f, kUnlimited, -1, 0};
   const uint8_t* codes = (const uint8_t*)ca.c.codes;
@@ -309,10 +322,10 @@ __device__ __forceinline__ void form_rows(const TdpDecodeArgs& a, const Line& l,
       // columns that the row attends to: numbers c_lo .. c_hi, and of a tree's tokens a word
       const int last = pk < kUnlimited - a.kkr ? least(pos_q, pk + a.kkr) : pos_q;
       r.c_lo = most(most(0, pos_q - a.k1w), pk - least(pk, a.kkl));
-      r.c_hi = ca.c.ancestors ? least(l.ctx - 1, last) : last;
+      r.c_hi = ca.c.ancestors ? least(ctx - 1, last) : last;
       if (ca.c.ancestors) {
         unsigned long long left = word;
-        for (int c = l.ctx; left; ++c, left &= left - 1)
+        for (int c = ctx; left; ++c, left &= left - 1)
           if (c >= r.c_lo && c <= last) r.tree |= left & (~left + 1);
       }
     }
@@ -390,6 +403,10 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
       mbar_init(&ms.v_empty[i], 1);
     }
     for (int i = 0; i < kMetas; ++i) mbar_init(&ms.meta_full[i], 4);
+    for (int i = 0; i < kItems; ++i) {
+      mbar_init(&ms.item_full[i], 1);
+      mbar_init(&ms.item_free[i], kConsumers);
+    }
     for (int x = 0; x < 2; ++x) {
       mbar_init(&ms.a_ready[x], 128);
       mbar_init(&ms.a_free[x], 1);
@@ -428,19 +445,58 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
   tc_fence_after();
   const uint32_t tmem = ms.tmem_base;
   volatile int* abort_flag = &ms.abort_flag;
-  Walk walk = start_walk(p, ms.total);
-  Piece s;
-  auto slabs_of = [&](const Columns& col) { return least(s.s1, (col.hi - col.lo + 128) / 128) - s.s0; };
-  auto tiles_of = [&]() { return walk.l.cnt * walk.l.groups - s.pair * 8 > 4 ? 2 : 1; };
   uint8_t* const sA = smem + C::kOffA;
   RowInfo* const sRows = reinterpret_cast<RowInfo*>(smem + C::kOffRows);
   __half* const sQ = reinterpret_cast<__half*>(smem + C::kOffQ);
   // (every lane has the same; the reduction tells the compiler so, which keeps what follows from it on the uniform datapath)
   auto uniform = [](int v) -> int { return __reduce_max_sync(0xffffffffu, v); };
+  // the next piece; 0: there is none, or a wait ran out.  The warp gives its place in the ring back when it has read what it needs.
+  auto next_item = [&](int count) -> int {
+    if (!__all_sync(0xffffffffu, mbar_wait(&ms.item_full[count % kItems], (count / kItems) & 1, abort_flag))) return 0;
+    return uniform(ms.items[count % kItems].n);
+  };
+  auto free_item = [&](int count) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&ms.item_free[count % kItems]);
+  };
 
   if (warp < 4) {
     set_regs<kRegsLaunch, kRegsIssue>();
-    if (warp == 0) {
+    if (warp == 1) {
+      // ------------------------------------------------------------------ pieces
+      Walk walk = start_walk(p, ms.total);
+      Piece s;
+      int count = 0;
+      bool more = true;
+      while (more) {
+        more = next_piece(p, walk, s);
+        Item it{};
+        if (more) {
+          const Columns col = columns_of(a, walk.l, s.pair);
+          it.n = least(s.s1, (col.hi - col.lo + 128) / 128) - s.s0;
+          it.g0 = s.pair * 8;
+          it.groups = walk.l.groups;
+          it.all_groups = walk.l.cnt * walk.l.groups;
+          it.tiles = it.all_groups - it.g0 > 4 ? 2 : 1;
+          it.first = col.lo + s.s0 * 128;
+          it.behind = col.hi + 1;
+          it.b = s.b;
+          it.head = s.head;
+          it.ctx = walk.l.ctx;
+          it.out = p.part + (size_t)s.id * 8 * (D + 2);
+          if (it.n <= 0) {   // (its slabs lie behind all columns: nothing seen)
+            if (lane < 8 && it.g0 + lane < it.all_groups) it.out[lane * (D + 2)] = -INFINITY, it.out[lane * (D + 2) + 1] = 0.f;
+            continue;
+          }
+        }
+        if (!__all_sync(0xffffffffu, mbar_wait(&ms.item_free[count % kItems], ((count / kItems) & 1) ^ 1, abort_flag))) break;
+        if (lane == 0) {
+          ms.items[count % kItems] = it;
+          mbar_arrive(&ms.item_full[count % kItems]);
+        }
+        ++count;
+      }
+    } else if (warp == 0) {
       // ------------------------------------------------------------------ products
       // (the whole warp walks the schedule converged and one elected lane issues)
       const bool leader = elect_one();
@@ -454,12 +510,12 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
       int kst = 0, kph = 0, vst = 0, vph = 0;   // the rings' next stages
       int pieces[2] = {0, 0}, pcount[2] = {0, 0};
       bool alive = true;
-      while (alive && next_piece(p, walk, s)) {
-        const Columns col = columns_of(a, walk.l, s.pair);
-        const int n = uniform(slabs_of(col));
-        if (n <= 0) continue;
-        const int tiles = uniform(tiles_of());
-        const int wide = uniform(col.hi + 1 - (col.lo + s.s0 * 128));   // columns from the first slab on
+      for (int count = 0; alive; ++count) {
+        const int n = next_item(count);
+        if (n == 0) break;
+        const Item& it = ms.items[count % kItems];
+        const int tiles = uniform(it.tiles), wide = uniform(it.behind - it.first);   // columns from the first slab on
+        free_item(count);
         // S_x of slab i into its scores, P_x V of slab i: all of the slab's columns, or as many blocks of 32 (16) as there are
         auto issue_s = [&](auto xc, int i) {
           constexpr int X = decltype(xc)::value;
@@ -536,34 +592,33 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
     uint64_t* const full = keys ? ms.k_full : ms.v_full;
     uint64_t* const empty = keys ? ms.k_empty : ms.v_empty;
     uint8_t* const ring = smem + (keys ? C::kOffK : C::kOffV);
-    int slab = 0, st = 0, ph = 0, piece = 0, formed = 0;   // slabs and pieces so far, the ring's next stage, A's formed
+    int slab = 0, st = 0, ph = 0, formed = 0;   // slabs so far, the ring's next stage, A's formed
     bool alive = true;
-    while (alive && next_piece(p, walk, s)) {
-      Columns col = columns_of(a, walk.l, s.pair);
-      const int n = uniform(slabs_of(col));
-      if (n <= 0) continue;
-      col.lo = uniform(col.lo), col.hi = uniform(col.hi);
-      s.b = uniform(s.b), s.head = uniform(s.head), s.s0 = uniform(s.s0);
-      const size_t part_rows = (size_t)ca.c.N << ca.page_log2, head_rows = (size_t)s.head << ca.page_log2;
+    for (int count = 0; alive; ++count) {
+      const int n = next_item(count);
+      if (n == 0) break;
+      const Item& it = ms.items[count % kItems];
+      const int b = uniform(it.b), head = uniform(it.head), first = uniform(it.first), behind = uniform(it.behind);
+      const bool forms = mine < uniform(it.tiles);
+      const size_t part_rows = (size_t)ca.c.N << ca.page_log2, head_rows = (size_t)head << ca.page_log2;
       constexpr int kRowBytes = TileLoader<D, CODE>::kChunks * 16;
       const size_t load_rows = (keys ? kPartK1 : kPartV1) * part_rows + head_rows, v_rows = kPartV1 * part_rows + head_rows;
       auto form = [&]() {
         if (!__all_sync(0xffffffffu, mbar_wait(&ms.a_free[mine], (formed & 1) ^ 1, abort_flag))) return false;
-        form_rows<T16, D, CODE>(a, walk.l, s, mine, w, lane, sA + mine * C::kTile, sQ + (mine * 4 + w) * D, sRows + (piece & 1) * 256 + mine * 128);
+        form_rows<T16, D, CODE>(a, it, mine, w, lane, sA + mine * C::kTile, sQ + (mine * 4 + w) * D, sRows + (count & 1) * 256 + mine * 128);
         fence_async_smem();
         mbar_arrive(&ms.a_ready[mine]);
         ++formed;
         return true;
       };
-      const bool forms = mine < tiles_of();
       if (!keys && forms) alive = form();
       int v_exp = 0;   // the largest exponent byte of V1's rows in this piece so far
-      int token = col.lo + s.s0 * 128 + w * 32 + lane;
-      auto page_of = [&](int t) { return t <= col.hi ? place_of(ca, s.b, t).page : -1; };
+      int token = first + w * 32 + lane;
+      auto page_of = [&](int t) { return t < behind ? place_of(ca, b, t).page : -1; };
       int page = page_of(token);
       for (int i = 0; i < n && alive; ++i, token += 128) {
         const int pos = slab + i, mt = pos % kMetas, token0 = token - lane;
-        const bool any = token0 <= col.hi;   // (32 columns that no row looks at are not loaded)
+        const bool any = token0 < behind;   // (32 columns that no row looks at are not loaded)
         TileLoader<D, CODE> tile;
         int ek = 0, ev = 0;
         const size_t row = (size_t)page * (4 * part_rows) + (token & (ca.c.page_size - 1));   // (but for the part and head)
@@ -607,7 +662,7 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
         if (keys && i == 0 && forms) alive = form();   // (the first keys are on their way before)
       }
       slab += n;
-      ++piece;
+      free_item(count);
     }
   } else {
     set_regs<kRegsLaunch, kRegsSoftmax>();
@@ -615,26 +670,24 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
     const int x = (warp - 12) >> 2, wq = warp & 3;
     const uint32_t lane_base = (uint32_t)(wq * 32) << 16;
     const uint32_t tS = tmem + lane_base + x * 128, tO = tmem + lane_base + C::kTmemO + x * D;
-    int slab = 0, scount = 0, piece = 0, mine = 0;   // slabs and pieces so far; this tile's
+    int slab = 0, scount = 0, mine = 0;   // slabs so far; this tile's, and its pieces
     bool alive = true;
-    while (alive && next_piece(p, walk, s)) {
-      const Columns col = columns_of(a, walk.l, s.pair);
-      const int n = uniform(slabs_of(col)), ctx = uniform(walk.l.ctx);
-      const bool used = s.pair * 8 + x * 4 + wq < walk.l.cnt * walk.l.groups;   // (the warp's rows are of a new token)
-      float* out = p.part + (size_t)(s.id * 8 + x * 4 + wq) * (D + 2);
-      if (n <= 0) {
-        if (lane == 0 && used) out[0] = -INFINITY, out[1] = 0.f;
-        continue;
-      }
-      if (x >= tiles_of()) {   // (no second tile)
+    for (int count = 0; alive; ++count) {
+      const int n = next_item(count);
+      if (n == 0) break;
+      const Item& it = ms.items[count % kItems];
+      const int first = uniform(it.first), behind = uniform(it.behind), ctx = uniform(it.ctx);
+      const bool used = it.g0 + x * 4 + wq < it.all_groups;   // (the warp's rows are of a new token)
+      float* const out = it.out + (x * 4 + wq) * (D + 2);
+      const bool second = uniform(it.tiles) == 2;
+      free_item(count);
+      if (x == 1 && !second) {
         slab += n;
-        ++piece;
         continue;
       }
-      const int first = uniform(col.lo + s.s0 * 128), behind = uniform(col.hi + 1);
       alive = __all_sync(0xffffffffu, mbar_wait(&ms.a_ready[x], mine & 1, abort_flag));
       if (!alive) break;
-      const RowInfo r = sRows[(piece & 1) * 256 + x * 128 + wq * 32 + lane];
+      const RowInfo r = sRows[(count & 1) * 256 + x * 128 + wq * 32 + lane];
       // --- slabs: a half of 64 columns at a time is read once, its maximum taken, and the row's reference raised where that is 2^8 above it
       float m_used = -INFINITY, l_sum = 0.f;
       int v_exp = 0;
@@ -760,7 +813,6 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
       }
       if (!alive) break;
       slab += n;
-      ++piece;
       // --- the group's sum: sum over its rows of 2^(m_row - m) acc V2, and of the sums.  V2's codes come while the last products run
       const uint8_t* codes = (const uint8_t*)ca.c.codes + r.v2_row * (size_t)(D * (CODE == TRITT_CODE_F16 ? 2 : 1));
       // (a row that is not there has number 0 and weight 0)
