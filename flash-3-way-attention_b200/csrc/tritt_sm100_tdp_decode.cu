@@ -211,6 +211,23 @@ __device__ __forceinline__ bool next_piece(const Params& p, Walk& w, Piece& s) {
   return true;
 }
 
+// Two fp32 numbers an instruction.
+__device__ __forceinline__ float2 fma_pair(float2 a, float b, float c) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %4};\n\tmov.b64 z, {%5, %5};\n\t"
+      "fma.rn.ftz.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float2 add_pair(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.ftz.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+
 // Four fp16 pairs times a power of two (exact above 2^-24).
 __device__ __forceinline__ uint4 times(uint4 v, uint32_t f) {
   const __half2 h = *reinterpret_cast<const __half2*>(&f);
@@ -248,6 +265,13 @@ template <int D, int CODE> struct TileLoader {   // a warp's 32 rows of one part
   // mine: the lane's own row, null: none (zeros)
   __device__ __forceinline__ void load(const uint8_t* mine, int lane) {
     const uint32_t lo = (uint32_t)(size_t)mine, hi = (uint32_t)((size_t)mine >> 32);
+    // rows that follow one another in a page (all 32, where a tile does not start or end in the middle of one)
+    const size_t first = (size_t)__shfl_sync(0xffffffffu, hi, 0) << 32 | __shfl_sync(0xffffffffu, lo, 0);
+    if (__all_sync(0xffffffffu, mine != nullptr && (size_t)mine == first + lane * (kChunks * 16))) {
+#pragma unroll
+      for (int it = 0; it < kChunks; ++it) v[it] = __ldg(reinterpret_cast<const uint4*>(first) + it * 32 + lane);
+      return;
+    }
 #pragma unroll
     for (int it = 0; it < kChunks; ++it) {
       const int idx = it * 32 + lane, row = idx / kChunks, ch = idx % kChunks;
@@ -516,70 +540,61 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
         const Item& it = ms.items[count % kItems];
         const int tiles = uniform(it.tiles), wide = uniform(it.behind - it.first);   // columns from the first slab on
         free_item(count);
-        // S_x of slab i into its scores, P_x V of slab i: all of the slab's columns, or as many blocks of 32 (16) as there are
-        auto issue_s = [&](auto xc, int i) {
-          constexpr int X = decltype(xc)::value;
-          if (X == 0 && !wait_all(&ms.k_full[kst], kph)) return false;
-          tc_fence_after();
-          const uint32_t bLo = kLo + kst * (C::kTile >> 4);
-          const int w = wide - i * 128;
-          if (w > 96) {
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-              const uint32_t kk = (k >> 2) * (16384 >> 4) + (k & 3) * 2;
-              if (leader) mma_ss_lo(tmem + X * 128, aLo + X * (C::kTile >> 4) + kk, bLo + kk, kHi, idesc_s, k > 0);
-            }
-          } else {
-            const uint32_t idesc = make_idesc_f16(128, (w + 31) / 32 * 32, 0, false, false);
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-              const uint32_t kk = (k >> 2) * (16384 >> 4) + (k & 3) * 2;
-              if (leader) mma_ss_lo(tmem + X * 128, aLo + X * (C::kTile >> 4) + kk, bLo + kk, kHi, idesc, k > 0);
-            }
-          }
-          commit(&ms.s_ready[X]);
-          if (i == n - 1) commit(&ms.a_free[X]);
-          if (X == tiles - 1) {
-            commit(&ms.k_empty[kst]);
-            if (++kst == NS) kst = 0, kph ^= 1;
-          }
-          return true;
-        };
-        auto issue_pv = [&](auto xc, int i) {
-          constexpr int X = decltype(xc)::value;
-          if (!wait_all(&ms.p_ready[X], pcount[X] & 1)) return false;
-          ++pcount[X];
-          if (X == 0 && !wait_all(&ms.v_full[vst], vph)) return false;
-          tc_fence_after();
-          const uint32_t bLo = vLo + vst * (C::kTile >> 4);
-          const int w = wide - i * 128;
-          if (w > 112) {
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              if (leader)
-                mma_ts_lo(tmem + C::kTmemO + X * D, tmem + X * 128 + k * 8, bLo + k * (2048 >> 4), kHi, idesc_pv, k > 0 || i > 0);
-          } else {
+        // step i: P_x V of slab i (all of its columns, or as many blocks of 16 as there are), S_x of slab i + 1 (as many of 32), for the
+        // tiles in turn.  (S_x overwrites P_x: the pipe runs it behind P_x V.  One copy of the code: the instruction caches are small)
+        for (int i = -1; i < n && alive; ++i)
 #pragma unroll 1
-            for (int k = 0; k * 16 < w; ++k)
-              if (leader)
-                mma_ts_lo(tmem + C::kTmemO + X * D, tmem + X * 128 + k * 8, bLo + k * (2048 >> 4), kHi, idesc_pv, k > 0 || i > 0);
+          for (int x = 0; x < tiles && alive; ++x) {
+            if (i < 0) {
+              alive = wait_all(&ms.a_ready[x], pieces[x] & 1);
+              if (!alive) break;
+            } else {
+              alive = wait_all(&ms.p_ready[x], pcount[x] & 1) && (x > 0 || wait_all(&ms.v_full[vst], vph));
+              if (!alive) break;
+              ++pcount[x];
+              tc_fence_after();
+              const uint32_t bLo = vLo + vst * (C::kTile >> 4), acc = tmem + C::kTmemO + x * D, pT = tmem + x * 128;
+              const int w = wide - i * 128;
+              if (w > 112) {
+                if (leader) {
+#pragma unroll
+                  for (int k = 0; k < 8; ++k) mma_ts_lo(acc, pT + k * 8, bLo + k * (2048 >> 4), kHi, idesc_pv, k > 0 || i > 0);
+                }
+              } else {
+#pragma unroll 1
+                for (int k = 0; k * 16 < w; ++k)
+                  if (leader) mma_ts_lo(acc, pT + k * 8, bLo + k * (2048 >> 4), kHi, idesc_pv, k > 0 || i > 0);
+              }
+              if (i == n - 1) commit(&ms.o_done[x]);
+              if (x == tiles - 1) {
+                commit(&ms.v_empty[vst]);
+                if (++vst == NS) vst = 0, vph ^= 1;
+              }
+            }
+            if (i + 1 < n) {
+              if (x == 0) {
+                alive = wait_all(&ms.k_full[kst], kph);
+                if (!alive) break;
+              }
+              tc_fence_after();
+              const uint32_t bLo = kLo + kst * (C::kTile >> 4), aL = aLo + x * (C::kTile >> 4), sT = tmem + x * 128;
+              const int w = wide - (i + 1) * 128;
+              const uint32_t idesc = w > 96 ? idesc_s : make_idesc_f16(128, (w + 31) / 32 * 32, 0, false, false);
+              if (leader) {
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                  const uint32_t kk = (k >> 2) * (16384 >> 4) + (k & 3) * 2;
+                  mma_ss_lo(sT, aL + kk, bLo + kk, kHi, idesc, k > 0);
+                }
+              }
+              commit(&ms.s_ready[x]);
+              if (i + 2 >= n) commit(&ms.a_free[x]);
+              if (x == tiles - 1) {
+                commit(&ms.k_empty[kst]);
+                if (++kst == NS) kst = 0, kph ^= 1;
+              }
+            }
           }
-          if (i == n - 1) commit(&ms.o_done[X]);
-          if (X == tiles - 1) {
-            commit(&ms.v_empty[vst]);
-            if (++vst == NS) vst = 0, vph ^= 1;
-          }
-          return true;
-        };
-        constexpr std::integral_constant<int, 0> ta{};
-        constexpr std::integral_constant<int, 1> tb{};
-        alive = wait_all(&ms.a_ready[0], pieces[0] & 1) && issue_s(ta, 0) &&
-                (tiles == 1 || (wait_all(&ms.a_ready[1], pieces[1] & 1) && issue_s(tb, 0)));
-        for (int i = 0; i < n && alive; ++i) {
-          // (S_x of the next slab overwrites P_x: the pipe runs it behind P_x V)
-          alive = issue_pv(ta, i) && (i + 1 >= n || issue_s(ta, i + 1));
-          if (alive && tiles == 2) alive = issue_pv(tb, i) && (i + 1 >= n || issue_s(tb, i + 1));
-        }
         ++pieces[0];
         pieces[1] += tiles - 1;
       }
@@ -742,16 +757,18 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
         if (t > 0 && v_now != v_exp) correct(v_now - v_exp < 126 ? __uint_as_float((uint32_t)(127 - (v_now - v_exp)) << 23) : 0.f);
         v_exp = v_now;
         float psum = 0.f;
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
+#pragma unroll 1
+        for (int hf = 0; hf < 2; ++hf) {   // (one copy of the code)
           uint32_t pk2[32];
+          const float f0 = hf ? f[2] : f[0], f1 = hf ? f[3] : f[1];
           if (some >> hf & 1) {
             uint32_t sr[64];
             tmem_ld64(tS + hf * 64, sr);
             tmem_wait_ld();
             if (!full) {
+              const uint32_t m0 = hf ? mask[2] : mask[0], m1 = hf ? mask[3] : mask[1];
 #pragma unroll
-              for (int e = 0; e < 64; ++e) sr[e] = mask[hf * 2 + e / 32] >> (e % 32) & 1 ? sr[e] : 0xff800000u;
+              for (int e = 0; e < 64; ++e) sr[e] = (e < 32 ? m0 : m1) >> (e % 32) & 1 ? sr[e] : 0xff800000u;
             }
             float mx;
             {
@@ -762,7 +779,7 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
 #pragma unroll
                 for (int e = 2; e < 16; e += 2) q[k] = fmaxf(q[k], fmaxf(__uint_as_float(sr[k * 16 + e]), __uint_as_float(sr[k * 16 + e + 1])));
               }
-              mx = fmaxf(fmaxf(q[0], q[1]) * f[hf * 2], fmaxf(q[2], q[3]) * f[hf * 2 + 1]);
+              mx = fmaxf(fmaxf(q[0], q[1]) * f0, fmaxf(q[2], q[3]) * f1);
             }
             const bool grow = mx > m_used + kGap;
             if (__any_sync(0xffffffffu, grow)) {
@@ -790,16 +807,15 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
               }
             }
             const float shift = kLift - (m_used == -INFINITY ? 0.f : m_used);
-            float p0 = 0.f, p1 = 0.f;
+            float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
             for (int c = 0; c < 64; c += 2) {
-              const float e0 = exp2f(fmaf(__uint_as_float(sr[c]), f[hf * 2 + c / 32], shift));
-              const float e1 = exp2f(fmaf(__uint_as_float(sr[c + 1]), f[hf * 2 + c / 32], shift));
-              p0 += e0;
-              p1 += e1;
-              pk2[c >> 1] = pack2<__half>(e0, e1);
+              const float2 z = fma_pair(make_float2(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), c < 32 ? f0 : f1, shift);
+              const float2 e = make_float2(exp2f(z.x), exp2f(z.y));
+              sum[c >> 1 & 1] = add_pair(sum[c >> 1 & 1], e);
+              pk2[c >> 1] = pack2<__half>(e.x, e.y);
             }
-            psum += p0 + p1;
+            psum += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
           } else {
 #pragma unroll
             for (int e = 0; e < 32; ++e) pk2[e] = 0u;
@@ -902,9 +918,14 @@ struct TdpJoinParams {
   int ctas;
 };
 
-// The next CTA behind c that has a step.
-__device__ __forceinline__ long long next_owner(long long c, long long total, int ctas) {
-  const long long x = (c + 1) * total / ctas;   // its first step
+// CTA c has the steps from c total / ctas to the next one's.  The first step behind CTA c's, and the CTA of a step.  (Not inlined: a
+// division of 64 bits is long.)
+__device__ __noinline__ long long behind_cta(long long c, long long total, int ctas) {
+  if (total < 1 << 20) return (uint32_t)(c + 1) * (uint32_t)total / (uint32_t)ctas;
+  return (c + 1) * total / ctas;
+}
+__device__ __noinline__ long long cta_of(long long x, long long total, int ctas) {
+  if (total < 1 << 20) return ((uint32_t)(x + 1) * (uint32_t)ctas - 1) / (uint32_t)total;
   return ((x + 1) * ctas - 1) / total;
 }
 
@@ -933,18 +954,15 @@ __global__ void __launch_bounds__(256) tdp_join_kernel(const __grid_constant__ T
     if (g0 + tid < groups) {
       const int g = i * e.line.groups + g0 + tid;
       const long long pair = (long long)head * e.line.pairs + g / 8, first = e.base + pair * e.line.slabs, last = first + e.line.slabs - 1;
-      // CTA c has the steps from c total / ctas to the next one's; a piece of each that has any
       const long long id = (e.pair_base + pair) * 8 + g % 8;
       long long c;
       int pieces = 0;
       for (long long x = first; x <= last;) {
-        // (a division of 64 bits takes as long as the loads)
-        c = total < 1 << 20 ? ((uint32_t)(x + 1) * (uint32_t)j.ctas - 1) / (uint32_t)total : ((x + 1) * j.ctas - 1) / total;
-        x = total < 1 << 20 ? (uint32_t)(c + 1) * (uint32_t)total / (uint32_t)j.ctas : (c + 1) * total / j.ctas;
+        c = cta_of(x, total, j.ctas);
+        x = behind_cta(c, total, j.ctas);
         m = fmaxf(m, j.part[(size_t)(id + c * 8) * (D + 2)]);
         if (pieces++ == 0) s_id[tid] = c;
       }
-      // (with fewer steps than CTAs pieces are those of single steps: not every CTA has one)
       s_pieces[tid] = pieces;
     }
 #pragma unroll
@@ -960,7 +978,7 @@ __global__ void __launch_bounds__(256) tdp_join_kernel(const __grid_constant__ T
     for (int k = 0; k < E; ++k) acc[k] *= w0;
     top = now;
     const int here = groups - g0 < 256 ? groups - g0 : 256;
-#pragma unroll 4
+#pragma unroll 1
     for (int t = warp; t < here; t += 8) {
       const int g = i * e.line.groups + g0 + t;
       const long long pair = (long long)head * e.line.pairs + g / 8, id = (e.pair_base + pair) * 8 + g % 8;
@@ -976,7 +994,7 @@ __global__ void __launch_bounds__(256) tdp_join_kernel(const __grid_constant__ T
         sum += mp == -INFINITY ? (lp != lp ? lp : 0.f) : lp * w;
 #pragma unroll
         for (int q = 0; q < E; ++q) acc[q] += w == 0.f ? 0.f : v[q] * w;
-        if (k > 1) c = next_owner(c, total, j.ctas);
+        if (k > 1) c = cta_of(behind_cta(c, total, j.ctas), total, j.ctas);   // (with fewer steps than CTAs not every CTA has one)
       }
     }
   }
