@@ -35,7 +35,7 @@ using namespace sm100;
 
 constexpr int kThreads = 640;
 constexpr int kRegsLaunch = 96;   // a thread; the soft-max warps take what the others give up
-constexpr int kRegsIssue = 32, kRegsLoad = 96, kRegsSoftmax = 128;
+constexpr int kRegsIssue = 32, kRegsLoad = 112, kRegsSoftmax = 112;
 static_assert(kRegsIssue + 2 * kRegsLoad + 2 * kRegsSoftmax <= 5 * kRegsLaunch, "more registers than the launch has");
 constexpr float kGap = 8.f;      // the accumulator is rescaled when a row's maximum grew by more than 2^8
 constexpr float kLift = 7.f;     // P is formed times 2^7: at most 2^15, normal down to 2^-21 of the reference
@@ -308,7 +308,7 @@ template <int D, int CODE> struct TileLoader {   // a warp's 32 rows of one part
 // A warp's 32 rows of a tile: token k of new token i each.  A = 2^-kDown q * code, q brought to [1, 2); the powers of two and alpha go to
 // the scores' scale.
 template <typename T16, int D, int CODE>
-__device__ __forceinline__ void form_rows(const TdpDecodeArgs& a, const Item& s, int x, int wq, int lane, uint8_t* tile, __half* sq, RowInfo* info) {
+__device__ __noinline__ void form_rows(const TdpDecodeArgs& a, const Item& s, int x, int wq, int lane, uint8_t* tile, __half* sq, RowInfo* info) {
   const CacheArgs& ca = a.cache;
   const int g = s.g0 + x * 4 + wq, ctx = s.ctx;
   const bool any = g < s.all_groups;
@@ -759,7 +759,6 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
         float psum = 0.f;
 #pragma unroll 1
         for (int hf = 0; hf < 2; ++hf) {   // (one copy of the code)
-          uint32_t pk2[32];
           const float f0 = hf ? f[2] : f[0], f1 = hf ? f[3] : f[1];
           if (some >> hf & 1) {
             uint32_t sr[64];
@@ -809,18 +808,25 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
             const float shift = kLift - (m_used == -INFINITY ? 0.f : m_used);
             float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
-            for (int c = 0; c < 64; c += 2) {
-              const float2 z = fma_pair(make_float2(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), c < 32 ? f0 : f1, shift);
-              const float2 e = make_float2(exp2f(z.x), exp2f(z.y));
-              sum[c >> 1 & 1] = add_pair(sum[c >> 1 & 1], e);
-              pk2[c >> 1] = pack2<__half>(e.x, e.y);
+            for (int q = 0; q < 2; ++q) {
+              uint32_t pk[16];
+#pragma unroll
+              for (int c = 0; c < 32; c += 2) {
+                const float2 z = fma_pair(make_float2(__uint_as_float(sr[q * 32 + c]), __uint_as_float(sr[q * 32 + c + 1])), q ? f1 : f0, shift);
+                const float2 e = make_float2(exp2f(z.x), exp2f(z.y));
+                sum[c >> 1 & 1] = add_pair(sum[c >> 1 & 1], e);
+                pk[c >> 1] = pack2<__half>(e.x, e.y);
+              }
+              tmem_st16(tS + hf * 32 + q * 16, pk);
             }
             psum += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-          } else {
+          } else if (hf * 64 < wid) {
+            uint32_t pk[16];
 #pragma unroll
-            for (int e = 0; e < 32; ++e) pk2[e] = 0u;
+            for (int e = 0; e < 16; ++e) pk[e] = 0u;
+            tmem_st16(tS + hf * 32, pk);
+            tmem_st16(tS + hf * 32 + 16, pk);
           }
-          if (hf * 64 < wid) tmem_st32(tS + hf * 32, pk2);
         }
         l_sum += bad ? __uint_as_float(0x7fffffffu) : psum;
         tmem_wait_st();
