@@ -839,12 +839,13 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
       const uint8_t* codes = (const uint8_t*)ca.c.codes + r.v2_row * (size_t)(D * (CODE == TRITT_CODE_F16 ? 2 : 1));
       // (a row that is not there has number 0 and weight 0)
       constexpr int kWords = CODE == TRITT_CODE_F16 ? 4 : 2;   // 16-byte words of 32 columns' codes
-      uint4 now[kWords], next[kWords];
+      uint4 even[kWords], odd[kWords];   // two blocks ahead: a row's codes lie apart from its neighbours', and come from L2
       auto load_codes = [&](uint4 (&v)[kWords], int ch) {
 #pragma unroll
         for (int k = 0; k < kWords; ++k) v[k] = __ldg(reinterpret_cast<const uint4*>(codes) + ch * kWords + k);
       };
-      load_codes(now, 0);
+      load_codes(even, 0);
+      load_codes(odd, 1);
       if ((r.flags & kRowNan) && l_sum > 0.f) l_sum = __uint_as_float(0x7fffffffu);
       float m_all = m_used;
 #pragma unroll
@@ -863,21 +864,19 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
       }
       ++mine;
       tc_fence_after();
-#pragma unroll 1
-      for (int ch = 0; ch < D / 32; ++ch) {
+      auto fold = [&](uint4 (&c)[kWords], int ch) {
         uint32_t o[32];
         tmem_ld32(tO + ch * 32, o);
-        if (ch + 1 < D / 32) load_codes(next, ch + 1);
         tmem_wait_ld(o);
         float v[32];
         auto times_codes = [&](uint32_t h, int at) {
-          const float2 c = unpack2<__half>(h);
-          v[at] = weight == 0.f ? 0.f : c.x * vscale * __uint_as_float(o[at]);
-          v[at + 1] = weight == 0.f ? 0.f : c.y * vscale * __uint_as_float(o[at + 1]);
+          const float2 f = unpack2<__half>(h);
+          v[at] = weight == 0.f ? 0.f : f.x * vscale * __uint_as_float(o[at]);
+          v[at + 1] = weight == 0.f ? 0.f : f.y * vscale * __uint_as_float(o[at + 1]);
         };
 #pragma unroll
         for (int k = 0; k < kWords; ++k) {
-          const uint32_t w[4] = {now[k].x, now[k].y, now[k].z, now[k].w};
+          const uint32_t w[4] = {c[k].x, c[k].y, c[k].z, c[k].w};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             if constexpr (CODE == TRITT_CODE_F16) {
@@ -889,8 +888,8 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
               times_codes(h1, k * 16 + e * 4 + 2);
             }
           }
-          now[k] = next[k];
         }
+        if (ch + 2 < D / 32) load_codes(c, ch + 2);
         // column sums over the warp: halves change hands until each lane has one column
 #pragma unroll
         for (int h = 16; h > 0; h >>= 1) {
@@ -902,6 +901,11 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
           }
         }
         if (used) out[2 + ch * 32 + lane] = v[0];
+      };
+#pragma unroll 1
+      for (int ch = 0; ch < D / 32; ch += 2) {
+        fold(even, ch);
+        fold(odd, ch + 1);
       }
       if (used && lane == 0) out[0] = m_all, out[1] = l_all;
       tc_fence_before();
