@@ -707,8 +707,10 @@ def test_the_librarys_own_refusals():
     assert lib.tritt_dps_append(none, rows, 1, 0.1, 1, p, 1 << 40, None, 0, None) == -16
     assert lib.tritt_dps_decode(none, rows, p, None, 1, 0.1, p, 1 << 40, None, 0, None) == -16
     c = C.byref(c)
-    assert lib.tritt_tdp_decode(c, rows, p, None, 1, 0.1, 1, 1, 1, 1, None, 0, None, 0, None) == -6
-    assert lib.tritt_tdp_decode(c, rows, p, None, 1, 0.1, 1, 1, 1, 1, p, 8, None, 0, None) == -6
+    wide = C.byref(_native.Cache(**{**good, "page_size": 4096}))   # (what fits in shared memory needs no workspace)
+    assert lib.tritt_decode_workspace(_native.OP_TDP_DECODE, wide, 1, 1 << 30, 1 << 30, 0) > 0
+    assert lib.tritt_tdp_decode(wide, rows, p, None, 1, 0.1, 9999, 9999, 1, 1, None, 0, None, 0, None) == -6
+    assert lib.tritt_tdp_decode(wide, rows, p, None, 1, 0.1, 9999, 9999, 1, 1, p, 8, None, 0, None) == -6
     assert lib.tritt_tdp_decode(c, rows, p, None, 1, 0.1, 1, -1, 1, 1, p, 1 << 40, None, 0, None) == -10
     assert lib.tritt_tdp_decode(c, rows, None, None, 1, 0.1, 1, 1, 1, 1, p, 1 << 40, None, 0, None) == -4
     assert lib.tritt_dps_append(c, rows, 1, 0.1, -1, p, 1 << 40, None, 0, None) == -10
