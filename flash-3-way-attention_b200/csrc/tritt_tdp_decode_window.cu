@@ -64,7 +64,7 @@ __global__ void __launch_bounds__(kWarps * 32) tdp_decode_window_kernel(const __
   const int head = blockIdx.x % ca.c.N, b = blockIdx.x / ca.c.N, i0 = blockIdx.y * p.tokens;
   const int ctx = context_of(ca, b), cnt = new_tokens(ca, b), ni = min(p.tokens, cnt - i0), want = min(p.tokens, ca.c.n - i0);
   // staged: K1, V1 [cols], K2, V2 [rows], then the exponent bytes of the rows' K2 and V2 and of the columns (0: not there, 255: NaN), queries,
-  // of each 32 columns those that are there and those that read as NaN, sums
+  // their words, of each 32 columns those that are there and those that read as NaN, sums
   uint8_t* const sK1 = smem;
   uint8_t* const sV1 = sK1 + p.cols * 2 * D;
   uint8_t* const sK2 = sV1 + p.cols * 2 * D;
@@ -75,7 +75,8 @@ __global__ void __launch_bounds__(kWarps * 32) tdp_decode_window_kernel(const __
   uint8_t* const sEv1 = sEk1 + p.cols;
   __half* const sQ = reinterpret_cast<__half*>(sEv1 + p.cols);          // [tokens][D]
   float* const sScale = reinterpret_cast<float*>(sQ + p.tokens * D);    // [tokens]
-  uint32_t* const sThere = reinterpret_cast<uint32_t*>(sScale + p.tokens);   // [cols / 32]
+  unsigned long long* const sWord = reinterpret_cast<unsigned long long*>(sScale + (p.tokens + 1) / 2 * 2);   // [tokens]
+  uint32_t* const sThere = reinterpret_cast<uint32_t*>(sWord + p.tokens);   // [cols / 32]
   uint32_t* const sNan = sThere + p.cols / 32;
   float* const sPart = reinterpret_cast<float*>(sNan + p.cols / 32);    // [tokens][tiles][D + 2]
   if (tid < 2) s_most[tid] = 0;
@@ -86,35 +87,50 @@ __global__ void __launch_bounds__(kWarps * 32) tdp_decode_window_kernel(const __
   const int end = ni > 0 ? ctx + i0 + ni : 0, lo_j = max(0, min(ctx, first_pos - a.k1w)), lo_k = max(0, min(ctx, first_pos - a.k2w));
   const int nj = ni > 0 ? end - lo_j : 0, nk = ni > 0 ? end - lo_k : 0;
   constexpr int L = D / 8;   // lanes of a row
-  auto stage = [&](int part, int lo, int n, int places, uint8_t* to, uint8_t* exps, int* most) {
-    for (int r0 = 0; r0 < (n + 31) / 32 * 32 && r0 < places; r0 += kWarps * 32 / L) {
-      const int r = r0 + tid / L, ch = tid % L;
-      uint4 h = make_uint4(0u, 0u, 0u, 0u);
-      int byte = 0;
-      if (r < n) {
-        const Place at = place_of(ca, b, lo + r);
-        if (at.page >= 0) {
-          const size_t row = row_of(ca, at, part, head);
-          Codes8<CODE> c;
-          c.load((const uint8_t*)ca.c.codes + row * (size_t)(D * (CODE == TRITT_CODE_F16 ? 2 : 1)), ch * 8);
-          byte = __ldg(ca.c.exponents + row);
-          uint32_t w[4];
-          c.halves(w);
-          h = make_uint4(w[0], w[1], w[2], w[3]);
-          byte = max(byte, 1);   // (a row that nobody has written is one of zeros)
-        }
+  // two parts of the same tokens; four rows of a thread at a time, whose loads overlap
+  auto stage = [&](int part, int part2, int lo, int n, int places, uint8_t* to, uint8_t* to2, uint8_t* exps, uint8_t* exps2, bool columns) {
+    constexpr int kStep = kWarps * 32 / L, kBatch = 4;
+    const int ch = tid % L;
+    for (int r0 = tid / L; r0 < (n + 31) / 32 * 32; r0 += kStep * kBatch) {
+      int page[kBatch], e1[kBatch], e2[kBatch];
+      Codes8<CODE> c1[kBatch], c2[kBatch];
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int r = r0 + k * kStep;
+        page[k] = r < n ? place_of(ca, b, lo + r).page : -1;
       }
-      if (r < places) {
-        *reinterpret_cast<uint4*>(to + staged<D>(r, ch)) = h;
-        if (ch == 0) exps[r] = (uint8_t)byte;
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const size_t at = row_of(ca, Place{max(page[k], 0), (lo + r0 + k * kStep) & (ca.c.page_size - 1)}, part, head);
+        const size_t at2 = at + (size_t)(part2 - part) * ((size_t)ca.c.N << ca.page_log2);
+        constexpr int kBytes = D * (CODE == TRITT_CODE_F16 ? 2 : 1);
+        c1[k].load((const uint8_t*)ca.c.codes + at * kBytes, ch * 8);
+        c2[k].load((const uint8_t*)ca.c.codes + at2 * kBytes, ch * 8);
+        e1[k] = __ldg(ca.c.exponents + at);
+        e2[k] = __ldg(ca.c.exponents + at2);
       }
-      if (most && ch == 0 && byte != 255 && byte > 0) atomicMax(most, byte);
+      int m1 = 0, m2 = 0;
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int r = r0 + k * kStep;
+        if (r >= places) break;
+        uint32_t w1[4], w2[4];
+        c1[k].halves(w1);
+        c2[k].halves(w2);
+        const uint32_t on = page[k] >= 0 ? 0xffffffffu : 0u;
+        *reinterpret_cast<uint4*>(to + staged<D>(r, ch)) = make_uint4(w1[0] & on, w1[1] & on, w1[2] & on, w1[3] & on);
+        *reinterpret_cast<uint4*>(to2 + staged<D>(r, ch)) = make_uint4(w2[0] & on, w2[1] & on, w2[2] & on, w2[3] & on);
+        e1[k] = on ? max(e1[k], 1) : 0;   // (a row that nobody has written is one of zeros)
+        e2[k] = on ? max(e2[k], 1) : 0;
+        if (ch == 0) exps[r] = (uint8_t)e1[k], exps2[r] = (uint8_t)e2[k];
+        m1 = max(m1, e1[k] == 255 ? 0 : e1[k]);
+        m2 = max(m2, e2[k] == 255 ? 0 : e2[k]);
+      }
+      if (columns && ch == 0) atomicMax(&s_most[0], m1), atomicMax(&s_most[1], m2);
     }
   };
-  stage(kPartK1, lo_j, nj, p.cols, sK1, sEk1, &s_most[0]);
-  stage(kPartV1, lo_j, nj, p.cols, sV1, sEv1, &s_most[1]);
-  stage(kPartK2, lo_k, nk, p.rows, sK2, sEk2, nullptr);
-  stage(kPartV2, lo_k, nk, p.rows, sV2, sEv2, nullptr);
+  stage(kPartK1, kPartV1, lo_j, nj, p.cols, sK1, sV1, sEk1, sEv1, true);
+  stage(kPartK2, kPartV2, lo_k, nk, p.rows, sK2, sV2, sEk2, sEv2, false);
   // queries, brought to [1, 2)
   for (int i = warp; i < ni; i += kWarps) {
     constexpr int E = D / 32;
@@ -131,6 +147,7 @@ __global__ void __launch_bounds__(kWarps * 32) tdp_decode_window_kernel(const __
     const float up = __uint_as_float((uint32_t)power << 23) * (a.scale2 < 0.f ? -1.f : 1.f);
 #pragma unroll
     for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(sQ + i * D + lane * E + e) = pack2<__half>(f[e] * up, f[e + 1] * up);
+    if (lane == 0) sWord[i] = ca.c.ancestors ? seen_word(ca, b, i0 + i) : 0;
     if (lane == 0) sScale[i] = fabsf(a.scale2) * __uint_as_float((uint32_t)(254 - power) << 23) * (float)(1 << kDown<CODE>);
   }
   __syncthreads();
@@ -156,11 +173,19 @@ __global__ void __launch_bounds__(kWarps * 32) tdp_decode_window_kernel(const __
   __syncthreads();
   const float k1_scale = ek1 > kUp<CODE> ? __uint_as_float((uint32_t)(ek1 - kUp<CODE>) << 23) : 0.f;
 
+  // (staged rows from a multiple of 8 on: where a thread's chunks lie does not change)
+  const uint8_t* key_at[D / 32];
+  uint32_t value_at[D / 16];
+#pragma unroll
+  for (int j = 0; j < D / 32; ++j) key_at[j] = sK1 + staged<D>(g, j * 4 + t);
+#pragma unroll
+  for (int d = 0; d < D / 16; ++d) value_at[d] = smem_u32(sV1 + staged<D>(lane & 15, d * 2 + (lane >> 4)));
+
   // --- units: 16 rows of one new token
   for (int u = warp; u < ni * p.tiles; u += kWarps) {
     const int i = u / p.tiles, row0 = u % p.tiles * 16;
     float* const out = sPart + (size_t)u * (D + 2);
-    const unsigned long long word = ca.c.ancestors ? seen_word(ca, b, i0 + i) : 0;
+    const unsigned long long word = sWord[i];
     const int pos_q = ctx + (ca.c.ancestors ? __popcll(word) - 1 : i0 + i), klo = max(0, pos_q - a.k2w);
     if (klo + row0 > pos_q) {   // (fewer rows than the most)
       if (lane == 0) out[0] = -INFINITY, out[1] = 0.f;
@@ -250,7 +275,7 @@ __global__ void __launch_bounds__(kWarps * 32) tdp_decode_window_kernel(const __
         for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
 #pragma unroll
         for (int j = 0; j < D / 32; ++j) {
-          const uint4 k = *reinterpret_cast<const uint4*>(sK1 + staged<D>(c0 + n * 8 + g, j * 4 + t));
+          const uint4 k = *reinterpret_cast<const uint4*>(key_at[j] + (c0 + n * 8) * (2 * D));
           mma_16816(s[n], af[2 * j], k.x, k.y);
           mma_16816(s[n], af[2 * j + 1], k.z, k.w);
         }
@@ -305,8 +330,7 @@ __global__ void __launch_bounds__(kWarps * 32) tdp_decode_window_kernel(const __
         for (int d = 0; d < D / 16; ++d) {
           // V1 of 16 tokens x 16 columns: four 8 x 8 blocks, transposed
           uint32_t v[4];
-          const int row = c0 + k2 * 16 + (lane & 15);
-          ldmatrix_x4_trans(v, smem_u32(sV1 + staged<D>(row, d * 2 + (lane >> 4))));
+          ldmatrix_x4_trans(v, value_at[d] + (c0 + k2 * 16) * (2 * D));
           mma_16816(acc[2 * d], pf[k2], v[0], v[1]);
           mma_16816(acc[2 * d + 1], pf[k2], v[2], v[3]);
         }
@@ -385,7 +409,7 @@ __global__ void __launch_bounds__(kWarps * 32) tdp_decode_window_kernel(const __
 }
 
 size_t smem_of(const WindowParams& p, int D) {
-  return (size_t)(p.cols + p.rows) * (4 * D + 2) + (size_t)p.tokens * (2 * D + 4) + (size_t)p.cols / 4 + (size_t)p.tokens * p.tiles * (D + 2) * 4 + 16;
+  return (size_t)(p.cols + p.rows) * (4 * D + 2) + (size_t)p.tokens * (2 * D + 12) + 4 + (size_t)p.cols / 4 + (size_t)p.tokens * p.tiles * (D + 2) * 4 + 16;
 }
 
 // What a call's blocks stage, and how many new tokens each takes: as few as fill the chip, for the more, the more read a row once.  False: too much.
