@@ -78,7 +78,8 @@ __global__ void __launch_bounds__(kWarps * 32) tdp_decode_window_kernel(const __
   unsigned long long* const sWord = reinterpret_cast<unsigned long long*>(sScale + (p.tokens + 1) / 2 * 2);   // [tokens]
   uint32_t* const sThere = reinterpret_cast<uint32_t*>(sWord + p.tokens);   // [cols / 32]
   uint32_t* const sNan = sThere + p.cols / 32;
-  float* const sPart = reinterpret_cast<float*>(sNan + p.cols / 32);    // [tokens][tiles][D + 2]
+  uint8_t* const sTree = reinterpret_cast<uint8_t*>(sNan + p.cols / 32);   // [tokens][64]: which new token is the d-th that a new token attends to
+  float* const sPart = reinterpret_cast<float*>(sTree + (ca.c.ancestors ? p.tokens * 64 : 0));   // [tokens][tiles][D + 2]
   if (tid < 2) s_most[tid] = 0;
   __syncthreads();
 
@@ -147,7 +148,13 @@ __global__ void __launch_bounds__(kWarps * 32) tdp_decode_window_kernel(const __
     const float up = __uint_as_float((uint32_t)power << 23) * (a.scale2 < 0.f ? -1.f : 1.f);
 #pragma unroll
     for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(sQ + i * D + lane * E + e) = pack2<__half>(f[e] * up, f[e + 1] * up);
-    if (lane == 0) sWord[i] = ca.c.ancestors ? seen_word(ca, b, i0 + i) : 0;
+    const unsigned long long word = ca.c.ancestors ? seen_word(ca, b, i0 + i) : 0;
+    if (lane == 0) sWord[i] = word;
+    if (ca.c.ancestors) {
+#pragma unroll
+      for (int m = lane; m < 64; m += 32)
+        if (word >> m & 1) sTree[i * 64 + __popcll(word & ((1ull << m) - 1))] = (uint8_t)m;
+    }
     if (lane == 0) sScale[i] = fabsf(a.scale2) * __uint_as_float((uint32_t)(254 - power) << 23) * (float)(1 << kDown<CODE>);
   }
   __syncthreads();
@@ -200,11 +207,7 @@ __global__ void __launch_bounds__(kWarps * 32) tdp_decode_window_kernel(const __
     for (int h = 0; h < 2; ++h) {
       const int pk = klo + row0 + g + h * 8;
       int token = pk;
-      if (ca.c.ancestors && pk >= ctx && pk <= pos_q) {
-        unsigned long long left = word;
-        for (int c = ctx; c < pk && left; ++c) left &= left - 1;
-        token = ctx + __ffsll(left) - 1;
-      }
+      if (ca.c.ancestors && pk >= ctx && pk <= pos_q) token = ctx + sTree[i * 64 + pk - ctx];
       bool on = pk <= pos_q;
       place[h] = on ? token - lo_k : 0;
       const int e1 = sEk2[place[h]], e2 = sEv2[place[h]];
@@ -219,11 +222,8 @@ __global__ void __launch_bounds__(kWarps * 32) tdp_decode_window_kernel(const __
       c_lo[h] = on ? max(max(0, pos_q - a.k1w), pk - min(pk, a.kkl)) : 1 << 30;
       c_hi[h] = !on ? -1 : ca.c.ancestors ? min(ctx - 1, last) : last;
       tree[h] = 0;
-      if (on && ca.c.ancestors) {
-        unsigned long long left = word;
-        for (int c = ctx; left; ++c, left &= left - 1)
-          if (c >= c_lo[h] && c <= last) tree[h] |= left & (~left + 1);
-      }
+      if (on && ca.c.ancestors && last >= ctx && last >= c_lo[h])   // (its tokens between the first and the last of the window)
+        tree[h] = word & (~0ull << sTree[i * 64 + max(c_lo[h] - ctx, 0)]) & (~0ull >> (63 - sTree[i * 64 + last - ctx]));
     }
     // A's fragments: elements 32 j + 8 t + 4 s + {0, 1 | 2, 3} of rows g, g + 8 in steps s = 0, 1
     uint32_t af[D / 16][4];
@@ -409,7 +409,7 @@ __global__ void __launch_bounds__(kWarps * 32) tdp_decode_window_kernel(const __
 }
 
 size_t smem_of(const WindowParams& p, int D) {
-  return (size_t)(p.cols + p.rows) * (4 * D + 2) + (size_t)p.tokens * (2 * D + 12) + 4 + (size_t)p.cols / 4 + (size_t)p.tokens * p.tiles * (D + 2) * 4 + 16;
+  return (size_t)(p.cols + p.rows) * (4 * D + 2) + (size_t)p.tokens * (2 * D + 12 + 64) + 4 + (size_t)p.cols / 4 + (size_t)p.tokens * p.tiles * (D + 2) * 4 + 16;
 }
 
 // What a call's blocks stage, and how many new tokens each takes: as few as fill the chip, for the more, the more read a row once.  False: too much.
