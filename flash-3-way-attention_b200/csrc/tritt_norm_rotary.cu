@@ -5,11 +5,15 @@
 //   dw = sum over rows of du h,   dx = r (g - h mean(g h)).
 // Everything between the load of a row and its store is fp32.
 //
-// Bound by HBM: forward one read and one write of the rows, backward two reads and one write.  A thread holds eight neighbouring
-// elements, D / 8 lanes a row; the two sums and the other half of a rotated pair cross lanes by shuffles.  The tables (a cosine and a sine, 8
-// bytes, for two elements) would be twice the traffic of 16-bit rows, so a thread keeps its position's values for four heads and,
-// where there are blocks enough, all three tensors.
+// Bound by HBM: forward one read and one write of the rows, backward two reads and one write.  D / 8 lanes take a row, eight elements each:
+// two groups of four that lie R / 2 apart, so that a thread holds both of each rotated pair (neighbours where there is no rotation or
+// neighbours are rotated).  With eight neighbours a lane and the other half by shuffles the forward executed 202 instructions for eight
+// elements, and instruction issue bounded it (4 x 16 heads x 2048 x 128 bf16: 53 us, the backward 121).  Two fp32 numbers an instruction.
+// The tables (a cosine and a sine, 8 bytes, for two elements) would be twice the traffic of 16-bit rows, so a thread keeps its position's
+// values for four heads and, where there are blocks enough, all three tensors.
 #include "tritt_common.cuh"
+
+#include <type_traits>
 
 namespace tritt {
 namespace {
@@ -25,47 +29,78 @@ struct NormParams {
   int* status;
 };
 
-template <typename T> struct Eight;   // eight elements, 16-byte accesses
-template <> struct Eight<float> {
-  float4 v[2];
-  __device__ __forceinline__ void load(const float* p) {
-    v[0] = __ldg(reinterpret_cast<const float4*>(p));
-    v[1] = __ldg(reinterpret_cast<const float4*>(p) + 1);
-  }
-  __device__ __forceinline__ void get(float (&f)[8]) const {
-    f[0] = v[0].x, f[1] = v[0].y, f[2] = v[0].z, f[3] = v[0].w, f[4] = v[1].x, f[5] = v[1].y, f[6] = v[1].z, f[7] = v[1].w;
-  }
-  static __device__ __forceinline__ void store(float* p, const float (&f)[8]) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
-  }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.ftz.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.ftz.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// A lane's eight elements as four pairs of neighbours: pairs 0, 1 from column a on, 2, 3 from column b on.
+struct Cols {
+  int a, b;
 };
-template <typename T> struct Eight16 {
-  uint4 v;
-  __device__ __forceinline__ void load(const T* p) { v = __ldg(reinterpret_cast<const uint4*>(p)); }
-  __device__ __forceinline__ void get(float (&f)[8]) const {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+// With the halves rotated, lane i of the first R / 8 takes columns 4 i .. and R / 2 + 4 i ..; any other lane eight neighbours.
+__device__ __forceinline__ Cols cols_of(int lane, int rot, int interleaved) {
+  if (!interleaved && lane * 8 < rot) return Cols{lane * 4, rot / 2 + lane * 4};
+  return Cols{lane * 8, lane * 8 + 4};
+}
+
+template <typename T> struct Eight {   // of a 16-bit type
+  uint2 v[2];
+  __device__ __forceinline__ void load(const T* p, Cols c) {
+    v[0] = __ldg(reinterpret_cast<const uint2*>(p + c.a));
+    v[1] = __ldg(reinterpret_cast<const uint2*>(p + c.b));
+  }
+  __device__ __forceinline__ void get(float2 (&f)[4]) const {
+    const uint32_t w[4] = {v[0].x, v[0].y, v[1].x, v[1].y};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      T lo, hi;
-      *reinterpret_cast<uint16_t*>(&lo) = (uint16_t)w[i];
-      *reinterpret_cast<uint16_t*>(&hi) = (uint16_t)(w[i] >> 16);
-      f[2 * i] = to_f(lo);
-      f[2 * i + 1] = to_f(hi);
+      if constexpr (std::is_same<T, __half>::value)
+        f[i] = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      else
+        f[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
     }
   }
-  static __device__ __forceinline__ void store(T* p, const float (&f)[8]) {
+  static __device__ __forceinline__ void store(T* p, Cols c, const float2 (&f)[4]) {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const T lo = from_f<T>(f[2 * i]), hi = from_f<T>(f[2 * i + 1]);
-      w[i] = (uint32_t)*reinterpret_cast<const uint16_t*>(&lo) | (uint32_t)*reinterpret_cast<const uint16_t*>(&hi) << 16;
+      if constexpr (std::is_same<T, __half>::value) {
+        const __half2 h = __floats2half2_rn(f[i].x, f[i].y);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(f[i].x, f[i].y);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
     }
-    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    *reinterpret_cast<uint2*>(p + c.a) = make_uint2(w[0], w[1]);
+    *reinterpret_cast<uint2*>(p + c.b) = make_uint2(w[2], w[3]);
   }
 };
-template <> struct Eight<__half> : Eight16<__half> {};
-template <> struct Eight<__nv_bfloat16> : Eight16<__nv_bfloat16> {};
+template <> struct Eight<float> {
+  float4 v[2];
+  __device__ __forceinline__ void load(const float* p, Cols c) {
+    v[0] = __ldg(reinterpret_cast<const float4*>(p + c.a));
+    v[1] = __ldg(reinterpret_cast<const float4*>(p + c.b));
+  }
+  __device__ __forceinline__ void get(float2 (&f)[4]) const {
+    f[0] = make_float2(v[0].x, v[0].y), f[1] = make_float2(v[0].z, v[0].w), f[2] = make_float2(v[1].x, v[1].y), f[3] = make_float2(v[1].z, v[1].w);
+  }
+  static __device__ __forceinline__ void store(float* p, Cols c, const float2 (&f)[4]) {
+    *reinterpret_cast<float4*>(p + c.a) = make_float4(f[0].x, f[0].y, f[1].x, f[1].y);
+    *reinterpret_cast<float4*>(p + c.b) = make_float4(f[2].x, f[2].y, f[3].x, f[3].y);
+  }
+};
 
 // Sum over the lanes of a row (a power of two of neighbouring lanes).
 template <int L> __device__ __forceinline__ float row_sum(float v) {
@@ -73,32 +108,38 @@ template <int L> __device__ __forceinline__ float row_sum(float v) {
   for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+__device__ __forceinline__ float dot(const float2 (&a)[4], const float2 (&b)[4]) {
+  float2 s = mul2(a[0], b[0]);
+#pragma unroll
+  for (int i = 1; i < 4; ++i) s = fma2(a[i], b[i], s);
+  return s.x + s.y;
+}
 
-// The eight weights of a thread's columns (1 where there are none).
-template <typename T> __device__ __forceinline__ void load_weights(const NormParams& p, int which, int head, int col, float (&w)[8]) {
+// The weights of a thread's columns (1 where there are none).
+template <typename T> __device__ __forceinline__ void load_weights(const NormParams& p, int which, int head, Cols c, float2 (&w)[4]) {
   const void* base = p.a.w[which];
-  const size_t off = (p.a.weight_heads ? (size_t)head * p.a.D : 0) + col;
+  const size_t off = p.a.weight_heads ? (size_t)head * p.a.D : 0;
   if (base == nullptr) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = 1.f;
+    for (int i = 0; i < 4; ++i) w[i] = both(1.f);
   } else if (p.a.weight_dtype == TRITT_F32) {
     Eight<float> v;
-    v.load((const float*)base + off);
+    v.load((const float*)base + off, c);
     v.get(w);
   } else {
     Eight<T> v;
-    v.load((const T*)base + off);
+    v.load((const T*)base + off, c);
     v.get(w);
   }
 }
 
-// Cosines and sines of a thread's eight columns: of each column of a half (halves), or of four pairs (interleaved).
+// Cosines and sines of a thread's four rotated pairs: (1, 0) where its columns are not rotated.
 struct Turn {
-  float c[8], s[8];
+  float c[4], s[4];
 };
-__device__ __forceinline__ void load_turn(const NormParams& p, int b, int t, int col, Turn& turn) {
-  const int R = p.a.rot;
-  if (col >= R) return;
+__device__ __forceinline__ Turn load_turn(const NormParams& p, int b, int t, int lane) {
+  Turn turn{{1.f, 1.f, 1.f, 1.f}, {0.f, 0.f, 0.f, 0.f}};
+  if (lane * 8 >= p.a.rot) return turn;
   long long at = t;
   if (p.a.positions) {
     const long long i = b * p.a.position_stride_b + t * p.a.position_stride_t;
@@ -108,46 +149,27 @@ __device__ __forceinline__ void load_turn(const NormParams& p, int b, int t, int
     if (p.status) atomicOr(p.status, 256);
     at = at < 0 ? 0 : p.a.table - 1;
   }
-  const size_t row = (size_t)at * (R / 2);
-  if (p.a.interleaved) {
-    const float4 c = __ldg(reinterpret_cast<const float4*>(p.a.cos + row + col / 2));
-    const float4 s = __ldg(reinterpret_cast<const float4*>(p.a.sin + row + col / 2));
-    turn.c[0] = c.x, turn.c[1] = c.y, turn.c[2] = c.z, turn.c[3] = c.w;
-    turn.s[0] = s.x, turn.s[1] = s.y, turn.s[2] = s.z, turn.s[3] = s.w;
-  } else {
-    const size_t i = row + (col < R / 2 ? col : col - R / 2);
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const float4 c = __ldg(reinterpret_cast<const float4*>(p.a.cos + i) + q);
-      const float4 s = __ldg(reinterpret_cast<const float4*>(p.a.sin + i) + q);
-      turn.c[4 * q] = c.x, turn.c[4 * q + 1] = c.y, turn.c[4 * q + 2] = c.z, turn.c[4 * q + 3] = c.w;
-      turn.s[4 * q] = s.x, turn.s[4 * q + 1] = s.y, turn.s[4 * q + 2] = s.z, turn.s[4 * q + 3] = s.w;
-    }
-  }
+  const size_t i = (size_t)at * (p.a.rot / 2) + lane * 4;   // (either way of pairing: lane i has pairs 4 i .. 4 i + 3)
+  const float4 c = __ldg(reinterpret_cast<const float4*>(p.a.cos + i)), s = __ldg(reinterpret_cast<const float4*>(p.a.sin + i));
+  turn.c[0] = c.x, turn.c[1] = c.y, turn.c[2] = c.z, turn.c[3] = c.w;
+  turn.s[0] = s.x, turn.s[1] = s.y, turn.s[2] = s.z, turn.s[3] = s.w;
+  return turn;
 }
 
-// Turns a row's eight elements (sign 1), or turns them back (-1).  All lanes of the row call it.
-__device__ __forceinline__ void rotate(const NormParams& p, const Turn& turn, float sign, int col, float (&u)[8]) {
-  const int R = p.a.rot;
-  if (R == 0) return;
-  if (p.a.interleaved) {
-    if (col < R) {
+// Turns a lane's eight elements (sign 1), or turns them back (-1).
+__device__ __forceinline__ void rotate(bool interleaved, const Turn& turn, float sign, float2 (&u)[4]) {
+  if (interleaved) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float x = u[2 * i], y = u[2 * i + 1], s = sign * turn.s[i];
-        u[2 * i] = x * turn.c[i] - y * s;
-        u[2 * i + 1] = y * turn.c[i] + x * s;
-      }
-    }
+    for (int i = 0; i < 4; ++i)
+      u[i] = fma2(make_float2(-u[i].y, u[i].x), both(sign * turn.s[i]), mul2(u[i], both(turn.c[i])));
     return;
   }
-  // the pair's other element is R / 2 columns on or back, R / 16 lanes
-  const bool first = col < R / 2;
-  const int lane = threadIdx.x & 31, other = col >= R ? lane : first ? lane + R / 16 : lane - R / 16;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float o = __shfl_sync(0xffffffffu, u[e], other);
-    if (col < R) u[e] = u[e] * turn.c[e] + (first ? -o : o) * (sign * turn.s[e]);
+  for (int i = 0; i < 2; ++i) {
+    const float2 c = make_float2(turn.c[2 * i], turn.c[2 * i + 1]), s = make_float2(sign * turn.s[2 * i], sign * turn.s[2 * i + 1]);
+    const float2 x = u[i], y = u[2 + i];
+    u[i] = fma2(y, make_float2(-s.x, -s.y), mul2(x, c));
+    u[2 + i] = fma2(x, s, mul2(y, c));
   }
 }
 
@@ -158,41 +180,38 @@ __device__ __forceinline__ size_t row_offset(const tritt_rows_t& r, int b, int n
 template <typename T, int D>
 __global__ void __launch_bounds__(kNormThreads) norm_rotary_fwd_kernel(const __grid_constant__ NormParams p) {
   constexpr int L = D / 8, kSlots = kNormThreads / L;
-  const int col = threadIdx.x % L * 8;
+  const int lane = threadIdx.x % L;
+  const Cols cols = cols_of(lane, p.a.rot, p.a.interleaved);
+  const bool interleaved = p.a.interleaved;
   const long long tokens = (long long)p.a.B * p.a.T;
-  // (lanes without a row of their own stay for the shuffles)
+  // (lanes without a row of their own stay for the sums)
   const long long slot = (long long)blockIdx.x * kSlots + threadIdx.x / L;
   const long long token = slot / p.chunks;
   const bool live = token < tokens;
   const int h0 = (int)(slot % p.chunks) * kHeads;
   const int b = live ? (int)(token / p.a.T) : 0, t = live ? (int)(token % p.a.T) : 0;
   Turn turn;
-  if (live && p.a.rot) load_turn(p, b, t, col, turn);
+  if (p.a.rot) turn = load_turn(p, b, t, lane);
   for (int which = blockIdx.y; which < 3; which += gridDim.y) {
     Eight<T> in[kHeads];
+    const T* from = (const T*)p.a.x[which].p + row_offset(p.a.x[which], b, h0, t);
+    T* to = (T*)p.a.y[which].p + row_offset(p.a.y[which], b, h0, t);
 #pragma unroll
     for (int i = 0; i < kHeads; ++i)
-      if (live && h0 + i < p.a.N) in[i].load((const T*)p.a.x[which].p + row_offset(p.a.x[which], b, h0 + i, t) + col);
-    float w[8];
-    if (!p.a.weight_heads) load_weights<T>(p, which, 0, col, w);
+      if (live && h0 + i < p.a.N) in[i].load(from + i * p.a.x[which].stride_n, cols);
+    float2 w[4];
+    if (!p.a.weight_heads) load_weights<T>(p, which, 0, cols, w);
 #pragma unroll
     for (int i = 0; i < kHeads; ++i) {
       const bool on = live && h0 + i < p.a.N;
-      float u[8], sq = 0.f;
-      if (on) {
-        in[i].get(u);
-      } else {
+      float2 u[4] = {both(0.f), both(0.f), both(0.f), both(0.f)};
+      if (on) in[i].get(u);
+      const float2 r = both(rsqrtf(row_sum<L>(dot(u, u)) * (1.f / D) + p.a.eps));
+      if (p.a.weight_heads && on) load_weights<T>(p, which, h0 + i, cols, w);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) u[e] = 0.f;
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sq = fmaf(u[e], u[e], sq);
-      const float r = rsqrtf(row_sum<L>(sq) * (1.f / D) + p.a.eps);
-      if (p.a.weight_heads && on) load_weights<T>(p, which, h0 + i, col, w);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) u[e] = u[e] * r * w[e];
-      rotate(p, turn, 1.f, col, u);
-      if (on) Eight<T>::store((T*)p.a.y[which].p + row_offset(p.a.y[which], b, h0 + i, t) + col, u);
+      for (int k = 0; k < 4; ++k) u[k] = mul2(mul2(u[k], r), w[k]);
+      if (p.a.rot) rotate(interleaved, turn, 1.f, u);
+      if (on) Eight<T>::store(to + i * p.a.y[which].stride_n, cols, u);
     }
   }
 }
@@ -203,64 +222,66 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kNormThreads) norm_rotary_bwd_kernel(const __grid_constant__ NormParams p) {
   constexpr int L = D / 8, kSlots = kNormThreads / L;
   __shared__ float sums[kSlots][D];
-  const int col = threadIdx.x % L * 8, slot = threadIdx.x / L;
+  const int lane = threadIdx.x % L, slot = threadIdx.x / L;
+  const Cols cols = cols_of(lane, p.a.rot, p.a.interleaved);
+  const bool interleaved = p.a.interleaved;
   const int which = blockIdx.y / p.chunks, h0 = blockIdx.y % p.chunks * kHeads;
   const long long tokens = (long long)p.a.B * p.a.T;
   const bool weights = p.partial != nullptr && p.a.dw[which] != nullptr;
-  float dw[kHeads][8];
+  const tritt_rows_t rx = p.a.x[which], ry = p.a.y[which], rd = p.a.dx[which];
+  float2 dw[kHeads][4];
 #pragma unroll
   for (int i = 0; i < kHeads; ++i)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) dw[i][e] = 0.f;
-  float w[8];
-  if (!p.a.weight_heads) load_weights<T>(p, which, 0, col, w);
+    for (int k = 0; k < 4; ++k) dw[i][k] = both(0.f);
+  float2 w[4];
+  if (!p.a.weight_heads) load_weights<T>(p, which, 0, cols, w);
   for (long long first = (long long)blockIdx.x * kSlots; first < tokens; first += (long long)gridDim.x * kSlots) {
     const long long token = first + slot;
     const bool live = token < tokens;
-    const int b = live ? (int)(token / p.a.T) : 0, t = live ? (int)(token % p.a.T) : 0;
+    const int b = live ? (int)(token / p.a.T) : 0, t = live ? (int)(token - (long long)b * p.a.T) : 0;
     Eight<T> in[kHeads], up[kHeads];
+    const T *x0 = (const T*)rx.p + row_offset(rx, b, h0, t), *y0 = (const T*)ry.p + row_offset(ry, b, h0, t);
+    T* d0 = (T*)rd.p + row_offset(rd, b, h0, t);
 #pragma unroll
     for (int i = 0; i < kHeads; ++i)
       if (live && h0 + i < p.a.N) {
-        in[i].load((const T*)p.a.x[which].p + row_offset(p.a.x[which], b, h0 + i, t) + col);
-        up[i].load((const T*)p.a.y[which].p + row_offset(p.a.y[which], b, h0 + i, t) + col);
+        in[i].load(x0 + i * rx.stride_n, cols);
+        up[i].load(y0 + i * ry.stride_n, cols);
       }
     Turn turn;
-    if (live && p.a.rot) load_turn(p, b, t, col, turn);
+    if (p.a.rot) turn = load_turn(p, b, t, lane);
 #pragma unroll
     for (int i = 0; i < kHeads; ++i) {
       const bool on = live && h0 + i < p.a.N;
-      float x[8], g[8], sq = 0.f, dot = 0.f;
+      float2 x[4] = {both(0.f), both(0.f), both(0.f), both(0.f)}, g[4] = {both(0.f), both(0.f), both(0.f), both(0.f)};
       if (on) {
         in[i].get(x);
         up[i].get(g);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = g[e] = 0.f;
       }
-      rotate(p, turn, -1.f, col, g);
+      if (p.a.rot) rotate(interleaved, turn, -1.f, g);
+      const float r = rsqrtf(row_sum<L>(dot(x, x)) * (1.f / D) + p.a.eps);
+      if (p.a.weight_heads && on) load_weights<T>(p, which, h0 + i, cols, w);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sq = fmaf(x[e], x[e], sq);
-      const float r = rsqrtf(row_sum<L>(sq) * (1.f / D) + p.a.eps);
-      if (p.a.weight_heads && on) load_weights<T>(p, which, h0 + i, col, w);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[e] *= r;
-        if (on) dw[i][e] = fmaf(g[e], x[e], dw[i][e]);
-        g[e] *= w[e];
-        dot = fmaf(g[e], x[e], dot);
+      for (int k = 0; k < 4; ++k) {
+        x[k] = mul2(x[k], both(r));
+        if (on) dw[i][k] = fma2(g[k], x[k], dw[i][k]);
+        g[k] = mul2(g[k], w[k]);
       }
-      const float mean = row_sum<L>(dot) * (1.f / D);
+      const float mean = row_sum<L>(dot(g, x)) * (-1.f / D);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) g[e] = r * (g[e] - x[e] * mean);
-      if (on) Eight<T>::store((T*)p.a.dx[which].p + row_offset(p.a.dx[which], b, h0 + i, t) + col, g);
+      for (int k = 0; k < 4; ++k) g[k] = mul2(fma2(x[k], both(mean), g[k]), both(r));
+      if (on) Eight<T>::store(d0 + i * rd.stride_n, cols, g);
     }
   }
   if (!weights) return;
   for (int i = 0; i < kHeads && h0 + i < p.a.N; ++i) {
     __syncthreads();
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sums[slot][col + e] = dw[i][e];
+    for (int k = 0; k < 2; ++k) {
+      *reinterpret_cast<float2*>(&sums[slot][cols.a + 2 * k]) = dw[i][k];
+      *reinterpret_cast<float2*>(&sums[slot][cols.b + 2 * k]) = dw[i][2 + k];
+    }
     __syncthreads();
     for (int c = threadIdx.x; c < D; c += kNormThreads) {
       float total = 0.f;
