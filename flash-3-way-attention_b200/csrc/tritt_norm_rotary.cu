@@ -183,13 +183,11 @@ __global__ void __launch_bounds__(kNormThreads) norm_rotary_fwd_kernel(const __g
   const int lane = threadIdx.x % L;
   const Cols cols = cols_of(lane, p.a.rot, p.a.interleaved);
   const bool interleaved = p.a.interleaved;
-  const long long tokens = (long long)p.a.B * p.a.T;
-  // (lanes without a row of their own stay for the sums)
-  const long long slot = (long long)blockIdx.x * kSlots + threadIdx.x / L;
-  const long long token = slot / p.chunks;
+  // (32 bits, which the host has seen to; lanes without a row of their own stay for the sums)
+  const uint32_t tokens = (uint32_t)p.a.B * p.a.T, slot = blockIdx.x * kSlots + threadIdx.x / L, token = slot / p.chunks;
   const bool live = token < tokens;
-  const int h0 = (int)(slot % p.chunks) * kHeads;
-  const int b = live ? (int)(token / p.a.T) : 0, t = live ? (int)(token % p.a.T) : 0;
+  const int h0 = (int)(slot - token * p.chunks) * kHeads;
+  const int b = live ? token / p.a.T : 0, t = live ? token - (uint32_t)b * p.a.T : 0;
   Turn turn;
   if (p.a.rot) turn = load_turn(p, b, t, lane);
   for (int which = blockIdx.y; which < 3; which += gridDim.y) {
@@ -216,17 +214,22 @@ __global__ void __launch_bounds__(kNormThreads) norm_rotary_fwd_kernel(const __g
   }
 }
 
-// A block takes kHeads heads of one tensor and tokens blockIdx.x, + gridDim.x, ... in groups, so that the weights' gradients add up
-// in registers: then over the block's rows, and by the kernel below over the blocks, always in the same order.
+// A block takes one tensor's rows of tokens blockIdx.x, + gridDim.x, ... in groups: neighbouring slots (D / 8 lanes) kHeads heads each of a
+// token, whose rows are neighbours where the tensors come out of one projection (a block for each four heads read 1 KB here and
+// there: 98 us instead of 87 for 4 x 16 heads x 2048 x 128 bf16).  A slot's heads stay the same, so the weights' gradients add up
+// in registers: then over the block's slots, and by the kernel below over the blocks, always in the same order.
 template <typename T, int D>
-__global__ void __launch_bounds__(kNormThreads) norm_rotary_bwd_kernel(const __grid_constant__ NormParams p) {
+__global__ void __launch_bounds__(kNormThreads, 2) norm_rotary_bwd_kernel(const __grid_constant__ NormParams p) {
   constexpr int L = D / 8, kSlots = kNormThreads / L;
   __shared__ float sums[kSlots][D];
   const int lane = threadIdx.x % L, slot = threadIdx.x / L;
   const Cols cols = cols_of(lane, p.a.rot, p.a.interleaved);
   const bool interleaved = p.a.interleaved;
-  const int which = blockIdx.y / p.chunks, h0 = blockIdx.y % p.chunks * kHeads;
-  const long long tokens = (long long)p.a.B * p.a.T;
+  const int here = p.chunks < kSlots ? p.chunks : kSlots, at_once = kSlots / here;   // heads' groups of a token, tokens
+  const int groups = (p.chunks + here - 1) / here, which = blockIdx.y / groups, chunk0 = blockIdx.y % groups * here;
+  const int chunk = chunk0 + slot % here, h0 = chunk * kHeads;
+  const bool used = slot < at_once * here && chunk < p.chunks;
+  const uint32_t tokens = (uint32_t)p.a.B * p.a.T;
   const bool weights = p.partial != nullptr && p.a.dw[which] != nullptr;
   const tritt_rows_t rx = p.a.x[which], ry = p.a.y[which], rd = p.a.dx[which];
   float2 dw[kHeads][4];
@@ -236,10 +239,10 @@ __global__ void __launch_bounds__(kNormThreads) norm_rotary_bwd_kernel(const __g
     for (int k = 0; k < 4; ++k) dw[i][k] = both(0.f);
   float2 w[4];
   if (!p.a.weight_heads) load_weights<T>(p, which, 0, cols, w);
-  for (long long first = (long long)blockIdx.x * kSlots; first < tokens; first += (long long)gridDim.x * kSlots) {
-    const long long token = first + slot;
-    const bool live = token < tokens;
-    const int b = live ? (int)(token / p.a.T) : 0, t = live ? (int)(token - (long long)b * p.a.T) : 0;
+  for (uint32_t first = blockIdx.x * at_once; first < tokens; first += gridDim.x * at_once) {
+    const uint32_t token = first + slot / here;
+    const bool live = used && token < tokens;
+    const int b = live ? token / p.a.T : 0, t = live ? token - (uint32_t)b * p.a.T : 0;
     Eight<T> in[kHeads], up[kHeads];
     const T *x0 = (const T*)rx.p + row_offset(rx, b, h0, t), *y0 = (const T*)ry.p + row_offset(ry, b, h0, t);
     T* d0 = (T*)rd.p + row_offset(rd, b, h0, t);
@@ -275,7 +278,8 @@ __global__ void __launch_bounds__(kNormThreads) norm_rotary_bwd_kernel(const __g
     }
   }
   if (!weights) return;
-  for (int i = 0; i < kHeads && h0 + i < p.a.N; ++i) {
+#pragma unroll
+  for (int i = 0; i < kHeads; ++i) {
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -283,10 +287,12 @@ __global__ void __launch_bounds__(kNormThreads) norm_rotary_bwd_kernel(const __g
       *reinterpret_cast<float2*>(&sums[slot][cols.b + 2 * k]) = dw[i][2 + k];
     }
     __syncthreads();
-    for (int c = threadIdx.x; c < D; c += kNormThreads) {
+    for (int x = threadIdx.x; x < here * D; x += kNormThreads) {
+      const int c = x % D, q = x / D, head = (chunk0 + q) * kHeads + i;
+      if (head >= p.a.N) continue;
       float total = 0.f;
-      for (int s = 0; s < kSlots; ++s) total += sums[s][c];
-      p.partial[(((size_t)which * p.a.N + h0 + i) * gridDim.x + blockIdx.x) * D + c] = total;
+      for (int s = q; s < at_once * here; s += here) total += sums[s][c];
+      p.partial[(((size_t)which * p.a.N + head) * gridDim.x + blockIdx.x) * D + c] = total;
     }
   }
 }
@@ -316,12 +322,15 @@ __global__ void __launch_bounds__(1024) norm_rotary_weights_kernel(const __grid_
   }
 }
 
-// Blocks of the backward along the tokens: as many as the chip holds at once (three of 256 threads an SM) over the heads' and tensors' groups.
-int bwd_blocks(const tritt_norm_rotary_t& a) {
+// The backward's grid: blocks along the tokens, as many as the chip holds at once (two an SM), and groups of a token's heads.
+struct Grid {
+  int blocks, groups;
+};
+Grid bwd_grid(const tritt_norm_rotary_t& a) {
   const int chunks = (a.N + kHeads - 1) / kHeads, slots = kNormThreads / (a.D / 8);
-  const long long tokens = (long long)a.B * a.T, most = (tokens + slots - 1) / slots;
-  const long long fill = (3LL * kSms + 3 * chunks - 1) / (3 * chunks);
-  return (int)(most < fill ? most : fill);
+  const int here = chunks < slots ? chunks : slots, groups = (chunks + here - 1) / here, at_once = slots / here;
+  const long long most = ((long long)a.B * a.T + at_once - 1) / at_once, fill = 2LL * kSms / (3 * groups);
+  return Grid{(int)(most < fill ? most : fill < 1 ? 1 : fill), groups};
 }
 
 int check(const tritt_norm_rotary_t* a, bool backward) {
@@ -336,6 +345,10 @@ int check(const tritt_norm_rotary_t* a, bool backward) {
   if (a->dtype != TRITT_F32 && a->dtype != TRITT_F16 && a->dtype != TRITT_BF16) {
     set_error("unknown dtype code %d", a->dtype);
     return -3;
+  }
+  if ((long long)a->B * a->T > (1LL << 30) || (long long)a->B * a->T * ((a->N + kHeads - 1) / kHeads) > (1LL << 31)) {
+    set_error("too many rows for one call (B*T = %lld); split the batch", (long long)a->B * a->T);
+    return -11;
   }
   if (a->weight_dtype != TRITT_F32 && a->weight_dtype != a->dtype) {
     set_error("weights must be of the rows' type or fp32");
@@ -378,10 +391,6 @@ int check(const tritt_norm_rotary_t* a, bool backward) {
 template <typename T, int D> int launch_fwd(const NormParams& p, cudaStream_t stream) {
   constexpr int kSlots = kNormThreads / (D / 8);
   const long long slots = (long long)p.a.B * p.a.T * p.chunks, blocks = (slots + kSlots - 1) / kSlots;
-  if (blocks > 0x7fffffff) {
-    set_error("too many rows for one call");
-    return -11;
-  }
   // one tensor a block until the chip is full several times over
   const dim3 grid((unsigned)blocks, blocks >= 8LL * kSms ? 1 : 3);
   norm_rotary_fwd_kernel<T, D><<<grid, kNormThreads, 0, stream>>>(p);
@@ -391,8 +400,9 @@ template <typename T, int D> int launch_fwd(const NormParams& p, cudaStream_t st
 }
 
 template <typename T, int D> int launch_bwd(const NormParams& p, cudaStream_t stream) {
-  const int blocks = bwd_blocks(p.a);
-  norm_rotary_bwd_kernel<T, D><<<dim3(blocks, 3 * p.chunks), kNormThreads, 0, stream>>>(p);
+  const Grid grid = bwd_grid(p.a);
+  const int blocks = grid.blocks;
+  norm_rotary_bwd_kernel<T, D><<<dim3(blocks, 3 * grid.groups), kNormThreads, 0, stream>>>(p);
   count_launch();
   TRITT_CUDA_OK(cudaGetLastError());
   if (!p.partial) return 0;
@@ -433,7 +443,7 @@ int tritt_qk_norm_rotary_fwd(const tritt_norm_rotary_t* a, int* status_word, tri
 
 size_t tritt_qk_norm_rotary_workspace(const tritt_norm_rotary_t* a) {
   if (!a || a->B <= 0 || a->N <= 0 || a->T <= 0 || a->D < 16 || a->D > 256 || !wants_weights(*a)) return 0;
-  return align_up((size_t)3 * a->N * bwd_blocks(*a) * a->D * 4, 256);
+  return align_up((size_t)3 * a->N * bwd_grid(*a).blocks * a->D * 4, 256);
 }
 
 int tritt_qk_norm_rotary_bwd(const tritt_norm_rotary_t* a, void* workspace, size_t workspace_bytes, int* status_word,
