@@ -18,6 +18,7 @@ struct WriteArgs {
 
 template <typename T, int CODE, int D>
 __global__ void __launch_bounds__(kThreads) cache_write_kernel(const __grid_constant__ WriteArgs w) {
+  let_next_start();
   constexpr int L = D / 8, kSlots = kThreads / L;
   const CacheArgs& a = w.cache;
   const int col = threadIdx.x % L * 8;
@@ -98,8 +99,6 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(const __grid_const
 // One warp a row: D / 8 of its lanes hold eight elements each.  The splits' maxima and sums are looked at twice, their results once.
 template <typename T, int CODE>
 __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ JoinArgs j) {
-  // (the split kernel may still be running when this one is launched early)
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   const CacheArgs& a = j.cache;
   const int lane = threadIdx.x & 31, col = lane * 8, D = a.c.D;
   const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
@@ -172,19 +171,11 @@ template <typename T, int CODE> int read_d(const ReadArgs& r, cudaStream_t s) {
     default: return read_for<T, CODE, 256>(r, s);
   }
 }
-template <typename T, int CODE> int join_for(const JoinArgs& j, cudaStream_t stream, bool early) {
+template <typename T, int CODE> int join_for(const JoinArgs& j, cudaStream_t stream) {
   const long long rows = (long long)j.cache.c.B * j.cache.c.N * j.cache.c.n;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)((rows + 3) / 4));
-  cfg.blockDim = dim3(128);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = early ? 1 : 0;
-  TRITT_CUDA_OK(cudaLaunchKernelEx(&cfg, join_kernel<T, CODE>, j));
+  join_kernel<T, CODE><<<(unsigned)((rows + 3) / 4), 128, 0, stream>>>(j);
   count_launch();
+  TRITT_CUDA_OK(cudaGetLastError());
   return 0;
 }
 
@@ -300,8 +291,8 @@ int launch_write(const CacheArgs& a, const tritt_rows_t* rows, int dtype, int pa
   return by_type(dtype, a.c.code, [&](auto t, auto code) { return write_d<decltype(t), decltype(code)::value>(w, stream); });
 }
 
-int launch_join(const JoinArgs& j, cudaStream_t stream, bool early) {
-  return by_type(j.dtype, j.cache.c.code, [&](auto t, auto code) { return join_for<decltype(t), decltype(code)::value>(j, stream, early); });
+int launch_join(const JoinArgs& j, cudaStream_t stream) {
+  return by_type(j.dtype, j.cache.c.code, [&](auto t, auto code) { return join_for<decltype(t), decltype(code)::value>(j, stream); });
 }
 
 }  // namespace tritt
@@ -359,7 +350,7 @@ int tritt_tdp_decode(const tritt_cache_t* c, const tritt_rows_t* q, void* o, flo
   JoinArgs j{a.cache, a.part, 0, dtype, o, lse, {}};
   j.splits = a.splits = simt_decode_splits(*c);
   if (int rc = simt_tdp_decode(a, (cudaStream_t)stream)) return rc;
-  return launch_join(j, (cudaStream_t)stream, false);
+  return launch_join(j, (cudaStream_t)stream);
 }
 
 int tritt_dps_append(const tritt_cache_t* c, const tritt_rows_t* rows, int dtype, float alpha, int k_diff, void* workspace,
@@ -379,11 +370,11 @@ int tritt_dps_append(const tritt_cache_t* c, const tritt_rows_t* rows, int dtype
   const CacheArgs cache = cache_args(*c, status_word);
   if (int rc = launch_write(cache, rows, dtype, 3, (cudaStream_t)stream)) return rc;
   DpsDecodeArgs a{cache, rows[1], dtype, kPartK1, kPartV1, 0, window(k_diff), 1, alpha * kLog2e, (float*)workspace, 0};
-  if (fast(TRITT_OP_DPS_APPEND, c->D, dtype, flags)) return mma_dps_decode(a, workspace, nullptr, nullptr, &rows[3], (cudaStream_t)stream);
+  if (fast(TRITT_OP_DPS_APPEND, c->D, dtype, flags)) return mma_dps_decode(a, workspace, nullptr, nullptr, &rows[3], true, (cudaStream_t)stream);
   JoinArgs j{cache, a.part, 0, dtype, nullptr, nullptr, rows[3]};
   j.splits = a.splits = simt_decode_splits(*c);
   if (int rc = simt_dps_decode(a, (cudaStream_t)stream)) return rc;
-  return launch_join(j, (cudaStream_t)stream, false);
+  return launch_join(j, (cudaStream_t)stream);
 }
 
 int tritt_dps_decode(const tritt_cache_t* c, const tritt_rows_t* q, void* o, float* m, int dtype, float alpha, void* workspace,
@@ -399,11 +390,11 @@ int tritt_dps_decode(const tritt_cache_t* c, const tritt_rows_t* q, void* o, flo
   if (int rc = check_scratch(need, workspace, workspace_bytes)) return rc;
   const CacheArgs cache = cache_args(*c, status_word);
   DpsDecodeArgs a{cache, *q, dtype, kPartK2, kPartV2, 1, 1 << 30, 0, alpha * kLog2e, (float*)workspace, 0};
-  if (fast(TRITT_OP_DPS_DECODE, c->D, dtype, flags)) return mma_dps_decode(a, workspace, o, m, nullptr, (cudaStream_t)stream);
+  if (fast(TRITT_OP_DPS_DECODE, c->D, dtype, flags)) return mma_dps_decode(a, workspace, o, m, nullptr, false, (cudaStream_t)stream);
   JoinArgs j{cache, a.part, 0, dtype, o, m, {}};
   j.splits = a.splits = simt_decode_splits(*c);
   if (int rc = simt_dps_decode(a, (cudaStream_t)stream)) return rc;
-  return launch_join(j, (cudaStream_t)stream, false);
+  return launch_join(j, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -252,6 +252,28 @@ __device__ __forceinline__ void join_into_cache(const CacheArgs& a, int b, int h
   }
 }
 
+// ---------------------------------------------------------------- kernels one behind the other
+// A kernel that may be launched before the one ahead of it in the stream has ended (`early`): it calls wait_for_previous() before it reads or
+// writes anything; the one ahead calls let_next_start() as soon as all its blocks are on the chip.  (The launch and the start of the blocks, 2 to 3 us,
+// then lie beside the kernel ahead.)
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+template <typename K, typename P> int launch_kernel_after(K kern, dim3 grid, int threads, size_t smem, cudaStream_t stream, bool early, const P& p) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = early ? 1 : 0;
+  TRITT_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, p));
+  count_launch();
+  return 0;
+}
+
 // ---------------------------------------------------------------- parts of a row's soft-max, and what becomes of them
 // Each split of a new token's attended tokens leaves its maximum (log2 units), sum and unnormalised result in the workspace,
 // [rows][splits][D + 2] fp32 (rows = (b * N + head) * n + i), and a second kernel joins them.
@@ -263,7 +285,7 @@ struct JoinArgs {
   float* lse;         // [B, N, n] or null
   tritt_rows_t v2;    // append: W = result * v2 goes to the cache, and the log-sum-exp
 };
-int launch_join(const JoinArgs& j, cudaStream_t stream, bool early);
+int launch_join(const JoinArgs& j, cudaStream_t stream);
 int launch_write(const CacheArgs& a, const tritt_rows_t* rows, int dtype, int parts, cudaStream_t stream);
 
 // The CUDA cores' kernels (any type, fp32 arithmetic): triple dot product, and one soft-max attention over two parts of the cache.
@@ -294,7 +316,8 @@ int window_tdp_decode(const TdpDecodeArgs& a, void* o, float* lse, cudaStream_t 
 // ... the soft-max attention with warp-level matrix instructions (the same)
 bool mma_dps_decode_supported(int D, int dtype);
 size_t mma_dps_decode_workspace(const tritt_cache_t& c);
-int mma_dps_decode(const DpsDecodeArgs& a, void* workspace, void* o, float* lse, const tritt_rows_t* v2, cudaStream_t stream);
+// (early: the kernel ahead in the stream is launch_write's)
+int mma_dps_decode(const DpsDecodeArgs& a, void* workspace, void* o, float* lse, const tritt_rows_t* v2, bool early, cudaStream_t stream);
 
 int simt_decode_splits(const tritt_cache_t& c);
 int simt_tdp_decode(const TdpDecodeArgs& a, cudaStream_t stream);

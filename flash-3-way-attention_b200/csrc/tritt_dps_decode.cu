@@ -48,6 +48,7 @@ struct Params {
   LineEntry* table;      // [B]
   float* part;           // [pieces][Q][D + 2]
   int ctas;
+  bool early;
 };
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -131,6 +132,8 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm<NT>) dps_decode_kern
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   uint8_t* ring = ring_all + warp * NS * S::kStage;
   uint64_t* full = s_full[warp];
+  wait_for_previous();
+  let_next_start();
   if (lane == 0) {
     for (int i = 0; i < NS; ++i) mbar_init(&full[i], 33);   // one arrival with the bulk copies' bytes, one of each lane
     fence_barrier_init();
@@ -609,7 +612,7 @@ struct DpsJoinParams {
 // One warp a row where a row has few pieces, else four that take its pieces in turn; D / 8 of a warp's lanes hold eight elements each.
 template <typename T, int CODE, int W>
 __global__ void __launch_bounds__(128) dps_join_kernel(const __grid_constant__ DpsJoinParams j) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  wait_for_previous();
   __shared__ float sm[4], sl[4], so[4][256];
   const CacheArgs& ca = j.a.cache;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = lane * 8, D = ca.c.D;
@@ -692,10 +695,7 @@ template <int D, int CODE, int NT, bool ONE, bool EXACT> int launch_kernel(Param
   constexpr int kSmem = smem_bytes<D, CODE, NT>();
   TRITT_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
   p.ctas = ctas = num_sms() * kBlocksPerSm<NT>;
-  kern<<<ctas, kWarps * 32, kSmem, stream>>>(p);
-  count_launch();
-  TRITT_CUDA_OK(cudaGetLastError());
-  return 0;
+  return launch_kernel_after(kern, dim3(ctas), kWarps * 32, kSmem, stream, p.early, p);
 }
 template <int D, int CODE, int NT> int launch(const Params& p, cudaStream_t stream, int& ctas) {
   if constexpr (NT == 1) {
@@ -723,12 +723,8 @@ template <typename T, int CODE> int launch_dps_join(const DpsJoinParams& j, cuda
   const long long rows = (long long)j.a.cache.c.B * j.a.cache.c.N * j.a.cache.c.n;
   // (pieces of a row: about ctas / rows and one more; four warps share more than two)
   if (rows * 2 < j.ctas)
-    dps_join_kernel<T, CODE, 4><<<(unsigned)rows, 128, 0, stream>>>(j);
-  else
-    dps_join_kernel<T, CODE, 1><<<(unsigned)((rows + 3) / 4), 128, 0, stream>>>(j);
-  count_launch();
-  TRITT_CUDA_OK(cudaGetLastError());
-  return 0;
+    return launch_kernel_after(dps_join_kernel<T, CODE, 4>, dim3((unsigned)rows), 128, 0, stream, true, j);
+  return launch_kernel_after(dps_join_kernel<T, CODE, 1>, dim3((unsigned)((rows + 3) / 4)), 128, 0, stream, true, j);
 }
 template <typename T> int join_by_code(const DpsJoinParams& j, cudaStream_t s) {
   const int code = j.a.cache.c.code;
@@ -745,10 +741,10 @@ size_t mma_dps_decode_workspace(const tritt_cache_t& c) {
   return table_bytes(c) + align_up((size_t)((long long)c.B * c.N * plan.groups + 4 * num_sms()) * 8 * plan.tiles * (c.D + 2) * 4, 256);
 }
 
-int mma_dps_decode(const DpsDecodeArgs& a, void* workspace, void* o, float* lse, const tritt_rows_t* v2, cudaStream_t stream) {
+int mma_dps_decode(const DpsDecodeArgs& a, void* workspace, void* o, float* lse, const tritt_rows_t* v2, bool early, cudaStream_t stream) {
   const tritt_cache_t& c = a.cache.c;
   const Plan plan = plan_of(c.n, c.D);
-  const Params p{a, (LineEntry*)workspace, (float*)((char*)workspace + table_bytes(c)), 0};
+  const Params p{a, (LineEntry*)workspace, (float*)((char*)workspace + table_bytes(c)), 0, early};
   int ctas = 0;
   if (int rc = c.D == 64 ? by_code<64>(p, plan.tiles, stream, ctas) : by_code<128>(p, plan.tiles, stream, ctas)) return rc;
   const DpsJoinParams j{a, p.table, p.part, ctas, 8 * plan.tiles, o, lse, v2 ? *v2 : tritt_rows_t{}};

@@ -308,6 +308,7 @@ __global__ void __launch_bounds__(1024) norm_rotary_weights_kernel(const __grid_
   const float* base = p.partial + ((size_t)which * p.a.N + head) * blocks * D;
   float total = 0.f;
   if (c < D)
+#pragma unroll 8
     for (int i = group; i < rows; i += 32) total += base[(size_t)i * D + c];
   sums[group][threadIdx.x % 32] = total;
   __syncthreads();

@@ -464,6 +464,7 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
     }
     if (lane == 0) ms.total = total;
   }
+  let_next_start();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -943,7 +944,7 @@ __device__ __noinline__ long long cta_of(long long x, long long total, int ctas)
 // results, whose weights no load waits for, and the warps' are added in order.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) tdp_join_kernel(const __grid_constant__ TdpJoinParams j) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  wait_for_previous();
   __shared__ float s_top[8], s_sum[8], so[8][D];
   __shared__ long long s_id[256];
   __shared__ int s_pieces[256];
@@ -1040,16 +1041,8 @@ int launch(const Params& p, const TdpJoinParams& j, cudaStream_t stream) {
     return -30;
   }
   TRITT_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmem));
-  kern<<<p.ctas, kThreads, Cfg<D>::kSmem, stream>>>(p);
-  count_launch();
-  TRITT_CUDA_OK(cudaGetLastError());
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)((long long)p.a.cache.c.B * p.a.cache.c.N * p.a.cache.c.n));
-  cfg.blockDim = dim3(256);
-  cfg.stream = stream;
-  TRITT_CUDA_OK(cudaLaunchKernelEx(&cfg, tdp_join_kernel<T16, D>, j));
-  count_launch();
-  return 0;
+  if (int rc = launch_kernel_after(kern, dim3(p.ctas), kThreads, Cfg<D>::kSmem, stream, false, p)) return rc;
+  return launch_kernel_after(tdp_join_kernel<T16, D>, dim3((unsigned)((long long)p.a.cache.c.B * p.a.cache.c.N * p.a.cache.c.n)), 256, 0, stream, true, j);
 }
 
 template <typename T16> int by_size(const Params& p, const TdpJoinParams& j, cudaStream_t s) {
