@@ -609,6 +609,12 @@ struct DpsJoinParams {
   tritt_rows_t v2;       // append: W = result * v2 goes to the cache, and the log-sum-exp
 };
 
+// The CTA of a step.
+__device__ __forceinline__ int cta_of(long long x, long long total, int parts) {
+  if (total < 1 << 20) return (int)(((uint32_t)(x + 1) * (uint32_t)parts - 1) / (uint32_t)total);   // (a division of 64 bits is long)
+  return (int)(((x + 1) * parts - 1) / total);
+}
+
 // One warp a row where a row has few pieces, else four that take its pieces in turn; D / 8 of a warp's lanes hold eight elements each.
 template <typename T, int CODE, int W>
 __global__ void __launch_bounds__(128) dps_join_kernel(const __grid_constant__ DpsJoinParams j) {
@@ -627,20 +633,41 @@ __global__ void __launch_bounds__(128) dps_join_kernel(const __grid_constant__ D
   for (int k = 0; k < 8; ++k) f[k] = 0.f;
   if (i < e.line.cnt) {
     const long long grp = (long long)head * e.line.groups + i / j.queries, first = e.base + grp * e.line.tiles;
-    // CTA c has the steps from c total / parts to the next one's
-    const long long c0 = ((first + 1) * parts - 1) / total, c1 = ((first + e.line.tiles) * parts - 1) / total;
-    for (long long c = c0 + (W == 1 ? 0 : warp); c <= c1; c += W) {
-      const float* p = j.part + ((size_t)(e.group_base + grp + c) * j.queries + i % j.queries) * (D + 2);
-      const float mp = p[0], lp = p[1];
-      if (mp == -INFINITY && lp == 0.f) continue;   // (its result is not written)
-      const float mn = fmaxf(m, mp), w0 = m == -INFINITY ? 0.f : exp2f(m - mn), w1 = mp == -INFINITY ? 1.f : exp2f(mp - mn);
-      l = l * w0 + lp * w1;
-      if (col < D) {
+    // CTA c has the steps from c total / parts to the next one's.  A lane looks at a piece's maximum and sum; then the results are added
+    // up, four pieces' loads in flight
+    const int c0 = cta_of(first, total, parts), count = cta_of(first + e.line.tiles - 1, total, parts) - c0 + 1;
+    const float* part = j.part + ((size_t)(e.group_base + grp + c0) * j.queries + i % j.queries) * (D + 2);
+    const size_t pitch = (size_t)j.queries * (D + 2);
+    for (int k0 = W == 1 ? 0 : warp * 32; k0 < count; k0 += 32 * W) {
+      const int mine = k0 + lane, here = count - k0 < 32 ? count - k0 : 32;
+      float mp = -INFINITY, lp = 0.f;
+      if (mine < count) mp = part[mine * pitch], lp = part[mine * pitch + 1];
+      float mn = fmaxf(m, mp);
 #pragma unroll
-        for (int k = 0; k < 8; k += 2) {
-          const float2 v = *reinterpret_cast<const float2*>(p + 2 + col + k);
-          f[k] = f[k] * w0 + v.x * w1;
-          f[k + 1] = f[k + 1] * w0 + v.y * w1;
+      for (int o = 16; o > 0; o >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+      const float w0 = m == -INFINITY ? 0.f : exp2f(m - mn);
+      // (a piece that has seen nothing has written no result; a maximum of -infinity with a sum of NaN is of a row that reads as NaN)
+      const float w1 = mp == -INFINITY ? 0.f : exp2f(mp - mn);
+      float add = mp == -INFINITY ? (lp != lp ? lp : 0.f) : lp * w1;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) add += __shfl_xor_sync(0xffffffffu, add, o);
+      l = (m == -INFINITY && l == 0.f ? 0.f : l * w0) + add;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) f[k] *= w0;
+#pragma unroll 1
+      for (int q = 0; q < here; q += 4) {
+        float2 v[4][4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            v[u][k] = q + u < here && col < D ? *reinterpret_cast<const float2*>(part + (k0 + q + u) * pitch + 2 + col + 2 * k) : make_float2(0.f, 0.f);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const float w = __shfl_sync(0xffffffffu, w1, (q + u) & 31);
+          if (q + u >= here || w == 0.f) continue;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) f[2 * k] = fmaf(v[u][k].x, w, f[2 * k]), f[2 * k + 1] = fmaf(v[u][k].y, w, f[2 * k + 1]);
         }
       }
       m = mn;
@@ -721,8 +748,8 @@ template <int D> int by_code(const Params& p, int tiles, cudaStream_t stream, in
 
 template <typename T, int CODE> int launch_dps_join(const DpsJoinParams& j, cudaStream_t stream) {
   const long long rows = (long long)j.a.cache.c.B * j.a.cache.c.N * j.a.cache.c.n;
-  // (pieces of a row: about ctas / rows and one more; four warps share more than two)
-  if (rows * 2 < j.ctas)
+  // (a row has about ctas / groups of new tokens pieces and one more; four warps share more than 64 of them)
+  if (rows / j.a.cache.c.n * 64 < j.ctas)
     return launch_kernel_after(dps_join_kernel<T, CODE, 4>, dim3((unsigned)rows), 128, 0, stream, true, j);
   return launch_kernel_after(dps_join_kernel<T, CODE, 1>, dim3((unsigned)((rows + 3) / 4)), 128, 0, stream, true, j);
 }

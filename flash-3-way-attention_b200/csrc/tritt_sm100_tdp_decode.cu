@@ -940,14 +940,15 @@ __device__ __noinline__ long long cta_of(long long x, long long total, int ctas)
   return ((x + 1) * ctas - 1) / total;
 }
 
-// One block a row.  A thread finds a group's pieces, whose maxima give the row's, 256 groups at a time; then the warps add up the groups'
-// results, whose weights no load waits for, and the warps' are added in order.
+// One block a row.  A thread finds the pieces of a group, 256 groups at a time, and their places form a line in shared memory; the line's maxima give
+// the row's, and the warps add up the results, four loads in flight; then the warps' sums are added in order.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) tdp_join_kernel(const __grid_constant__ TdpJoinParams j) {
   wait_for_previous();
+  constexpr int kLine = 1024;   // pieces at a time
   __shared__ float s_top[8], s_sum[8], so[8][D];
-  __shared__ long long s_id[256];
-  __shared__ int s_pieces[256];
+  __shared__ long long s_line[kLine];   // number of a piece's group among all results
+  __shared__ int s_count[8];
   const CacheArgs& ca = j.a.cache;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const long long row = blockIdx.x;
@@ -955,60 +956,87 @@ __global__ void __launch_bounds__(256) tdp_join_kernel(const __grid_constant__ T
   const LineEntry e = j.table[b], end = j.table[ca.c.B - 1];
   const long long total = end.base + (long long)end.line.pairs * end.line.slabs * ca.c.N;
   constexpr int E = D / 32;
-  float top = -INFINITY, sum = 0.f, acc[E];   // of this warp's groups
+  float top = -INFINITY, sum = 0.f, acc[E];   // of this warp's pieces
 #pragma unroll
   for (int k = 0; k < E; ++k) acc[k] = 0.f;
   const int groups = i < e.line.cnt ? e.line.groups : 0;
   for (int g0 = 0; g0 < groups; g0 += 256) {
-    float m = -INFINITY;
-    __syncthreads();
+    // this thread's group: its pieces are those of the CTAs that have steps of its pair
+    long long first = 0, id = 0;
+    int pieces = 0;
     if (g0 + tid < groups) {
       const int g = i * e.line.groups + g0 + tid;
-      const long long pair = (long long)head * e.line.pairs + g / 8, first = e.base + pair * e.line.slabs, last = first + e.line.slabs - 1;
-      const long long id = (e.pair_base + pair) * 8 + g % 8;
-      long long c;
-      int pieces = 0;
-      for (long long x = first; x <= last;) {
-        c = cta_of(x, total, j.ctas);
-        x = behind_cta(c, total, j.ctas);
-        m = fmaxf(m, j.part[(size_t)(id + c * 8) * (D + 2)]);
-        if (pieces++ == 0) s_id[tid] = c;
-      }
-      s_pieces[tid] = pieces;
+      const long long pair = (long long)head * e.line.pairs + g / 8;
+      first = e.base + pair * e.line.slabs;
+      id = (e.pair_base + pair) * 8 + g % 8;
+      for (long long x = first; x < first + e.line.slabs; ++pieces) x = behind_cta(cta_of(x, total, j.ctas), total, j.ctas);
     }
+    int at = pieces;   // its place in the line: the pieces before it
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (lane == 0) s_top[warp] = m;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, at, o);
+      if (lane >= o) at += v;
+    }
     __syncthreads();
-    float now = top;
+    if (lane == 31) s_count[warp] = at;
+    __syncthreads();
+    at -= pieces;
+    int all = 0;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) now = fmaxf(now, s_top[w]);
-    const float w0 = top == -INFINITY ? 0.f : exp2f(top - now);
-    sum *= top == -INFINITY && sum != sum ? 1.f : w0;
+    for (int w = 0; w < 8; ++w) {
+      if (w < warp) at += s_count[w];
+      all += s_count[w];
+    }
+    for (int l0 = 0; l0 < all; l0 += kLine) {
+      __syncthreads();
+      {
+        long long x = first;
+        for (int k = 0; k < pieces; ++k) {
+          const long long c = cta_of(x, total, j.ctas);
+          if (at + k >= l0 && at + k < l0 + kLine) s_line[at + k - l0] = id + c * 8;
+          x = behind_cta(c, total, j.ctas);
+        }
+      }
+      __syncthreads();
+      const int here = all - l0 < kLine ? all - l0 : kLine;
+      float m = -INFINITY;
+      for (int k = tid; k < here; k += 256) m = fmaxf(m, j.part[(size_t)s_line[k] * (D + 2)]);
 #pragma unroll
-    for (int k = 0; k < E; ++k) acc[k] *= w0;
-    top = now;
-    const int here = groups - g0 < 256 ? groups - g0 : 256;
+      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      if (lane == 0) s_top[warp] = m;
+      __syncthreads();
+      float now = top;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) now = fmaxf(now, s_top[w]);
+      const float w0 = top == -INFINITY ? 0.f : exp2f(top - now);
+      sum *= top == -INFINITY && sum != sum ? 1.f : w0;
+#pragma unroll
+      for (int k = 0; k < E; ++k) acc[k] *= w0;
+      top = now;
 #pragma unroll 1
-    for (int t = warp; t < here; t += 8) {
-      const int g = i * e.line.groups + g0 + t;
-      const long long pair = (long long)head * e.line.pairs + g / 8, id = (e.pair_base + pair) * 8 + g % 8;
-      long long c = s_id[t];
-      for (int k = s_pieces[t]; k > 0; --k) {
-        const float* p = j.part + (size_t)(id + c * 8) * (D + 2);
-        const float mp = p[0], lp = p[1];
-        float v[E];
+      for (int k0 = warp; k0 < here; k0 += 32) {
+        float mp[4], lp[4], v[4][E];
 #pragma unroll
-        for (int q = 0; q < E; ++q) v[q] = p[2 + q * 32 + lane];
-        // (a group that has seen nothing has written no result; a maximum of -infinity with a sum of NaN is a row that reads as NaN)
-        const float w = mp == -INFINITY ? 0.f : exp2f(mp - top);
-        sum += mp == -INFINITY ? (lp != lp ? lp : 0.f) : lp * w;
+        for (int u = 0; u < 4; ++u) {
+          const int k = k0 + u * 8;
+          const float* p = j.part + (size_t)s_line[k < here ? k : k0] * (D + 2);
+          mp[u] = k < here ? p[0] : -INFINITY;
+          lp[u] = k < here ? p[1] : 0.f;
 #pragma unroll
-        for (int q = 0; q < E; ++q) acc[q] += w == 0.f ? 0.f : v[q] * w;
-        if (k > 1) c = cta_of(behind_cta(c, total, j.ctas), total, j.ctas);   // (with fewer steps than CTAs not every CTA has one)
+          for (int q = 0; q < E; ++q) v[u][q] = p[2 + q * 32 + lane];
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          // (a group that has seen nothing has written no result; a maximum of -infinity with a sum of NaN is of a row that reads as NaN)
+          const float w = mp[u] == -INFINITY ? 0.f : exp2f(mp[u] - top);
+          sum += mp[u] == -INFINITY ? (lp[u] != lp[u] ? lp[u] : 0.f) : lp[u] * w;
+#pragma unroll
+          for (int q = 0; q < E; ++q) acc[q] += w == 0.f ? 0.f : v[u][q] * w;
+        }
       }
     }
   }
+  __syncthreads();
   if (lane == 0) s_sum[warp] = sum;
 #pragma unroll
   for (int k = 0; k < E; ++k) so[warp][k * 32 + lane] = acc[k];
