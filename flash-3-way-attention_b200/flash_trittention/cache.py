@@ -157,6 +157,11 @@ def _need_lse(cache):
 def cache_write(cache: TrittentionCache, table: Tensor, context: Tensor, k1: Tensor, k2: Tensor, v1: Tensor, v2: Tensor,
                 counts: Optional[Tensor] = None) -> None:
     """Quantises the new tokens' rows of K1, K2, SiLU(V1) and V2 into their places (``v1`` is the raw tensor); nothing else changes."""
+    if torch.compiler.is_compiling():
+        from . import ops
+
+        _cache(cache)
+        return ops.cache_write(cache.codes, cache.exponents, table, context, counts, k1, k2, v1, v2)
     done = _native.host_cache_write(*_cache(cache), table, context, counts, None, k1, k2, v1, v2)
     if done is not None:
         _native.host_result(done, "tritt_cache_write")
@@ -170,6 +175,10 @@ def cache_read(cache: TrittentionCache, table: Tensor, context: Tensor, n: int, 
                counts: Optional[Tensor] = None) -> Tuple[Tensor, ...]:
     """``n`` tokens of each sequence from token ``context[b]`` on, read back: the four parts ``[B, N, n, D]`` in ``dtype`` and, of a
     dot-product-sum cache, the log-sum-exps ``[B, N, n]``.  Zeros for tokens past ``counts[b]``."""
+    if torch.compiler.is_compiling():
+        from . import ops
+
+        return tuple(ops.cache_read(*_cache(cache), table, context, n, dtype, counts))
     out = _native.host_cache_read(*_cache(cache), table, context, counts, None, n, _native.dtype_code(dtype))
     if out is not None:
         return _native.host_result(out, "tritt_cache_read")
@@ -194,6 +203,13 @@ def tdp_decode(q: Tensor, cache: TrittentionCache, table: Tensor, context: Tenso
     cores.  No gradient flows through the cache.
     """
     flags, softmax_scale = _flags(input_precision), float(softmax_scale)
+    if torch.compiler.is_compiling():
+        from . import ops
+
+        _cache(cache)
+        o, lse = ops.tdp_decode(q, cache.codes, cache.exponents, table, context, softmax_scale, k1_window, k2_window, kk_left, kk_right, counts,
+                                ancestors, input_precision)
+        return (o, lse) if return_lse else o
     out = _native.host_decode(_native.OP_TDP_DECODE, *_cache(cache), table, context, counts, ancestors, flags, softmax_scale, q, k1_window,
                               k2_window, kk_left, kk_right, bool(return_lse))
     if out is not None:
@@ -217,6 +233,11 @@ def dps_append(cache: TrittentionCache, table: Tensor, context: Tensor, k1: Tens
     with ``position(t) - position(s) <= k_diff``, the row ``W = softmax(softmax_scale * k1[s].k2[t]) SiLU(v1[s]) * v2[t]`` and the
     log-sum-exp.  These do not depend on a query and are computed once.  Kernels as for ``tdp_decode``."""
     flags, softmax_scale = _flags(input_precision), float(softmax_scale)
+    if torch.compiler.is_compiling():
+        from . import ops
+
+        _need_lse(_cache(cache))
+        return ops.dps_append(*cache, table, context, k1, k2, v1, v2, softmax_scale, k_diff, counts, ancestors, input_precision)
     done = _native.host_decode(_native.OP_DPS_APPEND, *_cache(cache), table, context, counts, ancestors, flags, softmax_scale, k1, k2, v1, v2,
                                k_diff)
     if done is not None:
@@ -236,6 +257,11 @@ def dps_decode(q: Tensor, cache: TrittentionCache, table: Tensor, context: Tenso
     """Dot-product-sum attention of new tokens that ``dps_append`` has written: ``(o [B, N, n, D], m [B, N, n] fp32 log-sum-exp)``, as the module
     ``TrittentionTriton`` returns them.  Rows past ``counts[b]`` or of a free slot are 0 and ``-inf``.  Kernels as for ``tdp_decode``."""
     flags, softmax_scale = _flags(input_precision), float(softmax_scale)
+    if torch.compiler.is_compiling():
+        from . import ops
+
+        _need_lse(_cache(cache))
+        return ops.dps_decode(q, *cache, table, context, softmax_scale, counts, ancestors, input_precision)
     out = _native.host_decode(_native.OP_DPS_DECODE, *_cache(cache), table, context, counts, ancestors, flags, softmax_scale, q)
     if out is not None:
         return _native.host_result(out, "tritt_dps_decode")

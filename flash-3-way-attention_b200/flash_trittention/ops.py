@@ -13,18 +13,28 @@ one opaque node and needs no graph break.  ``flash_trittention()`` switches to t
 is being compiled; ``TrittentionTDP`` is a module for the triple-dot-product variant with the constructor /
 ``forward`` conventions of the reference's ``TrittentionTriton`` (returns ``(o, lse)``).
 
+What stands beside the attention, for which the reference has no counterpart, is registered in the same way, and
+its functions switch to these operators while they are compiled:
+
+    norm_rotary / norm_rotary_bwd                      (norms with the position rotation)
+    cache_write / cache_read / tdp_decode /
+    dps_append / dps_decode                            (the paged cache; the writes change their arguments)
+
 Importing this module does not load the CUDA library; the operators do, on their first call, and raise if it is
 missing (there is no CPU implementation behind them).
 """
-from typing import Optional, Tuple
+from typing import List, Optional, Tuple
 
 import torch
 import torch.nn as nn
 from torch import Tensor
 
 from . import _native
+from . import cache as _cache
+from . import norm_rotary as _norm_rotary
 
-__all__ = ["tdp_fwd", "tdp_bwd", "dps_fwd", "dps_bwd", "tdp_attention", "dps_attention", "TrittentionTDP"]
+__all__ = ["tdp_fwd", "tdp_bwd", "dps_fwd", "dps_bwd", "tdp_attention", "dps_attention", "TrittentionTDP", "norm_rotary", "norm_rotary_bwd",
+           "cache_write", "cache_read", "tdp_decode", "dps_append", "dps_decode"]
 
 
 def _check_inputs(q, k1, k2, v1, v2):
@@ -172,6 +182,122 @@ dps_fwd.register_autograd(_dps_backward, setup_context=_dps_setup)
 def dps_attention(q, k1, k2, v1, v2, softmax_scale=1 / 8, causal=True, k_diff=1024, convert_to_float32=False):
     """Differentiable dot-product-sum trittention through the registered operators: ``(o, m)``."""
     return dps_fwd(q, k1, k2, v1, v2, float(softmax_scale), bool(causal), int(k_diff), bool(convert_to_float32))
+
+
+# ------------------------------------------------------------------ norms with rotation
+
+@torch.library.custom_op("flash_trittention::norm_rotary", mutates_args=(), device_types="cuda")
+def norm_rotary(q: Tensor, k1: Tensor, k2: Tensor, q_weight: Optional[Tensor], k1_weight: Optional[Tensor], k2_weight: Optional[Tensor],
+                cos: Optional[Tensor], sin: Optional[Tensor], positions: Optional[Tensor], eps: float,
+                interleaved: bool) -> Tuple[Tensor, Tensor, Tensor]:
+    """The three results of ``qk_norm_rotary``."""
+    return _norm_rotary.norm_rotary_forward((q, k1, k2), (q_weight, k1_weight, k2_weight), cos, sin, positions, eps, interleaved)
+
+
+@norm_rotary.register_fake
+def _(q, k1, k2, q_weight, k1_weight, k2_weight, cos, sin, positions, eps, interleaved):
+    _norm_rotary._check((q, k1, k2), (q_weight, k1_weight, k2_weight), cos, sin, positions)
+    return tuple(torch.empty(q.shape, dtype=q.dtype, device=q.device) for _ in range(3))
+
+
+@torch.library.custom_op("flash_trittention::norm_rotary_bwd", mutates_args=(), device_types="cuda")
+def norm_rotary_bwd(q: Tensor, k1: Tensor, k2: Tensor, q_weight: Optional[Tensor], k1_weight: Optional[Tensor], k2_weight: Optional[Tensor],
+                    cos: Optional[Tensor], sin: Optional[Tensor], positions: Optional[Tensor], eps: float, interleaved: bool, d_q: Tensor,
+                    d_k1: Tensor, d_k2: Tensor, weights_too: List[bool]) -> List[Tensor]:
+    """``[dq, dk1, dk2]`` and the gradients of the weights that are wanted, in order."""
+    out = _norm_rotary.norm_rotary_backward((q, k1, k2), (q_weight, k1_weight, k2_weight), cos, sin, positions, eps, interleaved,
+                                            tuple(d.to(q.dtype) for d in (d_q, d_k1, d_k2)), tuple(weights_too))
+    return [g for g in out if g is not None]
+
+
+@norm_rotary_bwd.register_fake
+def _(q, k1, k2, q_weight, k1_weight, k2_weight, cos, sin, positions, eps, interleaved, d_q, d_k1, d_k2, weights_too):
+    return [torch.empty_like(x) for x in (q, k1, k2)] + [
+        torch.empty(w.shape, dtype=w.dtype, device=w.device) for w, want in zip((q_weight, k1_weight, k2_weight), weights_too)
+        if w is not None and want]
+
+
+def _norm_rotary_setup(ctx, inputs, output):
+    ctx.save_for_backward(*inputs[:9])
+    ctx.rest = tuple(inputs[9:])
+
+
+def _norm_rotary_backward(ctx, *dys):
+    wanted = [bool(w is not None and need) for w, need in zip(ctx.saved_tensors[3:6], ctx.needs_input_grad[3:6])]
+    out = norm_rotary_bwd(*ctx.saved_tensors, *ctx.rest, *dys, wanted)
+    weights = iter(out[3:])
+    return (*out[:3], *(next(weights) if w else None for w in wanted), None, None, None, None, None)
+
+
+norm_rotary.register_autograd(_norm_rotary_backward, setup_context=_norm_rotary_setup)
+
+
+# ------------------------------------------------------------------ the paged cache
+
+@torch.library.custom_op("flash_trittention::cache_write", mutates_args=("codes", "exponents"), device_types="cuda")
+def cache_write(codes: Tensor, exponents: Tensor, table: Tensor, context: Tensor, counts: Optional[Tensor], k1: Tensor, k2: Tensor, v1: Tensor,
+                v2: Tensor) -> None:
+    _cache.cache_write(_cache.TrittentionCache(codes, exponents), table, context, k1, k2, v1, v2, counts)
+
+
+@cache_write.register_fake
+def _(codes, exponents, table, context, counts, k1, k2, v1, v2):
+    return None
+
+
+@torch.library.custom_op("flash_trittention::cache_read", mutates_args=(), device_types="cuda")
+def cache_read(codes: Tensor, exponents: Tensor, lse: Optional[Tensor], table: Tensor, context: Tensor, n: int, dtype: torch.dtype,
+               counts: Optional[Tensor]) -> List[Tensor]:
+    return list(_cache.cache_read(_cache.TrittentionCache(codes, exponents, lse), table, context, n, dtype, counts))
+
+
+@cache_read.register_fake
+def _(codes, exponents, lse, table, context, n, dtype, counts):
+    shape = (table.shape[0], codes.shape[2], n)
+    parts = [torch.empty(*shape, codes.shape[4], dtype=dtype, device=codes.device) for _ in range(4)]
+    return parts if lse is None else parts + [torch.empty(shape, dtype=torch.float32, device=codes.device)]
+
+
+def _like_queries(q):
+    return torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
+
+
+@torch.library.custom_op("flash_trittention::tdp_decode", mutates_args=(), device_types="cuda")
+def tdp_decode(q: Tensor, codes: Tensor, exponents: Tensor, table: Tensor, context: Tensor, softmax_scale: float, k1_window: Optional[int],
+               k2_window: Optional[int], kk_left: Optional[int], kk_right: Optional[int], counts: Optional[Tensor],
+               ancestors: Optional[Tensor], input_precision: Optional[str]) -> Tuple[Tensor, Tensor]:
+    """``(o, lse)``."""
+    return _cache.tdp_decode(q, _cache.TrittentionCache(codes, exponents), table, context, softmax_scale, k1_window, k2_window, kk_left, kk_right,
+                             counts, ancestors, True, input_precision)
+
+
+@tdp_decode.register_fake
+def _(q, codes, exponents, table, context, softmax_scale, k1_window, k2_window, kk_left, kk_right, counts, ancestors, input_precision):
+    return _like_queries(q)
+
+
+@torch.library.custom_op("flash_trittention::dps_append", mutates_args=("codes", "exponents", "lse"), device_types="cuda")
+def dps_append(codes: Tensor, exponents: Tensor, lse: Tensor, table: Tensor, context: Tensor, k1: Tensor, k2: Tensor, v1: Tensor, v2: Tensor,
+               softmax_scale: float, k_diff: int, counts: Optional[Tensor], ancestors: Optional[Tensor], input_precision: Optional[str]) -> None:
+    _cache.dps_append(_cache.TrittentionCache(codes, exponents, lse), table, context, k1, k2, v1, v2, softmax_scale, k_diff, counts, ancestors,
+                      input_precision)
+
+
+@dps_append.register_fake
+def _(codes, exponents, lse, table, context, k1, k2, v1, v2, softmax_scale, k_diff, counts, ancestors, input_precision):
+    return None
+
+
+@torch.library.custom_op("flash_trittention::dps_decode", mutates_args=(), device_types="cuda")
+def dps_decode(q: Tensor, codes: Tensor, exponents: Tensor, lse: Tensor, table: Tensor, context: Tensor, softmax_scale: float,
+               counts: Optional[Tensor], ancestors: Optional[Tensor], input_precision: Optional[str]) -> Tuple[Tensor, Tensor]:
+    """``(o, m)``."""
+    return _cache.dps_decode(q, _cache.TrittentionCache(codes, exponents, lse), table, context, softmax_scale, counts, ancestors, input_precision)
+
+
+@dps_decode.register_fake
+def _(q, codes, exponents, lse, table, context, softmax_scale, counts, ancestors, input_precision):
+    return _like_queries(q)
 
 
 # ------------------------------------------------------------------ module

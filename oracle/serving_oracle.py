@@ -83,7 +83,26 @@ def tdp_row(q, k1, k2, v1, v2, ctx, i, alpha, windows=(None, None, None, None), 
     size = abs(alpha) * torch.einsum("d,jd,kd->jk", q.abs(), k1[rows].abs(), k2[rows].abs())
     pj, pk = pos[:, None], pos[None]
     seen = (at - pj <= k1w) & (at - pk <= k2w) & (pk - pj <= kkl) & (pj - pk <= kkr)
-    return _finish(s, size, seen, torch.einsum("jd,kd->jkd", v1[rows], v2[rows]))
+    if not bool(seen.any()):
+        return _nothing(q)
+    s = s.masked_fill(~seen, -math.inf)
+    lse = s.flatten().logsumexp(0)
+    p = (s - lse).exp()
+    v1, v2 = v1[rows], v2[rows]
+    o, mass = (v1 * (p @ v2)).sum(0), (v1.abs() * (p @ v2.abs())).sum(0)
+    return o, lse, mass, size[seen].max()
+
+
+def tdp_small(q, k1, k2, v1, v2, ctx, i, alpha, windows, ancestors, below):
+    """Sum of |v1 v2| over the attended pairs of ``tdp_row`` whose p is less than ``below`` times the largest, times the largest p."""
+    k1w, k2w, kkl, kkr = (1 << 40 if w is None else w for w in windows)
+    rows, pos, at = _tokens(ctx, i, ancestors)
+    s = alpha * torch.einsum("d,jd,kd->jk", q, k1[rows], k2[rows])
+    pj, pk = pos[:, None], pos[None]
+    s = s.masked_fill(~((at - pj <= k1w) & (at - pk <= k2w) & (pk - pj <= kkl) & (pj - pk <= kkr)), -math.inf)
+    top = s.max()
+    small = ((s < top + math.log(below)) & (s > -math.inf)).double()
+    return (top - s.flatten().logsumexp(0)).exp() * (v1[rows].abs() * (small @ v2[rows].abs())).sum(0)
 
 
 def dps_row(q, key, value, bias, ctx, i, alpha, window=None, ancestors=None):
@@ -97,10 +116,14 @@ def dps_row(q, key, value, bias, ctx, i, alpha, window=None, ancestors=None):
     return _finish(s, size, seen, value[rows])
 
 
+def _nothing(x):
+    zero = torch.zeros_like(x)
+    return zero, torch.tensor(-math.inf, dtype=torch.float64), zero, torch.tensor(0.0, dtype=torch.float64)
+
+
 def _finish(s, size, seen, w):
     if not bool(seen.any()):
-        zero = torch.zeros(w.shape[-1], dtype=torch.float64)
-        return zero, torch.tensor(-math.inf, dtype=torch.float64), zero, torch.tensor(0.0, dtype=torch.float64)
+        return _nothing(w[0])
     s, w = s[seen], w[seen]
     lse = s.logsumexp(0)
     p = (s - lse).exp()

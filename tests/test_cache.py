@@ -227,6 +227,226 @@ def test_tdp_decode(B, N, n, D, dtype, code, page, contexts, windows, parents, p
                                           input_precision=precision))
 
 
+LONG = [  # B N n D dtype code page contexts windows parents: what does not fit in shared memory, and a table much longer than its sequences
+    (1, 1, 1, 64, "fp16", "e4m3", 16, [1500], (None,) * 4, None),
+    (1, 2, 2, 64, "bf16", "int8", 64, [2047], (None,) * 4, None),
+    (3, 1, 1, 64, "fp16", "fp16", 32, [640, -1, 0], (None,) * 4, None),
+    (2, 1, 9, 64, "bf16", "fp16", 32, [640, 5], (500, 600, 100, 50), _tree(9, 3)),
+    (1, 1, 40, 64, "fp16", "e4m3", 64, [470], (30, None, 8, None), _tree(40, 2)),
+    (1, 1, 130, 64, "bf16", "e4m3", 16, [400], (None,) * 4, None),
+    (1, 1, 3, 64, "fp16", "fp16", 16, [1030], (None, 0, None, None), [-1, 0, 0]),
+    (1, 1, 2, 64, "fp16", "e4m3", 16, [900], (0, None, None, 0), None),
+    (1, 2, 2, 64, "bf16", "fp16", 256, [1000], (None, None, 0, 0), None),
+    (1, 2, 7, 128, "fp16", "e4m3", 16, [515], (None, 40, None, None), _tree(7, 2)),
+    (1, 1, 2, 128, "bf16", "fp16", 256, [1023], (None,) * 4, None),
+    (4, 1, 1, 128, "fp16", "int8", 16, [300, -1, 0, 129], (None,) * 4, None),
+    (2, 1, 5, 128, "bf16", "e4m3", 16, [700, 31], (300, 400, 64, 90), [-1, 0, 1, 0, 3]),
+    (1, 1, 64, 128, "fp16", "fp16", 128, [250], (200, 1000, None, 100), _tree(64, 1)),
+    (40, 3, 1, 64, "fp16", "e4m3", 16, [(37 * b) % 600 - 1 for b in range(40)], (None,) * 4, None),
+]
+
+
+def _widened(table, tokens, page):
+    """The table with places for ``tokens`` tokens, the new ones of no page."""
+    more = torch.full((table.shape[0], max(0, tokens // page - table.shape[1])), -1, dtype=torch.int32, device=table.device)
+    return torch.cat([table, more], 1)
+
+
+def _kernel_of_windows(bt, table, windows):
+    c, keep = ft.cache._describe(bt.cache, table, bt.context, bt.n, None, bt.ancestors)
+    w = [1 << 30 if x is None else x for x in windows[:2]]
+    return _native.lib().tritt_decode_workspace(_native.OP_TDP_DECODE, _native.C.byref(c), _native.dtype_code(bt.dt), *w, 0) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [1.0, 1e-3])
+@pytest.mark.parametrize("B,N,n,D,dtype,code,page,contexts,windows,parents", LONG)
+def test_tdp_decode_of_long_sequences(B, N, n, D, dtype, code, page, contexts, windows, parents, size):
+    """The kernel that forms the products of all pairs' tiles.  Its p are at most 2^15 and rounded to fp16: 2^-11 relative, and of a pair below 2^-21
+    of the largest 2^-32 of the largest.  With queries of 0.001 the log-sum-exp counts the attended pairs."""
+    bt = Batch(B, N, n, D, dtype, code, page, contexts, parents=parents, seed=11)
+    bt.q = bt.q * size
+    alpha = 1 / math.sqrt(D)
+    table = _widened(bt.table, 4096, page)
+    assert not _kernel_of_windows(bt, table, windows)
+    out, lse = ft.tdp_decode(bt.q.to(DEV), bt.cache, table, bt.context, alpha, *windows, ancestors=bt.ancestors, return_lse=True)
+    ft.check_status(DEV)
+    again = ft.tdp_decode(bt.q.to(DEV), bt.cache, table, bt.context, alpha, *windows, ancestors=bt.ancestors)
+    assert torch.equal(out, again)
+    for b, h, i in bt.rows():
+        if (b * 7 + h * 5 + i * 3) % max(1, B * N * n // 24):   # (some two dozen rows of each case)
+            continue
+        where, ctx, x = (b, h, i), bt.contexts[b], bt.seq.values[b][:, h]
+        if ctx < 0:
+            assert float(out[b, h, i].abs().max()) == 0 and float(lse[b, h, i]) == -math.inf
+            continue
+        args = (bt.q[b, h, i].double(), x[0], x[1], x[2], x[3], ctx, i, alpha, windows, bt.words)
+        o, want, mass, scores = orc.tdp_row(*args)
+        d = _score_error(D, float(scores), True, True)
+        bound = HALF_STEP[bt.dt] * o.abs() + (math.expm1(2 * d) + 2.0 ** -10) * (mass + o.abs()) + 2.0 ** -32 * orc.tdp_small(*args, 2.0 ** -20) + 2.0 ** -25
+        err = (out[b, h, i].double().cpu() - o).abs()
+        assert bool((err <= bound).all()), f"{where}: off by {float(err.max()):.3e}, bound {float(bound[err.argmax()]):.3e}"
+        assert abs(float(lse[b, h, i]) - float(want)) <= d + 2.0 ** -22 * (1 + abs(float(want))), (where, float(lse[b, h, i]), float(want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,N,n,D,dtype,code,page,contexts,windows,parents", TDP[:10])
+def test_tdp_decode_under_a_long_table(B, N, n, D, dtype, code, page, contexts, windows, parents):
+    """A table of more places than are in use takes another kernel where windows do not bound the tokens: the same definitions."""
+    bt = Batch(B, N, n, D, dtype, code, page, contexts, parents=parents)
+    alpha, table = 1 / math.sqrt(D), _widened(bt.table, 8192, page)
+    out, lse = ft.tdp_decode(bt.q.to(DEV), bt.cache, table, bt.context, alpha, *windows, ancestors=bt.ancestors, return_lse=True)
+    ft.check_status(DEV)
+    _tdp_check(bt, out, lse, windows, alpha, True)
+
+
+DPS_LONG = [  # B N n D dtype code page contexts k_diff parents
+    (1, 1, 1, 64, "fp16", "e4m3", 16, [9000], 1 << 20, None),
+    (40, 3, 1, 64, "bf16", "int8", 16, [(137 * b) % 2500 - 1 for b in range(40)], 1024, None),
+    (2, 2, 24, 128, "fp16", "fp16", 64, [3001, 64], 5000, _tree(24, 2)),
+    (2, 1, 33, 64, "bf16", "e4m3", 256, [2000, 700], 900, _tree(33, 3)),
+    (1, 1, 100, 128, "bf16", "e4m3", 16, [1500], 1024, None),
+    (1, 1, 300, 64, "fp16", "int8", 16, [800], 333, None),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [1.0, 1e-3])
+@pytest.mark.parametrize("B,N,n,D,dtype,code,page,contexts,k_diff,parents", DPS_LONG)
+def test_dps_decode_of_long_sequences(B, N, n, D, dtype, code, page, contexts, k_diff, parents, size):
+    bt = Batch(B, N, n, D, dtype, code, page, contexts, dps=True, parents=parents, seed=13)
+    bt.q = bt.q * size
+    alpha, table = 1 / math.sqrt(D), _widened(bt.table, 16384, page)
+    out, m = ft.dps_decode(bt.q.to(DEV), bt.cache, table, bt.context, alpha, ancestors=bt.ancestors)
+    ft.check_status(DEV)
+    _dps_check(bt, out, m, alpha, True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,N,n,D,dtype,code,page,contexts,k_diff,parents", DPS_LONG)
+def test_dps_append_counts_the_tokens_of_long_sequences(B, N, n, D, dtype, code, page, contexts, k_diff, parents):
+    """Keys of zeros make every score zero: the log-sum-exp is the logarithm of how many tokens are attended to, W their values' mean times V2."""
+    bt = Batch(B, N, n, D, dtype, code, page, contexts, dps=True, parents=parents, seed=17)
+    x = torch.ones(B, N, n, D, device=DEV, dtype=bt.dt)
+    ft.dps_append(bt.cache, _widened(bt.table, 16384, page), bt.context, x * 0, x * 0, x, x, 0.1, k_diff, ancestors=bt.ancestors)
+    back = ft.cache_read(bt.cache, bt.table, bt.context, n, torch.float32)
+    ft.check_status(DEV)
+    gated = back[2].double().cpu()
+    grid = {"fp16": 2.0 ** -11, "e4m3": 2.0 ** -4, "int8": 2.0 ** -7}[code]
+    for b, h, i in bt.rows():
+        ctx = contexts[b]
+        if ctx < 0:
+            continue
+        val = bt.seq.values[b][2, h].clone()
+        val[ctx:] = gated[b, h]
+        zero = torch.zeros(ctx + n, D, dtype=torch.float64)
+        y, lse, mass, _ = orc.dps_row(zero[0], zero, val, None, ctx, i, 0.1, k_diff, bt.words)
+        assert abs(float(back[4][b, h, i]) - float(lse)) <= 2.0 ** -22 * (1 + float(lse)), (b, h, i)
+        err = 2.0 ** -10 * mass                      # p = 1 is exact: what is left is the sums' and the code's rounding
+        got, top = back[3][b, h, i].double().cpu(), float((y.abs() + err).max())
+        rounding = (grid * y.abs() if code != "int8" else 0) + {"fp16": 2.0 ** -24, "e4m3": 2.0 ** -17, "int8": 2.0 ** -7}[code] * top
+        assert bool(((got - y).abs() <= err * (1 + 2 * grid) + rounding + 1e-30).all()), (b, h, i)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_long_sequences_with_bad_rows_missing_places_and_padding(D):
+    """NaN rows reach those that attend to them; a missing page is reported, its tokens left out; rows past a count and free slots are empty."""
+    parents = [-1, 0, 0, 1]
+    bt = Batch(3, 2, 4, D, "fp16", "e4m3", 16, [550, 550, -1], parents=parents, seed=5)
+    table = _widened(bt.table, 4096, 16)
+    counts = torch.tensor([4, 3, 4], dtype=torch.int32, device=DEV)
+    ask = lambda t, *w: ft.tdp_decode(bt.q.to(DEV), bt.cache, t, bt.context, 0.1, *w, ancestors=bt.ancestors, counts=counts, return_lse=True)  # noqa: E731
+    clean, clean_lse = ask(table, 500, 500)
+    ft.check_status(DEV)
+    empty = torch.zeros(3, 2, 4, dtype=torch.bool, device=DEV)
+    empty[1, :, 3] = empty[2] = True
+    assert not bool(clean[empty].any()) and bool((clean_lse[empty] == -math.inf).all()) and bool(torch.isfinite(clean_lse[~empty]).all())
+    place = lambda t, part: (bt.table[0, t // 16].long(), part, 0, t % 16)  # noqa: E731
+    for part in range(4):
+        held = [(place(t, part), bt.cache.exponents[place(t, part)].clone()) for t in (551, 300, 30)]
+        bt.cache.exponents[held[0][0]] = 255     # new token 1: tokens 1 and 3 attend to it
+        bt.cache.exponents[held[2][0]] = 255     # behind every window of 500
+        out, lse = ask(table, 500, 500)
+        hit = torch.zeros_like(empty)
+        hit[0, 0, 1] = hit[0, 0, 3] = True
+        assert bool(torch.isnan(out[hit]).all()) and torch.equal(out[~hit], clean[~hit]), part
+        if part < 2:
+            assert bool(torch.isnan(lse[hit]).all()), part
+        bt.cache.exponents[held[1][0]] = 255     # in everyone's window
+        hit[0, 0] = True
+        out, lse = ask(table, 500, 500)
+        assert bool(torch.isnan(out[hit]).all()) and torch.equal(out[~hit], clean[~hit]), part
+        for at, was in held:
+            bt.cache.exponents[at] = was
+    ft.check_status(DEV)
+    assert torch.equal(ask(table, 500, 500)[0], clean)
+    for page in (5000, -1, 1 << 30):
+        bad = table.clone()
+        bad[0, 10] = page                        # tokens 160 .. 175
+        out, lse = ask(bad, 500, 500)
+        with pytest.raises(_native.TrittError, match="place"):
+            ft.check_status(DEV)
+        assert torch.equal(out[1:], clean[1:]) and bool(torch.isfinite(out).all())
+        # the pairs that are left count: with queries of zeros the log-sum-exp is their number's logarithm
+        _, lse = ft.tdp_decode(torch.zeros_like(bt.q).to(DEV), bt.cache, bad, bt.context, 0.1, counts=counts, return_lse=True)
+        with pytest.raises(_native.TrittError, match="place"):
+            ft.check_status(DEV)
+        for i in range(4):
+            assert abs(float(lse[0, 0, i]) - 2 * math.log(550 + i + 1 - 16)) <= 1e-5
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_kernels_at_the_border_between_them(D):
+    """Windows on either side of what fits in shared memory give the same rows up to each kernel's own error, whichever kernel runs."""
+    bt = Batch(1, 2, 3, D, "bf16", "fp16", 16, [600], seed=3)
+    table, seen = _widened(bt.table, 4096, 16), set()
+    for w in (40, 100, 128, 160, 200, 256, 300, 350, 400, 450, 500, 599):
+        windows = (w, w, None, None)
+        seen.add(_kernel_of_windows(bt, table, windows))
+        out, lse = ft.tdp_decode(bt.q.to(DEV), bt.cache, table, bt.context, 0.1, *windows, return_lse=True)
+        _tdp_check(bt, out, lse, windows, 0.1, True)
+    assert seen == {False, True}
+    ft.check_status(DEV)
+
+
+@pytest.mark.gpu
+def test_long_sequences_in_graphs_and_on_another_stream():
+    bts = [Batch(2, 2, 3, 64, "bf16", "e4m3", 16, [790, 340], dps=True, seed=s) for s in (0, 50)]
+    tables = [_widened(bt.table, 4096, 16) for bt in bts]
+
+    def step(bt, table):
+        ft.dps_append(bt.cache, table, bt.context, bt.q, bt.q, bt.q, bt.q, 0.125, 64)
+        return [*ft.dps_decode(bt.q, bt.cache, table, bt.context, 0.125), ft.tdp_decode(bt.q, bt.cache, table, bt.context, 0.125)]
+
+    for bt in bts:
+        bt.q = bt.q.to(DEV)
+    want = [[t.clone() for t in step(*x)] for x in zip(bts, tables)]
+    streams, graphs, outs = [torch.cuda.Stream() for _ in bts], [], []
+    torch.cuda.synchronize()
+    for bt, table, s in zip(bts, tables, streams):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            outs.append(step(bt, table))
+        graphs.append(g)
+    for _ in range(5):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(want, outs):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+    for bt in bts:
+        bt.context.sub_(300)
+    for g in graphs:
+        g.replay()
+    torch.cuda.synchronize()
+    for bt, table, b in zip(bts, tables, outs):
+        assert all(torch.equal(x, y) for x, y in zip(step(bt, table), b))
+    ft.check_status(DEV)
+
+
 DPS = [  # B N n D dtype code page contexts k_diff parents
     (1, 1, 1, 64, "fp16", "e4m3", 16, [0], 1024, None),
     (3, 2, 1, 64, "bf16", "fp16", 16, [1, 40, -1], 1024, None),
