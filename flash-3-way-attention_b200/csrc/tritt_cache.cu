@@ -326,7 +326,7 @@ int tritt_decode_path(int op, int D, int dtype, int flags) { return fast(op, D, 
 size_t tritt_decode_workspace(int op, const tritt_cache_t* c, int dtype, int k1_window, int k2_window, int flags) {
   if (check_cache(c)) return 0;
   if (op == TRITT_OP_TDP_DECODE && fast(op, c->D, dtype, flags))
-    return window_tdp_decode_applies(*c, window(k1_window), window(k2_window)) ? 0 : sm100_tdp_decode_workspace(*c, window(k2_window));
+    return window_tdp_decode_applies(*c, window(k1_window), window(k2_window)) ? 0 : sm100_tdp_decode_workspace(*c);
   if (fast(op, c->D, dtype, flags)) return mma_dps_decode_workspace(*c);
   return part_bytes(*c, simt_decode_splits(*c));
 }

@@ -307,7 +307,7 @@ struct DpsDecodeArgs {
 };
 // ... on the tensor cores (16-bit queries, head dimension 64 or 128), both kernels of it
 bool sm100_tdp_decode_supported(int D, int dtype);
-size_t sm100_tdp_decode_workspace(const tritt_cache_t& c, int k2_window);
+size_t sm100_tdp_decode_workspace(const tritt_cache_t& c);
 int sm100_tdp_decode(const TdpDecodeArgs& a, void* workspace, void* o, float* lse, cudaStream_t stream);
 
 // ... with all of the windows in shared memory, where they fit (the same types; one kernel, no workspace)

@@ -51,7 +51,8 @@ template <int D> struct Cfg {
   static constexpr int kOffV = kOffK + kStages * kTile;
   static constexpr int kOffQ = kOffV + kStages * kTile;            // [8 warps][D] fp16
   static constexpr int kOffRows = kOffQ + 8 * D * 2;               // two pieces' [256] RowInfo
-  static constexpr int kOffMisc = kOffRows + 2 * 256 * 32;
+  static constexpr int kOffRun = kOffRows + 2 * 256 * 32;          // [8 warps][D] fp32
+  static constexpr int kOffMisc = kOffRun + 8 * D * 4;
   static constexpr int kSmem = kOffMisc + 1536;
   static constexpr int kTmemO = 256;                               // S_a | S_b | acc_a | acc_b
 };
@@ -78,9 +79,8 @@ constexpr int kRowNan = 256;
 struct __align__(16) Item {
   int n, tiles, first, behind;       // slabs, tiles; columns first .. behind - 1, 128 a slab
   int b, head, g0, groups;           // groups g0 .. of the sequence's line; groups of a new token
-  int all_groups, ctx, flags, pad;   // groups of all its new tokens
-  float* out;                        // [8][D + 2]: the groups' results
-  float* pad2;
+  int all_groups, ctx;               // groups of all its new tokens
+  int token[8];                      // of the soft-max warps' groups
 };
 constexpr int kItems = 4;
 constexpr int kConsumers = 17;       // warps that read them
@@ -104,15 +104,15 @@ struct Line {
   int pairs, slabs;      // pairs of tiles of a head; slabs of a pair (the most of any)
 };
 struct LineEntry {       // in the workspace, for the kernel that joins
-  long long base, pair_base;
+  long long base;
   Line line;
-  int pad;
 };
 
 struct Params {
   TdpDecodeArgs a;
   LineEntry* table;      // [B]
-  float* part;           // [pieces][8][D + 2]
+  float* part;           // [new tokens of all heads + CTAs][8][D + 2]: each of a CTA's soft-max warps' maximum, sum and result of one new
+                         // token; the CTAs that share a token, and the tokens that share a CTA, follow one another, so their sum numbers them
   int ctas;
 };
 
@@ -156,24 +156,21 @@ __device__ __forceinline__ Columns columns_of(const TdpDecodeArgs& a, const Line
 // Steps of a CTA: walks the line from the CTA's first step to its last.  (Where it stands is found by division once, then by counting.)
 struct Walk {
   long long left;           // steps
-  long long pair_base;      // pairs before the present one, of all sequences
   int b, head, pair, slab;
   Line l;
 };
 struct Piece {
   int b, head, pair, s0, s1;
-  long long id;             // pieces are numbered by pair + CTA: each new pair and each cut makes one
 };
 __device__ __forceinline__ Walk start_walk(const Params& p, long long total) {
   long long x = (long long)blockIdx.x * total / p.ctas;
-  Walk w{((long long)blockIdx.x + 1) * total / p.ctas - x, 0, 0, 0, 0, 0, {}};
+  Walk w{((long long)blockIdx.x + 1) * total / p.ctas - x, 0, 0, 0, 0, {}};
   if (w.left == 0) return w;
   w.l = line_of(p.a, 0);
   while (true) {
     const long long pairs = (long long)w.l.pairs * p.a.cache.c.N, here = pairs * w.l.slabs;
     if (x < here) break;
     x -= here;
-    w.pair_base += pairs;
     if (w.b + 1 >= p.a.cache.c.B) {   // (contexts that changed under the kernel)
       w.left = 0;
       return w;
@@ -184,13 +181,12 @@ __device__ __forceinline__ Walk start_walk(const Params& p, long long total) {
   w.slab = (int)(x - pair * w.l.slabs);
   w.head = (int)(pair / w.l.pairs);
   w.pair = (int)(pair - (long long)w.head * w.l.pairs);
-  w.pair_base += pair;
   return w;
 }
 __device__ __forceinline__ bool next_piece(const Params& p, Walk& w, Piece& s) {
   if (w.left <= 0) return false;
   while (w.slab == w.l.slabs) {   // the next pair, head, sequence (that has any)
-    if (w.l.slabs) ++w.pair_base, ++w.pair;
+    if (w.l.slabs) ++w.pair;
     w.slab = 0;
     if (w.pair < w.l.pairs) break;
     w.pair = 0;
@@ -205,7 +201,6 @@ __device__ __forceinline__ bool next_piece(const Params& p, Walk& w, Piece& s) {
   s.pair = w.pair;
   s.s0 = w.slab;
   s.s1 = w.l.slabs - w.slab < w.left ? w.l.slabs : w.slab + (int)w.left;
-  s.id = w.pair_base + blockIdx.x;
   w.left -= s.s1 - s.s0;
   w.slab = s.s1;
   return true;
@@ -446,21 +441,20 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
   }
   if (warp == 2) {
     // the whole line's length, and the sequence of this CTA's first step: 32 sequences at a time
-    long long total = 0, pairs = 0;
+    long long total = 0;
     for (int b0 = 0; b0 < ca.c.B; b0 += 32) {
       const int b = b0 + lane;
       Line l{};
       if (b < ca.c.B) l = line_of(a, b);
-      const long long np = (long long)l.pairs * ca.c.N, steps = np * l.slabs;
-      long long s = steps, q = np;   // sums up to this lane
+      const long long steps = (long long)l.pairs * ca.c.N * l.slabs;
+      long long s = steps;   // sums up to this lane
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const long long s2 = __shfl_up_sync(0xffffffffu, s, o), q2 = __shfl_up_sync(0xffffffffu, q, o);
-        if (lane >= o) s += s2, q += q2;
+        const long long s2 = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += s2;
       }
-      if (blockIdx.x == 0 && b < ca.c.B) p.table[b] = LineEntry{total + s - steps, pairs + q - np, l, 0};
+      if (blockIdx.x == 0 && b < ca.c.B) p.table[b] = LineEntry{total + s - steps, l};
       total += __shfl_sync(0xffffffffu, s, 31);
-      pairs += __shfl_sync(0xffffffffu, q, 31);
     }
     if (lane == 0) ms.total = total;
   }
@@ -493,6 +487,7 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
       Piece s;
       int count = 0;
       bool more = true;
+      long long last = -1;   // (lanes 0 to 7: of the soft-max warp with that number) where its previous group's results are
       while (more) {
         more = next_piece(p, walk, s);
         Item it{};
@@ -508,11 +503,18 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
           it.b = s.b;
           it.head = s.head;
           it.ctx = walk.l.ctx;
-          it.out = p.part + (size_t)s.id * 8 * (D + 2);
-          if (it.n <= 0) {   // (its slabs lie behind all columns: nothing seen)
-            if (lane < 8 && it.g0 + lane < it.all_groups) it.out[lane * (D + 2)] = -INFINITY, it.out[lane * (D + 2) + 1] = 0.f;
-            continue;
+          const int group = it.g0 + (lane & 7), token = least(group, it.all_groups - 1) / it.groups;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) it.token[k] = __shfl_sync(0xffffffffu, token, k);
+          const long long at = ((long long)s.b * ca.c.N + s.head) * ca.c.n + token + blockIdx.x;
+          if (lane < 8 && group < it.all_groups && at != last) {   // nothing seen so far
+            float* out = p.part + (size_t)(at * 8 + lane) * (D + 2);
+            out[0] = -INFINITY;
+            out[1] = 0.f;
+            last = at;
           }
+          __syncwarp();
+          if (it.n <= 0) continue;   // (its slabs lie behind all columns)
         }
         if (!__all_sync(0xffffffffu, mbar_wait(&ms.item_free[count % kItems], ((count / kItems) & 1) ^ 1, abort_flag))) break;
         if (lane == 0) {
@@ -687,6 +689,10 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
     const uint32_t lane_base = (uint32_t)(wq * 32) << 16;
     const uint32_t tS = tmem + lane_base + x * 128, tO = tmem + lane_base + C::kTmemO + x * D;
     int slab = 0, scount = 0, mine = 0;   // slabs so far; this tile's, and its pieces
+    // what the warp has of a new token runs along its pieces: maximum and sum here, the result in shared memory, a column a lane
+    float* const run = reinterpret_cast<float*>(smem + C::kOffRun) + (x * 4 + wq) * D + lane;
+    long long last = -1;
+    float m_run = -INFINITY, l_run = 0.f;
     bool alive = true;
     for (int count = 0; alive; ++count) {
       const int n = next_item(count);
@@ -694,7 +700,7 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
       const Item& it = ms.items[count % kItems];
       const int first = uniform(it.first), behind = uniform(it.behind), ctx = uniform(it.ctx);
       const bool used = it.g0 + x * 4 + wq < it.all_groups;   // (the warp's rows are of a new token)
-      float* const out = it.out + (x * 4 + wq) * (D + 2);
+      const long long at = ((long long)it.b * ca.c.N + it.head) * ca.c.n + it.token[x * 4 + wq] + blockIdx.x;
       const bool second = uniform(it.tiles) == 2;
       free_item(count);
       if (x == 1 && !second) {
@@ -848,13 +854,20 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
       load_codes(even, 0);
       load_codes(odd, 1);
       if ((r.flags & kRowNan) && l_sum > 0.f) l_sum = __uint_as_float(0x7fffffffu);
-      float m_all = m_used;
+      const bool more = at == last;   // (of the token that the previous piece was of)
+      last = at;
+      float m_all = more ? fmaxf(m_used, m_run) : m_used;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) m_all = fmaxf(m_all, __shfl_xor_sync(0xffffffffu, m_all, o));
       const float weight = m_used == -INFINITY ? 0.f : exp2f(m_used - m_all - kLift);
       float l_all = m_used == -INFINITY ? (l_sum != l_sum ? l_sum : 0.f) : l_sum * weight;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) l_all += __shfl_xor_sync(0xffffffffu, l_all, o);
+      const float keep_run = !more || m_run == -INFINITY ? 0.f : exp2f(m_run - m_all);
+      if (more) l_all += m_run == -INFINITY ? l_run : l_run * keep_run;
+      m_run = m_all;
+      l_run = l_all;
+      float* const out = p.part + (size_t)(at * 8 + x * 4 + wq) * (D + 2);
       // V1's and V2's powers of two (fp32's range is that of the result's own type and more)
       const int byte2 = r.flags & 255;
       const float vscale =
@@ -901,6 +914,8 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
             v[e] = keep + __shfl_xor_sync(0xffffffffu, give, h);
           }
         }
+        if (keep_run != 0.f) v[0] = fmaf(run[ch * 32], keep_run, v[0]);
+        run[ch * 32] = v[0];
         if (used) out[2 + ch * 32 + lane] = v[0];
       };
 #pragma unroll 1
@@ -940,67 +955,53 @@ __device__ __noinline__ long long cta_of(long long x, long long total, int ctas)
   return ((x + 1) * ctas - 1) / total;
 }
 
-// One block a row.  A thread finds the pieces of a group, 256 groups at a time, and their places form a line in shared memory; the line's maxima give
-// the row's, and the warps add up the results, four loads in flight; then the warps' sums are added in order.
+// One block a row.  The results of a row are those of the warps of the CTAs that have steps of it: a thread looks at one's maximum, then the warps
+// add them up in order, four loads in flight, and their sums are added in order.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) tdp_join_kernel(const __grid_constant__ TdpJoinParams j) {
   wait_for_previous();
-  constexpr int kLine = 1024;   // pieces at a time
+  constexpr int E = D / 32;
   __shared__ float s_top[8], s_sum[8], so[8][D];
-  __shared__ long long s_line[kLine];   // number of a piece's group among all results
-  __shared__ int s_count[8];
+  __shared__ float s_max[256];   // -infinity: none
   const CacheArgs& ca = j.a.cache;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const long long row = blockIdx.x;
   const int i = (int)(row % ca.c.n), head = (int)(row / ca.c.n % ca.c.N), b = (int)(row / ca.c.n / ca.c.N);
   const LineEntry e = j.table[b], end = j.table[ca.c.B - 1];
   const long long total = end.base + (long long)end.line.pairs * end.line.slabs * ca.c.N;
-  constexpr int E = D / 32;
-  float top = -INFINITY, sum = 0.f, acc[E];   // of this warp's pieces
+  float top = -INFINITY, sum = 0.f, acc[E];   // of this warp's results
 #pragma unroll
   for (int k = 0; k < E; ++k) acc[k] = 0.f;
-  const int groups = i < e.line.cnt ? e.line.groups : 0;
-  for (int g0 = 0; g0 < groups; g0 += 256) {
-    // this thread's group: its pieces are those of the CTAs that have steps of its pair
-    long long first = 0, id = 0;
-    int pieces = 0;
-    if (g0 + tid < groups) {
-      const int g = i * e.line.groups + g0 + tid;
-      const long long pair = (long long)head * e.line.pairs + g / 8;
-      first = e.base + pair * e.line.slabs;
-      id = (e.pair_base + pair) * 8 + g % 8;
-      for (long long x = first; x < first + e.line.slabs; ++pieces) x = behind_cta(cta_of(x, total, j.ctas), total, j.ctas);
-    }
-    int at = pieces;   // its place in the line: the pieces before it
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, at, o);
-      if (lane >= o) at += v;
-    }
-    __syncthreads();
-    if (lane == 31) s_count[warp] = at;
-    __syncthreads();
-    at -= pieces;
-    int all = 0;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) {
-      if (w < warp) at += s_count[w];
-      all += s_count[w];
-    }
-    for (int l0 = 0; l0 < all; l0 += kLine) {
-      __syncthreads();
-      {
-        long long x = first;
-        for (int k = 0; k < pieces; ++k) {
-          const long long c = cta_of(x, total, j.ctas);
-          if (at + k >= l0 && at + k < l0 + kLine) s_line[at + k - l0] = id + c * 8;
-          x = behind_cta(c, total, j.ctas);
+  if (i < e.line.cnt) {
+    // the row's groups, its pairs' steps, and the CTAs of those
+    const int ga = i * e.line.groups, gb = ga + e.line.groups, slabs = e.line.slabs;
+    const long long base = e.base + (long long)head * e.line.pairs * slabs;   // of the head
+    const long long xa = base + (long long)(ga / 8) * slabs, xb = base + (long long)((gb + 7) / 8) * slabs;
+    auto pair_of = [&](long long x) {   // (a division of 64 bits is long)
+      return (int)(xb - base < 1ll << 32 ? (uint32_t)(x - base) / (uint32_t)slabs : (x - base) / slabs);
+    };
+    const long long ca0 = cta_of(xa, total, j.ctas);
+    const int count = (int)(cta_of(xb - 1, total, j.ctas) - ca0 + 1) * 8;
+    const float* part = j.part + (size_t)(row + ca0) * 8 * (D + 2);
+    for (int k0 = 0; k0 < count; k0 += 256) {
+      const int k = k0 + tid;
+      float m = -INFINITY;
+      if (k < count) {
+        const long long c = ca0 + k / 8, x0 = behind_cta(c - 1, total, j.ctas), x1 = behind_cta(c, total, j.ctas);
+        const long long lo = x0 > xa ? x0 : xa, hi = x1 < xb ? x1 : xb;   // its steps of the row's pairs
+        if (lo < hi) {
+          // its groups of the row; the warp has one of them if there are eight, or a group of its number among fewer
+          const int g0 = most(ga, pair_of(lo) * 8), g1 = least(gb, pair_of(hi - 1) * 8 + 8);
+          if (((k - g0) & 7) < g1 - g0) m = part[(size_t)k * (D + 2)];
+          // (a maximum of -infinity with a sum of NaN is of a row that reads as NaN)
+          if (((k - g0) & 7) < g1 - g0 && m == -INFINITY) {
+            const float l = part[(size_t)k * (D + 2) + 1];
+            if (l != l) sum = l;
+          }
         }
       }
       __syncthreads();
-      const int here = all - l0 < kLine ? all - l0 : kLine;
-      float m = -INFINITY;
-      for (int k = tid; k < here; k += 256) m = fmaxf(m, j.part[(size_t)s_line[k] * (D + 2)]);
+      s_max[tid] = m;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
       if (lane == 0) s_top[warp] = m;
@@ -1009,34 +1010,35 @@ __global__ void __launch_bounds__(256) tdp_join_kernel(const __grid_constant__ T
 #pragma unroll
       for (int w = 0; w < 8; ++w) now = fmaxf(now, s_top[w]);
       const float w0 = top == -INFINITY ? 0.f : exp2f(top - now);
-      sum *= top == -INFINITY && sum != sum ? 1.f : w0;
+      if (top != -INFINITY) sum *= w0;
 #pragma unroll
-      for (int k = 0; k < E; ++k) acc[k] *= w0;
+      for (int q = 0; q < E; ++q) acc[q] *= w0;
       top = now;
+      const int here = least(count - k0, 256);
 #pragma unroll 1
-      for (int k0 = warp; k0 < here; k0 += 32) {
-        float mp[4], lp[4], v[4][E];
+      for (int q0 = warp; q0 < here; q0 += 32) {
+        float w[4], l[4], v[4][E];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          const int k = k0 + u * 8;
-          const float* p = j.part + (size_t)s_line[k < here ? k : k0] * (D + 2);
-          mp[u] = k < here ? p[0] : -INFINITY;
-          lp[u] = k < here ? p[1] : 0.f;
+          const int q = q0 + u * 8;
+          const float mq = q < here ? s_max[q] : -INFINITY;
+          w[u] = mq == -INFINITY ? 0.f : exp2f(mq - top);
+          const float* p = part + (size_t)(k0 + q) * (D + 2);
+          l[u] = mq == -INFINITY ? 0.f : p[1];
 #pragma unroll
-          for (int q = 0; q < E; ++q) v[u][q] = p[2 + q * 32 + lane];
+          for (int c = 0; c < E; ++c) v[u][c] = mq == -INFINITY ? 0.f : p[2 + c * 32 + lane];
         }
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          // (a group that has seen nothing has written no result; a maximum of -infinity with a sum of NaN is of a row that reads as NaN)
-          const float w = mp[u] == -INFINITY ? 0.f : exp2f(mp[u] - top);
-          sum += mp[u] == -INFINITY ? (lp[u] != lp[u] ? lp[u] : 0.f) : lp[u] * w;
+          if (lane == 0) sum += l[u] * w[u];   // (a thread's own NaN stays in its sum)
 #pragma unroll
-          for (int q = 0; q < E; ++q) acc[q] += w == 0.f ? 0.f : v[u][q] * w;
+          for (int c = 0; c < E; ++c) acc[c] += w[u] == 0.f ? 0.f : v[u][c] * w[u];
         }
       }
     }
   }
-  __syncthreads();
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) s_sum[warp] = sum;
 #pragma unroll
   for (int k = 0; k < E; ++k) so[warp][k * 32 + lane] = acc[k];
@@ -1087,10 +1089,8 @@ template <typename T16> int by_size(const Params& p, const TdpJoinParams& j, cud
 
 bool sm100_tdp_decode_supported(int D, int dtype) { return (D == 64 || D == 128) && (dtype == TRITT_F16 || dtype == TRITT_BF16); }
 
-size_t sm100_tdp_decode_workspace(const tritt_cache_t& c, int k2_window) {
-  const long long rows = (long long)c.page_size * c.table_pages + c.n, window = (long long)k2_window + 1;
-  const long long groups = ((rows < window ? rows : window) + 31) / 32, pairs = (c.n * groups + 7) / 8;
-  return align_up((size_t)c.B * sizeof(LineEntry), 256) + align_up((size_t)((long long)c.B * c.N * pairs + num_sms()) * 8 * (c.D + 2) * 4, 256);
+size_t sm100_tdp_decode_workspace(const tritt_cache_t& c) {
+  return align_up((size_t)c.B * sizeof(LineEntry), 256) + align_up((size_t)((long long)c.B * c.N * c.n + num_sms()) * 8 * (c.D + 2) * 4, 256);
 }
 
 int sm100_tdp_decode(const TdpDecodeArgs& a, void* workspace, void* o, float* lse, cudaStream_t stream) {
