@@ -121,8 +121,8 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm<NT>) dps_decode_kern
   constexpr int Q = 8 * NT, NQ = ONE ? 1 : 2;
   extern __shared__ __align__(128) uint8_t ring_all[];
   __shared__ uint64_t s_full[kWarps][NS];
-  __shared__ int s_abort;
-  __shared__ long long s_total;
+  __shared__ int s_abort, s_first;
+  __shared__ long long s_total, s_base, s_groups;
   __shared__ float4 s_side[kWarps][TK];   // of a tile's tokens: scale of scores, bias, scale of P
   __shared__ unsigned long long s_word[Q];
   __shared__ int s_lo[Q], s_pos[Q];
@@ -132,7 +132,6 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm<NT>) dps_decode_kern
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   uint8_t* ring = ring_all + warp * NS * S::kStage;
   uint64_t* full = s_full[warp];
-  wait_for_previous();
   let_next_start();
   if (lane == 0) {
     for (int i = 0; i < NS; ++i) mbar_init(&full[i], 33);   // one arrival with the bulk copies' bytes, one of each lane
@@ -157,28 +156,51 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm<NT>) dps_decode_kern
       groups += __shfl_sync(0xffffffffu, q, 31);
     }
     if (lane == 0) s_total = total, s_abort = 0;
+    // the sequence of this block's first step (a walk from sequence to sequence took 200 cycles each)
+    const int parts = parts_of(total, p.ctas);
+    const long long x = (long long)blockIdx.x * total / parts;
+    long long before = 0, groups_before = 0;
+    for (int b0 = 0; b0 < ca.c.B && (int)blockIdx.x < parts; b0 += 32) {
+      const int b = b0 + lane;
+      Line l{};
+      if (b < ca.c.B) l = line_of<TK, Q>(a, b);
+      const long long ng = (long long)l.groups * ca.c.N, steps = ng * l.tiles;
+      long long s = steps, q = ng;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long s2 = __shfl_up_sync(0xffffffffu, s, o), q2 = __shfl_up_sync(0xffffffffu, q, o);
+        if (lane >= o) s += s2, q += q2;
+      }
+      const uint32_t behind = __ballot_sync(0xffffffffu, x < before + s);
+      if (behind) {
+        if (lane == __ffs(behind) - 1) s_first = b, s_base = before + s - steps, s_groups = groups_before + q - ng;
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, s, 31);
+      groups_before += __shfl_sync(0xffffffffu, q, 31);
+    }
   }
   __syncthreads();
   const long long total = s_total;
   const int parts = parts_of(total, p.ctas);
-  if ((int)blockIdx.x >= parts) return;
-  long long x = (long long)blockIdx.x * total / parts, base = 0, group_base = 0;
+  if ((int)blockIdx.x >= parts) return wait_for_previous();   // (a kernel that ended without one would let the next start beside the previous)
+  long long x = (long long)blockIdx.x * total / parts, base = s_base, group_base = s_groups;
   const long long x_end = ((long long)blockIdx.x + 1) * total / parts;
-  if (x >= x_end) return;
+  if (x >= x_end) return wait_for_previous();
   const size_t part_rows = (size_t)ca.c.N << ca.page_log2;   // rows of one part of a page
   const size_t page_bytes = 4 * part_rows * RB;
   const int row_mask = ca.c.page_size - 1;
   int st = 0, phase = 0;   // the ring's next stage
-  int b = 0;
-  Line line = line_of<TK, Q>(a, 0);
-  bool alive = true;
+  int b = s_first;
+  Line line = line_of<TK, Q>(a, b);
+  bool alive = true, waited = false;
 
   while (x < x_end && alive) {
     // --- the next piece: tiles s0 .. s1 - 1 of one group of new tokens
     while (x >= base + (long long)line.groups * line.tiles * ca.c.N) {
       base += (long long)line.groups * line.tiles * ca.c.N;
       group_base += (long long)line.groups * ca.c.N;
-      if (++b >= ca.c.B) return;   // (contexts that changed under the kernel)
+      if (++b >= ca.c.B) return wait_for_previous();   // (contexts that changed under the kernel)
       line = line_of<TK, Q>(a, b);
     }
     const long long rel = x - base, grp = rel / line.tiles;
@@ -193,6 +215,16 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm<NT>) dps_decode_kern
     if (s0 >= tile1) {
       for (int i = tid; i < nq; i += kWarps * 32) part[i * (D + 2)] = -INFINITY, part[i * (D + 2) + 1] = 0.f;
       continue;
+    }
+
+    // --- the queries' rows, on their way while the ring is filled (those past the last: its own, not looked at)
+    uint4 raw[NT][D / 32];
+    constexpr int EPL = S::kWide ? 8 : 16;   // elements of 16 bytes of codes
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const uint16_t* q = (const uint16_t*)a.q.p + rows_at(a.q, b, head, i0 + min(nt * 8 + g, nq - 1)) + t * EPL;
+#pragma unroll
+      for (int k = 0; k < D / 32; ++k) raw[nt][k] = __ldg(reinterpret_cast<const uint4*>(q + k / (EPL / 8) * 4 * EPL + k % (EPL / 8) * 8));
     }
 
     // --- the ring: this warp takes tiles s0 + warp, + kWarps, ...
@@ -232,6 +264,9 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm<NT>) dps_decode_kern
       int pg[NS + 1];
 #pragma unroll
       for (int i = 0; i <= NS; ++i) pg[i] = find_page(s0 + warp + i * kWarps);
+      // (what is read above, no kernel that may still run has written)
+      if (!waited) wait_for_previous();
+      waited = true;
       int f = st;
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
@@ -249,28 +284,18 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm<NT>) dps_decode_kern
       const bool on = nt * 8 + g < nq;
       float f[D / 4];   // elements of this thread's positions, in the order of its fragments
       uint32_t big = 0;
-      const size_t off = on ? rows_at(a.q, b, head, i) : 0;
-      constexpr int EPL = S::kWide ? 8 : 16;   // elements of 16 bytes of codes
 #pragma unroll
-      for (int j = 0; j < D / (4 * EPL); ++j)
+      for (int k = 0; k < D / 32; ++k) {
+        const uint32_t w[4] = {raw[nt][k].x, raw[nt][k].y, raw[nt][k].z, raw[nt][k].w};
 #pragma unroll
-        for (int c = 0; c < EPL / 8; ++c) {
-          float v[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = 0.f;
-          const size_t at = off + j * 4 * EPL + t * EPL + c * 8;
-          if (on) {
-            if (a.dtype == TRITT_F16)
-              load8((const __half*)a.q.p + at, v);
-            else
-              load8((const __nv_bfloat16*)a.q.p + at, v);
-          }
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            f[j * EPL + c * 8 + e] = v[e];
-            big = max(big, __float_as_uint(v[e]) & 0x7fffffffu);
-          }
+        for (int e = 0; e < 4; ++e) {
+          const float2 v = a.dtype == TRITT_F16 ? unpack2<__half>(w[e]) : unpack2<__nv_bfloat16>(w[e]);
+          f[k * 8 + 2 * e] = on ? v.x : 0.f;
+          f[k * 8 + 2 * e + 1] = on ? v.y : 0.f;
         }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) big = max(big, __float_as_uint(f[k * 8 + e]) & 0x7fffffffu);
+      }
       big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
       big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
       const int up = max(min(254 - (int)(big >> 23), 253), 1);
@@ -577,26 +602,32 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm<NT>) dps_decode_kern
               f == 0.f ? make_float2(0.f, 0.f) : make_float2(acc[nt][mb][q] * f, acc[nt][mb][2 + q] * f);
       }
     __syncthreads();
-    for (int i = warp; i < nq; i += kWarps) {
+    if (tid < nq) {
       float top = -INFINITY, sum = 0.f;
 #pragma unroll
-      for (int k = 0; k < kWarps; ++k) top = fmaxf(top, s_m[k][i]);
+      for (int k = 0; k < kWarps; ++k) top = fmaxf(top, s_m[k][tid]);
 #pragma unroll
       for (int k = 0; k < kWarps; ++k)
-        sum += s_m[k][i] == -INFINITY ? (s_l[k][i] != s_l[k][i] ? s_l[k][i] : 0.f) : s_l[k][i] * exp2f(s_m[k][i] - top);
-      float* to = part + i * (D + 2);
-      if (lane == 0) to[0] = top, to[1] = sum;
+        sum += s_m[k][tid] == -INFINITY ? (s_l[k][tid] != s_l[k][tid] ? s_l[k][tid] : 0.f) : s_l[k][tid] * exp2f(s_m[k][tid] - top);
+      *reinterpret_cast<float2*>(part + tid * (D + 2)) = make_float2(top, sum);
+    }
+#pragma unroll 2
+    for (int x = tid; x < nq * (D / 4); x += kWarps * 32) {
+      const int i = x / (D / 4), c = x % (D / 4) * 4;
+      float4 v = *reinterpret_cast<const float4*>(&out[0][i][c]);
 #pragma unroll
-      for (int c = lane; c < D; c += 32) {
-        float v = out[0][i][c];
-#pragma unroll
-        for (int k = 1; k < kWarps; ++k) v += out[k][i][c];
-        to[2 + c] = v;
+      for (int k = 1; k < kWarps; ++k) {
+        const float4 o = *reinterpret_cast<const float4*>(&out[k][i][c]);
+        v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
       }
+      float2* to = reinterpret_cast<float2*>(part + i * (D + 2) + 2 + c);
+      to[0] = make_float2(v.x, v.y);
+      to[1] = make_float2(v.z, v.w);
     }
     fence_async_smem();   // (the next piece's copies come into the same memory)
     __syncthreads();
   }
+  if (!waited) wait_for_previous();
 }
 
 struct DpsJoinParams {

@@ -93,7 +93,7 @@ struct Misc {
   uint32_t tmem_base;
   int abort_flag;
   int first_b;
-  long long first_base, total;
+  long long first_base, total;   // of the sequence with this CTA's first step; of all
 };
 static_assert(sizeof(Misc) <= 1536, "shared memory of the barriers");
 
@@ -162,20 +162,15 @@ struct Walk {
 struct Piece {
   int b, head, pair, s0, s1;
 };
-__device__ __forceinline__ Walk start_walk(const Params& p, long long total) {
+__device__ __forceinline__ Walk start_walk(const Params& p, long long total, int b, long long base) {
   long long x = (long long)blockIdx.x * total / p.ctas;
-  Walk w{((long long)blockIdx.x + 1) * total / p.ctas - x, 0, 0, 0, 0, {}};
+  Walk w{((long long)blockIdx.x + 1) * total / p.ctas - x, b, 0, 0, 0, {}};
   if (w.left == 0) return w;
-  w.l = line_of(p.a, 0);
-  while (true) {
-    const long long pairs = (long long)w.l.pairs * p.a.cache.c.N, here = pairs * w.l.slabs;
-    if (x < here) break;
-    x -= here;
-    if (w.b + 1 >= p.a.cache.c.B) {   // (contexts that changed under the kernel)
-      w.left = 0;
-      return w;
-    }
-    w.l = line_of(p.a, ++w.b);
+  w.l = line_of(p.a, b);
+  x -= base;
+  if (x >= (long long)w.l.pairs * p.a.cache.c.N * w.l.slabs) {   // (contexts that changed under the kernel)
+    w.left = 0;
+    return w;
   }
   const long long pair = x / w.l.slabs;
   w.slab = (int)(x - pair * w.l.slabs);
@@ -457,6 +452,27 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
       total += __shfl_sync(0xffffffffu, s, 31);
     }
     if (lane == 0) ms.total = total;
+    // the sequence of this CTA's first step
+    const long long x = (long long)blockIdx.x * total / p.ctas;
+    long long before = 0;
+    for (int b0 = 0; b0 < ca.c.B && total > 0; b0 += 32) {
+      const int b = b0 + lane;
+      Line l{};
+      if (b < ca.c.B) l = line_of(a, b);
+      const long long steps = (long long)l.pairs * ca.c.N * l.slabs;
+      long long s = steps;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long s2 = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += s2;
+      }
+      const uint32_t behind = __ballot_sync(0xffffffffu, x < before + s);
+      if (behind) {
+        if (lane == __ffs(behind) - 1) ms.first_b = b, ms.first_base = before + s - steps;
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, s, 31);
+    }
   }
   let_next_start();
   tc_fence_before();
@@ -483,7 +499,7 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
     set_regs<kRegsLaunch, kRegsIssue>();
     if (warp == 1) {
       // ------------------------------------------------------------------ pieces
-      Walk walk = start_walk(p, ms.total);
+      Walk walk = start_walk(p, ms.total, ms.first_b, ms.first_base);
       Piece s;
       int count = 0;
       bool more = true;
