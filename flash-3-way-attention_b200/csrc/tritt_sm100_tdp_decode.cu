@@ -50,8 +50,8 @@ template <int D> struct Cfg {
   static constexpr int kOffK = 2 * kTile;
   static constexpr int kOffV = kOffK + kStages * kTile;
   static constexpr int kOffQ = kOffV + kStages * kTile;            // [8 warps][D] fp16
-  static constexpr int kOffRows = kOffQ + 8 * D * 2;               // two pieces' [256] RowInfo
-  static constexpr int kOffRun = kOffRows + 2 * 256 * 32;          // [8 warps][D] fp32
+  static constexpr int kOffRows = kOffQ + 8 * D * 2;               // [256] RowInfo
+  static constexpr int kOffRun = kOffRows + 256 * 32;          // [8 warps][D] fp32
   static constexpr int kOffMisc = kOffRun + 8 * D * 4;
   static constexpr int kSmem = kOffMisc + 1536;
   static constexpr int kTmemO = 256;                               // S_a | S_b | acc_a | acc_b
@@ -423,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
     }
     for (int x = 0; x < 2; ++x) {
       mbar_init(&ms.a_ready[x], 128);
-      mbar_init(&ms.a_free[x], 1);
+      mbar_init(&ms.a_free[x], 5);   // its last products, and four warps that have read what its rows are
       mbar_init(&ms.s_ready[x], 1);
       mbar_init(&ms.p_ready[x], 128);
       mbar_init(&ms.o_done[x], 1);
@@ -639,7 +639,7 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
       const size_t load_rows = (keys ? kPartK1 : kPartV1) * part_rows + head_rows, v_rows = kPartV1 * part_rows + head_rows;
       auto form = [&]() {
         if (!__all_sync(0xffffffffu, mbar_wait(&ms.a_free[mine], (formed & 1) ^ 1, abort_flag))) return false;
-        form_rows<T16, D, CODE>(a, it, mine, w, lane, sA + mine * C::kTile, sQ + (mine * 4 + w) * D, sRows + (count & 1) * 256 + mine * 128);
+        form_rows<T16, D, CODE>(a, it, mine, w, lane, sA + mine * C::kTile, sQ + (mine * 4 + w) * D, sRows + mine * 128);
         fence_async_smem();
         mbar_arrive(&ms.a_ready[mine]);
         ++formed;
@@ -725,7 +725,11 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
       }
       alive = __all_sync(0xffffffffu, mbar_wait(&ms.a_ready[x], mine & 1, abort_flag));
       if (!alive) break;
-      const RowInfo r = sRows[(count & 1) * 256 + x * 128 + wq * 32 + lane];
+      const RowInfo r = sRows[x * 128 + wq * 32 + lane];
+      __syncwarp();
+      // (without this the A of the next piece, and of the one behind it, might come while this warp is at the previous piece's sums: it would
+      // find the barrier two phases on, and other rows)
+      if (lane == 0) mbar_arrive(&ms.a_free[x]);
       // --- slabs: a half of 64 columns at a time is read once, its maximum taken, and the row's reference raised where that is 2^8 above it
       float m_used = -INFINITY, l_sum = 0.f;
       int v_exp = 0;

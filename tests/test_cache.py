@@ -290,6 +290,18 @@ def test_tdp_decode_of_long_sequences(B, N, n, D, dtype, code, page, contexts, w
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_short_sequences_under_a_long_table(D):
+    """Pieces of a slab or none, with one tile and with two, behind one another: every run the same bits."""
+    bt = Batch(40, 3, 1, D, "bf16", "int8", 16, [(37 * b) % 300 - 1 for b in range(40)], seed=19)
+    table, q = _widened(bt.table, 4096, 16), bt.q.to(DEV)
+    outs = [ft.tdp_decode(q, bt.cache, table, bt.context, 0.1, return_lse=True) for _ in range(60)]
+    ft.check_status(DEV)
+    assert all(torch.equal(o, outs[0][0]) and torch.equal(m, outs[0][1]) for o, m in outs)
+    _tdp_check(bt, *outs[0], (None,) * 4, 0.1, True, heads=(1,))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("B,N,n,D,dtype,code,page,contexts,windows,parents", TDP[:10])
 def test_tdp_decode_under_a_long_table(B, N, n, D, dtype, code, page, contexts, windows, parents):
     """A table of more places than are in use takes another kernel where windows do not bound the tokens: the same definitions."""
