@@ -227,6 +227,10 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm<NT>) dps_decode_kern
       for (int k = 0; k < D / 32; ++k) raw[nt][k] = __ldg(reinterpret_cast<const uint4*>(q + k / (EPL / 8) * 4 * EPL + k % (EPL / 8) * 8));
     }
 
+    unsigned long long words[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) words[nt] = warp == 0 && ca.c.ancestors && nt * 8 + g < nq ? seen_word(ca, b, i0 + nt * 8 + g) : 0;
+
     // --- the ring: this warp takes tiles s0 + warp, + kWarps, ...
     const uint8_t* key_rows = (const uint8_t*)ca.c.codes + (a.key_part * part_rows + ((size_t)head << ca.page_log2)) * RB;
     const long long to_values = (long long)(a.value_part - a.key_part) * (long long)part_rows;
@@ -306,7 +310,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm<NT>) dps_decode_kern
         qf[nt][s][1] = pack_half(f[s * 4 + 2] * mul, f[s * 4 + 3] * mul);
       }
       if (warp == 0 && t == 0) {
-        const unsigned long long word = on && ca.c.ancestors ? seen_word(ca, b, i) : 0;
+        const unsigned long long word = words[nt];
         const int pos = ctx + (ca.c.ancestors ? __popcll(word) - 1 : i);
         s_word[nt * 8 + g] = word;
         s_pos[nt * 8 + g] = on ? pos : -1;
@@ -316,8 +320,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm<NT>) dps_decode_kern
     }
     __syncthreads();
     // from lo_all on every query attends to all of the context (those that are not there take no part in this: their results are not looked at)
-    int lo_all = 0;
-    for (int i = 0; i < nq; ++i) lo_all = max(lo_all, s_lo[i]);
+    const int lo_all = __reduce_max_sync(0xffffffffu, lane < nq ? s_lo[lane] : 0);
     float qs[NT][NQ];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
