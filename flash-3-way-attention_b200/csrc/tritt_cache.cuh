@@ -130,7 +130,8 @@ template <int CODE> struct Codes8 {
       if constexpr (CODE == TRITT_CODE_E4M3)
         pair = __nv_cvt_float2_to_fp8x2(make_float2(f[i], f[i + 1]), __NV_SATFINITE, __NV_E4M3);
       else
-        pair = ((uint32_t)__float2int_rn(f[i]) & 255u) | ((uint32_t)__float2int_rn(f[i + 1]) & 255u) << 8;
+        // (1.5 * 2^23 more leaves the rounded integer in the lowest bits; conversions are slow)
+        pair = __byte_perm(__float_as_uint(f[i] + 12582912.f), __float_as_uint(f[i + 1] + 12582912.f), 0x0040) & 0xffffu;
       w[i / 4] |= pair << (8 * (i % 4));
     }
     v = make_uint2(w[0], w[1]);
@@ -198,20 +199,32 @@ template <int L> __device__ __forceinline__ uint32_t largest_of_row(uint32_t m) 
   for (int o = L / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
   return m;
 }
-// A row's eight elements of this lane into its place.  All L lanes of the row call it; `on` is theirs in common.
-template <int CODE, int L>
-__device__ __forceinline__ void store_row(const CacheArgs& a, bool on, Place at, int part, int head, int col, const float (&f)[8]) {
-  const int byte = exponent_byte<CODE>(largest_of_row<L>(largest8(f)));
-  if (!on) return;
+// Two 16-bit maxima at a time: of eight elements' magnitudes, in either half of the word, and as fp32 bits.
+__device__ __forceinline__ uint32_t largest_halves(uint4 v) {
+  const uint32_t m = 0x7fff7fffu;
+  const uint32_t w = __vmaxu2(__vmaxu2(v.x & m, v.y & m), __vmaxu2(v.z & m, v.w & m));
+  return max(w & 0xffffu, w >> 16);
+}
+template <int L> __device__ __forceinline__ uint32_t largest_of_two_rows(uint32_t m) {
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
+  return m;
+}
+template <typename T> __device__ __forceinline__ uint32_t bits_of_half(uint32_t h) {
+  T x;
+  *reinterpret_cast<uint16_t*>(&x) = (uint16_t)h;
+  return __float_as_uint(to_f(x));
+}
+// A row's eight elements of this lane as codes for the exponent `byte`.
+template <int CODE> __device__ __forceinline__ Codes8<CODE> codes_of(int byte, const float (&f)[8]) {
   const float scale = to_code_scale(byte);
   float y[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) y[e] = byte == 255 ? 0.f : f[e] * scale;
+  for (int e = 0; e < 8; ++e) y[e] = f[e] * scale;
   Codes8<CODE> codes;
   codes.encode(y);
-  const size_t row = row_of(a, at, part, head);
-  codes.store((uint8_t*)a.c.codes + row * (size_t)(a.c.D * (CODE == TRITT_CODE_F16 ? 2 : 1)), col);
-  if (col == 0) a.c.exponents[row] = (unsigned char)byte;
+  if (byte == 255) codes.v = {};   // (a row that is not finite)
+  return codes;
 }
 
 // Append: a warp's row (eight elements from column `col` on of its first lanes) times v2 becomes W in the cache, with its log-sum-exp.  All
@@ -243,12 +256,7 @@ __device__ __forceinline__ void join_into_cache(const CacheArgs& a, int b, int h
     a.c.lse[lse_of(a, at, head)] = lse;
   }
   if (col < D) {
-    const float scale = to_code_scale(byte);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = byte == 255 ? 0.f : f[e] * scale;
-    Codes8<CODE> codes;
-    codes.encode(f);
-    codes.store((uint8_t*)a.c.codes + to * (size_t)(D * (CODE == TRITT_CODE_F16 ? 2 : 1)), col);
+    codes_of<CODE>(byte, f).store((uint8_t*)a.c.codes + to * (size_t)(D * (CODE == TRITT_CODE_F16 ? 2 : 1)), col);
   }
 }
 
