@@ -8,7 +8,8 @@
 // Bound by HBM: forward one read and one write of the rows, backward two reads and one write.  D / 8 lanes take a row, eight elements each:
 // two groups of four that lie R / 2 apart, so that a thread holds both of each rotated pair (neighbours where there is no rotation or
 // neighbours are rotated).  With eight neighbours a lane and the other half by shuffles the forward executed 202 instructions for eight
-// elements, and instruction issue bounded it (4 x 16 heads x 2048 x 128 bf16: 53 us, the backward 121).  Two fp32 numbers an instruction.
+// elements, and instruction issue bounded it (4 x 16 heads x 2048 x 128 bf16: 53 us, the backward 121).  Two fp32 numbers an instruction: 49 us (4.1 TB/s)
+// and 86 (3.5 TB/s, of which the last sums take 4).
 // The tables (a cosine and a sine, 8 bytes, for two elements) would be twice the traffic of 16-bit rows, so a thread keeps its position's
 // values for four heads and, where there are blocks enough, all three tensors.
 #include "tritt_common.cuh"
@@ -216,7 +217,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_rotary_fwd_kernel(const __g
 
 // A block takes one tensor's rows of tokens blockIdx.x, + gridDim.x, ... in groups: neighbouring slots (D / 8 lanes) kHeads heads each of a
 // token, whose rows are neighbours where the tensors come out of one projection (a block for each four heads read 1 KB here and
-// there: 98 us instead of 87 for 4 x 16 heads x 2048 x 128 bf16).  A slot's heads stay the same, so the weights' gradients add up
+// there: 98 us instead of 86 for 4 x 16 heads x 2048 x 128 bf16).  A slot's heads stay the same, so the weights' gradients add up
 // in registers: then over the block's slots, and by the kernel below over the blocks, always in the same order.
 template <typename T, int D>
 __global__ void __launch_bounds__(kNormThreads, 2) norm_rotary_bwd_kernel(const __grid_constant__ NormParams p) {

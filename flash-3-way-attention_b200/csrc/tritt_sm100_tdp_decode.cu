@@ -21,8 +21,13 @@
 //                 the loads of a tile are in flight before its stage is free.  They form tile b's A, and tell its rows' masks and scales
 //   warps 8-11    values in the same way, and tile a's A
 //   warps 12-19   one row a thread: maximum, exponentials, P; at the end of a piece the group's sum
-// (Keys and values from the same warps: each tile's loads took 1.3 us that nothing hid, 690 us for 8 tokens over 2040 at D=128, 16 heads, of
-// which 290 were theirs.  A formed by the soft-max warps: 15 us a piece, of which the products of a narrow window are one.)
+// Measured: 8 tokens over 2040, 16 heads of 128, float16 codes 374 us (products alone would take 166, exponentials 122); one token over up to
+// 700, 4 sequences of 8 heads of 64, e4m3 31 us.  Of the first a pair of tiles' slab takes 5.1 thousand cycles: 3.2 in a tile's soft-max (a warp a
+// scheduler works alone for most of it), 1.9 from its P to the next scores; the change of pieces costs 17 thousand a piece, the
+// group's sums 8 and the rows' A 13 of them, side by side.  Of the second 10 of the first 19 thousand cycles are the way to the first A.
+// Keys and values from the same warps: 1.3 us a slab that nothing hid (690 us then).  A formed by the soft-max warps: 15 us a piece.  P in quarters
+// with the next quarter's scores on their way: 448 us instead of 374 (more votes, more registers than there are).  A's codes on their way
+// before the tile is free: 398, its rows loaded side by side: 500 (the loading warps' tiles no longer fit in registers).
 #include "tritt_cache.cuh"
 #include "tritt_sm100.cuh"
 #include "tritt_sm100_tdp.cuh"

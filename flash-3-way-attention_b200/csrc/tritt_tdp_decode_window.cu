@@ -6,10 +6,9 @@
 // rows k of one new token at a time (m16n8k16 products, A = alpha q*K2 formed in registers), walks the 32-column blocks j that any of them
 // attends to, and sums its rows times V2; the sums of a new token meet in shared memory, in order, and leave as the result: one launch.
 //
-// Bound by instruction issue (about 25 a column block of 16 rows and element of its fragments) and, for few rows, by the chain load, convert,
-// product, exponential.  The kernel with tcgen05 tiles of 128 x 128 cells, which a window of 129 x 144 fills to a half and whose pieces cost
-// 8 us each, took 115 us for trees of 16 under windows 128/128/32/32 (8 sequences of 16 heads, D=64), this one 16.
-// Beyond what shared memory holds, or where the rows are many (from about 400 x 400 at D=64 on), the other kernel is the faster.
+// Bound by instruction issue (1780 a unit of 16 rows under a window of 129 and a band of 65: 56 % of the issue slots) and, for few rows, by the
+// chain load, convert, product, exponential.  Trees of 16 under windows 128/128/32/32, 8 sequences of 16 heads, D=64, int8: 58 us; the kernel
+// with tcgen05 tiles of 128 x 128 cells, which such a window fills to a half: 120.
 #include "tritt_cache.cuh"
 #include "tritt_sm100.cuh"
 #include "tritt_sm100_tdp.cuh"
@@ -413,14 +412,25 @@ size_t smem_of(const WindowParams& p, int D) {
 }
 
 // What a call's blocks stage, and how many new tokens each takes: as few as fill the chip, for the more, the more read a row once.  False: too much.
-bool plan(const tritt_cache_t& c, int k1w, int k2w, WindowParams& p) {
+//
+// Of two kernels for D=64 this one is the faster up to about 28 thousand cells (rows by columns) a new token, the one with tcgen05 tiles beyond.
+// Without a band, windows of 128: 17 us (4 sequences of 8 heads, one token), 40 (32 of 16), 76 (8 of 16, 16 tokens) against 20, 60, 115; of 200: 23,
+// 81, 163 against 21, 58, 143; with a band of 65, windows of 200: 17, 60, 105 against 21, 62, 150; of 300: 23, 82, 263 against 25, 103, 262.
+// At D=128 shared memory ends at windows of about 128, where they are as fast (25, 93, 141 against 23, 86, 158; with the band 21, 73, 108 against 23,
+// 70, 158).
+constexpr long long kMostCells64 = 28000;
+bool plan(const tritt_cache_t& c, int k1w, int k2w, int kkl, int kkr, WindowParams& p) {
   const long long tokens = (long long)c.page_size * c.table_pages + c.n;   // a sequence's most
   const long long rows = tokens < (long long)k2w + 1 ? tokens : (long long)k2w + 1;
   if (rows > 1024) return false;
+  const long long band = (long long)kkl + kkr + 16;   // of a unit's 16 rows
+  long long seen = tokens < (long long)k1w + 1 ? tokens : (long long)k1w + 1;
+  if (band < seen) seen = band;
+  if (c.D == 64 && rows * seen > kMostCells64) return false;
   p.tiles = (int)(rows + 15) / 16;
   const int pairs = c.B * c.N, most = kPartBytes / (p.tiles * (c.D + 2) * 4);
   // one wave of two blocks an SM where there are not more sequences and heads (a second one of a third as many costs as much as the
-  // first: trees of 16 under windows of 129, 128 of them: 3 blocks each 84 us, 2 each 55), but at least two units a warp
+  // first: trees of 16 under windows of 129, 128 of them: 3 blocks each 84 us, 2 each 58), but at least two units a warp
   const int blocks = 2 * num_sms() / pairs;
   int per = blocks < 1 ? c.n : (c.n + blocks - 1) / blocks;
   const int least = (2 * kWarps + p.tiles - 1) / p.tiles;
@@ -459,9 +469,9 @@ template <typename T16, int D> int by_code(const WindowParams& p, cudaStream_t s
 
 }  // namespace
 
-bool window_tdp_decode_applies(const tritt_cache_t& c, int k1w, int k2w) {
+bool window_tdp_decode_applies(const tritt_cache_t& c, int k1w, int k2w, int kkl, int kkr) {
   WindowParams p{};
-  return plan(c, k1w, k2w, p);
+  return plan(c, k1w, k2w, kkl, kkr, p);
 }
 
 int window_tdp_decode(const TdpDecodeArgs& a, void* o, float* lse, cudaStream_t stream) {
@@ -469,7 +479,7 @@ int window_tdp_decode(const TdpDecodeArgs& a, void* o, float* lse, cudaStream_t 
   p.a = a;
   p.o = o;
   p.lse = lse;
-  plan(a.cache.c, a.k1w, a.k2w, p);
+  plan(a.cache.c, a.k1w, a.k2w, a.kkl, a.kkr, p);
   if (a.dtype == TRITT_F16) return a.cache.c.D == 64 ? by_code<__half, 64>(p, stream) : by_code<__half, 128>(p, stream);
   return a.cache.c.D == 64 ? by_code<__nv_bfloat16, 64>(p, stream) : by_code<__nv_bfloat16, 128>(p, stream);
 }
