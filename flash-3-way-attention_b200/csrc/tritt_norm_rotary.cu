@@ -12,6 +12,7 @@
 // and 86 (3.5 TB/s, of which the last sums take 4).
 // The tables (a cosine and a sine, 8 bytes, for two elements) would be twice the traffic of 16-bit rows, so a thread keeps its position's
 // values for four heads and, where there are blocks enough, all three tensors.
+#include "tritt_cache.cuh"
 #include "tritt_common.cuh"
 
 #include <type_traits>
@@ -26,7 +27,8 @@ constexpr int kHeads = 4;   // heads of a token that a group of lanes takes at a
 struct NormParams {
   tritt_norm_rotary_t a;
   int chunks;          // of kHeads heads
-  float* partial;      // backward: [3][N][gridDim.x][D]
+  int blocks, groups;  // backward: its grid
+  float* partial;      // backward: [3][heads, or groups of heads][blocks][D]
   int* status;
 };
 
@@ -219,9 +221,21 @@ __global__ void __launch_bounds__(kNormThreads) norm_rotary_fwd_kernel(const __g
 // token, whose rows are neighbours where the tensors come out of one projection (a block for each four heads read 1 KB here and
 // there: 98 us instead of 86 for 4 x 16 heads x 2048 x 128 bf16).  A slot's heads stay the same, so the weights' gradients add up
 // in registers: then over the block's slots, and by the kernel below over the blocks, always in the same order.
+//
+// Rows of 16-bit types come by asynchronous copies, kStages - 1 tokens ahead, each thread's into places of its own: loads to
+// registers, of which there are no more, waited for one token's rows while nothing else was on its way.
+constexpr int kStages = 3;
+constexpr int kStageBytes = kHeads * 4 * kNormThreads * 8;
+template <typename T> constexpr int kBwdSmem = sizeof(T) == 2 ? kStages * kStageBytes : 0;
+__device__ __forceinline__ void copy8(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kNormThreads, 2) norm_rotary_bwd_kernel(const __grid_constant__ NormParams p) {
   constexpr int L = D / 8, kSlots = kNormThreads / L;
+  constexpr bool kAsync = sizeof(T) == 2;
+  extern __shared__ __align__(16) uint8_t staged[];
   __shared__ float sums[kSlots][D];
   const int lane = threadIdx.x % L, slot = threadIdx.x / L;
   const Cols cols = cols_of(lane, p.a.rot, p.a.interleaved);
@@ -240,28 +254,61 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_rotary_bwd_kernel(const 
     for (int k = 0; k < 4; ++k) dw[i][k] = both(0.f);
   float2 w[4];
   if (!p.a.weight_heads) load_weights<T>(p, which, 0, cols, w);
-  for (uint32_t first = blockIdx.x * at_once; first < tokens; first += gridDim.x * at_once) {
+  const uint32_t step = gridDim.x * at_once;
+  uint2* const mine = reinterpret_cast<uint2*>(staged) + threadIdx.x;   // [stage][head][x, x, dy, dy][thread]
+  auto send = [&](uint32_t token, int stage) {
+    if constexpr (kAsync) {
+      if (used && token < tokens) {
+        const int b = token / p.a.T, t = token - (uint32_t)b * p.a.T;
+        const T *x0 = (const T*)rx.p + row_offset(rx, b, h0, t), *y0 = (const T*)ry.p + row_offset(ry, b, h0, t);
+        uint2* to = mine + stage * (kStageBytes / 8);
+#pragma unroll
+        for (int i = 0; i < kHeads; ++i)
+          if (h0 + i < p.a.N) {
+            const T *x = x0 + i * rx.stride_n, *y = y0 + i * ry.stride_n;
+            copy8(to + (i * 4 + 0) * kNormThreads, x + cols.a);
+            copy8(to + (i * 4 + 1) * kNormThreads, x + cols.b);
+            copy8(to + (i * 4 + 2) * kNormThreads, y + cols.a);
+            copy8(to + (i * 4 + 3) * kNormThreads, y + cols.b);
+          }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+  };
+  int stage = 0;
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) send(blockIdx.x * at_once + slot / here + s * step, s);
+  for (uint32_t first = blockIdx.x * at_once; first < tokens; first += step) {
     const uint32_t token = first + slot / here;
     const bool live = used && token < tokens;
     const int b = live ? token / p.a.T : 0, t = live ? token - (uint32_t)b * p.a.T : 0;
-    Eight<T> in[kHeads], up[kHeads];
-    const T *x0 = (const T*)rx.p + row_offset(rx, b, h0, t), *y0 = (const T*)ry.p + row_offset(ry, b, h0, t);
+    send(token + (kStages - 1) * step, stage == 0 ? kStages - 1 : stage - 1);
+    Eight<T> in[kAsync ? 1 : kHeads], up[kAsync ? 1 : kHeads];
     T* d0 = (T*)rd.p + row_offset(rd, b, h0, t);
+    if constexpr (!kAsync) {
+      const T *x0 = (const T*)rx.p + row_offset(rx, b, h0, t), *y0 = (const T*)ry.p + row_offset(ry, b, h0, t);
 #pragma unroll
-    for (int i = 0; i < kHeads; ++i)
-      if (live && h0 + i < p.a.N) {
-        in[i].load(x0 + i * rx.stride_n, cols);
-        up[i].load(y0 + i * ry.stride_n, cols);
-      }
+      for (int i = 0; i < kHeads; ++i)
+        if (live && h0 + i < p.a.N) {
+          in[i].load(x0 + i * rx.stride_n, cols);
+          up[i].load(y0 + i * ry.stride_n, cols);
+        }
+    }
     Turn turn;
     if (p.a.rot) turn = load_turn(p, b, t, lane);
+    if constexpr (kAsync) asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+    const uint2* from = mine + stage * (kStageBytes / 8);
 #pragma unroll
     for (int i = 0; i < kHeads; ++i) {
       const bool on = live && h0 + i < p.a.N;
       float2 x[4] = {both(0.f), both(0.f), both(0.f), both(0.f)}, g[4] = {both(0.f), both(0.f), both(0.f), both(0.f)};
       if (on) {
-        in[i].get(x);
-        up[i].get(g);
+        if constexpr (kAsync) {
+          in[0].v[0] = from[(i * 4 + 0) * kNormThreads], in[0].v[1] = from[(i * 4 + 1) * kNormThreads];
+          up[0].v[0] = from[(i * 4 + 2) * kNormThreads], up[0].v[1] = from[(i * 4 + 3) * kNormThreads];
+        }
+        in[kAsync ? 0 : i].get(x);
+        up[kAsync ? 0 : i].get(g);
       }
       if (p.a.rot) rotate(interleaved, turn, -1.f, g);
       const float r = rsqrtf(row_sum<L>(dot(x, x)) * (1.f / D) + p.a.eps);
@@ -277,8 +324,25 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_rotary_bwd_kernel(const 
       for (int k = 0; k < 4; ++k) g[k] = mul2(fma2(x[k], both(mean), g[k]), both(r));
       if (on) Eight<T>::store(d0 + i * rd.stride_n, cols, g);
     }
+    if (++stage == kStages) stage = 0;
   }
+  let_next_start();
   if (!weights) return;
+  if (!p.a.weight_heads) {   // (a sum for all of the block's heads)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+#pragma unroll
+      for (int i = 1; i < kHeads; ++i) dw[0][k] = make_float2(dw[0][k].x + dw[i][k].x, dw[0][k].y + dw[i][k].y);
+      *reinterpret_cast<float2*>(&sums[slot][(k < 2 ? cols.a : cols.b) + 2 * (k & 1)]) = dw[0][k];
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < D; c += kNormThreads) {
+      float total = 0.f;
+      for (int s = 0; s < at_once * here; ++s) total += sums[s][c];
+      p.partial[(((size_t)which * groups + blockIdx.y % groups) * gridDim.x + blockIdx.x) * D + c] = total;
+    }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < kHeads; ++i) {
     __syncthreads();
@@ -298,15 +362,16 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_rotary_bwd_kernel(const 
   }
 }
 
-// Adds up `rows` partial sums of each column: those of a head, or of all heads.  One block a (tensor, head or all), 32 columns a warp-row.
+// Adds up the blocks' sums of each column: those of a head, or of all heads' groups.  One block a (tensor, head or all), 32 columns a warp-row.
 template <typename T>
-__global__ void __launch_bounds__(1024) norm_rotary_weights_kernel(const __grid_constant__ NormParams p, int blocks) {
+__global__ void __launch_bounds__(1024) norm_rotary_weights_kernel(const __grid_constant__ NormParams p) {
+  wait_for_previous();
   __shared__ float sums[32][33];
-  const int which = blockIdx.z, head = blockIdx.y, D = p.a.D;
+  const int which = blockIdx.z, head = blockIdx.y, D = p.a.D, blocks = p.blocks;
   const int c = blockIdx.x * 32 + threadIdx.x % 32, group = threadIdx.x / 32;
   if (p.a.dw[which] == nullptr) return;
-  const int rows = p.a.weight_heads ? blocks : blocks * p.a.N;
-  const float* base = p.partial + ((size_t)which * p.a.N + head) * blocks * D;
+  const int sets = p.a.weight_heads ? p.a.N : p.groups, rows = p.a.weight_heads ? blocks : blocks * p.groups;
+  const float* base = p.partial + ((size_t)which * sets + head) * blocks * D;
   float total = 0.f;
   if (c < D)
 #pragma unroll 8
@@ -401,17 +466,15 @@ template <typename T, int D> int launch_fwd(const NormParams& p, cudaStream_t st
   return 0;
 }
 
-template <typename T, int D> int launch_bwd(const NormParams& p, cudaStream_t stream) {
+template <typename T, int D> int launch_bwd(NormParams p, cudaStream_t stream) {
   const Grid grid = bwd_grid(p.a);
-  const int blocks = grid.blocks;
-  norm_rotary_bwd_kernel<T, D><<<dim3(blocks, 3 * grid.groups), kNormThreads, 0, stream>>>(p);
-  count_launch();
-  TRITT_CUDA_OK(cudaGetLastError());
+  p.blocks = grid.blocks;
+  p.groups = grid.groups;
+  auto kern = norm_rotary_bwd_kernel<T, D>;
+  if (kBwdSmem<T>) TRITT_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kBwdSmem<T>));
+  if (int rc = launch_kernel_after(kern, dim3(p.blocks, 3 * p.groups), kNormThreads, kBwdSmem<T>, stream, false, p)) return rc;
   if (!p.partial) return 0;
-  norm_rotary_weights_kernel<T><<<dim3((D + 31) / 32, p.a.weight_heads ? p.a.N : 1, 3), 1024, 0, stream>>>(p, blocks);
-  count_launch();
-  TRITT_CUDA_OK(cudaGetLastError());
-  return 0;
+  return launch_kernel_after(norm_rotary_weights_kernel<T>, dim3((D + 31) / 32, p.a.weight_heads ? p.a.N : 1, 3), 1024, 0, stream, true, p);
 }
 
 template <typename T> int by_size(const NormParams& p, bool backward, cudaStream_t stream) {
@@ -439,7 +502,7 @@ extern "C" {
 
 int tritt_qk_norm_rotary_fwd(const tritt_norm_rotary_t* a, int* status_word, tritt_stream_t stream) {
   if (int rc = check(a, false)) return rc;
-  NormParams p{*a, (a->N + kHeads - 1) / kHeads, nullptr, status_word};
+  NormParams p{*a, (a->N + kHeads - 1) / kHeads, 0, 0, nullptr, status_word};
   return by_type(p, false, (cudaStream_t)stream);
 }
 
@@ -460,7 +523,7 @@ int tritt_qk_norm_rotary_bwd(const tritt_norm_rotary_t* a, void* workspace, size
     set_error("too many heads");
     return -11;
   }
-  NormParams p{*a, (a->N + kHeads - 1) / kHeads, need ? (float*)workspace : nullptr, status_word};
+  NormParams p{*a, (a->N + kHeads - 1) / kHeads, 0, 0, need ? (float*)workspace : nullptr, status_word};
   return by_type(p, true, (cudaStream_t)stream);
 }
 
