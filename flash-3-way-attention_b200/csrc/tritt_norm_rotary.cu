@@ -222,18 +222,20 @@ __global__ void __launch_bounds__(kNormThreads) norm_rotary_fwd_kernel(const __g
 // there: 98 us instead of 86 for 4 x 16 heads x 2048 x 128 bf16).  A slot's heads stay the same, so the weights' gradients add up
 // in registers: then over the block's slots, and by the kernel below over the blocks, always in the same order.
 //
-// Rows of 16-bit types come by asynchronous copies, kStages - 1 tokens ahead, each thread's into places of its own: loads to
-// registers, of which there are no more, waited for one token's rows while nothing else was on its way.
-constexpr int kStages = 3;
+// Rows of 16-bit types come by asynchronous copies, one or two tokens ahead, each thread's into places of its own: loads to
+// registers, of which there are no more, waited for one token's rows while nothing else was on its way.  SHARED: one weight for all heads, so one
+// sum, and registers for three blocks an SM.
+template <typename T, bool SHARED> constexpr int kPerSm = SHARED && sizeof(T) == 2 ? 3 : 2;
+template <bool SHARED> constexpr int kStages = SHARED ? 2 : 3;
 constexpr int kStageBytes = kHeads * 4 * kNormThreads * 8;
-template <typename T> constexpr int kBwdSmem = sizeof(T) == 2 ? kStages * kStageBytes : 0;
+template <typename T, bool SHARED> constexpr int kBwdSmem = sizeof(T) == 2 ? kStages<SHARED> * kStageBytes : 0;
 __device__ __forceinline__ void copy8(void* dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kNormThreads, 2) norm_rotary_bwd_kernel(const __grid_constant__ NormParams p) {
-  constexpr int L = D / 8, kSlots = kNormThreads / L;
+template <typename T, int D, bool SHARED>
+__global__ void __launch_bounds__(kNormThreads, kPerSm<T, SHARED>) norm_rotary_bwd_kernel(const __grid_constant__ NormParams p) {
+  constexpr int L = D / 8, kSlots = kNormThreads / L, kSums = SHARED ? 1 : kHeads, NS = kStages<SHARED>;
   constexpr bool kAsync = sizeof(T) == 2;
   extern __shared__ __align__(16) uint8_t staged[];
   __shared__ float sums[kSlots][D];
@@ -247,13 +249,13 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_rotary_bwd_kernel(const 
   const uint32_t tokens = (uint32_t)p.a.B * p.a.T;
   const bool weights = p.partial != nullptr && p.a.dw[which] != nullptr;
   const tritt_rows_t rx = p.a.x[which], ry = p.a.y[which], rd = p.a.dx[which];
-  float2 dw[kHeads][4];
+  float2 dw[kSums][4];
 #pragma unroll
-  for (int i = 0; i < kHeads; ++i)
+  for (int i = 0; i < kSums; ++i)
 #pragma unroll
     for (int k = 0; k < 4; ++k) dw[i][k] = both(0.f);
   float2 w[4];
-  if (!p.a.weight_heads) load_weights<T>(p, which, 0, cols, w);
+  if (SHARED) load_weights<T>(p, which, 0, cols, w);
   const uint32_t step = gridDim.x * at_once;
   uint2* const mine = reinterpret_cast<uint2*>(staged) + threadIdx.x;   // [stage][head][x, x, dy, dy][thread]
   auto send = [&](uint32_t token, int stage) {
@@ -277,12 +279,12 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_rotary_bwd_kernel(const 
   };
   int stage = 0;
 #pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) send(blockIdx.x * at_once + slot / here + s * step, s);
+  for (int s = 0; s < NS - 1; ++s) send(blockIdx.x * at_once + slot / here + s * step, s);
   for (uint32_t first = blockIdx.x * at_once; first < tokens; first += step) {
     const uint32_t token = first + slot / here;
     const bool live = used && token < tokens;
     const int b = live ? token / p.a.T : 0, t = live ? token - (uint32_t)b * p.a.T : 0;
-    send(token + (kStages - 1) * step, stage == 0 ? kStages - 1 : stage - 1);
+    send(token + (NS - 1) * step, stage == 0 ? NS - 1 : stage - 1);
     Eight<T> in[kAsync ? 1 : kHeads], up[kAsync ? 1 : kHeads];
     T* d0 = (T*)rd.p + row_offset(rd, b, h0, t);
     if constexpr (!kAsync) {
@@ -296,7 +298,7 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_rotary_bwd_kernel(const 
     }
     Turn turn;
     if (p.a.rot) turn = load_turn(p, b, t, lane);
-    if constexpr (kAsync) asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+    if constexpr (kAsync) asm volatile("cp.async.wait_group %0;" ::"n"(NS - 1) : "memory");
     const uint2* from = mine + stage * (kStageBytes / 8);
 #pragma unroll
     for (int i = 0; i < kHeads; ++i) {
@@ -312,11 +314,11 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_rotary_bwd_kernel(const 
       }
       if (p.a.rot) rotate(interleaved, turn, -1.f, g);
       const float r = rsqrtf(row_sum<L>(dot(x, x)) * (1.f / D) + p.a.eps);
-      if (p.a.weight_heads && on) load_weights<T>(p, which, h0 + i, cols, w);
+      if (!SHARED && on) load_weights<T>(p, which, h0 + i, cols, w);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         x[k] = mul2(x[k], both(r));
-        if (on) dw[i][k] = fma2(g[k], x[k], dw[i][k]);
+        if (on) dw[SHARED ? 0 : i][k] = fma2(g[k], x[k], dw[SHARED ? 0 : i][k]);
         g[k] = mul2(g[k], w[k]);
       }
       const float mean = row_sum<L>(dot(g, x)) * (-1.f / D);
@@ -324,17 +326,13 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_rotary_bwd_kernel(const 
       for (int k = 0; k < 4; ++k) g[k] = mul2(fma2(x[k], both(mean), g[k]), both(r));
       if (on) Eight<T>::store(d0 + i * rd.stride_n, cols, g);
     }
-    if (++stage == kStages) stage = 0;
+    if (++stage == NS) stage = 0;
   }
   let_next_start();
   if (!weights) return;
-  if (!p.a.weight_heads) {   // (a sum for all of the block's heads)
+  if (SHARED) {   // (a sum for all of the block's heads)
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-#pragma unroll
-      for (int i = 1; i < kHeads; ++i) dw[0][k] = make_float2(dw[0][k].x + dw[i][k].x, dw[0][k].y + dw[i][k].y);
-      *reinterpret_cast<float2*>(&sums[slot][(k < 2 ? cols.a : cols.b) + 2 * (k & 1)]) = dw[0][k];
-    }
+    for (int k = 0; k < 4; ++k) *reinterpret_cast<float2*>(&sums[slot][(k < 2 ? cols.a : cols.b) + 2 * (k & 1)]) = dw[0][k];
     __syncthreads();
     for (int c = threadIdx.x; c < D; c += kNormThreads) {
       float total = 0.f;
@@ -344,7 +342,7 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_rotary_bwd_kernel(const 
     return;
   }
 #pragma unroll
-  for (int i = 0; i < kHeads; ++i) {
+  for (int i = 0; i < kSums; ++i) {
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -389,14 +387,15 @@ __global__ void __launch_bounds__(1024) norm_rotary_weights_kernel(const __grid_
   }
 }
 
-// The backward's grid: blocks along the tokens, as many as the chip holds at once (two an SM), and groups of a token's heads.
+// The backward's grid: blocks along the tokens, as many as the chip holds at once, and groups of a token's heads.
 struct Grid {
   int blocks, groups;
 };
 Grid bwd_grid(const tritt_norm_rotary_t& a) {
   const int chunks = (a.N + kHeads - 1) / kHeads, slots = kNormThreads / (a.D / 8);
   const int here = chunks < slots ? chunks : slots, groups = (chunks + here - 1) / here, at_once = slots / here;
-  const long long most = ((long long)a.B * a.T + at_once - 1) / at_once, fill = 2LL * kSms / (3 * groups);
+  const long long per_sm = a.dtype == TRITT_F32 ? kPerSm<float, true> : a.weight_heads ? kPerSm<__half, false> : kPerSm<__half, true>;
+  const long long most = ((long long)a.B * a.T + at_once - 1) / at_once, fill = per_sm * kSms / (3 * groups);
   return Grid{(int)(most < fill ? most : fill < 1 ? 1 : fill), groups};
 }
 
@@ -470,9 +469,12 @@ template <typename T, int D> int launch_bwd(NormParams p, cudaStream_t stream) {
   const Grid grid = bwd_grid(p.a);
   p.blocks = grid.blocks;
   p.groups = grid.groups;
-  auto kern = norm_rotary_bwd_kernel<T, D>;
-  if (kBwdSmem<T>) TRITT_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kBwdSmem<T>));
-  if (int rc = launch_kernel_after(kern, dim3(p.blocks, 3 * p.groups), kNormThreads, kBwdSmem<T>, stream, false, p)) return rc;
+  auto run = [&](auto kern, int bytes) -> int {
+    if (bytes) TRITT_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    return launch_kernel_after(kern, dim3(p.blocks, 3 * p.groups), kNormThreads, bytes, stream, false, p);
+  };
+  if (int rc = p.a.weight_heads ? run(norm_rotary_bwd_kernel<T, D, false>, kBwdSmem<T, false>) : run(norm_rotary_bwd_kernel<T, D, true>, kBwdSmem<T, true>))
+    return rc;
   if (!p.partial) return 0;
   return launch_kernel_after(norm_rotary_weights_kernel<T>, dim3((D + 31) / 32, p.a.weight_heads ? p.a.N : 1, 3), 1024, 0, stream, true, p);
 }
