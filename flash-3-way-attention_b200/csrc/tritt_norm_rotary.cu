@@ -8,8 +8,8 @@
 // Bound by HBM: forward one read and one write of the rows, backward two reads and one write.  D / 8 lanes take a row, eight elements each:
 // two groups of four that lie R / 2 apart, so that a thread holds both of each rotated pair (neighbours where there is no rotation or
 // neighbours are rotated).  With eight neighbours a lane and the other half by shuffles the forward executed 202 instructions for eight
-// elements, and instruction issue bounded it (4 x 16 heads x 2048 x 128 bf16: 53 us, the backward 121).  Two fp32 numbers an instruction: 49 us (4.1 TB/s)
-// and 86 (3.5 TB/s, of which the last sums take 4).
+// elements, and instruction issue bounded it (4 x 16 heads x 2048 x 128 bf16: 53 us, the backward 121).  Two fp32 numbers an instruction: 39 us (5.1 TB/s);
+// the backward, whose chains of two sums over a row's lanes leave half of the issue slots, 70 (4.3 TB/s) and 4.5 for the weights' last sums.
 // The tables (a cosine and a sine, 8 bytes, for two elements) would be twice the traffic of 16-bit rows, so a thread keeps its position's
 // values for four heads and, where there are blocks enough, all three tensors.
 #include "tritt_cache.cuh"
@@ -219,12 +219,12 @@ __global__ void __launch_bounds__(kNormThreads) norm_rotary_fwd_kernel(const __g
 
 // A block takes one tensor's rows of tokens blockIdx.x, + gridDim.x, ... in groups: neighbouring slots (D / 8 lanes) kHeads heads each of a
 // token, whose rows are neighbours where the tensors come out of one projection (a block for each four heads read 1 KB here and
-// there: 98 us instead of 86 for 4 x 16 heads x 2048 x 128 bf16).  A slot's heads stay the same, so the weights' gradients add up
+// there: 98 us instead of 86, then, for 4 x 16 heads x 2048 x 128 bf16).  A slot's heads stay the same, so the weights' gradients add up
 // in registers: then over the block's slots, and by the kernel below over the blocks, always in the same order.
 //
 // Rows of 16-bit types come by asynchronous copies, one or two tokens ahead, each thread's into places of its own: loads to
-// registers, of which there are no more, waited for one token's rows while nothing else was on its way.  SHARED: one weight for all heads, so one
-// sum, and registers for three blocks an SM.
+// registers, of which there are no more, waited for one token's rows while nothing else was on its way (86 us then, 77 with the copies).  SHARED: one
+// weight for all heads, so one sum, and registers for three blocks an SM (73 us); tokens found by counting instead of division (70).
 template <typename T, bool SHARED> constexpr int kPerSm = SHARED && sizeof(T) == 2 ? 3 : 2;
 template <bool SHARED> constexpr int kStages = SHARED ? 2 : 3;
 constexpr int kStageBytes = kHeads * 4 * kNormThreads * 8;
@@ -258,10 +258,23 @@ __global__ void __launch_bounds__(kNormThreads, kPerSm<T, SHARED>) norm_rotary_b
   if (SHARED) load_weights<T>(p, which, 0, cols, w);
   const uint32_t step = gridDim.x * at_once;
   uint2* const mine = reinterpret_cast<uint2*>(staged) + threadIdx.x;   // [stage][head][x, x, dy, dy][thread]
-  auto send = [&](uint32_t token, int stage) {
+  // a thread's token as batch and position, found by division once, then step by step
+  struct Token {
+    uint32_t n;
+    int b, t;
+  };
+  const int step_b = (int)(step / (uint32_t)p.a.T), step_t = (int)(step - (uint32_t)step_b * p.a.T);
+  auto next = [&](Token k) {
+    k.n += step;
+    k.b += step_b;
+    k.t += step_t;
+    if (k.t >= p.a.T) k.t -= p.a.T, ++k.b;
+    return k;
+  };
+  auto send = [&](Token k, int stage) {
     if constexpr (kAsync) {
-      if (used && token < tokens) {
-        const int b = token / p.a.T, t = token - (uint32_t)b * p.a.T;
+      if (used && k.n < tokens) {
+        const int b = k.b, t = k.t;
         const T *x0 = (const T*)rx.p + row_offset(rx, b, h0, t), *y0 = (const T*)ry.p + row_offset(ry, b, h0, t);
         uint2* to = mine + stage * (kStageBytes / 8);
 #pragma unroll
@@ -278,13 +291,15 @@ __global__ void __launch_bounds__(kNormThreads, kPerSm<T, SHARED>) norm_rotary_b
     }
   };
   int stage = 0;
+  Token now{blockIdx.x * at_once + slot / here, 0, 0};
+  now.b = (int)(now.n / (uint32_t)p.a.T), now.t = (int)(now.n - (uint32_t)now.b * p.a.T);
+  Token ahead = now;
 #pragma unroll
-  for (int s = 0; s < NS - 1; ++s) send(blockIdx.x * at_once + slot / here + s * step, s);
-  for (uint32_t first = blockIdx.x * at_once; first < tokens; first += step) {
-    const uint32_t token = first + slot / here;
-    const bool live = used && token < tokens;
-    const int b = live ? token / p.a.T : 0, t = live ? token - (uint32_t)b * p.a.T : 0;
-    send(token + (NS - 1) * step, stage == 0 ? NS - 1 : stage - 1);
+  for (int s = 0; s < NS - 1; ++s, ahead = next(ahead)) send(ahead, s);
+  for (uint32_t first = blockIdx.x * at_once; first < tokens; first += step, now = next(now), ahead = next(ahead)) {
+    const bool live = used && now.n < tokens;
+    const int b = live ? now.b : 0, t = live ? now.t : 0;
+    send(ahead, stage == 0 ? NS - 1 : stage - 1);
     Eight<T> in[kAsync ? 1 : kHeads], up[kAsync ? 1 : kHeads];
     T* d0 = (T*)rd.p + row_offset(rd, b, h0, t);
     if constexpr (!kAsync) {
@@ -302,16 +317,17 @@ __global__ void __launch_bounds__(kNormThreads, kPerSm<T, SHARED>) norm_rotary_b
     const uint2* from = mine + stage * (kStageBytes / 8);
 #pragma unroll
     for (int i = 0; i < kHeads; ++i) {
+      // (what a row that is not there leaves in its lanes is not looked at: its sums cross no other row's)
       const bool on = live && h0 + i < p.a.N;
-      float2 x[4] = {both(0.f), both(0.f), both(0.f), both(0.f)}, g[4] = {both(0.f), both(0.f), both(0.f), both(0.f)};
-      if (on) {
-        if constexpr (kAsync) {
-          in[0].v[0] = from[(i * 4 + 0) * kNormThreads], in[0].v[1] = from[(i * 4 + 1) * kNormThreads];
-          up[0].v[0] = from[(i * 4 + 2) * kNormThreads], up[0].v[1] = from[(i * 4 + 3) * kNormThreads];
-        }
-        in[kAsync ? 0 : i].get(x);
-        up[kAsync ? 0 : i].get(g);
+      float2 x[4], g[4];
+      if constexpr (kAsync) {
+        in[0].v[0] = from[(i * 4 + 0) * kNormThreads], in[0].v[1] = from[(i * 4 + 1) * kNormThreads];
+        up[0].v[0] = from[(i * 4 + 2) * kNormThreads], up[0].v[1] = from[(i * 4 + 3) * kNormThreads];
+      } else if (!on) {
+        in[i] = up[i] = {};
       }
+      in[kAsync ? 0 : i].get(x);
+      up[kAsync ? 0 : i].get(g);
       if (p.a.rot) rotate(interleaved, turn, -1.f, g);
       const float r = rsqrtf(row_sum<L>(dot(x, x)) * (1.f / D) + p.a.eps);
       if (!SHARED && on) load_weights<T>(p, which, h0 + i, cols, w);
