@@ -141,47 +141,40 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm<NT>) dps_decode_kern
     fence_barrier_init();
   }
   if (warp == 0) {
-    // the whole line's length: 32 sequences at a time
-    long long total = 0, groups = 0;
-    for (int b0 = 0; b0 < ca.c.B; b0 += 32) {
+    // the whole line's length, 32 sequences at a time, and the sequence of this block's first step (a walk from sequence to sequence took 200
+    // cycles each)
+    long long total = 0, groups = 0, behind = 0, here = 0, groups_before = 0;   // steps, groups; of the lane's sequence: up to its end, its own
+    auto sums = [&](int b0, bool write) {
       const int b = b0 + lane;
       Line l{};
       if (b < ca.c.B) l = line_of<TK, Q>(a, b);
-      const long long ng = (long long)l.groups * ca.c.N, steps = ng * l.tiles;
-      long long s = steps, q = ng;   // sums up to this lane
+      const long long ng = (long long)l.groups * ca.c.N;
+      here = ng * l.tiles;
+      long long s = here, q = ng;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const long long s2 = __shfl_up_sync(0xffffffffu, s, o), q2 = __shfl_up_sync(0xffffffffu, q, o);
         if (lane >= o) s += s2, q += q2;
       }
-      if (blockIdx.x == 0 && b < ca.c.B) p.table[b] = LineEntry{total + s - steps, groups + q - ng, l};
-      total += __shfl_sync(0xffffffffu, s, 31);
-      groups += __shfl_sync(0xffffffffu, q, 31);
-    }
+      behind = total + s;
+      groups_before = groups + q - ng;
+      if (write && blockIdx.x == 0 && b < ca.c.B) p.table[b] = LineEntry{behind - here, groups_before, l};
+      total = __shfl_sync(0xffffffffu, behind, 31);
+      groups = __shfl_sync(0xffffffffu, groups + q, 31);
+    };
+    for (int b0 = 0; b0 < ca.c.B; b0 += 32) sums(b0, true);
     if (lane == 0) s_total = total, s_abort = 0;
-    // the sequence of this block's first step (a walk from sequence to sequence took 200 cycles each)
-    const int parts = parts_of(total, p.ctas);
-    const long long x = (long long)blockIdx.x * total / parts;
-    long long before = 0, groups_before = 0;
-    for (int b0 = 0; b0 < ca.c.B && (int)blockIdx.x < parts; b0 += 32) {
-      const int b = b0 + lane;
-      Line l{};
-      if (b < ca.c.B) l = line_of<TK, Q>(a, b);
-      const long long ng = (long long)l.groups * ca.c.N, steps = ng * l.tiles;
-      long long s = steps, q = ng;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long s2 = __shfl_up_sync(0xffffffffu, s, o), q2 = __shfl_up_sync(0xffffffffu, q, o);
-        if (lane >= o) s += s2, q += q2;
+    const long long x = (long long)blockIdx.x * total / parts_of(total, p.ctas);
+    int b0 = 0;
+    if (ca.c.B > 32) {
+      total = groups = 0;
+      for (; b0 < ca.c.B; b0 += 32) {
+        sums(b0, false);
+        if (x < total) break;
       }
-      const uint32_t behind = __ballot_sync(0xffffffffu, x < before + s);
-      if (behind) {
-        if (lane == __ffs(behind) - 1) s_first = b, s_base = before + s - steps, s_groups = groups_before + q - ng;
-        break;
-      }
-      before += __shfl_sync(0xffffffffu, s, 31);
-      groups_before += __shfl_sync(0xffffffffu, q, 31);
     }
+    const uint32_t found = __ballot_sync(0xffffffffu, x < behind);
+    if (found && lane == __ffs(found) - 1) s_first = b0 + lane, s_base = behind - here, s_groups = groups_before;
   }
   __syncthreads();
   const long long total = s_total;

@@ -97,8 +97,6 @@ struct Misc {
   Item items[kItems];
   uint32_t tmem_base;
   int abort_flag;
-  int first_b;
-  long long first_base, total;   // of the sequence with this CTA's first step; of all
 };
 static_assert(sizeof(Misc) <= 1536, "shared memory of the barriers");
 
@@ -439,45 +437,39 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
     tmem_alloc(&ms.tmem_base, 512);
     tmem_relinquish();
   }
-  if (warp == 2) {
-    // the whole line's length, and the sequence of this CTA's first step: 32 sequences at a time
-    long long total = 0;
-    for (int b0 = 0; b0 < ca.c.B; b0 += 32) {
+  Walk walk{};
+  if (warp == 1) {
+    // the whole line's length, 32 sequences at a time, and the sequence of this CTA's first step (a walk from sequence to sequence took 200
+    // cycles each)
+    long long total = 0, behind = 0, here = 0;   // steps; of the lane's sequence: those up to its end, its own
+    auto sums = [&](int b0, bool write) {
       const int b = b0 + lane;
       Line l{};
       if (b < ca.c.B) l = line_of(a, b);
-      const long long steps = (long long)l.pairs * ca.c.N * l.slabs;
-      long long s = steps;   // sums up to this lane
+      here = (long long)l.pairs * ca.c.N * l.slabs;
+      long long s = here;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const long long s2 = __shfl_up_sync(0xffffffffu, s, o);
         if (lane >= o) s += s2;
       }
-      if (blockIdx.x == 0 && b < ca.c.B) p.table[b] = LineEntry{total + s - steps, l};
-      total += __shfl_sync(0xffffffffu, s, 31);
-    }
-    if (lane == 0) ms.total = total;
-    // the sequence of this CTA's first step
-    const long long x = (long long)blockIdx.x * total / p.ctas;
-    long long before = 0;
-    for (int b0 = 0; b0 < ca.c.B && total > 0; b0 += 32) {
-      const int b = b0 + lane;
-      Line l{};
-      if (b < ca.c.B) l = line_of(a, b);
-      const long long steps = (long long)l.pairs * ca.c.N * l.slabs;
-      long long s = steps;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long s2 = __shfl_up_sync(0xffffffffu, s, o);
-        if (lane >= o) s += s2;
+      behind = total + s;
+      if (write && blockIdx.x == 0 && b < ca.c.B) p.table[b] = LineEntry{behind - here, l};
+      total = __shfl_sync(0xffffffffu, behind, 31);
+    };
+    for (int b0 = 0; b0 < ca.c.B; b0 += 32) sums(b0, true);
+    const long long steps = total, x = (long long)blockIdx.x * steps / p.ctas;
+    int b0 = 0;
+    if (ca.c.B > 32) {
+      total = 0;
+      for (; b0 < ca.c.B; b0 += 32) {
+        sums(b0, false);
+        if (x < total) break;
       }
-      const uint32_t behind = __ballot_sync(0xffffffffu, x < before + s);
-      if (behind) {
-        if (lane == __ffs(behind) - 1) ms.first_b = b, ms.first_base = before + s - steps;
-        break;
-      }
-      before += __shfl_sync(0xffffffffu, s, 31);
     }
+    const uint32_t found = __ballot_sync(0xffffffffu, x < behind);
+    const int at = found ? __ffs(found) - 1 : 0;
+    walk = start_walk(p, found ? steps : 0, b0 + at, __shfl_sync(0xffffffffu, behind - here, at));
   }
   let_next_start();
   tc_fence_before();
@@ -504,7 +496,6 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
     set_regs<kRegsLaunch, kRegsIssue>();
     if (warp == 1) {
       // ------------------------------------------------------------------ pieces
-      Walk walk = start_walk(p, ms.total, ms.first_b, ms.first_base);
       Piece s;
       int count = 0;
       bool more = true;

@@ -287,7 +287,8 @@ enum { TRITT_MAX_ANCESTORS = 64 };
  * It attends to the context[b] tokens before them and, of the new ones, to token m if bit m of ancestors[b][i] is set and m < i,
  * and to itself (ancestors null: to all m <= i).  Distances are counted along the tokens that it attends to: their positions are 0, 1, 2, ...
  * in order, its own is the last.  A place that the table or the cache does not have sets status bit 512 and is neither read
- * nor written; context[b] < 0 is an unused sequence: nothing of it is read or written, its results are those of no attended token.
+ * nor written; context[b] < 0 is an unused sequence: nothing of its cache is read or written, its results are those of no attended token.
+ * The arrays start as zeros; a row that nobody has written reads as zeros.
  */
 typedef struct {
   void* codes;                 /* [pages, 4, N, page_size, D] */
@@ -332,7 +333,8 @@ int tritt_dps_append(const tritt_cache_t* c, const tritt_rows_t* rows, int dtype
 int tritt_dps_decode(const tritt_cache_t* c, const tritt_rows_t* q, void* o, float* m, int dtype, float alpha, void* workspace,
                      size_t workspace_bytes, int* status_word, int flags, tritt_stream_t stream);
 /* Bytes of scratch for the three calls above (op: TRITT_OP_TDP_DECODE, TRITT_OP_DPS_APPEND, TRITT_OP_DPS_DECODE); the windows of the
-   triple dot product as above (0 for the others). */
+   triple dot product as above (0 for the others).  0: none is needed, or the description is refused.  Calls that may run at the same time need
+   scratch of their own. */
 size_t tritt_decode_workspace(int op, const tritt_cache_t* c, int dtype, int k1_window, int k2_window, int flags);
 /* Which kernel family such a call runs on (TRITT_PATH_SIMT or TRITT_PATH_TCGEN05; for the dot-product-sum the latter stands for warp-level
    matrix instructions). */
