@@ -21,13 +21,15 @@
 //                 the loads of a tile are in flight before its stage is free.  They form tile b's A, and tell its rows' masks and scales
 //   warps 8-11    values in the same way, and tile a's A
 //   warps 12-19   one row a thread: maximum, exponentials, P; at the end of a piece the group's sum
-// Measured: 8 tokens over 2040, 16 heads of 128, float16 codes 374 us (products alone would take 166, exponentials 122); one token over up to
-// 700, 4 sequences of 8 heads of 64, e4m3 31 us.  Of the first a pair of tiles' slab takes 5.1 thousand cycles: 3.2 in a tile's soft-max (a warp a
-// scheduler works alone for most of it), 1.9 from its P to the next scores; the change of pieces costs 17 thousand a piece, the
+// Measured: 8 tokens over 2040, 16 heads of 128, float16 codes 345 us (products alone would take 166, exponentials 122); one token over up to
+// 700, 4 sequences of 8 heads of 64, e4m3 30 us.  Of the first a pair of tiles' slab took 5.1 thousand cycles at 374 us: 3.2 in a tile's soft-max (a
+// warp a scheduler works alone for most of it), 1.9 from its P to the next scores; the change of pieces 17 thousand a piece, the
 // group's sums 8 and the rows' A 13 of them, side by side.  Of the second 10 of the first 19 thousand cycles are the way to the first A.
+// Registers decide: with 32 rows of 256 bytes at a time the loading warps need more than 112 (104: 407 us, 112: 374, and the soft-max warps at 104:
+// 421); with 16 rows 96 do, and the soft-max warps take 120 (344 us; 88 / 136: 397).
 // Keys and values from the same warps: 1.3 us a slab that nothing hid (690 us then).  A formed by the soft-max warps: 15 us a piece.  P in quarters
-// with the next quarter's scores on their way: 448 us instead of 374 (more votes, more registers than there are).  A's codes on their way
-// before the tile is free: 398, its rows loaded side by side: 500 (the loading warps' tiles no longer fit in registers).
+// with the next quarter's scores on their way: 388 us instead of 345 (more votes).  A's codes on their way before the tile is free: 387 to 400, its
+// rows loaded side by side: 500 (registers of the warps that form it).
 #include "tritt_cache.cuh"
 #include "tritt_sm100.cuh"
 #include "tritt_sm100_tdp.cuh"
@@ -40,7 +42,7 @@ using namespace sm100;
 
 constexpr int kThreads = 640;
 constexpr int kRegsLaunch = 96;   // a thread; the soft-max warps take what the others give up
-constexpr int kRegsIssue = 32, kRegsLoad = 112, kRegsSoftmax = 112;
+constexpr int kRegsIssue = 32, kRegsLoad = 96, kRegsSoftmax = 120;
 static_assert(kRegsIssue + 2 * kRegsLoad + 2 * kRegsSoftmax <= 5 * kRegsLaunch, "more registers than the launch has");
 constexpr float kGap = 8.f;      // the accumulator is rescaled when a row's maximum grew by more than 2^8
 constexpr float kLift = 7.f;     // P is formed times 2^7: at most 2^15, normal down to 2^-21 of the reference
@@ -254,30 +256,32 @@ __device__ __forceinline__ uint4 load16_if(const void* p, bool on) {   // zeros 
 
 template <int D, int CODE> struct TileLoader {   // a warp's 32 rows of one part of a slab
   static constexpr int kChunks = CODE == TRITT_CODE_F16 ? D / 8 : D / 16;   // of 16 bytes of codes, a row
-  uint4 v[kChunks];
+  static constexpr int kRows = kChunks > 8 ? 16 : 32;                       // at a time: 32 registers
+  static constexpr int kLoads = kChunks * kRows / 32;
+  uint4 v[kLoads];
   // mine: the lane's own row, null: none (zeros)
-  __device__ __forceinline__ void load(const uint8_t* mine, int lane) {
+  __device__ __forceinline__ void load(const uint8_t* mine, int lane, int from) {
     const uint32_t lo = (uint32_t)(size_t)mine, hi = (uint32_t)((size_t)mine >> 32);
     // rows that follow one another in a page (all 32, where a tile does not start or end in the middle of one)
     const size_t first = (size_t)__shfl_sync(0xffffffffu, hi, 0) << 32 | __shfl_sync(0xffffffffu, lo, 0);
     if (__all_sync(0xffffffffu, mine != nullptr && (size_t)mine == first + lane * (kChunks * 16))) {
 #pragma unroll
-      for (int it = 0; it < kChunks; ++it) v[it] = __ldg(reinterpret_cast<const uint4*>(first) + it * 32 + lane);
+      for (int it = 0; it < kLoads; ++it) v[it] = __ldg(reinterpret_cast<const uint4*>(first) + from * kChunks + it * 32 + lane);
       return;
     }
 #pragma unroll
-    for (int it = 0; it < kChunks; ++it) {
-      const int idx = it * 32 + lane, row = idx / kChunks, ch = idx % kChunks;
+    for (int it = 0; it < kLoads; ++it) {
+      const int idx = it * 32 + lane, row = from + idx / kChunks, ch = idx % kChunks;
       const uint32_t l = __shfl_sync(0xffffffffu, lo, row), h = __shfl_sync(0xffffffffu, hi, row);
       const size_t at = (size_t)h << 32 | l;
       v[it] = load16_if((const uint8_t*)at + ch * 16, at != 0);
     }
   }
   // to rows row0 .. row0 + 31 of a tile, each times the power of two of its lane
-  __device__ __forceinline__ void store(uint8_t* tile, int row0, uint32_t factor, int lane) {
+  __device__ __forceinline__ void store(uint8_t* tile, int row0, uint32_t factor, int lane, int from) {
 #pragma unroll
-    for (int it = 0; it < kChunks; ++it) {
-      const int idx = it * 32 + lane, row = idx / kChunks, ch = idx % kChunks;
+    for (int it = 0; it < kLoads; ++it) {
+      const int idx = it * 32 + lane, row = from + idx / kChunks, ch = idx % kChunks;
       const uint32_t f = __shfl_sync(0xffffffffu, factor, row);
       if constexpr (CODE == TRITT_CODE_F16) {
         *reinterpret_cast<uint4*>(tile + (ch >> 3) * 16384 + swz128(row0 + row, ch & 7)) = times(v[it], f);
@@ -656,7 +660,8 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
           if (keys) ek = __ldg(ca.c.exponents + row + load_rows);
           ev = __ldg(ca.c.exponents + row + v_rows);
         }
-        if (any) tile.load(page >= 0 ? (const uint8_t*)ca.c.codes + (row + load_rows) * kRowBytes : nullptr, lane);
+        const uint8_t* const codes = page >= 0 ? (const uint8_t*)ca.c.codes + (row + load_rows) * kRowBytes : nullptr;
+        if (any) tile.load(codes, lane, 0);
         const int next = i + 1 < n ? page_of(token + 128) : -1;
         int up;   // the row's power of two
         if (keys) {
@@ -684,7 +689,13 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
           v_exp = max(max(max(v_exp, m.v_exp[0]), m.v_exp[1]), max(m.v_exp[2], m.v_exp[3]));
           up = kUp<CODE> + ev - v_exp;
         }
-        if (any) tile.store(ring + st * C::kTile, w * 32, half_power(up), lane);
+        if (any) {
+          tile.store(ring + st * C::kTile, w * 32, half_power(up), lane, 0);
+          if constexpr (TileLoader<D, CODE>::kRows == 16) {
+            tile.load(codes, lane, 16);
+            tile.store(ring + st * C::kTile, w * 32, half_power(up), lane, 16);
+          }
+        }
         fence_async_smem();
         mbar_arrive(&full[st]);
         if (++st == NS) st = 0, ph ^= 1;
