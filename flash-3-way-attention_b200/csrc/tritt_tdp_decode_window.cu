@@ -7,11 +7,13 @@
 // attends to, and sums its rows times V2; the sums of a new token meet in shared memory, in order, and leave as the result: one launch.
 //
 // Bound by instruction issue (1780 a unit of 16 rows under a window of 129 and a band of 65: 56 % of the issue slots) and, for few rows, by the
-// chain load, convert, product, exponential.  Trees of 16 under windows 128/128/32/32, 8 sequences of 16 heads, D=64, int8: 58 us; the kernel
-// with tcgen05 tiles of 128 x 128 cells, which such a window fills to a half: 120.
+// chain load, convert, product, exponential.  Trees of 16 under windows 128/128/32/32, 8 sequences of 16 heads, D=64, int8, fp16
+// queries: 66 us (58 with bfloat16's); the kernel with tcgen05 tiles of 128 x 128 cells, which such a window fills to a half: 120.
 #include "tritt_cache.cuh"
 #include "tritt_sm100.cuh"
 #include "tritt_sm100_tdp.cuh"
+
+#include <type_traits>
 
 namespace tritt {
 namespace {
@@ -41,6 +43,11 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4],
 }
 __device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
   const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+// What the rounded product of `a` and `b` leaves of it (fp16 has it exactly)
+__device__ __forceinline__ uint32_t rest_half2(uint32_t a, uint32_t b, uint32_t product) {
+  const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b), __hneg2(*reinterpret_cast<const __half2*>(&product)));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 __device__ __forceinline__ uint32_t half_power(int e) {   // 2^e as a pair of fp16 (0 below its range; e <= 15)
@@ -224,8 +231,12 @@ __global__ void __launch_bounds__(kWarps * 32) tdp_decode_window_kernel(const __
       if (on && ca.c.ancestors && last >= ctx && last >= c_lo[h])   // (its tokens between the first and the last of the window)
         tree[h] = word & (~0ull << sTree[i * 64 + max(c_lo[h] - ctx, 0)]) & (~0ull >> (63 - sTree[i * 64 + last - ctx]));
     }
-    // A's fragments: elements 32 j + 8 t + 4 s + {0, 1 | 2, 3} of rows g, g + 8 in steps s = 0, 1
-    uint32_t af[D / 16][4];
+    // A's fragments: elements 32 j + 8 t + 4 s + {0, 1 | 2, 3} of rows g, g + 8 in steps s = 0, 1.  For fp16 each as its upper 11 bits and what
+    // they leave: under a narrow window a result has few terms whose errors could cancel.  (With the upper bits alone trees of 16 under a band of 65
+    // were off by 3.1e-4, 58 us; so by 2.3e-4, 66 us, where fp16's own rounding of the result is 2.1e-4; with P in two parts instead 2.9e-4, 68 us.
+    // bfloat16 rounds results by 1.7e-3.)
+    constexpr bool kRest = std::is_same<T16, __half>::value;
+    uint32_t af[D / 16][4], al[kRest ? D / 16 : 1][4];
 #pragma unroll
     for (int j = 0; j < D / 32; ++j) {
       const uint4 q = *reinterpret_cast<const uint4*>(sQ + i * D + j * 32 + t * 8);
@@ -240,6 +251,10 @@ __global__ void __launch_bounds__(kWarps * 32) tdp_decode_window_kernel(const __
           const uint32_t c0 = kDown<CODE> ? mul_half2(w0[2 * s + e], down) : w0[2 * s + e], c1 = kDown<CODE> ? mul_half2(w1[2 * s + e], down) : w1[2 * s + e];
           af[2 * j + s][2 * e] = mul_half2(c0, qw[2 * s + e]);
           af[2 * j + s][2 * e + 1] = mul_half2(c1, qw[2 * s + e]);
+          if constexpr (kRest) {
+            al[2 * j + s][2 * e] = rest_half2(c0, qw[2 * s + e], af[2 * j + s][2 * e]);
+            al[2 * j + s][2 * e + 1] = rest_half2(c1, qw[2 * s + e], af[2 * j + s][2 * e + 1]);
+          }
         }
     }
     // columns that any of the warp's rows attends to
@@ -277,6 +292,10 @@ __global__ void __launch_bounds__(kWarps * 32) tdp_decode_window_kernel(const __
           const uint4 k = *reinterpret_cast<const uint4*>(key_at[j] + (c0 + n * 8) * (2 * D));
           mma_16816(s[n], af[2 * j], k.x, k.y);
           mma_16816(s[n], af[2 * j + 1], k.z, k.w);
+          if constexpr (kRest) {
+            mma_16816(s[n], al[2 * j], k.x, k.y);
+            mma_16816(s[n], al[2 * j + 1], k.z, k.w);
+          }
         }
       }
       if (__any_sync(0xffffffffu, (mask[0] & mask[1]) != 0xffffffffu)) {

@@ -198,7 +198,7 @@ def tdp_decode(q: Tensor, cache: TrittentionCache, table: Tensor, context: Tenso
     type, or ``(o, lse)`` with the fp32 log-sum-exp ``[B, N, n]``.
 
     The mask is that of ``flash_trittention`` with ``causal``, over positions; a window of ``None`` has no limit.  A row past ``counts[b]`` or of a
-    free slot is 0, its log-sum-exp ``-inf``.  16-bit queries with head dimension 64 or 128 run on the tensor cores: operands of 11
+    free slot is 0, its log-sum-exp ``-inf``.  16-bit queries with head dimension 64 or 128 run on the tensor cores: operands of at least 11
     significant bits, fp32 sums and soft-max.  fp32 queries, other head dimensions and ``input_precision="ieee"`` run in fp32 on the CUDA
     cores.  No gradient flows through the cache.
     """
