@@ -49,6 +49,9 @@ constexpr float kLift = 7.f;     // P is formed times 2^7: at most 2^15, normal 
 constexpr int kMetas = 6;        // slabs whose descriptions are kept: two more than the ring's depth (one is overwritten when S of the slab
                                  // kMetas back is done, and the rows have then read that of the slab before it)
 constexpr int kUnlimited = 1 << 30;
+// The most of one sequence's head: groups of rows, whose numbers are 32-bit (65536 new tokens behind a million come to 2^31), and steps of the line, so that
+// those of all 65535 heads times the CTAs stay below 2^63 (2^39 steps of 2 us take two hours on all SMs).
+constexpr long long kMostGroups = 1ll << 30, kMostSteps = 1ll << 39;
 
 template <int D> struct Cfg {
   static constexpr int kTile = 128 * D * 2;
@@ -138,8 +141,14 @@ __device__ __forceinline__ Line line_of(const TdpDecodeArgs& a, int b) {
     return l;
   }
   l.groups = (least(l.ctx + l.cnt - 1, a.k2w) + 32) / 32;   // (rows: the window and the token itself)
-  l.pairs = (l.cnt * l.groups + 7) / 8;
   l.slabs = (least(l.ctx, a.k1w) + l.cnt + 127) / 128;
+  const long long all = (long long)l.cnt * l.groups, pairs = (all + 7) / 8;
+  if (all > kMostGroups || pairs * l.slabs > kMostSteps) {   // too much: reported, and left out like a sequence without new tokens
+    if (a.cache.status) atomicOr(a.cache.status, kStatusTdpDecode);
+    l.cnt = l.groups = l.pairs = l.slabs = 0;
+    return l;
+  }
+  l.pairs = (int)pairs;
   return l;
 }
 __device__ __forceinline__ Columns columns_of(const TdpDecodeArgs& a, const Line& l, int pair) {

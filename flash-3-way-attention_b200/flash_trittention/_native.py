@@ -231,7 +231,7 @@ STATUS_BITS = {1: "self-test kernel", 2: "triple-dot-product forward", 4: "tripl
                16: "soft-max attention forward (dot-product-sum)", 32: "soft-max attention backward (dot-product-sum)",
                64: "an input element beyond the fp16 operand range (65504) in an fp32 / wide-operand call",
                128: "wait-expiry self-test", 256: "a rotation whose position its tables do not have",
-               512: "a token without a place in its cache", 1024: "triple-dot-product attention over a cache"}
+               512: "a token without a place in its cache", 1024: "triple-dot-product attention over a cache (or more new tokens times cached ones than it can count)"}
 
 
 def _device_index(device) -> int:

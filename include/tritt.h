@@ -317,6 +317,8 @@ int tritt_cache_read(const tritt_cache_t* c, void* const* parts, float* lse, int
  * over pairs of attended tokens within the windows (distances of positions, as for tritt_tdp_fwd: q - j <= k1_window,
  * q - k <= k2_window, k - j <= kk_left, j - k <= kk_right).  o: [B, N, n, D] contiguous; lse [B, N, n] or null.
  * A token without an attended pair (i >= counts[b], context[b] < 0) gets o = 0, lse = -infinity.
+ * On the tensor cores a sequence has at most 2^30 (new token, 32 rows k of its window) groups and 2^39 products of 256 x 128 cells a head; one that has
+ * more sets status bit 1024 and gets no results (o = 0, lse = -infinity).
  */
 int tritt_tdp_decode(const tritt_cache_t* c, const tritt_rows_t* q, void* o, float* lse, int dtype, float alpha, int k1_window,
                      int k2_window, int kk_left, int kk_right, void* workspace, size_t workspace_bytes, int* status_word, int flags,
