@@ -250,7 +250,15 @@ int check_scratch(size_t need, const void* ws, size_t have) {
   return 0;
 }
 
-int check_out(const void* p) {
+int check_lse(const float* lse) {   // (null: not wanted)
+  if ((uintptr_t)lse & 3) {
+    set_error("the log-sum-exps' pointer is not aligned");
+    return -5;
+  }
+  return 0;
+}
+
+int check_out(const void* p, const float* lse) {
   if (!p) {
     set_error("null tensor pointer");
     return -4;
@@ -259,7 +267,7 @@ int check_out(const void* p) {
     set_error("tensor pointer is not 16-byte aligned");
     return -5;
   }
-  return 0;
+  return check_lse(lse);
 }
 
 bool fast(int op, int D, int dtype, int flags) {
@@ -303,7 +311,8 @@ int check_cache(const tritt_cache_t* c) {
     set_error("null cache pointer");
     return -4;
   }
-  if ((((uintptr_t)c->codes | (uintptr_t)c->exponents | (uintptr_t)c->lse) & 15) || (((uintptr_t)c->table | (uintptr_t)c->context) & 3)) {
+  if ((((uintptr_t)c->codes | (uintptr_t)c->exponents | (uintptr_t)c->lse) & 15) ||
+      (((uintptr_t)c->table | (uintptr_t)c->context | (uintptr_t)c->counts) & 3) || ((uintptr_t)c->ancestors & 7)) {
     set_error("cache pointer is not aligned");
     return -5;
   }
@@ -364,6 +373,7 @@ int tritt_cache_read(const tritt_cache_t* c, void* const* parts, float* lse, int
     set_error("null tensor pointer");
     return -4;
   }
+  if (int rc = check_lse(lse)) return rc;
   ReadArgs r{cache_args(*c, status_word), {parts[0], parts[1], parts[2], parts[3]}, c->lse ? lse : nullptr};
   for (int i = 0; i < 4; ++i) {
     const tritt_rows_t row{parts[i], 0, 0, 0};
@@ -387,7 +397,7 @@ int tritt_tdp_decode(const tritt_cache_t* c, const tritt_rows_t* q, void* o, flo
                      tritt_stream_t stream) {
   if (int rc = check_cache(c)) return rc;
   if (int rc = check_rows(q, 1, dtype)) return rc;
-  if (int rc = check_out(o)) return rc;
+  if (int rc = check_out(o, lse)) return rc;
   if (k1_window < 0 || k2_window < 0 || kk_left < 0 || kk_right < 0) {
     set_error("window arguments must be >= 0 (got %d, %d, %d, %d)", k1_window, k2_window, kk_left, kk_right);
     return -10;
@@ -432,7 +442,7 @@ int tritt_dps_decode(const tritt_cache_t* c, const tritt_rows_t* q, void* o, flo
                      size_t workspace_bytes, int* status_word, int flags, tritt_stream_t stream) {
   if (int rc = check_cache(c)) return rc;
   if (int rc = check_rows(q, 1, dtype)) return rc;
-  if (int rc = check_out(o)) return rc;
+  if (int rc = check_out(o, m)) return rc;
   if (!c->lse) {
     set_error("the cache has no log-sum-exps: it is not one of the dot-product-sum form");
     return -16;

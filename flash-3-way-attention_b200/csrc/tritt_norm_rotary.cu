@@ -463,6 +463,10 @@ int check(const tritt_norm_rotary_t* a, bool backward) {
     set_error("a rotation needs tables of cosines and sines on 16-byte boundaries");
     return -13;
   }
+  if (a->rot && ((uintptr_t)a->positions & (a->positions64 ? 7 : 3))) {
+    set_error("the positions' pointer is not aligned");
+    return -5;
+  }
   if (a->rot && !a->positions && a->T > a->table) {
     set_error("the tables have %d positions, the sequence %d", a->table, a->T);
     return -13;

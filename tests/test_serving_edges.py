@@ -39,3 +39,46 @@ def test_a_sequence_of_more_groups_than_can_be_numbered_is_reported():
     empty = torch.ones(3, 1, n, dtype=torch.bool, device=DEV)
     empty[1, :, :3] = False
     assert not bool(out[empty].any()) and bool((lse[empty] == -math.inf).all())
+
+
+# ---------------------------------------------------------------- pointers and sizes that the C entries refuse
+
+P = 1 << 20
+
+
+def _cache_calls(**kw):
+    lib, C = _native.lib(), _native.C
+    out, m = kw.pop("out", P), kw.pop("m", P)
+    c = C.byref(_native.Cache(**{**dict(codes=P, exponents=P, lse=P, pages=2, page_size=16, N=2, D=64, code=1, table=P, table_stride=2, table_pages=2,
+                                        context=P, B=1, n=1), **kw}))
+    rows, parts = (_native.Rows * 4)(*(_native.Rows(P, 64, 64, 64) for _ in range(4))), (C.c_void_p * 4)(P, P, P, P)
+    return dict(write=lambda: lib.tritt_cache_write(c, rows, 1, None, None), read=lambda: lib.tritt_cache_read(c, parts, m, 1, None, None),
+                tdp=lambda: lib.tritt_tdp_decode(c, rows, out, m, 1, 0.1, 1, 1, 1, 1, P, 1 << 40, None, 0, None),
+                append=lambda: lib.tritt_dps_append(c, rows, 1, 0.1, 1, P, 1 << 40, None, 0, None),
+                dps=lambda: lib.tritt_dps_decode(c, rows, out, m, 1, 0.1, P, 1 << 40, None, 0, None))
+
+
+# (every call below is refused before anything is launched: there is no GPU in it)
+@pytest.mark.parametrize("field,off", [("counts", 2), ("counts", 1), ("ancestors", 4), ("ancestors", 1), ("table", 2), ("context", 2)])
+def test_the_caches_pointers_that_are_not_aligned_are_refused(field, off):
+    for name, call in _cache_calls(**{field: P + off}).items():
+        assert call() == -5, name
+
+
+@pytest.mark.parametrize("off", [1, 2])
+def test_log_sum_exps_that_are_not_aligned_are_refused(off):
+    calls = _cache_calls(m=P + off)
+    assert [calls[name]() for name in ("read", "tdp", "dps")] == [-5] * 3
+
+
+def _norm_args(**kw):
+    rows = lambda: (_native.Rows * 3)(*(_native.Rows(P, 64, 64, 64) for _ in range(3)))  # noqa: E731
+    return _native.NormRotary(**{**dict(x=rows(), y=rows(), dx=rows(), B=1, N=1, T=1, D=64, dtype=1), **kw})
+
+
+@pytest.mark.parametrize("wide,off", [(0, 2), (0, 1), (1, 4), (1, 2)])
+def test_positions_that_are_not_aligned_are_refused(wide, off):
+    lib, C = _native.lib(), _native.C
+    a = _norm_args(rot=16, cos=P, sin=P, table=4, positions=P + off, positions64=wide)
+    assert lib.tritt_qk_norm_rotary_fwd(C.byref(a), None, None) == -5
+    assert lib.tritt_qk_norm_rotary_bwd(C.byref(a), P, 1 << 40, None, None) == -5
