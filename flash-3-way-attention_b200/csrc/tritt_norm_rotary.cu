@@ -408,12 +408,14 @@ struct Grid {
   int blocks, groups;
 };
 Grid bwd_grid(const tritt_norm_rotary_t& a) {
-  const int chunks = (a.N + kHeads - 1) / kHeads, slots = kNormThreads / (a.D / 8);
+  const int chunks = (int)(((long long)a.N + kHeads - 1) / kHeads), slots = kNormThreads / (a.D / 8);
   const int here = chunks < slots ? chunks : slots, groups = (chunks + here - 1) / here, at_once = slots / here;
   const long long per_sm = a.dtype == TRITT_F32 ? kPerSm<float, true> : a.weight_heads ? kPerSm<__half, false> : kPerSm<__half, true>;
   const long long most = ((long long)a.B * a.T + at_once - 1) / at_once, fill = per_sm * kSms / (3 * groups);
   return Grid{(int)(most < fill ? most : fill < 1 ? 1 : fill), groups};
 }
+
+bool wants_weights(const tritt_norm_rotary_t& a) { return a.dw[0] || a.dw[1] || a.dw[2]; }
 
 int check(const tritt_norm_rotary_t* a, bool backward) {
   if (!a || a->B <= 0 || a->N <= 0 || a->T <= 0) {
@@ -428,8 +430,14 @@ int check(const tritt_norm_rotary_t* a, bool backward) {
     set_error("unknown dtype code %d", a->dtype);
     return -3;
   }
-  if ((long long)a->B * a->T > (1LL << 30) || (long long)a->B * a->T * ((a->N + kHeads - 1) / kHeads) > (1LL << 31)) {
-    set_error("too many rows for one call (B*T = %lld); split the batch", (long long)a->B * a->T);
+  const long long tokens = (long long)a->B * a->T, chunks = ((long long)a->N + kHeads - 1) / kHeads;
+  if (tokens > (1LL << 30) || tokens * chunks > (1LL << 31)) {
+    set_error("too many rows for one call (B*T = %lld, N = %d); split the batch", tokens, a->N);
+    return -11;
+  }
+  // (the backward's grids have three times the groups of heads, and the heads, in a dimension that ends at 65535)
+  if (backward && (chunks * 3 > 65535 || (a->weight_heads && wants_weights(*a) && a->N > 65535))) {
+    set_error("too many heads for a backward call, N = %d", a->N);
     return -11;
   }
   if (a->weight_dtype != TRITT_F32 && a->weight_dtype != a->dtype) {
@@ -513,8 +521,6 @@ int by_type(const NormParams& p, bool backward, cudaStream_t stream) {
   return p.a.dtype == TRITT_F16 ? by_size<__half>(p, backward, stream) : by_size<__nv_bfloat16>(p, backward, stream);
 }
 
-bool wants_weights(const tritt_norm_rotary_t& a) { return a.dw[0] || a.dw[1] || a.dw[2]; }
-
 }  // namespace
 }  // namespace tritt
 
@@ -540,10 +546,6 @@ int tritt_qk_norm_rotary_bwd(const tritt_norm_rotary_t* a, void* workspace, size
   if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))) {
     set_error("workspace too small or misaligned: need %zu bytes, got %zu", need, workspace ? workspace_bytes : (size_t)0);
     return -6;
-  }
-  if (((long long)a->N + kHeads - 1) / kHeads * 3 > 65535) {
-    set_error("too many heads");
-    return -11;
   }
   NormParams p{*a, (a->N + kHeads - 1) / kHeads, 0, 0, need ? (float*)workspace : nullptr, status_word};
   return by_type(p, true, (cudaStream_t)stream);

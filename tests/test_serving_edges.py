@@ -82,3 +82,23 @@ def test_positions_that_are_not_aligned_are_refused(wide, off):
     a = _norm_args(rot=16, cos=P, sin=P, table=4, positions=P + off, positions64=wide)
     assert lib.tritt_qk_norm_rotary_fwd(C.byref(a), None, None) == -5
     assert lib.tritt_qk_norm_rotary_bwd(C.byref(a), P, 1 << 40, None, None) == -5
+
+
+@pytest.mark.parametrize("kw,backward", [(dict(N=2 ** 31 - 1, T=64), False), (dict(N=2 ** 31 - 1, T=64), True), (dict(N=2 ** 31 - 3, B=64), False),
+                                         (dict(N=90000), True), (dict(N=65536, weight_heads=1, weight_dtype=1), True)])
+def test_more_heads_than_a_grid_has_are_refused(kw, backward):
+    lib, C = _native.lib(), _native.C
+    a = _norm_args(**kw)
+    if backward:
+        a.w[0] = a.dw[0] = P
+        assert lib.tritt_qk_norm_rotary_bwd(C.byref(a), P, 1 << 60, None, None) == -11
+    else:
+        assert lib.tritt_qk_norm_rotary_fwd(C.byref(a), None, None) == -11
+
+
+def test_the_workspace_of_very_many_heads_is_counted():
+    """(Their groups were counted in 32 bits, which ended the process with a division by zero.)"""
+    lib, C = _native.lib(), _native.C
+    a = _norm_args(N=2 ** 31 - 1)
+    a.w[0] = a.dw[0] = P
+    assert lib.tritt_qk_norm_rotary_workspace(C.byref(a)) >= 3 * (2 ** 31 - 1) * 64 * 4
