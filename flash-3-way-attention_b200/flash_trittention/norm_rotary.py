@@ -9,6 +9,7 @@ import torch
 from torch import Tensor
 
 from . import _native
+from ._derivatives import Undifferentiable
 
 __all__ = ["qk_norm_rotary", "rotary_tables"]
 
@@ -135,14 +136,19 @@ class QkNormRotary(torch.autograd.Function):
         q, k1, k2, w_q, w_k1, w_k2, cos, sin, positions = ctx.saved_tensors
         if all(dy is None for dy in dys):
             return (None,) * 11
-        grads = norm_rotary_backward((q, k1, k2), (w_q, w_k1, w_k2), cos, sin, positions, *ctx.rest, dys, ctx.needs_input_grad[3:6])
+
+        def compute():
+            return norm_rotary_backward((q, k1, k2), (w_q, w_k1, w_k2), cos, sin, positions, *ctx.rest, dys, ctx.needs_input_grad[3:6])
+
+        # (with create_graph)
+        grads = Undifferentiable.apply("the gradient of qk_norm_rotary", compute, q, k1, k2, w_q, w_k1, w_k2, *dys) if torch.is_grad_enabled() else compute()
         return (*grads, None, None, None, None, None)
 
 
 def qk_norm_rotary(q: Tensor, k1: Tensor, k2: Tensor, q_weight: Optional[Tensor] = None, k1_weight: Optional[Tensor] = None,
                    k2_weight: Optional[Tensor] = None, cos: Optional[Tensor] = None, sin: Optional[Tensor] = None,
                    positions: Optional[Tensor] = None, eps: float = 1e-6, interleaved: bool = False) -> Tuple[Tensor, Tensor, Tensor]:
-    """``q, k1, k2`` normed for each head and rotated by their positions, in one pass; differentiable.
+    """``q, k1, k2`` normed for each head and rotated by their positions, in one pass; differentiable once (a second derivative raises).
 
     Each row ``x`` of a tensor ``[B, N, T, D]`` becomes ``u = x / sqrt(mean(x^2) + eps) * weight``, and of its first ``2 * cos.shape[1]``
     elements each pair ``(a, b)`` becomes ``(a c - b s, b c + a s)`` with the values of its position in ``cos`` and ``sin`` (see

@@ -1,4 +1,5 @@
 """Calls at the edges of the cache's operators and of the norms: sizes that 32 bits do not hold, derivatives that there are not, bad pointers."""
+import importlib
 import math
 
 import pytest
@@ -6,6 +7,7 @@ import torch
 
 import flash_trittention as ft
 from flash_trittention import _native
+from oracle import serving_oracle as orc
 from test_cache import DEV, Batch
 
 
@@ -39,6 +41,63 @@ def test_a_sequence_of_more_groups_than_can_be_numbered_is_reported():
     empty = torch.ones(3, 1, n, dtype=torch.bool, device=DEV)
     empty[1, :, :3] = False
     assert not bool(out[empty].any()) and bool((lse[empty] == -math.inf).all())
+
+
+# ---------------------------------------------------------------- derivatives that there are not
+
+def _norm_on_cpu(monkeypatch):
+    """The norm's two calls by torch operations in the place of the kernels."""
+    module = importlib.import_module("flash_trittention.norm_rotary")
+
+    def forward(xs, ws, cos, sin, positions, eps, interleaved):
+        return tuple(orc.norm_rotary(x.detach(), w.detach(), None, None, None, eps) for x, w in zip(xs, ws))
+
+    def backward(xs, ws, cos, sin, positions, eps, interleaved, dys, weights_too):
+        grads = []
+        for x, w, dy in zip(xs, ws, dys):
+            with torch.enable_grad():
+                x, w = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+                y = orc.norm_rotary(x, w, None, None, None, eps)
+            grads.append([torch.zeros_like(x), torch.zeros_like(w)] if dy is None else torch.autograd.grad(y, [x, w], dy.detach()))
+        return (*(g[0] for g in grads), *(g[1] if want else None for g, want in zip(grads, weights_too)))
+
+    monkeypatch.setattr(module, "norm_rotary_forward", forward)
+    monkeypatch.setattr(module, "norm_rotary_backward", backward)
+
+
+def _leaves(shape, dtype=torch.float64, device="cpu"):
+    g = torch.Generator().manual_seed(0)
+    return [torch.randn(shape, generator=g).to(device, dtype).requires_grad_(True) for _ in range(3)], [
+        (torch.rand(shape[-1], generator=g) + 0.5).to(device, dtype).requires_grad_(True) for _ in range(3)]
+
+
+def _second_derivatives_raise(f, leaves, like, what):
+    """``f``'s gradients with create_graph: as without, and nothing that depends on them can be differentiated, whatever else the loss has."""
+    plain = torch.autograd.grad(f(), leaves, torch.ones_like(like))
+    for dy in (torch.ones_like(like), torch.ones_like(like).requires_grad_(True)):   # (of a linear loss, and of any other)
+        grads = torch.autograd.grad(f(), leaves, dy, create_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(plain, grads))
+        for g in grads:
+            with pytest.raises(RuntimeError, match=what):
+                (g.float().square().sum() + sum(t.float().square().sum() for t in leaves)).backward(retain_graph=True)
+
+
+def test_a_second_derivative_of_the_norms_raises(monkeypatch):
+    _norm_on_cpu(monkeypatch)
+    xs, ws = _leaves((1, 2, 5, 16))
+    like = torch.empty(1, 2, 5, 16, dtype=torch.float64)
+    _second_derivatives_raise(lambda: sum(ft.qk_norm_rotary(*xs, *ws)), xs + ws, like, "qk_norm_rotary")
+    # frozen weights, and a result that the loss does not have
+    y = ft.qk_norm_rotary(*xs, *(w.detach() for w in ws))
+    grads = torch.autograd.grad(y[1].sum(), xs, create_graph=True, allow_unused=True)
+    with pytest.raises(RuntimeError, match="qk_norm_rotary"):
+        (grads[1].sum() + xs[1].square().sum()).backward()
+
+
+@pytest.mark.gpu
+def test_a_second_derivative_of_the_norms_kernels_raises():
+    xs, ws = _leaves((2, 3, 20, 64), torch.float32, DEV)
+    _second_derivatives_raise(lambda: sum(ft.qk_norm_rotary(*xs, *ws)), xs + ws, xs[0].detach(), "qk_norm_rotary")
 
 
 # ---------------------------------------------------------------- pointers and sizes that the C entries refuse
