@@ -12,6 +12,7 @@ import torch
 import torch.nn as nn
 
 from .. import _native
+from .._derivatives import Undifferentiable
 
 
 def _validate(q, k1, k2, v1, v2):
@@ -61,6 +62,13 @@ class TrittentionTritonFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_output, m_grad=None):
+        if torch.is_grad_enabled():   # (create_graph: a second derivative raises)
+            return Undifferentiable.apply("the gradient of TrittentionTriton", lambda: TrittentionTritonFunction._gradients(ctx, grad_output),
+                                          *ctx.saved_tensors[:5], grad_output)
+        return TrittentionTritonFunction._gradients(ctx, grad_output)
+
+    @staticmethod
+    def _gradients(ctx, grad_output):
         q, k1, k2, v1, v2, o, m = ctx.saved_tensors
         assert grad_output.shape == o.shape, f"Shape mismatch: O={o.shape}, dO={grad_output.shape}"
         assert o.device == grad_output.device, "O and dO must be on the same device"

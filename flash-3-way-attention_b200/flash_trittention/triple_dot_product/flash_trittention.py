@@ -13,6 +13,7 @@ import warnings
 import torch
 
 from .. import _native
+from .._derivatives import Undifferentiable
 from .kernels.utils import process_masking_variables
 
 
@@ -71,6 +72,13 @@ class FlashTrittention(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dO):
+        if torch.is_grad_enabled():   # (create_graph: a second derivative raises)
+            return Undifferentiable.apply("the gradient of flash_trittention", lambda: FlashTrittention._gradients(ctx, dO),
+                                          *ctx.saved_tensors[:5], dO)
+        return FlashTrittention._gradients(ctx, dO)
+
+    @staticmethod
+    def _gradients(ctx, dO):
         Q, K1, K2, V1, V2, O, lse = ctx.saved_tensors
         k1_window, k2_window, kk_left, kk_right = ctx.windows
         grads = _native.host_backward(_native.OP_TDP_BWD, Q, K1, K2, V1, V2, O, dO, lse, ctx.softmax_scale, ctx.causal,
@@ -102,7 +110,7 @@ def flash_trittention(
     convert_to_float32=False,
     input_precision=None,
 ):
-    """Triple-dot-product trittention, forward and (through autograd) backward.
+    """Triple-dot-product trittention, forward and (through autograd, once) backward.
 
     ``S[q,j,k] = softmax_scale * sum_h q[q,h] k1[j,h] k2[k,h]``; soft-max over the attended
     ``(j, k)``; ``out[q,h] = sum_jk P[q,j,k] SiLU(v1[j,h]) v2[k,h]``.  With ``causal`` a triple

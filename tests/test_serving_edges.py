@@ -100,6 +100,35 @@ def test_a_second_derivative_of_the_norms_kernels_raises():
     _second_derivatives_raise(lambda: sum(ft.qk_norm_rotary(*xs, *ws)), xs + ws, xs[0].detach(), "qk_norm_rotary")
 
 
+def _attentions():
+    return (("flash_trittention", lambda xs: ft.flash_trittention(*xs, 0.125, None, None, None, None)),
+            ("TrittentionTriton", lambda xs: ft.TrittentionTriton(softmax_scale=0.125)(*xs)[0]))
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_a_second_derivative_of_the_attentions_raises(which, monkeypatch):
+    """(With other calls in the place of the kernels': what is looked at is what autograd makes of their results.)"""
+    name, attend = _attentions()[which]
+    like = torch.empty(1, 2, 5, 16, dtype=torch.float64)
+    monkeypatch.setattr(_native, "host_forward", lambda op, q, k1, k2, v1, v2, *a: (q * k1 + k2 * v1 * v2, q.sum(-1), None)[: 2 + which])
+    monkeypatch.setattr(_native, "host_backward", lambda op, q, k1, k2, v1, v2, o, do, *a: (do * k1, do * q, do * v1 * v2, do * k2 * v2, do * k2 * v1))
+    xs = [torch.randn(like.shape, dtype=torch.float64).requires_grad_(True) for _ in range(5)]
+    _second_derivatives_raise(lambda: attend(xs), xs, like, name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", [0, 1])
+def test_a_second_derivative_of_the_attentions_kernels_raises(which):
+    name, attend = _attentions()[which]
+    xs = [(0.5 * torch.randn(1, 2, 64, 64, generator=torch.Generator().manual_seed(i))).to(DEV, torch.float32).requires_grad_(True) for i in range(5)]
+    got = torch.autograd.grad(attend(xs).sum(), xs, create_graph=True)
+    for g in got:
+        with pytest.raises(RuntimeError, match=name):
+            (g.sum() + xs[0].square().sum()).backward(retain_graph=True)
+    for a, b in zip(got, torch.autograd.grad(attend(xs).sum(), xs)):   # (the kernels' sums may be in another order)
+        assert float((a - b).abs().max()) <= 1e-3 * float(b.abs().max())
+
+
 # ---------------------------------------------------------------- pointers and sizes that the C entries refuse
 
 P = 1 << 20
