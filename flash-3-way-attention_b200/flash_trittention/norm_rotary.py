@@ -9,7 +9,7 @@ import torch
 from torch import Tensor
 
 from . import _native
-from ._derivatives import Undifferentiable
+from ._derivatives import Undifferentiable, forward_mode
 
 __all__ = ["qk_norm_rotary", "rotary_tables"]
 
@@ -148,7 +148,8 @@ class QkNormRotary(torch.autograd.Function):
 def qk_norm_rotary(q: Tensor, k1: Tensor, k2: Tensor, q_weight: Optional[Tensor] = None, k1_weight: Optional[Tensor] = None,
                    k2_weight: Optional[Tensor] = None, cos: Optional[Tensor] = None, sin: Optional[Tensor] = None,
                    positions: Optional[Tensor] = None, eps: float = 1e-6, interleaved: bool = False) -> Tuple[Tensor, Tensor, Tensor]:
-    """``q, k1, k2`` normed for each head and rotated by their positions, in one pass; differentiable once (a second derivative raises).
+    """``q, k1, k2`` normed for each head and rotated by their positions, in one pass; differentiable once, backwards (a second derivative and
+    forward mode raise).
 
     Each row ``x`` of a tensor ``[B, N, T, D]`` becomes ``u = x / sqrt(mean(x^2) + eps) * weight``, and of its first ``2 * cos.shape[1]``
     elements each pair ``(a, b)`` becomes ``(a c - b s, b c + a s)`` with the values of its position in ``cos`` and ``sin`` (see
@@ -171,6 +172,6 @@ def qk_norm_rotary(q: Tensor, k1: Tensor, k2: Tensor, q_weight: Optional[Tensor]
         from .ops import norm_rotary
 
         return norm_rotary(q, k1, k2, q_weight, k1_weight, k2_weight, cos, sin, positions, eps, bool(interleaved))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k1, k2, q_weight, k1_weight, k2_weight)):
+    if (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k1, k2, q_weight, k1_weight, k2_weight))) or forward_mode():
         return QkNormRotary.apply(q, k1, k2, q_weight, k1_weight, k2_weight, cos, sin, positions, eps, bool(interleaved))
     return norm_rotary_forward((q, k1, k2), (q_weight, k1_weight, k2_weight), cos, sin, positions, eps, bool(interleaved))

@@ -4,6 +4,7 @@ import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import flash_trittention as ft
 from flash_trittention import _native
@@ -98,6 +99,21 @@ def test_a_second_derivative_of_the_norms_raises(monkeypatch):
 def test_a_second_derivative_of_the_norms_kernels_raises():
     xs, ws = _leaves((2, 3, 20, 64), torch.float32, DEV)
     _second_derivatives_raise(lambda: sum(ft.qk_norm_rotary(*xs, *ws)), xs + ws, xs[0].detach(), "qk_norm_rotary")
+
+
+def test_a_tangent_through_the_norms_raises(monkeypatch):
+    _norm_on_cpu(monkeypatch)
+    xs, ws = _leaves((1, 2, 5, 16))
+    xs, ws = [x.detach() for x in xs], [w.detach() for w in ws]
+    want = ft.qk_norm_rotary(*xs, *ws)
+    with forward_ad.dual_level():
+        assert all(torch.equal(a, b) for a, b in zip(want, ft.qk_norm_rotary(*xs, *ws)))   # (no tensor with a tangent)
+        for i in range(6):
+            args = [forward_ad.make_dual(t, torch.ones_like(t)) if k == i else t for k, t in enumerate(xs + ws)]
+            with pytest.raises(RuntimeError, match="jvp"):
+                ft.qk_norm_rotary(*args)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda x: ft.qk_norm_rotary(x, *xs[1:], *ws)[0], (xs[0],), (xs[0],))
 
 
 def _attentions():
