@@ -30,6 +30,7 @@ import torch
 from torch import Tensor
 
 from . import _native
+from ._derivatives import Undifferentiable, forward_mode
 from .norm_rotary import HEAD_DIMS
 
 __all__ = ["TrittentionCache", "new_cache", "cache_write", "cache_read", "tree_ancestors", "tdp_decode", "dps_append", "dps_decode"]
@@ -149,6 +150,10 @@ def _flags(input_precision):
     return _native.FLAG_FORCE_SIMT if input_precision == "ieee" else 0
 
 
+def _wants_derivative(q):
+    return (torch.is_grad_enabled() and q.requires_grad) or forward_mode()
+
+
 def _need_lse(cache):
     if cache.lse is None:
         raise ValueError("the cache has no log-sum-exps: it is not one of the dot-product-sum form (new_cache(..., dps=True))")
@@ -200,7 +205,7 @@ def tdp_decode(q: Tensor, cache: TrittentionCache, table: Tensor, context: Tenso
     The mask is that of ``flash_trittention`` with ``causal``, over positions; a window of ``None`` has no limit.  A row past ``counts[b]`` or of a
     free slot is 0, its log-sum-exp ``-inf``.  16-bit queries with head dimension 64 or 128 run on the tensor cores: operands of at least 11
     significant bits, fp32 sums and soft-max.  fp32 queries, other head dimensions and ``input_precision="ieee"`` run in fp32 on the CUDA
-    cores.  No gradient flows through the cache.
+    cores.  No gradient flows through the cache, and there is none for ``q``: a backward pass through the result raises.
     """
     flags, softmax_scale = _flags(input_precision), float(softmax_scale)
     if torch.compiler.is_compiling():
@@ -210,6 +215,9 @@ def tdp_decode(q: Tensor, cache: TrittentionCache, table: Tensor, context: Tenso
         o, lse = ops.tdp_decode(q, cache.codes, cache.exponents, table, context, softmax_scale, k1_window, k2_window, kk_left, kk_right, counts,
                                 ancestors, input_precision)
         return (o, lse) if return_lse else o
+    if _wants_derivative(q):
+        return Undifferentiable.apply("tdp_decode", lambda: tdp_decode(q, cache, table, context, softmax_scale, k1_window, k2_window, kk_left, kk_right,
+                                                                       counts, ancestors, return_lse, input_precision), q)
     out = _native.host_decode(_native.OP_TDP_DECODE, *_cache(cache), table, context, counts, ancestors, flags, softmax_scale, q, k1_window,
                               k2_window, kk_left, kk_right, bool(return_lse))
     if out is not None:
@@ -255,13 +263,16 @@ def dps_decode(q: Tensor, cache: TrittentionCache, table: Tensor, context: Tenso
                counts: Optional[Tensor] = None, ancestors: Optional[Tensor] = None,
                input_precision: Optional[str] = None) -> Tuple[Tensor, Tensor]:
     """Dot-product-sum attention of new tokens that ``dps_append`` has written: ``(o [B, N, n, D], m [B, N, n] fp32 log-sum-exp)``, as the module
-    ``TrittentionTriton`` returns them.  Rows past ``counts[b]`` or of a free slot are 0 and ``-inf``.  Kernels as for ``tdp_decode``."""
+    ``TrittentionTriton`` returns them.  Rows past ``counts[b]`` or of a free slot are 0 and ``-inf``.  Kernels and derivatives (none) as for
+    ``tdp_decode``."""
     flags, softmax_scale = _flags(input_precision), float(softmax_scale)
     if torch.compiler.is_compiling():
         from . import ops
 
         _need_lse(_cache(cache))
         return ops.dps_decode(q, *cache, table, context, softmax_scale, counts, ancestors, input_precision)
+    if _wants_derivative(q):
+        return Undifferentiable.apply("dps_decode", lambda: dps_decode(q, cache, table, context, softmax_scale, counts, ancestors, input_precision), q)
     out = _native.host_decode(_native.OP_DPS_DECODE, *_cache(cache), table, context, counts, ancestors, flags, softmax_scale, q)
     if out is not None:
         return _native.host_result(out, "tritt_dps_decode")

@@ -116,6 +116,44 @@ def test_a_tangent_through_the_norms_raises(monkeypatch):
         torch.func.jvp(lambda x: ft.qk_norm_rotary(x, *xs[1:], *ws)[0], (xs[0],), (xs[0],))
 
 
+def _decodes(cache, table, ctx):
+    return {"tdp_decode": lambda q: ft.tdp_decode(q, cache, table, ctx, 0.1), "tdp_decode with lse": lambda q: ft.tdp_decode(q, cache, table, ctx, 0.1,
+            return_lse=True)[0], "dps_decode": lambda q: ft.dps_decode(q, cache, table, ctx, 0.1)[0]}
+
+
+def _decode_derivatives_raise(calls, q):
+    for name, call in calls.items():
+        want = call(q)
+        assert not want.requires_grad
+        leaf = q.clone().requires_grad_(True)
+        with torch.no_grad():
+            assert not call(leaf).requires_grad
+        o = call(leaf)
+        assert torch.equal(o.detach(), want)
+        with pytest.raises(RuntimeError, match=name[:10]):
+            (o.float().sum() + leaf.float().sum()).backward()
+        call(leaf).mul_(2)   # (a result like any other)
+        with forward_ad.dual_level():
+            assert torch.equal(call(q), want)
+            with pytest.raises(RuntimeError, match="jvp"):
+                call(forward_ad.make_dual(q, q))
+
+
+def test_derivatives_of_the_attention_over_a_cache_raise(monkeypatch):
+    """(With another call in the place of the kernels'.)"""
+    cache = ft.new_cache(1, 16, 2, 64, device="cpu", dps=True)
+    monkeypatch.setattr(_native, "host_decode", lambda op, *a: (a[9].detach() * 2, a[9].detach().sum(-1)))
+    q = torch.randn(1, 2, 3, 64)
+    _decode_derivatives_raise(_decodes(cache, torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)), q)
+
+
+@pytest.mark.gpu
+def test_derivatives_of_the_attention_over_a_cache_raise_on_the_gpu():
+    bt = Batch(1, 2, 3, 64, "fp16", "e4m3", 16, [20], dps=True)
+    _decode_derivatives_raise(_decodes(bt.cache, bt.table, bt.context), bt.q.to(DEV))
+    ft.check_status(DEV)
+
+
 def _attentions():
     return (("flash_trittention", lambda xs: ft.flash_trittention(*xs, 0.125, None, None, None, None)),
             ("TrittentionTriton", lambda xs: ft.TrittentionTriton(softmax_scale=0.125)(*xs)[0]))
