@@ -115,11 +115,11 @@ def norm_rotary_backward(xs, ws, cos, sin, positions, eps, interleaved, dys, wei
     out = []
     for i in range(3):
         a.y[i] = _native.rows(dys[i])
-        out.append(_native.strided(dxs[i]))   # (a layout that the kernel does not write gets a contiguous stand-in)
+        out.append(_native.strided(dxs[i]))   # (a layout that the kernel does not write gets a contiguous stand-in, and is copied)
         a.dx[i] = _native.rows(out[i])
         a.dw[i] = None if dws[i] is None else dws[i].data_ptr()
     _native.norm_rotary(a, xs[0].device, backward=True)
-    return (*out, *dws)
+    return (*(dx if o is dx else dx.copy_(o) for dx, o in zip(dxs, out)), *dws)
 
 
 class QkNormRotary(torch.autograd.Function):

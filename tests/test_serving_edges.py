@@ -1,4 +1,5 @@
 """Calls at the edges of the cache's operators and of the norms: sizes that 32 bits do not hold, derivatives that there are not, bad pointers."""
+import ctypes
 import importlib
 import math
 
@@ -7,7 +8,7 @@ import torch
 from torch.autograd import forward_ad
 
 import flash_trittention as ft
-from flash_trittention import _native
+from flash_trittention import _native, ops  # noqa: F401  (the operators, registered)
 from oracle import serving_oracle as orc
 from test_cache import DEV, Batch
 
@@ -99,6 +100,62 @@ def test_a_second_derivative_of_the_norms_raises(monkeypatch):
 def test_a_second_derivative_of_the_norms_kernels_raises():
     xs, ws = _leaves((2, 3, 20, 64), torch.float32, DEV)
     _second_derivatives_raise(lambda: sum(ft.qk_norm_rotary(*xs, *ws)), xs + ws, xs[0].detach(), "qk_norm_rotary")
+
+
+def _layouts(dtype, device):
+    """[2, 3, 20, 64] tensors: plain, parts of a projection, rows that are not contiguous, expanded over heads, off 16-byte boundaries."""
+    g = torch.Generator().manual_seed(4)
+    new = lambda *shape: torch.randn(shape, generator=g).to(device, dtype)  # noqa: E731
+    return {"plain": new(2, 3, 20, 64), "projection": new(2, 20, 5, 3, 64)[:, :, 1].transpose(1, 2), "columns": new(2, 3, 64, 20).transpose(2, 3),
+            "expanded": new(2, 1, 20, 64).expand(2, 3, 20, 64), "every other": new(2, 3, 20, 128)[..., ::2], "heads last": new(2, 64, 20, 3).transpose(1, 3),
+            "odd": new(2 * 3 * 20 * 64 + 1)[1:].view(2, 3, 20, 64)}
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_gradients_of_the_norms_have_the_declared_layout(dtype, monkeypatch):
+    """A compiler is told that the inputs' gradients are laid out as ``empty_like`` would.  (The kernel's place is taken by one that writes a
+    number for each tensor into every row that it is given.)"""
+    module = importlib.import_module("flash_trittention.norm_rotary")
+
+    def kernel(a, dev, backward):
+        for i in range(3):
+            r, size = a.dx[i], dtype.itemsize
+            for b in range(a.B):
+                for n in range(a.N):
+                    for t in range(a.T):
+                        at = r.p + size * (b * r.stride_b + n * r.stride_n + t * r.stride_t)
+                        ctypes.memmove(at, (ctypes.c_char * (size * a.D)).from_buffer_copy(torch.full((a.D,), i + 1.0).to(dtype).view(torch.uint8).numpy()),
+                                       size * a.D)
+
+    monkeypatch.setattr(_native, "host_norm_rotary_backward", lambda *a: None)
+    monkeypatch.setattr(_native, "norm_rotary", kernel)
+    layouts = _layouts(dtype, "cpu")
+    for name, x in layouts.items():
+        xs = (x, layouts["plain"], layouts["columns"])
+        out = module.norm_rotary_backward(xs, (None,) * 3, None, None, None, 1e-6, False, (layouts["plain"],) * 3, (False,) * 3)
+        for i, (dx, of) in enumerate(zip(out, xs)):
+            assert dx.stride() == torch.empty_like(of).stride(), name
+            assert bool((dx == i + 1).all()), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_the_norms_operators_on_other_layouts(dtype):
+    """Declared and real layouts, of the forward and of the backward; and the same numbers as of contiguous tensors."""
+    ns, layouts = torch.ops.flash_trittention, _layouts(dtype, DEV)
+    w = torch.rand(64, device=DEV) + 0.5
+    cos, sin = ft.rotary_tables(20, 32, device=DEV)
+    dys = [torch.randn(2, 3, 20, 64, device=DEV).to(dtype) for _ in range(3)]
+    checks = ("test_schema", "test_faketensor", "test_autograd_registration")
+    for name, x in layouts.items():
+        xs = [x, layouts["plain"], x]
+        args = (*xs, w, None, w, cos, sin, None, 1e-6, False)
+        torch.library.opcheck(ns.norm_rotary.default, args, test_utils=checks)
+        torch.library.opcheck(ns.norm_rotary_bwd.default, (*args, *dys, [True, False, True]), test_utils=checks)
+        got = ns.norm_rotary_bwd(*args, *dys, [True, False, True])
+        want = ns.norm_rotary_bwd(*(t.contiguous() for t in xs), *args[3:], *dys, [True, False, True])
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), name
+    ft.check_status(DEV)
 
 
 def test_a_tangent_through_the_norms_raises(monkeypatch):
