@@ -87,6 +87,17 @@ __device__ __forceinline__ float code_scale(int byte) {
   return byte == 255 ? __uint_as_float(0x7fffffffu) : __uint_as_float((uint32_t)byte << 23);
 }
 
+// Rows of a tile are brought to one exponent as fp16 numbers (the products' operands), which keeps all but 2^-14 of a row whose exponent is up to this
+// much below the largest one.  That largest row may be one that nobody attends to, so where exponents lie further apart each row keeps
+// its own, and scores and P are multiplied by it column by column (slower, and rare: rows of zeros do not count).
+constexpr int kSpread = 24;
+// An exponent byte, where it counts towards the least one of several: rows of zeros or next to it, NaN and those that are not there do not.
+__device__ __forceinline__ int least_byte(int byte) { return byte > 1 ? byte : 255; }
+// From this on a score's factor (of sums of products up to 2^24) is multiplied in before the maximum is subtracted: rounded with it, as one
+// multiplication and addition, scores near 2^25 would be off by enough to leave the range of P.
+constexpr float kLargeFactor = 1.f / 64;
+__device__ __forceinline__ float power_of_two(int e) { return exp2f((float)e); }   // any e
+
 // Eight codes of neighbouring elements: 16 bytes of fp16, 8 of the others.  A row that is not finite has zeros.
 template <int CODE> struct Codes8;
 template <> struct Codes8<TRITT_CODE_F16> {

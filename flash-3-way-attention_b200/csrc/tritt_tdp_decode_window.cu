@@ -61,9 +61,9 @@ template <int D> __device__ __forceinline__ int staged(int row, int chunk) {
 }
 
 template <typename T16, int D, int CODE>
-__global__ void __launch_bounds__(kWarps * 32) tdp_decode_window_kernel(const __grid_constant__ WindowParams p) {
+__global__ void __launch_bounds__(kWarps * 32, D == 64 ? 2 : 1) tdp_decode_window_kernel(const __grid_constant__ WindowParams p) {
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int s_most[2];
+  __shared__ int s_most[2], s_least[2];   // exponents of the staged rows of K1 and of V1
   const TdpDecodeArgs& a = p.a;
   const CacheArgs& ca = a.cache;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(kWarps * 32) tdp_decode_window_kernel(const __
   uint32_t* const sNan = sThere + p.cols / 32;
   uint8_t* const sTree = reinterpret_cast<uint8_t*>(sNan + p.cols / 32);   // [tokens][64]: which new token is the d-th that a new token attends to
   float* const sPart = reinterpret_cast<float*>(sTree + (ca.c.ancestors ? p.tokens * 64 : 0));   // [tokens][tiles][D + 2]
-  if (tid < 2) s_most[tid] = 0;
+  if (tid < 2) s_most[tid] = 0, s_least[tid] = 255;
   __syncthreads();
 
   // --- what these tokens attend to, by numbers in the sequence: columns lo_j .. end - 1, rows lo_k .. end - 1
@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(kWarps * 32) tdp_decode_window_kernel(const __
         e1[k] = __ldg(ca.c.exponents + at);
         e2[k] = __ldg(ca.c.exponents + at2);
       }
-      int m1 = 0, m2 = 0;
+      int m1 = 0, m2 = 0, n1 = 255, n2 = 255;
 #pragma unroll
       for (int k = 0; k < kBatch; ++k) {
         const int r = r0 + k * kStep;
@@ -132,8 +132,10 @@ __global__ void __launch_bounds__(kWarps * 32) tdp_decode_window_kernel(const __
         if (ch == 0) exps[r] = (uint8_t)e1[k], exps2[r] = (uint8_t)e2[k];
         m1 = max(m1, e1[k] == 255 ? 0 : e1[k]);
         m2 = max(m2, e2[k] == 255 ? 0 : e2[k]);
+        n1 = min(n1, least_byte(e1[k]));
+        n2 = min(n2, least_byte(e2[k]));
       }
-      if (columns && ch == 0) atomicMax(&s_most[0], m1), atomicMax(&s_most[1], m2);
+      if (columns && ch == 0) atomicMax(&s_most[0], m1), atomicMax(&s_most[1], m2), atomicMin(&s_least[0], n1), atomicMin(&s_least[1], n2);
     }
   };
   stage(kPartK1, kPartV1, lo_j, nj, p.cols, sK1, sV1, sEk1, sEv1, true);
@@ -164,19 +166,20 @@ __global__ void __launch_bounds__(kWarps * 32) tdp_decode_window_kernel(const __
     if (lane == 0) sScale[i] = fabsf(a.scale2) * __uint_as_float((uint32_t)(254 - power) << 23) * (float)(1 << kDown<CODE>);
   }
   __syncthreads();
-  // K1 and V1 to the largest exponent of all staged rows (exact above 2^-24 of fp16's range)
+  // K1 and V1 to the largest exponent of all staged rows, where they are near enough to each other
   const int ek1 = s_most[0], ev1 = s_most[1];
+  const bool wide_k = ek1 - s_least[0] > kSpread, wide_v = ev1 - s_least[1] > kSpread;
   {
-    auto bring = [&](uint8_t* at, const uint8_t* exps, int most) {
+    auto bring = [&](uint8_t* at, const uint8_t* exps, int most, bool wide) {
       for (int x = tid; x < nj * L; x += kWarps * 32) {
         const int r = x / L, byte = exps[r];
-        const uint32_t f = half_power(kUp<CODE> + (byte == 255 ? 0 : byte) - most);
+        const uint32_t f = half_power(wide ? kUp<CODE> : kUp<CODE> + (byte == 255 ? 0 : byte) - most);
         uint4& v = *reinterpret_cast<uint4*>(at + staged<D>(r, x % L));
         v = make_uint4(mul_half2(v.x, f), mul_half2(v.y, f), mul_half2(v.z, f), mul_half2(v.w, f));
       }
     };
-    bring(sK1, sEk1, ek1);
-    bring(sV1, sEv1, ev1);
+    bring(sK1, sEk1, ek1, wide_k);
+    bring(sV1, sEv1, ev1, wide_v);
     for (int w = warp; w < (nj + 31) / 32; w += kWarps) {
       const int e1 = sEk1[w * 32 + lane], e2 = sEv1[w * 32 + lane];
       const uint32_t there = __ballot_sync(0xffffffffu, e1 && e2), nan = __ballot_sync(0xffffffffu, e1 == 255 || e2 == 255);
@@ -184,7 +187,7 @@ __global__ void __launch_bounds__(kWarps * 32) tdp_decode_window_kernel(const __
     }
   }
   __syncthreads();
-  const float k1_scale = ek1 > kUp<CODE> ? __uint_as_float((uint32_t)(ek1 - kUp<CODE>) << 23) : 0.f;
+  const float k1_scale = wide_k ? 1.f : ek1 > kUp<CODE> ? __uint_as_float((uint32_t)(ek1 - kUp<CODE>) << 23) : 0.f;
 
   // (staged rows from a multiple of 8 on: where a thread's chunks lie does not change)
   const uint8_t* key_at[D / 32];
@@ -222,7 +225,7 @@ __global__ void __launch_bounds__(kWarps * 32) tdp_decode_window_kernel(const __
         if (ca.status) atomicOr(ca.status, kStatusPlace);
       }
       nan[h] = e1 == 255 || e2 == 255;   // (or, below, of a column that the row attends to)
-      scale[h] = on && e1 != 255 ? fmaxf(sScale[i] * __uint_as_float((uint32_t)e1 << 23) * k1_scale, 1e-37f) : 1e-37f;
+      scale[h] = on && e1 != 255 ? sScale[i] * __uint_as_float((uint32_t)e1 << 23) * k1_scale : 0.f;
       vweight[h] = on && e2 != 255 ? exp2f((float)(e2 - 127)) : 0.f;
       const int last = pk < (1 << 30) - a.kkr ? min(pos_q, pk + a.kkr) : pos_q;
       c_lo[h] = on ? max(max(0, pos_q - a.k1w), pk - min(pk, a.kkl)) : 1 << 30;
@@ -231,6 +234,9 @@ __global__ void __launch_bounds__(kWarps * 32) tdp_decode_window_kernel(const __
       if (on && ca.c.ancestors && last >= ctx && last >= c_lo[h])   // (its tokens between the first and the last of the window)
         tree[h] = word & (~0ull << sTree[i * 64 + max(c_lo[h] - ctx, 0)]) & (~0ull >> (63 - sTree[i * 64 + last - ctx]));
     }
+    const bool large = wide_k || __any_sync(0xffffffffu, scale[0] > kLargeFactor || scale[1] > kLargeFactor);
+    // (not 0: masked columns' -infinity stays one)
+    const float factor[2] = {large ? 1.f : fmaxf(scale[0], 1e-37f), large ? 1.f : fmaxf(scale[1], 1e-37f)};
     // A's fragments: elements 32 j + 8 t + 4 s + {0, 1 | 2, 3} of rows g, g + 8 in steps s = 0, 1.  For fp16 each as its upper 11 bits and what
     // they leave: under a narrow window a result has few terms whose errors could cancel.  (With the upper bits alone trees of 16 under a band of 65
     // were off by 3.1e-4, 58 us; so by 2.3e-4, 66 us, where fp16's own rounding of the result is 2.1e-4; with P in two parts instead 2.9e-4, 68 us.
@@ -263,6 +269,7 @@ __global__ void __launch_bounds__(kWarps * 32) tdp_decode_window_kernel(const __
     from = __reduce_min_sync(0xffffffffu, from);
     to = __reduce_max_sync(0xffffffffu, to);
     float acc[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    int v_exp[2] = {wide_v ? 0 : ev1, wide_v ? 0 : ev1};   // the exponent that a row's results count in
 #pragma unroll
     for (int n = 0; n < D / 8; ++n)
 #pragma unroll
@@ -298,6 +305,35 @@ __global__ void __launch_bounds__(kWarps * 32) tdp_decode_window_kernel(const __
           }
         }
       }
+      if (large) {
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float f = wide_k ? power_of_two(sEk1[c0 + n * 8 + 2 * t + e] - 127 - kUp<CODE>) : 1.f;
+            s[n][e] *= f * scale[0];
+            s[n][2 + e] *= f * scale[1];
+          }
+      }
+      if (wide_v) {   // the largest exponent of the rows that each of the two attends to
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          int top = v_exp[h];
+#pragma unroll
+          for (int n = 0; n < 4; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int byte = sEv1[c0 + n * 8 + 2 * t + e];
+              if ((mask[h] >> (n * 8 + 2 * t + e) & 1) && byte != 255) top = max(top, byte);
+            }
+          top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          const float grown = power_of_two(v_exp[h] - top);
+          v_exp[h] = top;
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n) acc[n][2 * h] *= grown, acc[n][2 * h + 1] *= grown;
+        }
+      }
       if (__any_sync(0xffffffffu, (mask[0] & mask[1]) != 0xffffffffu)) {
         const uint32_t b0 = mask[0] >> (2 * t), b1 = mask[1] >> (2 * t);
 #pragma unroll
@@ -314,7 +350,7 @@ __global__ void __launch_bounds__(kWarps * 32) tdp_decode_window_kernel(const __
         mx[h] = fmaxf(s[0][2 * h], s[0][2 * h + 1]);
 #pragma unroll
         for (int n = 1; n < 4; ++n) mx[h] = fmaxf(mx[h], fmaxf(s[n][2 * h], s[n][2 * h + 1]));
-        mx[h] *= scale[h];
+        mx[h] *= factor[h];
       }
       if (__any_sync(0xffffffffu, mx[0] > m[0] + kGap || mx[1] > m[1] + kGap)) {
         float corr[2];
@@ -338,8 +374,12 @@ __global__ void __launch_bounds__(kWarps * 32) tdp_decode_window_kernel(const __
       for (int n = 0; n < 4; ++n)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float p0 = exp2f(fmaf(s[n][2 * h], scale[h], shift[h])), p1 = exp2f(fmaf(s[n][2 * h + 1], scale[h], shift[h]));
+          float p0 = exp2f(fmaf(s[n][2 * h], factor[h], shift[h])), p1 = exp2f(fmaf(s[n][2 * h + 1], factor[h], shift[h]));
           l[h] += p0 + p1;
+          if (wide_v) {   // (a column that does not count has P = 0, and may have any exponent)
+            p0 *= power_of_two(min(0, sEv1[c0 + n * 8 + 2 * t] - v_exp[h]));
+            p1 *= power_of_two(min(0, sEv1[c0 + n * 8 + 2 * t + 1] - v_exp[h]));
+          }
           pf[n >> 1][(n & 1) * 2 + h] = pack2<__half>(p0, p1);
         }
 #pragma unroll
@@ -372,7 +412,7 @@ __global__ void __launch_bounds__(kWarps * 32) tdp_decode_window_kernel(const __
     }
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    const float v1_scale = exp2f((float)(ev1 - 127 - kUp<CODE>));
+    const float v1_scale[2] = {power_of_two(v_exp[0] - 127 - kUp<CODE>), power_of_two(v_exp[1] - 127 - kUp<CODE>)};
     float v[D / 4];   // columns 8 n + 2 t + e at 2 n + e
 #pragma unroll
     for (int n = 0; n < D / 8; ++n) {
@@ -380,7 +420,7 @@ __global__ void __launch_bounds__(kWarps * 32) tdp_decode_window_kernel(const __
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const float2 c = unpack2<__half>(*reinterpret_cast<const uint32_t*>(sV2 + staged<D>(place[h], n) + t * 4));
-        if (w[h] != 0.f) v[2 * n] = fmaf(c.x * w[h], acc[n][2 * h] * v1_scale, v[2 * n]), v[2 * n + 1] = fmaf(c.y * w[h], acc[n][2 * h + 1] * v1_scale, v[2 * n + 1]);
+        if (w[h] != 0.f) v[2 * n] = fmaf(c.x * w[h], acc[n][2 * h] * v1_scale[h], v[2 * n]), v[2 * n + 1] = fmaf(c.y * w[h], acc[n][2 * h + 1] * v1_scale[h], v[2 * n + 1]);
       }
     }
     // over the eight lanes of a column: halves change hands until each has D / 32 columns

@@ -1,0 +1,136 @@
+"""Attention over the cache beside rows that a new token does not attend to, and that are larger than its own by any power of two: another branch of a
+tree (a padded draft, say), a token outside the window or the band.  The result is that of the attended rows alone, as exact as without them."""
+import math
+
+import pytest
+import torch
+
+import flash_trittention as ft
+from oracle import serving_oracle as orc
+from test_cache import DEV, Batch, _check_result, _kernel_of_windows, _tree, _widened
+
+K1, K2, V1, V2 = range(4)
+
+
+def _enlarge(bt, b, token, parts, by):
+    """The rows of a token (every head) times 2^by, in the pages and in the 64-bit values."""
+    at = int(bt.table[b, token // bt.seq.page_size]), token % bt.seq.page_size
+    for part in parts:
+        byte = (bt.seq.exponents[at[0], part, :, at[1]].int() + by).clamp(2, 254)
+        bt.seq.exponents[at[0], part, :, at[1]] = byte.to(torch.uint8)
+        bt.seq.values[b][part, :, token] = orc.values(bt.seq.codes[at[0], part, :, at[1]], byte)
+    bt.cache.exponents.copy_(bt.seq.exponents)
+
+
+def _sees(bt, b, i, token, window):
+    """Whether new token i attends to a token, at a distance up to the window."""
+    ctx = bt.contexts[b]
+    rows, pos, at = orc._tokens(ctx, i, bt.words)
+    found = (rows == token).nonzero()
+    return len(found) > 0 and (window is None or at - int(pos[found[0, 0]]) <= window)
+
+
+TREES = [  # D dtype code n contexts parents hidden windows: hidden are (sequence, new token) or (sequence, token of the context)
+    (64, "fp16", "e4m3", 5, [40, 21], [-1, 0, 0, 1, 2], [(0, 42), (1, 22)], (None,) * 4),
+    (64, "bf16", "fp16", 7, [100], _tree(7, 2), [(0, 106), (0, 103)], (None,) * 4),
+    (64, "fp16", "int8", 16, [130, 300], _tree(16, 2), [(0, 130 + 9), (1, 300 + 14)], (100, 100, 32, 32)),
+    (128, "fp16", "fp16", 6, [70], [-1, 0, 0, 2, 1, 4], [(0, 72)], (None,) * 4),
+    (128, "bf16", "e4m3", 9, [60, 90], _tree(9, 3), [(0, 62), (1, 98)], (50, 70, 20, 40)),
+    (128, "bf16", "int8", 3, [200], [-1, -1, -1], [(0, 201)], (64, 64, None, None)),
+]
+
+
+def _tdp(bt, table, windows):
+    alpha = 1 / math.sqrt(bt.D)
+    out, lse = ft.tdp_decode(bt.q.to(DEV), bt.cache, table, bt.context, alpha, *windows, ancestors=bt.ancestors, return_lse=True)
+    ft.check_status(DEV)
+    return out, lse, alpha
+
+
+def _tdp_rows(bt, out, lse, windows, alpha, rows):
+    """Those rows against the definition, as the tests of the cache compare them (but for p below the kernels' range, which counts from the largest p
+    of the row's own tokens)."""
+    for b, h, i in rows:
+        ctx, x = bt.contexts[b], bt.seq.values[b][:, h]
+        ref = orc.tdp_row(bt.q[b, h, i].double(), x[0], x[1], x[2], x[3], ctx, i, alpha, windows, bt.words)
+        _check_result(out[b, h, i], lse[b, h, i], ref, bt.dt, bt.D, (ctx + bt.n) ** 2, True, True, (b, h, i))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("by", [18, 26, 40, 100, 200])
+@pytest.mark.parametrize("wide", [False])
+@pytest.mark.parametrize("D,dtype,code,n,contexts,parents,hidden,windows", TREES)
+def test_tdp_other_branches(D, dtype, code, n, contexts, parents, hidden, windows, wide, by):
+    bt = Batch(len(contexts), 2, n, D, dtype, code, 16, contexts, parents=parents, seed=21)
+    table = _widened(bt.table, 8192, 16) if wide else bt.table
+    if all(w is None for w in windows):
+        assert _kernel_of_windows(bt, table, windows) != wide   # (either kernel)
+    for b, token in hidden:
+        _enlarge(bt, b, token, range(4), by)
+    out, lse, alpha = _tdp(bt, table, windows)
+    again = _tdp(bt, table, windows)
+    blind = [(b, h, i) for b, h, i in bt.rows() if not any(s == b and _sees(bt, b, i, t, None) for s, t in hidden)]
+    assert len(blind) > 2 and len(blind) < len(contexts) * 2 * n
+    assert all(torch.equal(out[at], again[0][at]) and torch.equal(lse[at], again[1][at]) for at in blind)
+    _tdp_rows(bt, out, lse, windows, alpha, blind)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("by", [18, 26, 40, 100, 200])
+@pytest.mark.parametrize("D,dtype,code", [(64, "fp16", "e4m3"), (64, "bf16", "int8"), (128, "fp16", "fp16"), (128, "bf16", "e4m3")])
+@pytest.mark.parametrize("windows", [(40, 60, None, None)])
+def test_tdp_tokens_outside_the_window_of_some(D, dtype, code, windows, by):
+    """A chain: the token is behind the windows of the later new tokens, in those of the first ones."""
+    ctx, n = 330, 9
+    at = ctx + 3 - max(windows[:2]) - 1   # the new tokens before number 3 see it
+    bt = Batch(1, 2, n, D, dtype, code, 16, [ctx], seed=23)
+    for part in range(4):
+        _enlarge(bt, 0, at, [part], by)
+    out, lse, alpha = _tdp(bt, _widened(bt.table, 8192, 16), windows)
+    blind = [(b, h, i) for b, h, i in bt.rows() if not _sees(bt, b, i, at, max(windows[:2]))]
+    assert len(blind) == 2 * (n - 3)
+    _tdp_rows(bt, out, lse, windows, alpha, blind)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("by", [26, 60])
+@pytest.mark.parametrize("D,dtype,code,windows", [(64, "fp16", "e4m3", (128, 128, 16, 16)), (128, "bf16", "fp16", (96, 96, 16, 16))])
+def test_tdp_large_keys_that_are_attended(D, dtype, code, windows, by):
+    """A K1 row 2^by larger, of a sign that gives its pairs a score of no weight: the other rows' scores keep their bits."""
+    ctx = 200
+    bt = Batch(1, 1, 1, D, dtype, code, 16, [ctx], seed=25)
+    at = ctx - 30
+    x, q, alpha = bt.seq.values[0][:, 0], bt.q[0, 0, 0].double(), 1 / math.sqrt(D)
+    # among rows k of the band around it, all of one sign: K2 rows there equal
+    page = bt.seq.page_size
+    src = int(bt.table[0, at // page]), at % page
+    for t in range(at - 16, at + 17):
+        to = int(bt.table[0, t // page]), t % page
+        bt.seq.codes.view(torch.uint8)[to[0], K2, :, to[1]] = bt.seq.codes.view(torch.uint8)[src[0], K2, :, src[1]]
+        bt.seq.exponents[to[0], K2, :, to[1]] = bt.seq.exponents[src[0], K2, :, src[1]]
+        x[K2, t] = x[K2, at]
+    if float((q * x[K1, at] * x[K2, at]).sum()) > 0:
+        codes = bt.seq.codes[src[0], K1, 0, src[1]]
+        bt.seq.codes[src[0], K1, 0, src[1]] = (-codes.float()).to(codes.dtype)
+        x[K1, at] = -x[K1, at]
+    bt.cache.codes.view(torch.uint8).copy_(bt.seq.codes.view(torch.uint8))
+    _enlarge(bt, 0, at, [K1], by)
+    out, lse, alpha = _tdp(bt, _widened(bt.table, 4096, 16), windows)
+    # (the score's error counts from the sum of |products| of the pairs that carry weight: those without that row)
+    y = x.clone()
+    y[K1, at] = 0
+    plain = orc.tdp_row(q, y[0], y[1], y[2], y[3], ctx, 0, alpha, windows)
+    ref = orc.tdp_row(q, x[0], x[1], x[2], x[3], ctx, 0, alpha, windows)
+    assert float(ref[3]) > 2 ** 20
+    _check_result(out[0, 0, 0], lse[0, 0, 0], (ref[0], ref[1], ref[2], plain[3]), bt.dt, D, (ctx + 1) ** 2, True, True, windows)
+
+
+def test_the_oracle_counts_only_what_is_attended():
+    """(Of the tests themselves: a row that is hidden changes no reference, one that is not changes it.)"""
+    bt_values = torch.randn(4, 12, 16, generator=torch.Generator().manual_seed(0)).double()
+    words = ft.tree_ancestors([-1, 0, 0, 1])
+    q = torch.randn(16, generator=torch.Generator().manual_seed(1)).double()
+    row = lambda v, i: orc.tdp_row(q, *v, 8, i, 0.25, (None,) * 4, words)[0]  # noqa: E731
+    big = bt_values.clone()
+    big[:, 10] *= 2.0 ** 30   # new token 2
+    assert torch.equal(row(bt_values, 3), row(big, 3)) and torch.equal(row(bt_values, 1), row(big, 1)) and not torch.equal(row(bt_values, 2), row(big, 2))
