@@ -21,6 +21,9 @@
 // Where rows are few or new tokens many, the way to the first tile and each piece's end count as much as the bytes: 24 tokens over 3001, 4 x 16
 // heads of 128, fp16: 37 us, of which a tile of 16 rows takes 2.5 thousand cycles (two warps a scheduler, a chain of two products and a soft-max)
 // and a piece 10 (first rows, queries, joining of the warps).
+// A tile's rows may be hidden from some or all of its queries (another branch of a tree, before a window).  Where one could be so much larger than what
+// the queries attend to that their P would leave fp16's range (2^12), each query goes on with an exponent of its own, the largest of the rows
+// that it attends to.
 // Append forms P as the sum of two fp16 numbers (22 bits): its result is rounded again, to codes, and each element that a less exact one moves over
 // a border is off by a whole step (e4m3: 0.13 % of W's norm with one fp16 number, 2e-5 with two).
 #include "tritt_cache.cuh"
@@ -34,6 +37,7 @@ using namespace sm100;
 constexpr int kWarps = 4;
 constexpr int kLift = 5;        // P is formed times 2^5; the reference is raised when a score is 2^8 above it: at most 2^13
 constexpr float kGap = 8.f;
+constexpr int kHidden = 12;     // see above
 constexpr int kLeastSteps = 8;  // of a block: two tiles a warp
 
 // What the line of steps has of one sequence.
@@ -130,6 +134,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm<NT>) dps_decode_kern
   __shared__ unsigned long long s_word[Q];
   __shared__ int s_lo[Q], s_pos[Q];
   __shared__ float s_scale[Q], s_m[kWarps][Q], s_l[kWarps][Q];
+  __shared__ int s_own[kWarps][Q];   // queries' exponents, where they differ
   const DpsDecodeArgs& a = p.a;
   const CacheArgs& ca = a.cache;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -334,6 +339,8 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm<NT>) dps_decode_kern
       for (int q = 0; q < NQ; ++q) m[nt][q] = -INFINITY, l[nt][q] = 0.f;
     }
     int v_exp = 0;   // largest exponent byte of the values so far
+    int low = 255;   // least one that may have to be told from it: of the tiles with rows that some query does not attend to, and before them
+    bool own = false;
     for (int tile = s0 + warp; tile < tile1; tile += kWarps) {
       if (!__all_sync(0xffffffffu, mbar_wait(&full[st], phase, (volatile int*)&s_abort))) {
         // give copies still in flight a bounded chance to land before the block ends
@@ -352,7 +359,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm<NT>) dps_decode_kern
       bool plain = token0 >= lo_all && token0 + TK <= ctx && there == (1u << NB) - 1;
       {
         constexpr int PER = (TK + 31) / 32;
-        int ek[PER], ev[PER], most = 0;
+        int ek[PER], ev[PER], most = 0, fewest = 255;
         bool bad = false;
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
@@ -362,11 +369,24 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm<NT>) dps_decode_kern
           ev[k] = on ? from[S::kOffEv + token] : 0;
           bad = bad || ek[k] == 255 || ev[k] == 255;
           most = max(most, ev[k] == 255 ? 0 : ev[k]);
+          fewest = min(fewest, least_byte(ev[k]));
         }
         plain = !__any_sync(0xffffffffu, bad) && plain;
-        most = max(v_exp, (int)__reduce_max_sync(0xffffffffu, most));
+        most = __reduce_max_sync(0xffffffffu, most);
+        bool apart;
+        if (plain) {
+          apart = most > 1 && v_exp - most > kHidden;
+        } else {
+          low = min(min(low, least_byte(v_exp)), (int)__reduce_min_sync(0xffffffffu, fewest));
+          apart = max(v_exp, most) - low > kHidden;
+        }
+        most = max(v_exp, most);
+        if (apart && !own) {
+          own = true;
+          if (lane < Q) s_own[warp][lane] = v_exp;
+        }
         // (the products lie in the accumulator times 2^(largest exponent))
-        if (most > v_exp) {
+        if (most > v_exp && !own) {
           const float grown = v_exp ? power(v_exp - most) : 1.f;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
@@ -453,6 +473,76 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm<NT>) dps_decode_kern
             if (missing && ca.status) atomicOr(ca.status, kStatusPlace);
           }
         }
+      auto raise_reference = [&](int nt, const float (&mx)[NQ]) {
+        float corr[NQ];
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+          float v = fmaxf(mx[q], m[nt][q]);
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+          corr[q] = v == -INFINITY ? 1.f : exp2f(m[nt][q] - v);
+          m[nt][q] = v;
+          l[nt][q] *= corr[q];
+        }
+#pragma unroll
+        for (int mb = 0; mb < D / 16; ++mb)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if ((e & 1) < NQ) acc[nt][mb][e] *= corr[e & 1 ? NQ - 1 : 0];
+      };
+      // Queries with exponents of their own: these, and the rows' powers of two in the scores, from which P is formed; the sum is told beforehand of
+      // what that takes away
+      if (own) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float mx[NQ];
+#pragma unroll
+          for (int q = 0; q < NQ; ++q) {
+            int& mine = s_own[warp][nt * 8 + 2 * t + q];
+            const int old = m[nt][q] == -INFINITY ? 0 : mine;   // (0: nothing attended so far)
+            int now = old;
+            mx[q] = -INFINITY;
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const int byte = from[S::kOffEv + nb * 16 + h * 8 + actual_row<RB>(g)];
+                if (s[nt][nb][2 * h + q] != -INFINITY && byte != 255) now = max(now, byte);
+                mx[q] = fmaxf(mx[q], s[nt][nb][2 * h + q]);
+              }
+            now = max(now, __shfl_xor_sync(0xffffffffu, now, 4));
+            now = max(now, __shfl_xor_sync(0xffffffffu, now, 8));
+            now = max(now, __shfl_xor_sync(0xffffffffu, now, 16));
+            const float grown = power_of_two(old - now);
+#pragma unroll
+            for (int mb = 0; mb < D / 16; ++mb) acc[nt][mb][q] *= grown, acc[nt][mb][2 + q] *= grown;
+            __syncwarp();
+            if (g == 0) mine = now;
+            __syncwarp();
+          }
+          raise_reference(nt, mx);
+#pragma unroll
+          for (int q = 0; q < NQ; ++q) {
+            const float base = m[nt][q] == -INFINITY ? 0.f : m[nt][q];
+            const int mine = s_own[warp][nt * 8 + 2 * t + q];
+            float whole = 0.f, rest = 0.f;
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                float& v = s[nt][nb][2 * h + q];
+                whole += exp2f(v - base);
+                // (a row that the query does not attend to has -infinity, and may have any exponent)
+                v += (float)min(0, from[S::kOffEv + nb * 16 + h * 8 + actual_row<RB>(g)] - mine);
+                rest += exp2f(v - base);
+              }
+            l[nt][q] += whole - rest;
+          }
+        }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) vf[nb][0] = vf[nb][1] = 1 << kLift;
+      }
       // the reference (raised where a score is 2^8 above it), P
       uint32_t pf[NT][NB][2], pl[EXACT ? NT : 1][NB][2];
 #pragma unroll
@@ -466,24 +556,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm<NT>) dps_decode_kern
           for (int nb = 1; nb < NB; ++nb) mx[q] = fmaxf(mx[q], fmaxf(s[nt][nb][q], s[nt][nb][2 + q]));
           raise = raise || mx[q] > m[nt][q] + kGap;
         }
-        if (__any_sync(0xffffffffu, raise)) {
-          float corr[NQ];
-#pragma unroll
-          for (int q = 0; q < NQ; ++q) {
-            float v = fmaxf(mx[q], m[nt][q]);
-            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
-            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
-            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
-            corr[q] = v == -INFINITY ? 1.f : exp2f(m[nt][q] - v);
-            m[nt][q] = v;
-            l[nt][q] *= corr[q];
-          }
-#pragma unroll
-          for (int mb = 0; mb < D / 16; ++mb)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if ((e & 1) < NQ) acc[nt][mb][e] *= corr[e & 1 ? NQ - 1 : 0];
-        }
+        if (__any_sync(0xffffffffu, raise)) raise_reference(nt, mx);
 #pragma unroll
         for (int q = 0; q < NQ; ++q) base2[q] = m[nt][q] == -INFINITY ? 0.f : m[nt][q];   // (nothing attended so far: all P are 0)
 #pragma unroll
@@ -593,8 +666,9 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm<NT>) dps_decode_kern
         float top = -INFINITY;
 #pragma unroll
         for (int k = 0; k < kWarps; ++k) top = fmaxf(top, s_m[k][i]);
-        // (a warp without a value has v_exp 0 and adds nothing)
-        const float f = m[nt][q] == -INFINITY || v_exp == 0 ? 0.f : exp2f(m[nt][q] - top) * power(v_exp - 127) * (1.f / (1 << kLift));
+        // (a warp without a value has exponent 0 and adds nothing)
+        const int e = own ? s_own[warp][i] : v_exp;
+        const float f = m[nt][q] == -INFINITY || e == 0 ? 0.f : exp2f(m[nt][q] - top) * power(e - 127) * (1.f / (1 << kLift));
 #pragma unroll
         for (int mb = 0; mb < D / 16; ++mb)
           *reinterpret_cast<float2*>(&out[warp][i][g * (D / 8) + 2 * mb]) =

@@ -7,7 +7,7 @@ import torch
 
 import flash_trittention as ft
 from oracle import serving_oracle as orc
-from test_cache import DEV, Batch, _check_result, _kernel_of_windows, _tree, _widened
+from test_cache import DEV, Batch, _check_result, _kernel_of_windows, _score_error, _tree, _widened
 
 K1, K2, V1, V2 = range(4)
 
@@ -123,6 +123,60 @@ def test_tdp_large_keys_that_are_attended(D, dtype, code, windows, by):
     ref = orc.tdp_row(q, x[0], x[1], x[2], x[3], ctx, 0, alpha, windows)
     assert float(ref[3]) > 2 ** 20
     _check_result(out[0, 0, 0], lse[0, 0, 0], (ref[0], ref[1], ref[2], plain[3]), bt.dt, D, (ctx + 1) ** 2, True, True, windows)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("by", [14, 26, 40, 100, 200])
+@pytest.mark.parametrize("D,dtype,code,n,contexts,parents,hidden,windows", TREES)
+def test_dps_other_branches(D, dtype, code, n, contexts, parents, hidden, windows, by):
+    bt = Batch(len(contexts), 2, n, D, dtype, code, 16, contexts, dps=True, parents=parents, seed=27)
+    alpha = 1 / math.sqrt(D)
+    for b, token in hidden:
+        _enlarge(bt, b, token, range(4), by)
+    out, m = ft.dps_decode(bt.q.to(DEV), bt.cache, bt.table, bt.context, alpha, ancestors=bt.ancestors)
+    ft.check_status(DEV)
+    again = ft.dps_decode(bt.q.to(DEV), bt.cache, bt.table, bt.context, alpha, ancestors=bt.ancestors)
+    for b, h, i in bt.rows():
+        if any(s == b and _sees(bt, b, i, t, None) for s, t in hidden):
+            continue
+        assert torch.equal(out[b, h, i], again[0][b, h, i]) and torch.equal(m[b, h, i], again[1][b, h, i])
+        x = bt.seq.values[b][:, h]
+        ref = orc.dps_row(bt.q[b, h, i].double(), x[K2], x[V2], bt.seq.bias[b][h], contexts[b], i, alpha, None, bt.words)
+        _check_result(out[b, h, i], m[b, h, i], ref, bt.dt, D, contexts[b] + n, True, False, (b, h, i))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("by", [14, 26, 40, 100])
+@pytest.mark.parametrize("D,dtype,code", [(64, "fp16", "fp16"), (64, "bf16", "e4m3"), (128, "fp16", "int8"), (128, "bf16", "fp16")])
+def test_append_tokens_outside_the_window_of_some(D, dtype, code, by):
+    """The inner attention's window ends inside a tile: the rows before it are loaded with it."""
+    ctx, n, k_diff = 200, 11, 100
+    at = ctx + 4 - k_diff   # new tokens up to 4 see it
+    bt = Batch(1, 2, n, D, dtype, code, 16, [ctx], dps=True, seed=29)
+    _enlarge(bt, 0, at, [K1, V1], by)
+    x = torch.randn(1, n, 4, 2, D, generator=torch.Generator().manual_seed(5)).to(bt.dt)
+    k1, k2, v1, v2 = (x[:, :, i].transpose(1, 2) for i in range(4))
+    alpha = 1 / math.sqrt(D)
+    ft.dps_append(bt.cache, bt.table, bt.context, *(t.to(DEV) for t in (k1, k2, v1, v2)), alpha, k_diff)
+    back = [t.double().cpu() for t in ft.cache_read(bt.cache, bt.table, bt.context, n, torch.float32)]
+    ft.check_status(DEV)
+    grid = {"fp16": 2.0 ** -11, "e4m3": 2.0 ** -4, "int8": 2.0 ** -7}[code]
+    for h in range(2):
+        key, val = bt.seq.values[0][K1, h].clone(), bt.seq.values[0][V1, h].clone()
+        key[ctx:], val[ctx:] = back[0][0, h], back[2][0, h]
+        for i in range(4, n):
+            y, lse, mass, size = orc.dps_row(k2[0, h, i].double(), key, val, None, ctx, i, alpha, k_diff)
+            if i == 4:
+                assert float(size) > 2.0 ** by / 8   # (it sees the row)
+                continue
+            w, mass = y * v2[0, h, i].double(), mass * v2[0, h, i].double().abs()
+            d = _score_error(D, float(size), True, False)
+            err = (math.expm1(2 * d) + 2.0 ** -10) * (mass + w.abs())
+            top = float((w.abs() + err).max())
+            rounding = (grid * w.abs() if code != "int8" else 0) + {"fp16": 2.0 ** -24, "e4m3": 2.0 ** -17, "int8": 2.0 ** -7}[code] * top
+            bad = (back[3][0, h, i] - w).abs() - (err * (1 + 2 * grid) + rounding + 1e-30)
+            assert float(bad.max()) <= 0, (h, i, float(bad.max()))
+            assert abs(float(back[4][0, h, i]) - float(lse)) <= d + 2.0 ** -22 * (1 + abs(float(lse)))
 
 
 def test_the_oracle_counts_only_what_is_attended():
