@@ -787,6 +787,7 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
         tc_fence_after();
         // the accumulator times `corr` (s_ready of this slab was committed behind the previous slab's P V)
         auto correct = [&](float corr) {
+          tmem_wait_st();   // (it may be for the second or third time in this slab: what the last one wrote is read)
 #pragma unroll 1
           for (int ch = 0; ch < D / 16; ++ch) {
             uint32_t o[16];
