@@ -10,9 +10,12 @@
 // short sequence still uses all SMs, and nothing of it is known to the host.  A part that begins or ends inside a pair of tiles leaves its
 // groups' maxima, sums and results all the same; a second kernel joins all groups and pieces of a row in a fixed order.
 //
-// Codes become fp16 operands: a slab's rows, whose exponents differ, are brought to the largest one's by exact multiplications by powers of
-// two, whatever lies 2^-38 below is lost.  K1's exponent joins the scale of the scores, for each 32 columns; V1's runs along with the
+// Codes become fp16 operands: a slab's rows, whose exponents differ, are brought to the largest one's by multiplications by powers of
+// two.  K1's exponent joins the scale of the scores, for each 32 columns; V1's runs along with the
 // accumulator, which is multiplied where it grows.  A is rounded once to 11 bits, P (times 2^7, fp16's lower range) once.
+// Where exponents lie further apart than 2^24 (of 32 rows of K1, or of a piece's rows of V1), whoever attends to them, V1's rows keep their own from there to
+// the piece's end, and K1's those of the 32: the soft-max warps multiply scores by K1's before they use them, and P by V1's, relative to the largest one that the row
+// attends to.  (Below, the 8 tokens over 2040 with one row 2^40 larger, 20 tokens before the end: 870 us instead of 356.)
 //
 //   warp 1        walks the line and tells the others each piece (a pair of tiles, a range of slabs) by a ring in shared memory: what each
 //                 role kept of the walk before cost it registers that it had not, and spills go to L2 beside 213 KB of shared memory
@@ -62,8 +65,9 @@ template <int D> struct Cfg {
   static constexpr int kOffQ = kOffV + kStages * kTile;            // [8 warps][D] fp16
   static constexpr int kOffRows = kOffQ + 8 * D * 2;               // [256] RowInfo
   static constexpr int kOffRun = kOffRows + 256 * 32;          // [8 warps][D] fp32
-  static constexpr int kOffMisc = kOffRun + 8 * D * 4;
-  static constexpr int kSmem = kOffMisc + 1536;
+  static constexpr int kOffOwn = kOffRun + 8 * D * 4;              // [256] rows' own exponents of V1
+  static constexpr int kOffMisc = kOffOwn + 1024;
+  static constexpr int kSmem = kOffMisc + 3072;
   static constexpr int kTmemO = 256;                               // S_a | S_b | acc_a | acc_b
 };
 
@@ -71,8 +75,15 @@ struct __align__(16) Meta {   // of one slab, by the warp that loaded 32 of its 
   uint32_t there[4];      // rows that have a place
   uint32_t nan[4];        // rows that read as NaN (K1 or V1)
   float scale[4];         // of the 32 columns' scores
-  int v_exp[4];           // largest exponent byte of V1's rows
+  uint32_t span[4];       // exponent bytes of V1's rows
+  uint8_t ek[128], ev[128];
 };
+// The largest and the least of some exponent bytes in one word, of which the larger halves of two are those of both: the largest in the upper half, 255
+// less the least one (of rows of zeros: none) in the lower.  kApart: K1's rows have kept their own, which counts like V1's being too far apart.
+constexpr uint32_t kApart = 4096;
+__device__ __forceinline__ uint32_t span_of(int largest, int least) { return (uint32_t)largest << 16 | (uint32_t)(255 - least); }
+__device__ __forceinline__ uint32_t span_with(uint32_t a, uint4 b) { return __vmaxu2(__vmaxu2(__vmaxu2(a, b.x), b.y), __vmaxu2(b.z, b.w)); }
+__device__ __forceinline__ bool too_wide(uint32_t span) { return (span >> 16) + (span & 0xffffu) > 255u + kSpread; }
 
 // A row of a tile, by the thread that formed its A for the one that works on its scores.
 struct __align__(16) RowInfo {
@@ -103,7 +114,7 @@ struct Misc {
   uint32_t tmem_base;
   int abort_flag;
 };
-static_assert(sizeof(Misc) <= 1536, "shared memory of the barriers");
+static_assert(sizeof(Misc) <= 3072, "shared memory of the barriers");
 
 // What the line of steps has of one sequence.
 struct Line {
@@ -310,6 +321,86 @@ template <int D, int CODE> struct TileLoader {   // a warp's 32 rows of one part
     }
   }
 };
+
+// A row's slab where rows of K1 or V1 keep their exponents, and of large scores: what the soft-max warps do otherwise, column by column in two passes.
+// (Not inlined: rare, and registers are few.)  -> the row's reference, what its sum is multiplied by, what is added to it
+struct SlabApart {
+  uint32_t tS, tO;
+  int chunks, wid, up;       // of 16 columns of the accumulator; columns; kUp
+  uint32_t before, span;     // V1's exponents up to the slab before, and to this one
+  bool later;                // (the accumulator holds something)
+};
+__device__ __noinline__ float4 slab_apart(const Meta& m, SlabApart a, uint4 mask, float scale, float m_used, int* own) {
+  auto attended = [&](int c) { return (c < 64 ? c < 32 ? mask.x : mask.y : c < 96 ? mask.z : mask.w) >> (c & 31) & 1; };
+  auto score = [&](uint32_t s, int c) {   // in log2 units
+    const float block = m.scale[c >> 5];
+    return __uint_as_float(s) * (scale * (block < 0.f ? power_of_two(m.ek[c] - 127 - a.up) : block));
+  };
+  const bool wide = too_wide(a.span);
+  const int common = (int)(a.before >> 16);   // V1's exponent so far
+  // (0: nothing attended so far.  A common exponent may be of rows that this one does not attend to: then the least that all of them have)
+  const int old = !wide ? common : m_used == -INFINITY ? 0 : *own;
+  int now = !wide ? (int)(a.span >> 16) : m_used == -INFINITY ? 0 : too_wide(a.before) ? *own : most(common - kSpread, 1);
+  float mx = -INFINITY;
+#pragma unroll 1
+  for (int c0 = 0; c0 < 128 && c0 < a.wid; c0 += 16) {
+    uint32_t s[16];
+    __syncwarp();
+    tmem_ld16(a.tS + c0, s);
+    tmem_wait_ld(s);
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      if (attended(c0 + e)) {
+        mx = fmaxf(mx, score(s[e], c0 + e));
+        if (wide && m.ev[c0 + e] != 255) now = most(now, m.ev[c0 + e]);
+      }
+  }
+  const bool grow = mx > m_used + kGap;
+  const float corr = grow ? exp2f(m_used - mx) : 1.f;
+  if (grow) m_used = mx;
+  *own = now;
+  __syncwarp();
+  if (a.later) {
+    const float f = corr * power_of_two(old - now);
+#pragma unroll 1
+    for (int ch = 0; ch < a.chunks; ++ch) {
+      uint32_t o[16];
+      tmem_ld16(a.tO + ch * 16, o);
+      tmem_wait_ld(o);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+      tmem_st16(a.tO + ch * 16, o);
+    }
+  }
+  const float base = m_used == -INFINITY ? 0.f : m_used;
+  float sum = 0.f;
+#pragma unroll 1
+  for (int c0 = 0; c0 < 128 && c0 < a.wid; c0 += 32) {   // (P of 32 columns over the first half of theirs and before)
+    uint32_t pk[16];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      uint32_t s[16];
+      __syncwarp();
+      tmem_ld16(a.tS + c0 + half * 16, s);
+      tmem_wait_ld(s);
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) {
+        float v[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int c = c0 + half * 16 + e + k;
+          v[k] = attended(c) ? exp2f(score(s[e + k], c) - base + kLift) : 0.f;
+          sum += v[k];
+          if (wide) v[k] *= power_of_two(least(0, m.ev[c] - now));
+        }
+        pk[half * 8 + e / 2] = pack2<__half>(v[0], v[1]);
+      }
+    }
+    __syncwarp();
+    tmem_st16(a.tS + c0 / 2, pk);
+  }
+  return make_float4(m_used, corr, sum, 0.f);
+}
 
 // A warp's 32 rows of a tile: token k of new token i each.  A = 2^-kDown q * code, q brought to [1, 2); the powers of two and alpha go to
 // the scores' scale.
@@ -655,7 +746,7 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
         return true;
       };
       if (!keys && forms) alive = form();
-      int v_exp = 0;   // the largest exponent byte of V1's rows in this piece so far
+      uint32_t span = 0;   // of V1's rows in this piece so far
       int token = first + w * 32 + lane;
       auto page_of = [&](int t) { return t < behind ? place_of(ca, b, t).page : -1; };
       int page = page_of(token);
@@ -678,25 +769,30 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
           if (ek == 255) ek = 0;   // (its codes are zeros)
           if (ev == 255) ev = 0;
           const int ek_most = __reduce_max_sync(0xffffffffu, ek), ev_most = __reduce_max_sync(0xffffffffu, ev);
+          const int ev_least = __reduce_min_sync(0xffffffffu, least_byte(ev));
+          const bool apart = __any_sync(0xffffffffu, least_byte(ek) < ek_most - kSpread);
           alive = __all_sync(0xffffffffu, mbar_wait(&empty[st], ph ^ 1, abort_flag));
           if (!alive) break;
+          Meta& m = ms.meta[mt];
+          m.ek[w * 32 + lane] = (uint8_t)ek;
+          m.ev[w * 32 + lane] = (uint8_t)ev;
+          __syncwarp();
           if (lane == 0) {
-            Meta& m = ms.meta[mt];
             m.there[w] = there;
             m.nan[w] = nan;
-            m.scale[w] = ek_most > kUp<CODE> ? __uint_as_float((uint32_t)(ek_most - kUp<CODE>) << 23) : 0.f;
-            m.v_exp[w] = ev_most;
+            m.scale[w] = apart ? -1.f : ek_most > kUp<CODE> ? __uint_as_float((uint32_t)(ek_most - kUp<CODE>) << 23) : 0.f;
+            m.span[w] = span_of(ev_most, ev_least) | (apart ? kApart : 0u);
             mbar_arrive(&ms.meta_full[mt]);
           }
-          up = kUp<CODE> + ek - ek_most;
+          up = apart ? kUp<CODE> : kUp<CODE> + ek - ek_most;
         } else {
           if (ev == 255) ev = 0;
           alive = __all_sync(0xffffffffu, mbar_wait(&ms.meta_full[mt], (pos / kMetas) & 1, abort_flag)) &&
                   __all_sync(0xffffffffu, mbar_wait(&empty[st], ph ^ 1, abort_flag));
           if (!alive) break;
           const volatile Meta& m = ms.meta[mt];
-          v_exp = max(max(max(v_exp, m.v_exp[0]), m.v_exp[1]), max(m.v_exp[2], m.v_exp[3]));
-          up = kUp<CODE> + ev - v_exp;
+          span = span_with(span, make_uint4(m.span[0], m.span[1], m.span[2], m.span[3]));
+          up = too_wide(span) ? kUp<CODE> : kUp<CODE> + ev - (int)(span >> 16);
         }
         if (any) {
           tile.store(ring + st * C::kTile, w * 32, half_power(up), lane, 0);
@@ -723,6 +819,7 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
     int slab = 0, scount = 0, mine = 0;   // slabs so far; this tile's, and its pieces
     // what the warp has of a new token runs along its pieces: maximum and sum here, the result in shared memory, a column a lane
     float* const run = reinterpret_cast<float*>(smem + C::kOffRun) + (x * 4 + wq) * D + lane;
+    int* const own = reinterpret_cast<int*>(smem + C::kOffOwn) + x * 128 + wq * 32 + lane;   // the exponent that this row's results count in
     long long last = -1;
     float m_run = -INFINITY, l_run = 0.f;
     bool alive = true;
@@ -748,7 +845,8 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
       if (lane == 0) mbar_arrive(&ms.a_free[x]);
       // --- slabs: a half of 64 columns at a time is read once, its maximum taken, and the row's reference raised where that is 2^8 above it
       float m_used = -INFINITY, l_sum = 0.f;
-      int v_exp = 0;
+      uint32_t span = 0;   // as the loading warps have it
+      *own = 0;
       for (int t = 0; t < n; ++t, ++scount) {
         const int pos = slab + t, c0 = first + t * 128, wid = behind - c0;
         const Meta& m = ms.meta[pos % kMetas];
@@ -758,7 +856,7 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
         }
         const uint4 there = *reinterpret_cast<const uint4*>(m.there), nan = *reinterpret_cast<const uint4*>(m.nan);
         const float4 ks = *reinterpret_cast<const float4*>(m.scale);
-        const int4 ve = *reinterpret_cast<const int4*>(m.v_exp);
+        const uint4 spans = *reinterpret_cast<const uint4*>(m.span);
         const bool clean = wid >= 128 && (there.x & there.y & there.z & there.w) == 0xffffffffu && (nan.x | nan.y | nan.z | nan.w) == 0u;
         const bool full = __all_sync(0xffffffffu, clean && r.c_lo <= c0 && r.c_hi >= c0 + 127);
         uint32_t mask[4] = {0u, 0u, 0u, 0u};   // columns that count
@@ -781,7 +879,10 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
         }
         // (a scale of 0, of rows of zeros: any small one, so that masked columns' -infinity stays one)
         const float f[4] = {fmaxf(r.scale * ks.x, 1e-37f), fmaxf(r.scale * ks.y, 1e-37f), fmaxf(r.scale * ks.z, 1e-37f), fmaxf(r.scale * ks.w, 1e-37f)};
-        const int v_now = max(max(max(v_exp, ve.x), ve.y), max(ve.z, ve.w));
+        const uint32_t before = span;
+        span = span_with(span, spans);
+        const bool wide = too_wide(span);   // rows keep their exponents, in this slab and those behind it
+        const bool odd = __any_sync(0xffffffffu, wide || fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])) > kLargeFactor);
         alive = __all_sync(0xffffffffu, mbar_wait(&ms.s_ready[x], scount & 1, abort_flag));
         if (!alive) break;
         tc_fence_after();
@@ -798,78 +899,89 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
             tmem_st16(tO + ch * 16, o);
           }
         };
-        if (t > 0 && v_now != v_exp) correct(v_now - v_exp < 126 ? __uint_as_float((uint32_t)(127 - (v_now - v_exp)) << 23) : 0.f);
-        v_exp = v_now;
         float psum = 0.f;
+        if (odd) {
+          const uint4 attended = full ? make_uint4(~0u, ~0u, ~0u, ~0u) : make_uint4(mask[0], mask[1], mask[2], mask[3]);
+          const float4 v = slab_apart(m, SlabApart{tS, tO, D / 16, wid, kUp<CODE>, before, span, t > 0}, attended, r.scale, m_used, own);
+          m_used = v.x;
+          l_sum *= v.y;
+          psum = v.z;
+        } else {
+          if (span >> 16 != before >> 16) {
+            const int by = (int)(span >> 16) - (int)(before >> 16);
+            *own = (int)(span >> 16);
+            if (t > 0) correct(by < 126 ? __uint_as_float((uint32_t)(127 - by) << 23) : 0.f);
+          }
 #pragma unroll 1
-        for (int hf = 0; hf < 2; ++hf) {   // (one copy of the code)
-          const float f0 = hf ? f[2] : f[0], f1 = hf ? f[3] : f[1];
-          if (some >> hf & 1) {
-            uint32_t sr[64];
-            tmem_ld64(tS + hf * 64, sr);
-            tmem_wait_ld();
-            if (!full) {
-              const uint32_t m0 = hf ? mask[2] : mask[0], m1 = hf ? mask[3] : mask[1];
+          for (int hf = 0; hf < 2; ++hf) {   // (one copy of the code)
+            const float f0 = hf ? f[2] : f[0], f1 = hf ? f[3] : f[1];
+            if (some >> hf & 1) {
+              uint32_t sr[64];
+              tmem_ld64(tS + hf * 64, sr);
+              tmem_wait_ld();
+              if (!full) {
+                const uint32_t m0 = hf ? mask[2] : mask[0], m1 = hf ? mask[3] : mask[1];
 #pragma unroll
-              for (int e = 0; e < 64; ++e) sr[e] = (e < 32 ? m0 : m1) >> (e % 32) & 1 ? sr[e] : 0xff800000u;
-            }
-            float mx;
-            {
-              float q[4];
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                q[k] = fmaxf(__uint_as_float(sr[k * 16]), __uint_as_float(sr[k * 16 + 1]));
-#pragma unroll
-                for (int e = 2; e < 16; e += 2) q[k] = fmaxf(q[k], fmaxf(__uint_as_float(sr[k * 16 + e]), __uint_as_float(sr[k * 16 + e + 1])));
+                for (int e = 0; e < 64; ++e) sr[e] = (e < 32 ? m0 : m1) >> (e % 32) & 1 ? sr[e] : 0xff800000u;
               }
-              mx = fmaxf(fmaxf(q[0], q[1]) * f0, fmaxf(q[2], q[3]) * f1);
-            }
-            const bool grow = mx > m_used + kGap;
-            if (__any_sync(0xffffffffu, grow)) {
-              const float corr = grow ? exp2f(m_used - mx) : 1.f;
-              if (grow) {
-                m_used = mx;
-                l_sum *= corr;
-                psum *= corr;
+              float mx;
+              {
+                float q[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  q[k] = fmaxf(__uint_as_float(sr[k * 16]), __uint_as_float(sr[k * 16 + 1]));
+#pragma unroll
+                  for (int e = 2; e < 16; e += 2) q[k] = fmaxf(q[k], fmaxf(__uint_as_float(sr[k * 16 + e]), __uint_as_float(sr[k * 16 + e + 1])));
+                }
+                mx = fmaxf(fmaxf(q[0], q[1]) * f0, fmaxf(q[2], q[3]) * f1);
               }
-              if (t > 0) correct(corr);
-              if (hf == 1) {   // (this slab's first half, formed already)
+              const bool grow = mx > m_used + kGap;
+              if (__any_sync(0xffffffffu, grow)) {
+                const float corr = grow ? exp2f(m_used - mx) : 1.f;
+                if (grow) {
+                  m_used = mx;
+                  l_sum *= corr;
+                  psum *= corr;
+                }
+                if (t > 0) correct(corr);
+                if (hf == 1) {   // (this slab's first half, formed already)
 #pragma unroll 1
-                for (int q = 0; q < 2; ++q) {
-                  uint32_t o[16];
-                  tmem_wait_st();
-                  tmem_ld16(tS + q * 16, o);
-                  tmem_wait_ld();
+                  for (int q = 0; q < 2; ++q) {
+                    uint32_t o[16];
+                    tmem_wait_st();
+                    tmem_ld16(tS + q * 16, o);
+                    tmem_wait_ld();
 #pragma unroll
-                  for (int e = 0; e < 16; ++e) {
-                    const float2 v = unpack2<__half>(o[e]);
-                    o[e] = pack2<__half>(v.x * corr, v.y * corr);
+                    for (int e = 0; e < 16; ++e) {
+                      const float2 v = unpack2<__half>(o[e]);
+                      o[e] = pack2<__half>(v.x * corr, v.y * corr);
+                    }
+                    tmem_st16(tS + q * 16, o);
                   }
-                  tmem_st16(tS + q * 16, o);
                 }
               }
-            }
-            const float shift = kLift - (m_used == -INFINITY ? 0.f : m_used);
-            float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
+              const float shift = kLift - (m_used == -INFINITY ? 0.f : m_used);
+              float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
+              for (int q = 0; q < 2; ++q) {
+                uint32_t pk[16];
+#pragma unroll
+                for (int c = 0; c < 32; c += 2) {
+                  const float2 z = fma_pair(make_float2(__uint_as_float(sr[q * 32 + c]), __uint_as_float(sr[q * 32 + c + 1])), q ? f1 : f0, shift);
+                  const float2 e = make_float2(exp2f(z.x), exp2f(z.y));
+                  sum[c >> 1 & 1] = add_pair(sum[c >> 1 & 1], e);
+                  pk[c >> 1] = pack2<__half>(e.x, e.y);
+                }
+                tmem_st16(tS + hf * 32 + q * 16, pk);
+              }
+              psum += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+            } else if (hf * 64 < wid) {
               uint32_t pk[16];
 #pragma unroll
-              for (int c = 0; c < 32; c += 2) {
-                const float2 z = fma_pair(make_float2(__uint_as_float(sr[q * 32 + c]), __uint_as_float(sr[q * 32 + c + 1])), q ? f1 : f0, shift);
-                const float2 e = make_float2(exp2f(z.x), exp2f(z.y));
-                sum[c >> 1 & 1] = add_pair(sum[c >> 1 & 1], e);
-                pk[c >> 1] = pack2<__half>(e.x, e.y);
-              }
-              tmem_st16(tS + hf * 32 + q * 16, pk);
+              for (int e = 0; e < 16; ++e) pk[e] = 0u;
+              tmem_st16(tS + hf * 32, pk);
+              tmem_st16(tS + hf * 32 + 16, pk);
             }
-            psum += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-          } else if (hf * 64 < wid) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) pk[e] = 0u;
-            tmem_st16(tS + hf * 32, pk);
-            tmem_st16(tS + hf * 32 + 16, pk);
           }
         }
         l_sum += bad ? __uint_as_float(0x7fffffffu) : psum;
@@ -908,7 +1020,7 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
       // V1's and V2's powers of two (fp32's range is that of the result's own type and more)
       const int byte2 = r.flags & 255;
       const float vscale =
-          weight == 0.f || byte2 == 255 ? 0.f : weight * exp2f((float)(v_exp - 127 - kUp<CODE>)) * exp2f((float)(byte2 - 127));
+          weight == 0.f || byte2 == 255 ? 0.f : weight * exp2f((float)(*own - 127 - kUp<CODE>)) * exp2f((float)(byte2 - 127));
       if (!__all_sync(0xffffffffu, mbar_wait(&ms.o_done[x], mine & 1, abort_flag))) {
         alive = false;
         break;

@@ -166,7 +166,8 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 2 : 1) tdp_decode_windo
     if (lane == 0) sScale[i] = fabsf(a.scale2) * __uint_as_float((uint32_t)(254 - power) << 23) * (float)(1 << kDown<CODE>);
   }
   __syncthreads();
-  // K1 and V1 to the largest exponent of all staged rows, where they are near enough to each other
+  // K1 and V1 to the largest exponent of all staged rows, where they are near enough to each other (else, trees of 16 as above with one row 2^40 larger: 92 us,
+  // not 68)
   const int ek1 = s_most[0], ev1 = s_most[1];
   const bool wide_k = ek1 - s_least[0] > kSpread, wide_v = ev1 - s_least[1] > kSpread;
   {

@@ -58,7 +58,7 @@ def _tdp_rows(bt, out, lse, windows, alpha, rows):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("by", [18, 26, 40, 100, 200])
-@pytest.mark.parametrize("wide", [False])
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("D,dtype,code,n,contexts,parents,hidden,windows", TREES)
 def test_tdp_other_branches(D, dtype, code, n, contexts, parents, hidden, windows, wide, by):
     bt = Batch(len(contexts), 2, n, D, dtype, code, 16, contexts, parents=parents, seed=21)
@@ -78,9 +78,9 @@ def test_tdp_other_branches(D, dtype, code, n, contexts, parents, hidden, window
 @pytest.mark.gpu
 @pytest.mark.parametrize("by", [18, 26, 40, 100, 200])
 @pytest.mark.parametrize("D,dtype,code", [(64, "fp16", "e4m3"), (64, "bf16", "int8"), (128, "fp16", "fp16"), (128, "bf16", "e4m3")])
-@pytest.mark.parametrize("windows", [(40, 60, None, None)])
+@pytest.mark.parametrize("windows", [(40, 60, None, None), (300, 300, 20, 8)])
 def test_tdp_tokens_outside_the_window_of_some(D, dtype, code, windows, by):
-    """A chain: the token is behind the windows of the later new tokens, in those of the first ones."""
+    """A chain: the token is behind the windows of the later new tokens, in those of the first ones.  (Window kernel and the other.)"""
     ctx, n = 330, 9
     at = ctx + 3 - max(windows[:2]) - 1   # the new tokens before number 3 see it
     bt = Batch(1, 2, n, D, dtype, code, 16, [ctx], seed=23)
@@ -94,7 +94,8 @@ def test_tdp_tokens_outside_the_window_of_some(D, dtype, code, windows, by):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("by", [26, 60])
-@pytest.mark.parametrize("D,dtype,code,windows", [(64, "fp16", "e4m3", (128, 128, 16, 16)), (128, "bf16", "fp16", (96, 96, 16, 16))])
+@pytest.mark.parametrize("D,dtype,code,windows", [(64, "fp16", "e4m3", (128, 128, 16, 16)), (128, "bf16", "fp16", (96, 96, 16, 16)),
+                                                  (64, "fp16", "fp16", (None, None, 16, 16)), (128, "fp16", "int8", (None, None, 8, 16))])
 def test_tdp_large_keys_that_are_attended(D, dtype, code, windows, by):
     """A K1 row 2^by larger, of a sign that gives its pairs a score of no weight: the other rows' scores keep their bits."""
     ctx = 200
