@@ -93,8 +93,8 @@ __device__ __forceinline__ float code_scale(int byte) {
 constexpr int kSpread = 24;
 // An exponent byte, where it counts towards the least one of several: rows of zeros or next to it, NaN and those that are not there do not.
 __device__ __forceinline__ int least_byte(int byte) { return byte > 1 ? byte : 255; }
-// From this on a score's factor (of sums of products up to 2^24) is multiplied in before the maximum is subtracted: rounded with it, as one
-// multiplication and addition, scores near 2^25 would be off by enough to leave the range of P.
+// From this on a score's factor (its sum of products may be 2^30) is multiplied in, and rounded, before the maximum is subtracted: as one multiplication and
+// addition, scores from 2^25 on would be off from the rounded maximum by enough to leave the range of P.
 constexpr float kLargeFactor = 1.f / 64;
 __device__ __forceinline__ float power_of_two(int e) { return exp2f((float)e); }   // any e
 

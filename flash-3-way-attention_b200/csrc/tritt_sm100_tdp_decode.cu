@@ -334,7 +334,8 @@ __device__ __noinline__ float4 slab_apart(const Meta& m, SlabApart a, uint4 mask
   auto attended = [&](int c) { return (c < 64 ? c < 32 ? mask.x : mask.y : c < 96 ? mask.z : mask.w) >> (c & 31) & 1; };
   auto score = [&](uint32_t s, int c) {   // in log2 units
     const float block = m.scale[c >> 5];
-    return __uint_as_float(s) * (scale * (block < 0.f ? power_of_two(m.ek[c] - 127 - a.up) : block));
+    // (rounded, as the maximum was: not taken into the subtraction)
+    return __fmul_rn(__uint_as_float(s), scale * (block < 0.f ? power_of_two(m.ek[c] - 127 - a.up) : block));
   };
   const bool wide = too_wide(a.span);
   const int common = (int)(a.before >> 16);   // V1's exponent so far

@@ -189,3 +189,25 @@ def test_the_oracle_counts_only_what_is_attended():
     big = bt_values.clone()
     big[:, 10] *= 2.0 ** 30   # new token 2
     assert torch.equal(row(bt_values, 3), row(big, 3)) and torch.equal(row(bt_values, 1), row(big, 1)) and not torch.equal(row(bt_values, 2), row(big, 2))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("precision", ["ieee", None])
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("D,code", [(64, "fp16"), (64, "e4m3"), (128, "int8")])
+@pytest.mark.parametrize("size", [1e6, 1e9, 1e13])
+def test_scores_of_which_32_bits_hold_no_fraction(D, code, size, wide, precision):
+    """The largest score's pair has p = 1, however large it is: a mean of the attended products comes out, and that score as the log-sum-exp (whose
+    relative error is A's rounding and the sums')."""
+    bt = Batch(2, 2, 3, D, "bf16", code, 16, [90, 40], seed=31)
+    bt.q = (bt.q.float() * size).to(torch.bfloat16)
+    alpha = 1 / math.sqrt(D)
+    table = _widened(bt.table, 8192, 16) if wide else bt.table
+    out, lse = ft.tdp_decode(bt.q.to(DEV), bt.cache, table, bt.context, alpha, return_lse=True, input_precision=precision)
+    ft.check_status(DEV)
+    for b, h, i in bt.rows():
+        x, ctx = bt.seq.values[b][:, h], bt.contexts[b]
+        _, want, _, scores = orc.tdp_row(bt.q[b, h, i].double(), *x, ctx, i, alpha)
+        most = (x[V1, : ctx + i + 1].abs().amax(0) * x[V2, : ctx + i + 1].abs().amax(0))
+        assert bool((out[b, h, i].double().cpu().abs() <= most * (1 + 2.0 ** -7)).all()), (b, h, i)
+        assert abs(float(lse[b, h, i]) - float(want)) <= (2.0 ** -11 + (D + 64) * 2.0 ** -24) * float(scores), (b, h, i)
