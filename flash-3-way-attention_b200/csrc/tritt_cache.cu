@@ -387,7 +387,7 @@ int tritt_decode_path(int op, int D, int dtype, int flags) { return fast(op, D, 
 size_t tritt_decode_workspace(int op, const tritt_cache_t* c, int dtype, int k1_window, int k2_window, int flags) {
   if (check_cache(c)) return 0;
   if (op == TRITT_OP_TDP_DECODE && fast(op, c->D, dtype, flags))
-    return window_tdp_decode_applies(*c, window(k1_window), window(k2_window), 1 << 30, 1 << 30) ? 0 : sm100_tdp_decode_workspace(*c);
+    return window_tdp_decode_applies(*c, dtype, window(k1_window), window(k2_window), 1 << 30, 1 << 30) ? 0 : sm100_tdp_decode_workspace(*c);
   if (fast(op, c->D, dtype, flags)) return mma_dps_decode_workspace(*c);
   return part_bytes(*c, simt_decode_splits(*c));
 }
@@ -405,7 +405,7 @@ int tritt_tdp_decode(const tritt_cache_t* c, const tritt_rows_t* q, void* o, flo
   const size_t need = tritt_decode_workspace(TRITT_OP_TDP_DECODE, c, dtype, k1_window, k2_window, flags);
   if (int rc = check_scratch(need, workspace, workspace_bytes)) return rc;
   TdpDecodeArgs a{cache_args(*c, status_word), *q, dtype, window(k1_window), window(k2_window), window(kk_left), window(kk_right), alpha * kLog2e, (float*)workspace, 0};
-  if (fast(TRITT_OP_TDP_DECODE, c->D, dtype, flags) && window_tdp_decode_applies(*c, a.k1w, a.k2w, a.kkl, a.kkr))
+  if (fast(TRITT_OP_TDP_DECODE, c->D, dtype, flags) && window_tdp_decode_applies(*c, dtype, a.k1w, a.k2w, a.kkl, a.kkr))
     return window_tdp_decode(a, o, lse, (cudaStream_t)stream);
   if (fast(TRITT_OP_TDP_DECODE, c->D, dtype, flags)) return sm100_tdp_decode(a, workspace, o, lse, (cudaStream_t)stream);
   JoinArgs j{a.cache, a.part, 0, dtype, o, lse, {}};

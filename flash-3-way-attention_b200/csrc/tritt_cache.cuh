@@ -330,7 +330,7 @@ size_t sm100_tdp_decode_workspace(const tritt_cache_t& c);
 int sm100_tdp_decode(const TdpDecodeArgs& a, void* workspace, void* o, float* lse, cudaStream_t stream);
 
 // ... with all of the windows in shared memory, where they fit (the same types; one kernel, no workspace)
-bool window_tdp_decode_applies(const tritt_cache_t& c, int k1w, int k2w, int kkl, int kkr);
+bool window_tdp_decode_applies(const tritt_cache_t& c, int dtype, int k1w, int k2w, int kkl, int kkr);
 int window_tdp_decode(const TdpDecodeArgs& a, void* o, float* lse, cudaStream_t stream);
 // ... the soft-max attention with warp-level matrix instructions (the same)
 bool mma_dps_decode_supported(int D, int dtype);

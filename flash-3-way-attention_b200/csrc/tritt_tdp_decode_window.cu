@@ -471,22 +471,41 @@ size_t smem_of(const WindowParams& p, int D) {
   return (size_t)(p.cols + p.rows) * (4 * D + 2) + (size_t)p.tokens * (2 * D + 12 + 64) + 4 + (size_t)p.cols / 4 + (size_t)p.tokens * p.tiles * (D + 2) * 4 + 16;
 }
 
-// What a call's blocks stage, and how many new tokens each takes: as few as fill the chip, for the more, the more read a row once.  False: too much.
-//
-// Of two kernels for D=64 this one is the faster up to about 28 thousand cells (rows by columns) a new token, the one with tcgen05 tiles beyond.
-// Without a band, windows of 128: 17 us (4 sequences of 8 heads, one token), 40 (32 of 16), 76 (8 of 16, 16 tokens) against 20, 60, 115; of 200: 23,
-// 81, 163 against 21, 58, 143; with a band of 65, windows of 200: 17, 60, 105 against 21, 62, 150; of 300: 23, 82, 263 against 25, 103, 262.
-// At D=128 shared memory ends at windows of about 128, where they are as fast (25, 93, 141 against 23, 86, 158; with the band 21, 73, 108 against 23,
-// 70, 158).
-constexpr long long kMostCells64 = 28000;
-bool plan(const tritt_cache_t& c, int k1w, int k2w, int kkl, int kkr, WindowParams& p) {
+// Of the two kernels this one is the faster up to so many cells (rows by columns) a new token; beyond, the one with tcgen05 tiles.  That one's time goes by
+// slabs of 128 columns: at D=128, windows of 100, it takes half of what those of 128 do, so the border lies lower where one slab holds all columns, but
+// for calls that leave most SMs idle.  us, this kernel / that one, int8 codes; windows (band) of
+//                       one token, 4 x 8      one token, 32 x 16    trees of 16, 8 x 16   trees of 4, 2 x 16
+//   D=64  bf16  128     19 / 20               41 / 60               79 / 122              25 / 25
+//               160     21 / 20               49 / 60               137 / 143             27 / 25
+//               200     23 / 21               86 / 59               176 / 148             35 / 27
+//               300 (65) 23 / 25              85 / 110              -                     25 / 35
+//   D=64  fp16  128     21 / 21               47 / 60               94 / 122              27 / 25
+//               160     23 / 21               55 / 60               172 / 144             33 / 26
+//               300 (65) 25 / 25              93 / 109              -                     28 / 35
+//   D=128 bf16  80      14 / 21               50 / 49               73 / 82               23 / 25
+//               100     17 / 21               58 / 47               93 / 94               27 / 25
+//               128     25 / 25               90 / 95               133 / 188             31 / 35
+//               160     27 / 25               105 / 93              -                     -
+//   D=128 fp16  80      14 / 21               53 / 49               82 / 82               25 / 25
+//               100     17 / 21               62 / 47               109 / 93              31 / 25
+//               128     27 / 25               99 / 96               159 / 189             35 / 35
+//               160     31 / 25               115 / 93              -                     -
+// (fp16 queries cost more here: A in two parts.)
+long long most_cells(const tritt_cache_t& c, int dtype, long long columns) {
+  if (c.D == 64) return dtype == TRITT_F16 ? 25000 : 28000;
+  return columns <= 128 && (long long)c.B * c.N * c.n > num_sms() / 2 ? 7000 : 25000;
+}
+// What a call's blocks stage, and how many new tokens each takes: as few as fill the chip, for the more, the more read a row once.  False: not a call
+// for this kernel, or too much for shared memory.
+bool plan(const tritt_cache_t& c, int dtype, int k1w, int k2w, int kkl, int kkr, WindowParams& p) {
   const long long tokens = (long long)c.page_size * c.table_pages + c.n;   // a sequence's most
   const long long rows = tokens < (long long)k2w + 1 ? tokens : (long long)k2w + 1;
   if (rows > 1024) return false;
   const long long band = (long long)kkl + kkr + 16;   // of a unit's 16 rows
   long long seen = tokens < (long long)k1w + 1 ? tokens : (long long)k1w + 1;
   if (band < seen) seen = band;
-  if (c.D == 64 && rows * seen > kMostCells64) return false;
+  const long long old = (long long)c.page_size * c.table_pages;
+  if (rows * seen > most_cells(c, dtype, (old < k1w ? old : k1w) + c.n)) return false;
   p.tiles = (int)(rows + 15) / 16;
   const int pairs = c.B * c.N, most = kPartBytes / (p.tiles * (c.D + 2) * 4);
   // one wave of two blocks an SM where there are not more sequences and heads (a second one of a third as many costs as much as the
@@ -529,9 +548,9 @@ template <typename T16, int D> int by_code(const WindowParams& p, cudaStream_t s
 
 }  // namespace
 
-bool window_tdp_decode_applies(const tritt_cache_t& c, int k1w, int k2w, int kkl, int kkr) {
+bool window_tdp_decode_applies(const tritt_cache_t& c, int dtype, int k1w, int k2w, int kkl, int kkr) {
   WindowParams p{};
-  return plan(c, k1w, k2w, kkl, kkr, p);
+  return plan(c, dtype, k1w, k2w, kkl, kkr, p);
 }
 
 int window_tdp_decode(const TdpDecodeArgs& a, void* o, float* lse, cudaStream_t stream) {
@@ -539,7 +558,7 @@ int window_tdp_decode(const TdpDecodeArgs& a, void* o, float* lse, cudaStream_t 
   p.a = a;
   p.o = o;
   p.lse = lse;
-  plan(a.cache.c, a.k1w, a.k2w, a.kkl, a.kkr, p);
+  plan(a.cache.c, a.dtype, a.k1w, a.k2w, a.kkl, a.kkr, p);
   if (a.dtype == TRITT_F16) return a.cache.c.D == 64 ? by_code<__half, 64>(p, stream) : by_code<__half, 128>(p, stream);
   return a.cache.c.D == 64 ? by_code<__nv_bfloat16, 64>(p, stream) : by_code<__nv_bfloat16, 128>(p, stream);
 }

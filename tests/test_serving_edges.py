@@ -301,3 +301,17 @@ def test_the_workspace_of_very_many_heads_is_counted():
     a = _norm_args(N=2 ** 31 - 1)
     a.w[0] = a.dw[0] = P
     assert lib.tritt_qk_norm_rotary_workspace(C.byref(a)) >= 3 * (2 ** 31 - 1) * 64 * 4
+
+
+# ---------------------------------------------------------------- which kernel
+
+@pytest.mark.parametrize("B,N,n,D,dtype,window,windows_kernel", [
+    (32, 16, 1, 128, _native.BF16, 100, False), (8, 16, 16, 128, _native.F16, 100, False), (4, 8, 1, 128, _native.F16, 100, True),
+    (32, 16, 1, 128, _native.F16, 64, True), (8, 16, 16, 128, _native.BF16, 128, True), (32, 16, 1, 128, _native.BF16, 160, False),
+    (32, 16, 1, 64, _native.BF16, 160, True), (8, 16, 16, 64, _native.F16, 160, False), (8, 16, 16, 64, _native.F16, 128, True),
+    (4, 8, 1, 64, _native.BF16, 200, False)])
+def test_the_kernel_that_was_measured_to_be_faster_is_taken(B, N, n, D, dtype, window, windows_kernel):
+    lib, C = _native.lib(), _native.C
+    c = C.byref(_native.Cache(codes=P, exponents=P, pages=2, page_size=16, N=N, D=D, code=2, table=P, table_stride=256, table_pages=256, context=P, B=B, n=n))
+    # (the kernel of windows needs no workspace)
+    assert (lib.tritt_decode_workspace(_native.OP_TDP_DECODE, c, dtype, window, window, 0) == 0) == windows_kernel
