@@ -47,17 +47,18 @@ __device__ __forceinline__ size_t lse_of(const CacheArgs& a, Place at, int head)
   return (((size_t)at.page * a.c.N + head) << a.page_log2) + at.row;
 }
 
-// Tokens of sequence b before the new ones, at most what its table has places for (more is an error, and bounds every loop over them).
-__device__ __forceinline__ int context_of(const CacheArgs& a, int b) {
-  const int c = __ldg(a.c.context + b), most = a.c.table_pages << a.page_log2;
-  if (c > most && a.status) atomicOr(a.status, kStatusPlace);
-  return c < most ? c : most;
-}
 // New tokens that sequence b has in this call.
 __device__ __forceinline__ int new_tokens(const CacheArgs& a, int b) {
   if (__ldg(a.c.context + b) < 0) return 0;
   const int n = a.c.counts ? __ldg(a.c.counts + b) : a.c.n;
   return n < 0 ? 0 : n > a.c.n ? a.c.n : n;
+}
+// Tokens of sequence b before the new ones, at most what its table has places for (more is an error of a sequence that
+// has new ones, and the bound is one of every loop over them).
+__device__ __forceinline__ int context_of(const CacheArgs& a, int b) {
+  const int c = __ldg(a.c.context + b), most = a.c.table_pages << a.page_log2;
+  if (c > most && a.status && new_tokens(a, b) > 0) atomicOr(a.status, kStatusPlace);
+  return c < most ? c : most;
 }
 
 // Bit m: new token i attends to new token m (only with ancestors).

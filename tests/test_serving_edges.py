@@ -45,6 +45,29 @@ def test_a_sequence_of_more_groups_than_can_be_numbered_is_reported():
     assert not bool(out[empty].any()) and bool((lse[empty] == -math.inf).all())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("precision", ["ieee", None])
+def test_a_sequence_without_new_tokens_may_have_any_context(precision):
+    bt = Batch(3, 2, 4, 64, "bf16", "e4m3", 16, [30, 17, 21], dps=True, seed=8)
+    q = bt.q.to(DEV)
+    counts = torch.tensor([4, 0, -3], dtype=torch.int32, device=DEV)
+    table = torch.cat([bt.table, torch.full((3, 300), -1, dtype=torch.int32, device=DEV)], 1)   # (and the kernels of long tables)
+
+    def calls(context, table):
+        out = [ft.tdp_decode(q, bt.cache, table, context, 0.1, counts=counts, input_precision=precision)]
+        ft.cache_write(bt.cache, table, context, q, q, q, q, counts=counts)
+        ft.dps_append(bt.cache, table, context, q, q, q, q, 0.1, 20, counts=counts, input_precision=precision)
+        out += ft.dps_decode(q, bt.cache, table, context, 0.1, counts=counts, input_precision=precision)
+        out += ft.cache_read(bt.cache, table, context, 4, torch.float32, counts=counts)
+        ft.check_status(DEV)
+        return [t.clone() for t in out]
+
+    for t in (bt.table, table):
+        want = calls(bt.context, t)
+        again = calls(torch.tensor([30, 1 << 20, 2 ** 31 - 1], dtype=torch.int32, device=DEV), t)
+        assert all(torch.equal(a, b) for a, b in zip(want[1:], again[1:])) and torch.equal(want[0][1:], again[0][1:])
+
+
 # ---------------------------------------------------------------- derivatives that there are not
 
 def _norm_on_cpu(monkeypatch):
