@@ -270,6 +270,15 @@ int check_out(const void* p, const float* lse) {
   return check_lse(lse);
 }
 
+// (a scale that is not a number would come out of the kernels' maxima as one next to 0)
+int check_scale(float alpha) {
+  if (alpha - alpha != 0.f) {
+    set_error("the soft-max scale must be finite, got %f", alpha);
+    return -10;
+  }
+  return 0;
+}
+
 bool fast(int op, int D, int dtype, int flags) {
   if (flags & TRITT_FLAG_FORCE_SIMT) return false;
   return op == TRITT_OP_TDP_DECODE ? sm100_tdp_decode_supported(D, dtype) : mma_dps_decode_supported(D, dtype);
@@ -398,6 +407,7 @@ int tritt_tdp_decode(const tritt_cache_t* c, const tritt_rows_t* q, void* o, flo
   if (int rc = check_cache(c)) return rc;
   if (int rc = check_rows(q, 1, dtype)) return rc;
   if (int rc = check_out(o, lse)) return rc;
+  if (int rc = check_scale(alpha)) return rc;
   if (k1_window < 0 || k2_window < 0 || kk_left < 0 || kk_right < 0) {
     set_error("window arguments must be >= 0 (got %d, %d, %d, %d)", k1_window, k2_window, kk_left, kk_right);
     return -10;
@@ -422,6 +432,7 @@ int tritt_dps_append(const tritt_cache_t* c, const tritt_rows_t* rows, int dtype
     set_error("the cache has no log-sum-exps: it is not one of the dot-product-sum form");
     return -16;
   }
+  if (int rc = check_scale(alpha)) return rc;
   if (k_diff < 0) {
     set_error("k_diff must be >= 0, got %d", k_diff);
     return -10;
@@ -443,6 +454,7 @@ int tritt_dps_decode(const tritt_cache_t* c, const tritt_rows_t* q, void* o, flo
   if (int rc = check_cache(c)) return rc;
   if (int rc = check_rows(q, 1, dtype)) return rc;
   if (int rc = check_out(o, m)) return rc;
+  if (int rc = check_scale(alpha)) return rc;
   if (!c->lse) {
     set_error("the cache has no log-sum-exps: it is not one of the dot-product-sum form");
     return -16;

@@ -270,14 +270,14 @@ P = 1 << 20
 
 def _cache_calls(**kw):
     lib, C = _native.lib(), _native.C
-    out, m = kw.pop("out", P), kw.pop("m", P)
+    out, m, alpha = kw.pop("out", P), kw.pop("m", P), kw.pop("alpha", 0.1)
     c = C.byref(_native.Cache(**{**dict(codes=P, exponents=P, lse=P, pages=2, page_size=16, N=2, D=64, code=1, table=P, table_stride=2, table_pages=2,
                                         context=P, B=1, n=1), **kw}))
     rows, parts = (_native.Rows * 4)(*(_native.Rows(P, 64, 64, 64) for _ in range(4))), (C.c_void_p * 4)(P, P, P, P)
     return dict(write=lambda: lib.tritt_cache_write(c, rows, 1, None, None), read=lambda: lib.tritt_cache_read(c, parts, m, 1, None, None),
-                tdp=lambda: lib.tritt_tdp_decode(c, rows, out, m, 1, 0.1, 1, 1, 1, 1, P, 1 << 40, None, 0, None),
-                append=lambda: lib.tritt_dps_append(c, rows, 1, 0.1, 1, P, 1 << 40, None, 0, None),
-                dps=lambda: lib.tritt_dps_decode(c, rows, out, m, 1, 0.1, P, 1 << 40, None, 0, None))
+                tdp=lambda: lib.tritt_tdp_decode(c, rows, out, m, 1, alpha, 1, 1, 1, 1, P, 1 << 40, None, 0, None),
+                append=lambda: lib.tritt_dps_append(c, rows, 1, alpha, 1, P, 1 << 40, None, 0, None),
+                dps=lambda: lib.tritt_dps_decode(c, rows, out, m, 1, alpha, P, 1 << 40, None, 0, None))
 
 
 # (every call below is refused before anything is launched: there is no GPU in it)
@@ -291,6 +291,12 @@ def test_the_caches_pointers_that_are_not_aligned_are_refused(field, off):
 def test_log_sum_exps_that_are_not_aligned_are_refused(off):
     calls = _cache_calls(m=P + off)
     assert [calls[name]() for name in ("read", "tdp", "dps")] == [-5] * 3
+
+
+@pytest.mark.parametrize("alpha", [math.nan, math.inf, -math.inf])
+def test_a_scale_that_is_not_finite_is_refused(alpha):
+    calls = _cache_calls(alpha=alpha)
+    assert [calls[name]() for name in ("tdp", "append", "dps")] == [-10] * 3
 
 
 def _norm_args(**kw):
