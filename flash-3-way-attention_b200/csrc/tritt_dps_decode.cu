@@ -4,7 +4,7 @@
 // Bound by HBM: a cached row is read once for up to 8 NT new tokens, 2 flops a byte and token.  Each warp has a ring of its own in
 // shared memory, filled by bulk copies (16 rows each, whole pages' neighbours) and 4-byte asynchronous ones (exponents, biases): no registers
 // wait for memory and nearly no instructions address it (a first form with loads to registers executed 1046 instructions for 32
-// tokens, more than HBM leaves time for: 253 us for a token of 32 sequences of up to 8191, 16 heads of 64, e4m3; now 85, 5 TB/s).  Rows then go, as fp16, into warp-level matrix
+// tokens, more than HBM leaves time for: 253 us for a token of 32 sequences of up to 8191, 16 heads of 64, e4m3; now 90, 4.8 TB/s).  Rows then go, as fp16, into warp-level matrix
 // instructions with the cached rows as the 16-row operand:
 //   S^T[16 tokens x 8 queries] = K Q^T,   O^T[D x 8 queries] += V^T P^T
 // (one token is an eighth of a tile instead of a sixteenth, and a query's statistics lie in the threads that hold its results).  The contraction of S
@@ -19,11 +19,11 @@
 // Codes are exact as fp16, the scores' powers of two are applied in fp32; P is formed times 2^(its row's exponent - the largest so far + 13),
 // so that values of any size meet in one accumulator, and its sum is taken before that.  Queries are brought to [1, 2) by a power of two.
 // Where rows are few or new tokens many, the way to the first tile and each piece's end count as much as the bytes: 24 tokens over 3001, 4 x 16
-// heads of 128, fp16: 37 us, of which a tile of 16 rows takes 2.5 thousand cycles (two warps a scheduler, a chain of two products and a soft-max)
+// heads of 128, fp16: 38 us, of which a tile of 16 rows takes 2.5 thousand cycles (two warps a scheduler, a chain of two products and a soft-max)
 // and a piece 10 (first rows, queries, joining of the warps).
 // A tile's rows may be hidden from some or all of its queries (another branch of a tree, before a window).  Where one could be so much larger than what
 // the queries attend to that their P would leave fp16's range (2^12), each query goes on with an exponent of its own, the largest of the rows
-// that it attends to.
+// that it attends to (looking for it costs 1 to 3 %).
 // Append forms P as the sum of two fp16 numbers (22 bits): its result is rounded again, to codes, and each element that a less exact one moves over
 // a border is off by a whole step (e4m3: 0.13 % of W's norm with one fp16 number, 2e-5 with two).
 #include "tritt_cache.cuh"

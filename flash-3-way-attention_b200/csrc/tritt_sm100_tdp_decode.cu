@@ -24,15 +24,16 @@
 //                 the loads of a tile are in flight before its stage is free.  They form tile b's A, and tell its rows' masks and scales
 //   warps 8-11    values in the same way, and tile a's A
 //   warps 12-19   one row a thread: maximum, exponentials, P; at the end of a piece the group's sum
-// Measured: 8 tokens over 2040, 16 heads of 128, float16 codes 345 us (products alone would take 166, exponentials 122); one token over up to
-// 700, 4 sequences of 8 heads of 64, e4m3 30 us.  Of the first a pair of tiles' slab took 5.1 thousand cycles at 374 us: 3.2 in a tile's soft-max (a
-// warp a scheduler works alone for most of it), 1.9 from its P to the next scores; the change of pieces 17 thousand a piece, the
+// Measured: 8 tokens over 2040, 16 heads of 128, float16 codes 356 us (products alone would take 166, exponentials 122; 346 before it looked at how far
+// exponents lie apart); one token over up to 700, 4 sequences of 8 heads of 64, e4m3 31 us.
+// Stamps of an earlier form, which took 374 us for the first: a pair of tiles' slab 5.1 thousand cycles, of them 3.2 in a tile's soft-max (a
+// warp a scheduler works alone for most of it) and 1.9 from its P to the next scores; the change of pieces 17 thousand a piece, the
 // group's sums 8 and the rows' A 13 of them, side by side.  Of the second 10 of the first 19 thousand cycles are the way to the first A.
-// Registers decide: with 32 rows of 256 bytes at a time the loading warps need more than 112 (104: 407 us, 112: 374, and the soft-max warps at 104:
-// 421); with 16 rows 96 do, and the soft-max warps take 120 (344 us; 88 / 136: 397).
+// Tried on forms of 344 to 374 us.  Registers: with 32 rows of 256 bytes at a time the loading warps need more than 112 (104: 407 us, 112: 374, and the soft-max
+// warps at 104: 421); with 16 rows 96 do, and the soft-max warps take 120 (344 us; 88 / 136: 397).
 // Keys and values from the same warps: 1.3 us a slab that nothing hid (690 us then).  A formed by the soft-max warps: 15 us a piece.  P in quarters
 // with the next quarter's scores on their way: 388 us instead of 345 (more votes).  A's codes on their way before the tile is free: 387 to 400, its
-// rows loaded side by side: 500 (registers of the warps that form it).
+// rows loaded side by side: 500 (registers of the warps that form it).  What follows a slab whose exponents lie apart inside the common code: 366.
 #include "tritt_cache.cuh"
 #include "tritt_sm100.cuh"
 #include "tritt_sm100_tdp.cuh"

@@ -6,9 +6,9 @@
 // rows k of one new token at a time (m16n8k16 products, A = alpha q*K2 formed in registers), walks the 32-column blocks j that any of them
 // attends to, and sums its rows times V2; the sums of a new token meet in shared memory, in order, and leave as the result: one launch.
 //
-// Bound by instruction issue (1780 a unit of 16 rows under a window of 129 and a band of 65: 56 % of the issue slots) and, for few rows, by the
+// Bound by instruction issue (2000 a unit of 16 rows under a window of 129 and a band of 65, staging included: 54 % of the issue slots) and, for few rows, by the
 // chain load, convert, product, exponential.  Trees of 16 under windows 128/128/32/32, 8 sequences of 16 heads, D=64, int8, fp16
-// queries: 66 us (58 with bfloat16's); the kernel with tcgen05 tiles of 128 x 128 cells, which such a window fills to a half: 120.
+// queries: 68 us (61 with bfloat16's); the kernel with tcgen05 tiles of 128 x 128 cells, which such a window fills to a half: 120.
 #include "tritt_cache.cuh"
 #include "tritt_sm100.cuh"
 #include "tritt_sm100_tdp.cuh"
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 2 : 1) tdp_decode_windo
     const float factor[2] = {large ? 1.f : fmaxf(scale[0], 1e-37f), large ? 1.f : fmaxf(scale[1], 1e-37f)};
     // A's fragments: elements 32 j + 8 t + 4 s + {0, 1 | 2, 3} of rows g, g + 8 in steps s = 0, 1.  For fp16 each as its upper 11 bits and what
     // they leave: under a narrow window a result has few terms whose errors could cancel.  (With the upper bits alone trees of 16 under a band of 65
-    // were off by 3.1e-4, 58 us; so by 2.3e-4, 66 us, where fp16's own rounding of the result is 2.1e-4; with P in two parts instead 2.9e-4, 68 us.
+    // were off by 3.1e-4, 58 us; so by 2.3e-4, 66 us then, where fp16's own rounding of the result is 2.1e-4; with P in two parts instead 2.9e-4, 68 us.
     // bfloat16 rounds results by 1.7e-3.)
     constexpr bool kRest = std::is_same<T16, __half>::value;
     uint32_t af[D / 16][4], al[kRest ? D / 16 : 1][4];

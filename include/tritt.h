@@ -316,7 +316,7 @@ int tritt_cache_read(const tritt_cache_t* c, void* const* parts, float* lse, int
  *   S[q,j,k] = alpha sum_h q[q,h] K1[j,h] K2[k,h], soft-max over the attended pairs, o = sum P SiLU(V1)[j] V2[k]
  * over pairs of attended tokens within the windows (distances of positions, as for tritt_tdp_fwd: q - j <= k1_window,
  * q - k <= k2_window, k - j <= kk_left, j - k <= kk_right).  o: [B, N, n, D] contiguous; lse [B, N, n] or null.
- * A token without an attended pair (i >= counts[b], context[b] < 0) gets o = 0, lse = -infinity.
+ * A token without an attended pair (i >= counts[b], context[b] < 0) gets o = 0, lse = -infinity.  alpha is finite, here and below.
  * On the tensor cores a sequence has at most 2^30 (new token, 32 rows k of its window) groups and 2^39 products of 256 x 128 cells a head; one that has
  * more sets status bit 1024 and gets no results (o = 0, lse = -infinity).
  */
@@ -338,8 +338,8 @@ int tritt_dps_decode(const tritt_cache_t* c, const tritt_rows_t* q, void* o, flo
    triple dot product as above (0 for the others).  0: none is needed, or the description is refused.  Calls that may run at the same time need
    scratch of their own. */
 size_t tritt_decode_workspace(int op, const tritt_cache_t* c, int dtype, int k1_window, int k2_window, int flags);
-/* Which kernel family such a call runs on (TRITT_PATH_SIMT or TRITT_PATH_TCGEN05; for the dot-product-sum the latter stands for warp-level
-   matrix instructions). */
+/* Which kernel family such a call runs on: TRITT_PATH_SIMT (fp32 arithmetic on the CUDA cores) or, for those with matrix instructions, TRITT_PATH_TCGEN05,
+   which also stands for warp-level ones here (the dot-product sum, and the triple product under windows that fit in shared memory). */
 int tritt_decode_path(int op, int D, int dtype, int flags);
 
 #ifdef __cplusplus
