@@ -68,7 +68,7 @@ template <int D> struct Cfg {
   static constexpr int kOffRun = kOffRows + 256 * 32;          // [8 warps][D] fp32
   static constexpr int kOffOwn = kOffRun + 8 * D * 4;              // [256] rows' own exponents of V1
   static constexpr int kOffMisc = kOffOwn + 1024;
-  static constexpr int kSmem = kOffMisc + 3072;
+  static constexpr int kSmem = kOffMisc + 2816;
   static constexpr int kTmemO = 256;                               // S_a | S_b | acc_a | acc_b
 };
 
@@ -115,7 +115,7 @@ struct Misc {
   uint32_t tmem_base;
   int abort_flag;
 };
-static_assert(sizeof(Misc) <= 3072, "shared memory of the barriers");
+static_assert(sizeof(Misc) <= 2816, "shared memory of the barriers");
 
 // What the line of steps has of one sequence.
 struct Line {
