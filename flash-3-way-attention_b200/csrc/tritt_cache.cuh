@@ -88,10 +88,10 @@ __device__ __forceinline__ float code_scale(int byte) {
   return byte == 255 ? __uint_as_float(0x7fffffffu) : __uint_as_float((uint32_t)byte << 23);
 }
 
-// Rows of a tile are brought to one exponent as fp16 numbers (the products' operands), which keeps all but 2^-14 of a row whose exponent is up to this
-// much below the largest one.  That largest row may be one that nobody attends to, so where exponents lie further apart each row keeps
+// Rows of a tile are brought to one exponent as fp16 numbers (the products' operands): exactly for 8-bit codes and for the elements of fp16 codes down
+// to 2^-14 of their row's largest one, as long as exponents lie no further apart than this.  The largest row may be one that nobody attends to, so beyond each row keeps
 // its own, and scores and P are multiplied by it column by column (slower, and rare: rows of zeros do not count).
-constexpr int kSpread = 24;
+template <int CODE> constexpr int kSpread = CODE == TRITT_CODE_F16 ? 14 : CODE == TRITT_CODE_E4M3 ? 20 : 24;
 // An exponent byte, where it counts towards the least one of several: rows of zeros or next to it, NaN and those that are not there do not.
 __device__ __forceinline__ int least_byte(int byte) { return byte > 1 ? byte : 255; }
 // From this on a score's factor (its sum of products may be 2^30) is multiplied in, and rounded, before the maximum is subtracted: as one multiplication and

@@ -13,7 +13,7 @@
 // Codes become fp16 operands: a slab's rows, whose exponents differ, are brought to the largest one's by multiplications by powers of
 // two.  K1's exponent joins the scale of the scores, for each 32 columns; V1's runs along with the
 // accumulator, which is multiplied where it grows.  A is rounded once to 11 bits, P (times 2^7, fp16's lower range) once.
-// Where exponents lie further apart than 2^24 (of 32 rows of K1, or of a piece's rows of V1), whoever attends to them, V1's rows keep their own from there to
+// Where exponents lie further apart than 2^14 to 2^24, by the codes (of 32 rows of K1, or of a piece's rows of V1), whoever attends to them, V1's rows keep their own from there to
 // the piece's end, and K1's those of the 32: the soft-max warps multiply scores by K1's before they use them, and P by V1's, relative to the largest one that the row
 // attends to.  (Below, the 8 tokens over 2040 with one row 2^40 larger, 20 tokens before the end: 870 us instead of 356.)
 //
@@ -84,7 +84,7 @@ struct __align__(16) Meta {   // of one slab, by the warp that loaded 32 of its 
 constexpr uint32_t kApart = 4096;
 __device__ __forceinline__ uint32_t span_of(int largest, int least) { return (uint32_t)largest << 16 | (uint32_t)(255 - least); }
 __device__ __forceinline__ uint32_t span_with(uint32_t a, uint4 b) { return __vmaxu2(__vmaxu2(__vmaxu2(a, b.x), b.y), __vmaxu2(b.z, b.w)); }
-__device__ __forceinline__ bool too_wide(uint32_t span) { return (span >> 16) + (span & 0xffffu) > 255u + kSpread; }
+__device__ __forceinline__ bool too_wide(uint32_t span, int spread) { return (span >> 16) + (span & 0xffffu) > 255u + spread; }
 
 // A row of a tile, by the thread that formed its A for the one that works on its scores.
 struct __align__(16) RowInfo {
@@ -327,7 +327,7 @@ template <int D, int CODE> struct TileLoader {   // a warp's 32 rows of one part
 // (Not inlined: rare, and registers are few.)  -> the row's reference, what its sum is multiplied by, what is added to it
 struct SlabApart {
   uint32_t tS, tO;
-  int chunks, wid, up;       // of 16 columns of the accumulator; columns; kUp
+  int chunks, wid, up, spread;   // of 16 columns of the accumulator; columns; kUp, kSpread
   uint32_t before, span;     // V1's exponents up to the slab before, and to this one
   bool later;                // (the accumulator holds something)
 };
@@ -338,11 +338,11 @@ __device__ __noinline__ float4 slab_apart(const Meta& m, SlabApart a, uint4 mask
     // (rounded, as the maximum was: not taken into the subtraction)
     return __fmul_rn(__uint_as_float(s), scale * (block < 0.f ? power_of_two(m.ek[c] - 127 - a.up) : block));
   };
-  const bool wide = too_wide(a.span);
+  const bool wide = too_wide(a.span, a.spread);
   const int common = (int)(a.before >> 16);   // V1's exponent so far
   // (0: nothing attended so far.  A common exponent may be of rows that this one does not attend to: then the least that all of them have)
   const int old = !wide ? common : m_used == -INFINITY ? 0 : *own;
-  int now = !wide ? (int)(a.span >> 16) : m_used == -INFINITY ? 0 : too_wide(a.before) ? *own : most(common - kSpread, 1);
+  int now = !wide ? (int)(a.span >> 16) : m_used == -INFINITY ? 0 : too_wide(a.before, a.spread) ? *own : most(common - a.spread, 1);
   float mx = -INFINITY;
 #pragma unroll 1
   for (int c0 = 0; c0 < 128 && c0 < a.wid; c0 += 16) {
@@ -772,7 +772,7 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
           if (ev == 255) ev = 0;
           const int ek_most = __reduce_max_sync(0xffffffffu, ek), ev_most = __reduce_max_sync(0xffffffffu, ev);
           const int ev_least = __reduce_min_sync(0xffffffffu, least_byte(ev));
-          const bool apart = __any_sync(0xffffffffu, least_byte(ek) < ek_most - kSpread);
+          const bool apart = __any_sync(0xffffffffu, least_byte(ek) < ek_most - kSpread<CODE>);
           alive = __all_sync(0xffffffffu, mbar_wait(&empty[st], ph ^ 1, abort_flag));
           if (!alive) break;
           Meta& m = ms.meta[mt];
@@ -794,7 +794,7 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
           if (!alive) break;
           const volatile Meta& m = ms.meta[mt];
           span = span_with(span, make_uint4(m.span[0], m.span[1], m.span[2], m.span[3]));
-          up = too_wide(span) ? kUp<CODE> : kUp<CODE> + ev - (int)(span >> 16);
+          up = too_wide(span, kSpread<CODE>) ? kUp<CODE> : kUp<CODE> + ev - (int)(span >> 16);
         }
         if (any) {
           tile.store(ring + st * C::kTile, w * 32, half_power(up), lane, 0);
@@ -883,7 +883,7 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
         const float f[4] = {fmaxf(r.scale * ks.x, 1e-37f), fmaxf(r.scale * ks.y, 1e-37f), fmaxf(r.scale * ks.z, 1e-37f), fmaxf(r.scale * ks.w, 1e-37f)};
         const uint32_t before = span;
         span = span_with(span, spans);
-        const bool wide = too_wide(span);   // rows keep their exponents, in this slab and those behind it
+        const bool wide = too_wide(span, kSpread<CODE>);   // rows keep their exponents, in this slab and those behind it
         const bool odd = __any_sync(0xffffffffu, wide || fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])) > kLargeFactor);
         alive = __all_sync(0xffffffffu, mbar_wait(&ms.s_ready[x], scount & 1, abort_flag));
         if (!alive) break;
@@ -904,7 +904,7 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_decode_kernel(const __grid_co
         float psum = 0.f;
         if (odd) {
           const uint4 attended = full ? make_uint4(~0u, ~0u, ~0u, ~0u) : make_uint4(mask[0], mask[1], mask[2], mask[3]);
-          const float4 v = slab_apart(m, SlabApart{tS, tO, D / 16, wid, kUp<CODE>, before, span, t > 0}, attended, r.scale, m_used, own);
+          const float4 v = slab_apart(m, SlabApart{tS, tO, D / 16, wid, kUp<CODE>, kSpread<CODE>, before, span, t > 0}, attended, r.scale, m_used, own);
           m_used = v.x;
           l_sum *= v.y;
           psum = v.z;

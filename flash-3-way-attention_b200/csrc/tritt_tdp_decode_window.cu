@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 2 : 1) tdp_decode_windo
   // K1 and V1 to the largest exponent of all staged rows, where they are near enough to each other (else, trees of 16 as above with one row 2^40 larger: 92 us,
   // not 68)
   const int ek1 = s_most[0], ev1 = s_most[1];
-  const bool wide_k = ek1 - s_least[0] > kSpread, wide_v = ev1 - s_least[1] > kSpread;
+  const bool wide_k = ek1 - s_least[0] > kSpread<CODE>, wide_v = ev1 - s_least[1] > kSpread<CODE>;
   {
     auto bring = [&](uint8_t* at, const uint8_t* exps, int most, bool wide) {
       for (int x = tid; x < nj * L; x += kWarps * 32) {

@@ -93,6 +93,28 @@ def test_tdp_tokens_outside_the_window_of_some(D, dtype, code, windows, by):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("by", [12, 16, 19, 21, 23, 25])
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("D,dtype,code", [(64, "fp16", "fp16"), (64, "fp16", "e4m3"), (128, "fp16", "int8"), (128, "bf16", "fp16")])
+def test_tdp_small_elements_beside_a_larger_row(D, dtype, code, wide, by):
+    """A later token of the chain is larger; the first one attends to itself alone, and gets its own values' product, each element as the type rounds it
+    (bfloat16: times a row's other half step)."""
+    bt = Batch(2, 2, 4, D, dtype, code, 16, [0, 0], seed=33)
+    for token in (2, 3):
+        _enlarge(bt, 0, token, range(4), by)
+    table = _widened(bt.table, 8192, 16) if wide else bt.table
+    out, lse, alpha = _tdp(bt, table, (None,) * 4)
+    for b in range(2):
+        for h in range(2):
+            want = bt.seq.values[b][V1, h, 0] * bt.seq.values[b][V2, h, 0]
+            err = (out[b, h, 0].double().cpu() - want).abs()
+            # (P of a single pair is a power of two; elements of fp16 codes below 2^-14 of their row's largest lose bits: 2^-25 of it)
+            top = bt.seq.values[b][V1, h, 0].abs().max() * bt.seq.values[b][V2, h, 0].abs()
+            least = 2.0 ** -25 if bt.dt == torch.float16 else 0.0
+            assert bool((err <= torch.finfo(bt.dt).eps / 2 * want.abs() * (1 + 2.0 ** -10) + least + 2.0 ** -24 * top).all()), (b, h, float(err.max()))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("by", [26, 60])
 @pytest.mark.parametrize("D,dtype,code,windows", [(64, "fp16", "e4m3", (128, 128, 16, 16)), (128, "bf16", "fp16", (96, 96, 16, 16)),
                                                   (64, "fp16", "fp16", (None, None, 16, 16)), (128, "fp16", "int8", (None, None, 8, 16))])
