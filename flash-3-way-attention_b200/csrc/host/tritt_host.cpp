@@ -48,6 +48,8 @@ struct Entries {   // (the addresses come from Python, which has loaded the libr
   decltype(&tritt_dps_append) dps_append;
   decltype(&tritt_dps_decode) dps_decode;
   decltype(&tritt_decode_workspace) decode_workspace;
+  decltype(&tritt_qk_norm_rotary_axes_fwd) norm_axes_fwd;
+  decltype(&tritt_qk_norm_rotary_axes_bwd) norm_axes_bwd;
 } lib{};
 volatile int* status_words[kDevices] = {};
 std::map<std::array<int, 12>, size_t> workspace_sizes;
@@ -320,8 +322,18 @@ int* status_of(int device) {   // null: Python reports, or makes the word
   return lib.norm_fwd && status_words[device] && *status_words[device] == 0 ? const_cast<int*>(status_words[device]) : nullptr;
 }
 
+// The number of axes and the axis of each pair, as 33 bytes; null: there is one axis.
+bool read_axes(PyObject* o, tritt_axes_t& axes) {
+  axes = {};
+  if (o == nullptr) return true;
+  if (!PyBytes_Check(o) || PyBytes_GET_SIZE(o) != 33) return false;
+  axes.count = (unsigned char)PyBytes_AS_STRING(o)[0];
+  std::memcpy(axes.of, PyBytes_AS_STRING(o) + 1, 32);
+  return axes.count >= 1 && axes.count <= TRITT_MAX_AXES;
+}
+
 // q, k1, k2, three weights, cos, sin, positions, eps, interleaved
-bool read_norm(PyObject* const* a, Shape& s, tritt_norm_rotary_t& n) {
+bool read_norm(PyObject* const* a, Shape& s, tritt_norm_rotary_t& n, tritt_axes_t& axes) {
   if (!strided_shape(a[0], s)) return false;
   n = {};
   for (int i = 0; i < 3; ++i)
@@ -352,15 +364,18 @@ bool read_norm(PyObject* const* a, Shape& s, tritt_norm_rotary_t& n) {
     if (a[8] != Py_None) {
       const at::Tensor* p = plain(a[8], s.device);
       if (!p || (p->scalar_type() != at::kLong && p->scalar_type() != at::kInt)) return false;
-      if (!(p->dim() == 1 && p->size(0) == s.T) && !(p->dim() == 2 && p->size(0) == s.B && p->size(1) == s.T)) return false;
+      const int64_t lead = axes.count ? 1 : 0, dims = p->dim() - lead;   // (axes come first)
+      if (lead && (p->dim() < 2 || p->size(0) < axes.count || p->size(0) > TRITT_MAX_AXES)) return false;
+      if (!(dims == 1 && p->size(lead) == s.T) && !(dims == 2 && p->size(lead) == s.B && p->size(lead + 1) == s.T)) return false;
       n.positions = p->data_ptr();
       n.positions64 = p->scalar_type() == at::kLong;
       n.position_stride_t = p->stride(p->dim() - 1);
-      n.position_stride_b = p->dim() == 2 ? p->stride(0) : 0;
-    } else if (s.T > n.table) {
+      n.position_stride_b = dims == 2 ? p->stride(lead) : 0;
+      if (lead) axes.position_stride = p->stride(0);
+    } else if (s.T > n.table || axes.count) {
       return false;
     }
-  } else if (a[7] != Py_None || a[8] != Py_None) {
+  } else if (a[7] != Py_None || a[8] != Py_None || axes.count) {
     return false;
   }
   if (!read_float(a[9], n.eps) || !PyBool_Check(a[10])) return false;
@@ -368,12 +383,13 @@ bool read_norm(PyObject* const* a, Shape& s, tritt_norm_rotary_t& n) {
   return true;
 }
 
-// norm_rotary(q, k1, k2, weights..., cos, sin, positions, eps, interleaved) -> the three results, the library's error code, or None
+// norm_rotary(q, k1, k2, weights..., cos, sin, positions, eps, interleaved[, axes]) -> the three results, the library's error code, or None
 PyObject* norm_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   Shape s;
   tritt_norm_rotary_t args;
-  if (n != 11 || !read_norm(a, s, args)) Py_RETURN_NONE;
+  tritt_axes_t axes;
+  if (n < 11 || n > 12 || !read_axes(n == 12 ? a[11] : nullptr, axes) || !read_norm(a, s, args, axes)) Py_RETURN_NONE;
   int* const status = status_of(s.device);
   if (!status) Py_RETURN_NONE;
   const at::Tensor& q = THPVariable_Unpack(a[0]);
@@ -385,20 +401,24 @@ PyObject* norm_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
       out[i] = at::empty({s.B, s.N, s.T, s.D}, q.options());
       if (!fresh(out[i]) || !read_rows(out[i], args.y[i])) rc = kNotPlain;
     }
-    if (rc == 0) rc = lib.norm_fwd(&args, status, c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)s.device).stream());
+    if (rc == 0) {
+      const auto stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)s.device).stream();
+      rc = axes.count ? lib.norm_axes_fwd(&args, &axes, status, stream) : lib.norm_fwd(&args, status, stream);
+    }
   }
   if (rc == kNotPlain) Py_RETURN_NONE;
   return rc != 0 ? PyLong_FromLong(rc) : wrap_all(out, 3);
   END_HANDLE_TH_ERRORS
 }
 
-// norm_rotary_backward(the same, three gradients, three truth values: gradients of the weights) -> six gradients (None where
+// norm_rotary_backward(the same, three gradients, three truth values: gradients of the weights[, axes]) -> six gradients (None where
 // not wanted), the library's error code, or None
 PyObject* norm_rotary_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   Shape s;
   tritt_norm_rotary_t args;
-  if (n != 17 || !read_norm(a, s, args)) Py_RETURN_NONE;
+  tritt_axes_t axes;
+  if (n < 17 || n > 18 || !read_axes(n == 18 ? a[17] : nullptr, axes) || !read_norm(a, s, args, axes)) Py_RETURN_NONE;
   for (int i = 0; i < 3; ++i)
     if (!PyBool_Check(a[14 + i]) || a[11 + i] == Py_None || !read_rows(a[11 + i], s, args.y[i])) Py_RETURN_NONE;
   int* const status = status_of(s.device);
@@ -423,7 +443,10 @@ PyObject* norm_rotary_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
         scratch = at::empty({(int64_t)bytes}, out[0].options().dtype(at::kByte));
         if (!(w = fresh(scratch))) rc = kNotPlain;
       }
-      if (rc == 0) rc = lib.norm_bwd(&args, w, bytes, status, c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)s.device).stream());
+      if (rc == 0) {
+        const auto stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)s.device).stream();
+        rc = axes.count ? lib.norm_axes_bwd(&args, &axes, w, bytes, status, stream) : lib.norm_bwd(&args, w, bytes, status, stream);
+      }
     }
   }
   if (rc == kNotPlain) Py_RETURN_NONE;

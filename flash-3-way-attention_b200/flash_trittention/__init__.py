@@ -16,6 +16,7 @@ _LAZY_ATTRS = {
     # norms and position rotation of q, k1, k2, in front of either attention
     "qk_norm_rotary": (".norm_rotary", "qk_norm_rotary"),
     "rotary_tables": (".norm_rotary", "rotary_tables"),
+    "rotary_axes": (".norm_rotary", "rotary_axes"),
     # serving: a paged cache of quantised rows, and attention of new tokens over it
     "TrittentionCache": (".cache", "TrittentionCache"),
     "new_cache": (".cache", "new_cache"),

@@ -34,6 +34,7 @@ SYMBOLS = (
     "tritt_dps_bwd", "tritt_dps_bwd_saved", "tritt_selftest_umma", "tritt_selftest_wait_expiry", "tritt_tdp_fwd_noalloc",
     "tritt_noalloc_scratch_bytes", "tritt_selftest_bwd_registers",
     "tritt_tdp_bwd_plan", "tritt_qk_norm_rotary_fwd", "tritt_qk_norm_rotary_bwd", "tritt_qk_norm_rotary_workspace",
+    "tritt_qk_norm_rotary_axes_fwd", "tritt_qk_norm_rotary_axes_bwd",
     "tritt_cache_write", "tritt_cache_read", "tritt_tdp_decode", "tritt_dps_append", "tritt_dps_decode", "tritt_decode_workspace",
     "tritt_decode_path",
 )
@@ -65,6 +66,12 @@ class NormRotary(C.Structure):
                 ("position_stride_t", C.c_longlong), ("positions64", C.c_int), ("table", C.c_int), ("rot", C.c_int),
                 ("interleaved", C.c_int), ("weight_heads", C.c_int), ("weight_dtype", C.c_int), ("B", C.c_int), ("N", C.c_int),
                 ("T", C.c_int), ("D", C.c_int), ("dtype", C.c_int), ("eps", C.c_float)]
+
+
+class Axes(C.Structure):
+    """``tritt_axes_t``."""
+
+    _fields_ = [("position_stride", C.c_longlong), ("count", C.c_int), ("of", C.c_ubyte * 32)]
 
 
 class Cache(C.Structure):
@@ -121,7 +128,7 @@ def _load_host(L):
     _host.init(*(C.cast(getattr(L, "tritt_" + name), C.c_void_p).value for name in (
         "tdp_fwd", "tdp_bwd", "dps_fwd", "dps_bwd", "dps_bwd_saved", "workspace_bytes_flags", "tdp_fwd_workspace", "qk_norm_rotary_fwd",
         "qk_norm_rotary_bwd", "qk_norm_rotary_workspace", "cache_write", "cache_read", "tdp_decode", "dps_append", "dps_decode",
-        "decode_workspace")))
+        "decode_workspace", "qk_norm_rotary_axes_fwd", "qk_norm_rotary_axes_bwd")))
     for device, address in _status_ptr.items():
         _host.set_status(device, address)
     host_forward, host_backward = _host.forward, _host.backward
@@ -184,6 +191,8 @@ def lib():
                 norm, cache, rows = C.POINTER(NormRotary), C.POINTER(Cache), C.POINTER(Rows)
                 L.tritt_qk_norm_rotary_fwd.argtypes = [norm, vp, vp]
                 L.tritt_qk_norm_rotary_bwd.argtypes = [norm, vp, sz, vp, vp]
+                L.tritt_qk_norm_rotary_axes_fwd.argtypes = [norm, C.POINTER(Axes), vp, vp]
+                L.tritt_qk_norm_rotary_axes_bwd.argtypes = [norm, C.POINTER(Axes), vp, sz, vp, vp]
                 L.tritt_qk_norm_rotary_workspace.argtypes = [norm]
                 L.tritt_qk_norm_rotary_workspace.restype = sz
                 L.tritt_cache_write.argtypes = [cache, rows, i, vp, vp]
@@ -194,7 +203,7 @@ def lib():
                 L.tritt_decode_workspace.argtypes = [i, cache] + [i] * 4
                 L.tritt_decode_workspace.restype = sz
                 L.tritt_decode_path.argtypes = [i] * 4
-                for name in ("qk_norm_rotary_fwd", "qk_norm_rotary_bwd", "cache_write", "cache_read", "tdp_decode", "dps_append", "dps_decode",
+                for name in ("qk_norm_rotary_fwd", "qk_norm_rotary_bwd", "qk_norm_rotary_axes_fwd", "qk_norm_rotary_axes_bwd", "cache_write", "cache_read", "tdp_decode", "dps_append", "dps_decode",
                              "decode_path"):
                     getattr(L, "tritt_" + name).restype = i
                 _load_host(L)
@@ -504,7 +513,7 @@ def tdp_fwd_noalloc(q, k1, k2, v1, v2, o, lse, alpha, causal, k1w, k2w, kkl, kkr
     launches += 1
 
 
-def norm_rotary(a: NormRotary, dev: torch.device, backward: bool = False):
+def norm_rotary(a: NormRotary, dev: torch.device, backward: bool = False, axes: Axes | None = None):
     global launches
     check_status(dev, synchronize=False)
     L = lib()
@@ -512,9 +521,13 @@ def norm_rotary(a: NormRotary, dev: torch.device, backward: bool = False):
         if backward:
             n = int(L.tritt_qk_norm_rotary_workspace(C.byref(a)))
             ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-            rc = L.tritt_qk_norm_rotary_bwd(C.byref(a), 0 if ws is None else ws.data_ptr(), n, _status_address(dev), _stream(dev))
+            rest = (0 if ws is None else ws.data_ptr(), n, _status_address(dev), _stream(dev))
         else:
-            rc = L.tritt_qk_norm_rotary_fwd(C.byref(a), _status_address(dev), _stream(dev))
+            rest = (_status_address(dev), _stream(dev))
+        if axes is not None:
+            rc = (L.tritt_qk_norm_rotary_axes_bwd if backward else L.tritt_qk_norm_rotary_axes_fwd)(C.byref(a), C.byref(axes), *rest)
+        else:
+            rc = (L.tritt_qk_norm_rotary_bwd if backward else L.tritt_qk_norm_rotary_fwd)(C.byref(a), *rest)
     _check(rc, "tritt_qk_norm_rotary")
     launches += 1
 

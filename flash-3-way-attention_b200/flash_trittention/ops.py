@@ -23,7 +23,7 @@ its functions switch to these operators while they are compiled:
 Importing this module does not load the CUDA library; the operators do, on their first call, and raise if it is
 missing (there is no CPU implementation behind them).
 """
-from typing import List, Optional, Tuple
+from typing import List, Optional, Sequence, Tuple
 
 import torch
 import torch.nn as nn
@@ -189,29 +189,30 @@ def dps_attention(q, k1, k2, v1, v2, softmax_scale=1 / 8, causal=True, k_diff=10
 @torch.library.custom_op("flash_trittention::norm_rotary", mutates_args=(), device_types="cuda")
 def norm_rotary(q: Tensor, k1: Tensor, k2: Tensor, q_weight: Optional[Tensor], k1_weight: Optional[Tensor], k2_weight: Optional[Tensor],
                 cos: Optional[Tensor], sin: Optional[Tensor], positions: Optional[Tensor], eps: float,
-                interleaved: bool) -> Tuple[Tensor, Tensor, Tensor]:
+                interleaved: bool, axes: Optional[Sequence[int]] = None) -> Tuple[Tensor, Tensor, Tensor]:
     """The three results of ``qk_norm_rotary``."""
-    return _norm_rotary.norm_rotary_forward((q, k1, k2), (q_weight, k1_weight, k2_weight), cos, sin, positions, eps, interleaved)
+    return _norm_rotary.norm_rotary_forward((q, k1, k2), (q_weight, k1_weight, k2_weight), cos, sin, positions, eps, interleaved,
+                                            _norm_rotary._packed(axes, cos))
 
 
 @norm_rotary.register_fake
-def _(q, k1, k2, q_weight, k1_weight, k2_weight, cos, sin, positions, eps, interleaved):
-    _norm_rotary._check((q, k1, k2), (q_weight, k1_weight, k2_weight), cos, sin, positions)
+def _(q, k1, k2, q_weight, k1_weight, k2_weight, cos, sin, positions, eps, interleaved, axes=None):
+    _norm_rotary._check((q, k1, k2), (q_weight, k1_weight, k2_weight), cos, sin, positions, _norm_rotary._packed(axes, cos))
     return tuple(torch.empty(q.shape, dtype=q.dtype, device=q.device) for _ in range(3))
 
 
 @torch.library.custom_op("flash_trittention::norm_rotary_bwd", mutates_args=(), device_types="cuda")
 def norm_rotary_bwd(q: Tensor, k1: Tensor, k2: Tensor, q_weight: Optional[Tensor], k1_weight: Optional[Tensor], k2_weight: Optional[Tensor],
                     cos: Optional[Tensor], sin: Optional[Tensor], positions: Optional[Tensor], eps: float, interleaved: bool, d_q: Tensor,
-                    d_k1: Tensor, d_k2: Tensor, weights_too: List[bool]) -> List[Tensor]:
+                    d_k1: Tensor, d_k2: Tensor, weights_too: List[bool], axes: Optional[Sequence[int]] = None) -> List[Tensor]:
     """``[dq, dk1, dk2]`` and the gradients of the weights that are wanted, in order."""
     out = _norm_rotary.norm_rotary_backward((q, k1, k2), (q_weight, k1_weight, k2_weight), cos, sin, positions, eps, interleaved,
-                                            tuple(d.to(q.dtype) for d in (d_q, d_k1, d_k2)), tuple(weights_too))
+                                            tuple(d.to(q.dtype) for d in (d_q, d_k1, d_k2)), tuple(weights_too), _norm_rotary._packed(axes, cos))
     return [g for g in out if g is not None]
 
 
 @norm_rotary_bwd.register_fake
-def _(q, k1, k2, q_weight, k1_weight, k2_weight, cos, sin, positions, eps, interleaved, d_q, d_k1, d_k2, weights_too):
+def _(q, k1, k2, q_weight, k1_weight, k2_weight, cos, sin, positions, eps, interleaved, d_q, d_k1, d_k2, weights_too, axes=None):
     return [torch.empty_like(x) for x in (q, k1, k2)] + [
         torch.empty(w.shape, dtype=w.dtype, device=w.device) for w, want in zip((q_weight, k1_weight, k2_weight), weights_too)
         if w is not None and want]
@@ -219,14 +220,14 @@ def _(q, k1, k2, q_weight, k1_weight, k2_weight, cos, sin, positions, eps, inter
 
 def _norm_rotary_setup(ctx, inputs, output):
     ctx.save_for_backward(*inputs[:9])
-    ctx.rest = tuple(inputs[9:])
+    ctx.rest, ctx.axes = tuple(inputs[9:11]), inputs[11]
 
 
 def _norm_rotary_backward(ctx, *dys):
     wanted = [bool(w is not None and need) for w, need in zip(ctx.saved_tensors[3:6], ctx.needs_input_grad[3:6])]
-    out = norm_rotary_bwd(*ctx.saved_tensors, *ctx.rest, *dys, wanted)
+    out = norm_rotary_bwd(*ctx.saved_tensors, *ctx.rest, *dys, wanted, ctx.axes)
     weights = iter(out[3:])
-    return (*out[:3], *(next(weights) if w else None for w in wanted), None, None, None, None, None)
+    return (*out[:3], *(next(weights) if w else None for w in wanted), None, None, None, None, None, None)
 
 
 norm_rotary.register_autograd(_norm_rotary_backward, setup_context=_norm_rotary_setup)

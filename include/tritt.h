@@ -271,6 +271,19 @@ int tritt_qk_norm_rotary_bwd(const tritt_norm_rotary_t* a, void* workspace, size
                              tritt_stream_t stream);
 size_t tritt_qk_norm_rotary_workspace(const tritt_norm_rotary_t* a);
 
+/* The same with positions that have several axes (time, row and column of a video's tokens): rotated pair i takes its cosine and sine from the
+   position's row along axis `of`.  The position of element (b, t) along axis x stands at x*position_stride + b*position_stride_b + t*position_stride_t
+   of `positions`, which must not be null. */
+enum { TRITT_MAX_AXES = 4 };
+typedef struct {
+  long long position_stride;
+  int count;                  /* axes, 1 to TRITT_MAX_AXES */
+  unsigned char of[32];       /* of pair i: bits 2 (i % 4) and the next of byte i / 4 */
+} tritt_axes_t;
+int tritt_qk_norm_rotary_axes_fwd(const tritt_norm_rotary_t* a, const tritt_axes_t* axes, int* status_word, tritt_stream_t stream);
+int tritt_qk_norm_rotary_axes_bwd(const tritt_norm_rotary_t* a, const tritt_axes_t* axes, void* workspace, size_t workspace_bytes, int* status_word,
+                                  tritt_stream_t stream);
+
 /* What an element of a cache is held in. */
 enum { TRITT_CODE_F16 = 0, TRITT_CODE_E4M3 = 1, TRITT_CODE_INT8 = 2 };
 enum { TRITT_MAX_ANCESTORS = 64 };

@@ -11,17 +11,22 @@ CODES = {"fp16": torch.float16, "e4m3": torch.float8_e4m3fn, "int8": torch.int8}
 TOP = {"e4m3": 448.0, "int8": 127.0}
 
 
-def norm_rotary(x, w, cos, sin, positions, eps=1e-6, interleaved=False):
-    """fp64 result for one tensor [B, N, T, D] (differentiable)."""
+def norm_rotary(x, w, cos, sin, positions, eps=1e-6, interleaved=False, axes=None):
+    """fp64 result for one tensor [B, N, T, D] (differentiable).  axes: that of each pair, positions are then [axes, (B,) T]."""
     B, N, T, D = x.shape
     u = x / (x.pow(2).mean(-1, keepdim=True) + eps).sqrt()
     if w is not None:
         u = u * (w[None, :, None, :] if w.dim() == 2 else w)
     if cos is None:
         return u
-    at = torch.arange(T).expand(B, T) if positions is None else positions.long().expand(B, T)
-    at = at.clamp(0, cos.shape[0] - 1)
-    c, s, half = cos.double()[at][:, None], sin.double()[at][:, None], cos.shape[1]
+    half = cos.shape[1]
+    if axes is None:
+        at = torch.arange(T).expand(B, T) if positions is None else positions.long().expand(B, T)
+        at = at.clamp(0, cos.shape[0] - 1)
+        c, s = cos.double()[at][:, None], sin.double()[at][:, None]
+    else:
+        at = torch.stack([positions[a].long().expand(B, T) for a in axes], -1).clamp(0, cos.shape[0] - 1)   # [B, T, pairs]
+        c, s = (torch.stack([t.double()[at[..., i], i] for i in range(half)], -1)[:, None] for t in (cos, sin))
     first = slice(0, 2 * half, 2) if interleaved else slice(0, half)
     second = slice(1, 2 * half, 2) if interleaved else slice(half, 2 * half)
     a, b = u[..., first], u[..., second]
