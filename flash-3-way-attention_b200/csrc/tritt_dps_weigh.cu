@@ -1,0 +1,232 @@
+// The attention weight of cached tokens in the dot-product sum: what new tokens' queries give them through K2, and what the new tokens' own k2 give them through K1.
+//
+//   w[x] = decay w[x] + sum_i exp(alpha q_i.K2[x] + lse[x] - m_i) + sum_i [p_i - x <= k_diff] exp(alpha k2_i.K1[x] - lse[p_i]),   x <= p_i = context + i
+// The soft-maxes' sums are known (m, lse), so a cached row is read once, each token's sum has one owner, and nothing is joined.  Bound by the bytes of K1 and K2.
+//
+// A warp takes 16 tokens: their rows go from memory straight into the fragments of warp-level matrix instructions (eight new tokens the other side, in shared memory in the order of
+// the fragments), exact as fp16 codes; each row's exponent, and the new row's, multiply the sums.  fp32 rows are two fp16 numbers (22 bits), as the products are
+// summed in fp32 all the same.
+#include "tritt_weigh.cuh"
+
+#include <type_traits>
+
+namespace tritt {
+namespace {
+
+constexpr int kThreads = 256, kTokens = 128;   // of a block at a time
+constexpr int kSms = 148;
+
+struct Params {
+  CacheArgs cache;
+  tritt_weights_t w;
+  tritt_rows_t rows[2];   // q, k2
+  const float* m;
+  int k_diff, repeat;     // repeat: times that a block takes kTokens
+  int chunk;              // new tokens at a time (a multiple of 8)
+  float scale2;
+};
+
+struct __align__(16) Query {
+  float scale, minus;     // of its scores (log2 units); what is subtracted (natural units)
+  int last, pad;          // the last token that it attends to; -1: none
+};
+
+// Bytes of a chunk's fragments for each new token, and how many of them are taken at once.
+template <typename T, int D> constexpr int kBytesEach = 2 * D * 2 * (std::is_same<T, float>::value ? 2 : 1);
+template <typename T, int D> constexpr int kMostChunk = 32768 / kBytesEach<T, D> < 64 ? 32768 / kBytesEach<T, D> : 64;
+static_assert(kMostChunk<float, 256> == 16 && kMostChunk<__half, 64> == 64, "chunks are multiples of 8");
+
+template <typename T, int D, int CODE> __global__ void __launch_bounds__(kThreads) dps_weigh_kernel(const __grid_constant__ Params p) {
+  using Rows = RowFragments<D, CODE>;
+  constexpr bool kWide = std::is_same<T, float>::value;
+  constexpr int kSteps = Rows::kSteps, kHalves = kWide ? 2 : 1;
+  constexpr bool kBoth = Rows::kWords <= 16;   // rows of both parts on their way together
+  extern __shared__ __align__(16) uint2 frags[];   // [part][8 new tokens][hi, lo][step][lane]
+  __shared__ Query queries[2][64];
+  const CacheArgs& a = p.cache;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, c = lane % 4;
+  const int bh = blockIdx.y, b = bh / a.c.N, head = bh - b * a.c.N;
+  if (__ldg(a.c.context + b) < 0) return;
+  const int ctx = context_of(a, b), cnt = new_tokens(a, b), end = weighed_tokens(a, p.w, ctx + cnt);
+  const int first = blockIdx.x * p.repeat * kTokens;
+  const int behind = ctx - (p.k_diff < ctx ? p.k_diff : ctx);   // the first token that any new one's k2 attends to
+  const int chunks = (cnt + p.chunk - 1) / p.chunk;
+  const uint8_t* codes = (const uint8_t*)a.c.codes;
+  constexpr size_t kRow = D * Rows::kSize;
+
+  for (int r = 0; r < p.repeat && first + r * kTokens < end; ++r) {
+    const int x0 = first + r * kTokens + warp * 16;
+    Place at{-1, 0};
+    if (x0 < end) {
+      at = place_of(a, b, x0);   // (16 tokens lie in one page)
+      if (at.page < 0 && a.status) atomicOr(a.status, kStatusPlace);
+    }
+    const bool there = at.page >= 0, inner = there && x0 + 15 >= behind;
+    const size_t row_k2 = there ? row_of(a, at, kPartK2, head) : 0, row_k1 = there ? row_of(a, at, kPartK1, head) : 0;
+    const float* lse_row = a.c.lse + (there ? lse_of(a, at, head) : 0);
+    Rows rows[kBoth ? 2 : 1];
+    float scale[2][2], lse[2] = {0.f, 0.f};
+    if (there) {
+      rows[0].load(codes + row_k2 * kRow, lane);
+      if (kBoth && inner) rows[kBoth].load(codes + row_k1 * kRow, lane);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        scale[0][h] = code_scale(__ldg(a.c.exponents + row_k2 + g + 8 * h));
+        scale[1][h] = inner ? code_scale(__ldg(a.c.exponents + row_k1 + g + 8 * h)) : 0.f;
+        lse[h] = __ldg(lse_row + g + 8 * h);
+      }
+    }
+    const int mine = x0 + g + (c == 1 ? 8 : 0);   // the token whose weight this lane writes
+    float sum = 0.f;
+    if (c < 2 && mine < end && mine < ctx) sum = faded(p.w, b, head, mine);
+    float gain[2] = {0.f, 0.f};
+    for (int q0 = 0, chunk = 0; chunk < chunks; ++chunk, q0 += p.chunk) {
+      const int here = cnt - q0 < p.chunk ? cnt - q0 : p.chunk, tiles = (here + 7) / 8;
+      if (r == 0 || chunks > 1) {   // the new tokens' rows as fragments
+        if (r || chunk) __syncthreads();
+        for (int i = warp; i < 2 * tiles * 8; i += kThreads / 32) {
+          const int part = i >= tiles * 8, n = i - part * tiles * 8;
+          const bool on = n < here;
+          const T* row = (const T*)p.rows[part].p + (on ? rows_at(p.rows[part], b, head, q0 + n) : 0);
+          float4 f[D > 128 ? 2 : 1];
+          uint32_t top = 0;
+#pragma unroll
+          for (int k = 0; k < (D > 128 ? 2 : 1); ++k) {
+            f[k] = on && lane + 32 * k < D / 4 ? load4(row + (lane + 32 * k) * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+            top = max(top, largest4(f[k]));
+          }
+          const int field = (int)(largest_of_row<32>(top) >> 23);
+          const float up = to_operand(field);
+#pragma unroll
+          for (int k = 0; k < (D > 128 ? 2 : 1); ++k) {
+            const int col = (lane + 32 * k) * 4;
+            if (col >= D) continue;
+            float4 v = f[k];
+            v.x *= up, v.y *= up, v.z *= up, v.w *= up;
+            if (field == 255) v = make_float4(0.f, 0.f, 0.f, 0.f);
+            const auto slot = Rows::slot_of(col);
+            uint2* to = frags + ((size_t)((part * tiles + n / 8) * kHalves) * kSteps + slot.step) * 32 + n % 8 * 4 + slot.c;
+            const uint2 hi = make_uint2(pack_halves(v.x, v.y), pack_halves(v.z, v.w));
+            to[0] = hi;
+            if constexpr (kWide) to[kSteps * 32] = make_uint2(pack_rests(v.x, v.y, hi.x), pack_rests(v.z, v.w, hi.y));
+          }
+          if (lane == 0) {
+            Query q{p.scale2 * from_operand(field), 0.f, -1, 0};
+            if (on) {
+              q.last = ctx + q0 + n;
+              if (part == 0) {
+                q.minus = __ldg(p.m + (size_t)bh * a.c.n + q0 + n);
+              } else {
+                const Place own = place_of(a, b, ctx + q0 + n);
+                if (own.page >= 0)
+                  q.minus = __ldg(a.c.lse + lse_of(a, own, head));
+                else
+                  q.last = -1;
+              }
+              if (q.minus == -INFINITY) q.last = -1;
+            }
+            queries[part][n] = q;
+          }
+        }
+        __syncthreads();
+      }
+      if (!there) continue;
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {
+        if (part && !inner) break;
+        Rows& now = rows[kBoth ? part : 0];
+        if (!kBoth && (part || chunk)) now.load(codes + (part ? row_k1 : row_k2) * kRow, lane);
+        uint32_t frag[kSteps][4];
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) now.step(s, frag[s]);
+        for (int t = 0; t < tiles; ++t) {
+          float d[4] = {0.f, 0.f, 0.f, 0.f};
+          const uint2* from = frags + (size_t)((part * tiles + t) * kHalves) * kSteps * 32 + lane;
+#pragma unroll
+          for (int s = 0; s < kSteps; ++s) {
+            mma_16816(d, frag[s], from[s * 32]);
+            if constexpr (kWide) mma_16816(d, frag[s], from[(kSteps + s) * 32]);
+          }
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const Query q = queries[part][t * 8 + 2 * c + k];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int x = x0 + g + 8 * h;
+              const bool on = x <= q.last && (part == 0 || q.last - x <= p.k_diff);
+              const float less = part == 0 ? lse[h] - q.minus : -q.minus;
+              gain[h] += on ? exp2f(fmaf(d[2 * h + k] * scale[part][h], q.scale, less * kLog2e)) : 0.f;
+            }
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      gain[h] += __shfl_xor_sync(0xffffffffu, gain[h], 1);
+      gain[h] += __shfl_xor_sync(0xffffffffu, gain[h], 2);
+    }
+    if (c < 2 && mine < end) *weight_of(p.w, b, head, mine) = sum + (c ? gain[1] : gain[0]);
+  }
+}
+
+template <typename T, int D, int CODE> int launch(Params p, cudaStream_t stream) {
+  const tritt_cache_t& c = p.cache.c;
+  const int most = kMostChunk<T, D>, n8 = (c.n + 7) / 8 * 8;
+  p.chunk = n8 < most ? n8 : most;
+  const int bytes = p.chunk * kBytesEach<T, D>;
+  long long tokens = (long long)c.table_pages * c.page_size;
+  const int length = p.w.after_length < p.w.before_length ? p.w.after_length : p.w.before_length;
+  if (length < tokens) tokens = length;
+  const long long blocks = (tokens + kTokens - 1) / kTokens;
+  // the new rows are formed once a block: it takes several times kTokens where there are blocks enough for all SMs several times over
+  long long repeat = blocks * c.B * c.N / (kSms * 16);
+  p.repeat = (int)(repeat < 1 ? 1 : repeat > 8 ? 8 : repeat);
+  const dim3 grid((unsigned)((blocks + p.repeat - 1) / p.repeat), c.B * c.N);
+  dps_weigh_kernel<T, D, CODE><<<grid, kThreads, bytes, stream>>>(p);
+  count_launch();
+  TRITT_CUDA_OK(cudaGetLastError());
+  return 0;
+}
+
+template <typename T, int CODE> int by_size(const Params& p, cudaStream_t stream) {
+  switch (p.cache.c.D) {
+    case 16: return launch<T, 16, CODE>(p, stream);
+    case 32: return launch<T, 32, CODE>(p, stream);
+    case 64: return launch<T, 64, CODE>(p, stream);
+    case 128: return launch<T, 128, CODE>(p, stream);
+    default: return launch<T, 256, CODE>(p, stream);
+  }
+}
+template <typename T> int by_code(const Params& p, cudaStream_t stream) {
+  switch (p.cache.c.code) {
+    case TRITT_CODE_F16: return by_size<T, TRITT_CODE_F16>(p, stream);
+    case TRITT_CODE_E4M3: return by_size<T, TRITT_CODE_E4M3>(p, stream);
+    default: return by_size<T, TRITT_CODE_INT8>(p, stream);
+  }
+}
+
+}  // namespace
+}  // namespace tritt
+
+using namespace tritt;
+
+extern "C" int tritt_dps_weigh(const tritt_cache_t* c, const tritt_weights_t* w, const tritt_rows_t* q, const tritt_rows_t* k2, const float* m, int dtype,
+                               float alpha, int k_diff, int* status_word, tritt_stream_t stream) {
+  if (int rc = check_cache(c)) return rc;
+  if (int rc = check_weights(c, w)) return rc;
+  if (int rc = check_rows(q, 1, dtype)) return rc;
+  if (int rc = check_rows(k2, 1, dtype)) return rc;
+  if (int rc = check_weigh_scores(m, alpha)) return rc;
+  if (!c->lse) {
+    set_error("the cache has no log-sum-exps: it is not one of the dot-product-sum form");
+    return -16;
+  }
+  if (k_diff < 0) {
+    set_error("k_diff must be >= 0, got %d", k_diff);
+    return -10;
+  }
+  Params p{cache_args(*c, status_word), *w, {*q, *k2}, m, k_diff, 0, 0, alpha * kLog2e};
+  if (dtype == TRITT_F32) return by_code<float>(p, (cudaStream_t)stream);
+  return dtype == TRITT_F16 ? by_code<__half>(p, (cudaStream_t)stream) : by_code<__nv_bfloat16>(p, (cudaStream_t)stream);
+}

@@ -26,6 +26,10 @@ _LAZY_ATTRS = {
     "tdp_decode": (".cache", "tdp_decode"),
     "dps_append": (".cache", "dps_append"),
     "dps_decode": (".cache", "dps_decode"),
+    # ... and which of its tokens are kept: the attention weight that each has got, and eviction by it
+    "tdp_weigh": (".eviction", "tdp_weigh"),
+    "dps_weigh": (".eviction", "dps_weigh"),
+    "cache_evict": (".eviction", "cache_evict"),
     # raises if a kernel of an earlier call gave up on a bounded barrier wait (not in the reference)
     "check_status": ("._native", "check_status"),
 }

@@ -36,7 +36,7 @@ SYMBOLS = (
     "tritt_tdp_bwd_plan", "tritt_qk_norm_rotary_fwd", "tritt_qk_norm_rotary_bwd", "tritt_qk_norm_rotary_workspace",
     "tritt_qk_norm_rotary_axes_fwd", "tritt_qk_norm_rotary_axes_bwd",
     "tritt_cache_write", "tritt_cache_read", "tritt_tdp_decode", "tritt_dps_append", "tritt_dps_decode", "tritt_decode_workspace",
-    "tritt_decode_path",
+    "tritt_decode_path", "tritt_tdp_weigh", "tritt_tdp_weigh_workspace", "tritt_dps_weigh", "tritt_cache_evict",
 )
 
 _lib = None
@@ -81,6 +81,14 @@ class Cache(C.Structure):
                 ("N", C.c_int), ("D", C.c_int), ("code", C.c_int), ("table", C.c_void_p), ("table_stride", C.c_longlong),
                 ("table_pages", C.c_int), ("context", C.c_void_p), ("counts", C.c_void_p), ("ancestors", C.c_void_p), ("B", C.c_int),
                 ("n", C.c_int)]
+
+
+class Weights(C.Structure):
+    """``tritt_weights_t``."""
+
+    _fields_ = [("before", C.c_void_p), ("after", C.c_void_p), ("before_stride_b", C.c_longlong), ("before_stride_n", C.c_longlong),
+                ("after_stride_b", C.c_longlong), ("after_stride_n", C.c_longlong), ("before_length", C.c_int), ("after_length", C.c_int),
+                ("decay", C.c_float)]
 
 
 def host_forward(*args):
@@ -203,7 +211,13 @@ def lib():
                 L.tritt_decode_workspace.argtypes = [i, cache] + [i] * 4
                 L.tritt_decode_workspace.restype = sz
                 L.tritt_decode_path.argtypes = [i] * 4
-                for name in ("qk_norm_rotary_fwd", "qk_norm_rotary_bwd", "qk_norm_rotary_axes_fwd", "qk_norm_rotary_axes_bwd", "cache_write", "cache_read", "tdp_decode", "dps_append", "dps_decode",
+                weights = C.POINTER(Weights)
+                L.tritt_tdp_weigh.argtypes = [cache, weights, rows, vp, i, f] + [i] * 4 + [vp, sz, vp, vp]
+                L.tritt_tdp_weigh_workspace.argtypes = [cache, i, i]
+                L.tritt_tdp_weigh_workspace.restype = sz
+                L.tritt_dps_weigh.argtypes = [cache, weights, rows, rows, vp, i, f, i, vp, vp]
+                L.tritt_cache_evict.argtypes = [cache, weights, vp, C.c_longlong] + [i] * 4 + [vp] * 4
+                for name in ("tdp_weigh", "dps_weigh", "cache_evict", "qk_norm_rotary_fwd", "qk_norm_rotary_bwd", "qk_norm_rotary_axes_fwd", "qk_norm_rotary_axes_bwd", "cache_write", "cache_read", "tdp_decode", "dps_append", "dps_decode",
                              "decode_path"):
                     getattr(L, "tritt_" + name).restype = i
                 _load_host(L)
@@ -593,3 +607,38 @@ def dps_decode(c: Cache, q, o, m, alpha, flags=0):
 
 def decode_path(op, D, dtype, flags=0) -> int:
     return lib().tritt_decode_path(op, D, dtype, flags)
+
+
+def tdp_weigh(c: Cache, w: Weights, q, lse, alpha, k1w, k2w, kkl, kkr):
+    global launches
+    dev = q.device
+    check_status(dev, synchronize=False)
+    with _on_device(dev):
+        ws = torch.empty(max(int(lib().tritt_tdp_weigh_workspace(C.byref(c), k1w, k2w)), 256), dtype=torch.uint8, device=dev)
+        rc = lib().tritt_tdp_weigh(C.byref(c), C.byref(w), C.byref(rows(q)), lse.data_ptr(), dtype_code(q.dtype), alpha, k1w, k2w, kkl, kkr,
+                                   ws.data_ptr(), ws.numel(), _status_address(dev), _stream(dev))
+    _check(rc, "tritt_tdp_weigh")
+    launches += 1
+
+
+def dps_weigh(c: Cache, w: Weights, q, k2, m, alpha, k_diff):
+    global launches
+    dev = q.device
+    check_status(dev, synchronize=False)
+    with _on_device(dev):
+        rc = lib().tritt_dps_weigh(C.byref(c), C.byref(w), C.byref(rows(q)), C.byref(rows(k2)), m.data_ptr(), dtype_code(q.dtype), alpha, k_diff,
+                                   _status_address(dev), _stream(dev))
+    _check(rc, "tritt_dps_weigh")
+    launches += 1
+
+
+def cache_evict(c: Cache, w: Weights, table_out, keep, first, recent, context_out, kept):
+    global launches
+    dev = kept.device
+    check_status(dev, synchronize=False)
+    where = (0, 0, 0) if table_out is None else (table_out.data_ptr(), table_out.stride(0), table_out.shape[1])
+    with _on_device(dev):
+        rc = lib().tritt_cache_evict(C.byref(c), C.byref(w), *where, keep, first, recent, context_out.data_ptr(), kept.data_ptr(), _status_address(dev),
+                                     _stream(dev))
+    _check(rc, "tritt_cache_evict")
+    launches += 1

@@ -31,6 +31,7 @@ from torch import Tensor
 
 from . import _native
 from . import cache as _cache
+from . import eviction as _eviction
 from . import norm_rotary as _norm_rotary
 
 __all__ = ["tdp_fwd", "tdp_bwd", "dps_fwd", "dps_bwd", "tdp_attention", "dps_attention", "TrittentionTDP", "norm_rotary", "norm_rotary_bwd",
@@ -299,6 +300,46 @@ def dps_decode(q: Tensor, codes: Tensor, exponents: Tensor, lse: Tensor, table: 
 @dps_decode.register_fake
 def _(q, codes, exponents, lse, table, context, softmax_scale, counts, ancestors, input_precision):
     return _like_queries(q)
+
+
+# ------------------------------------------------------------------ weights of cached tokens, and eviction
+# (`weights` None: those of before stand where the new ones go)
+
+@torch.library.custom_op("flash_trittention::tdp_weigh", mutates_args=("out",), device_types="cuda")
+def tdp_weigh(out: Tensor, weights: Optional[Tensor], q: Tensor, lse: Tensor, codes: Tensor, exponents: Tensor, table: Tensor, context: Tensor, softmax_scale: float,
+              k1_window: Optional[int], k2_window: Optional[int], kk_left: Optional[int], kk_right: Optional[int], counts: Optional[Tensor], decay: float) -> None:
+    _eviction.tdp_weigh(out if weights is None else weights, q, lse, _cache.TrittentionCache(codes, exponents), table, context, softmax_scale, k1_window, k2_window, kk_left,
+                        kk_right, counts, decay, out)
+
+
+@tdp_weigh.register_fake
+def _(out, weights, q, lse, codes, exponents, table, context, softmax_scale, k1_window, k2_window, kk_left, kk_right, counts, decay):
+    return None
+
+
+@torch.library.custom_op("flash_trittention::dps_weigh", mutates_args=("out",), device_types="cuda")
+def dps_weigh(out: Tensor, weights: Optional[Tensor], q: Tensor, k2: Tensor, m: Tensor, codes: Tensor, exponents: Tensor, lse: Tensor, table: Tensor, context: Tensor,
+              softmax_scale: float, k_diff: int, counts: Optional[Tensor], decay: float) -> None:
+    _eviction.dps_weigh(out if weights is None else weights, q, k2, m, _cache.TrittentionCache(codes, exponents, lse), table, context, softmax_scale, k_diff, counts, decay, out)
+
+
+@dps_weigh.register_fake
+def _(out, weights, q, k2, m, codes, exponents, lse, table, context, softmax_scale, k_diff, counts, decay):
+    return None
+
+
+@torch.library.custom_op("flash_trittention::cache_evict", mutates_args=("codes", "exponents", "lse", "weights_out"), device_types="cuda")
+def cache_evict(codes: Tensor, exponents: Tensor, lse: Optional[Tensor], weights_out: Tensor, weights: Optional[Tensor], table: Tensor, context: Tensor, keep: int,
+                first: int, recent: int, table_out: Optional[Tensor]) -> Tuple[Tensor, Tensor]:
+    """``(context, kept)``."""
+    return _eviction.cache_evict(weights_out if weights is None else weights, _cache.TrittentionCache(codes, exponents, lse), table, context, keep, first, recent, table_out,
+                                 weights_out)
+
+
+@cache_evict.register_fake
+def _(codes, exponents, lse, weights_out, weights, table, context, keep, first, recent, table_out):
+    B, N = table.shape[0], codes.shape[2]
+    return torch.empty(B, dtype=torch.int32, device=codes.device), torch.empty(B, N, keep, dtype=torch.int32, device=codes.device)
 
 
 # ------------------------------------------------------------------ module

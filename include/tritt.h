@@ -355,6 +355,52 @@ size_t tritt_decode_workspace(int op, const tritt_cache_t* c, int dtype, int k1_
    which also stands for warp-level ones here (the dot-product sum, and the triple product under windows that fit in shared memory). */
 int tritt_decode_path(int op, int D, int dtype, int flags);
 
+/* ------------------------------------------------------------------------------------------------------------------------
+ * Which tokens of a cache are worth keeping: the attention weight that each has got, and a cache with the heaviest ones alone.
+ */
+
+/* Weights of tokens, fp32: that of token x of sequence b and head n at before + b*before_stride_b + n*before_stride_n + x, x < before_length; the
+   new ones at `after` in the same way (the same place as `before`, or another).  The weigh calls write, of every sequence with context[b] >= 0,
+     after[x] = (x < context[b] ? decay * before[x] : 0) + what the call's new tokens add,   x < context[b] + (its new tokens)
+   and nothing else (decay 0 does not read `before`).  A token beyond either length sets status bit 512 and is left out.  decay is finite, >= 0. */
+typedef struct {
+  const float* before;
+  float* after;
+  long long before_stride_b, before_stride_n, after_stride_b, after_stride_n;
+  int before_length, after_length;
+  float decay;
+} tritt_weights_t;
+
+/*
+ * Triple dot product: each new token i adds sum_k P_i[x,k] + sum_j P_i[j,x] to token x, with P_i[j,k] = exp(S_i[j,k] - lse_i) over the pairs that it attends to
+ * (tritt_tdp_decode; 2 in all for each token and head).  lse: [B, N, n], as tritt_tdp_decode has written it; a token whose lse is -infinity adds nothing.
+ * No ancestors: drafts are weighed once they are accepted.  Sums are formed in a fixed order, a call repeats itself bit for bit.
+ */
+int tritt_tdp_weigh(const tritt_cache_t* c, const tritt_weights_t* w, const tritt_rows_t* q, const float* lse, int dtype, float alpha, int k1_window,
+                    int k2_window, int kk_left, int kk_right, void* workspace, size_t workspace_bytes, int* status_word, tritt_stream_t stream);
+/* Bytes of scratch for it: 12 bytes for each token within the windows, for each head and each SM.  Calls that may run at the same time need scratch of their own. */
+size_t tritt_tdp_weigh_workspace(const tritt_cache_t* c, int k1_window, int k2_window);
+/*
+ * Dot-product sum: each new token i adds exp(alpha q_i.K2[x] + lse[x] - m_i) to the tokens x that its query attends to (tritt_dps_decode), and
+ * exp(alpha k2_i.K1[x] - lse[i]) to those that its k2 attends to (tritt_dps_append, whose k_diff).  k2: the unrounded rows; m: [B, N, n].  An m or lse that is
+ * -infinity adds nothing.  No ancestors.
+ */
+int tritt_dps_weigh(const tritt_cache_t* c, const tritt_weights_t* w, const tritt_rows_t* q, const tritt_rows_t* k2, const float* m, int dtype, float alpha,
+                    int k_diff, int* status_word, tritt_stream_t stream);
+
+/*
+ * Keeps `keep` tokens of each sequence and head (of c->context tokens; c->n and c->counts are not looked at): the `first` first, the `recent` last, and of the others those with
+ * the largest w->before (ties: the lower number; NaN counts as the largest), first + recent <= keep.  Their rows and log-sum-exps move to the places of tokens 0, 1, 2, ...
+ * in order, and their weights to w->after; kept [B, N, keep] gets their numbers, -1 behind the last, context_out [B] the tokens that are left.  A sequence that has no more than
+ * `keep` tokens keeps all of them; context[b] < 0 stays as it is.
+ * table_out null: in place (the places behind the last kept token keep what they hold).  Else the rows go to the pages of table_out, [B, table_out_pages] with stride
+ * table_out_stride, of which none may be one that the call reads, and the old ones stay as they are.  A page that several sequences share must not be written.
+ * A place that there is not sets status bit 512; what it should have held, or should hold, is left out.
+ * w->decay is not looked at.  w->after may be w->before (with the same strides), or must not overlap it; after_length >= keep.
+ */
+int tritt_cache_evict(const tritt_cache_t* c, const tritt_weights_t* w, const int* table_out, long long table_out_stride, int table_out_pages, int keep, int first,
+                      int recent, int* context_out, int* kept, int* status_word, tritt_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -157,3 +157,37 @@ class Sequences:
                 if lse is not None:
                     self.lse[page, :, row] = lse[b][:, t].float()
         self.bias = None if lse is None else [x.float().double() for x in lse]
+
+
+def tdp_weights(q, k1, k2, ctx, i, alpha, windows, lse):
+    """What new token i and one head add to each token's weight: q [D], cached values [tokens, D] in 64 bits.  -> (sums [tokens], largest sum of |alpha q k1 k2| over the
+    attended pairs)."""
+    k1w, k2w, kkl, kkr = (1 << 40 if w is None else w for w in windows)
+    gain, at = torch.zeros(k1.shape[0], dtype=torch.float64), ctx + i
+    s = alpha * torch.einsum("d,jd,kd->jk", q, k1[:at + 1], k2[:at + 1])
+    size = abs(alpha) * torch.einsum("d,jd,kd->jk", q.abs(), k1[:at + 1].abs(), k2[:at + 1].abs())
+    pj, pk = torch.arange(at + 1)[:, None], torch.arange(at + 1)[None]
+    seen = (at - pj <= k1w) & (at - pk <= k2w) & (pk - pj <= kkl) & (pj - pk <= kkr)
+    p = torch.where(seen, (s - lse).exp(), 0.0)
+    gain[:at + 1] = p.sum(1) + p.sum(0)
+    return gain, torch.where(seen, size, 0.0).max()
+
+
+def dps_weights(q, k2_new, k1, k2, bias, ctx, i, alpha, k_diff, m):
+    """The same of the dot-product sum; bias [tokens] holds the cached log-sum-exps."""
+    gain, at = torch.zeros(k1.shape[0], dtype=torch.float64), ctx + i
+    lo = max(0, at - k_diff)
+    gain[:at + 1] = (alpha * (k2[:at + 1] @ q) + bias[:at + 1] - m).exp()
+    gain[lo:at + 1] += (alpha * (k1[lo:at + 1] @ k2_new) - bias[at]).exp()
+    size = max((alpha * (k2[:at + 1].abs() @ q.abs())).abs().max(), (alpha * (k1[lo:at + 1].abs() @ k2_new.abs())).abs().max())
+    return gain, size
+
+
+def evicted(weights, ctx, keep, first, recent):
+    """Numbers of the tokens that one sequence and head keeps, of `ctx` with these weights."""
+    if ctx <= keep:
+        return list(range(ctx))
+    key = lambda x: (-math.inf if math.isnan(weights[x]) else -weights[x], x)  # noqa: E731 (the largest first, then the lowest number)
+    nan = [x for x in range(first, ctx - recent) if math.isnan(weights[x])]
+    rest = sorted((x for x in range(first, ctx - recent) if not math.isnan(weights[x])), key=key)
+    return sorted(list(range(first)) + (nan + rest)[: keep - first - recent] + list(range(ctx - recent, ctx)))
