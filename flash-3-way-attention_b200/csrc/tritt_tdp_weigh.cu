@@ -1,4 +1,5 @@
-// The attention weight of cached tokens in the triple dot product, with warp-level matrix instructions: any head dimension.
+// The attention weight of cached tokens in the triple dot product, with warp-level matrix instructions: head dimensions
+// 16, 32 and 256 (64 and 128 run on tcgen05).
 //
 //   P[j, k] = exp(alpha sum_h q[h] K1[j, h] K2[k, h] - lse),   w[x] = decay w[x] + sum_i (sum_k P_i[x, k] + sum_j P_i[j, x])
 // For one new token and a tile of 128 tokens k the operand A[k] = q * K2[k] is formed once, as two fp16 numbers an element (22 bits: 16-bit queries times any code are exact), in the order of the
@@ -191,7 +192,6 @@ template <typename T, int D, int CODE> __global__ void __launch_bounds__(kThread
 
 // Adds up a head's slots, and the weights of before.
 __global__ void __launch_bounds__(256) tdp_weigh_join_kernel(const __grid_constant__ TdpWeighArgs p) {
-  wait_for_previous();
   __shared__ long long scan[33];
   const CacheArgs& a = p.cache;
   const int bh = blockIdx.y, b = bh / a.c.N, head = bh - b * a.c.N;
@@ -199,29 +199,30 @@ __global__ void __launch_bounds__(256) tdp_weigh_join_kernel(const __grid_consta
   const int ctx = context_of(a, b), end = weighed_tokens(a, p.w, ctx + new_tokens(a, b)), x = blockIdx.x * 256 + threadIdx.x;
   if ((int)blockIdx.x * 256 >= end) return;
   // steps of all sequences, and of those before this one
-  long long all = 0, before = 0, total;
+  long long all = 0, before = 0, total, ahead;
   for (int i = threadIdx.x; i < a.c.B; i += 256) {
     const long long v = weigh_line(p, i).unit * a.c.N;
     all += v;
     if (i < b) before += v;
   }
   block_scan(all, scan, total);
-  long long ahead;
   block_scan(before, scan, ahead);
-  if (x >= end) return;
-  float v = x < ctx ? faded(p.w, b, head, x) : 0.f;
   const WeighLine l = weigh_line(p, b);
-  if (l.unit > 0 && x >= l.base && x <= l.last) {
+  float v = x < ctx && x < end ? faded(p.w, b, head, x) : 0.f, sum = 0.f;
+  const bool any = l.unit > 0 && x >= l.base && x <= l.last;
+  int c0 = 0, c1 = -1;   // CTAs that have steps of this head
+  if (any) {
     const long long s0 = ahead + head * l.unit, s1 = s0 + l.unit - 1;
-    const int parts = weigh_parts(p, total), c0 = (int)(((s0 + 1) * parts + total - 1) / total) - 1, c1 = (int)(((s1 + 1) * parts + total - 1) / total) - 1;
-    float sum = 0.f;
-    for (int i = c0; i <= c1; ++i) {
-      const float* slot = p.part + ((size_t)i + bh) * p.sums * p.span + (x - l.base);
-      for (int k = 0; k < p.sums; ++k) sum += slot[(size_t)k * p.span];
-    }
-    v += sum;
+    const int parts = weigh_parts(p, total);
+    c0 = (int)(((s0 + 1) * parts + total - 1) / total) - 1;
+    c1 = (int)(((s1 + 1) * parts + total - 1) / total) - 1;
   }
-  *weight_of(p.w, b, head, x) = v;
+  wait_for_previous();   // (what is above depends on the call's arguments alone)
+  const float* slot = p.part + ((size_t)c0 + bh) * p.sums * p.span + (any ? x - l.base : 0);
+  const int terms = (c1 - c0 + 1) * p.sums;
+#pragma unroll 8
+  for (int i = 0; i < terms; ++i) sum += slot[(size_t)i * p.span];
+  if (x < end) *weight_of(p.w, b, head, x) = v + sum;
 }
 
 template <typename T, int D, int CODE> int launch(const TdpWeighArgs& p, cudaStream_t stream) {
@@ -236,8 +237,6 @@ template <typename T, int CODE> int by_size(const TdpWeighArgs& p, cudaStream_t 
   switch (p.cache.c.D) {
     case 16: return launch<T, 16, CODE>(p, stream);
     case 32: return launch<T, 32, CODE>(p, stream);
-    case 64: return launch<T, 64, CODE>(p, stream);
-    case 128: return launch<T, 128, CODE>(p, stream);
     default: return launch<T, 256, CODE>(p, stream);
   }
 }
@@ -333,8 +332,10 @@ int tritt_tdp_weigh(const tritt_cache_t* c, const tritt_weights_t* w, const trit
   }
   auto window = [](int v) { return v < kUnlimited ? v : kUnlimited; };
   TdpWeighArgs p{cache_args(*c, status_word), *w, *q, lse, dtype, window(k1_window), window(k2_window), window(kk_left), window(kk_right), alpha * kLog2e,
-                 (float*)workspace, kWeighCtas, weigh_span(*c, window(k1_window), window(k2_window)), 2};
-  if (int rc = mma_tdp_weigh(p, (cudaStream_t)stream)) return rc;
+                 (float*)workspace, kWeighCtas, weigh_span(*c, window(k1_window), window(k2_window)), 0};
+  const bool fast = sm100_tdp_weigh_supported(c->D);
+  p.sums = fast ? 3 : 2;
+  if (int rc = fast ? sm100_tdp_weigh(p, (cudaStream_t)stream) : mma_tdp_weigh(p, (cudaStream_t)stream)) return rc;
   return launch_tdp_weigh_join(p, (cudaStream_t)stream);
 }
 

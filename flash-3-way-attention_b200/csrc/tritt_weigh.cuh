@@ -311,6 +311,9 @@ __device__ __forceinline__ float* weigh_slot(const TdpWeighArgs& a, int b, int h
   return a.part + ((size_t)blockIdx.x + (size_t)b * a.cache.c.N + head) * a.sums * a.span;
 }
 
+// on the tensor cores (head dimension 64 or 128; three sums a slot), and with warp-level matrix instructions (two)
+bool sm100_tdp_weigh_supported(int D);
+int sm100_tdp_weigh(const TdpWeighArgs& a, cudaStream_t stream);
 int mma_tdp_weigh(const TdpWeighArgs& a, cudaStream_t stream);
 int launch_tdp_weigh_join(const TdpWeighArgs& a, cudaStream_t stream);
 
