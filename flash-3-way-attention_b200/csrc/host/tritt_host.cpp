@@ -50,6 +50,10 @@ struct Entries {   // (the addresses come from Python, which has loaded the libr
   decltype(&tritt_decode_workspace) decode_workspace;
   decltype(&tritt_qk_norm_rotary_axes_fwd) norm_axes_fwd;
   decltype(&tritt_qk_norm_rotary_axes_bwd) norm_axes_bwd;
+  decltype(&tritt_tdp_weigh) tdp_weigh;
+  decltype(&tritt_tdp_weigh_workspace) tdp_weigh_workspace;
+  decltype(&tritt_dps_weigh) dps_weigh;
+  decltype(&tritt_cache_evict) cache_evict;
 } lib{};
 volatile int* status_words[kDevices] = {};
 std::map<std::array<int, 12>, size_t> workspace_sizes;
@@ -598,6 +602,97 @@ PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// Weights [B, N, tokens] of a cache's tokens and where the new ones go (None: to the same place).
+bool read_weights(PyObject* before, PyObject* after, const tritt_cache_t& c, int device, tritt_weights_t& w) {
+  w = {};
+  const at::Tensor* t[2] = {plain(before, device), after == Py_None ? nullptr : plain(after, device)};
+  if (after == Py_None) t[1] = t[0];
+  for (const at::Tensor* x : t)
+    if (!x || x->dim() != 3 || x->scalar_type() != at::kFloat || x->size(0) != c.B || x->size(1) != c.N || x->size(2) > INT_MAX ||
+        (x->size(2) > 1 && x->stride(2) != 1) || x->requires_grad())
+      return false;
+  if (t[0]->data_ptr() == t[1]->data_ptr() && t[0]->strides() != t[1]->strides()) return false;
+  auto stride = [](const at::Tensor* x, int i) { return x->size(i) > 1 ? (long long)x->stride(i) : 0; };
+  w.before = (const float*)t[0]->data_ptr(), w.after = (float*)t[1]->data_ptr();
+  w.before_stride_b = stride(t[0], 0), w.before_stride_n = stride(t[0], 1), w.after_stride_b = stride(t[1], 0), w.after_stride_n = stride(t[1], 1);
+  w.before_length = (int)t[0]->size(2), w.after_length = (int)t[1]->size(2);
+  return true;
+}
+
+// weigh(codes, exponents, lse, table, context, counts, None, weights, out, decay, scale, q, log-sum-exps, then
+//   tdp: four windows;   dps: k2, k_diff) -> the library's error code (0: done), or None
+PyObject* weigh(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  int tokens, device, w[4] = {0, 0, 0, 0};
+  float scale;
+  tritt_cache_t c;
+  tritt_weights_t weights;
+  tritt_rows_t q, k2;
+  const float* sums;
+  Shape s;
+  const bool tdp = n == 17;
+  if ((!tdp && n != 15) || !(tokens = new_count(a[11])) || !read_cache(a, tokens, c, device) || !read_weights(a[7], a[8], c, device, weights) ||
+      !read_float(a[9], weights.decay) || !read_float(a[10], scale) || !read_new(a + 11, 1, c, device, s, &q) ||
+      !dense(a[12], device, at::kFloat, {c.B, c.N, tokens}, 4, sums) || (!tdp && (!c.lse || !is_tensor(a[13]) || !read_rows(a[13], s, k2))))
+    Py_RETURN_NONE;
+  for (int i = 0; i < (tdp ? 4 : 1); ++i)
+    if (!read_int(a[(tdp ? 13 : 14) + i], tdp ? 1 << 30 : -1, w[i]) || w[i] < 0) Py_RETURN_NONE;
+  int* const status = status_of(device);
+  if (!status) Py_RETURN_NONE;
+  at::Tensor scratch;
+  int rc = 0;
+  {
+    Unlocked unlocked;
+    void* const stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
+    if (tdp) {
+      const size_t bytes = std::max<size_t>(lib.tdp_weigh_workspace(&c, w[0], w[1]), 256);
+      scratch = at::empty({(int64_t)bytes}, THPVariable_Unpack(a[11]).options().dtype(at::kByte));
+      void* const ws = fresh(scratch);
+      rc = ws ? lib.tdp_weigh(&c, &weights, &q, sums, s.dtype, scale, w[0], w[1], w[2], w[3], ws, bytes, status, stream) : kNotPlain;
+    } else {
+      rc = lib.dps_weigh(&c, &weights, &q, &k2, sums, s.dtype, scale, w[0], status, stream);
+    }
+  }
+  if (rc == kNotPlain) Py_RETURN_NONE;
+  return PyLong_FromLong(rc);
+  END_HANDLE_TH_ERRORS
+}
+
+// cache_evict(codes, exponents, lse, table, context, None, None, weights, out, keep, first, recent, table_out) -> (context, kept), the library's error
+// code, or None
+PyObject* cache_evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  int device, keep, first, recent;
+  tritt_cache_t c;
+  tritt_weights_t weights;
+  if (n != 13 || !read_cache(a, 1, c, device) || !read_weights(a[7], a[8], c, device, weights) || !read_int(a[9], -1, keep) ||
+      !read_int(a[10], -1, first) || !read_int(a[11], -1, recent) || keep < 1 || keep > weights.after_length)
+    Py_RETURN_NONE;
+  const at::Tensor* table = a[12] == Py_None ? nullptr : plain(a[12], device);
+  if (a[12] != Py_None && (!table || table->dim() != 2 || table->scalar_type() != at::kInt || table->size(0) != c.B || table->size(1) > INT_MAX ||
+                           (table->size(1) > 1 && table->stride(1) != 1)))
+    Py_RETURN_NONE;
+  int* const status = status_of(device);
+  if (!status) Py_RETURN_NONE;
+  weights.decay = 1.f;
+  const at::Tensor& context = THPVariable_Unpack(a[4]);
+  at::Tensor out[2];
+  int rc = 0;
+  {
+    Unlocked unlocked;
+    out[0] = at::empty({c.B}, context.options());
+    out[1] = at::empty({c.B, c.N, keep}, context.options());
+    int *left = (int*)fresh(out[0]), *kept = (int*)fresh(out[1]);
+    rc = left && kept ? lib.cache_evict(&c, &weights, table ? (const int*)table->data_ptr() : nullptr, table ? (long long)table->stride(0) : 0,
+                                        table ? (int)table->size(1) : 0, keep, first, recent, left, kept, status,
+                                        c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream())
+                      : kNotPlain;
+  }
+  if (rc == kNotPlain) Py_RETURN_NONE;
+  return rc != 0 ? PyLong_FromLong(rc) : wrap_all(out, 2);
+  END_HANDLE_TH_ERRORS
+}
+
 // init(addresses of the entry points, in the order of Entries)
 PyObject* init(PyObject*, PyObject* args) {
   constexpr Py_ssize_t kEntries = sizeof(Entries) / sizeof(void*);
@@ -635,6 +730,8 @@ PyMethodDef methods[] = {{"init", init, METH_VARARGS, nullptr},
                          {"cache_write", (PyCFunction)(void (*)(void))cache_write, METH_FASTCALL, nullptr},
                          {"cache_read", (PyCFunction)(void (*)(void))cache_read, METH_FASTCALL, nullptr},
                          {"decode", (PyCFunction)(void (*)(void))decode, METH_FASTCALL, nullptr},
+                         {"weigh", (PyCFunction)(void (*)(void))weigh, METH_FASTCALL, nullptr},
+                         {"cache_evict", (PyCFunction)(void (*)(void))cache_evict, METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -27,13 +27,24 @@ struct Params {
   int keep, first, recent;
   int* context_out;
   int* kept;
+  int ranks;              // CTAs of a cluster that moves rows
 };
 
-// A weight's bits in the order of the weights: a NaN as the largest, zeros of either sign alike.
-__device__ __forceinline__ uint32_t order_of(float v) {
-  const uint32_t u = __float_as_uint(v);   // (comparisons of numbers would take the smallest for zeros)
-  if ((u & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;
-  if (u << 1 == 0u) return 0x80000000u;
+// Tokens of a sequence, negative: it is not used.  (Those that have no weights are reported and left out.)
+__device__ __forceinline__ int tokens_of(const Params& p, int b) {
+  const int given = __ldg(p.cache.c.context + b);
+  if (given < 0) return given;
+  const int ctx = context_of(p.cache, b);
+  if (ctx > p.w.before_length && p.cache.status) atomicOr(p.cache.status, kStatusPlace);
+  return ctx < p.w.before_length ? ctx : p.w.before_length;
+}
+
+// A weight's bits in the order of the weights: a NaN as the largest, zeros of either sign alike.  (Bits from the load on: as a number the smallest would be taken for a zero, whose comparisons with
+// fast arithmetic they are.)
+__device__ __forceinline__ uint32_t order_of(uint32_t u) {
+  const uint32_t size = u & 0x7fffffffu;
+  if (size > 0x7f800000u) return 0xffffffffu;
+  if (size == 0u) return 0x80000000u;
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
@@ -59,47 +70,70 @@ __device__ __forceinline__ uint32_t scan1024(uint32_t v, uint32_t* tmp, uint32_t
   return v + (warp ? before : 0u);
 }
 
-__global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __grid_constant__ Params p) {
-  __shared__ uint32_t hist[3][kBins], tmp[32], found[2], counts[2];
+// HELD: a thread's weights, kHeld neighbours of them, stay in its registers (a CTA has at most kHeld * 1024); else they are read again for each pass.
+constexpr int kHeld = 16;
+template <bool HELD> __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __grid_constant__ Params p) {
+  __shared__ __align__(8) uint32_t hist[3][kBins], tmp[32], found[2], counts[2];
   let_next_start();
   const CacheArgs& a = p.cache;
   const cg::cluster_group cluster = cg::this_cluster();
   const int rank = blockIdx.x, ranks = gridDim.x, tid = threadIdx.x;
   const int bh = blockIdx.y, b = bh / a.c.N, head = bh - b * a.c.N;
-  const int given = __ldg(a.c.context + b), ctx = given < 0 ? given : context_of(a, b);
+  const int ctx = tokens_of(p, b);
   if (rank == 0 && head == 0 && tid == 0) p.context_out[b] = ctx < p.keep ? ctx : p.keep;
   int* const kept = p.kept + (size_t)bh * p.keep;
   if (ctx <= p.keep) {   // (all of a cluster's CTAs)
     for (int r = rank * kSelectThreads + tid; r < p.keep; r += ranks * kSelectThreads) kept[r] = r < ctx ? r : -1;
     return;
   }
-  if (ctx > p.w.before_length && a.status) atomicOr(a.status, kStatusPlace);
-  const float* const w = p.w.before + b * p.w.before_stride_b + head * p.w.before_stride_n;
-  auto key = [&](int x) { return order_of(x < p.w.before_length ? __ldg(w + x) : 0.f); };
+  const uint32_t* const w = reinterpret_cast<const uint32_t*>(p.w.before) + b * p.w.before_stride_b + head * p.w.before_stride_n;
+  auto key = [&](int x) { return order_of(__ldg(w + x)); };
   const int lo = p.first, hi = ctx - p.recent, need = p.keep - p.first - p.recent;
   const int each = (hi - lo + ranks - 1) / ranks, x0 = lo + rank * each, x1 = x0 + each < hi ? x0 + each : hi;   // this CTA's tokens
+  const int own = (each + kSelectThreads - 1) / kSelectThreads, own0 = x0 + tid * own;                           // HELD: this thread's, from own0 on
+  uint32_t held[HELD ? kHeld : 1];
+  if constexpr (HELD) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      if (i < own && own0 + i < x1) held[i] = key(own0 + i);
+  }
+  auto each_key = [&](auto&& f) {
+    if constexpr (HELD) {
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i)
+        if (i < own && own0 + i < x1) f(held[i]);
+    } else {
+      for (int x = x0 + tid; x < x1; x += kSelectThreads) f(key(x));
+    }
+  };
   for (int r = rank * kSelectThreads + tid; r < p.first; r += ranks * kSelectThreads) kept[r] = r;
   for (int r = rank * kSelectThreads + tid; r < p.recent; r += ranks * kSelectThreads) kept[p.keep - p.recent + r] = ctx - p.recent + r;
   if (need == 0) return;
 
   for (int i = tid; i < 3 * kBins; i += kSelectThreads) (&hist[0][0])[i] = 0;
+  if (tid < 2) counts[tid] = 0;
   __syncthreads();
   uint32_t prefix = 0, mask = 0, left = (uint32_t)need;   // digits found so far; tokens still to be found among those that have them
+#pragma unroll 1
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
-    for (int x = x0 + tid; x < x1; x += kSelectThreads) {
-      const uint32_t k = key(x);
-      if ((k & mask) == prefix) atomicAdd(&hist[pass][k >> shift & (bins - 1)], 1u);
-    }
-    cluster.sync();
+    uint32_t* const h = hist[pass];
+    each_key([&](uint32_t k) {
+      if ((k & mask) == prefix) atomicAdd(&h[k >> shift & (bins - 1)], 1u);
+    });
+    if (ranks > 1)
+      cluster.sync();
+    else
+      __syncthreads();
     // the counts of all CTAs, from the largest digit down: two digits a thread
     const int d = bins - 1 - 2 * tid;
     uint32_t n0 = 0, n1 = 0;
     if (d > 0)
+#pragma unroll 8
       for (int i = 0; i < ranks; ++i) {
-        const uint32_t* other = cluster.map_shared_rank(&hist[pass][0], i);
-        n0 += other[d];
-        n1 += other[d - 1];
+        const uint2 other = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(h, i) + (d - 1));
+        n0 += other.y;
+        n1 += other.x;
       }
     uint32_t total;
     const uint32_t behind = scan1024(n0 + n1, tmp, total), before = behind - n0 - n1;
@@ -114,42 +148,59 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __gr
     left = found[1];
   }
   // kept: weights above `prefix`, and the first `left` tokens of that weight.  Those of the CTAs before this one:
-  if (tid < 2) counts[tid] = 0;
-  __syncthreads();
   uint32_t more = 0, same = 0;
-  for (int x = x0 + tid; x < x1; x += kSelectThreads) {
-    const uint32_t k = key(x);
+  each_key([&](uint32_t k) {
     more += k > prefix;
     same += k == prefix;
+  });
+  const uint32_t own_more = more, own_same = same;
+  if (ranks > 1) {
+    more = __reduce_add_sync(0xffffffffu, more);
+    same = __reduce_add_sync(0xffffffffu, same);
+    if (tid % 32 == 0) {
+      atomicAdd(&counts[0], more);   // (whole numbers: in any order)
+      atomicAdd(&counts[1], same);
+    }
+    cluster.sync();
+    more = same = 0;
+#pragma unroll 8
+    for (int i = 0; i < rank; ++i) {
+      const uint2 other = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(&counts[0], i));
+      more += other.x;
+      same += other.y;
+    }
+  } else {
+    more = same = 0;
   }
-  more = __reduce_add_sync(0xffffffffu, more);
-  same = __reduce_add_sync(0xffffffffu, same);
-  if (tid % 32 == 0) {
-    atomicAdd(&counts[0], more);   // (whole numbers: in any order)
-    atomicAdd(&counts[1], same);
+  uint32_t total;
+  if constexpr (HELD) {
+    const uint32_t scan = scan1024(own_more | own_same << 16, tmp, total);   // (kHeld * 1024 of either at most)
+    more += (scan & 0xffffu) - own_more;
+    same += (scan >> 16) - own_same;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      if (i < own && own0 + i < x1) {
+        const bool is_more = held[i] > prefix, is_same = held[i] == prefix;
+        if (is_more || (is_same && same < left)) kept[p.first + more + (same < left ? same : left)] = own0 + i;
+        more += is_more;
+        same += is_same;
+      }
+  } else {
+    for (int x = x0; x < x1; x += kSelectThreads) {
+      const uint32_t k = x + tid < x1 ? key(x + tid) : 0u;
+      const bool is_more = x + tid < x1 && k > prefix, is_same = x + tid < x1 && k == prefix;
+      const uint32_t scan = scan1024((uint32_t)is_more | (uint32_t)is_same << 16, tmp, total);   // (1024 of either at most)
+      const uint32_t m = more + (scan & 0xffffu) - is_more, s = same + (scan >> 16) - is_same;   // before this token
+      if (is_more || (is_same && s < left)) kept[p.first + m + (s < left ? s : left)] = x + tid;
+      more += total & 0xffffu;
+      same += total >> 16;
+    }
   }
-  cluster.sync();
-  more = same = 0;
-  for (int i = 0; i < rank; ++i) {
-    const uint32_t* other = cluster.map_shared_rank(&counts[0], i);
-    more += other[0];
-    same += other[1];
-  }
-  for (int x = x0; x < x1; x += kSelectThreads) {
-    const uint32_t k = x + tid < x1 ? key(x + tid) : 0u;
-    const bool is_more = x + tid < x1 && k > prefix, is_same = x + tid < x1 && k == prefix;
-    uint32_t total;
-    const uint32_t scan = scan1024((uint32_t)is_more | (uint32_t)is_same << 16, tmp, total);   // (1024 of either at most)
-    const uint32_t m = more + (scan & 0xffffu) - is_more, s = same + (scan >> 16) - is_same;   // before this token
-    if (is_more || (is_same && s < left)) kept[p.first + m + (s < left ? s : left)] = x + tid;
-    more += total & 0xffffu;
-    same += total >> 16;
-  }
-  cluster.sync();   // (the others read this CTA's counts)
+  if (ranks > 1) cluster.sync();   // (the others read this CTA's counts)
 }
 
 // ---------------------------------------------------------------- moving
-constexpr int kMoveThreads = 256, kRing = 4;
+constexpr int kMoveThreads = 256, kRing = 4, kMoveCtas = 4 * kSms;
 
 template <int W> struct Move {   // pieces of W bytes of a row
   static constexpr int kLanes = W / 16, kAtOnce = kMoveThreads / kLanes;
@@ -177,9 +228,11 @@ template <int W> __global__ void __launch_bounds__(kMoveThreads) evict_move_kern
   __shared__ long long from[kRing][M::kRows], to[kRing][M::kRows];   // numbers of a tile's rows, -1: none
   wait_for_previous();
   const CacheArgs& a = p.cache;
-  const int tid = threadIdx.x, piece = blockIdx.x, part = blockIdx.y, bh = blockIdx.z, b = bh / a.c.N, head = bh - b * a.c.N;
-  if (__ldg(a.c.context + b) < 0) return;
-  const int ctx = context_of(a, b), count = ctx < p.keep ? ctx : p.keep;
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int ranks = p.ranks, rank = blockIdx.x % ranks;
+  const int tid = threadIdx.x, piece = blockIdx.x / ranks, part = blockIdx.y, bh = blockIdx.z, b = bh / a.c.N, head = bh - b * a.c.N;
+  const int ctx = tokens_of(p, b), count = ctx < p.keep ? ctx : p.keep;
+  if (ctx < 0) return;
   const bool in_place = p.table_out == nullptr;
   const float* const before = p.w.before + b * p.w.before_stride_b + head * p.w.before_stride_n;
   float* const after = p.w.after + b * p.w.after_stride_b + head * p.w.after_stride_n;
@@ -200,7 +253,7 @@ template <int W> __global__ void __launch_bounds__(kMoveThreads) evict_move_kern
   auto find = [&](int tile) {   // places of a tile's rows
 #pragma unroll
     for (int k = 0; k < M::kOwn; ++k) {
-      const int at = tid + k * kMoveThreads, r = tile * M::kRows + at;
+      const int at = tid + k * kMoveThreads, r = (tile * ranks + rank) * M::kRows + at;
       if (at >= M::kRows) break;
       long long f = -1, t = -1;
       if (r < count) {
@@ -228,14 +281,13 @@ template <int W> __global__ void __launch_bounds__(kMoveThreads) evict_move_kern
     }
 #pragma unroll
     for (int k = 0; k < M::kOwn; ++k) {
-      const int i = tid + k * kMoveThreads, r = tile * M::kRows + i;
+      const int i = tid + k * kMoveThreads, r = (tile * ranks + rank) * M::kRows + i;
       if (i >= M::kRows) break;
       const long long f = at[i];
       if (f >= 0 && exponents) ex[k] = __ldcg(a.c.exponents + f);
       if (f >= 0 && lse) lx[k] = __ldcg(a.c.lse + lse_row(a, f, head));
       if (weights && r < count) {
-        const int x = __ldcg(kept + r);
-        wx[k] = x < p.w.before_length ? __ldcg(before + x) : 0.f;
+        wx[k] = __ldcg(before + __ldcg(kept + r));
       }
     }
   };
@@ -248,7 +300,7 @@ template <int W> __global__ void __launch_bounds__(kMoveThreads) evict_move_kern
     }
 #pragma unroll
     for (int k = 0; k < M::kOwn; ++k) {
-      const int i = tid + k * kMoveThreads, r = tile * M::kRows + i;
+      const int i = tid + k * kMoveThreads, r = (tile * ranks + rank) * M::kRows + i;
       if (i >= M::kRows) break;
       const long long t = at[i];
       if (t >= 0 && exponents) a.c.exponents[t] = ex[k];
@@ -256,29 +308,53 @@ template <int W> __global__ void __launch_bounds__(kMoveThreads) evict_move_kern
       if (weights && r < count) after[r] = wx[k];
     }
   };
-  const int tiles = (count + M::kRows - 1) / M::kRows;
+  const int tiles = (count + M::kRows * ranks - 1) / (M::kRows * ranks);
   if (tiles == 0) return;
+  auto sync = [&]() {
+    if (ranks > 1)
+      cluster.sync();
+    else
+      __syncthreads();
+  };
   // Before a tile is written its rows, and those of all tiles before it, have been read by all threads (the barrier behind their loads); the next tile's, on their way then, lie behind what is written.
   // The ring's place that `find` fills was last read by the stores of two tiles ago, before the last barrier.
   find(0);
   __syncthreads();
   load(0, v[0], e[0], l[0], wt[0]);
   if (tiles > 1) find(1);
-  __syncthreads();
+  sync();
   for (int i = 0; i < tiles; i += 2) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       if (i + k >= tiles) break;
       if (i + k + 1 < tiles) load(i + k + 1, v[1 - k], e[1 - k], l[1 - k], wt[1 - k]);
       if (i + k + 2 < tiles) find(i + k + 2);
-      __syncthreads();
+      sync();
       store(i + k, v[k], e[k], l[k], wt[k]);
     }
   }
 }
 
-template <int W> int launch_move(const Params& p, int row_bytes, cudaStream_t stream) {
-  return launch_kernel_after(evict_move_kernel<W>, dim3(row_bytes / W, 4, p.cache.c.B * p.cache.c.N), kMoveThreads, 0, stream, true, p);
+template <int W> int launch_move(Params p, int row_bytes, cudaStream_t stream) {
+  const int pieces = row_bytes / W;
+  // as many CTAs as keep all SMs' loads in flight, while each has two tiles
+  const long long streams = 4LL * p.cache.c.B * p.cache.c.N * pieces;
+  while (p.ranks < kMostCluster && streams * p.ranks < kMoveCtas && p.keep > 2 * Move<W>::kRows * p.ranks) p.ranks *= 2;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(pieces * p.ranks, 4, p.cache.c.B * p.cache.c.N);
+  cfg.blockDim = dim3(kMoveThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2]{};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = p.ranks;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  TRITT_CUDA_OK(cudaLaunchKernelEx(&cfg, evict_move_kernel<W>, p));
+  count_launch();
+  return 0;
 }
 
 int check(const tritt_cache_t* c, const tritt_weights_t* w, const Params& p) {
@@ -322,7 +398,7 @@ extern "C" int tritt_cache_evict(const tritt_cache_t* c, const tritt_weights_t* 
                                  int first, int recent, int* context_out, int* kept, int* status_word, tritt_stream_t stream) {
   if (int rc = check_cache(c)) return rc;
   if (int rc = check_weights(c, w)) return rc;
-  Params p{cache_args(*c, status_word), *w, table_out, table_out_stride, table_out_pages, keep, first, recent, context_out, kept};
+  Params p{cache_args(*c, status_word), *w, table_out, table_out_stride, table_out_pages, keep, first, recent, context_out, kept, 1};
   if (int rc = check(c, w, p)) return rc;
   p.cache.c.n = 1;   // (places are reported of every sequence in use)
   p.cache.c.counts = nullptr;
@@ -330,7 +406,7 @@ extern "C" int tritt_cache_evict(const tritt_cache_t* c, const tritt_weights_t* 
   long long tokens = (long long)c->table_pages * c->page_size;
   if (w->before_length < tokens) tokens = w->before_length;
   int ranks = 1;
-  while (ranks < kMostCluster && tokens > 4096LL * ranks && 2LL * ranks * c->B * c->N <= 2 * kSms) ranks *= 2;
+  while (ranks < kMostCluster && tokens > 2048LL * ranks && 2LL * ranks * c->B * c->N <= kSms) ranks *= 2;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(ranks, c->B * c->N);
   cfg.blockDim = dim3(kSelectThreads);
@@ -341,14 +417,13 @@ extern "C" int tritt_cache_evict(const tritt_cache_t* c, const tritt_weights_t* 
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  TRITT_CUDA_OK(cudaLaunchKernelEx(&cfg, evict_select_kernel, p));
+  if (tokens <= (long long)kHeld * kSelectThreads * ranks)
+    TRITT_CUDA_OK(cudaLaunchKernelEx(&cfg, evict_select_kernel<true>, p));
+  else
+    TRITT_CUDA_OK(cudaLaunchKernelEx(&cfg, evict_select_kernel<false>, p));
   count_launch();
-  // Pieces of rows: the widest with which there are blocks enough to keep all SMs' loads in flight (each block takes all of a head's kept tokens, one tile after the other).
   const int row_bytes = c->D * code_bytes(c->code);
-  const long long parts = 4LL * c->B * c->N;
-  int piece = row_bytes < 128 ? row_bytes : 128;
-  while (piece > 32 && parts * (row_bytes / piece) < 4 * kSms) piece /= 2;
-  switch (piece) {
+  switch (row_bytes < 128 ? row_bytes : 128) {
     case 16: return launch_move<16>(p, row_bytes, (cudaStream_t)stream);
     case 32: return launch_move<32>(p, row_bytes, (cudaStream_t)stream);
     case 64: return launch_move<64>(p, row_bytes, (cudaStream_t)stream);

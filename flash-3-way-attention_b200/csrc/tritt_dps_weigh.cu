@@ -36,11 +36,15 @@ template <typename T, int D> constexpr int kBytesEach = 2 * D * 2 * (std::is_sam
 template <typename T, int D> constexpr int kMostChunk = 32768 / kBytesEach<T, D> < 64 ? 32768 / kBytesEach<T, D> : 64;
 static_assert(kMostChunk<float, 256> == 16 && kMostChunk<__half, 64> == 64, "chunks are multiples of 8");
 
-template <typename T, int D, int CODE> __global__ void __launch_bounds__(kThreads) dps_weigh_kernel(const __grid_constant__ Params p) {
+// Blocks an SM: registers for the bytes of rows that are to be in flight.
+template <int D, int CODE> constexpr int kPerSm = RowFragments<D, CODE>::kWords <= 4 ? 3 : RowFragments<D, CODE>::kWords <= 16 ? 2 : 1;
+
+template <typename T, int D, int CODE> __global__ void __launch_bounds__(kThreads, kPerSm<D, CODE>) dps_weigh_kernel(const __grid_constant__ Params p) {
   using Rows = RowFragments<D, CODE>;
   constexpr bool kWide = std::is_same<T, float>::value;
   constexpr int kSteps = Rows::kSteps, kHalves = kWide ? 2 : 1;
   constexpr bool kBoth = Rows::kWords <= 16;   // rows of both parts on their way together
+  constexpr bool kAhead = Rows::kWords <= 8;   // ... and two tiles' (registers)
   extern __shared__ __align__(16) uint2 frags[];   // [part][8 new tokens][hi, lo][step][lane]
   __shared__ Query queries[2][64];
   const CacheArgs& a = p.cache;
@@ -54,31 +58,42 @@ template <typename T, int D, int CODE> __global__ void __launch_bounds__(kThread
   const uint8_t* codes = (const uint8_t*)a.c.codes;
   constexpr size_t kRow = D * Rows::kSize;
 
-  for (int r = 0; r < p.repeat && first + r * kTokens < end; ++r) {
+  // a tile of 128 tokens, 16 a warp: the warp's rows, on their way from `fetch` on
+  struct Tile {
+    Rows rows[kBoth ? 2 : 1];
+    size_t row_k2, row_k1;
+    uint8_t byte[2][2];
+    float lse[2], before;
+    bool there, inner;
+  };
+  auto fetch = [&](int r, Tile& t) {
     const int x0 = first + r * kTokens + warp * 16;
     Place at{-1, 0};
     if (x0 < end) {
       at = place_of(a, b, x0);   // (16 tokens lie in one page)
       if (at.page < 0 && a.status) atomicOr(a.status, kStatusPlace);
     }
-    const bool there = at.page >= 0, inner = there && x0 + 15 >= behind;
-    const size_t row_k2 = there ? row_of(a, at, kPartK2, head) : 0, row_k1 = there ? row_of(a, at, kPartK1, head) : 0;
-    const float* lse_row = a.c.lse + (there ? lse_of(a, at, head) : 0);
-    Rows rows[kBoth ? 2 : 1];
-    float scale[2][2], lse[2] = {0.f, 0.f};
-    if (there) {
-      rows[0].load(codes + row_k2 * kRow, lane);
-      if (kBoth && inner) rows[kBoth].load(codes + row_k1 * kRow, lane);
+    t.there = at.page >= 0;
+    t.inner = t.there && x0 + 15 >= behind;
+    t.row_k2 = t.there ? row_of(a, at, kPartK2, head) : 0;
+    t.row_k1 = t.there ? row_of(a, at, kPartK1, head) : 0;
+    if (t.there) {
+      t.rows[0].load(codes + t.row_k2 * kRow, lane);
+      if (kBoth && t.inner) t.rows[kBoth].load(codes + t.row_k1 * kRow, lane);
+      const float* lse_row = a.c.lse + lse_of(a, at, head);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        scale[0][h] = code_scale(__ldg(a.c.exponents + row_k2 + g + 8 * h));
-        scale[1][h] = inner ? code_scale(__ldg(a.c.exponents + row_k1 + g + 8 * h)) : 0.f;
-        lse[h] = __ldg(lse_row + g + 8 * h);
+        t.byte[0][h] = __ldg(a.c.exponents + t.row_k2 + g + 8 * h);
+        t.byte[1][h] = t.inner ? __ldg(a.c.exponents + t.row_k1 + g + 8 * h) : 0;
+        t.lse[h] = __ldg(lse_row + g + 8 * h);
       }
     }
     const int mine = x0 + g + (c == 1 ? 8 : 0);   // the token whose weight this lane writes
-    float sum = 0.f;
-    if (c < 2 && mine < end && mine < ctx) sum = faded(p.w, b, head, mine);
+    t.before = 0.f;
+    if (c < 2 && mine < end && mine < ctx) t.before = faded(p.w, b, head, mine);
+  };
+  auto work = [&](int r, Tile& t) {
+    const int x0 = first + r * kTokens + warp * 16, mine = x0 + g + (c == 1 ? 8 : 0);
     float gain[2] = {0.f, 0.f};
     for (int q0 = 0, chunk = 0; chunk < chunks; ++chunk, q0 += p.chunk) {
       const int here = cnt - q0 < p.chunk ? cnt - q0 : p.chunk, tiles = (here + 7) / 8;
@@ -130,18 +145,19 @@ template <typename T, int D, int CODE> __global__ void __launch_bounds__(kThread
         }
         __syncthreads();
       }
-      if (!there) continue;
+      if (!t.there) continue;
 #pragma unroll
       for (int part = 0; part < 2; ++part) {
-        if (part && !inner) break;
-        Rows& now = rows[kBoth ? part : 0];
-        if (!kBoth && (part || chunk)) now.load(codes + (part ? row_k1 : row_k2) * kRow, lane);
+        if (part && !t.inner) break;
+        Rows& now = t.rows[kBoth ? part : 0];
+        if (!kBoth && (part || chunk)) now.load(codes + (part ? t.row_k1 : t.row_k2) * kRow, lane);
+        const float scale[2] = {code_scale(t.byte[part][0]), code_scale(t.byte[part][1])};
         uint32_t frag[kSteps][4];
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) now.step(s, frag[s]);
-        for (int t = 0; t < tiles; ++t) {
+        for (int i = 0; i < tiles; ++i) {
           float d[4] = {0.f, 0.f, 0.f, 0.f};
-          const uint2* from = frags + (size_t)((part * tiles + t) * kHalves) * kSteps * 32 + lane;
+          const uint2* from = frags + (size_t)((part * tiles + i) * kHalves) * kSteps * 32 + lane;
 #pragma unroll
           for (int s = 0; s < kSteps; ++s) {
             mma_16816(d, frag[s], from[s * 32]);
@@ -149,13 +165,13 @@ template <typename T, int D, int CODE> __global__ void __launch_bounds__(kThread
           }
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            const Query q = queries[part][t * 8 + 2 * c + k];
+            const Query q = queries[part][i * 8 + 2 * c + k];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const int x = x0 + g + 8 * h;
               const bool on = x <= q.last && (part == 0 || q.last - x <= p.k_diff);
-              const float less = part == 0 ? lse[h] - q.minus : -q.minus;
-              gain[h] += on ? exp2f(fmaf(d[2 * h + k] * scale[part][h], q.scale, less * kLog2e)) : 0.f;
+              const float less = part == 0 ? t.lse[h] - q.minus : -q.minus;
+              gain[h] += on ? exp2f(fmaf(d[2 * h + k] * scale[h], q.scale, less * kLog2e)) : 0.f;
             }
           }
         }
@@ -166,7 +182,26 @@ template <typename T, int D, int CODE> __global__ void __launch_bounds__(kThread
       gain[h] += __shfl_xor_sync(0xffffffffu, gain[h], 1);
       gain[h] += __shfl_xor_sync(0xffffffffu, gain[h], 2);
     }
-    if (c < 2 && mine < end) *weight_of(p.w, b, head, mine) = sum + (c ? gain[1] : gain[0]);
+    if (c < 2 && mine < end) *weight_of(p.w, b, head, mine) = t.before + (c ? gain[1] : gain[0]);
+  };
+  int tiles_here = end > first ? (end - first + kTokens - 1) / kTokens : 0;
+  if (tiles_here > p.repeat) tiles_here = p.repeat;
+  if constexpr (kAhead) {   // the next tile's rows are on their way while one is worked on
+    Tile even, odd;
+    if (tiles_here > 0) fetch(0, even);
+    for (int r = 0; r < tiles_here; r += 2) {
+      if (r + 1 < tiles_here) fetch(r + 1, odd);
+      work(r, even);
+      if (r + 1 >= tiles_here) break;
+      if (r + 2 < tiles_here) fetch(r + 2, even);
+      work(r + 1, odd);
+    }
+  } else {
+    Tile tile;
+    for (int r = 0; r < tiles_here; ++r) {
+      fetch(r, tile);
+      work(r, tile);
+    }
   }
 }
 
@@ -180,7 +215,7 @@ template <typename T, int D, int CODE> int launch(Params p, cudaStream_t stream)
   if (length < tokens) tokens = length;
   const long long blocks = (tokens + kTokens - 1) / kTokens;
   // the new rows are formed once a block: it takes several times kTokens where there are blocks enough for all SMs several times over
-  long long repeat = blocks * c.B * c.N / (kSms * 16);
+  long long repeat = blocks * c.B * c.N / (kSms * 3);
   p.repeat = (int)(repeat < 1 ? 1 : repeat > 8 ? 8 : repeat);
   const dim3 grid((unsigned)((blocks + p.repeat - 1) / p.repeat), c.B * c.N);
   dps_weigh_kernel<T, D, CODE><<<grid, kThreads, bytes, stream>>>(p);

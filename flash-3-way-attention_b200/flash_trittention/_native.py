@@ -117,11 +117,20 @@ def host_cache_read(*args):
 
 
 def host_decode(*args):
-    """and ``tdp_decode``, ``dps_append`` and ``dps_decode``."""
+    """``tdp_decode``, ``dps_append`` and ``dps_decode``,"""
+
+
+def host_weigh(*args):
+    """``tdp_weigh`` and ``dps_weigh``,"""
+
+
+def host_evict(*args):
+    """``cache_evict``."""
 
 
 def _load_host(L):
     global _host, host_forward, host_backward, host_norm_rotary, host_norm_rotary_backward, host_cache_write, host_cache_read, host_decode
+    global host_weigh, host_evict
     try:
         host = importlib.import_module("._host", __package__)
         built_for = getattr(host, "torch_version", "another version")
@@ -136,12 +145,13 @@ def _load_host(L):
     _host.init(*(C.cast(getattr(L, "tritt_" + name), C.c_void_p).value for name in (
         "tdp_fwd", "tdp_bwd", "dps_fwd", "dps_bwd", "dps_bwd_saved", "workspace_bytes_flags", "tdp_fwd_workspace", "qk_norm_rotary_fwd",
         "qk_norm_rotary_bwd", "qk_norm_rotary_workspace", "cache_write", "cache_read", "tdp_decode", "dps_append", "dps_decode",
-        "decode_workspace", "qk_norm_rotary_axes_fwd", "qk_norm_rotary_axes_bwd")))
+        "decode_workspace", "qk_norm_rotary_axes_fwd", "qk_norm_rotary_axes_bwd", "tdp_weigh", "tdp_weigh_workspace", "dps_weigh", "cache_evict")))
     for device, address in _status_ptr.items():
         _host.set_status(device, address)
     host_forward, host_backward = _host.forward, _host.backward
     host_norm_rotary, host_norm_rotary_backward = _host.norm_rotary, _host.norm_rotary_backward
     host_cache_write, host_cache_read, host_decode = _host.cache_write, _host.cache_read, _host.decode
+    host_weigh, host_evict = _host.weigh, _host.cache_evict
 
 
 def lib():

@@ -73,7 +73,11 @@ def tdp_weigh(weights: Tensor, q: Tensor, lse: Tensor, cache: TrittentionCache, 
         _cache(cache)
         return ops.tdp_weigh(weights if out is None else out, None if out is None else weights, q, lse, cache.codes, cache.exponents, table, context, softmax_scale,
                              k1_window, k2_window, kk_left, kk_right, counts, decay)
-    q, = _check_new(_cache(cache), table, (q,))
+    done = _native.host_weigh(*_cache(cache), table, context, counts, None, weights, out, decay, softmax_scale, q, lse, k1_window, k2_window, kk_left, kk_right)
+    if done is not None:
+        _native.host_result(done, "tritt_tdp_weigh")
+        return
+    q, = _check_new(cache, table, (q,))
     c, keep = _describe(cache, table, context, q.shape[2], counts, None)
     w, lse = _weights(cache, table, weights, out, decay), _sums("lse", lse, q)
     windows = [_UNLIMITED if v is None else min(int(v), _UNLIMITED) for v in (k1_window, k2_window, kk_left, kk_right)]
@@ -93,6 +97,10 @@ def dps_weigh(weights: Tensor, q: Tensor, k2: Tensor, m: Tensor, cache: Trittent
         from . import ops
 
         return ops.dps_weigh(weights if out is None else out, None if out is None else weights, q, k2, m, *cache, table, context, softmax_scale, k_diff, counts, decay)
+    done = _native.host_weigh(*cache, table, context, counts, None, weights, out, decay, softmax_scale, q, m, k2, k_diff)
+    if done is not None:
+        _native.host_result(done, "tritt_dps_weigh")
+        return
     q, k2 = _check_new(cache, table, (q, k2))
     c, keep = _describe(cache, table, context, q.shape[2], counts, None)
     w, m = _weights(cache, table, weights, out, decay), _sums("m", m, q)
@@ -120,7 +128,10 @@ def cache_evict(weights: Tensor, cache: TrittentionCache, table: Tensor, context
 
         return ops.cache_evict(*_cache(cache), weights if weights_out is None else weights_out, None if weights_out is None else weights, table, context, keep, first, recent,
                                table_out)
-    c, alive = _describe(_cache(cache), table, context, 1, None, None)
+    out = _native.host_evict(*_cache(cache), table, context, None, None, weights, weights_out, keep, first, recent, table_out)
+    if out is not None:
+        return _native.host_result(out, "tritt_cache_evict")
+    c, alive = _describe(cache, table, context, 1, None, None)
     dev, page = cache.codes.device, cache.codes.shape[3]
     w = _weights(cache, table, weights, weights_out)
     if w.after_length < keep:

@@ -395,7 +395,7 @@ int tritt_dps_weigh(const tritt_cache_t* c, const tritt_weights_t* w, const trit
  * `keep` tokens keeps all of them; context[b] < 0 stays as it is.
  * table_out null: in place (the places behind the last kept token keep what they hold).  Else the rows go to the pages of table_out, [B, table_out_pages] with stride
  * table_out_stride, of which none may be one that the call reads, and the old ones stay as they are.  A page that several sequences share must not be written.
- * A place that there is not sets status bit 512; what it should have held, or should hold, is left out.
+ * A place that there is not sets status bit 512; what it should have held, or should hold, is left out.  So does a token beyond before_length.
  * w->decay is not looked at.  w->after may be w->before (with the same strides), or must not overlap it; after_length >= keep.
  */
 int tritt_cache_evict(const tritt_cache_t* c, const tritt_weights_t* w, const int* table_out, long long table_out_stride, int table_out_pages, int keep, int first,

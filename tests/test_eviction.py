@@ -113,7 +113,7 @@ TDP = [  # B N n D dtype code page contexts windows counts
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("B,N,n,D,dtype,code,page,contexts,windows,counts", TDP)
-def test_tdp_weigh(B, N, n, D, dtype, code, page, contexts, windows, counts):
+def test_tdp_weigh(B, N, n, D, dtype, code, page, contexts, windows, counts, monkeypatch):
     bt = Weighed(B, N, n, D, dtype, code, page, contexts, windows=windows, counts=counts)
     got = bt.run()
     ft.check_status(DEV)
@@ -126,9 +126,11 @@ def test_tdp_weigh(B, N, n, D, dtype, code, page, contexts, windows, counts):
     ft.check_status(DEV)
     assert torch.equal(before.cpu(), bt.before)
     bt.check(out, 0.75, stale=torch.full_like(bt.before, 7.0))
-    # nothing of before counts, whatever it is; the same bits again
-    again = [bt.run(torch.full_like(before, math.nan), torch.zeros_like(before), 0.0) for _ in range(2)]
+    # nothing of before counts, whatever it is; the same bits again, and without the host extension
+    again = [bt.run(torch.full_like(before, math.nan), torch.zeros_like(before), 0.0)]
     bt.check(again[0], 0.0, stale=torch.zeros_like(bt.before))
+    monkeypatch.setattr(_native, "host_weigh", lambda *a: None)
+    again.append(bt.run(torch.full_like(before, math.nan), torch.zeros_like(before), 0.0))
     assert torch.equal(*again)
 
 
@@ -152,7 +154,7 @@ DPS = [  # B N n D dtype code page contexts k_diff counts
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("B,N,n,D,dtype,code,page,contexts,k_diff,counts", DPS)
-def test_dps_weigh(B, N, n, D, dtype, code, page, contexts, k_diff, counts):
+def test_dps_weigh(B, N, n, D, dtype, code, page, contexts, k_diff, counts, monkeypatch):
     bt = Weighed(B, N, n, D, dtype, code, page, contexts, dps=True, k_diff=k_diff, counts=counts)
     got = bt.run()
     ft.check_status(DEV)
@@ -162,8 +164,10 @@ def test_dps_weigh(B, N, n, D, dtype, code, page, contexts, k_diff, counts):
     bt.run(before, out, 0.75, torch.nn.functional.pad(bt.table, (0, 40), value=0))
     ft.check_status(DEV)
     bt.check(out, 0.75, stale=torch.full_like(bt.before, 7.0))
-    again = [bt.run(torch.full_like(before, math.nan), torch.zeros_like(before), 0.0) for _ in range(2)]
+    again = [bt.run(torch.full_like(before, math.nan), torch.zeros_like(before), 0.0)]
     bt.check(again[0], 0.0, stale=torch.zeros_like(bt.before))
+    monkeypatch.setattr(_native, "host_weigh", lambda *a: None)
+    again.append(bt.run(torch.full_like(before, math.nan), torch.zeros_like(before), 0.0))
     assert torch.equal(*again)
 
 
@@ -358,9 +362,12 @@ EVICT = [  # B N D code page contexts keep first recent dps
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("elsewhere", [False, True])
+@pytest.mark.parametrize("elsewhere,host", [(False, True), (True, True), (True, False)])
 @pytest.mark.parametrize("B,N,D,code,page,contexts,keep,first,recent,dps", EVICT)
-def test_evict(B, N, D, code, page, contexts, keep, first, recent, dps, elsewhere):
+def test_evict(B, N, D, code, page, contexts, keep, first, recent, dps, elsewhere, host, monkeypatch):
+    _native.lib()
+    if not host:
+        monkeypatch.setattr(_native, "host_evict", lambda *a: None)
     bt = Full(B, N, D, code, page, contexts, length=max(max(contexts), keep) + 2, dps=dps)
     most = max(contexts)
     before = bt.rows(bt.table, most)
