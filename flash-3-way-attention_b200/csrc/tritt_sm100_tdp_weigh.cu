@@ -9,10 +9,12 @@
 //
 // The line of steps (tritt_weigh.cuh) is cut in equal parts, one for each CTA.
 //   warp 1        walks the line and tells the others each piece (a new token, a tile of k, a range of tiles of j) by a ring in shared memory
-//   warp 0        issues tcgen05.mma: eight or sixteen for a tile, into four buffers of scores in tensor memory in turn
-//   warps 4-7     tiles of K1: 8-bit codes through registers, the next tile's on their way while one is converted; fp16 codes by asynchronous copies
+//   warp 0        issues tcgen05.mma: eight or sixteen for a tile, K1 from tensor memory, into three buffers of scores in turn
+//   warps 2, 3    fetch K1 several tiles ahead, 64 rows of a tile each: pages, exponents, and the codes of what lies in one page by a TMA copy
+//   warps 4-7     turn a row a thread into fp16 and store it in tensor memory (with both operands in shared memory its bandwidth would be all that the products leave nothing of)
 //   warps 8-11    Q for the piece after the present one, and its columns' powers of two
-//   warps 12-19   two warpgroups, 64 columns each: exponentials and sums
+//   warps 12-27   four warpgroups, 32 columns each: exponentials and sums.  Four warps a scheduler: with two, of 64 columns each, registers and the way from a tile's scores to the
+//                 next one's left half of the exponentials' time unused
 #include "tritt_sm100.cuh"
 #include "tritt_weigh.cuh"
 
@@ -20,14 +22,18 @@ namespace tritt {
 namespace {
 using namespace sm100;
 
-constexpr int kThreads = 640;
-constexpr int kRegsLaunch = 96;   // a thread; the warps that sum take what the others give up
-constexpr int kRegsIssue = 40, kRegsLoad = 80, kRegsForm = 88, kRegsSum = 136;
-static_assert(kRegsIssue + kRegsLoad + kRegsForm + 2 * kRegsSum <= 5 * kRegsLaunch, "more registers than the launch has");
-constexpr int kMetas = 8;         // tiles whose rows are described: a stage is written when the products of the tile `stages` back are done, which had waited for the sums of the one four further back
-constexpr int kItems = 4, kConsumers = 17;
-constexpr int kScores = 4;        // buffers of scores
+constexpr int kThreads = 896;
+constexpr int kRegsLaunch = 72;   // a thread; the warps that sum take what the others give up
+constexpr int kRegsIssue = 40, kRegsConvert = 56, kRegsForm = 56, kRegsSum = 88;
+static_assert(kRegsIssue + kRegsConvert + kRegsForm + 4 * kRegsSum <= 7 * kRegsLaunch, "more registers than the launch has");
+constexpr int kSums = 5;          // of a slot: four of the rows, one of the columns
+constexpr int kMetas = 8;         // tiles whose rows are described
+constexpr int kItems = 4;
+constexpr int kScores = 3;        // buffers of scores
 
+// Columns' powers of two join Q as long as the exponents of a warpgroup's 32 lie no further apart than this: Q then has its 22 bits, counted from the largest product of a row, down to fp16's smallest numbers.  Beyond,
+// and where a row is not finite, scores are multiplied column by column.
+template <int CODE> constexpr int kSpread = CODE == TRITT_CODE_F16 ? 13 : CODE == TRITT_CODE_E4M3 ? 9 : 8;
 // q (below 4) times a code times 2^-kDown fits fp16
 template <int CODE> constexpr int kDown = CODE == TRITT_CODE_F16 ? 2 : 0;
 
@@ -39,34 +45,46 @@ struct __align__(16) Item {       // a piece; n < 0: there is no more
   int pad[3];
 };
 struct __align__(16) Meta {       // of a tile of K1
-  uint8_t exponent[128];
-  uint32_t there[4];
+  uint16_t row[128];              // exponent byte; kOff: the new token does not attend to it
 };
+constexpr int kOff = 256;
 struct __align__(16) Columns {    // of a tile of Q
-  float scale[128];
-  uint32_t there[4];
-  int largest[4], field, pad[3];  // exponent bytes that 32 columns' are relative to; q's
+  float scale[128];               // (apart) of scores
+  uint32_t there[4];              // of 32 columns: those that have a place and are attended to
+  int largest[4];                 // the largest of their exponent bytes
+  int apart[4];                   // whether each has its own power of two
+  int field;                      // q's exponent
+  int pad[3];
+};
+template <int D, int CODE> struct Cfg {
+  static constexpr int kTile = 128 * D * 2;
+  static constexpr int kRow = D * (CODE == TRITT_CODE_F16 ? 2 : 1);                      // bytes of a row of codes
+  static constexpr int kPitch = kRow < 128 ? kRow : 128, kBoxes = kRow / kPitch;         // as TMA leaves it: boxes of 64 or 128 bytes
+  static constexpr int kRaw = 128 * kRow;                                                // a tile of codes
+  static constexpr int kDepth = CODE == TRITT_CODE_F16 ? (D == 128 ? 2 : 6) : (D == 128 ? 5 : 8);   // tiles of codes on their way
+  static constexpr int kOperands = D == 128 ? 2 : 4, kOperandCols = D / 2;               // tiles of K1 in tensor memory, behind the scores
+  static constexpr int kTmemA = kScores * 128;
+  static_assert(kTmemA + kOperands * kOperandCols <= 512, "tensor memory");
+  static constexpr int kOffQ = 0;                      // [2][hi, lo]
+  static constexpr int kOffRaw = 4 * kTile;            // [kDepth]
+  static constexpr int kOffMisc = kOffRaw + kDepth * kRaw;
 };
 struct Misc {
-  uint64_t k_full[4], k_empty[4], meta_full[kMetas], q_full[2], q_free[2], s_full[kScores], s_free[kScores], item_full[kItems], item_free[kItems];
+  uint64_t raw_full[8], raw_free[8], a_full[4], a_free[4], meta_full[kMetas], meta_free[kMetas], q_full[2], q_free[2], s_full[kScores], s_free[kScores], item_full[kItems],
+      item_free[kItems];
   Item items[kItems];
   Meta meta[kMetas];
   Columns columns[2];
-  float sums[2][2][4][64];        // [warpgroup][parity of the piece][warp][column]
+  float sums[4][2][4][32];        // [warpgroup][parity of the piece][warp][column]
   long long scan[33], at[2];
   uint32_t tmem_base;
   int abort_flag;
 };
-template <int D> struct Cfg {
-  static constexpr int kTile = 128 * D * 2;
-  static constexpr int kStages = D == 128 ? 2 : 4;
-  static_assert(kStages + kScores <= kMetas, "descriptions of tiles in use");
-  static constexpr int kOffQ = 0;                      // [2][hi, lo]
-  static constexpr int kOffK = 4 * kTile;
-  static constexpr int kOffMisc = kOffK + kStages * kTile;
-  static constexpr int kSmem = kOffMisc + (int)sizeof(Misc);
-  static_assert(kSmem <= 227 * 1024, "shared memory");
-};
+template <int D, int CODE> constexpr int kSmem = Cfg<D, CODE>::kOffMisc + (int)sizeof(Misc);
+constexpr int kConsumers = 1 + 2 + 4 + 4 + 16;   // warps that read an item
+
+__device__ __forceinline__ int most(int x, int y) { return x > y ? x : y; }
+__device__ __forceinline__ int least_of(int x, int y) { return x < y ? x : y; }
 
 __device__ __forceinline__ float2 mul_pair(float2 a, float2 b) {
   float2 r;
@@ -109,16 +127,10 @@ __device__ __forceinline__ uint4 load16_if(const void* p, bool on) {   // zeros 
       : "l"(p), "r"((int)on));
   return v;
 }
-// 16 bytes to shared memory, zeros where not (src is then any address that can be read)
-__device__ __forceinline__ void copy16_if(void* dst, const void* src, bool on) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(on ? 16 : 0) : "memory");
-}
-
 template <typename T, int D, int CODE>
-__global__ void __launch_bounds__(kThreads, 1) tdp_weigh_sm100_kernel(const __grid_constant__ TdpWeighArgs p) {
-  using C = Cfg<D>;
+__global__ void __launch_bounds__(kThreads, 1) tdp_weigh_sm100_kernel(const __grid_constant__ TdpWeighArgs p, const __grid_constant__ CUtensorMap map) {
+  using C = Cfg<D, CODE>;
   using R = RowChunks<D, CODE>;
-  constexpr int NS = C::kStages;
   extern __shared__ __align__(1024) uint8_t smem[];
   Misc& ms = *reinterpret_cast<Misc*>(smem + C::kOffMisc);
   const CacheArgs& a = p.cache;
@@ -129,18 +141,25 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_weigh_sm100_kernel(const __gr
   find_sequence(p, (long long)blockIdx.x * total / weigh_parts(p, total), ms.scan, ms.at);
   if (tid == 32) {
     ms.abort_flag = (smem_u32(smem) & 1023u) != 0;
-    for (int i = 0; i < NS; ++i) {
-      mbar_init(&ms.k_full[i], 128);
-      mbar_init(&ms.k_empty[i], 1);
+    for (int i = 0; i < C::kDepth; ++i) {
+      mbar_init(&ms.raw_full[i], 2);
+      mbar_init(&ms.raw_free[i], 4);
     }
-    for (int i = 0; i < kMetas; ++i) mbar_init(&ms.meta_full[i], 4);
+    for (int i = 0; i < C::kOperands; ++i) {
+      mbar_init(&ms.a_full[i], 128);
+      mbar_init(&ms.a_free[i], 1);
+    }
+    for (int i = 0; i < kMetas; ++i) {
+      mbar_init(&ms.meta_full[i], 2);
+      mbar_init(&ms.meta_free[i], 16);
+    }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&ms.q_full[i], 128);
-      mbar_init(&ms.q_free[i], 9);   // its last products, and eight warps that have read its columns
+      mbar_init(&ms.q_free[i], 17);   // its last products, and sixteen warps that have read its columns
     }
     for (int i = 0; i < kScores; ++i) {
       mbar_init(&ms.s_full[i], 1);
-      mbar_init(&ms.s_free[i], 8);
+      mbar_init(&ms.s_free[i], 16);
     }
     for (int i = 0; i < kItems; ++i) {
       mbar_init(&ms.item_full[i], 1);
@@ -156,10 +175,10 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_weigh_sm100_kernel(const __gr
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = ms.tmem_base;
+  auto uniform = [](int v) -> int { return __reduce_max_sync(0xffffffffu, v); };
+  const uint32_t tmem = (uint32_t)uniform((int)ms.tmem_base);   // (every lane has the same: told so, the compiler keeps the products' addresses on the uniform datapath)
   volatile int* const abort_flag = &ms.abort_flag;
   auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag)); };
-  auto uniform = [](int v) -> int { return __reduce_max_sync(0xffffffffu, v); };
   // the next piece's tiles; negative: there is none, or a wait ran out.  The warp gives its place in the ring back when it has read what it needs.
   auto next_item = [&](int count) -> int {
     if (!wait_all(&ms.item_full[count % kItems], (count / kItems) & 1)) return -1;
@@ -212,8 +231,8 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_weigh_sm100_kernel(const __gr
       };
       constexpr uint32_t idesc = make_idesc_f16(128, 128, 0, false, false);
       constexpr uint32_t kHi = desc_hi(1024);
-      const uint32_t qLo = desc_lo(smem_u32(smem + C::kOffQ), 16), kLo = desc_lo(smem_u32(smem + C::kOffK), 16);
-      int kst = 0, kph = 0, pieces = 0;
+      const uint32_t qLo = desc_lo(smem_u32(smem + C::kOffQ), 16);
+      int pieces = 0;
       uint32_t tiles = 0;
       bool alive = true;
       for (int count = 0; alive; ++count) {
@@ -224,150 +243,155 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_weigh_sm100_kernel(const __gr
         const int buf = pieces & 1;
         alive = wait_all(&ms.q_full[buf], (pieces >> 1) & 1);
         for (int i = 0; i < n && alive; ++i, ++tiles) {
-          const uint32_t sb = tiles % kScores;
-          alive = wait_all(&ms.k_full[kst], kph) && wait_all(&ms.s_free[sb], ((tiles / kScores) & 1) ^ 1);
+          const uint32_t sb = tiles % kScores, ab = tiles % C::kOperands;
+          alive = wait_all(&ms.a_full[ab], (tiles / C::kOperands) & 1) && wait_all(&ms.s_free[sb], ((tiles / kScores) & 1) ^ 1);
           if (!alive) break;
           tc_fence_after();
-          const uint32_t aLo = kLo + kst * (C::kTile >> 4), bLo = qLo + buf * (2 * C::kTile >> 4), to = tmem + sb * 128;
+          const uint32_t a_at = tmem + C::kTmemA + ab * C::kOperandCols, bLo = qLo + buf * (2 * C::kTile >> 4), to = tmem + sb * 128;
           if (leader) {
 #pragma unroll
             for (int k = 0; k < D / 8; ++k) {
-              const uint32_t s = k % (D / 16), kk = (s >> 2) * (16384 >> 4) + (s & 3) * 2;
-              mma_ss_lo(to, aLo + kk, bLo + (k / (D / 16)) * (C::kTile >> 4) + kk, kHi, idesc, k > 0);
+              const uint32_t s = k % (D / 16);
+              mma_ts_lo(to, a_at + s * 8, bLo + (k / (D / 16)) * (C::kTile >> 4) + (s >> 2) * (16384 >> 4) + (s & 3) * 2, kHi, idesc, k > 0);
             }
           }
-          commit(&ms.k_empty[kst]);
+          commit(&ms.a_free[ab]);
           commit(&ms.s_full[sb]);
           if (i == n - 1) commit(&ms.q_free[buf]);
-          if (++kst == NS) kst = 0, kph ^= 1;
         }
         ++pieces;
       }
-    }
-  } else if (warp < 8) {
-    set_regs<kRegsLaunch, kRegsLoad>();
-    // ------------------------------------------------------------------ tiles of K1
-    const int w = warp & 3;
-    uint8_t* const ring = smem + C::kOffK;
-    const int chunk = lane % R::kChunks, row0 = lane / R::kChunks;
-    int st = 0, ph = 0;
-    uint32_t tiles = 0;
-    bool alive = true;
-    // a lane's own row of a tile: its address (null: not there, or nobody looks at it), its exponent, and where it is described
-    const uint8_t* mine = nullptr;
-    int exponent = 0;
-    auto find = [&](const Item& it, int x) {
-      Place at{-1, 0};
-      if (x >= it.j_lo && x <= it.pos) {
-        at = place_of(a, it.b, x);
-        if (at.page < 0 && a.status) atomicOr(a.status, kStatusPlace);
-      }
-      mine = nullptr;
-      exponent = 0;
-      if (at.page >= 0) {
-        const size_t r = row_of(a, at, kPartK1, it.head);
-        mine = codes + r * R::kBytes;
-        exponent = __ldg(a.c.exponents + r);
-      }
-    };
-    auto describe = [&](bool there, int e) {
-      Meta& m = ms.meta[tiles % kMetas];
-      m.exponent[w * 32 + lane] = (uint8_t)e;
-      const uint32_t word = __ballot_sync(0xffffffffu, there);
-      if (lane == 0) m.there[w] = word;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&ms.meta_full[tiles % kMetas]);
-    };
-    if constexpr (CODE == TRITT_CODE_F16) {
-      // the codes are the operand: copied as they are, a tile behind the one that is waited for
-      bool waiting = false;
-      auto finish = [&](int stage, bool last) {   // the tile of that stage has come
-        if (last)
-          asm volatile("cp.async.wait_group 0;" ::: "memory");
-        else
-          asm volatile("cp.async.wait_group 1;" ::: "memory");
-        fence_async_smem();
-        mbar_arrive(&ms.k_full[stage]);
-      };
-      for (int count = 0; alive; ++count) {
-        const int n = next_item(count);
-        if (n < 0) break;
-        const Item it = ms.items[count % kItems];
-        free_item(count);
-        for (int i = 0; i < n && alive; ++i, ++tiles) {
-          find(it, (it.s0 + i) * 128 + w * 32 + lane);
-          if (waiting && NS == 2 && !__all_sync(0xffffffffu, mbar_test(&ms.k_empty[st], ph ^ 1))) {   // (with two stages the one to be filled may wait for the one on its way)
-            finish(st ? st - 1 : NS - 1, true);
-            waiting = false;
-          }
-          alive = wait_all(&ms.k_empty[st], ph ^ 1);
-          if (!alive) break;
-          uint8_t* const tile = ring + st * C::kTile;
-#pragma unroll
-          for (int k = 0; k < R::kChunks; ++k) {
-            const int row = row0 + k * R::kStep;
-            const uint8_t* from = R::row(mine, row);
-            copy16_if(tile + (chunk >> 3) * 16384 + swz128(w * 32 + row, chunk & 7), from ? from + chunk * 16 : codes, from != nullptr);
-          }
-          asm volatile("cp.async.commit_group;" ::: "memory");
-          describe(mine != nullptr, exponent);
-          if (waiting) finish(st ? st - 1 : NS - 1, false);
-          waiting = true;
-          if (++st == NS) st = 0, ph ^= 1;
-        }
-        // (a piece's last tile is not left waiting for the next piece)
-        if (waiting && alive) finish(st ? st - 1 : NS - 1, true);
-        waiting = false;
-      }
-      asm volatile("cp.async.wait_group 0;" ::: "memory");
     } else {
-      uint4 now[R::kChunks];
+      // ------------------------------------------------------------------ K1 on its way
+      // A lane has two rows of 64.  Pages are looked up three tiles ahead of the copies, exponents read one ahead.
+      const int r0 = (warp - 2) * 64 + lane * 2;
+      const int seg_log2 = a.page_log2 < 6 ? a.page_log2 : 6, seg = 1 << seg_log2;   // rows that lie in one page, ...
+      const int lanes = seg / 2, lane0 = lane & ~(lanes - 1);                        // ... which neighbouring lanes have
+      const uint32_t mask = lanes == 32 ? 0xffffffffu : (1u << lanes) - 1;
+      uint32_t tiles = 0;
+      bool alive = true;
+      if (lane == 0) tma_prefetch_desc(&map);
       for (int count = 0; alive; ++count) {
         const int n = next_item(count);
         if (n < 0) break;
         const Item it = ms.items[count % kItems];
         free_item(count);
         if (n == 0) continue;
-        auto load = [&](uint4 (&v)[R::kChunks]) {
-#pragma unroll
-          for (int k = 0; k < R::kChunks; ++k) {
-            const uint8_t* from = R::row(mine, row0 + k * R::kStep);
-            v[k] = load16_if(from + chunk * 16, from != nullptr);
-          }
+        const int x0 = it.s0 * 128 + r0;
+        // the page of the lane's rows of the piece's i-th tile, as the table has it (not looked at here, so that nothing waits for it); -1: nobody looks at them, or the table has none
+        auto attended = [&](int i) { return i < n && x0 + i * 128 + 1 >= it.j_lo && x0 + i * 128 <= it.pos; };
+        auto page_of = [&](int i) {
+          const int at = (x0 + i * 128) >> a.page_log2;
+          int page = -1;
+          if (attended(i) && at < a.c.table_pages) page = __ldg(a.c.table + it.b * a.c.table_stride + at);
+          return page;
         };
-        find(it, it.s0 * 128 + w * 32 + lane);
-        load(now);
-        for (int i = 0; i < n && alive; ++i, ++tiles) {
-          const bool there = mine != nullptr;
-          const int e = exponent;
-          if (i + 1 < n) find(it, (it.s0 + i + 1) * 128 + w * 32 + lane);
-          alive = wait_all(&ms.k_empty[st], ph ^ 1);
-          if (!alive) break;
-          uint8_t* const tile = ring + st * C::kTile;
-          describe(there, e);
-#pragma unroll
-          for (int k = 0; k < R::kChunks; ++k) {
-            const int row = w * 32 + row0 + k * R::kStep;
-            uint4 lo, hi;
-            bytes_to_halves<CODE>(now[k].x, lo.x, lo.y);
-            bytes_to_halves<CODE>(now[k].y, lo.z, lo.w);
-            bytes_to_halves<CODE>(now[k].z, hi.x, hi.y);
-            bytes_to_halves<CODE>(now[k].w, hi.z, hi.w);
-            *reinterpret_cast<uint4*>(tile + (chunk >> 2) * 16384 + swz128(row, 2 * chunk & 7)) = lo;
-            *reinterpret_cast<uint4*>(tile + (chunk >> 2) * 16384 + swz128(row, (2 * chunk + 1) & 7)) = hi;
+        struct Two {
+          size_t row;
+          uint32_t exponents;
+          bool there;
+        };
+        auto read = [&](int i, int page) {
+          Two t{0, 0, page >= 0 && page < a.c.pages};
+          if (t.there) {
+            t.row = row_of(a, Place{page, (x0 + i * 128) & (a.c.page_size - 1)}, kPartK1, it.head);
+            t.exponents = __ldg(reinterpret_cast<const uint16_t*>(a.c.exponents + t.row));
+          } else if (attended(i) && a.status) {
+            atomicOr(a.status, kStatusPlace);
           }
-          if (i + 1 < n) load(now);
-          fence_async_smem();
-          mbar_arrive(&ms.k_full[st]);
-          if (++st == NS) st = 0, ph ^= 1;
+          return t;
+        };
+        Two now = read(0, page_of(0));
+        int page1 = page_of(1), page2 = page_of(2);
+        for (int i = 0; i < n && alive; ++i, ++tiles) {
+          const int page3 = page_of(i + 3);
+          const Two next = read(i + 1, page1);
+          const uint32_t slot = tiles % C::kDepth, mt = tiles % kMetas;
+          alive = wait_all(&ms.raw_free[slot], ((tiles / C::kDepth) & 1) ^ 1) && wait_all(&ms.meta_free[mt], ((tiles / kMetas) & 1) ^ 1);
+          if (!alive) break;
+          const uint32_t found = __ballot_sync(0xffffffffu, now.there);
+          uint32_t bytes = 0;
+          for (int l = 0; l < 32; l += lanes)
+            if (found >> l & mask) bytes += seg * C::kRow;
+          if (lane == 0) mbar_arrive_expect_tx(&ms.raw_full[slot], bytes);
+          const uint32_t of = found >> lane0 & mask;
+          if (of && lane == lane0 + __ffs(of) - 1) {   // (all of the page's rows that the tile has may be read, whether somebody looks at them or not)
+            const int at = r0 & ~(seg - 1);
+            uint8_t* const to = smem + C::kOffRaw + slot * C::kRaw + at * C::kPitch;
+#pragma unroll
+            for (int x = 0; x < C::kBoxes; ++x)   // (the cache has fewer than 2^31 rows: one has 64 bytes at least)
+              tma_load_3d(to + x * 128 * C::kPitch, &map, &ms.raw_full[slot], x * 64, (int)(now.row - (r0 - at)), 0);
+          }
+          const int x = x0 + i * 128;
+          const uint32_t lo = now.there && x >= it.j_lo && x <= it.pos ? now.exponents & 255 : kOff;
+          const uint32_t hi = now.there && x + 1 >= it.j_lo && x + 1 <= it.pos ? now.exponents >> 8 : kOff;
+          *reinterpret_cast<uint32_t*>(&ms.meta[mt].row[r0]) = lo | hi << 16;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ms.meta_full[mt]);
+          now = next;
+          page1 = page2;
+          page2 = page3;
         }
+      }
+      if (*abort_flag) {   // give copies still in flight a bounded chance to land before the CTA retires
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000) {
+        }
+      }
+    }
+  } else if (warp < 8) {
+    set_regs<kRegsLaunch, kRegsConvert>();
+    // ------------------------------------------------------------------ codes to fp16 in tensor memory: a row a thread
+    const int row = tid - 128;
+    const uint32_t t_lane = (uint32_t)(warp & 3) << 21;
+    uint32_t tiles = 0;
+    bool alive = true;
+    for (int count = 0; alive; ++count) {
+      const int n = next_item(count);
+      if (n < 0) break;
+      free_item(count);
+      for (int i = 0; i < n && alive; ++i, ++tiles) {
+        const uint32_t ab = tiles % C::kOperands, slot = tiles % C::kDepth;
+        alive = wait_all(&ms.raw_full[slot], (tiles / C::kDepth) & 1) && wait_all(&ms.a_free[ab], ((tiles / C::kOperands) & 1) ^ 1);
+        if (!alive) break;
+        tc_fence_after();
+        const uint8_t* const from = smem + C::kOffRaw + slot * C::kRaw;
+        const uint32_t to = tmem + C::kTmemA + ab * C::kOperandCols + t_lane;
+        auto chunk = [&](int c) {   // 16 bytes of the thread's row
+          const uint32_t off = (c * 16 / C::kPitch) * (128 * C::kPitch) + row * C::kPitch + c * 16 % C::kPitch;
+          return *reinterpret_cast<const uint4*>(from + (off ^ (off >> 7 & (C::kPitch / 16 - 1)) << 4));   // (swizzled)
+        };
+        constexpr int kParts = D / 32;   // of 32 elements, 16 columns of tensor memory
+#pragma unroll
+        for (int h = 0; h < kParts; ++h) {
+          uint32_t v[16];
+          constexpr int kEach = C::kRow / kParts / 16;
+#pragma unroll
+          for (int c = 0; c < kEach; ++c) {
+            const uint4 x = chunk(h * kEach + c);
+            if constexpr (CODE == TRITT_CODE_F16) {
+              v[4 * c] = x.x, v[4 * c + 1] = x.y, v[4 * c + 2] = x.z, v[4 * c + 3] = x.w;
+            } else {
+              bytes_to_halves<CODE>(x.x, v[8 * c], v[8 * c + 1]);
+              bytes_to_halves<CODE>(x.y, v[8 * c + 2], v[8 * c + 3]);
+              bytes_to_halves<CODE>(x.z, v[8 * c + 4], v[8 * c + 5]);
+              bytes_to_halves<CODE>(x.w, v[8 * c + 6], v[8 * c + 7]);
+            }
+          }
+          tmem_st16(to + h * 16, v);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ms.raw_free[slot]);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&ms.a_full[ab]);
       }
     }
   } else if (warp < 12) {
     set_regs<kRegsLaunch, kRegsForm>();
     // ------------------------------------------------------------------ Q
     const int w = warp & 3, chunk = lane % R::kChunks, row0 = lane / R::kChunks;
-    constexpr int kEach = CODE == TRITT_CODE_F16 ? 8 : 16, kAtOnce = R::kChunks < 8 ? R::kChunks : 8;   // elements of a chunk; chunks on their way together
+    constexpr int kEach = CODE == TRITT_CODE_F16 ? 8 : 16, kAtOnce = 4;   // elements of a chunk; chunks on their way together
     int pieces = 0;
     bool alive = true;
     for (int count = 0; alive; ++count) {
@@ -400,28 +424,33 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_weigh_sm100_kernel(const __gr
       uint32_t top = 0;
 #pragma unroll
       for (int e = 0; e < kEach; ++e) top = max(top, __float_as_uint(q[e]) & 0x7fffffffu);
-      const int field = (int)(__reduce_max_sync(0xffffffffu, top) >> 23), largest = uniform(byte == 255 ? 0 : byte);
+      const int field = (int)(__reduce_max_sync(0xffffffffu, top) >> 23);
       const float up = to_operand(field) * (1.f / (1 << kDown<CODE>));
 #pragma unroll
       for (int e = 0; e < kEach; ++e) q[e] = field == 255 ? 0.f : q[e] * up;
       const uint32_t there = __ballot_sync(0xffffffffu, mine != nullptr);
       alive = wait_all(&ms.q_free[buf], ((pieces >> 1) & 1) ^ 1);
       if (!alive) break;
+      const int largest = uniform(byte), least = -uniform(-least_byte(byte));   // (least: 255 if all rows are zeros)
+      const bool apart = largest == 255 || (least < 255 && largest - least > kSpread<CODE>);
+      // (a row that is not finite has 255: the others' are relative to 254 then, for what they are worth beside a NaN)
+      const float own_scale = mine == nullptr || byte <= 1 ? 1.f : byte == 255 ? __uint_as_float(0x7fffffffu) : power_of_two(byte - least_of(largest, 254));
       Columns& col = ms.columns[buf];
-      col.scale[w * 32 + lane] = mine == nullptr ? 0.f : byte == 255 ? __uint_as_float(0x7fffffffu) : power_of_two(byte - largest);
+      col.scale[w * 32 + lane] = own_scale;
       if (lane == 0) {
         col.there[w] = there;
-        col.largest[w] = largest;
+        col.largest[w] = least_of(largest, 254);
+        col.apart[w] = apart;
         col.field = field;   // (all four warps the same)
       }
       uint8_t* const hi_tile = smem + C::kOffQ + buf * 2 * C::kTile;
       uint8_t* const lo_tile = hi_tile + C::kTile;
-      auto put = [&](int row, int at16, const uint32_t (&h)[4], int e0) {   // eight elements, 16 bytes of either number
+      auto put = [&](int row, int at16, const uint32_t (&h)[4], int e0, float by) {   // eight elements, 16 bytes of either number
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[x]));
-          const float va = q[e0 + 2 * x] * f.x, vb = q[e0 + 2 * x + 1] * f.y;
+          const float va = q[e0 + 2 * x] * f.x * by, vb = q[e0 + 2 * x + 1] * f.y * by;
           hi[x] = pack_halves(va, vb);
           lo[x] = pack_rests(va, vb, hi[x]);
         }
@@ -440,17 +469,18 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_weigh_sm100_kernel(const __gr
 #pragma unroll
         for (int x = 0; x < kAtOnce; ++x) {
           const int row = w * 32 + row0 + (k0 + x) * R::kStep;
+          const float by = __shfl_sync(0xffffffffu, apart ? 1.f : own_scale, row0 + (k0 + x) * R::kStep);
           if constexpr (CODE == TRITT_CODE_F16) {
             const uint32_t h[4] = {v[x].x, v[x].y, v[x].z, v[x].w};
-            put(row, chunk, h, 0);
+            put(row, chunk, h, 0, by);
           } else {
             uint32_t h[4];
             bytes_to_halves<CODE>(v[x].x, h[0], h[1]);
             bytes_to_halves<CODE>(v[x].y, h[2], h[3]);
-            put(row, 2 * chunk, h, 0);
+            put(row, 2 * chunk, h, 0, by);
             bytes_to_halves<CODE>(v[x].z, h[0], h[1]);
             bytes_to_halves<CODE>(v[x].w, h[2], h[3]);
-            put(row, 2 * chunk + 1, h, kEach / 2);
+            put(row, 2 * chunk + 1, h, kEach / 2, by);
           }
         }
       }
@@ -460,9 +490,9 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_weigh_sm100_kernel(const __gr
     }
   } else {
     set_regs<kRegsLaunch, kRegsSum>();
-    // ------------------------------------------------------------------ sums: a row a thread, 64 columns
+    // ------------------------------------------------------------------ sums: a row a thread, 32 columns
     const int wg = (warp - 12) / 4, wq = warp & 3, row = wq * 32 + lane;
-    const uint32_t t_lane = (uint32_t)(wq * 32) << 16;
+    const uint32_t t_col = tmem + wg * 32 + ((uint32_t)(wq * 32) << 16);
     int pieces = 0;
     uint32_t tiles = 0;
     bool alive = true;
@@ -470,112 +500,105 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_weigh_sm100_kernel(const __gr
       const int n = next_item(count);
       if (n < 0) break;
       const Item& it = ms.items[count % kItems];
-      const int pos = it.pos, base = it.base, s0 = it.s0, k0 = it.kg * 128 + wg * 64, k_lo = it.k_lo, j_lo = it.j_lo;
+      const int pos = it.pos, base = it.base, last = it.last, s0 = it.s0, k0 = it.kg * 128 + wg * 32, k_lo = it.k_lo;
       const float minus = -it.minus;
       float* const slot = weigh_slot(p, it.b, it.head);
       float* const row_sums = slot + (size_t)wg * p.span;   // (each thread's own rows, here and where they are cleared)
-      float* const col_sums = slot + (size_t)2 * p.span;
+      float* const col_sums = slot + (size_t)4 * p.span;
       if (it.fresh) {
-        for (int x = row; x <= it.last - base; x += 128) row_sums[x] = 0.f;
-        if (row < 64)
-          for (int x = wg * 64 + row; x <= it.last - base; x += 128) col_sums[x] = 0.f;
+        for (int x = row; x <= last - base; x += 128) row_sums[x] = 0.f;
+        if (row < 32)
+          for (int x = wg * 32 + row; x <= last - base; x += 128) col_sums[x] = 0.f;
       }
-      const int last = it.last;
       free_item(count);
       if (n == 0) continue;
       const int buf = pieces & 1;
       alive = wait_all(&ms.q_full[buf], (pieces >> 1) & 1);
       if (!alive) break;
       const Columns& col = ms.columns[buf];
-      const uint32_t there0 = col.there[2 * wg], there1 = col.there[2 * wg + 1];
-      const int field = col.field, power0 = col.largest[2 * wg] + field - 382 + kDown<CODE>, power1 = col.largest[2 * wg + 1] + field - 382 + kDown<CODE>;
-      const bool all_there = (there0 & there1) == 0xffffffffu;
-      float2 column[32];
+      const uint32_t there = col.there[wg];
+      const int field = col.field;
+      const bool apart = col.apart[wg];
+      // what a row's scores are multiplied by: its power of two with that of the columns, q and Q (beyond fp32's range scores have no use for), and the scale
+      const int power = col.largest[wg] + field - 382 + 127 + kDown<CODE>;
+      const float scale = field == 255 ? __uint_as_float(0x7fffffffu) : field == 0 ? 0.f : p.scale2;
+      const bool all_there = there == 0xffffffffu && !apart;
+      float2 column[16];
 #pragma unroll
-      for (int c = 0; c < 32; ++c) column[c] = make_float2(0.f, 0.f);
+      for (int c = 0; c < 16; ++c) column[c] = make_float2(0.f, 0.f);
       for (int i = 0; i < n; ++i, ++tiles) {
         const uint32_t sb = tiles % kScores, mt = tiles % kMetas;
         const int j = (s0 + i) * 128 + row;
-        float* const mine = row_sums + (j - base);
-        const float before = j <= last ? *mine : 0.f;
-        alive = wait_all(&ms.meta_full[mt], (tiles / kMetas) & 1);
-        if (!alive) break;
-        const int e = ms.meta[mt].exponent[row];
-        const bool on = (ms.meta[mt].there[wq] >> lane & 1) && j >= j_lo && j <= pos;
-        // the row's power of two with that of the columns, q and Q (beyond fp32's range scores have no use for)
-        auto factor = [&](int power) {
-          power += e;
-          power = power < -126 ? -126 : power > 127 ? 127 : power;
-          return e == 255 || field == 255 ? __uint_as_float(0x7fffffffu) : field == 0 ? 0.f : p.scale2 * power_of_two(power);
-        };
-        const float f0 = factor(power0), f1 = factor(power1);
-        const int c_lo = (k_lo > j - p.kkr ? k_lo : j - p.kkr) - k0, c_hi = on ? (p.kkl < pos - j ? j + p.kkl : pos) - k0 : -1;
-        const bool plain = __all_sync(0xffffffffu, all_there && c_lo <= 0 && c_hi >= 63);
         alive = wait_all(&ms.s_full[sb], (tiles / kScores) & 1);
         if (!alive) break;
         tc_fence_after();
-        float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
-        auto half = [&](int h, float f, auto masked) {
-          uint32_t s[32];
-          tmem_ld32(tmem + sb * 128 + wg * 64 + h * 32 + t_lane, s);
-          // bits of the columns that the row has pairs with
-          uint32_t seen = 0xffffffffu;
-          if constexpr (masked.value) {
-            const int lo = c_lo - h * 32, hi = c_hi - h * 32;
-            seen = h ? there1 : there0;
-            if (lo > 0) seen &= lo > 31 ? 0u : 0xffffffffu << lo;
-            if (hi < 31) seen &= hi < 0 ? 0u : 0xffffffffu >> (31 - hi);
-          }
-          tmem_wait_ld(s);
-          if (h) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&ms.s_free[sb]);
-          }
-          const float4* by = reinterpret_cast<const float4*>(col.scale + wg * 64 + h * 32);
-#pragma unroll
-          for (int c = 0; c < 32; c += 4) {
-            const float4 g = by[c / 4];
-            float2 x = fma_pair(mul_pair(make_float2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), make_float2(g.x, g.y)), f, minus);
-            float2 y = fma_pair(mul_pair(make_float2(__uint_as_float(s[c + 2]), __uint_as_float(s[c + 3])), make_float2(g.z, g.w)), f, minus);
-            x.x = exp2f(x.x), x.y = exp2f(x.y), y.x = exp2f(y.x), y.y = exp2f(y.y);
-            if constexpr (masked.value) {
-              x.x = seen >> c & 1 ? x.x : 0.f, x.y = seen >> (c + 1) & 1 ? x.y : 0.f;
-              y.x = seen >> (c + 2) & 1 ? y.x : 0.f, y.y = seen >> (c + 3) & 1 ? y.y : 0.f;
-            }
-            sum0 = add_pair(sum0, x);
-            sum1 = add_pair(sum1, y);
-            column[h * 16 + c / 2] = add_pair(column[h * 16 + c / 2], x);
-            column[h * 16 + c / 2 + 1] = add_pair(column[h * 16 + c / 2 + 1], y);
-          }
-        };
-        if (plain) {
-          half(0, f0, std::false_type{});
-          half(1, f1, std::false_type{});
-        } else {
-          half(0, f0, std::true_type{});
-          half(1, f1, std::true_type{});
+        uint32_t s[32];
+        tmem_ld32(t_col + sb * 128, s);
+        // the thread's row, beside the load
+        alive = wait_all(&ms.meta_full[mt], (tiles / kMetas) & 1);
+        if (!alive) break;
+        const int e = ms.meta[mt].row[row], f = least_of(most((e & 255) + power, 1), 254);
+        const float factor = (e & 255) == 255 ? __uint_as_float(0x7fffffffu) : scale * __uint_as_float((uint32_t)f << 23);
+        const int c_lo = most(k_lo, j - p.kkr) - k0, c_hi = e < kOff ? (p.kkl < pos - j ? j + p.kkl : pos) - k0 : -1;   // columns that it has pairs with
+        const bool plain = __all_sync(0xffffffffu, all_there && c_lo <= 0 && c_hi >= 31);
+        tmem_wait_ld(s);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&ms.s_free[sb]);
+          mbar_arrive(&ms.meta_free[mt]);
         }
-        if (j <= last) *mine = before + ((sum0.x + sum0.y) + (sum1.x + sum1.y));
+        float2 x[16];
+#pragma unroll
+        for (int c = 0; c < 16; ++c) x[c] = make_float2(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1]));
+        if (plain) {
+#pragma unroll
+          for (int c = 0; c < 16; ++c) x[c] = fma_pair(x[c], factor, minus);
+        } else {   // scores of pairs that there are not become minus infinity; where columns' exponents are apart, each has its own factor
+          uint32_t seen = there;
+          if (c_lo > 0) seen &= c_lo > 31 ? 0u : 0xffffffffu << c_lo;
+          if (c_hi < 31) seen &= c_hi < 0 ? 0u : 0xffffffffu >> (31 - c_hi);
+          if (apart) {
+            const float2* by = reinterpret_cast<const float2*>(col.scale + wg * 32);
+#pragma unroll
+            for (int c = 0; c < 16; ++c) x[c] = mul_pair(x[c], by[c]);
+          }
+#pragma unroll
+          for (int c = 0; c < 16; ++c) {
+            x[c] = fma_pair(x[c], factor, minus);
+            x[c].x = seen >> (2 * c) & 1 ? x[c].x : -INFINITY;
+            x[c].y = seen >> (2 * c + 1) & 1 ? x[c].y : -INFINITY;
+          }
+        }
+        float2 sum[2];
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+          x[c].x = exp2f(x[c].x), x[c].y = exp2f(x[c].y);
+          sum[c % 2] = c < 2 ? x[c] : add_pair(sum[c % 2], x[c]);
+          column[c] = add_pair(column[c], x[c]);
+        }
+        const float2 both = add_pair(sum[0], sum[1]);
+        // (no thread but this one adds to the place, in order)
+        if (j <= last) asm volatile("red.relaxed.gpu.global.add.f32 [%0], %1;" ::"l"(row_sums + (j - base)), "f"(both.x + both.y) : "memory");
       }
       if (!alive) break;
       __syncwarp();
       if (lane == 0) mbar_arrive(&ms.q_free[buf]);
-      // the columns' sums over the rows: halves change hands within the warp until a lane has columns 2 lane and the next; then over the four warps
+      // the columns' sums over the rows: halves change hands within the warp until a lane has one column; then over the four warps
       float* v = reinterpret_cast<float*>(column);
 #pragma unroll
       for (int h = 16; h > 0; h >>= 1) {
         const bool upper = lane & h;
 #pragma unroll
-        for (int x = 0; x < 2 * h; ++x) {
-          const float give = upper ? v[x] : v[x + 2 * h], keep = upper ? v[x + 2 * h] : v[x];
+        for (int x = 0; x < h; ++x) {
+          const float give = upper ? v[x] : v[x + h], keep = upper ? v[x + h] : v[x];
           v[x] = keep + __shfl_xor_sync(0xffffffffu, give, h);
         }
       }
-      float(&sums)[4][64] = ms.sums[wg][buf];
-      *reinterpret_cast<float2*>(&sums[wq][2 * lane]) = make_float2(v[0], v[1]);
+      float(&sums)[4][32] = ms.sums[wg][buf];
+      sums[wq][lane] = v[0];
       named_bar_sync(1 + wg, 128);   // (the other parity's numbers have been read by then)
-      if (row < 64 && k0 + row <= last) col_sums[k0 + row - base] += (sums[0][row] + sums[1][row]) + (sums[2][row] + sums[3][row]);
+      if (row < 32 && k0 + row <= last) col_sums[k0 + row - base] += (sums[0][row] + sums[1][row]) + (sums[2][row] + sums[3][row]);
       ++pieces;
     }
   }
@@ -588,8 +611,20 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_weigh_sm100_kernel(const __gr
 }
 
 template <typename T, int D, int CODE> int launch(const TdpWeighArgs& p, cudaStream_t stream) {
-  TRITT_CUDA_OK(cudaFuncSetAttribute(tdp_weigh_sm100_kernel<T, D, CODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmem));
-  tdp_weigh_sm100_kernel<T, D, CODE><<<p.ctas, kThreads, Cfg<D>::kSmem, stream>>>(p);
+  using C = Cfg<D, CODE>;
+  const tritt_cache_t& c = p.cache.c;
+  // all rows of the cache, boxes of what a page has of 64 rows
+  CUtensorMap map{};
+  if (int rc = make_tmap_codes(&map, c.codes, C::kRow, (uint64_t)c.pages * 4 * c.N * c.page_size, C::kPitch, c.page_size < 64 ? c.page_size : 64)) return rc;
+  // (warpgroups share out the registers that the kernel is launched with: with fewer those that raise their count would wait for good)
+  cudaFuncAttributes attr;
+  TRITT_CUDA_OK(cudaFuncGetAttributes(&attr, tdp_weigh_sm100_kernel<T, D, CODE>));
+  if (attr.numRegs != kRegsLaunch) {
+    set_error("the weights' kernel was built for %d registers a thread instead of %d", attr.numRegs, kRegsLaunch);
+    return -30;
+  }
+  TRITT_CUDA_OK(cudaFuncSetAttribute(tdp_weigh_sm100_kernel<T, D, CODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem<D, CODE>));
+  tdp_weigh_sm100_kernel<T, D, CODE><<<p.ctas, kThreads, kSmem<D, CODE>, stream>>>(p, map);
   count_launch();
   TRITT_CUDA_OK(cudaGetLastError());
   return 0;

@@ -334,7 +334,7 @@ int tritt_tdp_weigh(const tritt_cache_t* c, const tritt_weights_t* w, const trit
   TdpWeighArgs p{cache_args(*c, status_word), *w, *q, lse, dtype, window(k1_window), window(k2_window), window(kk_left), window(kk_right), alpha * kLog2e,
                  (float*)workspace, kWeighCtas, weigh_span(*c, window(k1_window), window(k2_window)), 0};
   const bool fast = sm100_tdp_weigh_supported(c->D);
-  p.sums = fast ? 3 : 2;
+  p.sums = fast ? 5 : 2;
   if (int rc = fast ? sm100_tdp_weigh(p, (cudaStream_t)stream) : mma_tdp_weigh(p, (cudaStream_t)stream)) return rc;
   return launch_tdp_weigh_join(p, (cudaStream_t)stream);
 }

@@ -168,7 +168,7 @@ inline int weigh_span(const tritt_cache_t& c, int k1w, int k2w) {
   if (reach < tokens) tokens = reach;
   return (int)((tokens + 127) / 128 * 128);
 }
-constexpr int kWeighCtas = 148, kWeighSums = 3;   // the most sums of a slot
+constexpr int kWeighCtas = 148, kWeighSums = 5;   // the most sums of a slot
 
 // Sum of v over the block's threads, and the sum of those before this one.  `tmp`: 33 numbers of shared memory; all threads call it.
 __device__ __forceinline__ long long block_scan(long long v, long long* tmp, long long& total) {
@@ -311,7 +311,7 @@ __device__ __forceinline__ float* weigh_slot(const TdpWeighArgs& a, int b, int h
   return a.part + ((size_t)blockIdx.x + (size_t)b * a.cache.c.N + head) * a.sums * a.span;
 }
 
-// on the tensor cores (head dimension 64 or 128; three sums a slot), and with warp-level matrix instructions (two)
+// on the tensor cores (head dimension 64 or 128; five sums a slot), and with warp-level matrix instructions (two)
 bool sm100_tdp_weigh_supported(int D);
 int sm100_tdp_weigh(const TdpWeighArgs& a, cudaStream_t stream);
 int mma_tdp_weigh(const TdpWeighArgs& a, cudaStream_t stream);
