@@ -10,7 +10,7 @@
 // The line of steps (tritt_weigh.cuh) is cut in equal parts, one for each CTA.
 //   warp 1        walks the line and tells the others each piece (a new token, a tile of k, a range of tiles of j) by a ring in shared memory
 //   warp 0        issues tcgen05.mma: eight or sixteen for a tile, K1 from tensor memory, into three buffers of scores in turn
-//   warps 2, 3    fetch K1 several tiles ahead, 64 rows of a tile each: pages, exponents, and the codes of what lies in one page by a TMA copy
+//   warps 2, 3    fetch tiles of K1 in turn, several ahead: pages, exponents, and the codes of what lies in one page by a TMA copy
 //   warps 4-7     turn a row a thread into fp16 and store it in tensor memory (with both operands in shared memory its bandwidth would be all that the products leave nothing of)
 //   warps 8-11    Q for the piece after the present one, and its columns' powers of two
 //   warps 12-27   four warpgroups, 32 columns each: exponentials and sums.  Four warps a scheduler: with two, of 64 columns each, registers and the way from a tile's scores to the
@@ -27,7 +27,7 @@ constexpr int kRegsLaunch = 72;   // a thread; the warps that sum take what the 
 constexpr int kRegsIssue = 40, kRegsConvert = 56, kRegsForm = 56, kRegsSum = 88;
 static_assert(kRegsIssue + kRegsConvert + kRegsForm + 4 * kRegsSum <= 7 * kRegsLaunch, "more registers than the launch has");
 constexpr int kSums = 5;          // of a slot: four of the rows, one of the columns
-constexpr int kMetas = 8;         // tiles whose rows are described
+constexpr int kMetas = 16;        // tiles whose rows are described
 constexpr int kItems = 4;
 constexpr int kScores = 3;        // buffers of scores
 
@@ -45,9 +45,9 @@ struct __align__(16) Item {       // a piece; n < 0: there is no more
   int pad[3];
 };
 struct __align__(16) Meta {       // of a tile of K1
-  uint16_t row[128];              // exponent byte; kOff: the new token does not attend to it
+  uint16_t row[128];              // exponent byte; kOff: the new token does not attend to it; kPlain: it attends to all of the tile's, and they are finite
 };
-constexpr int kOff = 256;
+constexpr int kOff = 256, kPlain = 512;
 struct __align__(16) Columns {    // of a tile of Q
   float scale[128];               // (apart) of scores
   uint32_t there[4];              // of 32 columns: those that have a place and are attended to
@@ -62,15 +62,20 @@ template <int D, int CODE> struct Cfg {
   static constexpr int kPitch = kRow < 128 ? kRow : 128, kBoxes = kRow / kPitch;         // as TMA leaves it: boxes of 64 or 128 bytes
   static constexpr int kRaw = 128 * kRow;                                                // a tile of codes
   static constexpr int kDepth = CODE == TRITT_CODE_F16 ? (D == 128 ? 2 : 6) : (D == 128 ? 5 : 8);   // tiles of codes on their way
-  static constexpr int kOperands = D == 128 ? 2 : 4, kOperandCols = D / 2;               // tiles of K1 in tensor memory, behind the scores
+  static constexpr int kOperands = 2, kOperandCols = D / 2;                                // tiles of K1 in tensor memory, behind the scores
   static constexpr int kTmemA = kScores * 128;
   static_assert(kTmemA + kOperands * kOperandCols <= 512, "tensor memory");
+  // (the warps that convert say with the barrier of a tile's scores that it is described: they get there when the products of kOperands tiles back are done, and so the barrier's phase before)
+  static_assert(kOperands < kScores, "arrivals in the phase of another tile");
+  // Tile t is described when its codes may be fetched: those of kDepth tiles back have been converted then, so the products of kOperands further back are done, which had waited for the scores of kScores further
+  // back to be read.
+  static_assert(kDepth + kOperands + kScores <= kMetas, "descriptions of tiles in use");
   static constexpr int kOffQ = 0;                      // [2][hi, lo]
   static constexpr int kOffRaw = 4 * kTile;            // [kDepth]
   static constexpr int kOffMisc = kOffRaw + kDepth * kRaw;
 };
 struct Misc {
-  uint64_t raw_full[8], raw_free[8], a_full[4], a_free[4], meta_full[kMetas], meta_free[kMetas], q_full[2], q_free[2], s_full[kScores], s_free[kScores], item_full[kItems],
+  uint64_t raw_full[8], raw_free[8], a_full[4], a_free[4], q_full[2], q_free[2], s_full[kScores], s_free[kScores], item_full[kItems],
       item_free[kItems];
   Item items[kItems];
   Meta meta[kMetas];
@@ -142,23 +147,19 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_weigh_sm100_kernel(const __gr
   if (tid == 32) {
     ms.abort_flag = (smem_u32(smem) & 1023u) != 0;
     for (int i = 0; i < C::kDepth; ++i) {
-      mbar_init(&ms.raw_full[i], 2);
+      mbar_init(&ms.raw_full[i], 1);
       mbar_init(&ms.raw_free[i], 4);
     }
     for (int i = 0; i < C::kOperands; ++i) {
       mbar_init(&ms.a_full[i], 128);
       mbar_init(&ms.a_free[i], 1);
     }
-    for (int i = 0; i < kMetas; ++i) {
-      mbar_init(&ms.meta_full[i], 2);
-      mbar_init(&ms.meta_free[i], 16);
-    }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&ms.q_full[i], 128);
       mbar_init(&ms.q_free[i], 17);   // its last products, and sixteen warps that have read its columns
     }
     for (int i = 0; i < kScores; ++i) {
-      mbar_init(&ms.s_full[i], 1);
+      mbar_init(&ms.s_full[i], 5);   // the products, and four warps that have seen the tile's description
       mbar_init(&ms.s_free[i], 16);
     }
     for (int i = 0; i < kItems; ++i) {
@@ -263,12 +264,12 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_weigh_sm100_kernel(const __gr
       }
     } else {
       // ------------------------------------------------------------------ K1 on its way
-      // A lane has two rows of 64.  Pages are looked up three tiles ahead of the copies, exponents read one ahead.
-      const int r0 = (warp - 2) * 64 + lane * 2;
-      const int seg_log2 = a.page_log2 < 6 ? a.page_log2 : 6, seg = 1 << seg_log2;   // rows that lie in one page, ...
-      const int lanes = seg / 2, lane0 = lane & ~(lanes - 1);                        // ... which neighbouring lanes have
+      // A lane has four rows.  Of the warp's tiles pages are looked up three ahead of the copies, exponents read one ahead.
+      const int r0 = lane * 4, mine = warp - 2;
+      const int seg_log2 = a.page_log2 < 7 ? a.page_log2 : 7, seg = 1 << seg_log2;   // rows that lie in one page, ...
+      const int lanes = seg / 4, lane0 = lane & ~(lanes - 1);                        // ... which neighbouring lanes have
       const uint32_t mask = lanes == 32 ? 0xffffffffu : (1u << lanes) - 1;
-      uint32_t tiles = 0;
+      uint32_t before = 0;   // tiles of the pieces so far
       bool alive = true;
       if (lane == 0) tma_prefetch_desc(&map);
       for (int count = 0; alive; ++count) {
@@ -276,62 +277,78 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_weigh_sm100_kernel(const __gr
         if (n < 0) break;
         const Item it = ms.items[count % kItems];
         free_item(count);
-        if (n == 0) continue;
-        const int x0 = it.s0 * 128 + r0;
-        // the page of the lane's rows of the piece's i-th tile, as the table has it (not looked at here, so that nothing waits for it); -1: nobody looks at them, or the table has none
-        auto attended = [&](int i) { return i < n && x0 + i * 128 + 1 >= it.j_lo && x0 + i * 128 <= it.pos; };
+        const int f = (int)((before ^ mine) & 1), own = (n - f + 1) / 2;   // the warp's first tile of the piece, and how many it has
+        const int x0 = (it.s0 + f) * 128 + r0;
+        // the page of the lane's rows of the warp's i-th tile, as the table has it (not looked at here, so that nothing waits for it); -1: nobody looks at them, or the table has none
+        auto attended = [&](int i) { return i < own && x0 + i * 256 + 3 >= it.j_lo && x0 + i * 256 <= it.pos; };
         auto page_of = [&](int i) {
-          const int at = (x0 + i * 128) >> a.page_log2;
+          const int at = (x0 + i * 256) >> a.page_log2;
           int page = -1;
           if (attended(i) && at < a.c.table_pages) page = __ldg(a.c.table + it.b * a.c.table_stride + at);
           return page;
         };
-        struct Two {
+        struct Four {
           size_t row;
           uint32_t exponents;
           bool there;
         };
         auto read = [&](int i, int page) {
-          Two t{0, 0, page >= 0 && page < a.c.pages};
+          Four t{0, 0, page >= 0 && page < a.c.pages};
           if (t.there) {
-            t.row = row_of(a, Place{page, (x0 + i * 128) & (a.c.page_size - 1)}, kPartK1, it.head);
-            t.exponents = __ldg(reinterpret_cast<const uint16_t*>(a.c.exponents + t.row));
+            t.row = row_of(a, Place{page, (x0 + i * 256) & (a.c.page_size - 1)}, kPartK1, it.head);
+            t.exponents = __ldg(reinterpret_cast<const uint32_t*>(a.c.exponents + t.row));
           } else if (attended(i) && a.status) {
             atomicOr(a.status, kStatusPlace);
           }
           return t;
         };
-        Two now = read(0, page_of(0));
-        int page1 = page_of(1), page2 = page_of(2);
-        for (int i = 0; i < n && alive; ++i, ++tiles) {
-          const int page3 = page_of(i + 3);
-          const Two next = read(i + 1, page1);
-          const uint32_t slot = tiles % C::kDepth, mt = tiles % kMetas;
-          alive = wait_all(&ms.raw_free[slot], ((tiles / C::kDepth) & 1) ^ 1) && wait_all(&ms.meta_free[mt], ((tiles / kMetas) & 1) ^ 1);
-          if (!alive) break;
-          const uint32_t found = __ballot_sync(0xffffffffu, now.there);
-          uint32_t bytes = 0;
-          for (int l = 0; l < 32; l += lanes)
-            if (found >> l & mask) bytes += seg * C::kRow;
-          if (lane == 0) mbar_arrive_expect_tx(&ms.raw_full[slot], bytes);
-          const uint32_t of = found >> lane0 & mask;
-          if (of && lane == lane0 + __ffs(of) - 1) {   // (all of the page's rows that the tile has may be read, whether somebody looks at them or not)
-            const int at = r0 & ~(seg - 1);
-            uint8_t* const to = smem + C::kOffRaw + slot * C::kRaw + at * C::kPitch;
+        // (four steps a round, so that what is on its way stays in the registers that it comes to: a move would wait for it)
+        int page[4] = {page_of(0), page_of(1), page_of(2), -1};
+        Four four[2];
+        four[0] = read(0, page[0]);
+        for (int i0 = 0; i0 < own && alive; i0 += 4) {
 #pragma unroll
-            for (int x = 0; x < C::kBoxes; ++x)   // (the cache has fewer than 2^31 rows: one has 64 bytes at least)
-              tma_load_3d(to + x * 128 * C::kPitch, &map, &ms.raw_full[slot], x * 64, (int)(now.row - (r0 - at)), 0);
+          for (int u = 0; u < 4; ++u) {
+            const int i = i0 + u;
+            if (i >= own || !alive) break;
+            page[(u + 3) % 4] = page_of(i + 3);
+            four[(u + 1) % 2] = read(i + 1, page[(u + 1) % 4]);
+            const Four& now = four[u % 2];
+            const uint32_t tile = before + f + 2 * i, slot = tile % C::kDepth;
+            alive = wait_all(&ms.raw_free[slot], ((tile / C::kDepth) & 1) ^ 1);
+            if (!alive) break;
+            const uint32_t found = __ballot_sync(0xffffffffu, now.there);
+            uint32_t bytes = 128 * C::kRow;
+            if (found != 0xffffffffu) {
+              bytes = 0;
+              for (int l = 0; l < 32; l += lanes)
+                if (found >> l & mask) bytes += seg * C::kRow;
+            }
+            // the tile's description; who has seen the codes come has seen it
+            const int x = x0 + i * 256;
+            uint32_t e[4];
+            bool plain = now.there && x >= it.j_lo && x + 3 <= it.pos;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              e[k] = now.exponents >> 8 * k & 255;
+              plain = plain && e[k] != 255;
+              if (!now.there || x + k < it.j_lo || x + k > it.pos) e[k] = kOff;
+            }
+            const uint32_t flag = __all_sync(0xffffffffu, plain) ? kPlain | kPlain << 16 : 0u;
+            *reinterpret_cast<uint2*>(&ms.meta[tile % kMetas].row[r0]) = make_uint2(e[0] | e[1] << 16 | flag, e[2] | e[3] << 16 | flag);
+            __syncwarp();
+            if (lane == 0) mbar_arrive_expect_tx(&ms.raw_full[slot], bytes);
+            const uint32_t of = found >> lane0 & mask;
+            if (of && lane == lane0 + __ffs(of) - 1) {   // (all of the page's rows that the tile has may be read, whether somebody looks at them or not)
+              const int at = r0 & ~(seg - 1);
+              uint8_t* const to = smem + C::kOffRaw + slot * C::kRaw + at * C::kPitch;
+#pragma unroll
+              for (int x = 0; x < C::kBoxes; ++x)   // (the cache has fewer than 2^31 rows: one has 64 bytes at least)
+                tma_load_3d(to + x * 128 * C::kPitch, &map, &ms.raw_full[slot], x * 64, (int)(now.row - (r0 - at)), 0);
+            }
           }
-          const int x = x0 + i * 128;
-          const uint32_t lo = now.there && x >= it.j_lo && x <= it.pos ? now.exponents & 255 : kOff;
-          const uint32_t hi = now.there && x + 1 >= it.j_lo && x + 1 <= it.pos ? now.exponents >> 8 : kOff;
-          *reinterpret_cast<uint32_t*>(&ms.meta[mt].row[r0]) = lo | hi << 16;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&ms.meta_full[mt]);
-          now = next;
-          page1 = page2;
-          page2 = page3;
         }
+        before += n;
       }
       if (*abort_flag) {   // give copies still in flight a bounded chance to land before the CTA retires
         const long long t0 = clock64();
@@ -351,7 +368,7 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_weigh_sm100_kernel(const __gr
       if (n < 0) break;
       free_item(count);
       for (int i = 0; i < n && alive; ++i, ++tiles) {
-        const uint32_t ab = tiles % C::kOperands, slot = tiles % C::kDepth;
+        const uint32_t ab = tiles % C::kOperands, slot = tiles % C::kDepth, sb = tiles % kScores;
         alive = wait_all(&ms.raw_full[slot], (tiles / C::kDepth) & 1) && wait_all(&ms.a_free[ab], ((tiles / C::kOperands) & 1) ^ 1);
         if (!alive) break;
         tc_fence_after();
@@ -381,7 +398,10 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_weigh_sm100_kernel(const __gr
           tmem_st16(to + h * 16, v);
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&ms.raw_free[slot]);
+        if (lane == 0) {
+          mbar_arrive(&ms.raw_free[slot]);
+          mbar_arrive(&ms.s_full[sb]);
+        }
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(&ms.a_full[ab]);
@@ -493,8 +513,7 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_weigh_sm100_kernel(const __gr
     // ------------------------------------------------------------------ sums: a row a thread, 32 columns
     const int wg = (warp - 12) / 4, wq = warp & 3, row = wq * 32 + lane;
     const uint32_t t_col = tmem + wg * 32 + ((uint32_t)(wq * 32) << 16);
-    int pieces = 0;
-    uint32_t tiles = 0;
+    int pieces = 0, sb = 0, sph = 0, mt = 0;   // the next buffer of scores, the next description
     bool alive = true;
     for (int count = 0; alive; ++count) {
       const int n = next_item(count);
@@ -522,42 +541,37 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_weigh_sm100_kernel(const __gr
       // what a row's scores are multiplied by: its power of two with that of the columns, q and Q (beyond fp32's range scores have no use for), and the scale
       const int power = col.largest[wg] + field - 382 + 127 + kDown<CODE>;
       const float scale = field == 255 ? __uint_as_float(0x7fffffffu) : field == 0 ? 0.f : p.scale2;
-      const bool all_there = there == 0xffffffffu && !apart;
+      // whether the rows of a plain tile have pairs with all of the 32 columns
+      const bool plain = there == 0xffffffffu && !apart && field != 255 && k0 >= k_lo && k0 + 31 <= pos && p.kkl >= pos && p.kkr >= pos;
       float2 column[16];
 #pragma unroll
       for (int c = 0; c < 16; ++c) column[c] = make_float2(0.f, 0.f);
-      for (int i = 0; i < n; ++i, ++tiles) {
-        const uint32_t sb = tiles % kScores, mt = tiles % kMetas;
-        const int j = (s0 + i) * 128 + row;
-        alive = wait_all(&ms.s_full[sb], (tiles / kScores) & 1);
+      float* to = row_sums + (s0 * 128 + row - base);   // (a slot has room for all of a tile's rows)
+      for (int i = 0; i < n; ++i, to += 128) {
+        alive = wait_all(&ms.s_full[sb], sph);
         if (!alive) break;
         tc_fence_after();
         uint32_t s[32];
         tmem_ld32(t_col + sb * 128, s);
-        // the thread's row, beside the load
-        alive = wait_all(&ms.meta_full[mt], (tiles / kMetas) & 1);
-        if (!alive) break;
-        const int e = ms.meta[mt].row[row], f = least_of(most((e & 255) + power, 1), 254);
-        const float factor = (e & 255) == 255 ? __uint_as_float(0x7fffffffu) : scale * __uint_as_float((uint32_t)f << 23);
-        const int c_lo = most(k_lo, j - p.kkr) - k0, c_hi = e < kOff ? (p.kkl < pos - j ? j + p.kkl : pos) - k0 : -1;   // columns that it has pairs with
-        const bool plain = __all_sync(0xffffffffu, all_there && c_lo <= 0 && c_hi >= 31);
+        const int e = ms.meta[mt].row[row];   // (the thread's row, beside the load)
+        float factor = scale * __uint_as_float((uint32_t)least_of(most((e & 255) + power, 1), 254) << 23);
         tmem_wait_ld(s);
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&ms.s_free[sb]);
-          mbar_arrive(&ms.meta_free[mt]);
-        }
+        if (lane == 0) mbar_arrive(&ms.s_free[sb]);
         float2 x[16];
 #pragma unroll
         for (int c = 0; c < 16; ++c) x[c] = make_float2(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1]));
-        if (plain) {
+        if (plain && (e & kPlain)) {   // (all of the warp's rows alike)
 #pragma unroll
           for (int c = 0; c < 16; ++c) x[c] = fma_pair(x[c], factor, minus);
         } else {   // scores of pairs that there are not become minus infinity; where columns' exponents are apart, each has its own factor
+          const int j = (s0 + i) * 128 + row;
+          const int c_lo = most(k_lo, j - p.kkr) - k0, c_hi = !(e & kOff) ? (p.kkl < pos - j ? j + p.kkl : pos) - k0 : -1;   // columns that the row has pairs with
           uint32_t seen = there;
           if (c_lo > 0) seen &= c_lo > 31 ? 0u : 0xffffffffu << c_lo;
           if (c_hi < 31) seen &= c_hi < 0 ? 0u : 0xffffffffu >> (31 - c_hi);
+          if ((e & 255) == 255) factor = __uint_as_float(0x7fffffffu);
           if (apart) {
             const float2* by = reinterpret_cast<const float2*>(col.scale + wg * 32);
 #pragma unroll
@@ -579,7 +593,9 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_weigh_sm100_kernel(const __gr
         }
         const float2 both = add_pair(sum[0], sum[1]);
         // (no thread but this one adds to the place, in order)
-        if (j <= last) asm volatile("red.relaxed.gpu.global.add.f32 [%0], %1;" ::"l"(row_sums + (j - base)), "f"(both.x + both.y) : "memory");
+        asm volatile("red.relaxed.gpu.global.add.f32 [%0], %1;" ::"l"(to), "f"(both.x + both.y) : "memory");
+        if (++sb == kScores) sb = 0, sph ^= 1;
+        mt = (mt + 1) % kMetas;
       }
       if (!alive) break;
       __syncwarp();
@@ -613,9 +629,9 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_weigh_sm100_kernel(const __gr
 template <typename T, int D, int CODE> int launch(const TdpWeighArgs& p, cudaStream_t stream) {
   using C = Cfg<D, CODE>;
   const tritt_cache_t& c = p.cache.c;
-  // all rows of the cache, boxes of what a page has of 64 rows
+  // all rows of the cache, boxes of what a page has of 128 rows
   CUtensorMap map{};
-  if (int rc = make_tmap_codes(&map, c.codes, C::kRow, (uint64_t)c.pages * 4 * c.N * c.page_size, C::kPitch, c.page_size < 64 ? c.page_size : 64)) return rc;
+  if (int rc = make_tmap_codes(&map, c.codes, C::kRow, (uint64_t)c.pages * 4 * c.N * c.page_size, C::kPitch, c.page_size < 128 ? c.page_size : 128)) return rc;
   // (warpgroups share out the registers that the kernel is launched with: with fewer those that raise their count would wait for good)
   cudaFuncAttributes attr;
   TRITT_CUDA_OK(cudaFuncGetAttributes(&attr, tdp_weigh_sm100_kernel<T, D, CODE>));
