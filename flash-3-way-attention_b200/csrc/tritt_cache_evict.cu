@@ -5,7 +5,7 @@
 // through distributed shared memory; the weights are read from L2 after the first pass.
 //
 // Moved by another kernel, bound by the bytes of the kept rows, read and written once.  In place: a kept token's new place is never behind its old one, so rows that are taken in order
-// and written when all rows up to them have been read overwrite nothing that is still to be read.  One block takes a piece of 32 to 128 bytes of all rows of one part of a head (the
+// and written when all rows up to them have been read overwrite nothing that is still to be read.  One block, or a cluster whose blocks keep step, takes a piece of up to 64 bytes of all rows of one part of a head (the
 // parts, heads and pieces of rows are independent), with the next tile's rows on their way while one is written.
 #include "tritt_weigh.cuh"
 
@@ -402,11 +402,12 @@ extern "C" int tritt_cache_evict(const tritt_cache_t* c, const tritt_weights_t* 
   if (int rc = check(c, w, p)) return rc;
   p.cache.c.n = 1;   // (places are reported of every sequence in use)
   p.cache.c.counts = nullptr;
-  // A cluster for a head: a CTA takes a few thousand weights, and there are no more of them than the chip holds at once.
+  // A cluster for a head as far as the weights do not fit in one CTA's registers (fewer and larger clusters: eight CTAs a head of 65001 weights took 39 us, some of them behind others), and not more CTAs
+  // than the chip holds at once.
   long long tokens = (long long)c->table_pages * c->page_size;
   if (w->before_length < tokens) tokens = w->before_length;
   int ranks = 1;
-  while (ranks < kMostCluster && tokens > 2048LL * ranks && 2LL * ranks * c->B * c->N <= kSms) ranks *= 2;
+  while (ranks < kMostCluster && tokens > (long long)kHeld * kSelectThreads * ranks && 2LL * ranks * c->B * c->N <= kSms) ranks *= 2;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(ranks, c->B * c->N);
   cfg.blockDim = dim3(kSelectThreads);
@@ -423,10 +424,9 @@ extern "C" int tritt_cache_evict(const tritt_cache_t* c, const tritt_weights_t* 
     TRITT_CUDA_OK(cudaLaunchKernelEx(&cfg, evict_select_kernel<false>, p));
   count_launch();
   const int row_bytes = c->D * code_bytes(c->code);
-  switch (row_bytes < 128 ? row_bytes : 128) {
+  switch (row_bytes < 64 ? row_bytes : 64) {
     case 16: return launch_move<16>(p, row_bytes, (cudaStream_t)stream);
     case 32: return launch_move<32>(p, row_bytes, (cudaStream_t)stream);
-    case 64: return launch_move<64>(p, row_bytes, (cudaStream_t)stream);
-    default: return launch_move<128>(p, row_bytes, (cudaStream_t)stream);
+    default: return launch_move<64>(p, row_bytes, (cudaStream_t)stream);
   }
 }

@@ -36,6 +36,174 @@ template <typename T, int D> constexpr int kBytesEach = 2 * D * 2 * (std::is_sam
 template <typename T, int D> constexpr int kMostChunk = 32768 / kBytesEach<T, D> < 64 ? 32768 / kBytesEach<T, D> : 64;
 static_assert(kMostChunk<float, 256> == 16 && kMostChunk<__half, 64> == 64, "chunks are multiples of 8");
 
+// The rows q and k2 of new tokens q0 .. q0 + here - 1 as fragments, eight tokens a tile, and what their scores need, by all of a block's warps.
+template <typename T, int D, int CODE>
+__device__ __forceinline__ void form_queries(const Params& p, int b, int head, int ctx, int q0, int here, int tiles, uint2* frags, Query (&queries)[2][64]) {
+  using Rows = RowFragments<D, CODE>;
+  constexpr bool kWide = std::is_same<T, float>::value;
+  constexpr int kSteps = Rows::kSteps, kHalves = kWide ? 2 : 1;
+  const CacheArgs& a = p.cache;
+  const int lane = threadIdx.x % 32;
+  for (int i = threadIdx.x / 32; i < 2 * tiles * 8; i += kThreads / 32) {
+    const int part = i >= tiles * 8, n = i - part * tiles * 8;
+    const bool on = n < here;
+    const T* row = (const T*)p.rows[part].p + (on ? rows_at(p.rows[part], b, head, q0 + n) : 0);
+    float4 f[D > 128 ? 2 : 1];
+    uint32_t top = 0;
+#pragma unroll
+    for (int k = 0; k < (D > 128 ? 2 : 1); ++k) {
+      f[k] = on && lane + 32 * k < D / 4 ? load4(row + (lane + 32 * k) * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+      top = max(top, largest4(f[k]));
+    }
+    const int field = (int)(largest_of_row<32>(top) >> 23);
+    const float up = to_operand(field);
+#pragma unroll
+    for (int k = 0; k < (D > 128 ? 2 : 1); ++k) {
+      const int col = (lane + 32 * k) * 4;
+      if (col >= D) continue;
+      float4 v = f[k];
+      v.x *= up, v.y *= up, v.z *= up, v.w *= up;
+      if (field == 255) v = make_float4(0.f, 0.f, 0.f, 0.f);
+      const auto slot = Rows::slot_of(col);
+      uint2* to = frags + ((size_t)((part * tiles + n / 8) * kHalves) * kSteps + slot.step) * 32 + n % 8 * 4 + slot.c;
+      const uint2 hi = make_uint2(pack_halves(v.x, v.y), pack_halves(v.z, v.w));
+      to[0] = hi;
+      if constexpr (kWide) to[kSteps * 32] = make_uint2(pack_rests(v.x, v.y, hi.x), pack_rests(v.z, v.w, hi.y));
+    }
+    if (lane == 0) {
+      Query q{p.scale2 * from_operand(field), 0.f, -1, 0};
+      if (on) {
+        q.last = ctx + q0 + n;
+        if (part == 0) {
+          q.minus = __ldg(p.m + ((size_t)b * a.c.N + head) * a.c.n + q0 + n);
+        } else {
+          const Place own = place_of(a, b, ctx + q0 + n);
+          if (own.page >= 0)
+            q.minus = __ldg(a.c.lse + lse_of(a, own, head));
+          else
+            q.last = -1;
+        }
+        if (q.minus == -INFINITY) q.last = -1;
+      }
+      queries[part][n] = q;
+    }
+  }
+}
+
+// A few new tokens, rows of up to 128 bytes: 32 tokens a warp at a time, in two products' fragments, whose scores then change lanes so that each lane has one token, its row's exponent, its
+// log-sum-exp and its weight (with two tokens a lane of four and eight columns for one new token the kernel above executed four times the instructions: 178 us for 32 x 16 heads over
+// 8191, e4m3).
+constexpr int kFew = 4, kFewTokens = 256;   // new tokens at most; of a block at a time
+template <int D, int CODE> constexpr bool kFewApplies = RowFragments<D, CODE>::kWords <= 8;
+
+template <typename T, int D, int CODE> __global__ void __launch_bounds__(kThreads, RowFragments<D, CODE>::kWords <= 4 ? 3 : 2) dps_weigh_few_kernel(const __grid_constant__ Params p) {
+  using Rows = RowFragments<D, CODE>;
+  constexpr bool kWide = std::is_same<T, float>::value;
+  constexpr int kSteps = Rows::kSteps, kHalves = kWide ? 2 : 1;
+  extern __shared__ __align__(16) uint2 frags[];   // [part][hi, lo][step][lane]
+  __shared__ Query queries[2][64];
+  const CacheArgs& a = p.cache;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int bh = blockIdx.y, b = bh / a.c.N, head = bh - b * a.c.N;
+  if (__ldg(a.c.context + b) < 0) return;
+  const int ctx = context_of(a, b), cnt = new_tokens(a, b), end = weighed_tokens(a, p.w, ctx + cnt);
+  const int first = blockIdx.x * p.repeat * kFewTokens + warp * 32;
+  if ((int)blockIdx.x * p.repeat * kFewTokens >= end) return;
+  const int behind = ctx - (p.k_diff < ctx ? p.k_diff : ctx);   // the first token that any new one's k2 attends to
+  const uint8_t* codes = (const uint8_t*)a.c.codes;
+  constexpr size_t kRow = D * Rows::kSize;
+  const size_t part_rows = (size_t)a.c.N << a.page_log2;
+
+  struct Step {
+    Rows k2[2], k1[2];
+    uint32_t byte;        // K2's exponent, K1's
+    float lse, before;
+    uint32_t there;       // bit t: the 16 tokens have a place
+    bool inner;
+  };
+  auto fetch = [&](int r, Step& t) {
+    const int x0 = first + r * kFewTokens, x = x0 + lane;
+    Place at{-1, 0};
+    if (x < end) {
+      at = place_of(a, b, x);
+      if (at.page < 0 && a.status) atomicOr(a.status, kStatusPlace);
+    }
+    const bool on = at.page >= 0;
+    const size_t row = on ? row_of(a, at, kPartK2, head) : 0;
+    t.inner = x0 + 31 >= behind;
+    t.byte = 0;
+    t.lse = t.before = 0.f;
+    if (on) {
+      t.lse = __ldg(a.c.lse + lse_of(a, at, head));
+      t.byte = __ldg(a.c.exponents + row);
+      if (t.inner) t.byte |= (uint32_t)__ldg(a.c.exponents + row - part_rows) << 8;   // (K1's row lies a part ahead)
+    }
+    if (x < end && x < ctx) t.before = faded(p.w, b, head, x);
+    t.there = 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const size_t base = (size_t)__shfl_sync(0xffffffffu, (uint32_t)(row >> 32), 16 * h) << 32 | __shfl_sync(0xffffffffu, (uint32_t)row, 16 * h);
+      if (!__shfl_sync(0xffffffffu, (int)on, 16 * h)) continue;
+      t.there |= 1u << h;
+      t.k2[h].load(codes + base * kRow, lane);
+      if (t.inner) t.k1[h].load(codes + (base - part_rows) * kRow, lane);
+    }
+  };
+  auto work = [&](int r, const Step& t) {
+    const int x0 = first + r * kFewTokens, x = x0 + lane;
+    float sum = t.before;
+    if (t.there && cnt > 0) {
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {
+        if (part && !t.inner) break;
+        float d[2][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) d[h][k] = 0.f;
+#pragma unroll
+          for (int s = 0; s < kSteps; ++s) {
+            uint32_t frag[4];
+            (part ? t.k1[h] : t.k2[h]).step(s, frag);
+            const uint2* from = frags + (size_t)(part * kHalves * kSteps + s) * 32 + lane;
+            mma_16816(d[h], frag, from[0]);
+            if constexpr (kWide) mma_16816(d[h], frag, from[kSteps * 32]);
+          }
+        }
+        const float scale = code_scale(t.byte >> 8 * part & 255);
+        const bool there = t.there >> (lane / 16) & 1;
+#pragma unroll
+        for (int n = 0; n < kFew; ++n) {
+          if (n >= cnt) break;
+          // the score of this lane's token: row lane % 16 of half lane / 16
+          const int from = lane % 8 * 4 + n / 2;
+          const float s0 = __shfl_sync(0xffffffffu, d[0][n % 2], from), s1 = __shfl_sync(0xffffffffu, d[0][2 + n % 2], from);
+          const float s2 = __shfl_sync(0xffffffffu, d[1][n % 2], from), s3 = __shfl_sync(0xffffffffu, d[1][2 + n % 2], from);
+          const float score = lane < 16 ? (lane < 8 ? s0 : s1) : (lane < 24 ? s2 : s3);
+          const Query q = queries[part][n];
+          const bool on = there && x <= q.last && (part == 0 || q.last - x <= p.k_diff);
+          const float less = part == 0 ? t.lse - q.minus : -q.minus;
+          sum += on ? exp2f(fmaf(score * scale, q.scale, less * kLog2e)) : 0.f;
+        }
+      }
+    }
+    if (x < end) *weight_of(p.w, b, head, x) = sum;
+  };
+  int steps = (end - first + kFewTokens - 1) / kFewTokens;
+  if (steps > p.repeat) steps = p.repeat;   // (of this warp; none if it lies behind the end)
+  Step even, odd;
+  if (steps > 0) fetch(0, even);
+  if (cnt > 0) form_queries<T, D, CODE>(p, b, head, ctx, 0, cnt, 1, frags, queries);
+  __syncthreads();
+  for (int r = 0; r < steps; r += 2) {   // the next step's rows are on their way while one is worked on
+    if (r + 1 < steps) fetch(r + 1, odd);
+    work(r, even);
+    if (r + 1 >= steps) break;
+    if (r + 2 < steps) fetch(r + 2, even);
+    work(r + 1, odd);
+  }
+}
+
 // Blocks an SM: registers for the bytes of rows that are to be in flight.
 template <int D, int CODE> constexpr int kPerSm = RowFragments<D, CODE>::kWords <= 4 ? 3 : RowFragments<D, CODE>::kWords <= 16 ? 2 : 1;
 
@@ -99,50 +267,7 @@ template <typename T, int D, int CODE> __global__ void __launch_bounds__(kThread
       const int here = cnt - q0 < p.chunk ? cnt - q0 : p.chunk, tiles = (here + 7) / 8;
       if (r == 0 || chunks > 1) {   // the new tokens' rows as fragments
         if (r || chunk) __syncthreads();
-        for (int i = warp; i < 2 * tiles * 8; i += kThreads / 32) {
-          const int part = i >= tiles * 8, n = i - part * tiles * 8;
-          const bool on = n < here;
-          const T* row = (const T*)p.rows[part].p + (on ? rows_at(p.rows[part], b, head, q0 + n) : 0);
-          float4 f[D > 128 ? 2 : 1];
-          uint32_t top = 0;
-#pragma unroll
-          for (int k = 0; k < (D > 128 ? 2 : 1); ++k) {
-            f[k] = on && lane + 32 * k < D / 4 ? load4(row + (lane + 32 * k) * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
-            top = max(top, largest4(f[k]));
-          }
-          const int field = (int)(largest_of_row<32>(top) >> 23);
-          const float up = to_operand(field);
-#pragma unroll
-          for (int k = 0; k < (D > 128 ? 2 : 1); ++k) {
-            const int col = (lane + 32 * k) * 4;
-            if (col >= D) continue;
-            float4 v = f[k];
-            v.x *= up, v.y *= up, v.z *= up, v.w *= up;
-            if (field == 255) v = make_float4(0.f, 0.f, 0.f, 0.f);
-            const auto slot = Rows::slot_of(col);
-            uint2* to = frags + ((size_t)((part * tiles + n / 8) * kHalves) * kSteps + slot.step) * 32 + n % 8 * 4 + slot.c;
-            const uint2 hi = make_uint2(pack_halves(v.x, v.y), pack_halves(v.z, v.w));
-            to[0] = hi;
-            if constexpr (kWide) to[kSteps * 32] = make_uint2(pack_rests(v.x, v.y, hi.x), pack_rests(v.z, v.w, hi.y));
-          }
-          if (lane == 0) {
-            Query q{p.scale2 * from_operand(field), 0.f, -1, 0};
-            if (on) {
-              q.last = ctx + q0 + n;
-              if (part == 0) {
-                q.minus = __ldg(p.m + (size_t)bh * a.c.n + q0 + n);
-              } else {
-                const Place own = place_of(a, b, ctx + q0 + n);
-                if (own.page >= 0)
-                  q.minus = __ldg(a.c.lse + lse_of(a, own, head));
-                else
-                  q.last = -1;
-              }
-              if (q.minus == -INFINITY) q.last = -1;
-            }
-            queries[part][n] = q;
-          }
-        }
+        form_queries<T, D, CODE>(p, b, head, ctx, q0, here, tiles, frags, queries);
         __syncthreads();
       }
       if (!t.there) continue;
@@ -207,12 +332,22 @@ template <typename T, int D, int CODE> __global__ void __launch_bounds__(kThread
 
 template <typename T, int D, int CODE> int launch(Params p, cudaStream_t stream) {
   const tritt_cache_t& c = p.cache.c;
-  const int most = kMostChunk<T, D>, n8 = (c.n + 7) / 8 * 8;
-  p.chunk = n8 < most ? n8 : most;
-  const int bytes = p.chunk * kBytesEach<T, D>;
   long long tokens = (long long)c.table_pages * c.page_size;
   const int length = p.w.after_length < p.w.before_length ? p.w.after_length : p.w.before_length;
   if (length < tokens) tokens = length;
+  if constexpr (kFewApplies<D, CODE>) {
+    if (c.n <= kFew) {
+      const long long blocks = (tokens + kFewTokens - 1) / kFewTokens, repeat = blocks * c.B * c.N / (kSms * 12);
+      p.repeat = (int)(repeat < 1 ? 1 : repeat > 8 ? 8 : repeat);
+      dps_weigh_few_kernel<T, D, CODE><<<dim3((unsigned)((blocks + p.repeat - 1) / p.repeat), c.B * c.N), kThreads, 8 * kBytesEach<T, D>, stream>>>(p);
+      count_launch();
+      TRITT_CUDA_OK(cudaGetLastError());
+      return 0;
+    }
+  }
+  const int most = kMostChunk<T, D>, n8 = (c.n + 7) / 8 * 8;
+  p.chunk = n8 < most ? n8 : most;
+  const int bytes = p.chunk * kBytesEach<T, D>;
   const long long blocks = (tokens + kTokens - 1) / kTokens;
   // the new rows are formed once a block: it takes several times kTokens where there are blocks enough for all SMs several times over
   long long repeat = blocks * c.B * c.N / (kSms * 3);
