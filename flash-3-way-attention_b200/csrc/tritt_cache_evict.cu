@@ -310,26 +310,27 @@ template <int W> __global__ void __launch_bounds__(kMoveThreads) evict_move_kern
   };
   const int tiles = (count + M::kRows * ranks - 1) / (M::kRows * ranks);
   if (tiles == 0) return;
-  auto sync = [&]() {
-    if (ranks > 1)
-      cluster.sync();
-    else
-      __syncthreads();
-  };
-  // Before a tile is written its rows, and those of all tiles before it, have been read by all threads (the barrier behind their loads); the next tile's, on their way then, lie behind what is written.
-  // The ring's place that `find` fills was last read by the stores of two tiles ago, before the last barrier.
+  // Before a tile is written its rows, and those of all tiles before it, have been read by all threads of the block, or in place of the cluster (the barrier behind their loads); the next tile's, on their way
+  // then, lie behind what is written.  The ring's place that `find` fills was last read by the stores of two tiles ago, before the last barrier.
+  // A cluster's barrier waits for the thread's loads, so the next tile's are sent behind it; a block's does not, and they are sent ahead of it.
+  const bool clustered = in_place && ranks > 1;
   find(0);
   __syncthreads();
   load(0, v[0], e[0], l[0], wt[0]);
   if (tiles > 1) find(1);
-  sync();
+  __syncthreads();
   for (int i = 0; i < tiles; i += 2) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       if (i + k >= tiles) break;
-      if (i + k + 1 < tiles) load(i + k + 1, v[1 - k], e[1 - k], l[1 - k], wt[1 - k]);
+      const bool more = i + k + 1 < tiles;
+      if (more && !clustered) load(i + k + 1, v[1 - k], e[1 - k], l[1 - k], wt[1 - k]);
       if (i + k + 2 < tiles) find(i + k + 2);
-      sync();
+      if (clustered)
+        cluster.sync();
+      else
+        __syncthreads();
+      if (more && clustered) load(i + k + 1, v[1 - k], e[1 - k], l[1 - k], wt[1 - k]);
       store(i + k, v[k], e[k], l[k], wt[k]);
     }
   }

@@ -96,7 +96,7 @@ __device__ __forceinline__ void form_queries(const Params& p, int b, int head, i
 constexpr int kFew = 4, kFewTokens = 256;   // new tokens at most; of a block at a time
 template <int D, int CODE> constexpr bool kFewApplies = RowFragments<D, CODE>::kWords <= 8;
 
-template <typename T, int D, int CODE> __global__ void __launch_bounds__(kThreads, RowFragments<D, CODE>::kWords <= 4 ? 3 : 2) dps_weigh_few_kernel(const __grid_constant__ Params p) {
+template <typename T, int D, int CODE> __global__ void __launch_bounds__(kThreads, 2) dps_weigh_few_kernel(const __grid_constant__ Params p) {
   using Rows = RowFragments<D, CODE>;
   constexpr bool kWide = std::is_same<T, float>::value;
   constexpr int kSteps = Rows::kSteps, kHalves = kWide ? 2 : 1;
@@ -121,14 +121,20 @@ template <typename T, int D, int CODE> __global__ void __launch_bounds__(kThread
     uint32_t there;       // bit t: the 16 tokens have a place
     bool inner;
   };
-  auto fetch = [&](int r, Step& t) {
+  // the page of the lane's token, as the table has it (a step before it is needed, and not looked at here, so that nothing waits for it); -1: the token is not there, or the table has none
+  int steps = end > first ? (end - first + kFewTokens - 1) / kFewTokens : 0;   // of this warp
+  if (steps > p.repeat) steps = p.repeat;
+  auto page_of = [&](int r) {
+    const int x = first + r * kFewTokens + lane, i = x >> a.page_log2;
+    int page = -1;
+    if (r < steps && x < end && i < a.c.table_pages) page = __ldg(a.c.table + b * a.c.table_stride + i);
+    return page;
+  };
+  auto fetch = [&](int r, Step& t, int page) {
     const int x0 = first + r * kFewTokens, x = x0 + lane;
-    Place at{-1, 0};
-    if (x < end) {
-      at = place_of(a, b, x);
-      if (at.page < 0 && a.status) atomicOr(a.status, kStatusPlace);
-    }
-    const bool on = at.page >= 0;
+    const bool on = page >= 0 && page < a.c.pages;
+    if (x < end && !on && a.status) atomicOr(a.status, kStatusPlace);
+    const Place at{page, x & (a.c.page_size - 1)};
     const size_t row = on ? row_of(a, at, kPartK2, head) : 0;
     t.inner = x0 + 31 >= behind;
     t.byte = 0;
@@ -189,17 +195,19 @@ template <typename T, int D, int CODE> __global__ void __launch_bounds__(kThread
     }
     if (x < end) *weight_of(p.w, b, head, x) = sum;
   };
-  int steps = (end - first + kFewTokens - 1) / kFewTokens;
-  if (steps > p.repeat) steps = p.repeat;   // (of this warp; none if it lies behind the end)
   Step even, odd;
-  if (steps > 0) fetch(0, even);
+  int page_even = page_of(0), page_odd = page_of(1);
+  if (steps > 0) fetch(0, even, page_even);
+  page_even = page_of(2);
   if (cnt > 0) form_queries<T, D, CODE>(p, b, head, ctx, 0, cnt, 1, frags, queries);
   __syncthreads();
   for (int r = 0; r < steps; r += 2) {   // the next step's rows are on their way while one is worked on
-    if (r + 1 < steps) fetch(r + 1, odd);
+    if (r + 1 < steps) fetch(r + 1, odd, page_odd);
+    page_odd = page_of(r + 3);
     work(r, even);
     if (r + 1 >= steps) break;
-    if (r + 2 < steps) fetch(r + 2, even);
+    if (r + 2 < steps) fetch(r + 2, even, page_even);
+    page_even = page_of(r + 4);
     work(r + 1, odd);
   }
 }
