@@ -110,12 +110,22 @@ template <bool HELD> __global__ void __launch_bounds__(kSelectThreads) evict_sel
   for (int r = rank * kSelectThreads + tid; r < p.recent; r += ranks * kSelectThreads) kept[p.keep - p.recent + r] = ctx - p.recent + r;
   if (need == 0) return;
 
-  for (int i = tid; i < 3 * kBins; i += kSelectThreads) (&hist[0][0])[i] = 0;
+  const bool few = HELD && ranks == 1 && own == 1;
+  if (!few)
+    for (int i = tid; i < 3 * kBins; i += kSelectThreads) (&hist[0][0])[i] = 0;
   if (tid < 2) counts[tid] = 0;
   __syncthreads();
   uint32_t prefix = 0, mask = 0, left = (uint32_t)need;   // digits found so far; tokens still to be found among those that have them
+  if (few) {   // a weight a thread: bit by bit, the block counted by its barrier
+    const bool mine = own0 < x1;
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t next = prefix | 1u << bit;
+      if (__syncthreads_count(mine && held[0] >= next) >= need) prefix = next;
+    }
+    left = (uint32_t)(need - __syncthreads_count(mine && held[0] > prefix));
+  }
 #pragma unroll 1
-  for (int pass = 0; pass < 3; ++pass) {
+  for (int pass = few ? 3 : 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
     uint32_t* const h = hist[pass];
     each_key([&](uint32_t k) {

@@ -81,7 +81,6 @@ struct Misc {
   Meta meta[kMetas];
   Columns columns[2];
   float sums[4][2][4][32];        // [warpgroup][parity of the piece][warp][column]
-  long long scan[33], at[2];
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -141,9 +140,6 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_weigh_sm100_kernel(const __gr
   const CacheArgs& a = p.cache;
   const uint8_t* const codes = (const uint8_t*)a.c.codes;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  const long long total = all_steps(p, ms.scan);
-  if ((int)blockIdx.x >= weigh_parts(p, total)) return;
-  find_sequence(p, (long long)blockIdx.x * total / weigh_parts(p, total), ms.scan, ms.at);
   if (tid == 32) {
     ms.abort_flag = (smem_u32(smem) & 1023u) != 0;
     for (int i = 0; i < C::kDepth; ++i) {
@@ -194,7 +190,7 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_weigh_sm100_kernel(const __gr
     set_regs<kRegsLaunch, kRegsIssue>();
     if (warp == 1) {
       // ------------------------------------------------------------------ pieces
-      WeighWalk walk = weigh_start(p, total, (int)ms.at[0], ms.at[1]);
+      WeighWalk walk = weigh_start(p, weigh_part(p));   // (a CTA without a part has no pieces)
       WeighPiece s;
       bool more = !*abort_flag;
       for (int count = 0; more; ++count) {

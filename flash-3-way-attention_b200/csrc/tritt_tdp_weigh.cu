@@ -23,8 +23,8 @@ template <int D> struct Shared {
   float columns[8][128];            // of each warp
   float scale[128];                 // of the scores with each token k
   float q[D];
-  long long scan[33], at[2];
   uint32_t there[4];                // tokens k that have a place
+  int field;                        // q's exponent
   int largest;                      // of their exponent bytes
 };
 
@@ -37,10 +37,7 @@ template <typename T, int D, int CODE> __global__ void __launch_bounds__(kThread
   const CacheArgs& a = p.cache;
   const uint8_t* codes = (const uint8_t*)a.c.codes;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, g = lane / 4, c = lane % 4;
-  const long long total = all_steps(p, sh.scan);
-  if ((int)blockIdx.x >= weigh_parts(p, total)) return;
-  find_sequence(p, (long long)blockIdx.x * total / weigh_parts(p, total), sh.scan, sh.at);
-  WeighWalk walk = weigh_start(p, total, (int)sh.at[0], sh.at[1]);
+  WeighWalk walk = weigh_start(p, weigh_part(p));   // (each warp for itself)
   WeighPiece s;
   while (weigh_next(p, walk, s)) {
     float* const rows_sum = weigh_slot(p, s.b, s.head);
@@ -68,7 +65,7 @@ template <typename T, int D, int CODE> __global__ void __launch_bounds__(kThread
         if (lane + 32 * k < D / 4)
           *reinterpret_cast<float4*>(sh.q + (lane + 32 * k) * 4) =
               field == 255 ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(f[k].x * up, f[k].y * up, f[k].z * up, f[k].w * up);
-      if (lane == 0) sh.at[0] = field, sh.largest = 0;
+      if (lane == 0) sh.field = field, sh.largest = 0;
     }
     const int k = s.kg * 128 + tid;   // (of the first four warps)
     int byte = 0;
@@ -86,7 +83,7 @@ template <typename T, int D, int CODE> __global__ void __launch_bounds__(kThread
     __syncthreads();
     if (tid < 128 && own.page >= 0 && byte != 255) atomicMax(&sh.largest, byte);
     __syncthreads();
-    const int field = (int)sh.at[0], largest = sh.largest;
+    const int field = sh.field, largest = sh.largest;
     if (tid < 128) sh.scale[tid] = own.page < 0 ? 0.f : byte == 255 ? __uint_as_float(0x7fffffffu) : power_of_two(byte - largest);
     // A
     for (int x = tid; x < 128 * (D / 4); x += kThreads) {
@@ -192,32 +189,22 @@ template <typename T, int D, int CODE> __global__ void __launch_bounds__(kThread
 
 // Adds up a head's slots, and the weights of before.
 __global__ void __launch_bounds__(256) tdp_weigh_join_kernel(const __grid_constant__ TdpWeighArgs p) {
-  __shared__ long long scan[33];
   const CacheArgs& a = p.cache;
   const int bh = blockIdx.y, b = bh / a.c.N, head = bh - b * a.c.N;
   if (__ldg(a.c.context + b) < 0) return;
   const int ctx = context_of(a, b), end = weighed_tokens(a, p.w, ctx + new_tokens(a, b)), x = blockIdx.x * 256 + threadIdx.x;
   if ((int)blockIdx.x * 256 >= end) return;
-  // steps of all sequences, and of those before this one
-  long long all = 0, before = 0, total, ahead;
-  for (int i = threadIdx.x; i < a.c.B; i += 256) {
-    const long long v = weigh_line(p, i).unit * a.c.N;
-    all += v;
-    if (i < b) before += v;
-  }
-  block_scan(all, scan, total);
-  block_scan(before, scan, ahead);
   const WeighLine l = weigh_line(p, b);
   float v = x < ctx && x < end ? faded(p.w, b, head, x) : 0.f, sum = 0.f;
   const bool any = l.unit > 0 && x >= l.base && x <= l.last;
+  wait_for_previous();   // (what is above depends on the call's arguments alone)
   int c0 = 0, c1 = -1;   // CTAs that have steps of this head
   if (any) {
-    const long long s0 = ahead + head * l.unit, s1 = s0 + l.unit - 1;
+    const long long total = __ldcg(p.table + a.c.B), s0 = __ldcg(p.table + b) + head * l.unit, s1 = s0 + l.unit;
     const int parts = weigh_parts(p, total);
-    c0 = (int)(((s0 + 1) * parts + total - 1) / total) - 1;
-    c1 = (int)(((s1 + 1) * parts + total - 1) / total) - 1;
+    c0 = (int)quotient((s0 + 1) * parts - 1, total);   // (the largest part that begins no later than step s0)
+    c1 = (int)quotient(s1 * parts - 1, total);
   }
-  wait_for_previous();   // (what is above depends on the call's arguments alone)
   const float* slot = p.part + ((size_t)c0 + bh) * p.sums * p.span + (any ? x - l.base : 0);
   const int terms = (c1 - c0 + 1) * p.sums;
 #pragma unroll 8
@@ -248,6 +235,7 @@ template <typename T> int by_code(const TdpWeighArgs& p, cudaStream_t stream) {
   }
 }
 
+size_t table_bytes(const tritt_cache_t& c) { return align_up(((size_t)c.B + 1) * 8, 256); }
 size_t slots_bytes(const tritt_cache_t& c, int span) { return (size_t)(kWeighCtas + (long long)c.B * c.N) * kWeighSums * span * 4; }
 
 }  // namespace
@@ -312,7 +300,7 @@ extern "C" {
 
 size_t tritt_tdp_weigh_workspace(const tritt_cache_t* c, int k1_window, int k2_window) {
   if (check_cache(c) || k1_window < 0 || k2_window < 0) return 0;
-  return slots_bytes(*c, weigh_span(*c, k1_window < kUnlimited ? k1_window : kUnlimited, k2_window < kUnlimited ? k2_window : kUnlimited));
+  return table_bytes(*c) + slots_bytes(*c, weigh_span(*c, k1_window < kUnlimited ? k1_window : kUnlimited, k2_window < kUnlimited ? k2_window : kUnlimited));
 }
 
 int tritt_tdp_weigh(const tritt_cache_t* c, const tritt_weights_t* w, const tritt_rows_t* q, const float* lse, int dtype, float alpha, int k1_window,
@@ -332,7 +320,7 @@ int tritt_tdp_weigh(const tritt_cache_t* c, const tritt_weights_t* w, const trit
   }
   auto window = [](int v) { return v < kUnlimited ? v : kUnlimited; };
   TdpWeighArgs p{cache_args(*c, status_word), *w, *q, lse, dtype, window(k1_window), window(k2_window), window(kk_left), window(kk_right), alpha * kLog2e,
-                 (float*)workspace, kWeighCtas, weigh_span(*c, window(k1_window), window(k2_window)), 0};
+                 (long long*)workspace, (float*)((uint8_t*)workspace + table_bytes(*c)), kWeighCtas, weigh_span(*c, window(k1_window), window(k2_window)), 0};
   const bool fast = sm100_tdp_weigh_supported(c->D);
   p.sums = fast ? 5 : 2;
   if (int rc = fast ? sm100_tdp_weigh(p, (cudaStream_t)stream) : mma_tdp_weigh(p, (cudaStream_t)stream)) return rc;

@@ -121,7 +121,8 @@ struct TdpWeighArgs {
   const float* lse;
   int dtype, k1w, k2w, kkl, kkr;
   float scale2;          // alpha * log2(e)
-  float* part;           // the workspace, see below
+  long long* table;      // the workspace: steps before each sequence, and of all ...
+  float* part;           // ... and slots, see below
   int ctas, span, sums;  // sums of a slot
 };
 
@@ -170,46 +171,57 @@ inline int weigh_span(const tritt_cache_t& c, int k1w, int k2w) {
 }
 constexpr int kWeighCtas = 148, kWeighSums = 5;   // the most sums of a slot
 
-// Sum of v over the block's threads, and the sum of those before this one.  `tmp`: 33 numbers of shared memory; all threads call it.
-__device__ __forceinline__ long long block_scan(long long v, long long* tmp, long long& total) {
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32;
-  long long s = v;
+// (a division of 64 bits is long, and few are needed)
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+  return ((unsigned long long)(a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
+}
+// CTAs that the line is cut among: each has a step at least.  Part i begins with step i * total / parts.
+__device__ __forceinline__ int weigh_parts(const TdpWeighArgs& a, long long total) { return total < a.ctas ? (int)total : a.ctas; }
+// The line's length, where this CTA's part begins, and the sequence that the step is of, with the number of the steps before its first.  A warp calls it together; that of the first CTA leaves the steps before each
+// sequence, and of all, in the workspace for the kernel that joins.
+struct WeighPart {
+  long long total, first, before;
+  int b;
+};
+__device__ __forceinline__ WeighPart weigh_part(const TdpWeighArgs& a) {
+  const int lane = threadIdx.x % 32;
+  WeighPart w{0, 0, 0, 0};
+  long long own = 0, behind = 0;   // steps of the lane's sequence, and of those up to it
+  auto sums = [&](int b0) {
+    const int b = b0 + lane;
+    own = b < a.cache.c.B ? weigh_line(a, b).unit * a.cache.c.N : 0;
+    long long s = own;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long u = __shfl_up_sync(0xffffffffu, s, o);
-    if (lane >= o) s += u;
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long u = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += u;
+    }
+    behind = w.before + s;
+  };
+  for (int b0 = 0; b0 < a.cache.c.B; b0 += 32) {
+    sums(b0);
+    if (blockIdx.x == 0 && b0 + lane < a.cache.c.B) a.table[b0 + lane] = behind - own;
+    w.before = __shfl_sync(0xffffffffu, behind, 31);
   }
-  __syncthreads();
-  if (lane == 31) tmp[warp] = s;
-  __syncthreads();
-  long long before = 0, all = 0;
-  for (int i = 0; i < warps; ++i) {
-    const long long u = tmp[i];
-    if (i < warp) before += u;
-    all += u;
+  w.total = w.before;
+  if (blockIdx.x == 0 && lane == 0) a.table[a.cache.c.B] = w.total;
+  const int parts = weigh_parts(a, w.total);
+  if ((int)blockIdx.x >= parts) return w;
+  w.first = quotient((long long)blockIdx.x * w.total, parts);
+  int b0 = 0;
+  if (a.cache.c.B > 32) {
+    w.before = 0;
+    for (;; b0 += 32) {
+      sums(b0);
+      const long long next = __shfl_sync(0xffffffffu, behind, 31);
+      if (w.first < next) break;
+      w.before = next;
+    }
   }
-  total = all;
-  return before + s - v;
-}
-// Steps of all sequences.
-__device__ __forceinline__ long long all_steps(const TdpWeighArgs& a, long long* tmp) {
-  long long v = 0, total;
-  for (int b = threadIdx.x; b < a.cache.c.B; b += blockDim.x) v += weigh_line(a, b).unit * a.cache.c.N;
-  block_scan(v, tmp, total);
-  return total;
-}
-// The sequence that step x is of, and the number of the steps before its first (in `at`, two numbers of shared memory).
-__device__ __forceinline__ void find_sequence(const TdpWeighArgs& a, long long x, long long* tmp, long long* at) {
-  long long run = 0;
-  for (int b0 = 0; b0 < a.cache.c.B; b0 += blockDim.x) {
-    const int b = b0 + threadIdx.x;
-    const long long v = b < a.cache.c.B ? weigh_line(a, b).unit * a.cache.c.N : 0;
-    long long total;
-    const long long before = run + block_scan(v, tmp, total);
-    if (v > 0 && x >= before && x < before + v) at[0] = b, at[1] = before;
-    run += total;
-  }
-  __syncthreads();
+  const int at = __ffs(__ballot_sync(0xffffffffu, w.first < behind)) - 1;
+  w.b = b0 + at;
+  w.before = __shfl_sync(0xffffffffu, behind - own, at);
+  return w;
 }
 // The i-th new token in the order of the line.  Later ones attend to more: in steps that are prime to their number and near its golden section, every stretch of the line has early
 // and late ones alike.
@@ -228,9 +240,6 @@ __device__ __forceinline__ int weigh_step(int cnt) {
   }
 }
 
-// CTAs that the line is cut among: each has a step at least.  Part i begins with step i * total / parts.
-__device__ __forceinline__ int weigh_parts(const TdpWeighArgs& a, long long total) { return total < a.ctas ? (int)total : a.ctas; }
-
 // A CTA's way along its part of the line.
 struct WeighPiece {
   int b, head, i, kg, s0, s1;   // token, tile of k, tiles of j (absolute)
@@ -243,21 +252,22 @@ struct WeighWalk {
   WeighLine l;
   bool fresh;
 };
-__device__ __forceinline__ WeighWalk weigh_start(const TdpWeighArgs& a, long long total, int b, long long before) {
-  const int parts = weigh_parts(a, total);
-  long long x = (long long)blockIdx.x * total / parts;
-  WeighWalk w{((long long)blockIdx.x + 1) * total / parts - x, b, 0, 0, 0, 0, 0, 1, {}, true};
-  w.l = weigh_line(a, b);
-  x -= before;
-  w.head = (int)(x / w.l.unit);
+__device__ __forceinline__ WeighWalk weigh_start(const TdpWeighArgs& a, const WeighPart& part) {
+  WeighWalk w{0, part.b, 0, 0, 0, 0, 0, 1, {}, true};
+  const int parts = weigh_parts(a, part.total);
+  if ((int)blockIdx.x >= parts) return w;
+  long long x = part.first - part.before;
+  w.left = quotient(((long long)blockIdx.x + 1) * part.total, parts) - part.first;
+  w.l = weigh_line(a, part.b);
+  w.head = (int)quotient(x, w.l.unit);
   x -= w.head * w.l.unit;
   const long long of_token = (long long)w.l.groups * w.l.slabs;
-  w.n = (int)(x / of_token);
+  w.n = (int)quotient(x, of_token);
   x -= w.n * of_token;
-  w.group = (int)(x / w.l.slabs);
+  w.group = (int)quotient(x, w.l.slabs);
   w.slab = (int)(x - (long long)w.group * w.l.slabs);
   w.step = weigh_step(w.l.cnt);
-  w.token = (int)((long long)w.n * w.step % w.l.cnt);
+  w.token = (int)((long long)w.n * w.step - quotient((long long)w.n * w.step, w.l.cnt) * w.l.cnt);
   return w;
 }
 __device__ __forceinline__ bool weigh_next(const TdpWeighArgs& a, WeighWalk& w, WeighPiece& s) {

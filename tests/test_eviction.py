@@ -676,5 +676,5 @@ def test_the_library_refuses():
     assert evict(keep=0) == -10 and evict(first=5, recent=5) == -10 and evict(first=-1) == -10 and evict(keep=17) == -1 and evict(left=None) == -4
     assert evict(left=p) == -4 and evict(kept=p + 2) == -5 and evict(out=(p, 0, 0)) == -12 and evict(out=(p, 0, 1), keep=17, w=dict(after_length=32)) == -12
     assert L.tritt_tdp_weigh_workspace(_native.Cache(**good), -1, 0) == 0
-    # 148 CTAs and a head, five sums of one tile of 128 tokens
-    assert L.tritt_tdp_weigh_workspace(_native.Cache(**good), 1 << 30, 0) == 149 * 5 * 128 * 4
+    # a small table; of 148 CTAs and a head five sums of one tile of 128 tokens
+    assert L.tritt_tdp_weigh_workspace(_native.Cache(**good), 1 << 30, 0) == 256 + 149 * 5 * 128 * 4
