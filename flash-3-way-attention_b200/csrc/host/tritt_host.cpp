@@ -613,6 +613,9 @@ bool read_weights(PyObject* before, PyObject* after, const tritt_cache_t& c, int
       return false;
   if (t[0]->data_ptr() == t[1]->data_ptr() && t[0]->strides() != t[1]->strides()) return false;
   auto stride = [](const at::Tensor* x, int i) { return x->size(i) > 1 ? (long long)x->stride(i) : 0; };
+  // (places that are several tokens': Python refuses them)
+  const long long L = t[1]->size(2), sb = stride(t[1], 0), sn = stride(t[1], 1);
+  if (!((c.N == 1 || sn >= L) && (c.B == 1 || sb >= (c.N == 1 ? L : c.N * sn))) && !((c.B == 1 || sb >= L) && (c.N == 1 || sn >= (c.B == 1 ? L : c.B * sb)))) return false;
   w.before = (const float*)t[0]->data_ptr(), w.after = (float*)t[1]->data_ptr();
   w.before_stride_b = stride(t[0], 0), w.before_stride_n = stride(t[0], 1), w.after_stride_b = stride(t[1], 0), w.after_stride_n = stride(t[1], 1);
   w.before_length = (int)t[0]->size(2), w.after_length = (int)t[1]->size(2);

@@ -357,8 +357,9 @@ template <typename T, int D, int CODE> int launch(Params p, cudaStream_t stream)
   p.chunk = n8 < most ? n8 : most;
   const int bytes = p.chunk * kBytesEach<T, D>;
   const long long blocks = (tokens + kTokens - 1) / kTokens;
-  // the new rows are formed once a block: it takes several times kTokens where there are blocks enough for all SMs several times over
-  long long repeat = blocks * c.B * c.N / (kSms * 3);
+  // the new rows are formed once a block: as many blocks as the chip holds at once (two an SM), each for as many times kTokens as that leaves
+  // (24 tokens over 3001, 4 x 16 heads of 128, fp16 codes: 29 us, with half as many tokens a block 36)
+  long long repeat = blocks * c.B * c.N / (kSms * 2);
   p.repeat = (int)(repeat < 1 ? 1 : repeat > 8 ? 8 : repeat);
   const dim3 grid((unsigned)((blocks + p.repeat - 1) / p.repeat), c.B * c.N);
   dps_weigh_kernel<T, D, CODE><<<grid, kThreads, bytes, stream>>>(p);

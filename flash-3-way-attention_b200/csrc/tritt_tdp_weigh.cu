@@ -235,8 +235,14 @@ template <typename T> int by_code(const TdpWeighArgs& p, cudaStream_t stream) {
   }
 }
 
+// Slots take a number for each token that a table has room for, whatever the contexts, and heads may be many: a call takes as many sequences at a time as keep them below this.
+constexpr long long kMostSlots = 1ll << 30;
+int sequences_at_once(const tritt_cache_t& c, int span) {
+  const long long heads = kMostSlots / (kWeighSums * 4ll * span) - kWeighCtas, n = heads / c.N;
+  return (int)(n < 1 ? 1 : n < c.B ? n : c.B);
+}
 size_t table_bytes(const tritt_cache_t& c) { return align_up(((size_t)c.B + 1) * 8, 256); }
-size_t slots_bytes(const tritt_cache_t& c, int span) { return (size_t)(kWeighCtas + (long long)c.B * c.N) * kWeighSums * span * 4; }
+size_t slots_bytes(const tritt_cache_t& c, int span) { return (size_t)(kWeighCtas + (long long)sequences_at_once(c, span) * c.N) * kWeighSums * span * 4; }
 
 }  // namespace
 
@@ -323,8 +329,22 @@ int tritt_tdp_weigh(const tritt_cache_t* c, const tritt_weights_t* w, const trit
                  (long long*)workspace, (float*)((uint8_t*)workspace + table_bytes(*c)), kWeighCtas, weigh_span(*c, window(k1_window), window(k2_window)), 0};
   const bool fast = sm100_tdp_weigh_supported(c->D);
   p.sums = fast ? 5 : 2;
-  if (int rc = fast ? sm100_tdp_weigh(p, (cudaStream_t)stream) : mma_tdp_weigh(p, (cudaStream_t)stream)) return rc;
-  return launch_tdp_weigh_join(p, (cudaStream_t)stream);
+  const int most = sequences_at_once(*c, p.span), size = dtype == TRITT_F32 ? 4 : 2;
+  for (int b0 = 0; b0 < c->B; b0 += most) {
+    TdpWeighArgs s = p;   // of sequences b0 and on
+    tritt_cache_t& some = s.cache.c;
+    some.B = c->B - b0 < most ? c->B - b0 : most;
+    some.table += b0 * c->table_stride;
+    some.context += b0;
+    if (some.counts) some.counts += b0;
+    s.q.p = (const uint8_t*)q->p + b0 * q->stride_b * size;
+    s.lse += (size_t)b0 * c->N * c->n;
+    s.w.before += b0 * w->before_stride_b;
+    s.w.after += b0 * w->after_stride_b;
+    if (int rc = fast ? sm100_tdp_weigh(s, (cudaStream_t)stream) : mma_tdp_weigh(s, (cudaStream_t)stream)) return rc;
+    if (int rc = launch_tdp_weigh_join(s, (cudaStream_t)stream)) return rc;
+  }
+  return 0;
 }
 
 }  // extern "C"

@@ -154,12 +154,11 @@ __device__ __forceinline__ WeighLine weigh_line(const TdpWeighArgs& a, int b) {
   l.base = (lo_j < lo_k ? l.j0 : l.k0) * 128;
   l.slabs = l.last / 128 - l.j0 + 1;
   l.groups = l.last / 128 - l.k0 + 1;
-  l.unit = (long long)l.cnt * l.groups * l.slabs;
-  if (l.unit > kMostWeighSteps && a.cache.status) atomicOr(a.cache.status, kStatusTdpDecode);
-  if (l.slabs <= 0 || l.groups <= 0 || l.unit > kMostWeighSteps) {
-    l.cnt = l.groups = l.slabs = 0;
-    l.unit = 0;
-  }
+  const long long of_token = (long long)l.groups * l.slabs;
+  const bool much = l.slabs > 0 && l.groups > 0 && l.cnt > kMostWeighSteps / of_token;   // reported, and left out
+  if (much && a.cache.status) atomicOr(a.cache.status, kStatusTdpDecode);
+  if (l.slabs <= 0 || l.groups <= 0 || much) l.cnt = l.groups = l.slabs = 0;
+  l.unit = l.cnt * of_token;
   return l;
 }
 // 128-token tiles that a slot has room for: what the windows and the new tokens can touch, at most the table (or the weights)

@@ -40,6 +40,11 @@ def _weights(cache, table, weights, out, decay=1.0):
             raise ValueError(f"{name} must have their tokens next to one another, got strides {t.stride()}")
         if t.requires_grad:
             raise ValueError(f"{name} are sums that calls add to: no gradient flows through them")
+    room = 1
+    for size, step in sorted(((n, st) for n, st in zip(out.shape, out.stride()) if n > 1), key=lambda x: x[1]):
+        if step < room:
+            raise ValueError(f"the new weights have places that are several tokens' (strides {out.stride()} of shape {list(out.shape)})")
+        room = step * size
     if out.data_ptr() == weights.data_ptr() and out.stride() != weights.stride():
         raise ValueError("the new weights start where the old ones do, but are laid out in another way")
     if not (math.isfinite(decay) and decay >= 0):

@@ -279,6 +279,32 @@ def test_nothing_attended_missing_places_and_short_weights(form, D):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 32])
+def test_a_table_far_longer_than_the_sequences(D):
+    """Scratch for all of a table's tokens: a call takes some sequences at a time."""
+    B = 40
+    bt = Weighed(B, 2, 1, D, "fp16", "int8", 256, [b * 31 % 90 - 1 for b in range(B)], strided=False)
+    table = torch.nn.functional.pad(bt.table, (0, 1024 - bt.table.shape[1]), value=0)
+    c = _native.Cache(codes=bt.cache.codes.data_ptr(), exponents=bt.cache.exponents.data_ptr(), pages=bt.cache.codes.shape[0], page_size=256, N=2, D=D, code=2,
+                      table=table.data_ptr(), table_stride=1024, table_pages=1024, context=bt.context.data_ptr(), B=B, n=1)
+    whole = (148 + 2 * B) * 5 * 256 * 1024 * 4
+    assert 0 < _native.lib().tritt_tdp_weigh_workspace(c, 1 << 30, 1 << 30) < min(whole, 1 << 30)
+    bt.check(bt.run(table=table))
+    ft.check_status(DEV)
+
+
+@pytest.mark.gpu
+def test_weights_that_share_places_are_refused():
+    bt = Weighed(2, 2, 1, 64, "bf16", "e4m3", 16, [20, 10])
+    for w in (torch.zeros(1, 2, 40, device=DEV).expand(2, 2, 40), torch.zeros(2, 1, 40, device=DEV).expand(2, 2, 40), torch.zeros(400, device=DEV).as_strided((2, 2, 40), (39, 80, 1))):
+        with pytest.raises(ValueError):
+            bt.run(weights=torch.zeros(2, 2, 40, device=DEV), out=w)
+    out = torch.zeros(400, device=DEV).as_strided((2, 2, 40), (50, 100, 1))   # (sequences within heads)
+    bt.run(weights=bt.before.to(DEV), out=out[:, :, : bt.length])
+    bt.check(out[:, :, : bt.length], stale=torch.zeros_like(bt.before))
+
+
+@pytest.mark.gpu
 def test_many_sequences_and_heads():
     """More sequences than a block has threads, most of them short or unused: the line over all of them."""
     B = 700
@@ -456,6 +482,16 @@ def test_shared_pages_and_places_that_there_are_not():
 
 
 @pytest.mark.gpu
+def test_eviction_with_weights_for_fewer_tokens():
+    bt = Full(1, 2, 64, "int8", 16, [100], length=60)
+    _, kept = ft.cache_evict(bt.weights.to(DEV), bt.cache, bt.table, bt.context, 20, 2, 3)
+    with pytest.raises(_native.TrittError):
+        ft.check_status(DEV)
+    for h in range(2):
+        assert kept[0, h].tolist() == orc.evicted(bt.weights[0, h].tolist(), 60, 20, 2, 3)
+
+
+@pytest.mark.gpu
 def test_evict_in_a_graph_and_again():
     """Captured, replayed while contexts and weights change; twice in a row, in place."""
     bt = Full(2, 2, 64, "fp16", 16, [90, 50], dps=True)
@@ -628,6 +664,10 @@ def test_refusals(monkeypatch):
     base = torch.zeros(2 * 40)
     with pytest.raises(ValueError):   # one place, two layouts
         tdp(w=base[:64].view(1, 2, 32), out=base.view(1, 2, 40))
+    for x in (torch.zeros(1, 1, 32).expand(1, 2, 32), base.as_strided((1, 2, 32), (80, 20, 1))):   # one place, several tokens
+        for call in (tdp, dps, evict):
+            with pytest.raises(ValueError):
+                call(w=x)
     for kw in (dict(keep=0), dict(first=-1), dict(recent=-1), dict(first=5, recent=5), dict(keep=33), dict(weights_out=torch.zeros(1, 2, 8)),
                dict(table_out=table.long()), dict(table_out=torch.zeros(2, 2, dtype=torch.int32)), dict(keep=17, table_out=table[:, :1]),
                dict(table_out=table[0]), dict(keep=1 << 40)):
