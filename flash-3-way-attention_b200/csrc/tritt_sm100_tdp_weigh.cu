@@ -168,6 +168,8 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_weigh_sm100_kernel(const __gr
     tmem_alloc(&ms.tmem_base, 512);
     tmem_relinquish();
   }
+  WeighWalk walk{};
+  if (warp == 1) walk = weigh_start(p, weigh_part(p));   // (beside the others' preparations; a CTA without a part has no pieces)
   let_next_start();
   tc_fence_before();
   __syncthreads();
@@ -190,7 +192,6 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_weigh_sm100_kernel(const __gr
     set_regs<kRegsLaunch, kRegsIssue>();
     if (warp == 1) {
       // ------------------------------------------------------------------ pieces
-      WeighWalk walk = weigh_start(p, weigh_part(p));   // (a CTA without a part has no pieces)
       WeighPiece s;
       bool more = !*abort_flag;
       for (int count = 0; more; ++count) {

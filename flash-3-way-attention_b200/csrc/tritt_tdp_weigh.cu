@@ -207,8 +207,13 @@ __global__ void __launch_bounds__(256) tdp_weigh_join_kernel(const __grid_consta
   }
   const float* slot = p.part + ((size_t)c0 + bh) * p.sums * p.span + (any ? x - l.base : 0);
   const int terms = (c1 - c0 + 1) * p.sums;
-#pragma unroll 8
-  for (int i = 0; i < terms; ++i) sum += slot[(size_t)i * p.span];
+  for (int i0 = 0; i0 < terms; i0 += 16) {   // (sixteen on their way together, the last ones too)
+    float some[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) some[k] = i0 + k < terms ? __ldcg(slot + (size_t)(i0 + k) * p.span) : 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) sum += some[k];
+  }
   if (x < end) *weight_of(p.w, b, head, x) = v + sum;
 }
 
