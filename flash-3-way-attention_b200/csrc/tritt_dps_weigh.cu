@@ -91,124 +91,156 @@ __device__ __forceinline__ void form_queries(const Params& p, int b, int head, i
 }
 
 // A few new tokens, rows of up to 128 bytes: 32 tokens a warp at a time, in two products' fragments, whose scores then change lanes so that each lane has one token, its row's exponent, its
-// log-sum-exp and its weight (with two tokens a lane of four and eight columns for one new token the kernel above executed four times the instructions: 178 us for 32 x 16 heads over
-// 8191, e4m3).
+// log-sum-exp and its weight (with two tokens a lane of four and eight columns for one new token the kernel below executed four times the instructions: 178 us for 32 x 16 heads over
+// 8191, e4m3).  A warp's rows, K2's and then, where a new token's k2 attends to them, K1's, come by asynchronous copies into places of its own, two steps ahead (a step ahead in
+// registers: 105 us; so 75, and 84 with three steps ahead for two blocks an SM).
 constexpr int kFew = 4, kFewTokens = 256;   // new tokens at most; of a block at a time
 template <int D, int CODE> constexpr bool kFewApplies = RowFragments<D, CODE>::kWords <= 8;
+template <int D, int CODE> struct FewStage {   // of a warp
+  uint8_t codes[32 * D * RowFragments<D, CODE>::kSize];
+  float lse[32], before[32];
+  uint8_t exponent[32];
+};
+constexpr int kFewStages = 3;
+template <int D, int CODE> constexpr int kFewSmem = kThreads / 32 * kFewStages * (int)sizeof(FewStage<D, CODE>);
 
-template <typename T, int D, int CODE> __global__ void __launch_bounds__(kThreads, 2) dps_weigh_few_kernel(const __grid_constant__ Params p) {
+__device__ __forceinline__ void copy_if(void* dst, const void* src, bool on) {   // 16 bytes, zeros where not (src: an address that can be read)
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4_if(void* dst, const void* src, bool on) {   // four bytes
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "r"(on ? 4 : 0) : "memory");
+}
+
+template <typename T, int D, int CODE> __global__ void __launch_bounds__(kThreads, RowFragments<D, CODE>::kWords <= 4 ? 3 : 2) dps_weigh_few_kernel(const __grid_constant__ Params p) {
   using Rows = RowFragments<D, CODE>;
+  using Stage = FewStage<D, CODE>;
   constexpr bool kWide = std::is_same<T, float>::value;
-  constexpr int kSteps = Rows::kSteps, kHalves = kWide ? 2 : 1;
-  extern __shared__ __align__(16) uint2 frags[];   // [part][hi, lo][step][lane]
+  constexpr int kSteps = Rows::kSteps, kHalves = kWide ? 2 : 1, NS = kFewStages;
+  constexpr int kRow = D * Rows::kSize, kChunks = kRow / 16;
+  extern __shared__ __align__(16) uint8_t smem[];   // stages of the warps, then fragments [part][hi, lo][step][lane]
   __shared__ Query queries[2][64];
   const CacheArgs& a = p.cache;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  Stage* const stages = reinterpret_cast<Stage*>(smem) + warp * NS;
+  uint2* const frags = reinterpret_cast<uint2*>(smem + kFewSmem<D, CODE>);
   const int bh = blockIdx.y, b = bh / a.c.N, head = bh - b * a.c.N;
   if (__ldg(a.c.context + b) < 0) return;
   const int ctx = context_of(a, b), cnt = new_tokens(a, b), end = weighed_tokens(a, p.w, ctx + cnt);
   const int first = blockIdx.x * p.repeat * kFewTokens + warp * 32;
   if ((int)blockIdx.x * p.repeat * kFewTokens >= end) return;
   const int behind = ctx - (p.k_diff < ctx ? p.k_diff : ctx);   // the first token that any new one's k2 attends to
-  const uint8_t* codes = (const uint8_t*)a.c.codes;
-  constexpr size_t kRow = D * Rows::kSize;
+  const uint8_t* const codes = (const uint8_t*)a.c.codes;
   const size_t part_rows = (size_t)a.c.N << a.page_log2;
-
-  struct Step {
-    Rows k2[2], k1[2];
-    uint32_t byte;        // K2's exponent, K1's
-    float lse, before;
-    uint32_t there;       // bit t: the 16 tokens have a place
-    bool inner;
-  };
-  // the page of the lane's token, as the table has it (a step before it is needed, and not looked at here, so that nothing waits for it); -1: the token is not there, or the table has none
-  int steps = end > first ? (end - first + kFewTokens - 1) / kFewTokens : 0;   // of this warp
+  int steps = end > first ? (end - first + kFewTokens - 1) / kFewTokens : 0;   // of this warp, 32 tokens each
   if (steps > p.repeat) steps = p.repeat;
+  auto inner = [&](int r) { return cnt > 0 && first + r * kFewTokens + 31 >= behind; };
+
+  // the page of the lane's token, as the table has it (a step before it is needed, and not looked at here, so that nothing waits for it); -1: the token is not there, or the table has none
   auto page_of = [&](int r) {
     const int x = first + r * kFewTokens + lane, i = x >> a.page_log2;
     int page = -1;
     if (r < steps && x < end && i < a.c.table_pages) page = __ldg(a.c.table + b * a.c.table_stride + i);
     return page;
   };
-  auto fetch = [&](int r, Step& t, int page) {
-    const int x0 = first + r * kFewTokens, x = x0 + lane;
-    const bool on = page >= 0 && page < a.c.pages;
-    if (x < end && !on && a.status) atomicOr(a.status, kStatusPlace);
-    const Place at{page, x & (a.c.page_size - 1)};
-    const size_t row = on ? row_of(a, at, kPartK2, head) : 0;
-    t.inner = x0 + 31 >= behind;
-    t.byte = 0;
-    t.lse = t.before = 0.f;
-    if (on) {
-      t.lse = __ldg(a.c.lse + lse_of(a, at, head));
-      t.byte = __ldg(a.c.exponents + row);
-      if (t.inner) t.byte |= (uint32_t)__ldg(a.c.exponents + row - part_rows) << 8;   // (K1's row lies a part ahead)
+  // What is sent next: K2's rows of step `ahead`, or its K1's; one group of copies each, empty ones at the end.
+  int ahead = 0, slot = 0, page = page_of(0);
+  bool second = false;
+  size_t row = 0;             // number of the lane's K2 row
+  bool on = false;
+  auto send = [&]() {
+    if (ahead < steps) {
+      Stage& to = stages[slot];
+      const int x = first + ahead * kFewTokens + lane;
+      if (!second) {
+        on = page >= 0 && page < a.c.pages;
+        if (x < end && !on && a.status) atomicOr(a.status, kStatusPlace);
+        const Place at{page, x & (a.c.page_size - 1)};
+        row = on ? row_of(a, at, kPartK2, head) : 0;
+        copy4_if(&to.lse[lane], on ? a.c.lse + lse_of(a, at, head) : a.c.lse, on);
+        page = page_of(ahead + 1);
+        const bool old = x < end && x < ctx && p.w.decay != 0.f;
+        copy4_if(&to.before[lane], old ? p.w.before + b * p.w.before_stride_b + head * p.w.before_stride_n + x : p.w.before, old);
+      }
+      const size_t mine = second ? row - part_rows : row;   // (K1's rows lie a part ahead)
+      if (lane % 4 == 0) copy4_if(&to.exponent[lane], on ? a.c.exponents + mine : a.c.exponents, on);
+#pragma unroll
+      for (int k = 0; k < kChunks; ++k) {
+        const int at = k * 32 + lane, from = at / (16 * kChunks) * 16;   // (16 tokens' rows follow one another)
+        const size_t base = (size_t)__shfl_sync(0xffffffffu, (uint32_t)(mine >> 32), from) << 32 | __shfl_sync(0xffffffffu, (uint32_t)mine, from);
+        const bool there = __shfl_sync(0xffffffffu, (int)on, from);
+        copy_if(to.codes + at * 16, there ? codes + base * kRow + at % (16 * kChunks) * 16 : codes, there);
+      }
+      if (!second && inner(ahead)) {
+        second = true;
+      } else {
+        second = false;
+        ++ahead;
+      }
+      if (++slot == NS) slot = 0;
     }
-    if (x < end && x < ctx) t.before = faded(p.w, b, head, x);
-    t.there = 0;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  // the scores of the 32 tokens of a stage, and what they add to them
+  auto gain = [&](const Stage& from, int part, int x, float lse) {
+    float d[2][4];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const size_t base = (size_t)__shfl_sync(0xffffffffu, (uint32_t)(row >> 32), 16 * h) << 32 | __shfl_sync(0xffffffffu, (uint32_t)row, 16 * h);
-      if (!__shfl_sync(0xffffffffu, (int)on, 16 * h)) continue;
-      t.there |= 1u << h;
-      t.k2[h].load(codes + base * kRow, lane);
-      if (t.inner) t.k1[h].load(codes + (base - part_rows) * kRow, lane);
-    }
-  };
-  auto work = [&](int r, const Step& t) {
-    const int x0 = first + r * kFewTokens, x = x0 + lane;
-    float sum = t.before;
-    if (t.there && cnt > 0) {
+      Rows rows;
+      rows.load_copy(from.codes + h * 16 * kRow, lane);
 #pragma unroll
-      for (int part = 0; part < 2; ++part) {
-        if (part && !t.inner) break;
-        float d[2][4];
+      for (int k = 0; k < 4; ++k) d[h][k] = 0.f;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) d[h][k] = 0.f;
-#pragma unroll
-          for (int s = 0; s < kSteps; ++s) {
-            uint32_t frag[4];
-            (part ? t.k1[h] : t.k2[h]).step(s, frag);
-            const uint2* from = frags + (size_t)(part * kHalves * kSteps + s) * 32 + lane;
-            mma_16816(d[h], frag, from[0]);
-            if constexpr (kWide) mma_16816(d[h], frag, from[kSteps * 32]);
-          }
-        }
-        const float scale = code_scale(t.byte >> 8 * part & 255);
-        const bool there = t.there >> (lane / 16) & 1;
-#pragma unroll
-        for (int n = 0; n < kFew; ++n) {
-          if (n >= cnt) break;
-          // the score of this lane's token: row lane % 16 of half lane / 16
-          const int from = lane % 8 * 4 + n / 2;
-          const float s0 = __shfl_sync(0xffffffffu, d[0][n % 2], from), s1 = __shfl_sync(0xffffffffu, d[0][2 + n % 2], from);
-          const float s2 = __shfl_sync(0xffffffffu, d[1][n % 2], from), s3 = __shfl_sync(0xffffffffu, d[1][2 + n % 2], from);
-          const float score = lane < 16 ? (lane < 8 ? s0 : s1) : (lane < 24 ? s2 : s3);
-          const Query q = queries[part][n];
-          const bool on = there && x <= q.last && (part == 0 || q.last - x <= p.k_diff);
-          const float less = part == 0 ? t.lse - q.minus : -q.minus;
-          sum += on ? exp2f(fmaf(score * scale, q.scale, less * kLog2e)) : 0.f;
-        }
+      for (int s = 0; s < kSteps; ++s) {
+        uint32_t frag[4];
+        rows.step(s, frag);
+        const uint2* f = frags + (size_t)(part * kHalves * kSteps + s) * 32 + lane;
+        mma_16816(d[h], frag, f[0]);
+        if constexpr (kWide) mma_16816(d[h], frag, f[kSteps * 32]);
       }
     }
-    if (x < end) *weight_of(p.w, b, head, x) = sum;
+    const float scale = code_scale(from.exponent[lane]);
+    float sum = 0.f;
+#pragma unroll
+    for (int n = 0; n < kFew; ++n) {
+      if (n >= cnt) break;
+      // the score of this lane's token: row lane % 16 of half lane / 16
+      const int at = lane % 8 * 4 + n / 2;
+      const float s0 = __shfl_sync(0xffffffffu, d[0][n % 2], at), s1 = __shfl_sync(0xffffffffu, d[0][2 + n % 2], at);
+      const float s2 = __shfl_sync(0xffffffffu, d[1][n % 2], at), s3 = __shfl_sync(0xffffffffu, d[1][2 + n % 2], at);
+      const float score = lane < 16 ? (lane < 8 ? s0 : s1) : (lane < 24 ? s2 : s3);
+      const Query q = queries[part][n];
+      const bool seen = x <= q.last && (part == 0 || q.last - x <= p.k_diff);
+      const float less = part == 0 ? lse - q.minus : -q.minus;
+      sum += seen ? exp2f(fmaf(score * scale, q.scale, less * kLog2e)) : 0.f;
+    }
+    return sum;
   };
-  Step even, odd;
-  int page_even = page_of(0), page_odd = page_of(1);
-  if (steps > 0) fetch(0, even, page_even);
-  page_even = page_of(2);
+  for (int k = 0; k < NS - 1; ++k) send();
   if (cnt > 0) form_queries<T, D, CODE>(p, b, head, ctx, 0, cnt, 1, frags, queries);
   __syncthreads();
-  for (int r = 0; r < steps; r += 2) {   // the next step's rows are on their way while one is worked on
-    if (r + 1 < steps) fetch(r + 1, odd, page_odd);
-    page_odd = page_of(r + 3);
-    work(r, even);
-    if (r + 1 >= steps) break;
-    if (r + 2 < steps) fetch(r + 2, even, page_even);
-    page_even = page_of(r + 4);
-    work(r + 1, odd);
+  int use = 0;
+  int there_page = page_of(0);   // (whether the step's tokens have places, for what they get)
+  for (int r = 0; r < steps; ++r) {
+    const int x = first + r * kFewTokens + lane;
+    const bool there = there_page >= 0 && there_page < a.c.pages;
+    there_page = page_of(r + 1);
+    float sum = 0.f;
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+      if (part && !inner(r)) break;
+      asm volatile("cp.async.wait_group %0;" ::"n"(NS - 2) : "memory");
+      __syncwarp();
+      const Stage& from = stages[use];
+      if (part == 0 && p.w.decay != 0.f) sum = p.w.decay * from.before[lane];
+      if (cnt > 0) {
+        const float more = gain(from, part, x, part == 0 ? from.lse[lane] : 0.f);
+        if (there) sum += more;
+      }
+      __syncwarp();   // (the stage has been read)
+      if (++use == NS) use = 0;
+      send();
+    }
+    if (x < end) *weight_of(p.w, b, head, x) = sum;
   }
 }
 
@@ -347,7 +379,9 @@ template <typename T, int D, int CODE> int launch(Params p, cudaStream_t stream)
     if (c.n <= kFew) {
       const long long blocks = (tokens + kFewTokens - 1) / kFewTokens, repeat = blocks * c.B * c.N / (kSms * 12);
       p.repeat = (int)(repeat < 1 ? 1 : repeat > 8 ? 8 : repeat);
-      dps_weigh_few_kernel<T, D, CODE><<<dim3((unsigned)((blocks + p.repeat - 1) / p.repeat), c.B * c.N), kThreads, 8 * kBytesEach<T, D>, stream>>>(p);
+      const int bytes = kFewSmem<D, CODE> + 8 * kBytesEach<T, D>;
+      TRITT_CUDA_OK(cudaFuncSetAttribute(dps_weigh_few_kernel<T, D, CODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+      dps_weigh_few_kernel<T, D, CODE><<<dim3((unsigned)((blocks + p.repeat - 1) / p.repeat), c.B * c.N), kThreads, bytes, stream>>>(p);
       count_launch();
       TRITT_CUDA_OK(cudaGetLastError());
       return 0;

@@ -62,7 +62,10 @@ template <int D, int CODE> struct RowFragments {
   static constexpr int kWords = kLane / 4;
   uint32_t v[2][kWords];
   // row: the first of the 16 (they follow one another)
-  __device__ __forceinline__ void load(const uint8_t* row, int lane) {
+  __device__ __forceinline__ void load(const uint8_t* row, int lane) { load_by(row, lane, [](const auto* p) { return __ldg(p); }); }
+  // ... of a copy of the rows in shared memory
+  __device__ __forceinline__ void load_copy(const uint8_t* row, int lane) { load_by(row, lane, [](const auto* p) { return *p; }); }
+  template <typename F> __device__ __forceinline__ void load_by(const uint8_t* row, int lane, F&& get) {
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const uint8_t* p = row + (size_t)(lane / 4 + 8 * r) * (D * kSize) + lane % 4 * kChunk;
@@ -70,22 +73,16 @@ template <int D, int CODE> struct RowFragments {
       for (int i = 0; i < kChunks; ++i) {
         uint32_t* to = v[r] + i * (kChunk / 4);
         if constexpr (kChunk == 16) {
-          const uint4 x = __ldg(reinterpret_cast<const uint4*>(p + i * 64));
+          const uint4 x = get(reinterpret_cast<const uint4*>(p + i * 64));
           to[0] = x.x, to[1] = x.y, to[2] = x.z, to[3] = x.w;
         } else if constexpr (kChunk == 8) {
-          const uint2 x = __ldg(reinterpret_cast<const uint2*>(p));
+          const uint2 x = get(reinterpret_cast<const uint2*>(p));
           to[0] = x.x, to[1] = x.y;
         } else {
-          to[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+          to[0] = get(reinterpret_cast<const uint32_t*>(p));
         }
       }
     }
-  }
-  __device__ __forceinline__ void clear() {
-#pragma unroll
-    for (int r = 0; r < 2; ++r)
-#pragma unroll
-      for (int i = 0; i < kWords; ++i) v[r][i] = 0;
   }
   // fragments of one instruction
   __device__ __forceinline__ void step(int s, uint32_t (&a)[4]) const {
