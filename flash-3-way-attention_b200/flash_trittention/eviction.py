@@ -69,7 +69,7 @@ def tdp_weigh(weights: Tensor, q: Tensor, lse: Tensor, cache: TrittentionCache, 
     for the same arguments; a token whose ``lse`` is ``-inf`` adds nothing.  Of the new tokens' own weights what was there before does not count.  Weights of tokens past ``context[b] + counts[b]`` and of free
     slots stay; a token that ``weights`` has no place for is reported by the next call or ``check_status()``.
 
-    ``out``: the new weights go there, and ``weights`` stays (drafts that may be rejected, say).  Drafts are weighed once they are accepted, as a chain.
+    ``out``: the new weights go there, and ``weights`` stays (drafts that may be rejected, say); of its memory it is ``weights`` itself or shares none with it.  Drafts are weighed once they are accepted, as a chain.
     Scores have at least 22 significant bits, everything else is fp32; a call repeats itself bit for bit."""
     softmax_scale, decay = float(softmax_scale), float(decay)
     if torch.compiler.is_compiling():
@@ -121,7 +121,7 @@ def cache_evict(weights: Tensor, cache: TrittentionCache, table: Tensor, context
     behind the last.  A sequence that has no more than ``keep`` tokens keeps them all, a free slot of the batch stays one.
 
     The kept rows, exponents and log-sum-exps become tokens ``0, 1, 2, ...``, and so do their weights; the pages behind them are free (what they hold is left as it is).  A page that several sequences
-    share must not be written: with ``table_out`` (int32 ``[B, pages]``, of pages that the call does not read) the rows go there and the old ones stay, and with ``weights_out`` (float32 ``[B, N, tokens]``)
+    share must not be written: with ``table_out`` (int32 ``[B, pages]``, of pages that the call does not read) the rows go there and the old ones stay, and with ``weights_out`` (float32 ``[B, N, tokens]``, of memory that ``weights`` has no part of)
     the weights."""
     keep, first, recent = int(keep), int(first), int(recent)
     if keep < 1 or first < 0 or recent < 0 or first + recent > keep:

@@ -20,7 +20,7 @@
  *     is OR-ed with a non-zero code by a kernel whose bounded barrier wait ran out (1 tensor-core
  *     self-test, 2 / 4 triple-dot-product forward / backward, 8 misaligned shared memory, 16 / 32
  *     soft-max attention forward / backward of the dot-product-sum path, 128 wait-expiry self-test, 1024
- *     triple-dot-product attention over a cache) or,
+ *     triple-dot-product attention over a cache, or its weights) or,
  *     bit 64, by the fp16 operand conversion of an fp32 / wide-operand call that met an element beyond 65504,
  *     bit 256, by a rotation whose position its tables do not have, bit 512, by a call that met a place its cache does not have;
  *     the caller zeroes and reads it.  A non-zero word means the results of that call are invalid;
@@ -394,7 +394,7 @@ int tritt_dps_weigh(const tritt_cache_t* c, const tritt_weights_t* w, const trit
  * the largest w->before (ties: the lower number; NaN counts as the largest), first + recent <= keep.  Their rows and log-sum-exps move to the places of tokens 0, 1, 2, ...
  * in order, and their weights to w->after; kept [B, N, keep] gets their numbers, -1 behind the last, context_out [B] the tokens that are left.  A sequence that has no more than
  * `keep` tokens keeps all of them; context[b] < 0 stays as it is.
- * table_out null: in place (the places behind the last kept token keep what they hold).  Else the rows go to the pages of table_out, [B, table_out_pages] with stride
+ * table_out null, or c->table itself: in place (the places behind the last kept token keep what they hold).  Else the rows go to the pages of table_out, [B, table_out_pages] with stride
  * table_out_stride, of which none may be one that the call reads, and the old ones stay as they are.  A page that several sequences share must not be written.
  * A place that there is not sets status bit 512; what it should have held, or should hold, is left out.  So does a token beyond before_length.
  * w->decay is not looked at.  w->after may be w->before (with the same strides), or must not overlap it; after_length >= keep.

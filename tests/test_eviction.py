@@ -433,6 +433,28 @@ def test_evict(B, N, D, code, page, contexts, keep, first, recent, dps, elsewher
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("B,N,D,ctx,keep", [(1, 1, 64, 9000, 6000), (1, 2, 16, 40000, 30000), (2, 2, 128, 700, 600)])
+@pytest.mark.parametrize("table_too", [False, True])
+def test_rows_to_other_pages_and_weights_in_place(B, N, D, ctx, keep, table_too):
+    """Few heads and many tokens: several blocks move one head's rows.  A table that is the one for reading is a call in place."""
+    bt = Full(B, N, D, "fp16", 64, [ctx] * B, length=ctx + 3)
+    few = -(-keep // 64)
+    old = bt.cache.codes.shape[0]
+    bt.cache = ft.TrittentionCache(*(None if t is None else torch.cat((t, torch.zeros((B * few, *t.shape[1:]), dtype=t.dtype, device=DEV))) for t in bt.cache))
+    table_out = bt.table if table_too else torch.arange(old, old + B * few, device=DEV).view(B, few).int()
+    before, weights = bt.rows(bt.table, ctx), bt.weights.to(DEV)
+    left, kept = ft.cache_evict(weights, bt.cache, bt.table, bt.context, keep, 2, 7, table_out=table_out)
+    ft.check_status(DEV)
+    after = bt.rows(table_out, keep)
+    for b in range(B):
+        for h in range(N):
+            want = orc.evicted(bt.weights[b, h].tolist(), ctx, keep, 2, 7)
+            assert int(left[b]) == keep and kept[b, h].tolist() == want
+            assert torch.equal(weights[b, h].cpu(), torch.cat((bt.weights[b, h, want], bt.weights[b, h, keep:])))
+            assert all(torch.equal(y[b, :, h], x[b, :, h][:, want]) for x, y in zip(before, after))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("ctx", [300, 30000])
 def test_order_of_weights(ctx):
     """Infinities, NaN, zeros of either sign, negative ones, numbers next to one another; one CTA and a cluster."""
