@@ -6,6 +6,8 @@
 // A warp takes 16 tokens: their rows go from memory straight into the fragments of warp-level matrix instructions (eight new tokens the other side, in shared memory in the order of
 // the fragments), exact as fp16 codes; each row's exponent, and the new row's, multiply the sums.  fp32 rows are two fp16 numbers (22 bits), as the products are
 // summed in fp32 all the same.
+// Measured: a token of 32 x 16 heads of 64 over up to 8191, e4m3, 75 us (278 MB, 3.7 TB/s; 70 % of the issue slots); 24 tokens over 3001, 4 x 16 heads of 128, fp16 codes 31 us (78 MB; a block's way to its first
+// tile, and one tile behind the other).
 #include "tritt_weigh.cuh"
 
 #include <type_traits>

@@ -13,7 +13,7 @@
 // The tables (a cosine and a sine, 8 bytes, for two elements) would be twice the traffic of 16-bit rows, so a thread keeps its position's
 // values for four heads and, where there are blocks enough, all three tensors.
 // Positions of several axes are kernels of their own (AXES): the same, but that a lane whose four pairs are not all of one axis takes their values one
-// by one.  4 x 16 heads x 2048 x 128 bf16, three axes: forward 45.4 us one after the other and 45.9 in turn, 44.6 with one axis; backward 74 and 75.
+// by one.  4 x 16 heads x 2048 x 128 bf16, three axes: forward 45.4 us one axis after the other and 45.9 in turn, 44.6 with one axis; forward and backward 136 in turn (132 with one).
 #include "tritt_cache.cuh"
 #include "tritt_common.cuh"
 
