@@ -1,5 +1,5 @@
 // The attention weight of cached tokens in the triple dot product, with warp-level matrix instructions: head dimensions
-// 16, 32 and 256 (64 and 128 run on tcgen05).
+// 16, 32 and 256 (64 and 128 run on tcgen05, or where their rows fit in shared memory as the windows' kernel).
 //
 //   P[j, k] = exp(alpha sum_h q[h] K1[j, h] K2[k, h] - lse),   w[x] = decay w[x] + sum_i (sum_k P_i[x, k] + sum_j P_i[j, x])
 // For one new token and a tile of 128 tokens k the operand A[k] = q * K2[k] is formed once, as two fp16 numbers an element (22 bits: 16-bit queries times any code are exact), in the order of the
@@ -332,6 +332,7 @@ int tritt_tdp_weigh(const tritt_cache_t* c, const tritt_weights_t* w, const trit
   auto window = [](int v) { return v < kUnlimited ? v : kUnlimited; };
   TdpWeighArgs p{cache_args(*c, status_word), *w, *q, lse, dtype, window(k1_window), window(k2_window), window(kk_left), window(kk_right), alpha * kLog2e,
                  (long long*)workspace, (float*)((uint8_t*)workspace + table_bytes(*c)), kWeighCtas, weigh_span(*c, window(k1_window), window(k2_window)), 0};
+  if (window_tdp_weigh_applies(p)) return window_tdp_weigh(p, (cudaStream_t)stream);
   const bool fast = sm100_tdp_weigh_supported(c->D);
   p.sums = fast ? 5 : 2;
   const int most = sequences_at_once(*c, p.span), size = dtype == TRITT_F32 ? 4 : 2;

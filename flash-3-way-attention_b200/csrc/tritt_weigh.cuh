@@ -321,6 +321,9 @@ __device__ __forceinline__ float* weigh_slot(const TdpWeighArgs& a, int b, int h
 bool sm100_tdp_weigh_supported(int D);
 int sm100_tdp_weigh(const TdpWeighArgs& a, cudaStream_t stream);
 int mma_tdp_weigh(const TdpWeighArgs& a, cudaStream_t stream);
+// where the rows fit in shared memory: one launch, which writes the new weights, too
+bool window_tdp_weigh_applies(const TdpWeighArgs& a);
+int window_tdp_weigh(const TdpWeighArgs& a, cudaStream_t stream);
 int launch_tdp_weigh_join(const TdpWeighArgs& a, cudaStream_t stream);
 
 }  // namespace tritt

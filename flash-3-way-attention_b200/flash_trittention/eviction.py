@@ -70,7 +70,7 @@ def tdp_weigh(weights: Tensor, q: Tensor, lse: Tensor, cache: TrittentionCache, 
     slots stay; a token that ``weights`` has no place for is reported by the next call or ``check_status()``.
 
     ``out``: the new weights go there, and ``weights`` stays (drafts that may be rejected, say); of its memory it is ``weights`` itself or shares none with it.  Drafts are weighed once they are accepted, as a chain.
-    Scores have at least 22 significant bits, everything else is fp32; a call repeats itself bit for bit."""
+    Elements of ``q * K2`` have 22 significant bits (above 2^-30 of the largest possible), everything else is fp32; a call repeats itself bit for bit."""
     softmax_scale, decay = float(softmax_scale), float(decay)
     if torch.compiler.is_compiling():
         from . import ops

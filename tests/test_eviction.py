@@ -278,6 +278,115 @@ def test_nothing_attended_missing_places_and_short_weights(form, D):
     assert not bool(got.isnan().any())
 
 
+def _longer(bt, pages=256):
+    """A table with room for so many tokens more that the tiles of a call's kernel do not stay in shared memory."""
+    return torch.nn.functional.pad(bt.table, (0, pages), value=0)
+
+
+WINDOWS = [  # B N n D dtype code page contexts windows counts
+    (2, 3, 1, 64, "bf16", "int8", 16, [500, 130], (128, 128, 32, 32), None),
+    (1, 2, 16, 64, "fp16", "e4m3", 64, [333], (128, 128, 32, 32), None),
+    (3, 1, 37, 64, "bf16", "fp16", 16, [200, 0, -1], (64, 64, 64, 64), [37, 20, 5]),
+    (1, 1, 5, 64, "fp32", "fp16", 16, [300], (40, 150, 5, 9), None),
+    (1, 1, 5, 64, "fp16", "int8", 32, [300], (150, 40, 9, 5), None),
+    (2, 2, 3, 64, "bf16", "e4m3", 16, [90, 15], (0, 0, 0, 0), None),
+    (2, 1, 9, 64, "fp16", "fp16", 128, [255, 256], (7, 120, 0, 3), [9, 0]),
+    (1, 2, 16, 128, "bf16", "fp16", 16, [222], (128, 128, 32, 32), None),
+    (2, 1, 3, 128, "fp32", "e4m3", 32, [300, 31], (100, 64, 20, 0), None),
+    (1, 3, 21, 128, "fp16", "int8", 16, [140], (31, 33, None, 10), None),
+    (40, 8, 1, 64, "bf16", "int8", 16, [b * 29 % 210 for b in range(40)], (100, 100, None, None), None),
+    (1, 1, 2, 64, "bf16", "int8", 256, [1500], (1200, 1200, 16, 16), None),
+    (1, 1, 60, 64, "fp16", "fp16", 16, [100], (90, 90, 20, 20), None),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,N,n,D,dtype,code,page,contexts,windows,counts", WINDOWS)
+def test_tdp_weigh_under_windows(B, N, n, D, dtype, code, page, contexts, windows, counts):
+    """All that a head's tokens attend to stays in shared memory: one kernel.  The table's length is of no account."""
+    bt = Weighed(B, N, n, D, dtype, code, page, contexts, windows=windows, counts=counts)
+    before = _native.lib().tritt_kernel_launches()
+    got = bt.run()
+    assert _native.lib().tritt_kernel_launches() - before == 1
+    ft.check_status(DEV)
+    bt.check(got)
+    out = torch.full((N, B, bt.length), 7.0, device=DEV).transpose(0, 1)
+    bt.run(bt.before.to(DEV), out, 0.75, _longer(bt))
+    bt.check(out, 0.75, stale=torch.full_like(bt.before, 7.0))
+    again = [bt.run(torch.full_like(got, math.nan), torch.zeros_like(got), 0.0) for _ in range(2)]
+    ft.check_status(DEV)
+    bt.check(again[0], 0.0, stale=torch.zeros_like(bt.before))
+    assert torch.equal(*again)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_queries_whose_elements_are_far_apart(dtype, D):
+    """Large ones meet zeros of K2; small ones, some of them less than fp16 has next to those, make the scores."""
+    bt = Batch(1, 1, 3, D, dtype, "fp16", 16, [150])
+    x = _randn(4, 1, 153, D, seed=3).double()
+    x[1, :, :, : D // 2] = 0
+    q = _randn(1, 1, 3, D, seed=4)
+    q[..., D // 2:] *= 2.0 ** -12
+    bt.q = q.to(bt.dt)
+    seq = orc.Sequences([x], "fp16", 16, bt.seq.codes.shape[0], bt.seq.table)
+    k1, k2 = seq.values[0][0, 0], seq.values[0][1, 0]
+    cache = ft.TrittentionCache(seq.codes.to(DEV), seq.exponents.to(DEV))
+    alpha = 2.0 ** 9
+    for windows, table in (((None,) * 4, bt.table), ((100, 100, 20, 20), bt.table), ((None,) * 4, _longer(bt))):
+        sums, gain, most, size = torch.zeros(1, 1, 3), torch.zeros(153, dtype=torch.float64), 0.0, 0.0
+        for i in range(3):
+            qi, zero = bt.q[0, 0, i].double(), torch.zeros_like(k1)
+            sums[0, 0, i] = orc.tdp_row(qi, k1, k2, zero, zero, 150, i, alpha, windows)[1]
+            one, s = orc.tdp_weights(qi, k1, k2, 150, i, alpha, windows, float(sums[0, 0, i]))
+            gain, most, size = gain + torch.nn.functional.pad(one, (0, 153 - one.shape[0])), max(most, abs(float(sums[0, 0, i]))), max(size, float(s))
+        out = torch.zeros(1, 1, 153, device=DEV)
+        ft.tdp_weigh(out, bt.q.to(DEV), sums.to(DEV), cache, table, bt.context, alpha, *windows)
+        ft.check_status(DEV)
+        err = (out[0, 0].double().cpu() - gain).abs()
+        assert bool((err <= _bound(D, 3, 153, size, most, gain, 0 * gain)).all()), float((err / gain).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("windows", [(None,) * 4, (60, 60, 20, 20)])
+@pytest.mark.parametrize("long", [False, True])
+def test_odd_rows_and_places_under_windows_and_long_tables(windows, long, D):
+    """A row that is not finite, a page that there is not, and a table that ends before the tokens do, in each of the kernels."""
+    def batch(**kw):
+        bt = Weighed(2, 2, 3, D, "bf16", "e4m3", 16, [100, 60], windows=windows, **kw)
+        return bt, (_longer(bt) if long else bt.table)
+    bt, table = batch()
+    page, row = int(bt.seq.table[0, 6]), 102 % 16
+    bt.cache.exponents[page, :2, 0, row] = 255     # of the last new token of the first head
+    got = bt.run(table=table).cpu()
+    ft.check_status(DEV)
+    assert bool(got[0, 0, 90:103].isnan().all()) and not bool(got[0, 1].isnan().any()) and not bool(got[1].isnan().any())
+    hidden, table = batch(counts=[2, 3])
+    hidden.cache.exponents[page, :2, 0, row] = 255
+    hidden.check(hidden.run(table=table))
+    ft.check_status(DEV)
+    bt, table = batch()
+    full = bt.run(table=table).cpu()
+    table = table.clone()
+    table[0, 5] = -1
+    part = bt.run(table=table).cpu()
+    with pytest.raises(_native.TrittError):
+        ft.check_status(DEV)
+    assert torch.equal(part[0, :, 80:96], bt.before[0, :, 80:96]) and torch.equal(part[1], full[1])
+    assert bool((part[0, :, :103] <= full[0, :, :103] * (1 + 1e-5)).all()) and bool((part[0, :, 96:100] > bt.before[0, :, 96:100]).all())
+    got = bt.run(table=bt.table[:, :6].contiguous()).cpu()
+    with pytest.raises(_native.TrittError):
+        ft.check_status(DEV)
+    assert not bool(got.isnan().any())
+    bt.sums[:] = -math.inf
+    got = bt.run(table=_longer(bt) if long else bt.table).cpu()
+    ft.check_status(DEV)
+    for b, c in enumerate(bt.contexts):
+        assert torch.equal(got[b, :, :c], bt.before[b, :, :c]) and float(got[b, :, c:c + 3].abs().max()) == 0
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("D", [64, 32])
 def test_a_table_far_longer_than_the_sequences(D):
