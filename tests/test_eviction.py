@@ -743,6 +743,39 @@ def test_library_operators_and_compiled_calls():
     ft.check_status(DEV)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMS)
+def test_queries_that_want_gradients_and_results_elsewhere(form):
+    """While a model is trained its queries have a history, of which the weights know nothing; eager and compiled, with new weights and rows in other places."""
+    bt = Weighed(2, 2, 2, 64, "bf16", "int8", 16, [60, 21], **form)
+    sums, table = bt.sums.to(DEV), bt.table
+    few = 2
+    old = bt.cache.codes.shape[0]
+    cache = [None if t is None else torch.cat((t, torch.zeros((2 * few, *t.shape[1:]), dtype=t.dtype, device=DEV))) for t in bt.cache]
+    table_out = torch.arange(old, old + 2 * few, device=DEV).view(2, few).int()
+
+    def step(x, y, weights, out, short, codes, exponents, lse):
+        q, k2, c = x * 1.0, y * 1.0, ft.TrittentionCache(codes, exponents, lse)
+        if bt.k_diff is None:
+            ft.tdp_weigh(weights, q, sums, c, table, bt.context, bt.alpha, out=out)
+        else:
+            ft.dps_weigh(weights, q, k2, sums, c, table, bt.context, bt.alpha, bt.k_diff, out=out)
+        return (*ft.cache_evict(out, c, table, bt.context + 2, 20, 1, 2, table_out, short), (q * q).sum())
+
+    got = []
+    for f in (step, torch.compile(step, fullgraph=True, backend="aot_eager")):
+        x, y = bt.q.to(DEV).requires_grad_(True), bt.k2.to(DEV).requires_grad_(True)
+        args = [bt.before.to(DEV), torch.zeros(2, 2, bt.length, device=DEV), torch.full((2, 2, 25), 3.0, device=DEV), *(None if t is None else t.clone() for t in cache)]
+        left, kept, loss = f(x, y, *args)
+        loss.backward()
+        assert torch.equal(x.grad, 2 * x.detach()) and torch.equal(args[0].cpu(), bt.before)
+        bt.check(args[1].detach(), stale=torch.zeros_like(bt.before))
+        got.append([left, kept, *(t.detach() for t in args if t is not None)])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    assert float(got[0][4][:, :, 20:].min()) == 3.0
+    ft.check_status(DEV)
+
+
 # ---------------------------------------------------------------- refusals, on the CPU
 
 def _cpu(dps=False):
