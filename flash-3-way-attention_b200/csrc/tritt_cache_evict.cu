@@ -413,9 +413,9 @@ extern "C" int tritt_cache_evict(const tritt_cache_t* c, const tritt_weights_t* 
                                  int first, int recent, int* context_out, int* kept, int* status_word, tritt_stream_t stream) {
   if (int rc = check_cache(c)) return rc;
   if (int rc = check_weights(c, w)) return rc;
-  if (table_out && table_out == c->table && (c->B == 1 || table_out_stride == c->table_stride)) table_out = nullptr;   // (in place, after all)
   Params p{cache_args(*c, status_word), *w, table_out, table_out_stride, table_out_pages, keep, first, recent, context_out, kept, 1};
   if (int rc = check(c, w, p)) return rc;
+  if (table_out && table_out == c->table && (c->B == 1 || table_out_stride == c->table_stride)) p.table_out = nullptr;   // (in place, after all)
   p.cache.c.n = 1;   // (places are reported of every sequence in use)
   p.cache.c.counts = nullptr;
   // A cluster for a head as far as the weights do not fit in one CTA's registers (fewer and larger clusters: eight CTAs a head of 65001 weights took 39 us, some of them behind others), and not more CTAs

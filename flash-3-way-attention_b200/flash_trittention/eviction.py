@@ -121,7 +121,7 @@ def cache_evict(weights: Tensor, cache: TrittentionCache, table: Tensor, context
     behind the last.  A sequence that has no more than ``keep`` tokens keeps them all, a free slot of the batch stays one.
 
     The kept rows, exponents and log-sum-exps become tokens ``0, 1, 2, ...``, and so do their weights; the pages behind them are free (what they hold is left as it is).  A page that several sequences
-    share must not be written: with ``table_out`` (int32 ``[B, pages]``, of pages that the call does not read) the rows go there and the old ones stay, and with ``weights_out`` (float32 ``[B, N, tokens]``, of memory that ``weights`` has no part of)
+    share must not be written: with ``table_out`` (int32 ``[B, pages]``, of pages that the call does not read, or ``table`` itself: in place) the rows go there and the old ones stay, and with ``weights_out`` (float32 ``[B, N, tokens]``, of memory that ``weights`` has no part of)
     the weights."""
     keep, first, recent = int(keep), int(first), int(recent)
     if keep < 1 or first < 0 or recent < 0 or first + recent > keep:
