@@ -458,7 +458,8 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_weigh_sm100_kernel(const __gr
       const int largest = uniform(byte), least = -uniform(-least_byte(byte));   // (least: 255 if all rows are zeros)
       const bool apart = largest == 255 || (least < 255 && largest - least > kSpread<CODE>);
       // (a row that is not finite has 255: the others' are relative to 254 then, for what they are worth beside a NaN)
-      const float own_scale = mine == nullptr || byte <= 1 ? 1.f : byte == 255 ? __uint_as_float(0x7fffffffu) : power_of_two(byte - least_of(largest, 254));
+      // (byte 1 is that of rows of zeros, and of all that are too small for a lower one: their codes may be as large as any)
+      const float own_scale = byte == 0 ? 0.f : byte == 255 ? __uint_as_float(0x7fffffffu) : power_of_two(byte - least_of(largest, 254));
       Columns& col = ms.columns[buf];
       col.scale[w * 32 + lane] = own_scale;
       if (lane == 0) {

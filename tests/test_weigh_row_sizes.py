@@ -1,0 +1,75 @@
+"""The attention weight of cached tokens beside rows of any size: rows next to zero, and rows that a token does not attend to and that are larger than its own by any power of two.
+
+Tolerances: ``_bound`` of ``test_eviction``, counted from the arithmetic there."""
+import pytest
+import torch
+
+import flash_trittention as ft
+from flash_trittention import _native
+from oracle import serving_oracle as orc
+from tests.test_cache import Batch, _randn
+from tests.test_eviction import DEV, _bound, _longer
+
+K1, K2 = 0, 1
+CODES = ["fp16", "e4m3", "int8"]
+
+
+def _gains(bt, alpha, windows, silent=()):
+    """Log-sum-exps of the new tokens (-inf of the silent ones, which add nothing), what the others add, the largest |lse| and the largest sum of |products|."""
+    sums = torch.full((bt.B, bt.N, bt.n), -torch.inf)
+    tokens = max(c + bt.n for c in bt.contexts)
+    gain, most, size = torch.zeros(bt.B, bt.N, tokens, dtype=torch.float64), 0.0, 0.0
+    for b, h, i in bt.rows():
+        if i in silent:
+            continue
+        ctx, q = bt.contexts[b], bt.q[b, h, i].double()
+        x = bt.seq.values[b][:, h]
+        zero = torch.zeros_like(x[K1])
+        seen = torch.arange(x.shape[1]) <= ctx + i
+        k1, k2 = (torch.where(seen[:, None], x[part], 0.0) for part in (K1, K2))
+        sums[b, h, i] = orc.tdp_row(q, torch.nan_to_num(k1), torch.nan_to_num(k2), zero, zero, ctx, i, alpha, windows)[1]
+        one, s = orc.tdp_weights(q, k1, k2, ctx, i, alpha, windows, float(sums[b, h, i]))
+        gain[b, h, : one.shape[0]] += one
+        most, size = max(most, abs(float(sums[b, h, i]))), max(size, float(s))
+    return sums, gain, most, size
+
+
+def _check(bt, alpha, windows, table, launches, silent=()):
+    sums, gain, most, size = _gains(bt, alpha, windows, silent)
+    out = torch.zeros(gain.shape, device=DEV)
+    before = _native.lib().tritt_kernel_launches()
+    ft.tdp_weigh(out, bt.q.to(DEV), sums.to(DEV), bt.cache, table, bt.context, alpha, *windows)
+    if launches is not None:   # (which of the kernels it was)
+        assert _native.lib().tritt_kernel_launches() - before == launches
+    ft.check_status(DEV)
+    got = out.double().cpu()
+    for b in range(bt.B):
+        end = bt.contexts[b] + bt.n
+        err, bound = (got[b, :, :end] - gain[b, :, :end]).abs(), _bound(bt.D, bt.n, end, size, most, gain[b, :, :end], 0 * gain[b, :, :end])
+        assert bool((err <= bound).all()), f"sequence {b}: {float((err / bound).max()):.3g} bounds, {float(err.max()):.3e} off"
+
+
+def _put(bt, b, token, part, rows):
+    """Rows [N, D] in 64 bits in the place of a token's, quantised, in the pages and in the 64-bit values."""
+    codes, byte, value = orc.quantise(rows, bt.code)
+    page, row = int(bt.seq.table[b, token // bt.seq.page_size]), token % bt.seq.page_size
+    as_bytes = lambda t: t if t.element_size() > 1 else t.view(torch.uint8)  # noqa: E731
+    as_bytes(bt.seq.codes)[page, part, :, row] = as_bytes(codes)
+    bt.seq.exponents[page, part, :, row] = byte
+    bt.seq.values[b][part, :, token] = value
+    bt.cache = ft.TrittentionCache(bt.seq.codes.to(DEV), bt.seq.exponents.to(DEV))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("D,long", [(64, False), (64, True), (128, False), (128, True), (32, True), (256, True)])
+@pytest.mark.parametrize("part", [K1, K2])
+def test_rows_next_to_zero(part, D, long, code):
+    """Some rows are so small that their exponent byte is 1, the least, but their codes are not zeros; others are zeros.  Their scores are nothing beside the ordinary ones'."""
+    bt = Batch(1, 2, 3, D, "bf16", code, 16, [200], seed=41)
+    for token in range(4, 203, 7):
+        size = (1e-37 if code == "int8" else 1e-36) if token % 3 else 0.0
+        _put(bt, 0, token, part, _randn(2, D, seed=token).double() * size)
+    page, row = int(bt.seq.table[0, 0]), 4
+    assert int(bt.seq.exponents[page, part, 0, row]) == 1 and bool((bt.seq.codes[page, part, 0, row].float() != 0).any())
+    _check(bt, 0.2, (None,) * 4, _longer(bt) if long else bt.table, 2 if long else None)
