@@ -59,6 +59,11 @@ def _sums(name, t, q):
     return t.detach().contiguous()
 
 
+def _same_places(table, other):
+    """Whether two tables of as many sequences are one as far as both reach."""
+    return table.data_ptr() == other.data_ptr() and all(s == t for n, m, s, t in zip(table.shape, other.shape, table.stride(), other.stride()) if min(n, m) > 1)
+
+
 def tdp_weigh(weights: Tensor, q: Tensor, lse: Tensor, cache: TrittentionCache, table: Tensor, context: Tensor, softmax_scale: float = 1 / 8,
               k1_window: Optional[int] = None, k2_window: Optional[int] = None, kk_left: Optional[int] = None, kk_right: Optional[int] = None,
               counts: Optional[Tensor] = None, decay: float = 1.0, out: Optional[Tensor] = None) -> None:
@@ -144,7 +149,8 @@ def cache_evict(weights: Tensor, cache: TrittentionCache, table: Tensor, context
     if table_out is not None:
         if table_out.shape[:1] != table.shape[:1] or table_out.dim() != 2 or table_out.dtype != torch.int32 or table_out.device != dev or table_out.shape[1] * page < keep:
             raise ValueError(f"table_out must be int32 [{table.shape[0]}, pages for {keep} tokens] on {dev}, got {table_out.dtype} {list(table_out.shape)} on {table_out.device}")
-        table_out = table_out if table_out.stride(1) == 1 else table_out.contiguous()
+        # (decided before either is laid out for the library, which knows a call in place by the pointer)
+        table_out = None if _same_places(table, table_out) else table_out if table_out.stride(1) == 1 else table_out.contiguous()
     context_out = torch.empty(c.B, dtype=torch.int32, device=dev)
     kept = torch.empty(c.B, c.N, keep, dtype=torch.int32, device=dev)
     _native.cache_evict(c, w, table_out, keep, first, recent, context_out, kept)
