@@ -374,7 +374,7 @@ template <typename T, int D, int CODE> __global__ void __launch_bounds__(kThread
 
 template <typename T, int D, int CODE> int launch(Params p, cudaStream_t stream) {
   const tritt_cache_t& c = p.cache.c;
-  long long tokens = (long long)c.table_pages * c.page_size;
+  long long tokens = (long long)c.table_pages * c.page_size + c.n;   // (weights of tokens behind the table's end are written, and the tokens reported)
   const int length = p.w.after_length < p.w.before_length ? p.w.after_length : p.w.before_length;
   if (length < tokens) tokens = length;
   if constexpr (kFewApplies<D, CODE>) {
