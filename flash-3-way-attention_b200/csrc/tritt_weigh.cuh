@@ -144,7 +144,8 @@ __device__ __forceinline__ WeighLine weigh_line(const TdpWeighArgs& a, int b) {
     return l;
   }
   const int lo_j = l.ctx - (a.k1w < l.ctx ? a.k1w : l.ctx), lo_k = l.ctx - (a.k2w < l.ctx ? a.k2w : l.ctx);
-  const int places = a.cache.c.table_pages << a.cache.page_log2;   // (tokens behind the table's end are not there, and the slots have no room for them)
+  const int places = a.cache.c.table_pages << a.cache.page_log2;   // (tokens behind the table's end are not there, and the slots have no room for them: reported)
+  if (l.cnt > places - l.ctx && a.cache.status) atomicOr(a.cache.status, kStatusPlace);
   l.last = (l.cnt < places - l.ctx ? l.ctx + l.cnt : places) - 1;
   l.j0 = lo_j / 128;
   l.k0 = lo_k / 128;

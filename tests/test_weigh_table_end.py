@@ -8,7 +8,7 @@ import flash_trittention as ft
 from flash_trittention import _native
 from tests.test_eviction import DEV, Weighed
 
-FORMS = [dict(k_diff=50, dps=True), dict(k_diff=1000, dps=True)]
+FORMS = [dict(k_diff=None, dps=False), dict(k_diff=50, dps=True), dict(k_diff=1000, dps=True)]
 
 
 @pytest.mark.gpu
