@@ -58,7 +58,7 @@ constexpr int kOff = 256, kPlain = 512;
 struct __align__(16) Columns {    // of a tile of Q
   float scale[128];               // (apart) of scores
   uint32_t there[4];              // of 32 columns: those that have a place and are attended to
-  int largest[4];                 // the largest of their exponent bytes
+  int middle[4];                  // the exponent byte that their powers of two are relative to
   int apart[4];                   // whether each has its own power of two
   int field;                      // q's exponent
   int pad[3];
@@ -97,9 +97,10 @@ constexpr int kConsumers = 1 + 2 + 4 + 4 + 16;   // warps that read an item
 __device__ __forceinline__ int most(int x, int y) { return x > y ? x : y; }
 __device__ __forceinline__ int least_of(int x, int y) { return x < y ? x : y; }
 
+// (with numbers below fp32's normal ones: see scaled_score)
 __device__ __forceinline__ float2 mul_pair(float2 a, float2 b) {
   float2 r;
-  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.ftz.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
       : "=f"(r.x), "=f"(r.y)
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return r;
@@ -107,7 +108,7 @@ __device__ __forceinline__ float2 mul_pair(float2 a, float2 b) {
 __device__ __forceinline__ float2 fma_pair(float2 a, float b, float c) {
   float2 r;
   asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %4};\n\tmov.b64 z, {%5, %5};\n\t"
-      "fma.rn.ftz.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
       : "=f"(r.x), "=f"(r.y)
       : "f"(a.x), "f"(a.y), "f"(b), "f"(c));
   return r;
@@ -455,16 +456,26 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_weigh_sm100_kernel(const __gr
       const uint32_t there = __ballot_sync(0xffffffffu, mine != nullptr);
       alive = wait_all(&ms.q_free[buf], ((pieces >> 1) & 1) ^ 1);
       if (!alive) break;
-      const int largest = uniform(byte), least = -uniform(-least_byte(byte));   // (least: 255 if all rows are zeros)
-      const bool apart = largest == 255 || (least < 255 && largest - least > kSpread<CODE>);
-      // (a row that is not finite has 255: the others' are relative to 254 then, for what they are worth beside a NaN)
-      // (byte 1 is that of rows of zeros, and of all that are too small for a lower one: their codes may be as large as any)
-      const float own_scale = byte == 0 ? 0.f : byte == 255 ? __uint_as_float(0x7fffffffu) : power_of_two(byte - least_of(largest, 254));
+      // byte 1 is that of rows of zeros, which do not count, and of all that are too small for a lower one: their codes may be as large as any
+      if (__any_sync(0xffffffffu, byte == 1)) {
+        uint32_t bits = byte == 1 ? 0u : 1u;
+        if (byte == 1)
+#pragma unroll 1
+          for (int c = 0; c < R::kChunks; ++c) {
+            const uint4 x = __ldg(reinterpret_cast<const uint4*>(mine) + c);
+            bits |= x.x | x.y | x.z | x.w;
+          }
+        if (bits == 0) byte = 0;
+      }
+      const int largest = uniform(byte == 255 ? 0 : byte), least = -uniform(byte == 0 ? -255 : -byte);   // (of rows that are finite; least: 255 if all are zeros)
+      const bool apart = __any_sync(0xffffffffu, byte == 255) || (least < 255 && largest - least > kSpread<CODE>);
+      const int middle = apart ? middle_byte<CODE>(largest) : largest;
+      const float own_scale = byte == 0 ? 0.f : byte == 255 ? __uint_as_float(0x7fffffffu) : relative_power(byte - middle);
       Columns& col = ms.columns[buf];
       col.scale[w * 32 + lane] = own_scale;
       if (lane == 0) {
         col.there[w] = there;
-        col.largest[w] = least_of(largest, 254);
+        col.middle[w] = middle;
         col.apart[w] = apart;
         col.field = field;   // (all four warps the same)
       }
@@ -544,7 +555,7 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_weigh_sm100_kernel(const __gr
       const int field = col.field;
       const bool apart = col.apart[wg];
       // what a row's scores are multiplied by: its power of two with that of the columns, q and Q (beyond fp32's range scores have no use for), and the scale
-      const int power = col.largest[wg] + field - 382 + 127 + kDown<CODE>;
+      const int power = col.middle[wg] + field - 382 + 127 + kDown<CODE>;
       const float scale = field == 255 ? __uint_as_float(0x7fffffffu) : field == 0 ? 0.f : p.scale2;
       // whether the rows of a plain tile have pairs with all of the 32 columns
       const bool plain = there == 0xffffffffu && !apart && field != 255 && k0 >= k_lo && k0 + 31 <= pos && p.kkl >= pos && p.kkr >= pos;

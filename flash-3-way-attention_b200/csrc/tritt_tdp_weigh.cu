@@ -83,8 +83,8 @@ template <typename T, int D, int CODE> __global__ void __launch_bounds__(kThread
     __syncthreads();
     if (tid < 128 && own.page >= 0 && byte != 255) atomicMax(&sh.largest, byte);
     __syncthreads();
-    const int field = sh.field, largest = sh.largest;
-    if (tid < 128) sh.scale[tid] = own.page < 0 ? 0.f : byte == 255 ? __uint_as_float(0x7fffffffu) : power_of_two(byte - largest);
+    const int field = sh.field, middle = middle_byte<CODE>(sh.largest);
+    if (tid < 128) sh.scale[tid] = own.page < 0 ? 0.f : byte == 255 ? __uint_as_float(0x7fffffffu) : relative_power(byte - middle);
     // A
     for (int x = tid; x < 128 * (D / 4); x += kThreads) {
       const int col = x / (D / 4), h = x % (D / 4) * 4, kk = s.kg * 128 + col;
@@ -129,8 +129,8 @@ template <typename T, int D, int CODE> __global__ void __launch_bounds__(kThread
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int e = __ldg(a.c.exponents + row + g + 8 * h), j = x0 + g + 8 * h;
-        // 2^e of the row, the largest of the columns, q and A
-        int power = e + largest - 254 + field - 128 + kDown<CODE>;
+        // 2^e of the row, that of the columns' in the middle, q and A
+        int power = e + middle - 254 + field - 128 + kDown<CODE>;
         power = power < -126 ? -126 : power > 127 ? 127 : power;
         scale[h] = e == 255 || field == 255 ? __uint_as_float(0x7fffffffu) : field == 0 ? 0.f : p.scale2 * power_of_two(power);
         const bool on = j >= j_lo && j <= pos;
@@ -155,7 +155,7 @@ template <typename T, int D, int CODE> __global__ void __launch_bounds__(kThread
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const bool on = col + e >= c_lo[h] && col + e <= c_hi[h] && (there >> e & 1);
-            const float prob = on ? exp2f(fmaf(d[2 * h + e] * (e ? by.y : by.x), scale[h], -lse2)) : 0.f;
+            const float prob = on ? exp2f(scaled_score(d[2 * h + e], e ? by.y : by.x, scale[h], lse2)) : 0.f;
             sum[h] += prob;
             column[t][e] += prob;
           }

@@ -169,11 +169,11 @@ template <typename T, int D, int CODE> __global__ void __launch_bounds__(kThread
     }
   }
   __syncthreads();
-  const int top = *largest;
-  for (int x = warp; x < padded_j / 32; x += kWarps) {   // scales of K1's rows, relative to the largest, and words of those that are there
+  const int middle = middle_byte<CODE>(*largest);
+  for (int x = warp; x < padded_j / 32; x += kWarps) {   // scales of K1's rows, and words of those that are there
     const int e = reinterpret_cast<const int*>(sScale1)[x * 32 + lane];
     const uint32_t there = __ballot_sync(0xffffffffu, e >= 0);
-    sScale1[x * 32 + lane] = e < 0 ? 0.f : e == 255 ? __uint_as_float(0x7fffffffu) : power_of_two(e - top);
+    sScale1[x * 32 + lane] = e < 0 ? 0.f : e == 255 ? __uint_as_float(0x7fffffffu) : relative_power(e - middle);
     if (lane == 0) sThere[x] = there;
   }
   __syncthreads();
@@ -227,8 +227,8 @@ template <typename T, int D, int CODE> __global__ void __launch_bounds__(kThread
         if (seen && !on && t == 0 && ca.status) atomicOr(ca.status, kStatusPlace);
         from[h] = on ? (k_at[h] - a.kkl > j_lo ? k_at[h] - a.kkl : j_lo) : 1 << 30;
         to[h] = !on ? -1 : a.kkr < pos - k_at[h] ? k_at[h] + a.kkr : pos;
-        // 2^e of the row, the largest of the columns, q and the operand
-        int power = e2[h] + top - 254 + field - 128 + kDown<CODE>;
+        // 2^e of the row, that of the columns' in the middle, q and the operand
+        int power = e2[h] + middle - 254 + field - 128 + kDown<CODE>;
         power = power < -126 ? -126 : power > 127 ? 127 : power;
         scale[h] = e2[h] == 255 || field == 255 ? __uint_as_float(0x7fffffffu) : field == 0 ? 0.f : a.scale2 * power_of_two(power);
       }
@@ -302,8 +302,8 @@ template <typename T, int D, int CODE> __global__ void __launch_bounds__(kThread
           float x[4];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            x[2 * h] = fmaf(s[2 * h] * by.x, scale[h], -lse2);
-            x[2 * h + 1] = fmaf(s[2 * h + 1] * by.y, scale[h], -lse2);
+            x[2 * h] = scaled_score(s[2 * h], by.x, scale[h], lse2);
+            x[2 * h + 1] = scaled_score(s[2 * h + 1], by.y, scale[h], lse2);
             if (!all) {
               x[2 * h] = mask[h] >> (n * 8 + 2 * t) & 1 ? x[2 * h] : -INFINITY;
               x[2 * h + 1] = mask[h] >> (n * 8 + 2 * t + 1) & 1 ? x[2 * h + 1] : -INFINITY;

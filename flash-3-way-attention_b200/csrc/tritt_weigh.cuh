@@ -29,6 +29,22 @@ __device__ __forceinline__ float to_operand(int field) { return field == 0 || fi
 __device__ __forceinline__ float from_operand(int field) {
   return field == 255 ? __uint_as_float(0x7fffffffu) : field <= 1 ? 0.f : __uint_as_float((uint32_t)(field - 1) << 23);
 }
+// Where rows of one operand have powers of two of their own, a score is multiplied by its row's, relative to that of this exponent byte (largest: the largest byte of a row that is finite), and that one joins the other
+// row's.  Rows may be as far apart as fp32 has numbers, the largest one is often one that the token does not attend to, and the score of the smallest has to be right beside it: so the factors reach from 2^-149, below fp32's
+// normal numbers, to 2^kMostPower, which brings no sum of products (below 2^38, 2^27.7, 2^24 with 256 elements) to infinity.
+template <int CODE> constexpr int kMostPower = CODE == TRITT_CODE_F16 ? 90 : CODE == TRITT_CODE_E4M3 ? 100 : 103;
+template <int CODE> __device__ __forceinline__ int middle_byte(int largest) {
+  return largest <= 127 ? largest : largest - kMostPower<CODE> > 127 ? largest - kMostPower<CODE> : 127;
+}
+__device__ __forceinline__ float relative_power(int e) {   // 2^e, e <= 127; 0 below 2^-149
+  return __uint_as_float(e >= -126 ? (uint32_t)(e + 127) << 23 : e >= -149 ? 1u << (e + 149) : 0u);
+}
+// sum * column * row - minus with numbers below fp32's normal ones (which the compiler's own arithmetic takes for zeros here)
+__device__ __forceinline__ float scaled_score(float sum, float column, float row, float minus) {
+  float x;
+  asm("{\n\t.reg .f32 t;\n\tmul.rn.f32 t, %1, %2;\n\tfma.rn.f32 %0, t, %3, %4;\n\t}" : "=f"(x) : "f"(sum), "f"(column), "f"(row), "f"(-minus));
+  return x;
+}
 __device__ __forceinline__ uint32_t pack_halves(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);

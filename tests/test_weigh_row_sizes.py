@@ -73,3 +73,57 @@ def test_rows_next_to_zero(part, D, long, code):
     page, row = int(bt.seq.table[0, 0]), 4
     assert int(bt.seq.exponents[page, part, 0, row]) == 1 and bool((bt.seq.codes[page, part, 0, row].float() != 0).any())
     _check(bt, 0.2, (None,) * 4, _longer(bt) if long else bt.table, 2 if long else None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("D,long", [(64, False), (64, True), (128, True), (32, True)])
+def test_rows_next_to_zero_whose_partners_are_large(D, long, code):
+    """Pairs of a token with itself alone: a row of 1e-36 meets one of 1e36, and the score is an ordinary one; so are the other pairs', whose rows are ordinary."""
+    bt = Batch(1, 2, 2, D, "bf16", code, 16, [200], seed=43)
+    for token in range(5, 202, 9):
+        for part, size in ((K1, 1e36), (K2, 1e-36)) if token % 2 else ((K1, 1e-36), (K2, 1e36)):
+            _put(bt, 0, token, part, _randn(2, D, seed=token + part).clamp(-3, 3).double() * size)
+    windows = (None, None, 0, 0)
+    _check(bt, 0.2, windows, _longer(bt) if long else bt.table, None)
+
+
+def _enlarge(bt, b, token, part, by):
+    """A token's rows times 2^by (None: not finite), in the pages and in the 64-bit values."""
+    page, row = int(bt.seq.table[b, token // bt.seq.page_size]), token % bt.seq.page_size
+    old = bt.seq.exponents[page, part, :, row].int()
+    byte = torch.full_like(old, 255) if by is None else (old + by).clamp(2, 254)
+    bt.seq.exponents[page, part, :, row] = byte.to(torch.uint8)
+    bt.seq.values[b][part, :, token] = orc.values(bt.seq.codes[page, part, :, row], byte)
+    bt.cache.exponents.copy_(bt.seq.exponents)
+
+
+BY = [12, 30, 100, 200, None]
+KERNELS = [(64, False), (64, True), (128, False), (128, True), (32, True)]   # D, a long table: each of the kernels
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("by", BY)
+@pytest.mark.parametrize("part", [K1, K2])
+@pytest.mark.parametrize("windows", [(None,) * 4, (100, 100, 20, 20)])
+@pytest.mark.parametrize("D,long", KERNELS)
+def test_later_tokens_that_are_larger(D, long, windows, part, by):
+    """The new tokens before it do not attend to the last one, whatever it holds; it adds nothing itself (its log-sum-exp is -inf)."""
+    bt = Batch(1, 2, 4, D, "bf16", "e4m3", 16, [150], seed=45)
+    _enlarge(bt, 0, 153, part, by)
+    _check(bt, 0.2, windows, _longer(bt) if long else bt.table, None, silent=(3,))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("by", BY)
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("windows,hidden,part", [((20, 100, 8, 8), 70, K2), ((100, 20, 8, 8), 70, K1), ((40, 60, None, None), 61, K2), ((60, 40, None, None), 61, K1),
+                                                 ((40, 40, 16, 16), 45, K1), ((40, 40, 16, 16), 45, K2), ((20, None, 8, 8), 31, K2), ((None, 20, 8, 8), 31, K1)])
+@pytest.mark.parametrize("D,long", KERNELS)
+def test_tokens_outside_the_windows_or_the_band(D, long, windows, hidden, part, code, by):
+    """A row of the context that no pair of the windows and the band has, but that lies among those that are looked at."""
+    bt = Batch(1, 1, 2, D, "fp16", code, 16, [190], seed=47)
+    _enlarge(bt, 0, 191 - hidden, part, by)
+    if hidden == 61:
+        assert 191 - hidden >= 190 - 60   # (the first new token attends to it; it adds nothing)
+    _check(bt, 0.2, windows, _longer(bt) if long else bt.table, None, silent=(0,) if hidden == 61 else ())
