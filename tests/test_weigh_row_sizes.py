@@ -1,6 +1,8 @@
 """The attention weight of cached tokens beside rows of any size: rows next to zero, and rows that a token does not attend to and that are larger than its own by any power of two.
 
 Tolerances: ``_bound`` of ``test_eviction``, counted from the arithmetic there."""
+import math
+
 import pytest
 import torch
 
@@ -8,7 +10,7 @@ import flash_trittention as ft
 from flash_trittention import _native
 from oracle import serving_oracle as orc
 from tests.test_cache import Batch, _randn
-from tests.test_eviction import DEV, _bound, _longer
+from tests.test_eviction import DEV, Weighed, _bound, _longer
 
 K1, K2 = 0, 1
 CODES = ["fp16", "e4m3", "int8"]
@@ -127,3 +129,20 @@ def test_tokens_outside_the_windows_or_the_band(D, long, windows, hidden, part, 
     if hidden == 61:
         assert 191 - hidden >= 190 - 60   # (the first new token attends to it; it adds nothing)
     _check(bt, 0.2, windows, _longer(bt) if long else bt.table, None, silent=(0,) if hidden == 61 else ())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("rows,queries", [(2.0 ** 100, 2.0 ** -100), (2.0 ** -100, 2.0 ** 100), (2.0 ** 60, 2.0 ** -60)])
+@pytest.mark.parametrize("D,n,form", [(64, 2, "tdp"), (64, 60, "tdp"), (128, 2, "tdp"), (32, 2, "tdp"), (64, 2, "dps"), (128, 9, "dps"), (32, 3, "dps"), (256, 2, "dps")])
+def test_queries_and_rows_of_opposite_sizes(form, D, n, rows, queries, dtype, code):
+    """The scores are ordinary ones: all rows (of K1 in the triple product) are times a power of two, the queries, and the new tokens' k2, times its inverse."""
+    kw = dict(k_diff=50, dps=True) if form == "dps" else {}
+    bt = Weighed(1, 1, n, D, dtype, code, 16, [150], **kw)   # (of ordinary sizes: scaled by powers of two all scores keep their values)
+    for part in (K1, K2) if form == "dps" else (K1,):
+        for token in range(150 + n):
+            _enlarge(bt, 0, token, part, round(math.log2(rows)))
+    bt.q, bt.k2 = bt.q * queries, bt.k2 * queries
+    bt.check(bt.run())
+    ft.check_status(DEV)
