@@ -68,7 +68,10 @@ def _packed(axes, cos):
         return None
     if cos is None:
         raise ValueError("axes without cos and sin")
-    return _pack_axes(tuple(axes), cos.shape[-1])
+    try:
+        return _pack_axes(tuple(axes), cos.shape[-1])
+    except TypeError:   # (while a graph with symbols for sizes is traced: they are no keys of what is kept)
+        return _pack_axes(tuple(int(a) for a in axes), int(cos.shape[-1]))
 
 
 def _check(xs, ws, cos, sin, positions, axes=None):
