@@ -410,8 +410,8 @@ int make_tmap_3d(CUtensorMap* out, const void* base, int elem_bytes, uint64_t co
 // The same over rows that are `row_stride` elements apart (heads `head_stride`): the rows of a query shard.
 int make_tmap_rows(CUtensorMap* out, const void* base, uint64_t cols, uint64_t rows, uint64_t bn, uint64_t row_stride,
                    uint64_t head_stride, uint32_t box_rows);
-// Rows of 64 or more bytes (as 16-bit elements), in boxes of 64 or 128 bytes of `box_rows` rows with the swizzle of that width.
-int make_tmap_codes(CUtensorMap* out, const void* base, uint64_t row_bytes, uint64_t rows, uint32_t box_bytes, uint32_t box_rows);
+// Pages of `rows` rows of 64 or more bytes (as 16-bit elements), in boxes of 64 or 128 bytes of `box_rows` rows with the swizzle of that width.
+int make_tmap_codes(CUtensorMap* out, const void* base, uint64_t row_bytes, uint64_t rows, uint64_t pages, uint32_t box_bytes, uint32_t box_rows);
 // An fp32 tensor as the destination of TMA reduce-adds of 32-column pieces (128-byte rows, 128-byte swizzle).
 int make_tmap_3d_f32(CUtensorMap* out, const void* base, uint64_t cols, uint64_t rows, uint64_t bn, uint32_t box_cols,
                      uint32_t box_rows);

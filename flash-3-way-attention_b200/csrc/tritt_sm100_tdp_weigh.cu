@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_weigh_sm100_kernel(const __gr
         const Item it = ms.items[count % kItems];
         free_item(count);
         const int f = (int)((before ^ mine) & 1), own = (n - f + 1) / 2;   // the warp's first tile of the piece, and how many it has
-        const int x0 = (it.s0 + f) * 128 + r0;
+        const int x0 = (it.s0 + f) * 128 + r0, row_in_page = (kPartK1 * a.c.N + it.head) << a.page_log2;
         // the page of the lane's rows of the warp's i-th tile, as the table has it (not looked at here, so that nothing waits for it); -1: nobody looks at them, or the table has none
         auto attended = [&](int i) { return i < own && x0 + i * 256 + 3 >= it.j_lo && x0 + i * 256 <= it.pos; };
         auto page_of = [&](int i) {
@@ -293,15 +293,14 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_weigh_sm100_kernel(const __gr
           return page;
         };
         struct Four {
-          size_t row;
+          int page;
           uint32_t exponents;
           bool there;
         };
         auto read = [&](int i, int page) {
-          Four t{0, 0, page >= 0 && page < a.c.pages};
+          Four t{page, 0, page >= 0 && page < a.c.pages};
           if (t.there) {
-            t.row = row_of(a, Place{page, (x0 + i * 256) & (a.c.page_size - 1)}, kPartK1, it.head);
-            t.exponents = __ldg(reinterpret_cast<const uint32_t*>(a.c.exponents + t.row));
+            t.exponents = __ldg(reinterpret_cast<const uint32_t*>(a.c.exponents + row_of(a, Place{page, (x0 + i * 256) & (a.c.page_size - 1)}, kPartK1, it.head)));
           } else if (attended(i) && a.status) {
             atomicOr(a.status, kStatusPlace);
           }
@@ -348,8 +347,8 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_weigh_sm100_kernel(const __gr
               const int at = r0 & ~(seg - 1);
               uint8_t* const to = smem + C::kOffRaw + slot * C::kRaw + at * C::kPitch;
 #pragma unroll
-              for (int x = 0; x < C::kBoxes; ++x)   // (the cache has fewer than 2^31 rows: one has 64 bytes at least)
-                tma_load_3d(to + x * 128 * C::kPitch, &map, &ms.raw_full[slot], x * 64, (int)(now.row - (r0 - at)), 0);
+              for (int c = 0; c < C::kBoxes; ++c)   // (rows are numbered within their page: the cache may have more than an int)
+                tma_load_3d(to + c * 128 * C::kPitch, &map, &ms.raw_full[slot], c * 64, row_in_page + (x & (a.c.page_size - 1)) - (r0 - at), now.page);
             }
           }
         }
@@ -645,9 +644,13 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_weigh_sm100_kernel(const __gr
 template <typename T, int D, int CODE> int launch(const TdpWeighArgs& p, cudaStream_t stream) {
   using C = Cfg<D, CODE>;
   const tritt_cache_t& c = p.cache.c;
-  // all rows of the cache, boxes of what a page has of 128 rows
+  // all pages of the cache, boxes of what one has of 128 rows
+  if (4LL * c.N * c.page_size >= 1LL << 31) {
+    set_error("pages of %d heads and %d tokens have too many rows for one call", c.N, c.page_size);
+    return -11;
+  }
   CUtensorMap map{};
-  if (int rc = make_tmap_codes(&map, c.codes, C::kRow, (uint64_t)c.pages * 4 * c.N * c.page_size, C::kPitch, c.page_size < 128 ? c.page_size : 128)) return rc;
+  if (int rc = make_tmap_codes(&map, c.codes, C::kRow, (uint64_t)4 * c.N * c.page_size, c.pages, C::kPitch, c.page_size < 128 ? c.page_size : 128)) return rc;
   // (warpgroups share out the registers that the kernel is launched with: with fewer those that raise their count would wait for good)
   cudaFuncAttributes attr;
   TRITT_CUDA_OK(cudaFuncGetAttributes(&attr, tdp_weigh_sm100_kernel<T, D, CODE>));

@@ -60,8 +60,8 @@ int make_tmap_rows(CUtensorMap* out, const void* base, uint64_t cols, uint64_t r
                    head_stride, 64, box_rows);
 }
 
-int make_tmap_codes(CUtensorMap* out, const void* base, uint64_t row_bytes, uint64_t rows, uint32_t box_bytes, uint32_t box_rows) {
-  return encode_3d(out, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, box_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, base, row_bytes / 2, rows, 1,
+int make_tmap_codes(CUtensorMap* out, const void* base, uint64_t row_bytes, uint64_t rows, uint64_t pages, uint32_t box_bytes, uint32_t box_rows) {
+  return encode_3d(out, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, box_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, base, row_bytes / 2, rows, pages,
                    row_bytes / 2, rows * row_bytes / 2, box_bytes / 2, box_rows);
 }
 
