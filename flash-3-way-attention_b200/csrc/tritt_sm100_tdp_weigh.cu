@@ -629,9 +629,13 @@ __global__ void __launch_bounds__(kThreads, 1) tdp_weigh_sm100_kernel(const __gr
       float(&sums)[4][32] = ms.sums[wg][buf];
       sums[wq][lane] = v[0];
       named_bar_sync(1 + wg, 128);   // (the other parity's numbers have been read by then)
+      if (__any_sync(0xffffffffu, *abort_flag)) break;
       if (row < 32 && k0 + row <= last) col_sums[k0 + row - base] += (sums[0][row] + sums[1][row]) + (sums[2][row] + sums[3][row]);
       ++pieces;
     }
+    // The warpgroup's barrier has no limit of its own.  A warp whose wait ran out arrives, once, at the one that it leaves out, after the flag is set; the others see the flag behind that barrier, leave, and arrive at the next in
+    // the same way, which nobody waits at without having seen it.
+    if (__any_sync(0xffffffffu, *abort_flag)) named_bar_arrive(1 + wg, 128);
   }
 
   // ------------------------------------------------------------------ teardown
