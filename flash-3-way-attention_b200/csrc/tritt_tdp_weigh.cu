@@ -240,14 +240,16 @@ template <typename T> int by_code(const TdpWeighArgs& p, cudaStream_t stream) {
   }
 }
 
-// Slots take a number for each token that a table has room for, whatever the contexts, and heads may be many: a call takes as many sequences at a time as keep them below this.
+// Slots take a number for each token that a table has room for, whatever the contexts, and heads may be many: a call takes as many sequences at a time as keep them below this, but one at least, and has a slot for each CTA
+// (fewer CTAs would be that much slower, whatever the contexts are).
 constexpr long long kMostSlots = 1ll << 30;
+int sums_of(const tritt_cache_t& c) { return sm100_tdp_weigh_supported(c.D) ? 5 : 2; }
 int sequences_at_once(const tritt_cache_t& c, int span) {
-  const long long heads = kMostSlots / (kWeighSums * 4ll * span) - kWeighCtas, n = heads / c.N;
+  const long long heads = kMostSlots / (sums_of(c) * 4ll * span) - kWeighCtas, n = heads / c.N;
   return (int)(n < 1 ? 1 : n < c.B ? n : c.B);
 }
 size_t table_bytes(const tritt_cache_t& c) { return align_up(((size_t)c.B + 1) * 8, 256); }
-size_t slots_bytes(const tritt_cache_t& c, int span) { return (size_t)(kWeighCtas + (long long)sequences_at_once(c, span) * c.N) * kWeighSums * span * 4; }
+size_t slots_bytes(const tritt_cache_t& c, int span) { return (size_t)(kWeighCtas + (long long)sequences_at_once(c, span) * c.N) * sums_of(c) * span * 4; }
 
 }  // namespace
 
@@ -334,7 +336,7 @@ int tritt_tdp_weigh(const tritt_cache_t* c, const tritt_weights_t* w, const trit
                  (long long*)workspace, (float*)((uint8_t*)workspace + table_bytes(*c)), kWeighCtas, weigh_span(*c, window(k1_window), window(k2_window)), 0};
   if (window_tdp_weigh_applies(p)) return window_tdp_weigh(p, (cudaStream_t)stream);
   const bool fast = sm100_tdp_weigh_supported(c->D);
-  p.sums = fast ? 5 : 2;
+  p.sums = sums_of(*c);
   const int most = sequences_at_once(*c, p.span), size = dtype == TRITT_F32 ? 4 : 2;
   for (int b0 = 0; b0 < c->B; b0 += most) {
     TdpWeighArgs s = p;   // of sequences b0 and on

@@ -182,7 +182,7 @@ inline int weigh_span(const tritt_cache_t& c, int k1w, int k2w) {
   if (reach < tokens) tokens = reach;
   return (int)((tokens + 127) / 128 * 128);
 }
-constexpr int kWeighCtas = 148, kWeighSums = 5;   // the most sums of a slot
+constexpr int kWeighCtas = 148;
 
 // (a division of 64 bits is long, and few are needed)
 __device__ __forceinline__ long long quotient(long long a, long long b) {

@@ -378,8 +378,8 @@ typedef struct {
  */
 int tritt_tdp_weigh(const tritt_cache_t* c, const tritt_weights_t* w, const tritt_rows_t* q, const float* lse, int dtype, float alpha, int k1_window,
                     int k2_window, int kk_left, int kk_right, void* workspace, size_t workspace_bytes, int* status_word, tritt_stream_t stream);
-/* Bytes of scratch for it: 20 bytes for each token that the windows and the table have room for, for each SM and for each head of as many sequences as keep it at about 1 GB (a call takes the others
-   behind them).  Calls that may run at the same time need scratch of their own. */
+/* Bytes of scratch for it: 20 (head dimensions 64 and 128) or 8 for each token that the windows and the table have room for, whatever the contexts are, for each of 148 blocks and for each head of the sequences that
+   are taken at a time: as many as keep it below 2^30 bytes, one at least.  So a table of 2^17 tokens and 16 heads without windows takes 430 MB, one of 2^20 tokens 3.4 GB.  Calls that may run at the same time need scratch of their own. */
 size_t tritt_tdp_weigh_workspace(const tritt_cache_t* c, int k1_window, int k2_window);
 /*
  * Dot-product sum: each new token i adds exp(alpha q_i.K2[x] + lse[x] - m_i) to the tokens x that its query attends to (tritt_dps_decode), and
