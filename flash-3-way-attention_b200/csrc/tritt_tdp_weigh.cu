@@ -191,9 +191,17 @@ template <typename T, int D, int CODE> __global__ void __launch_bounds__(kThread
 __global__ void __launch_bounds__(256) tdp_weigh_join_kernel(const __grid_constant__ TdpWeighArgs p) {
   const CacheArgs& a = p.cache;
   const int bh = blockIdx.y, b = bh / a.c.N, head = bh - b * a.c.N;
-  if (__ldg(a.c.context + b) < 0) return;
+  // (a kernel that ended without a wait would let the next one, and who uses the scratch after it, start beside the previous: of blocks that have nothing to do the first waits all the same)
+  const bool first = blockIdx.x == 0 && blockIdx.y == 0;
+  if (__ldg(a.c.context + b) < 0) {
+    if (first) wait_for_previous();
+    return;
+  }
   const int ctx = context_of(a, b), end = weighed_tokens(a, p.w, ctx + new_tokens(a, b)), x = blockIdx.x * 256 + threadIdx.x;
-  if ((int)blockIdx.x * 256 >= end) return;
+  if ((int)blockIdx.x * 256 >= end) {
+    if (first) wait_for_previous();
+    return;
+  }
   const WeighLine l = weigh_line(p, b);
   float v = x < ctx && x < end ? faded(p.w, b, head, x) : 0.f, sum = 0.f;
   const bool any = l.unit > 0 && x >= l.base && x <= l.last;

@@ -1,7 +1,14 @@
 """No warp of the weights' kernel on the tensor cores waits for good for one that gave up.  Nothing makes a wait run out on the GPU: the source is read, and the one barrier without a limit
 is gone through in a model of four warps, in every order of their steps."""
+import glob
 import os
 import re
+
+import pytest
+import torch
+
+import flash_trittention as ft
+from tests.test_eviction import DEV, Weighed
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "flash-3-way-attention_b200", "csrc")
 
@@ -64,3 +71,41 @@ def _ends(arrive, look, pieces=3, warps=4):
 def test_every_order_of_leaving_ends():
     assert _ends(True, True)
     assert not _ends(False, False) and not _ends(True, False) and not _ends(False, True)
+
+
+def test_a_kernel_that_may_start_early_waits_for_the_one_ahead():
+    """(Else the next one in the stream, which waits for it alone, starts beside the one ahead.)  Who returns ahead of the wait waits first, the first block at least."""
+    kernels = 0
+    for path in glob.glob(os.path.join(CSRC, "*.cu")):
+        text = re.sub(r"//.*", "", open(path).read())
+        for body in re.split(r"\n(?=template|__global__|}  // namespace)", text):
+            if "__global__" not in body or "wait_for_previous();" not in body:
+                continue
+            kernels += 1
+            last = body.rindex("wait_for_previous();")
+            early = [m.start() for m in re.finditer(r"\breturn;", body[:last])]
+            for at in early:
+                assert re.search(r"(wait_for_previous\(\);\s*)$", body[:at]), (path, body[max(0, at - 100):at + 7])
+    assert kernels >= 5
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 32])
+def test_free_slots_alone_and_then_others_in_a_graph(D):
+    """A call of a batch that has no sequence in use, and one whose scratch follows it."""
+    idle, bt = Weighed(3, 2, 2, D, "bf16", "e4m3", 16, [-1, -1, -1], length=40), Weighed(2, 2, 2, D, "bf16", "e4m3", 16, [90, 41])
+    table = torch.nn.functional.pad(bt.table, (0, 200), value=0)
+    args = [(b.before.to(DEV), b.q.to(DEV), b.sums.to(DEV), b) for b in (idle, bt)]
+    outs = [torch.full_like(a[0], 5.0) for a in args]
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=side):
+        for _ in range(3):
+            for (before, q, sums, b), out in zip(args, outs):
+                ft.tdp_weigh(before, q, sums, b.cache, table if b is bt else torch.zeros(3, 200, dtype=torch.int32, device=DEV), b.context, b.alpha, out=out)
+    for _ in range(20):
+        graph.replay()
+    torch.cuda.synchronize()
+    ft.check_status(DEV)
+    assert bool((outs[0] == 5.0).all())
+    bt.check(outs[1], stale=torch.full_like(bt.before, 5.0))
