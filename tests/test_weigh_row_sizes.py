@@ -146,3 +146,19 @@ def test_queries_and_rows_of_opposite_sizes(form, D, n, rows, queries, dtype, co
     bt.q, bt.k2 = bt.q * queries, bt.k2 * queries
     bt.check(bt.run())
     ft.check_status(DEV)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("by", BY)
+@pytest.mark.parametrize("part", [K1, K2])
+@pytest.mark.parametrize("D,n,code", [(64, 4, "e4m3"), (64, 9, "fp16"), (128, 4, "int8"), (32, 3, "fp16"), (256, 4, "e4m3")])
+def test_later_tokens_that_are_larger_in_the_dot_product_sum(D, n, code, part, by):
+    """The new tokens before it do not attend to the last one, whatever it holds."""
+    kw = dict(dps=True, k_diff=40)
+    bt, kept = (Weighed(1, 2, n, D, "bf16", code, 16, [130], counts=c, **kw) for c in (None, [n - 1]))
+    bt.gain, bt.sums, bt.cache, bt.size, bt.most = kept.gain, kept.sums, kept.cache, kept.size, kept.most
+    page, row = int(bt.seq.table[0, (130 + n - 1) // 16]), (130 + n - 1) % 16
+    bt.cache.lse[page, :, row] = -math.inf
+    _enlarge(bt, 0, 130 + n - 1, part, by)
+    bt.check(bt.run())
+    ft.check_status(DEV)
