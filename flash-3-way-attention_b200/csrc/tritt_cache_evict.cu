@@ -7,7 +7,8 @@
 // Moved by another kernel, bound by the bytes of the kept rows, read and written once.  In place: a kept token's new place is never behind its old one, so rows that are taken in order
 // and written when all rows up to them have been read overwrite nothing that is still to be read.  One block, or a cluster whose blocks keep step, takes a piece of up to 64 bytes of all rows of one part of a head (the
 // parts, heads and pieces of rows are independent), with the next tile's rows on their way while one is written.
-// Measured: 8 x 16 heads of 64, float16 codes, from 8191 tokens to 4096 118 us (chosen 13, moved 105: 5.0 TB/s; in place 118); 16 heads of 128 from 65001 to 16384 132 us (23, 108; in place 152, its clusters' barriers);
+// Measured: 8 x 16 heads of 64, float16 codes, from 8191 tokens to 4096 118 us (chosen 13, moved 105: 5.0 TB/s); 16 heads of 128 from 65001 to 16384 132 us (23, 108);
+// with L2 flushed before the call 121 and 135, and in place 127 and 154 (clusters' barriers);
 // 4 x 8 heads of 64, e4m3, from 700 to 512 15 us.  Moved in pieces of 32 bytes without clusters the second took 220 us, by clusters whose barrier waited for the next tile's loads 128; pieces of 128 bytes take 2 % less, eight loads a thread in
 // place of four 18 % more (registers); chosen by weights read again
 // for each pass by clusters of eight 49.

@@ -6,8 +6,9 @@
 // A warp takes 16 tokens: their rows go from memory straight into the fragments of warp-level matrix instructions (eight new tokens the other side, in shared memory in the order of
 // the fragments), exact as fp16 codes; each row's exponent, and the new row's, multiply the sums.  fp32 rows are two fp16 numbers (22 bits), as the products are
 // summed in fp32 all the same.
-// Measured: a token of 32 x 16 heads of 64 over up to 8191, e4m3, 75 us (278 MB, 3.7 TB/s; 70 % of the issue slots); 24 tokens over 3001, 4 x 16 heads of 128, fp16 codes 31 us (78 MB; a block's way to its first
-// tile, and one tile behind the other).
+// Measured: a token of 32 x 16 heads of 64 over up to 8191, e4m3, 73 us (278 MB, 3.8 TB/s; 70 % of the issue slots); 24 tokens over 3001, 4 x 16 heads of 128, fp16 codes 27 to 31 us (78 MB; a block's way to its first
+// tile, and one tile behind the other).  One token of 32 x 16 heads over up to 8191 otherwise: head dimension 16, int8 57 us (floor by bytes 15), 32, fp16 codes 70 (43), 128, e4m3 117 (79), 128, fp16 codes 205 (151; rows of
+// 256 bytes, by the kernel for several tokens); over up to 4095 head dimension 256, fp16 codes 257 (166), int8 403 (85: fragments of 16 steps beside the rows of both parts, of which 570 to 660 bytes a thread are spilled).
 #include "tritt_weigh.cuh"
 
 #include <type_traits>

@@ -8,12 +8,14 @@
 // Bound by HBM: forward one read and one write of the rows, backward two reads and one write.  D / 8 lanes take a row, eight elements each:
 // two groups of four that lie R / 2 apart, so that a thread holds both of each rotated pair (neighbours where there is no rotation or
 // neighbours are rotated).  With eight neighbours a lane and the other half by shuffles the forward executed 202 instructions for eight
-// elements, and instruction issue bounded it (4 x 16 heads x 2048 x 128 bf16: 53 us, the backward 121).  Two fp32 numbers an instruction: 39 us (5.1 TB/s);
-// the backward, whose chains of two sums over a row's lanes leave half of the issue slots, 70 (4.3 TB/s) and 4.5 for the weights' last sums.
+// elements, and instruction issue bounded it (4 x 16 heads x 2048 x 128 bf16: 53 us, the backward 121).  Two fp32 numbers an instruction: 38 us without rotation
+// (5.3 TB/s), 41 with positions 0, 1, 2, ... and 43 with an array of them, whose load comes before that of the tables; the backward, whose chains of two sums over a row's lanes leave half of the issue slots, 69, 72 and 74
+// (4.1 to 4.4 TB/s) and 4 to 5 for the weights' last sums.  (Kernels by themselves.)
 // The tables (a cosine and a sine, 8 bytes, for two elements) would be twice the traffic of 16-bit rows, so a thread keeps its position's
 // values for four heads and, where there are blocks enough, all three tensors.
 // Positions of several axes are kernels of their own (AXES): the same, but that a lane whose four pairs are not all of one axis takes their values one
-// by one.  4 x 16 heads x 2048 x 128 bf16, three axes: forward 45.4 us one axis after the other and 45.9 in turn, 44.6 with one axis; forward and backward 136 in turn (132 with one).
+// by one.  4 x 16 heads x 2048 x 128 bf16, three axes: calls of the forward 45.6 us one axis after the other and 46.3 in turn, 45.1 with one axis; forward and backward
+// 134 to 136 in turn (132 with one).
 #include "tritt_cache.cuh"
 #include "tritt_common.cuh"
 

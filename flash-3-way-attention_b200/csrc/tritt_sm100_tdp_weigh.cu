@@ -3,12 +3,13 @@
 //   P[j, k] = exp(alpha sum_h q[h] K1[j, h] K2[k, h] - lse);   of each new token its row sums go to the tokens j, its column sums to the tokens k
 // For one new token and a tile of 128 tokens k the operand Q[k] = q * K2[k] is formed once; tiles of 128 tokens j then stream by as S = K1 Q^T.  K1's codes are exact as fp16 numbers, Q is held in two (22 bits: of
 // 16-bit queries and any codes exact), which doubles the products and costs nothing at head dimension 64, where the exponentials take twice as long as they do.  The rows' powers of two stay out of the operands: a
-// score is multiplied by its column's, relative to the largest of 32, and by its row's.  A row's sum is one thread's, over its 32 columns, and leaves after each tile; a column's is kept in registers by 128 threads, a number each, until the tokens j have all
+// score is multiplied by its column's, relative to the largest of 32 (or, where those are far apart, to one in the middle), and by its row's.  A row's sum is one thread's, over its 32 columns, and leaves after each tile; a column's is kept in registers by 128 threads, a number each, until the tokens j have all
 // been, and then added up over them.  No row needs another's maximum: lse is known.
 // What bounds it: exponentials, one a pair (16 a clock and SM), take 1024 clocks a tile of 128 x 128, the products 512 at D = 64 and 1024 at D = 128; a tile takes 1500 and 1700.  930 instructions a scheduler and tile
 // fill 57 % of the issue slots, the rest is the way of each warp from one tile's scores to the next.  At D = 128 with fp16 codes the tiles of K1, 32 KB each, come from L2 at 4.9 TB/s.
-// Measured: one token of 2 x 16 heads of 64 over 4095 and 3098 tokens, int8 codes 172 us (exponentials alone 94, products 33, both numbers of Q 65); 8 tokens over 2040, 16 heads of 128, float16 codes 227 to
-// 259 us (119, 84, 165); one token of 4 x 8 heads over up to 700 24 us, of which the way to the first scores takes 7.
+// Measured: one token of 2 x 16 heads of 64 over 4095 and 3098 tokens, int8 codes 172 us (exponentials alone 94, products 33, both numbers of Q 65); 8 tokens over 2040, 16 heads of 128, float16 codes 224 to
+// 230 us (119, 84, 165) at 1965 MHz, and 260 in a run of more than a third of a second, when the power limit (990 W) has taken the clock to 1570 MHz; one token of 4 x 8 heads over up to 700 24 us, of which the way to the first
+// scores takes 7.
 //
 // The line of steps (tritt_weigh.cuh) is cut in equal parts, one for each CTA.
 //   warp 1        walks the line and tells the others each piece (a new token, a tile of k, a range of tiles of j) by a ring in shared memory
@@ -18,7 +19,7 @@
 //   warps 8-11    Q for the piece after the present one, and its columns' powers of two
 //   warps 12-27   four warpgroups, 32 columns each: exponentials and sums.  Four warps a scheduler: with two, of 64 columns each, registers and the way from a tile's scores to the
 //                 next one's left half of the exponentials' time unused
-// Before (us, the first two of these cases): warp-level products, all in a block of eight warps 631 / 1149; two warpgroups that sum 64 columns, K1 through registers or by copies into shared memory 220 / 298; K1
+// Before (us, the first two of these cases, ten calls each, before the power limit counts): warp-level products, all in a block of eight warps 631 / 1149; two warpgroups that sum 64 columns, K1 through registers or by copies into shared memory 220 / 298; K1
 // through tensor memory by four warps that also fetched it 250 / 367; four warpgroups of 32 columns 193 / 264; fetched by two warps in turn, fewer instructions in the sums 188 / 238; one barrier for a tile's scores
 // and its rows' exponents 177 / 227.  Tried: halves of 16 columns with the next half on its way 193 / 263 (registers); a polynomial on the multiply-add units for 2, 4, 8 of 16 pairs - / 236, 196 / 261, 237 / 307
 // (instructions); no exponentials at all, wrong, for the time: 135 / 213.
@@ -33,7 +34,6 @@ constexpr int kThreads = 896;
 constexpr int kRegsLaunch = 72;   // a thread; the warps that sum take what the others give up
 constexpr int kRegsIssue = 40, kRegsConvert = 56, kRegsForm = 56, kRegsSum = 88;
 static_assert(kRegsIssue + kRegsConvert + kRegsForm + 4 * kRegsSum <= 7 * kRegsLaunch, "more registers than the launch has");
-constexpr int kSums = 5;          // of a slot: four of the rows, one of the columns
 constexpr int kMetas = 16;        // tiles whose rows are described
 constexpr int kItems = 4;
 constexpr int kScores = 3;        // buffers of scores

@@ -5,6 +5,8 @@
 // For one new token and a tile of 128 tokens k the operand A[k] = q * K2[k] is formed once, as two fp16 numbers an element (22 bits: 16-bit queries times any code are exact), in the order of the
 // fragments; each warp takes 16 rows j of K1 straight from memory, and its scores' exponentials add up along both sides: over k in the warp's registers to one number a row, over j in as many as it
 // has columns, which leave at the end of the tile.  Sums go to slots of the CTA (see the line in tritt_weigh.cuh), each number by one thread, and a second kernel adds the slots up.
+// Measured: one token of 2 x 16 heads over 2047 and 1050 tokens, int8 codes 82 us at head dimension 16, 97 at 32, 397 at 256 (430 with float16 codes); of 4 x 8 heads of 32 over up to 700, e4m3 28; 8 tokens over 2040,
+// 16 heads of 32, float16 codes 500.  Bound by instructions: a product of 16 x 8 x 16 is one for each warp and step, twice, and an exponential, its mask and its two sums follow for each pair.
 #include "tritt_weigh.cuh"
 
 #include <cmath>
@@ -251,7 +253,7 @@ template <typename T> int by_code(const TdpWeighArgs& p, cudaStream_t stream) {
 // Slots take a number for each token that a table has room for, whatever the contexts, and heads may be many: a call takes as many sequences at a time as keep them below this, but one at least, and has a slot for each CTA
 // (fewer CTAs would be that much slower, whatever the contexts are).
 constexpr long long kMostSlots = 1ll << 30;
-int sums_of(const tritt_cache_t& c) { return sm100_tdp_weigh_supported(c.D) ? 5 : 2; }
+int sums_of(const tritt_cache_t& c) { return sm100_tdp_weigh_supported(c.D) ? 5 : 2; }   // (on tcgen05 four of the rows and one of the columns)
 int sequences_at_once(const tritt_cache_t& c, int span) {
   const long long heads = kMostSlots / (sums_of(c) * 4ll * span) - kWeighCtas, n = heads / c.N;
   return (int)(n < 1 ? 1 : n < c.B ? n : c.B);
