@@ -376,16 +376,16 @@ template <typename T, int D, int CODE> __global__ void __launch_bounds__(kThread
 // goes through; few cells more, half a million in all, are made up for by the launch that it saves.  With one block an SM (head dimension 128, or more than half the shared memory), its heads have to fit on the SMs at once.
 // us, the other / this; bfloat16 queries, int8 codes at 64 and float16 at 128; windows (band to either side) of
 //                      one token, 4 x 8   one token, 32 x 16   4 tokens, 2 x 16   16 tokens, 8 x 16
-//   64   64 (64)       14 / 10            52 / 29              19 / 13            110 / 42
-//        128 (32)      15 / 11            52 / 37              20 / 15            110 / 55
-//        128           14 / 13            52 / 46              20 / 19            110 / 79
-//        256 (32)      17 / 12            72 / 63              23 / 17            182 / 89
+//   64   64 (64)       14 / 10            52 / 29              20 / 13            114 / 37
+//        128 (32)      15 / 11            52 / 37              20 / 16            115 / 51
+//        128           14 / 13            52 / 46              20 / 19            114 / 81
+//        256 (32)      17 / 12            72 / 63              24 / 17            186 / 89
 //        256           16 / 19            77 / 103             26 / 32            203 / 218
 //        512 (32)      19 / 14            108 / -              32 / 23            315 / 220
-//   128  64 (64)       15 / 11            53 / 55              22 / 16            115 / 52
-//        128 (32)      15 / 12            55 / 70              22 / 17            116 / 74
-//        128           15 / 14            54 / 85              22 / 20            116 / 122
-//        256 (32)      18 / 14            84 / 131             27 / 22            187 / -
+//   128  64 (64)       15 / 11            53 / 55              22 / 15            119 / 49
+//        128 (32)      15 / 12            55 / 70              23 / 17            127 / 74
+//        128           15 / 14            54 / 85              23 / 20            128 / 118
+//        256 (32)      18 / 14            84 / 131             28 / 22            194 / -
 bool faster(const tritt_cache_t& c, long long places, long long reach_k, long long reach_j, long long band) {
   auto least = [](long long x, long long y) { return x < y ? x : y; };
   auto tiled = [&](long long tokens) { return tokens < places ? tokens + 127 : (tokens + 127) / 128 * 128; };   // (a window begins anywhere in a tile)
